@@ -519,3 +519,106 @@ def attention(q, k, v, scale=None, out=None, check=None):
         if st != 0:
             raise _lib.L3dError(8, "l3d_attention", f"kernel status word {st} (bounded wait expired)")
     return out
+
+
+# ------------------------------------- serving many requests around one context
+class LoraAdapters:
+    """Low-rank adapters of the requests that share a projection, laid out once:
+    adapter i adds scales[i] * b[i] @ (a[i] @ x), a[i] [rank, K], b[i] [N, rank]
+    CUDA tensors of any float dtype (kept as bf16, ranks padded to a common
+    multiple of 16).  Weights must be finite."""
+
+    def __init__(self, a, b, scales=None):
+        a, b = list(a), list(b)
+        if not a or len(a) != len(b):
+            raise ValueError("LoraAdapters needs as many a as b, at least one")
+        _check_cuda(*a, *b)
+        K, N, dev = a[0].shape[1], b[0].shape[0], a[0].device
+        ranks = [t.shape[0] for t in a]
+        for i, (u, w) in enumerate(zip(a, b)):
+            if u.dim() != 2 or w.dim() != 2 or u.shape[1] != K or w.shape != (N, ranks[i]):
+                raise ValueError(f"adapter {i}: a [rank, {K}] and b [{N}, rank] expected")
+        scales = [1.0] * len(a) if scales is None else [float(v) for v in scales]
+        if len(scales) != len(a):
+            raise ValueError("LoraAdapters needs one scale per adapter")
+        R = max(16, -(-max(ranks) // 16) * 16)
+        self.n, self.k, self.rank, self.count = N, K, R, len(a)
+        self.a = torch.zeros((len(a), R, K), dtype=torch.bfloat16, device=dev)
+        self.b = torch.zeros((len(a), N, R), dtype=torch.bfloat16, device=dev)
+        for i, (u, w) in enumerate(zip(a, b)):
+            self.a[i, :ranks[i]] = u
+            self.b[i, :, :ranks[i]] = w
+        self.scales = torch.tensor(scales, dtype=torch.float32, device=dev)
+        self.ranks = torch.tensor(ranks, dtype=torch.int32, device=dev)
+        # A row of another request meets these weights multiplied by zero.
+        if not (all(np.isfinite(scales)) and bool(torch.isfinite(self.a).all())
+                and bool(torch.isfinite(self.b).all())):
+            raise ValueError("LoraAdapters: weights and scales must be finite")
+
+
+def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, gate=None, out=None,
+                out_dtype=None):
+    """`linear` with the low-rank adapter of each row's request beside the shared
+    projection: y = residual + gate * act(x . W^T + bias + s_a B_a A_a x), where
+    a = ids[i] for the i-th of ids.numel() equal groups of rows (one id per row,
+    or per request); an id outside [0, adapters.count) means no adapter."""
+    _check_cuda(x, weight, ids, bias, residual, gate, out)
+    n, k = weight.shape
+    x2 = x.reshape(-1, k)
+    m = x2.shape[0]
+    if out is not None:
+        y = out.view(-1, n)
+    else:
+        y = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+    need = _lib.lib().l3d_lora_linear_workspace_size(m, adapters.rank)
+    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
+    r2 = None if residual is None else residual.reshape(-1, n)
+    call("l3d_lora_linear", ref(desc(x2)), ref(desc(weight)), ref(desc(bias)),
+         ref(desc(adapters.a)), ref(desc(adapters.b)), ref(desc(adapters.scales)),
+         ref(desc(adapters.ranks)), ref(desc(ids.reshape(-1))), ACT_CODES[act], ref(desc(r2)),
+         ref(desc(gate)), ref(desc(y)), ws.data_ptr(), need, _s(x))
+    return y.reshape(*x.shape[:-1], n)
+
+
+def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None, causal=False,
+                            scale=None, out=None):
+    """exact_sdpa_heads (crate/runtime/attention_math.rs:199-259) for a batch that
+    shares a prefix of keys: q [B, Hq, N, D] over prefix_k / prefix_v [Hkv, P, D]
+    (one copy for the batch) and the first lengths[b] of each element's own k / v
+    [B, Hkv, S, D] (lengths None: all S); causal: the rows are the last N of their
+    element's own sequence.  BF16 or F16, D = 64 or 128; `out` defaults as in
+    `attention`."""
+    _check_cuda(q, prefix_k, prefix_v, k, v, lengths, out)
+    B, H, N, D = q.shape
+    if out is None:
+        out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
+    Hkv, P = prefix_k.shape[:2]
+    need = _lib.lib().l3d_shared_prefix_attention_workspace_size(
+        B, H, Hkv, N, P, 0 if k is None else k.shape[2], D)
+    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    call("l3d_shared_prefix_attention", ref(desc(q)), ref(desc(prefix_k)), ref(desc(prefix_v)),
+         ref(desc(k)), ref(desc(v)), ref(desc(lengths)), int(bool(causal)),
+         D ** -0.5 if scale is None else float(scale), ref(desc(out)),
+         ws.data_ptr() if need else None, need, _s(q))
+    return out
+
+
+NORMS = {"layer": 1, "rms": 2}
+
+
+def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, res_scale=1.0,
+                           weight=None, bias=None, shift=None, scale=None, norm="rms", eps=1e-6,
+                           post_eps=None, next_norm=True, inplace=False):
+    """Block seam with a norm on either side of the residual:
+    r = res_scale * x + gate * (Norm(h)[*post_weight][+post_bias]);
+    y = Norm(r)[*weight][+bias][*(1+scale)+shift]; returns (r, y).  `norm` is
+    "rms" or "layer"; next_norm=False (the last block) returns (r, None); with
+    inplace=True the residual stream x is updated in place (r is x)."""
+    _check_cuda(x, h, post_weight, post_bias, gate, weight, bias, shift, scale)
+    r = x if inplace else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if next_norm else None
+    call("l3d_sandwich_residual_norm", ref(desc(x)), ref(desc(h)), NORMS[norm],
+         ref(desc(post_weight)), ref(desc(post_bias)), ref(desc(gate)), float(res_scale),
+         ref(desc(weight)), ref(desc(bias)), ref(desc(shift)), ref(desc(scale)),
+         eps if post_eps is None else post_eps, eps, ref(desc(r)), ref(desc(y)), _s(x))
+    return r, y

@@ -423,6 +423,74 @@ int l3d_attention_selftest_timeout(const l3d_tensor* q, const l3d_tensor* k,
                                    void* workspace, size_t workspace_bytes,
                                    uint32_t wait_limit_ms, l3d_stream stream);
 
+/* ---- serving many requests: adapters, shared prefixes, sandwich norms ------------ */
+
+/* Workspace bytes for l3d_lora_linear with m rows and adapters padded to rank r. */
+size_t l3d_lora_linear_workspace_size(int64_t m, int64_t r);
+
+/* One projection shared by the rows of many requests, each with a low-rank
+ * adapter of its own (no counterpart in the reference, which serves one
+ * checkpoint: it composes Linear::forward, crate/runtime/nn_blocks.rs:82):
+ *   y[m] = residual[m] + gate * act( W x[m] + bias + scale[a] B_a (A_a x[m]) )
+ * a = ids[m / (M / G)] for ids [G] I32/I64 with M % G == 0 (one id per row, or
+ * per request of equal rows); rows whose id is outside [0, adapters) take the
+ * projection alone.  x [.., k] BF16, 16-byte aligned rows; weight [n, k] BF16
+ * as for l3d_linear_ex; lora_a [adapters, R, k] and lora_b [adapters, n, R]
+ * BF16 contiguous, R a multiple of 16 up to 256, zero beyond an adapter's own
+ * rank; scale [adapters] F32; ranks [adapters] I32 (NULL: all R) lets the
+ * kernels skip the zero ranks.  The adapters must be finite: a row of another
+ * request meets them multiplied by zero.  bias, act, residual, gate as for
+ * l3d_linear_ex; y BF16 or F32; y must not overlap x (it may be residual).
+ * A_a x is accumulated in f32 and enters the second product as bf16 (as a
+ * sum of two bf16 parts when y is F32). */
+int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight, const l3d_tensor* bias,
+                    const l3d_tensor* lora_a, const l3d_tensor* lora_b,
+                    const l3d_tensor* lora_scale, const l3d_tensor* ranks, const l3d_tensor* ids,
+                    int act, const l3d_tensor* residual, const l3d_tensor* gate,
+                    const l3d_tensor* y, void* workspace, size_t workspace_bytes,
+                    l3d_stream stream);
+
+/* Workspace bytes for l3d_shared_prefix_attention (0: none needed). */
+size_t l3d_shared_prefix_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t n,
+                                                  int64_t p, int64_t s, int64_t d);
+
+/* The attention core (exact_sdpa_heads, crate/runtime/attention_math.rs:199-259)
+ * for a batch whose elements attend to one shared prefix of keys and to keys
+ * of their own: out[b, h, i] = softmax over {prefix keys} u {own keys
+ * j < lengths[b]} of scale q.k, times v.  q and out [B, Hq, N, D]; prefix_k and
+ * prefix_v [Hkv, P, D], one copy for the batch; k and v [B, Hkv, S, D], or both
+ * NULL; lengths [B] I32/I64 or NULL (all S), values clamped to [0, S]; Hq a
+ * multiple of Hkv, query head h reading key head h / (Hq / Hkv).  causal: the
+ * N rows are the last N of their element's own sequence, row i sees the own
+ * keys j <= lengths[b] - N + i (and the whole prefix).  Own keys past
+ * lengths[b] are never used, whatever they hold.  A row with no keys gives
+ * zeros.  BF16 or F16, D = 64 or 128, head dim contiguous, strides otherwise
+ * free in multiples of 16 bytes; softmax and sums in f32, probabilities
+ * rounded to the input type for the second product.  scale must be positive. */
+int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor* prefix_k,
+                                const l3d_tensor* prefix_v, const l3d_tensor* k,
+                                const l3d_tensor* v, const l3d_tensor* lengths, int causal,
+                                float scale, const l3d_tensor* out, void* workspace,
+                                size_t workspace_bytes, l3d_stream stream);
+
+/* Block seam with a norm on either side of the residual, one HBM pass:
+ *   n     = Norm(h) [* post_weight] [+ post_bias]
+ *   r_out = res_scale * x + [gate *] n
+ *   y     = Norm(r) [* weight] [+ bias] [* (1 + scale) + shift]
+ * norm: 1 LayerNorm (biased variance), 2 RMS norm (v / sqrt(mean(v^2) + eps)),
+ * for both; y is formed from r before r is rounded.  y NULL: no next norm (the
+ * last block).  weights and biases [C]; gate, shift, scale [C], [B, C] or
+ * [B, 1, C] as for l3d_layer_norm_modulate; rows up to 24576 elements.  r_out
+ * may be x itself and y may be h itself.  The reference composes such seams
+ * from crate/runtime/trellis2_blocks.rs:280-286 (norms) and :627-645 (gate and
+ * residual). */
+int l3d_sandwich_residual_norm(const l3d_tensor* x, const l3d_tensor* h, int norm,
+                               const l3d_tensor* post_weight, const l3d_tensor* post_bias,
+                               const l3d_tensor* gate, float res_scale, const l3d_tensor* weight,
+                               const l3d_tensor* bias, const l3d_tensor* shift,
+                               const l3d_tensor* scale, float post_eps, float eps,
+                               const l3d_tensor* r_out, const l3d_tensor* y, l3d_stream stream);
+
 /* ---- GGUF tensor index (the on-disk format feeding a13) ------------------------ */
 
 /* One tensor of a GGUF file.  name points into the caller's buffer (not

@@ -1,0 +1,221 @@
+"""GPU parity: a projection with low-rank adapters of many requests
+(l3d_lora_linear) against the f64 sum of the same bf16 operands.
+
+Bounds: f32 accumulation of both products (2e-5 of the sum of the terms'
+magnitudes, as for the dense linear); A x rounded to bf16 before the second
+product (2^-9 of its terms; 2^-17 where y is F32 and it enters as two bf16
+parts), times the activation's largest derivative (< 1.13); for a bf16 y its
+rounding (2^-8) and the 16-bit activation forms (3e-4 |z|)."""
+import numpy as np
+import pytest
+
+from conftest import rng
+from test_gpu_qlinear import _act_ref
+
+pytestmark = pytest.mark.gpu
+
+
+def _case(ops, dev, M, N, K, ranks, ids, act=None, res=False, gate=False, ydt="bf16", bias=True,
+          seed=0, x=None):
+    import torch
+
+    r = rng(700 + seed + M + N + K)
+
+    def up(a, dt=torch.bfloat16):
+        t = torch.from_numpy(np.ascontiguousarray(a, np.float32)).to(dev).to(dt)
+        return t, t.float().cpu().numpy().astype(np.float64)
+
+    xt, xv = up(r.standard_normal((M, K)))
+    if x is not None:
+        x.copy_(xt)
+        xt = x
+    wt, wv = up(r.standard_normal((N, K)) / np.sqrt(K))
+    ab = [(up(r.standard_normal((k, K)) / np.sqrt(K)), up(0.5 * r.standard_normal((N, k)) / np.sqrt(k)))
+          for k in ranks]
+    scales = [0.5 + 0.5 * i for i in range(len(ranks))]
+    ad = ops.LoraAdapters([a[0] for a, _ in ab], [b[0] for _, b in ab], scales)
+    z, mag = xv @ wv.T, np.abs(xv) @ np.abs(wv).T
+    bt = None
+    if bias:
+        bt, bv = up(0.1 * r.standard_normal(N), torch.float32)
+        z = z + bv
+    ids = np.asarray(ids)
+    per = np.repeat(ids, M // ids.size)
+    low = np.zeros_like(z)
+    for i, ((_, av), (_, bv)) in enumerate(ab):
+        rows = per == i
+        z[rows] += scales[i] * (xv[rows] @ av.T) @ bv.T
+        mag[rows] += scales[i] * (np.abs(xv[rows]) @ np.abs(av).T) @ np.abs(bv).T
+        low[rows] += scales[i] * np.abs(xv[rows] @ av.T) @ np.abs(bv).T
+    bound = 1.13 * (2e-5 * mag + low * (2.0 ** -9 if ydt == "bf16" else 2.0 ** -17)) + 1e-6
+    ref = _act_ref(act, z)
+    tdt = torch.float32 if ydt == "f32" else torch.bfloat16
+    kw = {"act": act, "bias": bt, "out_dtype": tdt}
+    if res:
+        rt, rv = up(r.standard_normal((M, N)), tdt)
+        gv = 1.0
+        if gate:
+            kw["gate"], gv = up(0.5 + r.random(N), torch.float32)
+        ref = rv + gv * ref
+        bound = bound * np.max(np.abs(gv))
+        kw.update(residual=rt, out=rt)
+    if ydt == "bf16":
+        bound = bound + np.abs(ref) * 2.0 ** -8 + (3e-4 * np.abs(z) if act else 0.0)
+    else:
+        bound = bound + 1e-6 * np.abs(ref)
+    got = ops.lora_linear(xt, wt, ad, torch.from_numpy(ids).to(dev), **kw)
+    torch.cuda.synchronize()
+    err = np.abs(got.float().cpu().numpy() - ref)
+    assert np.all(err <= bound), f"max err {err.max():.3e}, worst ratio {(err / bound).max():.2f}"
+    return ad, xt, wt, got
+
+
+@pytest.mark.parametrize("M,N,K,ranks,A_ids", [
+    (1, 64, 64, [16], "all0"),
+    (1, 2048, 1024, [8, 16], "row"),
+    (3, 77, 72, [1, 5], "row"),
+    (16, 2048, 2048, [16] * 8, "row"),
+    (16, 1000, 264, [4, 64, 16], "row"),
+    (64, 512, 520, [64, 32, 16] * 11, "row"),     # more adapters than fit one stage
+    (127, 200, 128, [24] * 40, "row"),
+    (129, 384, 256, [48, 3], "row"),
+    (300, 264, 520, [33, 128], "request"),
+    (640, 1024, 1024, [256, 16], "row"),          # the largest rank
+    (1000, 520, 328, [16, 8, 64], "scene"),
+    (1, 8, 8, [1], "none"),
+])
+@pytest.mark.parametrize("ydt", ["bf16", "f32"])
+def test_lora_linear(ops, dev, M, N, K, ranks, A_ids, ydt):
+    r, A = rng(M * 13 + N), len(ranks)
+    if A_ids == "all0":
+        ids = np.zeros(M, np.int64)
+    elif A_ids == "none":
+        ids = np.full(M, -1, np.int64)
+    elif A_ids == "request":  # M / 3 rows per id
+        ids = np.asarray([1, -1, 0], np.int32)
+    elif A_ids == "scene":
+        ids = np.sort(r.integers(-1, A, M)).astype(np.int32)
+    else:  # any adapter, or none (on either side of the range), for each row
+        ids = r.integers(-2, A + 1, M).astype(np.int64)
+    _case(ops, dev, M, N, K, ranks, ids, ydt=ydt)
+
+
+@pytest.mark.parametrize("M,N,K", [(5, 136, 512), (200, 300, 256), (1500, 768, 512)])
+@pytest.mark.parametrize("act,res,gate,ydt,bias", [
+    ("gelu_erf", False, False, "bf16", True),
+    ("gelu", True, True, "bf16", True),
+    ("silu", True, False, "f32", False),
+    (None, True, True, "f32", True),
+    (None, True, True, "bf16", False),
+])
+def test_lora_linear_epilogue(ops, dev, M, N, K, act, res, gate, ydt, bias):
+    ids = rng(M).integers(-1, 3, M).astype(np.int32)
+    _case(ops, dev, M, N, K, [16, 32, 8], ids, act, res, gate, ydt, bias)
+
+
+@pytest.mark.parametrize("M", [1, 2, 15, 16, 17, 31, 32, 33, 63, 65, 128, 255, 257, 512, 1025])
+def test_lora_linear_row_counts(ops, dev, M):
+    _case(ops, dev, M, 320, 320, [16, 32], rng(M).integers(-1, 2, M).astype(np.int32), "silu")
+
+
+def test_lora_linear_many_tiles(ops, dev):
+    """More tiles than blocks: each block works through several, with other adapters in each."""
+    _case(ops, dev, 5000, 2560, 192, [16, 32, 64, 16], rng(9).integers(-1, 4, 5000).astype(np.int32))
+
+
+def test_lora_linear_strided_rows(ops, dev):
+    """x and out as column ranges of wider matrices; nothing else is written."""
+    import torch
+
+    xw = torch.zeros(70, 512, device=dev, dtype=torch.bfloat16)
+    ids = rng(3).integers(-1, 2, 70).astype(np.int32)
+    ad, x, w, _ = _case(ops, dev, 70, 96, 256, [16, 16], ids, bias=False, x=xw[:, 128:384])
+    wide = torch.full((70, 100), 7.0, device=dev, dtype=torch.bfloat16)  # rows of 200 bytes
+    ops.lora_linear(x, w, ad, torch.from_numpy(ids).to(dev), out=wide[:, 2:98])
+    want = ops.lora_linear(x, w, ad, torch.from_numpy(ids).to(dev))
+    assert torch.equal(wide[:, 2:98], want)
+    assert (wide[:, :2] == 7).all() and (wide[:, 98:] == 7).all()
+
+
+def test_lora_linear_rows_are_independent(ops, dev):
+    """A row's result depends on its own input and adapter alone: not on what
+    other rows hold (even NaN), and equal on every call."""
+    import torch
+
+    ids = rng(4).integers(-1, 5, 200).astype(np.int32)
+    ad, x, w, y = _case(ops, dev, 200, 512, 512, [16] * 5, ids, bias=False)
+    t = torch.from_numpy(ids).to(dev)
+    x2 = x.clone()
+    x2[::2] = float("nan")
+    got = ops.lora_linear(x2, w, ad, t)
+    assert torch.equal(got[1::2], y[1::2]) and torch.isnan(got[::2]).all()
+    for _ in range(3):
+        assert torch.equal(ops.lora_linear(x, w, ad, t), y)
+
+
+def test_lora_linear_without_adapters_is_linear(ops, dev):
+    import torch
+
+    ids = np.full(300, -1, np.int32)
+    ad, x, w, y = _case(ops, dev, 300, 512, 512, [16], ids, bias=False)
+    want = x.double() @ w.double().T
+    assert ((y.double() - want).abs() <= want.abs() * 2.0 ** -8 + 1e-3).all()
+
+
+def test_lora_linear_empty_and_shapes(ops, dev):
+    import torch
+
+    ad, x, w, _ = _case(ops, dev, 12, 64, 64, [16], np.zeros(12, np.int32), bias=False)
+    none = torch.zeros(0, device=dev, dtype=torch.int32)
+    assert ops.lora_linear(x[:0], w, ad, none).shape == (0, 64)
+    y = ops.lora_linear(x.view(3, 4, 64), w, ad, torch.tensor([0, -1, 0], device=dev))
+    assert y.shape == (3, 4, 64)
+    assert torch.equal(y[0], ops.lora_linear(x[:4], w, ad, torch.zeros(4, device=dev, dtype=torch.int64)))
+
+
+def test_lora_linear_other_stream_and_graph(ops, dev):
+    import torch
+
+    ids = rng(6).integers(-1, 2, 160).astype(np.int32)
+    ad, x, w, y = _case(ops, dev, 160, 512, 512, [16, 32], ids, bias=False)
+    t = torch.from_numpy(ids).to(dev)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        other = ops.lora_linear(x, w, ad, t)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            kept = ops.lora_linear(x, w, ad, t)
+        g.replay()
+        g.replay()
+    s.synchronize()
+    assert torch.equal(other, y) and torch.equal(kept, y)
+
+
+def test_lora_linear_refusals(pkg, ops, dev):
+    import torch
+
+    ad, x, w, y = _case(ops, dev, 12, 64, 64, [16], np.zeros(12, np.int32), bias=False)
+    t = torch.zeros(12, device=dev, dtype=torch.int32)
+    bad = [
+        (dict(x=x.float()), "BF16"), (dict(weight=w.float()), "BF16"),
+        (dict(ids=t.float()), "I32 or I64"), (dict(ids=t[:5]), "divide evenly"),
+        (dict(gate=torch.ones(64, device=dev)), "needs a residual"),
+        (dict(bias=torch.ones(63, device=dev)), "bias"),
+        (dict(residual=y.float()), "dtype"),
+        (dict(weight=torch.zeros(32, 64, device=dev, dtype=torch.bfloat16)), "lora_b"),
+        (dict(x=torch.zeros(12, 72, device=dev, dtype=torch.bfloat16)[:, 4:68]), "aligned"),
+        (dict(out_dtype=torch.float16), "y must be"),
+    ]
+    for kw, match in bad:
+        args = {"x": x, "weight": w, "adapters": ad, "ids": t} | kw
+        with pytest.raises(pkg._lib.L3dError, match=match):
+            ops.lora_linear(**args)
+    with pytest.raises(ValueError, match="finite"):
+        ops.LoraAdapters([torch.full((4, 64), float("inf"), device=dev)], [torch.zeros(64, 4, device=dev)])
+    with pytest.raises(ValueError, match="expected"):
+        ops.LoraAdapters([torch.zeros(4, 64, device=dev)], [torch.zeros(64, 5, device=dev)])
+    with pytest.raises(ValueError):
+        ops.LoraAdapters([], [])
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.lora_linear(x.cpu(), w, ad, t)
