@@ -1,66 +1,664 @@
 // Attention for a batch whose elements share a prefix of keys, plus each
-// element's own keys:
+// element's own keys, on the 5th-generation tensor cores:
 //   out[b, h, i] = sum_j softmax_j(scale q[b, h, i] . K[j]) V[j]
 // over the prefix keys j < P (one copy for the whole batch) and the own keys
 // j < lengths[b] of element b; with `causal`, row i sees the own keys up to
 // its own place, j <= lengths[b] - N + i.  Query heads h share the key head
-// h / (Hq / Hkv).  The reference's attention core is exact_sdpa_heads
+// h / G, G = Hq / Hkv.  The reference's attention core is exact_sdpa_heads
 // (crate/runtime/attention_math.rs:199-259); a shared prefix would be copied
 // into every batch element there.
+//
+// The query rows of one key head are numbered f = (b N + i) G + g: a tile of
+// 128 rows holds the rows of several query heads, and, for the prefix, of
+// several batch elements, so that the prefix keys are read once per tile of
+// rows and not once per element.  A block takes one item:
+//   packed   (row tiles over the whole batch) x (a chunk of prefix tiles), and
+//            (row tiles of one element) x (a chunk of its own key tiles);
+//   joint    (row tiles of one element) x (a chunk of prefix, then own tiles).
+// An item that sees all the keys of its rows stores the output; otherwise it
+// stores its part's O / l and log2 of its sum in f32, and combine_kernel
+// weighs the parts of each row.  Parts have fixed places, so results do not
+// depend on the order in which blocks run.
+//
+// Within an item the roles are those of attn.cu: a TMA warp fills a ring of
+// 128-key K and V tiles; MMA warps issue S = Q K^T and O += P V (P read from
+// tensor memory); four softmax warps per row tile, one row per thread, which
+// also load Q (their rows have no common stride) and zero the V rows past an
+// element's keys: a masked probability is 0, but 0 x NaN is not.
+// Every mbarrier wait is bounded (%globaltimer, 2 s); on expiry the block
+// records an error in the device's status word and stops.
+#include <type_traits>
+
+#include "attn.cuh"
 #include "common.cuh"
+#include "tc.cuh"
 
 namespace l3d {
 namespace pattn {
 
-struct Params {
-  int B, Hq, Hkv, N, D;
-  int64_t P, S;
-  const void *q, *pk, *pv, *k, *v;
-  void* out;
-  int64_t qb, qh, qn, pkh, pkn, pvh, pvn, kb, kh, kn, vb, vh, vn, ob, oh, on;  // element strides
-  const void* lengths;  // [B] or null (= S)
-  int len64, causal;
-  float scale;
+using namespace l3d::attn;
+
+constexpr int BQ = 128, BKV = 128;
+constexpr int TMEM_COLS = 512;
+constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
+// As in attn.cu: the running max moves only when it grows past 2^8.
+constexpr float RESCALE_LOG2 = 8.f;
+
+__device__ int g_pattn_status;
+
+// NT row tiles of 128 rows per block.
+template <int D, int NT>
+struct Cfg {
+  static constexpr int DC = D / 64;
+  static constexpr int Q_BYTES = BQ * D * 2;
+  static constexpr int KV_BYTES = BKV * D * 2;
+  static constexpr int STAGES = (227 * 1024 - 256 - NT * Q_BYTES) / (2 * KV_BYTES) < 6
+                                    ? (227 * 1024 - 256 - NT * Q_BYTES) / (2 * KV_BYTES) : 6;
+  static constexpr int SMEM = NT * Q_BYTES + STAGES * 2 * KV_BYTES + 256;
+  static constexpr uint32_t COL_S = 0, COL_O = NT * BKV;
+  // P_t has columns of its own where they fit, so that S_t(j + 1) is computed
+  // while the softmax of tile j runs; otherwise it goes over S_t.
+  static constexpr bool SEP_P = COL_O + NT * D + NT * (BKV / 2) <= TMEM_COLS;
+  static constexpr uint32_t COL_P = SEP_P ? COL_O + NT * D : COL_S;
+  static constexpr uint32_t P_STRIDE = SEP_P ? BKV / 2 : BKV;
+  static constexpr int NMMA = SEP_P ? NT : 1;
+  static constexpr int THREADS = (1 + NMMA + 4 * NT) * 32;
+  static constexpr int POLY = D == 64 ? 2 : 0;  // of 8 pairs of P, those of ex2_poly2
+  static_assert(COL_O + NT * D <= TMEM_COLS, "TMEM budget");
+  static_assert((2 * STAGES + 5 * NT + NMMA) * 8 + 16 <= 256, "barrier area");
 };
 
-// One query row per warp, keys one at a time, the head dim over the lanes.
+struct View {        // a K or V map: heads listed before rows; 0 for a broadcast dimension
+  int hn, hm, bm;
+};
+
+struct Params {
+  int B, N, G, Hkv;
+  int RG, F;                 // rows of one element, of the batch (per key head)
+  int64_t P, S;
+  View pk, pv, k, v;
+  const void* q;
+  void* out;
+  int64_t qb, qh, qn, ob, oh, on;  // element strides
+  const void* lengths;       // [B] or null (= S)
+  int len64, causal;
+  float scale_log2;          // softmax scale * log2(e), > 0
+  float *part_o, *part_l;    // [slots, Hkv, F, D], [slots, Hkv, F]; slots > 1
+  int slots, slots_p;        // parts of a row; those of the prefix (packed)
+  int joint;
+  int prefix_items, tiles_p, tiles_o;  // row tiles (of NT x 128) of the batch, of one element
+  int chunk_p, chunk_o;      // key tiles of an item
+  uint64_t wait_ns;
+};
+
+__device__ __forceinline__ int64_t own_length(const Params& p, int b) {
+  if (!p.lengths) return p.S;
+  const int64_t v = p.len64 ? static_cast<const int64_t*>(p.lengths)[b]
+                            : static_cast<const int32_t*>(p.lengths)[b];
+  return v < 0 ? 0 : v < p.S ? v : p.S;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
+  return pack_bf16x2(a, b);
+}
+template <> __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+// As make_idesc, for either 16-bit type.
 template <typename T>
-__global__ void __launch_bounds__(128) row_kernel(const Params p) {
-  const int lane = threadIdx.x & 31, E = p.D / 32;
-  const int64_t row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= int64_t(p.B) * p.Hq * p.N) return;
-  const int64_t i = row % p.N, h = row / p.N % p.Hq, b = row / p.N / p.Hq;
-  const int64_t kvh = h / (p.Hq / p.Hkv);
-  const T* qr = static_cast<const T*>(p.q) + b * p.qb + h * p.qh + i * p.qn;
-  float q[4], o[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int e = 0; e < E; ++e) q[e] = to_f(qr[lane + 32 * e]) * p.scale;
-  float m = -INFINITY, l = 0.f;
-  auto key = [&](const T* kr, const T* vr) {
-    float s = 0.f;
-    for (int e = 0; e < E; ++e) s = fmaf(q[e], to_f(kr[lane + 32 * e]), s);
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) s += __shfl_xor_sync(0xffffffffu, s, x);
-    const float mn = fmaxf(m, s);
-    const float alpha = mn == -INFINITY ? 1.f : expf(m - mn);
-    const float pr = mn == -INFINITY ? 0.f : expf(s - mn);
-    l = l * alpha + pr;
-    for (int e = 0; e < E; ++e) o[e] = o[e] * alpha + pr * to_f(vr[lane + 32 * e]);
-    m = mn;
-  };
-  for (int64_t j = 0; j < p.P; ++j)
-    key(static_cast<const T*>(p.pk) + kvh * p.pkh + j * p.pkn,
-        static_cast<const T*>(p.pv) + kvh * p.pvh + j * p.pvn);
-  int64_t len = p.S;
-  if (p.lengths) {
-    const int64_t v = p.len64 ? static_cast<const int64_t*>(p.lengths)[b] : static_cast<const int32_t*>(p.lengths)[b];
-    len = v < 0 ? 0 : v < p.S ? v : p.S;
+constexpr uint32_t idesc_of(int m, int n) {
+  return make_idesc(m, n) & ~(sizeof(T) == 2 && std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u);
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
+    prefix_kernel(const __grid_constant__ CUtensorMap map_pk,
+                  const __grid_constant__ CUtensorMap map_pv,
+                  const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const Params p) {
+  using C = Cfg<D, NT>;
+  constexpr uint32_t IDESC_S = idesc_of<T>(128, BKV);
+  constexpr uint32_t IDESC_O = idesc_of<T>(128, D) | (1u << 16);  // B (V) MN-major
+  int* const status = &g_pattn_status;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  if (smem_u32(smem_raw) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, ST_MISALIGNED);
+    return;
   }
-  if (p.causal && len - p.N + i + 1 < len) len = len - p.N + i + 1;
-  for (int64_t j = 0; j < len; ++j)
-    key(static_cast<const T*>(p.k) + b * p.kb + kvh * p.kh + j * p.kn,
-        static_cast<const T*>(p.v) + b * p.vb + kvh * p.vh + j * p.vn);
-  T* orow = static_cast<T*>(p.out) + b * p.ob + h * p.oh + i * p.on;
-  for (int e = 0; e < E; ++e) orow[lane + 32 * e] = from_f<T>(l != 0.f ? o[e] / l : 0.f);
+  uint8_t* sq = smem_raw;                            // [NT][DC][128 x 64]
+  uint8_t* sk = sq + NT * C::Q_BYTES;                // [STAGES][DC][128 x 64]
+  uint8_t* sv = sk + C::STAGES * C::KV_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sv + C::STAGES * C::KV_BYTES);
+  uint64_t* q_full = bars;                           // [NT]
+  uint64_t* kv_full = q_full + NT;                   // [STAGES]
+  uint64_t* kv_empty = kv_full + C::STAGES;          // [STAGES]
+  uint64_t* s_full = kv_empty + C::STAGES;           // [NT]
+  uint64_t* p_full = s_full + NT;                    // [NT]
+  uint64_t* pv_done = p_full + NT;                   // [NT] (SEP_P: every P V; else the last)
+  uint64_t* s_free = pv_done + NT;                   // [NT] (SEP_P only)
+  uint64_t* mma_drain = s_free + NT;                 // [NMMA] abort teardown only
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + C::NMMA);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + C::NMMA + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+  // ---- this block's item: rows [f0, fend) of key head h, prefix tiles
+  // [pa, pa + np), own tiles [sa, sa + nkv - np) of element b.
+  int idx = blockIdx.x;
+  int f0, fend, h, b = 0, pa, np, sa = 0, nkv, slot;
+  int64_t len = 0;
+  if (idx < p.prefix_items) {
+    const int qt = idx % p.tiles_p;
+    idx /= p.tiles_p;
+    h = idx % p.Hkv;
+    slot = idx / p.Hkv;
+    f0 = qt * (NT * BQ);
+    fend = p.F;
+    const int tiles = int((p.P + BKV - 1) / BKV);
+    pa = slot * p.chunk_p;
+    np = max(min(p.chunk_p, tiles - pa), 0);
+    nkv = np;
+  } else {
+    idx -= p.prefix_items;
+    const int qt = idx % p.tiles_o;
+    idx /= p.tiles_o;
+    h = idx % p.Hkv;
+    idx /= p.Hkv;
+    b = idx % p.B;
+    const int part = idx / p.B;
+    f0 = b * p.RG + qt * (NT * BQ);
+    fend = (b + 1) * p.RG;
+    len = own_length(p, b);
+    // Own keys that the last of the item's rows sees.
+    int64_t seen = len;
+    if (p.causal) {
+      const int64_t last = (min(f0 + NT * BQ, fend) - 1 - b * p.RG) / p.G;
+      seen = max(min(len, len - p.N + last + 1), int64_t(0));
+    }
+    const int own = int((seen + BKV - 1) / BKV);
+    const int pre = p.joint ? int((p.P + BKV - 1) / BKV) : 0;
+    const int c0 = part * p.chunk_o;
+    const int c1 = min(c0 + p.chunk_o, pre + own);
+    pa = min(c0, pre);
+    np = max(min(c1, pre) - pa, 0);
+    sa = max(c0 - pre, 0);
+    nkv = max(c1 - c0, 0);
+    slot = (p.joint ? 0 : p.slots_p) + part;
+  }
+  const int ntv = min((fend - f0 + BQ - 1) / BQ, NT);  // row tiles that hold rows
+  const int nmma = C::SEP_P ? ntv : 1;
+  int nload[C::STAGES];
+#pragma unroll
+  for (int s = 0; s < C::STAGES; ++s) nload[s] = 0;
+  // Key tile j (K and V) into ring stage j % STAGES (thread 0).
+  auto load_kv = [&](int j) {
+    const int s = j % C::STAGES;
+    ++nload[s];
+    mbar_expect_tx(&kv_full[s], 2 * C::KV_BYTES);
+    const bool pre = j < np;
+    const int row = (pre ? pa + j : sa + j - np) * BKV;
+    auto put = [&](uint8_t* dst, const CUtensorMap* map, const View& w) {
+      const int hh = h * w.hm, bb = pre ? 0 : b * w.bm;
+      for (int dc = 0; dc < C::DC; ++dc)
+        tma_load_4d(dst + dc * (BKV * 128), map, &kv_full[s], dc * 64, w.hn ? hh : row,
+                    w.hn ? row : hh, bb);
+    };
+    put(sk + s * C::KV_BYTES, pre ? &map_pk : &map_k, pre ? p.pk : p.k);
+    put(sv + s * C::KV_BYTES, pre ? &map_pv : &map_v, pre ? p.pv : p.v);
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], nmma);
+    }
+    for (int t = 0; t < NT; ++t) {
+      mbar_init(&q_full[t], 4);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&s_free[t], 4);
+      mbar_init(&pv_done[t], 1);
+    }
+    for (int w = 0; w < C::NMMA; ++w) mbar_init(&mma_drain[w], 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    for (int j = 0; j < nkv && j < C::STAGES; ++j) load_kv(j);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, p.wait_ns);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      for (int j = C::STAGES; j < nkv && !*abort_flag; ++j) {
+        if (!wait(&kv_empty[j % C::STAGES], ((j / C::STAGES) - 1) & 1)) break;
+        load_kv(j);
+      }
+    }
+  } else if (warp <= C::NMMA) {
+    // ------------------------------------------------------------------ MMA
+    constexpr int TPW = NT / C::NMMA;
+    const int t0 = (warp - 1) * TPW;
+    const int t1 = min(t0 + TPW, ntv);  // this warp's row tiles: t0 .. t1 - 1
+    if (lane == 0 && t0 < t1 && nkv > 0) {
+      auto issue_s = [&](int t, int j) {
+        const uint8_t* kt = sk + (j % C::STAGES) * C::KV_BYTES;
+        const uint8_t* qt = sq + t * C::Q_BYTES;
+#pragma unroll
+        for (int dc = 0; dc < C::DC; ++dc) {
+          const uint64_t da = smem_desc_sw128(qt + dc * (BQ * 128));
+          const uint64_t db = smem_desc_sw128(kt + dc * (BKV * 128));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            umma_f16<IDESC_S>(tmem_base + C::COL_S + t * BKV, da + uint64_t(2 * k),
+                              db + uint64_t(2 * k), (dc | k) ? 1u : 0u);
+        }
+        umma_commit(&s_full[t]);
+      };
+      auto issue_pv = [&](int t, int j) {
+        const uint64_t db = smem_desc_sw128_mn(sv + (j % C::STAGES) * C::KV_BYTES, BKV * 128);
+        const uint32_t ta = tmem_base + C::COL_P + t * C::P_STRIDE;
+#pragma unroll
+        for (int ks = 0; ks < BKV / 16; ++ks)
+          umma_f16_ts<IDESC_O>(tmem_base + C::COL_O + t * D, ta + uint32_t(ks * 8),
+                               db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
+      };
+      bool ok = true;
+      for (int t = t0; ok && t < t1; ++t) ok = wait(&q_full[t], 0);
+      ok = ok && wait(&kv_full[0], 0);
+      if (ok) {
+        tc_fence_after();
+        for (int t = t0; t < t1; ++t) issue_s(t, 0);
+      }
+      for (int j = 0; ok && j < nkv; ++j) {
+        const bool more = j + 1 < nkv;
+        bool kv_ready = !more;
+        auto wait_kv = [&]() {
+          if (!kv_ready) kv_ready = wait(&kv_full[(j + 1) % C::STAGES], ((j + 1) / C::STAGES) & 1);
+          return kv_ready;
+        };
+        for (int t = t0; ok && t < t1; ++t) {
+          if constexpr (C::SEP_P) {
+            // S_t(j+1) once the softmax warps have copied S_t(j), then P_t(j) V.
+            if (more) {
+              if (!wait_kv() || !wait(&s_free[t], j & 1)) { ok = false; break; }
+              tc_fence_after();
+              issue_s(t, j + 1);
+            }
+            if (!wait(&p_full[t], j & 1)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv(t, j);
+            umma_commit(&pv_done[t]);
+            if (t == t1 - 1) umma_commit(&kv_empty[j % C::STAGES]);
+          } else {
+            // P_t(j) V, then S_t(j+1) over the consumed P_t(j).
+            if (!wait(&p_full[t], j & 1)) { ok = false; break; }
+            tc_fence_after();
+            issue_pv(t, j);
+            if (t == t1 - 1) umma_commit(&kv_empty[j % C::STAGES]);
+            if (more) {
+              if (!wait_kv()) { ok = false; break; }
+              tc_fence_after();
+              issue_s(t, j + 1);
+            } else {
+              umma_commit(&pv_done[t]);
+            }
+          }
+        }
+      }
+    }
+  } else if ((warp - 1 - C::NMMA) >> 2 < ntv) {
+    // ------------------------------------------------------ softmax / epilogue
+    const int t = (warp - 1 - C::NMMA) >> 2;
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int f = f0 + t * BQ + r;
+    const bool valid = f < fend;
+    const bool active = f - lane < fend;  // the warp holds rows
+    // Row f = (fb N + fi) G + fg.
+    const int ff = valid ? f : fend - 1;
+    const int fb = ff / p.RG, fi = (ff - fb * p.RG) / p.G, fg = ff - fb * p.RG - fi * p.G;
+    {
+      const T* qr = static_cast<const T*>(p.q) + fb * p.qb + int64_t(h * p.G + fg) * p.qh + fi * p.qn;
+      uint8_t* qt = sq + t * C::Q_BYTES + r * 128;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 u = make_uint4(0, 0, 0, 0);
+        if (valid) u = __ldg(reinterpret_cast<const uint4*>(qr) + c);
+        *reinterpret_cast<uint4*>(qt + (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4)) = u;
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_full[t]);
+    }
+    // Own keys that this row sees.
+    const int64_t lim = p.causal ? min(len, len - p.N + fi + 1) : len;
+    const uint32_t lane_off = uint32_t(quarter * 32) << 16;
+    const uint32_t t_s = tmem_base + C::COL_S + t * BKV + lane_off;
+    const uint32_t t_o = tmem_base + C::COL_O + t * D + lane_off;
+    const uint32_t t_p = tmem_base + C::COL_P + t * C::P_STRIDE + lane_off;
+    const float2 sc2 = f2(p.scale_log2);
+    float m = -INFINITY;                         // running max, log2 units
+    float2 l2 = f2(0.f);                         // running row sum (two halves)
+    bool ok = true;
+    for (int j = 0; j < nkv; ++j) {
+      if (!wait(&s_full[t], j & 1)) { ok = false; break; }
+      tc_fence_after();
+      const bool pre = j < np;
+      const int64_t key0 = int64_t(pre ? pa + j : sa + j - np) * BKV;
+      // V rows past the element's keys may hold anything (S(j) complete means
+      // that the tile has landed).
+      const int held = int(min(pre ? int64_t(BKV) : len - key0, int64_t(BKV)));
+      if (r >= held) {
+        uint8_t* vr = sv + (j % C::STAGES) * C::KV_BYTES + r * 128;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c)
+          *reinterpret_cast<uint4*>(vr + (c >> 3) * (BKV * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+      }
+      if (held < BKV) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      bool pv_waited = !C::SEP_P || j == 0;
+      auto wait_pv = [&]() {  // P_t(j-1) V has read P_t and O_t is stable
+        if (pv_waited) return true;
+        pv_waited = wait(&pv_done[t], (j - 1) & 1);
+        tc_fence_after();
+        return pv_waited;
+      };
+      if (!active) {  // no rows: keep the other warps' pace
+        if constexpr (C::SEP_P) {
+          if (lane == 0) mbar_arrive(&s_free[t]);
+        }
+        if (!wait_pv()) { ok = false; break; }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+        continue;
+      }
+      float sv_[BKV];
+#pragma unroll
+      for (int c = 0; c < BKV; c += 64) tmem_ld64(t_s + uint32_t(c), sv_ + c);
+      if constexpr (C::SEP_P) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[t]);
+      }
+      const int64_t kv64 = (pre ? p.P : lim) - key0;  // keys of this tile that the row sees
+      if (kv64 < BKV) {
+        const int kvalid = int(max(kv64, int64_t(0)));
+#pragma unroll
+        for (int e = 0; e < BKV; ++e)
+          if (e >= kvalid) sv_[e] = -INFINITY;
+      }
+      __syncwarp();
+      float mx0 = sv_[0], mx1 = sv_[1];
+#pragma unroll
+      for (int e = 2; e < BKV; e += 2) {
+        mx0 = fmaxf(mx0, sv_[e]);
+        mx1 = fmaxf(mx1, sv_[e + 1]);
+      }
+      const float mxs = fmaxf(mx0, mx1) * p.scale_log2;  // scale > 0
+      const bool grow = mxs > m + RESCALE_LOG2;          // always on the first key a row sees
+      const float m_new = grow ? mxs : m;
+      const float alpha = grow ? ex2f(m - m_new) : 1.f;  // 0 on the first
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        if (!wait_pv()) { ok = false; break; }
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          float o[32];
+          tmem_ld32(t_o + uint32_t(c), o);
+          uint32_t u[32];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
+            u[e] = __float_as_uint(v.x);
+            u[e + 1] = __float_as_uint(v.y);
+          }
+          tmem_st32u(t_o + uint32_t(c), u);
+        }
+      }
+      // P = exp2(s * scale * log2 e - m); a row that has seen no key yet has
+      // m = -inf and all its scores masked: subtract 0, so that P = 0.
+      const float2 nm2 = f2(m_new == -INFINITY ? 0.f : -m_new);
+      l2 = mul2(l2, f2(alpha));
+      uint32_t u[BKV / 2];
+#pragma unroll
+      for (int e = 0; e < BKV; e += 2) {
+        const float2 x = fma2(make_float2(sv_[e], sv_[e + 1]), sc2, nm2);
+        const float2 pr = ((e >> 1) & 7) < C::POLY ? ex2_poly2(x)
+                                                   : make_float2(ex2f(x.x), ex2f(x.y));
+        l2 = add2(l2, pr);
+        u[e >> 1] = pack_pair<T>(pr.x, pr.y);
+      }
+      if (!wait_pv()) { ok = false; break; }
+#pragma unroll
+      for (int c = 0; c < BKV / 2; c += 32) tmem_st32u(t_p + uint32_t(c), u + c);
+      tmem_wait_st();
+      m = m_new;
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[t]);
+    }
+    // Epilogue, after the last P V: the output, or this part's O / l and log2 sum.
+    if (ok && nkv > 0)
+      ok = mbar_wait_idle(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0, abort_flag, status, ST_TIMEOUT, p.wait_ns);
+    if (ok && active) {
+      tc_fence_after();
+      // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)
+      const float l = m == -INFINITY && l2.x == l2.x && l2.y == l2.y ? 0.f : l2.x + l2.y;
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
+      const int64_t pr = (int64_t(slot) * p.Hkv + h) * p.F + f;
+      if (p.slots > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
+      T* orow = static_cast<T*>(p.out) + fb * p.ob + int64_t(h * p.G + fg) * p.oh + fi * p.on;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (nkv > 0) {
+          tmem_ld32(t_o + uint32_t(c), o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
+          if (p.slots > 1) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float w[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) w[e] = o[8 * q + e];
+              *reinterpret_cast<uint4*>(orow + c + 8 * q) = pack(w, T());
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // Teardown, as in attn.cu: after an abort nothing the block started may
+  // still be running when it frees TMEM and exits.
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (warp >= 1 && warp <= C::NMMA && lane == 0) {
+      umma_commit(&mma_drain[warp - 1]);
+      mbar_drain(&mma_drain[warp - 1], 0, p.wait_ns);
+    }
+    if (threadIdx.x == 0) {
+#pragma unroll
+      for (int s = 0; s < C::STAGES; ++s)
+        if (nload[s] > 0) mbar_drain(&kv_full[s], uint32_t(nload[s] - 1) & 1u, p.wait_ns);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(TMEM_COLS));
+  }
+}
+
+// The parts of each row weighed by 2^(their log2 sum - the largest): one warp
+// per row, D / 32 elements per lane.
+constexpr int MAX_SLOTS = 64;
+template <typename T, int D>
+__global__ void __launch_bounds__(256) combine_kernel(const Params p) {
+  constexpr int E = D / 32;
+  const int lane = threadIdx.x & 31;
+  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);  // h F + f
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (row >= int64_t(p.Hkv) * p.F) return;
+  const int64_t stride = int64_t(p.Hkv) * p.F;
+  float w[MAX_SLOTS / 32], mx = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
+    const int s = lane + 32 * i;
+    w[i] = s < p.slots ? p.part_l[s * stride + row] : -INFINITY;
+    mx = fmaxf(mx, w[i]);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
+    w[i] = w[i] == -INFINITY ? 0.f : exp2f(w[i] - mx);
+    sum += w[i];
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  float acc[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
+    const int n = min(p.slots - 32 * i, 32);
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float ws = __shfl_sync(0xffffffffu, w[i], s);
+      if (ws == 0.f) continue;  // a part without keys
+      const float* src = p.part_o + ((32 * i + s) * stride + row) * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        acc[0] = fmaf(ws, v.x, acc[0]);
+        acc[1] = fmaf(ws, v.y, acc[1]);
+        acc[2] = fmaf(ws, v.z, acc[2]);
+        acc[3] = fmaf(ws, v.w, acc[3]);
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(ws, v.x, acc[0]);
+        acc[1] = fmaf(ws, v.y, acc[1]);
+      }
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  const int f = int(row % p.F), h = int(row / p.F);
+  const int fb = f / p.RG, fi = (f - fb * p.RG) / p.G, fg = f - fb * p.RG - fi * p.G;
+  T* orow = static_cast<T*>(p.out) + fb * p.ob + int64_t(h * p.G + fg) * p.oh + fi * p.on + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; ++e) orow[e] = from_f<T>(acc[e] * inv);
+}
+
+// How the rows and keys are divided into items (host).
+struct Plan {
+  int nt, joint, tiles_p, tiles_o, chunk_p, chunk_o, slots_p, slots, items;
+};
+
+static Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t P, int64_t S) {
+  auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t RG = N * (Hq / Hkv), F = B * RG;
+  const int64_t kp = up(P, BKV), ko = up(S, BKV);
+  Plan pl{};
+  // One row tile per block while an element's rows fit it.
+  pl.nt = RG <= BQ && (S > 0 || F <= BQ) ? 1 : 2;
+  const int64_t rows = int64_t(pl.nt) * BQ;
+  pl.tiles_p = int(up(F, rows));
+  pl.tiles_o = int(up(RG, rows));
+  // Packed rows share the prefix between elements; joint items need no parts.
+  // Work in (row tile) x (key tile):
+  const int64_t packed = Hkv * (pl.tiles_p * kp + B * pl.tiles_o * ko);
+  const int64_t joint = Hkv * B * pl.tiles_o * (kp + ko);
+  pl.joint = S > 0 && joint * 10 <= packed * 11;
+  const int64_t work = pl.joint ? joint : packed;
+  int64_t chunk = up(work, sm_count());
+  if (chunk < 2) chunk = 2;
+  const int64_t kmax = pl.joint ? kp + ko : kp > ko ? kp : ko;
+  const int64_t half = MAX_SLOTS / 2;
+  if (chunk * half < kmax) chunk = up(kmax, half);
+  if (pl.joint) {
+    pl.chunk_o = int(chunk);
+    pl.slots = int(up(kp + ko, chunk));
+    if (pl.slots < 1) pl.slots = 1;
+    pl.items = int(Hkv * B * pl.tiles_o * pl.slots);
+  } else {
+    pl.chunk_p = pl.chunk_o = int(chunk);
+    pl.slots_p = int(up(kp, chunk));
+    const int64_t so = up(ko, chunk);
+    if (pl.slots_p + so < 1) pl.slots_p = 1;
+    pl.slots = pl.slots_p + int(so);
+    pl.items = int(Hkv * (pl.tiles_p * pl.slots_p + B * pl.tiles_o * so));
+  }
+  return pl;
+}
+
+template <typename T, int D, int NT>
+static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int items, cudaStream_t s) {
+  auto k = prefix_kernel<T, D, NT>;
+  const cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<D, NT>::SMEM);
+  if (e != cudaSuccess) return e;
+  k<<<unsigned(items), Cfg<D, NT>::THREADS, Cfg<D, NT>::SMEM, s>>>(maps[0], maps[1], maps[2], maps[3], p);
+  if (p.slots <= 1) return cudaGetLastError();
+  // The combination may be scheduled while the items finish; it waits for them.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((int64_t(p.Hkv) * p.F + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p);
+}
+
+template <typename T>
+static cudaError_t launch_d(int D, int nt, const CUtensorMap (&maps)[4], const Params& p, int items,
+                            cudaStream_t s) {
+  if (D == 64) return nt == 1 ? launch<T, 64, 1>(maps, p, items, s) : launch<T, 64, 2>(maps, p, items, s);
+  return nt == 1 ? launch<T, 128, 1>(maps, p, items, s) : launch<T, 128, 2>(maps, p, items, s);
+}
+
+// The map of a K or V view [B, H, rows, D]; a broadcast dimension (stride 0)
+// is described once.
+static bool make_view(CUtensorMap* m, View* w, const void* base, int64_t B, int64_t H, int64_t rows,
+                      int64_t D, int64_t sb, int64_t sh, int64_t sn) {
+  w->bm = B > 1 && sb == 0 ? 0 : 1;
+  w->hm = H > 1 && sh == 0 ? 0 : 1;
+  return make_map4(m, base, w->bm ? B : 1, w->hm ? H : 1, rows, D, sn, sh, sb, BKV, &w->hn);
+}
+
+cudaError_t status_read(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_pattn_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_pattn_status, &zero, sizeof(int));
+  }
+  return e;
 }
 
 }  // namespace pattn
@@ -71,8 +669,10 @@ using namespace l3d;
 extern "C" size_t l3d_shared_prefix_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv,
                                                              int64_t n, int64_t p, int64_t s,
                                                              int64_t d) {
-  (void)b; (void)hq; (void)hkv; (void)n; (void)p; (void)s; (void)d;
-  return 0;
+  if (b <= 0 || hq <= 0 || hkv <= 0 || n <= 0 || p < 0 || s < 0 || d <= 0 || hq % hkv) return 0;
+  const l3d::pattn::Plan pl = l3d::pattn::make_plan(b, hq, hkv, n, p, s);
+  // O and the log2 sums of each row's parts, in f32.
+  return pl.slots > 1 ? size_t(pl.slots) * size_t(b) * size_t(hq) * size_t(n) * (size_t(d) + 1) * 4 : 0;
 }
 
 extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor* prefix_k,
@@ -123,6 +723,10 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
   const int64_t big = int64_t(1) << 30;
   if (B > 65535 || Hq > 65535 || N > big || P > big || S > big || B * Hq * N > big)
     return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large", op);
+  const l3d_tensor* kvs[] = {prefix_k, prefix_v, k, v};
+  for (const l3d_tensor* t : kvs)
+    if (t && t->dims[t->ndim - 2] > 1 && t->strides[t->ndim - 2] == 0)
+      return fail(L3D_E_ALIGN, "%s: the keys must not be expanded (stride 0)", op);
   const size_t need = l3d_shared_prefix_attention_workspace_size(B, Hq, Hkv, N, P, S, D);
   if (need && (!workspace || workspace_bytes < need))
     return fail(L3D_E_WORKSPACE, "%s: workspace of %zu bytes required", op, need);
@@ -140,27 +744,41 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
       if (t->dims[d] > 1 && t->strides[d] % 8)
         return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
   }
+  const Plan pl = make_plan(B, Hq, Hkv, N, P, S);
   Params p{};
-  p.B = int(B); p.Hq = int(Hq); p.Hkv = int(Hkv); p.N = int(N); p.D = int(D);
+  p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);
+  p.RG = int(N * p.G); p.F = int(B) * p.RG;
   p.P = P; p.S = S;
-  p.q = elem_ptr(q); p.pk = elem_ptr(prefix_k); p.pv = elem_ptr(prefix_v);
-  p.k = k ? elem_ptr(k) : nullptr; p.v = v ? elem_ptr(v) : nullptr;
+  p.q = elem_ptr(q);
   p.out = const_cast<char*>(elem_ptr(out));
   p.qb = q->strides[0]; p.qh = q->strides[1]; p.qn = q->strides[2];
   p.ob = out->strides[0]; p.oh = out->strides[1]; p.on = out->strides[2];
-  p.pkh = prefix_k->strides[0]; p.pkn = prefix_k->strides[1];
-  p.pvh = prefix_v->strides[0]; p.pvn = prefix_v->strides[1];
-  if (k) {
-    p.kb = k->strides[0]; p.kh = k->strides[1]; p.kn = k->strides[2];
-    p.vb = v->strides[0]; p.vh = v->strides[1]; p.vn = v->strides[2];
-  }
   p.lengths = lengths ? elem_ptr(lengths) : nullptr;
   p.len64 = lengths && lengths->dtype == L3D_I64;
   p.causal = causal != 0;
-  p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f;
+  p.slots = pl.slots; p.slots_p = pl.slots_p; p.joint = pl.joint;
+  p.tiles_p = pl.tiles_p; p.tiles_o = pl.tiles_o;
+  p.chunk_p = pl.chunk_p; p.chunk_o = pl.chunk_o;
+  p.prefix_items = pl.joint ? 0 : int(Hkv) * pl.tiles_p * pl.slots_p;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_l = p.part_o + size_t(pl.slots) * Hkv * p.F * D;
+  p.wait_ns = l3d::tc::WAIT_LIMIT_NS;
+  // Views without elements are never read; any valid map stands in for theirs.
+  CUtensorMap maps[4];
+  bool ok = true;
+  if (P > 0)
+    ok = make_view(&maps[0], &p.pk, elem_ptr(prefix_k), 1, Hkv, P, D, 0, prefix_k->strides[0], prefix_k->strides[1]) &&
+         make_view(&maps[1], &p.pv, elem_ptr(prefix_v), 1, Hkv, P, D, 0, prefix_v->strides[0], prefix_v->strides[1]);
+  if (ok && S > 0)
+    ok = make_view(&maps[2], &p.k, elem_ptr(k), B, Hkv, S, D, k->strides[0], k->strides[1], k->strides[2]) &&
+         make_view(&maps[3], &p.v, elem_ptr(v), B, Hkv, S, D, v->strides[0], v->strides[1], v->strides[2]);
+  if (!ok) return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed", op);
+  if (P == 0 && S > 0) { maps[0] = maps[2]; maps[1] = maps[3]; }
+  if (S == 0 && P > 0) { maps[2] = maps[0]; maps[3] = maps[1]; }
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  const unsigned grid = unsigned((B * Hq * N + 3) / 4);
-  if (q->dtype == L3D_BF16) row_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(p);
-  else row_kernel<__half><<<grid, 128, 0, s>>>(p);
-  return check_launch(op);
+  const cudaError_t e = q->dtype == L3D_BF16 ? launch_d<__nv_bfloat16>(int(D), pl.nt, maps, p, pl.items, s)
+                                             : launch_d<__half>(int(D), pl.nt, maps, p, pl.items, s);
+  if (e != cudaSuccess) return fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  return L3D_OK;
 }
