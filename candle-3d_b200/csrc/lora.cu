@@ -4,87 +4,611 @@
 // projection is the reference's Linear::forward / ops::mul_mat_add
 // (crate/runtime/nn_blocks.rs:82,179-195) with the element-wise ops of its
 // blocks; the adapters have no counterpart there.
+//
+// Two launches.  shrink_kernel forms t[m] = scale_a A_a x[m] (rank columns)
+// in f32 and stores it as two bf16 parts.  lora_gemm_kernel then runs one product whose K
+// axis is x's, followed by the ranks of the adapters that occur in a 128-row
+// tile, 16 at a time: a slot multiplies the 128 x 16 piece of t, zero in the
+// rows of other adapters, by the BN x 16 piece of B_a.  The zeros add nothing,
+// so a row's result does not depend on its neighbours; and each B_a is read
+// once per tile however many rows use it, which is all that a row-by-row
+// batch has to read.
+//
+// lora_gemm_kernel is persistent, one block per SM, 128 x BN tiles, K in steps
+// of 64 through a ring of shared-memory stages:
+//   warp 0       TMA: x and W tiles (128B swizzle); in the slot stages the
+//                B_a pieces (32-byte rows, 32B swizzle), up to four per stage;
+//   warp 1       tcgen05.mma (M 128, N BN, K 16) into a double-buffered TMEM
+//                accumulator;
+//   warps 2..5   one row per thread: the tile's list of distinct adapters, and
+//                the t pieces of the slot stages, written to shared memory;
+//   warps 6..13  epilogue: TMEM lane quarter = warp % 4, half of the columns
+//                each; bias, activation, gated residual, store.
+// It is launched while shrink_kernel still runs (its x W^T part does not need
+// t); the t warps wait for it.  Every mbarrier wait is bounded (%globaltimer,
+// 2 s); on expiry the block records an error in the device's status word,
+// stops issuing work and still releases its TMEM.
 #include "act.cuh"
 #include "common.cuh"
+#include "epilogue.cuh"
+#include "tc.cuh"
 
 namespace l3d {
 namespace lora {
 
+using namespace l3d::tc;
+
 struct Params {
   int M, N, K, R, A;
-  const __nv_bfloat16 *x, *w, *a, *b;
-  int64_t x_ld, w_ld, y_ld, res_ld;
+  const __nv_bfloat16 *x, *a;
+  int64_t x_ld, y_ld, res_ld;
   const float* scale;     // [A]
   const int32_t* ranks;   // [A] or null (= R)
   const void* ids;        // row m has id ids[m / per]
   int ids64, per;
   const void* bias;
-  int bias_dtype;
+  int bias_dtype, bias_vec;
   const void* gate;
   int gate_dtype;
   const void* res;
+  int res_vec;
   void* y;
-  int y_dtype, act;
-  float* t;               // [M, R] scale_a A_a x[m]
+  int y_dtype, y_vec, act;
+  __nv_bfloat16* t;       // [PARTS, M, R] scale_a A_a x[m] and its rounding error
+  uint64_t wait_ns;
 };
+
+// t enters the second product as the sum of two bf16 numbers: one alone would
+// be off by up to 2^-8 of B_a t, as much as the rounding of a bf16 y; the pair
+// is off by 2^-16 and costs one more K-16 product per slot (4% at rank 64 and
+// K = 1536).
+constexpr int PARTS = 2;
+
+__device__ int g_lora_status;
+constexpr int ST_TIMEOUT = 5;
 
 __device__ __forceinline__ int adapter_of(const Params& p, int m) {
   const int g = m / p.per;
   const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[g] : static_cast<const int32_t*>(p.ids)[g];
   return id >= 0 && id < p.A ? int(id) : -1;
 }
-__device__ __forceinline__ float vec_at(const void* v, int dtype, int i) {
-  return dtype == L3D_F32 ? static_cast<const float*>(v)[i]
-                          : __bfloat162float(static_cast<const __nv_bfloat16*>(v)[i]);
+// Slots of 16 ranks that adapter a takes.
+__device__ __forceinline__ int slots_of(const Params& p, int a) {
+  return ((p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R) + 15) / 16;
 }
 
-// One row per block, one rank per warp at a time.
-__global__ void __launch_bounds__(256) shrink_kernel(const Params p) {
-  const int m = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int a = adapter_of(p, m);
-  const int rank = a < 0 ? 0 : p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R;
-  const __nv_bfloat16* xr = p.x + int64_t(m) * p.x_ld;
-  for (int r = warp; r < p.R; r += 8) {
-    float acc = 0.f;
-    if (r < rank) {
-      const __nv_bfloat16* ar = p.a + (int64_t(a) * p.R + r) * p.K;
-      for (int k = lane; k < p.K; k += 32) acc = fmaf(to_f(xr[k]), to_f(ar[k]), acc);
+// --------------------------------------------------------------------- shrink
+__device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// t for a group of 16 MT WR rows; 8 warps = WR (rows) x WN (32 ranks each) x
+// WK (K interleaved in chunks of 32, summed through shared memory in a fixed
+// order).  A lane loads 8 consecutive k of a row at once and uses them as the
+// operands of two K-16 products: both operands permute k alike, so the sums
+// are the same and every load is 16 bytes.  blockIdx.y strides over the
+// distinct adapters of the group.
+template <int MT, int WR, int WN, int WK>
+__global__ void __launch_bounds__(256, 2) shrink_kernel(const Params p) {
+  constexpr int ROWS = 16 * MT * WR, NT = 4, RB = 32 * WN;
+  static_assert(WR * WN * WK == 8, "eight warps");
+  __shared__ float red[WK][ROWS][RB + 4];
+  __shared__ int s_id[ROWS], s_list[ROWS], s_wcount[8];
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wk = warp % WK, wn = (warp / WK) % WN, wr = warp / (WK * WN);
+  const int g = lane >> 2, t4 = lane & 3;
+  const int m0 = blockIdx.x * ROWS;
+  // The distinct adapters of the group, in the order of their first rows.
+  const int mine = tid < ROWS && m0 + tid < p.M ? adapter_of(p, m0 + tid) : -1;
+  if (tid < ROWS) s_id[tid] = mine;
+  __syncthreads();
+  bool first = mine >= 0;
+  for (int q = 0; first && q < tid; ++q) first = s_id[q] != mine;
+  const uint32_t firsts = __ballot_sync(0xffffffffu, first);
+  if (lane == 0) s_wcount[warp] = __popc(firsts);
+  __syncthreads();
+  int before = 0, count = 0;
+#pragma unroll
+  for (int w = 0; w < (ROWS + 31) / 32; ++w) {
+    if (w < warp) before += s_wcount[w];
+    count += s_wcount[w];
+  }
+  if (first) s_list[before + __popc(firsts & ((1u << lane) - 1))] = mine;
+  __syncthreads();
+  const __nv_bfloat16* xr[MT][2];
+  bool xok[MT][2];
+#pragma unroll
+  for (int i = 0; i < MT; ++i)
+#pragma unroll
+    for (int hf = 0; hf < 2; ++hf) {
+      const int m = m0 + (wr * MT + i) * 16 + hf * 8 + g;
+      xok[i][hf] = m < p.M;
+      xr[i][hf] = p.x + int64_t(xok[i][hf] ? m : 0) * p.x_ld + 8 * t4;
     }
+  const int chunks = (p.K + 31) / 32;
+  for (int d = blockIdx.y; d < count; d += gridDim.y) {
+    const int a = s_list[d];
+    const int rank = slots_of(p, a) * 16;
+    for (int r0 = 0; r0 < rank; r0 += RB) {
+      const int rb = r0 + wn * 32;
+      const int nt = min((rank - rb) / 8, NT);  // 8-rank tiles of this warp
+      float c[MT][NT][4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
-    if (lane == 0) p.t[int64_t(m) * p.R + r] = r < rank ? acc * p.scale[a] : 0.f;
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
+      const __nv_bfloat16* ar = p.a + (int64_t(a) * p.R + rb + g) * p.K + 8 * t4;
+      if (nt > 0) {
+#pragma unroll 2
+        for (int kc = wk; kc < chunks; kc += WK) {
+          const int k = kc * 32;
+          const bool kok = k + 8 * t4 < p.K;
+          uint4 xv[MT][2], av[NT];
+          const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf)
+              xv[i][hf] = kok && xok[i][hf] ? __ldg(reinterpret_cast<const uint4*>(xr[i][hf] + k)) : zero;
+#pragma unroll
+          for (int j = 0; j < NT; ++j)
+            av[j] = kok && j < nt ? __ldg(reinterpret_cast<const uint4*>(ar + int64_t(8 * j) * p.K + k)) : zero;
+#pragma unroll
+          for (int j = 0; j < NT; ++j) {
+            if (j < nt) {
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                mma_16816(c[i][j], xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y, av[j].x, av[j].y);
+                mma_16816(c[i][j], xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w, av[j].z, av[j].w);
+              }
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          const int row = (wr * MT + i) * 16 + g, col = wn * 32 + j * 8 + 2 * t4;
+          *reinterpret_cast<float2*>(&red[wk][row][col]) = make_float2(c[i][j][0], c[i][j][1]);
+          *reinterpret_cast<float2*>(&red[wk][row + 8][col]) = make_float2(c[i][j][2], c[i][j][3]);
+        }
+      __syncthreads();
+      const float sc = p.scale[a];
+      for (int e = tid; e < ROWS * RB; e += 256) {
+        const int row = e / RB, col = e % RB;
+        if (s_id[row] != a || r0 + col >= rank) continue;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) v += red[w][row][col];
+        v *= sc;
+        const int64_t at = int64_t(m0 + row) * p.R + r0 + col;
+        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+        p.t[at] = hi;
+        p.t[int64_t(p.M) * p.R + at] = __float2bfloat16_rn(v - __bfloat162float(hi));
+      }
+      __syncthreads();
+    }
   }
 }
 
-// 16 rows x 16 columns per block.
-__global__ void __launch_bounds__(256) expand_kernel(const Params p) {
-  __shared__ float sx[16][17], sw[16][17];
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int m = blockIdx.y * 16 + ty, n = blockIdx.x * 16 + tx, nl = blockIdx.x * 16 + ty;
-  float acc = 0.f;
-  for (int k0 = 0; k0 < p.K; k0 += 16) {
-    const int k = k0 + tx;
-    sx[ty][tx] = m < p.M && k < p.K ? to_f(p.x[int64_t(m) * p.x_ld + k]) : 0.f;
-    sw[ty][tx] = nl < p.N && k < p.K ? to_f(p.w[int64_t(nl) * p.w_ld + k]) : 0.f;
-    __syncthreads();
+// ----------------------------------------------------------------------- gemm
+constexpr int BM = 128, BK = 64;
+constexpr int A_BYTES = BM * BK * 2;
+constexpr int SLOT_A = BM * 32;          // a t piece: 128 rows of 32 bytes
+constexpr int PER_STAGE = A_BYTES / (PARTS * SLOT_A);  // slots of a stage
+constexpr int THREADS = 14 * 32;
+
+template <int BN>
+struct Cfg {
+  static constexpr int B_BYTES = BN * BK * 2;
+  static constexpr int SLOT_B = BN * 32;
+  static constexpr int NST = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int LISTS = 2 * (2 * BM + 1) * 4 + BM * 4 + 64;
+  static constexpr int SMEM = NST * (A_BYTES + B_BYTES) + 512 + LISTS;
+  static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;  // a power of two
+  static_assert(SMEM <= 227 * 1024, "shared memory budget");
+  static_assert((4 * NST + 9) * 8 + 16 <= 512, "barrier area");
+};
+
+// K-major operand of 32-byte rows, 32B-swizzled: 8-row groups 256 B apart.
+__device__ __forceinline__ uint64_t smem_desc_sw32(const void* tile) {
+  const uint64_t addr = smem_u32(tile);
+  uint64_t d = 0;
+  d |= (addr >> 4) & 0x3fffull;
+  d |= uint64_t(1) << 16;
+  d |= uint64_t(256 >> 4) << 32;
+  d |= uint64_t(1) << 46;
+  d |= uint64_t(6) << 61;                // SWIZZLE_32B
+  return d;
+}
+
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+    lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
+                     const __grid_constant__ CUtensorMap map_b, const Params p) {
+  using C = Cfg<BN>;
+  constexpr int NST = C::NST;
+  constexpr uint32_t IDESC = make_idesc(BM, BN);
+  int* const status = &g_lora_status;
+  extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: 1024-byte aligned
+  uint8_t* sa = smem;
+  uint8_t* sb = sa + NST * A_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sb + NST * C::B_BYTES);
+  uint64_t* full = bars;                 // [NST] TMA landed
+  uint64_t* empty = full + NST;          // [NST] MMA has read the stage
+  uint64_t* tgo = empty + NST;           // [NST] the stage is free for t pieces
+  uint64_t* tfull = tgo + NST;           // [NST] the t pieces of a slot stage are written
+  uint64_t* acc_full = tfull + NST;      // [2]
+  uint64_t* acc_empty = acc_full + 2;    // [2]
+  uint64_t* list_full = acc_empty + 2;   // [2]
+  uint64_t* list_empty = list_full + 2;  // [2]
+  uint64_t* drain = list_empty + 2;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1) + 1;
+  // Per tile parity: the distinct adapters and the first slot of each; the
+  // last entry of `first` + 1 is the number of slots (kept in `total`).
+  int* ids = reinterpret_cast<int*>(bars + 64);
+  int* list_id = ids + BM;               // [2][BM]
+  int* list_end = list_id + 2 * BM;      // [2][BM] slots up to and with this adapter
+  int* total = list_end + 2 * BM;        // [2]
+  int* wsum = total + 2;                 // [8] per-warp sums of the list builders
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int num_n = (p.N + BN - 1) / BN;
+  const int tiles = ((p.M + BM - 1) / BM) * num_n;
+  const int kblocks = (p.K + BK - 1) / BK;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < NST; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+      mbar_init(&tgo[s], 1);
+      mbar_init(&tfull[s], 4);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 8);
+      mbar_init(&list_full[i], 4);
+      mbar_init(&list_empty[i], 2);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(C::TMEM));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, p.wait_ns);
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      int it = 0;  // ring position
+      bool ok = true;
+      int nt = 0;
+      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++nt) {
+        const int m0 = (tile / num_n) * BM, n0 = (tile % num_n) * BN;
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % NST;
+          if (it >= NST && !wait(&empty[s], (it / NST - 1) & 1)) { ok = false; break; }
+          mbar_expect_tx(&full[s], A_BYTES + C::B_BYTES);
+          tma_load_2d(sa + s * A_BYTES, &map_x, &full[s], kb * BK, m0);
+          tma_load_2d(sb + s * C::B_BYTES, &map_w, &full[s], kb * BK, n0);
+        }
+        const int lb = nt & 1;
+        if (!ok || !wait(&list_full[lb], (nt >> 1) & 1)) break;
+        const int slots = total[lb];
+        int d = 0, first = 0;  // adapter of the slot, its first slot
+        for (int q0 = 0; q0 < slots; q0 += PER_STAGE, ++it) {
+          const int s = it % NST, n = min(PER_STAGE, slots - q0);
+          if (it >= NST && !wait(&empty[s], (it / NST - 1) & 1)) { ok = false; break; }
+          mbar_arrive(&tgo[s]);
+          mbar_expect_tx(&full[s], n * C::SLOT_B);
+          for (int q = q0; q < q0 + n; ++q) {
+            while (q >= list_end[lb * BM + d]) first = list_end[lb * BM + d++];
+            tma_load_3d(sb + s * C::B_BYTES + (q - q0) * C::SLOT_B, &map_b, &full[s], (q - first) * 16,
+                        n0, list_id[lb * BM + d]);
+          }
+        }
+        mbar_arrive(&list_empty[lb]);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA
+    if (lane == 0) {
+      int it = 0, nt = 0;
+      uint32_t tph = 0;  // parity of each stage's next tfull phase
+      bool ok = true;
+      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++nt) {
+        const int acc = nt & 1;
+        if (nt >= 2 && !wait(&acc_empty[acc], (nt / 2 - 1) & 1)) break;
+        tc_fence_after();
+        const uint32_t d = tmem_base + uint32_t(acc * BN);
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % NST;
+          if (!wait(&full[s], (it / NST) & 1)) { ok = false; break; }
+          tc_fence_after();
+          const uint64_t da = smem_desc_sw128(sa + s * A_BYTES), db = smem_desc_sw128(sb + s * C::B_BYTES);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) acc = fmaf(sx[ty][i], sw[tx][i], acc);
-    __syncthreads();
+          for (int k = 0; k < BK / 16; ++k)
+            umma_f16<IDESC>(d, da + uint64_t(2 * k), db + uint64_t(2 * k), (kb | k) ? 1u : 0u);
+          umma_commit(&empty[s]);
+        }
+        if (!ok || !wait(&list_full[acc], (nt >> 1) & 1)) break;
+        const int slots = total[acc];
+        mbar_arrive(&list_empty[acc]);
+        for (int q0 = 0; q0 < slots; q0 += PER_STAGE, ++it) {
+          const int s = it % NST, n = min(PER_STAGE, slots - q0);
+          if (!wait(&full[s], (it / NST) & 1) || !wait(&tfull[s], (tph >> s) & 1)) { ok = false; break; }
+          tph ^= 1u << s;
+          tc_fence_after();
+          for (int q = 0; q < n; ++q)
+            for (int part = 0; part < PARTS; ++part)
+              umma_f16<IDESC>(d, smem_desc_sw32(sa + s * A_BYTES + (q * PARTS + part) * SLOT_A),
+                              smem_desc_sw32(sb + s * C::B_BYTES + q * C::SLOT_B), 1u);
+          umma_commit(&empty[s]);
+        }
+        if (ok) umma_commit(&acc_full[acc]);
+      }
+    }
+  } else if (warp < 6) {
+    // -------------------------------------- adapter lists and t pieces
+    const int r = threadIdx.x - 64;  // row of the tile
+    // (The stage of a t piece is signalled by the producer: a wait on `empty`
+    // from here could be more than one phase ahead of it.)
+    int it = 0, nt = 0;
+    uint32_t tph = 0;  // parity of each stage's next tgo phase
+    bool ok = true, arrived = false;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++nt) {
+      const int m = (tile / num_n) * BM + r, lb = nt & 1;
+      const int a = m < p.M ? adapter_of(p, m) : -1;
+      if (nt >= 2) ok = wait(&list_empty[lb], (nt / 2 - 1) & 1) && ok;
+      ids[r] = a;
+      // The first row of each adapter takes a place; ends are running sums.
+      const uint32_t same = __match_any_sync(0xffffffffu, a);
+      // All four warps leave together when a wait of any has run out.
+      uint32_t all_ok;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.and.pred q, 1, 128, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(all_ok)
+          : "r"(uint32_t(ok))
+          : "memory");
+      if (!all_ok) break;
+      bool first = a >= 0 && (same & ((1u << lane) - 1)) == 0;
+      for (int q = 0; first && q < (r & ~31); ++q) first = ids[q] != a;
+      const uint32_t mask = __ballot_sync(0xffffffffu, first);
+      int n = first ? slots_of(p, a) : 0;
+      int sum = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+      }
+      if (lane == 31) {
+        wsum[warp - 2] = sum;
+        wsum[4 + warp - 2] = __popc(mask);
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      int base = 0, place = __popc(mask & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (w < warp - 2) { base += wsum[w]; place += wsum[4 + w]; }
+        all += wsum[w];
+      }
+      if (first) {
+        list_id[lb * BM + place] = a;
+        list_end[lb * BM + place] = base + sum;
+      }
+      if (r == 0) total[lb] = all;
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      if (lane == 0) mbar_arrive(&list_full[lb]);
+      it += kblocks;
+      if (all > 0 && !arrived) {
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // shrink_kernel's t
+        arrived = true;
+      }
+      const __nv_bfloat16* trow = p.t + int64_t(m < p.M ? m : 0) * p.R;
+      int d = 0, start = 0;
+      for (int q0 = 0; ok && q0 < all; q0 += PER_STAGE, ++it) {
+        const int s = it % NST, cnt = min(PER_STAGE, all - q0);
+        ok = __all_sync(0xffffffffu, wait(&tgo[s], (tph >> s) & 1));
+        if (!ok) break;
+        tph ^= 1u << s;
+        for (int q = q0; q < q0 + cnt; ++q) {
+          while (q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
+          const bool mine = a >= 0 && list_id[lb * BM + d] == a;
+          for (int part = 0; part < PARTS; ++part) {
+            uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
+            if (mine) {
+              const uint4* src = reinterpret_cast<const uint4*>(trow + int64_t(part) * p.M * p.R + (q - start) * 16);
+              v0 = __ldcg(src);
+              v1 = __ldcg(src + 1);
+            }
+            uint8_t* dst = sa + s * A_BYTES + ((q - q0) * PARTS + part) * SLOT_A + r * 32;
+            const int sw = ((r >> 2) & 1) << 4;
+            *reinterpret_cast<uint4*>(dst + sw) = v0;
+            *reinterpret_cast<uint4*>(dst + (16 ^ sw)) = v1;
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&tfull[s]);
+      }
+    }
+  } else {
+    // ------------------------------------------------------------- epilogue
+    const int quarter = warp & 3, half = (warp - 6) >> 2;
+    // 32-column chunks of this warp: [c_lo, c_hi).
+    const int c_lo = BN >= 64 ? half * (BN / 2) : half * 32;
+    const int c_hi = BN >= 64 ? c_lo + BN / 2 : min(c_lo + 32, BN);
+    int nt = 0;
+    for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++nt) {
+      const int m0 = (tile / num_n) * BM, n0 = (tile % num_n) * BN, acc = nt & 1;
+      if (!__all_sync(0xffffffffu, mbar_wait_idle(&acc_full[acc], (nt / 2) & 1, abort_flag, status,
+                                                   ST_TIMEOUT, p.wait_ns)))
+        break;
+      tc_fence_after();
+      const int row = m0 + quarter * 32 + lane;
+      const uint32_t ta = tmem_base + uint32_t(acc * BN) + (uint32_t(quarter * 32) << 16);
+#pragma unroll 1
+      for (int c = c_lo; c < c_hi; c += 32) {
+        const int col0 = n0 + c;
+        if (col0 >= p.N) break;
+        float v[32];
+        tmem_ld32(ta + uint32_t(c), v);
+        if (row < p.M) {
+          if (p.bias) gemm::add_bias<32>(p, col0, v);
+          if (p.act || p.res) gemm::epi_post<32>(p, row, col0, v);
+          if (p.y_dtype == L3D_BF16) {
+            __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + int64_t(row) * p.y_ld + col0;
+            if (col0 + 32 <= p.N && p.y_vec) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float f[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) f[e] = v[q * 8 + e];
+                *reinterpret_cast<uint4*>(yr + q * 8) = pack(f, __nv_bfloat16());
+              }
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col0 + i < p.N) yr[i] = __float2bfloat16_rn(v[i]);
+            }
+          } else {
+            float* yr = static_cast<float*>(p.y) + int64_t(row) * p.y_ld + col0;
+            if (col0 + 32 <= p.N && p.y_vec) {
+#pragma unroll
+              for (int q = 0; q < 8; ++q)
+                *reinterpret_cast<float4*>(yr + q * 4) =
+                    make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 32; ++i)
+                if (col0 + i < p.N) yr[i] = v[i];
+            }
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&acc_empty[acc]);
+    }
   }
-  if (m >= p.M || n >= p.N) return;
-  const int a = adapter_of(p, m);
-  if (a >= 0) {
-    const __nv_bfloat16* br = p.b + (int64_t(a) * p.N + n) * p.R;
-    for (int r = 0; r < p.R; ++r) acc = fmaf(p.t[int64_t(m) * p.R + r], to_f(br[r]), acc);
+
+  // Teardown: after an abort, wait (bounded) for the MMAs this block issued,
+  // and give TMA loads still in flight 1 ms to land.
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && threadIdx.x == 32) {
+    umma_commit(drain);
+    mbar_drain(drain, 0, p.wait_ns);
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 1000000ull) {
+    }
   }
-  if (p.bias) acc += vec_at(p.bias, p.bias_dtype, n);
-  acc = act_dyn(p.act, acc);
-  if (p.res) acc = fmaf(p.gate ? vec_at(p.gate, p.gate_dtype, n) : 1.f, acc,
-                        (p.y_dtype == L3D_F32
-                            ? static_cast<const float*>(p.res)[int64_t(m) * p.res_ld + n]
-                            : to_f(static_cast<const __nv_bfloat16*>(p.res)[int64_t(m) * p.res_ld + n])));
-  if (p.y_dtype == L3D_F32) static_cast<float*>(p.y)[int64_t(m) * p.y_ld + n] = acc;
-  else static_cast<__nv_bfloat16*>(p.y)[int64_t(m) * p.y_ld + n] = __float2bfloat16_rn(acc);
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(C::TMEM));
+  }
+}
+
+// ------------------------------------------------------------------------ host
+// bf16 [rows, cols], row stride ld elements; box 64 columns x box_rows, 128B swizzle.
+static bool make_map2(CUtensorMap* m, const void* base, uint64_t rows, uint64_t cols, uint64_t ld,
+                      uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {cols, rows};
+  const cuuint64_t strides[1] = {ld * 2};
+  const cuuint32_t box[2] = {uint32_t(BK), box_rows};
+  const cuuint32_t es[2] = {1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+// lora_b [A, n, R]: box 16 ranks x box_rows x 1, 32B swizzle (rows past n read as zero).
+static bool make_map_b(CUtensorMap* m, const void* base, uint64_t A, uint64_t n, uint64_t R,
+                       uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[3] = {R, n, A};
+  const cuuint64_t strides[2] = {R * 2, n * R * 2};
+  const cuuint32_t box[3] = {16u, box_rows, 1u};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_32B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int BN>
+static cudaError_t launch_gemm(const CUtensorMap& mx, const void* w, int64_t w_ld, const void* b,
+                               const Params& p, cudaStream_t s) {
+  auto k = lora_gemm_kernel<BN>;
+  cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<BN>::SMEM);
+  if (e != cudaSuccess) return e;
+  CUtensorMap mw, mb;
+  if (!make_map2(&mw, w, uint64_t(p.N), uint64_t(p.K), uint64_t(w_ld), BN) ||
+      !make_map_b(&mb, b, uint64_t(p.A), uint64_t(p.N), uint64_t(p.R), BN))
+    return cudaErrorInvalidValue;
+  const int64_t tiles = int64_t((p.M + BM - 1) / BM) * ((p.N + BN - 1) / BN);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(tiles < sm_count() ? tiles : sm_count()));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = Cfg<BN>::SMEM;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, mx, mw, mb, p);
+}
+
+// The tile width with the least estimated time: rounds of the device x the K
+// steps of a tile, each as long as its products (2 BN clocks) or its loads.
+static int pick_bn(int64_t M, int64_t N) {
+  int best = 256;
+  double least = 1e300;
+  for (int bn = 256; bn >= 32; bn /= 2) {
+    const int64_t tiles = ((M + BM - 1) / BM) * ((N + bn - 1) / bn);
+    const double rounds = double((tiles + sm_count() - 1) / sm_count());
+    const double step = 2.0 * bn > 200 + 1.0 * bn ? 2.0 * bn : 200 + 1.0 * bn;
+    if (rounds * step < least * 0.999) {
+      least = rounds * step;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+cudaError_t status_read(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_lora_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_lora_status, &zero, sizeof(int));
+  }
+  return e;
 }
 
 }  // namespace lora
@@ -94,7 +618,7 @@ using namespace l3d;
 
 extern "C" size_t l3d_lora_linear_workspace_size(int64_t m, int64_t r) {
   if (m < 0 || r < 0) return 0;
-  return size_t(m) * size_t(r) * 4 + 256;
+  return size_t(m) * size_t(r) * 4 + 256;  // A x in bf16, and its rounding error
 }
 
 extern "C" int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight,
@@ -206,26 +730,53 @@ extern "C" int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight,
   Params p{};
   p.M = int(M); p.N = int(n); p.K = int(k); p.R = int(R); p.A = int(A);
   p.x = reinterpret_cast<const __nv_bfloat16*>(elem_ptr(x));
-  p.w = reinterpret_cast<const __nv_bfloat16*>(elem_ptr(weight));
   p.a = reinterpret_cast<const __nv_bfloat16*>(elem_ptr(lora_a));
-  p.b = reinterpret_cast<const __nv_bfloat16*>(elem_ptr(lora_b));
-  p.x_ld = x_ld; p.w_ld = w_ld; p.y_ld = y_ld; p.res_ld = res_ld;
+  p.x_ld = x_ld; p.y_ld = y_ld; p.res_ld = res_ld;
   p.scale = reinterpret_cast<const float*>(elem_ptr(lora_scale));
   p.ranks = ranks ? reinterpret_cast<const int32_t*>(elem_ptr(ranks)) : nullptr;
   p.ids = elem_ptr(ids);
   p.ids64 = ids->dtype == L3D_I64;
   p.per = int(M / ids->dims[0]);
+  auto aligned = [](const void* q, int64_t ld_bytes) {
+    return reinterpret_cast<uintptr_t>(q) % 16 == 0 && ld_bytes % 16 == 0;
+  };
+  const int es = dtype_size(y->dtype);
   p.bias = bias ? elem_ptr(bias) : nullptr;
   p.bias_dtype = bias ? bias->dtype : L3D_F32;
+  p.bias_vec = aligned(p.bias, 0);
   p.gate = gate ? elem_ptr(gate) : nullptr;
   p.gate_dtype = gate ? gate->dtype : L3D_F32;
   p.res = residual ? elem_ptr(residual) : nullptr;
+  p.res_vec = aligned(p.res, res_ld * es);
   p.y = const_cast<char*>(elem_ptr(y));
   p.y_dtype = y->dtype;
+  p.y_vec = aligned(p.y, y_ld * es);
   p.act = act;
-  p.t = static_cast<float*>(workspace);
+  p.t = static_cast<__nv_bfloat16*>(workspace);
+  p.wait_ns = l3d::tc::WAIT_LIMIT_NS;
+  CUtensorMap mx;
+  if (!make_map2(&mx, p.x, uint64_t(M), uint64_t(k), uint64_t(x_ld), BM))
+    return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed for x", op);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  shrink_kernel<<<unsigned(M), 256, 0, s>>>(p);
-  expand_kernel<<<dim3(unsigned((n + 15) / 16), unsigned((M + 15) / 16)), 256, 0, s>>>(p);
-  return check_launch(op);
+  // Few rows: 16 per block, all warps along K, the group's adapters in
+  // parallel blocks.  Many: 64 per block, so that A is read less often.
+  if (M <= int64_t(sm_count()) * 64) {
+    const int64_t y_blocks = A < M ? (A < 16 ? A : 16) : (M < 16 ? M : 16);
+    const int64_t groups = (M + 15) / 16;
+    shrink_kernel<1, 1, 1, 8><<<dim3(unsigned(groups), unsigned(groups > sm_count() ? 1 : y_blocks)), 256, 0, s>>>(p);
+  } else {
+    shrink_kernel<2, 2, 2, 2><<<dim3(unsigned((M + 63) / 64), 1), 256, 0, s>>>(p);
+  }
+  if (cudaGetLastError() != cudaSuccess) return fail(L3D_E_CUDA, "%s: launch failed", op);
+  const void* w = elem_ptr(weight);
+  const void* b = elem_ptr(lora_b);
+  cudaError_t e;
+  switch (pick_bn(M, n)) {
+    case 32: e = launch_gemm<32>(mx, w, w_ld, b, p, s); break;
+    case 64: e = launch_gemm<64>(mx, w, w_ld, b, p, s); break;
+    case 128: e = launch_gemm<128>(mx, w, w_ld, b, p, s); break;
+    default: e = launch_gemm<256>(mx, w, w_ld, b, p, s); break;
+  }
+  if (e != cudaSuccess) return fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  return L3D_OK;
 }

@@ -323,6 +323,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   } else if ((warp - 1 - C::NMMA) >> 2 < ntv) {
     // ------------------------------------------------------ softmax / epilogue
     const int t = (warp - 1 - C::NMMA) >> 2;
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // the warp's lanes stay together
+      return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    };
     const int quarter = warp & 3;
     const int r = quarter * 32 + lane;
     const int f = f0 + t * BQ + r;
@@ -355,7 +358,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     float2 l2 = f2(0.f);                         // running row sum (two halves)
     bool ok = true;
     for (int j = 0; j < nkv; ++j) {
-      if (!wait(&s_full[t], j & 1)) { ok = false; break; }
+      if (!wait_all(&s_full[t], j & 1)) { ok = false; break; }
       tc_fence_after();
       const bool pre = j < np;
       const int64_t key0 = int64_t(pre ? pa + j : sa + j - np) * BKV;
@@ -373,7 +376,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
       bool pv_waited = !C::SEP_P || j == 0;
       auto wait_pv = [&]() {  // P_t(j-1) V has read P_t and O_t is stable
         if (pv_waited) return true;
-        pv_waited = wait(&pv_done[t], (j - 1) & 1);
+        pv_waited = wait_all(&pv_done[t], (j - 1) & 1);
         tc_fence_after();
         return pv_waited;
       };
@@ -452,7 +455,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     }
     // Epilogue, after the last P V: the output, or this part's O / l and log2 sum.
     if (ok && nkv > 0)
-      ok = mbar_wait_idle(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0, abort_flag, status, ST_TIMEOUT, p.wait_ns);
+      ok = wait_all(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0);
     if (ok && active) {
       tc_fence_after();
       // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)

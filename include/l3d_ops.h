@@ -441,8 +441,8 @@ size_t l3d_lora_linear_workspace_size(int64_t m, int64_t r);
  * kernels skip the zero ranks.  The adapters must be finite: a row of another
  * request meets them multiplied by zero.  bias, act, residual, gate as for
  * l3d_linear_ex; y BF16 or F32; y must not overlap x (it may be residual).
- * A_a x is accumulated in f32 and enters the second product as bf16 (as a
- * sum of two bf16 parts when y is F32). */
+ * A_a x is accumulated in f32 and enters the second product as the sum of two
+ * bf16 parts. */
 int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight, const l3d_tensor* bias,
                     const l3d_tensor* lora_a, const l3d_tensor* lora_b,
                     const l3d_tensor* lora_scale, const l3d_tensor* ranks, const l3d_tensor* ids,
