@@ -161,7 +161,8 @@ extern "C" const char* l3d_last_error(void) { return l3d::g_last_error.c_str(); 
 extern "C" int l3d_kernel_status(int* status, int reset) {
   using namespace l3d;
   if (!status) return fail(L3D_E_NULL, "l3d_kernel_status: status is required");
-  cudaError_t (*const words[])(int*, int) = {norm_status_read, pattn::status_read, lora::status_read};
+  cudaError_t (*const words[])(int*, int) = {norm_status_read, sandwich::status_read,
+                                               pattn::status_read, lora::status_read};
   *status = 0;
   for (auto read : words) {
     int one = 0;

@@ -7,6 +7,7 @@
 // (crate/runtime/trellis2_blocks.rs:280-286,627-645, crate/runtime/vggt.rs:104-123);
 // here x and h are read once and r and y written once.
 #include "common.cuh"
+#include "ring.cuh"
 
 namespace l3d {
 namespace sandwich {
@@ -21,6 +22,7 @@ struct Params {
   ChanVec pw, pb, gate;        // after the block
   ChanVec w, b, scale, shift;  // before the next one
   float res_scale, post_eps, eps;
+  int norm;
 };
 
 constexpr int kBlock = 256;
@@ -46,11 +48,10 @@ __device__ __forceinline__ float chan_or(const ChanVec& v, int64_t b, int64_t c,
 }
 
 // Mean (0 for RMS) and 1 / sqrt(.. + eps) of the C values at s, by the whole block.
-template <int NORM>
-__device__ __forceinline__ void block_stats(const float* s, int64_t C, float eps, float* red,
+__device__ __forceinline__ void block_stats(int norm, const float* s, int64_t C, float eps, float* red,
                                             float& mean, float& inv) {
   mean = 0.f;
-  if constexpr (NORM == NORM_LAYER) {
+  if (norm == NORM_LAYER) {
     float a = 0.f;
     for (int64_t c = threadIdx.x; c < C; c += kBlock) a += s[c];
     mean = block_sum(a, red) / float(C);
@@ -65,7 +66,7 @@ __device__ __forceinline__ void block_stats(const float* s, int64_t C, float eps
 
 // One row per block at a time, the row held in shared memory as f32; any
 // row length, alignment and strides.
-template <typename T, int NORM>
+template <typename T>
 __global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
   extern __shared__ float s[];
   __shared__ float red[kBlock / 32];
@@ -76,7 +77,7 @@ __global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
     for (int64_t c = threadIdx.x; c < p.C; c += kBlock) s[c] = to_f(hr[c]);
     __syncthreads();
     float mean, inv;
-    block_stats<NORM>(s, p.C, p.post_eps, red, mean, inv);
+    block_stats(p.norm, s, p.C, p.post_eps, red, mean, inv);
     T* rr = static_cast<T*>(p.r) + row_offset(p.rm, row);
     for (int64_t c = threadIdx.x; c < p.C; c += kBlock) {
       const float n = (s[c] - mean) * inv * chan_or(p.pw, 0, c, 1.f) + chan_or(p.pb, 0, c, 0.f);
@@ -86,13 +87,397 @@ __global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
     }
     __syncthreads();
     if (p.y) {
-      block_stats<NORM>(s, p.C, p.eps, red, mean, inv);
+      block_stats(p.norm, s, p.C, p.eps, red, mean, inv);
       T* yr = static_cast<T*>(p.y) + row_offset(p.ym, row);
       for (int64_t c = threadIdx.x; c < p.C; c += kBlock) {
         const float n = (s[c] - mean) * inv * chan_or(p.w, 0, c, 1.f) + chan_or(p.b, 0, c, 0.f);
         yr[c] = from_f<T>(fmaf(n, 1.f + chan_or(p.scale, b, c, 0.f), chan_or(p.shift, b, c, 0.f)));
       }
       __syncthreads();
+    }
+  }
+}
+
+// The per-channel vectors are folded into f32 coefficients in shared memory,
+//   r = res_scale x + A1 (h - mean) inv + B1,  A1 = gate post_weight, B1 = gate post_bias
+//   y = A2 (r - mean) inv + B2,  A2 = weight (1 + scale), B2 = bias (1 + scale) + shift
+// B1 and B2 only where one of their vectors is given.
+struct Coefs {
+  int has_b1, has_b2;
+  int ld;                  // floats of a coefficient row (a multiple of 4)
+  int chan_vec;            // the vectors are 16-byte aligned
+};
+
+// Place of channel c in a coefficient row read in vectors of VEC: in planes of
+// four floats, so that consecutive vectors lie 16 bytes apart and their loads
+// meet no bank twice.
+template <int VEC>
+__device__ __forceinline__ int coef_at(int c, int ld) {
+  if constexpr (VEC == 8) return ((c >> 2) & 1) * (ld / 2) + (c >> 3) * 4 + (c & 3);
+  else return c;
+}
+
+// One channel, or VEC consecutive ones, of batch element b folded into `coef`.
+template <int VEC>
+__device__ __forceinline__ void fold(const Params& p, const Coefs& k, float* coef, int64_t b) {
+  const int C = int(p.C);
+  float* row = coef;
+  float *a1 = row, *a2 = row + k.ld, *b1 = row + 2 * k.ld, *b2 = row + (2 + k.has_b1) * k.ld;
+  if (VEC > 1 && k.chan_vec) {
+    for (int c = int(threadIdx.x) * VEC; c < C; c += int(blockDim.x) * VEC) {
+      float g[VEC], w[VEC], t[VEC];
+      auto get = [&](const ChanVec& v, int64_t bb, float none, float (&o)[VEC]) {
+        if (v.ptr) {
+          load_chan<VEC>(v, bb, c, o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) o[e] = none;
+        }
+      };
+      auto put = [&](float* dst, const float (&o)[VEC]) {
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4)
+          *reinterpret_cast<float4*>(dst + coef_at<VEC>(c + e, k.ld)) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+      };
+      get(p.gate, b, 1.f, g);
+      get(p.pw, 0, 1.f, w);
+      get(p.scale, b, 0.f, t);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) { w[e] *= g[e]; t[e] += 1.f; }
+      put(a1, w);
+      if (k.has_b1) {
+        get(p.pb, 0, 0.f, w);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] *= g[e];
+        put(b1, w);
+      }
+      get(p.w, 0, 1.f, w);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] *= t[e];
+      put(a2, w);
+      if (k.has_b2) {
+        get(p.b, 0, 0.f, w);
+        get(p.shift, b, 0.f, g);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) w[e] = fmaf(w[e], t[e], g[e]);
+        put(b2, w);
+      }
+    }
+  } else {
+    for (int c = threadIdx.x; c < C; c += blockDim.x) {
+      const int at = coef_at<VEC>(c, k.ld);
+      const float g = chan_or(p.gate, b, c, 1.f), t = 1.f + chan_or(p.scale, b, c, 0.f);
+      a1[at] = g * chan_or(p.pw, 0, c, 1.f);
+      if (k.has_b1) b1[at] = g * chan_or(p.pb, 0, c, 0.f);
+      a2[at] = t * chan_or(p.w, 0, c, 1.f);
+      if (k.has_b2) b2[at] = fmaf(t, chan_or(p.b, 0, c, 0.f), chan_or(p.shift, b, c, 0.f));
+    }
+  }
+}
+
+// row_offset for fewer than 2^32 rows: a 64-bit division is a call, around which
+// a row held in registers would be spilled.
+__device__ __forceinline__ int64_t row_offset32(const RowMap& m, uint32_t r) {
+  int64_t off = m.base;
+#pragma unroll
+  for (int i = 4; i >= 1; --i) {
+    if (i < m.nd) {
+      const uint32_t d = uint32_t(m.dims[i]), q = r / d;
+      off += int64_t(r - q * d) * m.strides[i];
+      r = q;
+    }
+  }
+  return off + int64_t(r) * m.strides[0];
+}
+
+// Sum over the G threads of a row, the same value in each of them.  `red`: two
+// buffers in turn, since a warp can be one sum ahead of another, not two.
+template <int G>
+__device__ __forceinline__ float group_sum(float v, float* red, int& turn) {
+#pragma unroll
+  for (int o = (G < 32 ? G : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  if constexpr (G > 32) {
+    constexpr int W = G / 32;
+    const int grp = threadIdx.x / G;
+    float* r = red + turn * 16 + grp * W;
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) r[(threadIdx.x % G) >> 5] = v;
+    asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(G) : "memory");
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < W; ++i) v += r[i];
+  }
+  return v;
+}
+// Whether `ok` holds in all threads of the unit.
+template <int G>
+__device__ __forceinline__ bool unit_all(bool ok) {
+  if constexpr (G <= 32) {
+    return __all_sync(0xffffffffu, ok);
+  } else {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+        "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"(uint32_t(ok)), "r"(1 + int(threadIdx.x / G)), "n"(G)
+        : "memory");
+    return r != 0;
+  }
+}
+
+// The ring kernel (16-byte aligned rows): one block per SM (fewer for few rows),
+// a contiguous range of rows each, worked through by units of max(G, 32)
+// threads.  G threads hold a row's h in registers as f32 (64 elements a thread,
+// 32 of f32 rows), and r in its place; G = 8 puts four rows in a warp.  Each
+// unit keeps kSlots packs of rows (x and h) in shared memory that bulk copies
+// fill ahead of it, so that the loads in flight do not occupy registers; its
+// first thread issues the next copy once the unit has read a slot.
+// Both norms' sums are taken in two passes over the registers (mean, then
+// centred squares: one pass of shifted moments loses digits where one channel
+// lies far out).
+constexpr int kThreads = 384;
+constexpr int kSlots = 2;
+
+struct Ring {
+  int64_t rows_per_batch;  // rows that share per-batch vectors (all, without such vectors)
+  int units;               // per block
+  uint32_t row_bytes;
+  uint64_t wait_ns;
+};
+
+__device__ int g_sandwich_status;
+
+template <typename T, int G, int NORM>
+__global__ void __launch_bounds__(kThreads, 1)
+    ring_kernel(const Params p, const Coefs kc, const Ring sp) {
+  constexpr int VEC = Vec16<T>::N, NV = 8, P = VEC / 2;  // vectors of a thread, pairs of a vector
+  constexpr int U = G < 32 ? 32 : G, RPU = U / G;        // threads and rows of a unit
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ float red[32];
+  float* coef = reinterpret_cast<float*>(smem);
+  uint8_t* slots = smem + size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
+  const uint32_t slot_bytes = 2 * RPU * sp.row_bytes;    // the pack's h rows, then its x rows
+  uint64_t* full = reinterpret_cast<uint64_t*>(slots + size_t(sp.units) * kSlots * slot_bytes);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + sp.units * kSlots);
+  const int unit = threadIdx.x / U, tu = threadIdx.x % U;
+  const int t = threadIdx.x % G, sub = tu / G;           // thread of the row, row of the pack
+  const int nvec = int(p.C) / VEC;
+  const int64_t lo = p.rows * blockIdx.x / gridDim.x, hi = p.rows * (blockIdx.x + 1) / gridDim.x;
+  const int64_t packs = (hi - lo + RPU - 1) / RPU;       // pack k: rows lo + k RPU ..
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < sp.units * kSlots; ++i) ring_bar_init(&full[i], 2 * RPU);
+    *abort_flag = 0;
+    ring_init_fence();
+  }
+  __syncthreads();
+  const bool works = unit < sp.units;                    // the other threads only fold
+  uint8_t* my_slots = slots + size_t(works ? unit : 0) * kSlots * slot_bytes;
+  uint64_t* my_full = full + (works ? unit : 0) * kSlots;
+  // The unit's n-th pack (pack n units + unit) into slot n % kSlots.
+  auto issue = [&](int64_t n) {
+    const int64_t k = n * sp.units + unit;
+    if (k >= packs) return;
+    uint8_t* slot = my_slots + (n % kSlots) * slot_bytes;
+    uint64_t* bar = &my_full[n % kSlots];
+    for (int i = 0; i < RPU; ++i) {
+      const int64_t row = lo + k * RPU + i;
+      if (row < hi) {
+        ring_load(slot + i * sp.row_bytes, static_cast<const T*>(p.h) + row_offset32(p.hm, uint32_t(row)),
+                  sp.row_bytes, bar);
+        ring_load(slot + (RPU + i) * sp.row_bytes,
+                  static_cast<const T*>(p.x) + row_offset32(p.xm, uint32_t(row)), sp.row_bytes, bar);
+      } else {
+        ring_arrive(bar);
+        ring_arrive(bar);
+      }
+    }
+  };
+  if (works && tu == 0)
+    for (int n = 0; n < kSlots; ++n) issue(n);
+  const float inv_c = 1.f / float(p.C);
+  const float2 rs = f2(p.res_scale);
+  int turn = 0;
+  bool dead = false;
+  int64_t n = 0;  // the unit's next pack
+  for (int64_t s0 = lo; s0 < hi;) {
+    // Rows [s0, s1): one batch element's.
+    const int64_t b = s0 / sp.rows_per_batch;
+    const int64_t s1 = min((b + 1) * sp.rows_per_batch, hi);
+    if (s0 != lo) __syncthreads();
+    fold<VEC>(p, kc, coef, b);
+    __syncthreads();
+    // Vector i of this thread of coefficient row k.
+    auto coefs = [&](int k, int i, float2 (&o)[P]) {
+      const float* c = coef + k * kc.ld + (t + i * G) * 4;
+#pragma unroll
+      for (int e = 0; e < P; e += 2) {
+        const float4 v = *reinterpret_cast<const float4*>(c + (e / 2) * (kc.ld / 2));
+        o[e] = make_float2(v.x, v.y);
+        o[e + 1] = make_float2(v.z, v.w);
+      }
+    };
+    for (; works && !dead; ++n) {
+      const int64_t row0 = lo + (n * sp.units + unit) * RPU;  // first row of the pack
+      if (row0 >= s1) break;
+      const int slot = int(n % kSlots);
+      if (!unit_all<G>(ring_wait(&my_full[slot], uint32_t(n / kSlots) & 1u, abort_flag, sp.wait_ns, false,
+                                 &g_sandwich_status))) {
+        dead = true;
+        break;
+      }
+      const int64_t row = row0 + sub;
+      const bool valid = row >= s0 && row < s1;
+      const uint32_t at = uint32_t(valid ? row : s0);
+      const uint4* hs = reinterpret_cast<const uint4*>(my_slots + slot * slot_bytes + sub * sp.row_bytes) + t;
+      const uint4* xs = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(hs) + RPU * sp.row_bytes);
+      float2 f[NV][P];
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int e = 0; e < P; ++e) f[i][e] = f2(0.f);
+        if (t + i * G < nvec) unpack2(hs[i * G], f[i], T());
+      }
+      // Mean and 1 / sqrt(mean square + eps) of the row in f (zero past its end).
+      float2 nm = f2(0.f);
+      auto stats = [&](float eps) {
+        if constexpr (NORM == NORM_LAYER) {
+          float2 s = f[0][0];
+#pragma unroll
+          for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < P; ++e)
+              if (i + e > 0) s = add2(s, f[i][e]);
+          nm = f2(-group_sum<G>(s.x + s.y, red, turn) * inv_c);
+        }
+        float2 q = f2(0.f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (NORM == NORM_LAYER && t + i * G >= nvec) continue;
+#pragma unroll
+          for (int e = 0; e < P; ++e) {
+            const float2 d = NORM == NORM_LAYER ? add2(f[i][e], nm) : f[i][e];
+            q = fma2(d, d, q);
+          }
+        }
+        return f2(1.f / sqrtf(fmaf(group_sum<G>(q.x + q.y, red, turn), inv_c, eps)));
+      };
+      float2 iv = stats(p.post_eps);
+      {
+        uint4* rd = reinterpret_cast<uint4*>(static_cast<T*>(p.r) + row_offset32(p.rm, at)) + t;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (t + i * G >= nvec) continue;
+          float2 a[P], c[P], x[P];
+          coefs(0, i, a);
+          if (kc.has_b1) coefs(2, i, c);
+          unpack2(xs[i * G], x, T());
+#pragma unroll
+          for (int e = 0; e < P; ++e) {
+            const float2 d = mul2(NORM == NORM_LAYER ? add2(f[i][e], nm) : f[i][e], iv);
+            const float2 base = kc.has_b1 ? fma2(rs, x[e], c[e]) : mul2(rs, x[e]);
+            f[i][e] = fma2(a[e], d, base);
+          }
+          if (valid) st_act_raw(rd + i * G, pack2(f[i], T()));
+        }
+      }
+      // The slot has been read; a pack that reaches into the next batch
+      // element is taken up again there.
+      const bool whole = RPU == 1 || row0 + RPU <= s1 || s1 == hi;
+      if (whole) {
+        if constexpr (G <= 32) __syncwarp();
+        else unit_all<G>(true);
+        if (tu == 0) issue(n + kSlots);
+      }
+      if (p.y) {
+        iv = stats(p.eps);
+        uint4* yd = reinterpret_cast<uint4*>(static_cast<T*>(p.y) + row_offset32(p.ym, at)) + t;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+          if (t + i * G >= nvec) continue;
+          float2 a[P], c[P];
+          coefs(1, i, a);
+          if (kc.has_b2) coefs(2 + kc.has_b1, i, c);
+#pragma unroll
+          for (int e = 0; e < P; ++e) {
+            const float2 d = mul2(NORM == NORM_LAYER ? add2(f[i][e], nm) : f[i][e], iv);
+            f[i][e] = kc.has_b2 ? fma2(a[e], d, c[e]) : mul2(a[e], d);
+          }
+          if (valid) st_act_raw(yd + i * G, pack2(f[i], T()));
+        }
+      }
+      if (!whole) break;
+    }
+    s0 = s1;
+  }
+  // After an abort no copy may still be in flight when the block exits.
+  if (dead && tu == 0)
+    for (int64_t k = n; k < n + kSlots; ++k)
+      if (k * sp.units + unit < packs)
+        ring_wait(&my_full[k % kSlots], uint32_t(k / kSlots) & 1u, abort_flag, sp.wait_ns, true, &g_sandwich_status);
+}
+
+// The element kernel (any alignment): G threads per row, 32 elements a thread,
+// blocks that keep to one batch element.
+struct Blocks {
+  int64_t rows, rows_per_block;  // of a batch element
+  int per_batch;
+};
+template <typename T, int G, int NORM>
+__global__ void __launch_bounds__(kBlock, 2)
+    elem_kernel(const Params p, const Coefs kc, const Blocks sp) {
+  constexpr int NE = 32, RPB = kBlock / G;
+  extern __shared__ __align__(16) float coef[];
+  __shared__ float red[32];
+  const int t = threadIdx.x % G, C = int(p.C);
+  const int64_t b = blockIdx.x / sp.per_batch;
+  const int64_t first = int64_t(blockIdx.x % sp.per_batch) * sp.rows_per_block;
+  const int64_t last = min(first + sp.rows_per_block, sp.rows);
+  fold<1>(p, kc, coef, b);
+  __syncthreads();
+  const float *a1 = coef, *a2 = coef + kc.ld, *b1 = coef + 2 * kc.ld, *b2 = coef + (2 + kc.has_b1) * kc.ld;
+  const float inv_c = 1.f / float(C);
+  int turn = 0;
+  for (int64_t row = first + threadIdx.x / G; row < last; row += RPB) {
+    const uint32_t at = uint32_t(b * sp.rows + row);
+    const T* hs = static_cast<const T*>(p.h) + row_offset32(p.hm, at);
+    const T* xs = static_cast<const T*>(p.x) + row_offset32(p.xm, at);
+    T* rd = static_cast<T*>(p.r) + row_offset32(p.rm, at);
+    T* yd = p.y ? static_cast<T*>(p.y) + row_offset32(p.ym, at) : nullptr;
+    float f[NE];
+#pragma unroll
+    for (int i = 0; i < NE; ++i) f[i] = t + i * G < C ? to_f(hs[t + i * G]) : 0.f;
+    float nm = 0.f;
+    auto stats = [&](float eps) {
+      if constexpr (NORM == NORM_LAYER) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NE; ++i) s += f[i];
+        nm = -group_sum<G>(s, red, turn) * inv_c;
+      }
+      float q = 0.f;
+#pragma unroll
+      for (int i = 0; i < NE; ++i) {
+        const float d = NORM == NORM_LAYER ? (t + i * G < C ? f[i] + nm : 0.f) : f[i];
+        q = fmaf(d, d, q);
+      }
+      return 1.f / sqrtf(fmaf(group_sum<G>(q, red, turn), inv_c, eps));
+    };
+    float iv = stats(p.post_eps);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int c = t + i * G;
+      if (c >= C) continue;
+      const float base = fmaf(p.res_scale, to_f(xs[c]), kc.has_b1 ? b1[c] : 0.f);
+      f[i] = fmaf(a1[c], (f[i] + nm) * iv, base);
+      rd[c] = from_f<T>(f[i]);
+    }
+    if (!p.y) continue;
+    iv = stats(p.eps);
+#pragma unroll
+    for (int i = 0; i < NE; ++i) {
+      const int c = t + i * G;
+      if (c < C) yd[c] = from_f<T>(fmaf(a2[c], (f[i] + nm) * iv, kc.has_b2 ? b2[c] : 0.f));
     }
   }
 }
@@ -112,14 +497,93 @@ static int check_like(const l3d_tensor* t, const l3d_tensor* x, const char* op, 
   return L3D_OK;
 }
 
+constexpr int kSmem = 227 * 1024 - 1024;
+constexpr const char* kNoSmem = "l3d_sandwich_residual_norm: cannot reserve shared memory";
+
+// Returns 1 when launched, 0 when the row does not fit this kernel, or fails.
+template <typename T, int G, int NORM>
+static int launch_ring(const Params& p, const Coefs& kc, Ring sp, size_t coef, cudaStream_t s) {
+  constexpr int U = G < 32 ? 32 : G, RPU = U / G;
+  const size_t slot = size_t(kSlots) * (2 * RPU * sp.row_bytes + 8);
+  if (coef + slot + 16 > size_t(kSmem)) return 0;
+  auto k = ring_kernel<T, G, NORM>;
+  if (set_smem_limit(reinterpret_cast<const void*>(k), kSmem) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
+  const int64_t packs = (p.rows + RPU - 1) / RPU;
+  const int64_t blocks = packs < sm_count() ? packs : sm_count();
+  const int64_t per_block = ((p.rows + blocks - 1) / blocks + RPU - 1) / RPU;
+  int64_t units = kThreads / U;
+  if (units > per_block) units = per_block;
+  const int64_t room = int64_t((size_t(kSmem) - coef - 16) / slot);
+  sp.units = int(units < room ? units : room);
+  k<<<unsigned(blocks), kThreads, coef + size_t(sp.units) * slot + 16, s>>>(p, kc, sp);
+  return 1;
+}
+
+template <typename T, int G, int NORM>
+static int launch_elem(const Params& p, const Coefs& kc, int64_t batches, size_t coef, cudaStream_t s) {
+  constexpr int RPB = kBlock / G;
+  if (coef > 100 * 1024) return 0;
+  auto k = elem_kernel<T, G, NORM>;
+  if (set_smem_limit(reinterpret_cast<const void*>(k), 100 * 1024) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
+  Blocks sp{};
+  sp.rows = p.rows / batches;
+  // Two waves of blocks, shared out between the batch elements.
+  const int64_t most = (sp.rows + RPB - 1) / RPB;
+  int64_t per = int64_t(sm_count()) * 4 / batches;
+  per = per < 1 ? 1 : per > most ? most : per;
+  sp.rows_per_block = ((sp.rows + per - 1) / per + RPB - 1) / RPB * RPB;
+  sp.per_batch = int((sp.rows + sp.rows_per_block - 1) / sp.rows_per_block);
+  k<<<unsigned(sp.per_batch) * unsigned(batches), kBlock, coef, s>>>(p, kc, sp);
+  return 1;
+}
+
 template <typename T, int NORM>
-static int launch(const Params& p, cudaStream_t s) {
-  auto k = row_kernel<T, NORM>;
+static int try_fast(const Params& p, bool vec_ok, bool chan_vec, int64_t batches, cudaStream_t s) {
+  if (p.rows >= (int64_t(1) << 31)) return 0;
+  Coefs kc{};
+  kc.has_b1 = p.pb.ptr != nullptr;
+  kc.has_b2 = p.b.ptr || p.shift.ptr;
+  kc.ld = int((p.C + 7) & ~int64_t(7));
+  kc.chan_vec = chan_vec;
+  const size_t coef = size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
+  if (vec_ok) {
+    Ring sp{};
+    sp.rows_per_batch = p.rows / batches;
+    sp.row_bytes = uint32_t(p.C * sizeof(T));
+    sp.wait_ns = 2000000000ull;
+    constexpr int E = 8 * Vec16<T>::N;  // elements of a thread
+    const int rc = p.C <= 8 * E ? launch_ring<T, 8, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 32 * E ? launch_ring<T, 32, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 64 * E ? launch_ring<T, 64, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 128 * E ? launch_ring<T, 128, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 256 * E ? launch_ring<T, 256, NORM>(p, kc, sp, coef, s) : 0;
+    if (rc) return rc;
+  }
+  return p.C <= 32 * 32 ? launch_elem<T, 32, NORM>(p, kc, batches, coef, s)
+         : p.C <= 256 * 32 ? launch_elem<T, 256, NORM>(p, kc, batches, coef, s) : 0;
+}
+
+template <typename T>
+static int launch(const Params& p, bool vec_ok, bool chan_vec, int64_t batches, cudaStream_t s) {
+  const int rc = p.norm == NORM_LAYER ? try_fast<T, NORM_LAYER>(p, vec_ok, chan_vec, batches, s)
+                                      : try_fast<T, NORM_RMS>(p, vec_ok, chan_vec, batches, s);
+  if (rc) return rc < 0 ? -rc : L3D_OK;
+  // Rows too long for either (or 2^31 of them): a block per row.
+  auto k = row_kernel<T>;
   if (set_smem_limit(reinterpret_cast<const void*>(k), int(kMaxC * 4)) != cudaSuccess)
     return fail(L3D_E_CUDA, "l3d_sandwich_residual_norm: cannot reserve shared memory");
   const int64_t cap = int64_t(sm_count()) * 8;
   k<<<unsigned(p.rows < cap ? p.rows : cap), kBlock, size_t(p.C) * 4, s>>>(p);
   return L3D_OK;
+}
+
+cudaError_t status_read(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_sandwich_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_sandwich_status, &zero, sizeof(int));
+  }
+  return e;
 }
 
 }  // namespace sandwich
@@ -182,9 +646,19 @@ extern "C" int l3d_sandwich_residual_norm(const l3d_tensor* x, const l3d_tensor*
   p.res_scale = res_scale;
   p.post_eps = post_eps;
   p.eps = eps;
+  p.norm = norm;
+  // 16-byte vectors where every row of every activation is so aligned.
+  const int vec = 16 / dtype_size(x->dtype);
+  auto rows_ok = [&](const l3d_tensor* t, const RowMap& m) {
+    return !t || (reinterpret_cast<uintptr_t>(t->data) % 16 == 0 && rowmap_aligned(m, vec));
+  };
+  const bool vec_ok = p.C % vec == 0 && rows_ok(x, p.xm) && rows_ok(h, p.hm) && rows_ok(r_out, p.rm) &&
+                      rows_ok(y, p.ym);
+  const bool per_batch = p.gate.bstride || p.shift.bstride || p.scale.bstride;
+  const int64_t batches = per_batch ? B : 1;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   L3D_DISPATCH_FLOAT(x->dtype, T, {
-    rc = norm == NORM_LAYER ? launch<T, NORM_LAYER>(p, s) : launch<T, NORM_RMS>(p, s);
+    rc = launch<T>(p, vec_ok, al, batches, s);
   });
   return rc ? rc : check_launch(op);
 }
