@@ -10,6 +10,7 @@ The library is required: importing this module on a machine without the built
 from __future__ import annotations
 
 import ctypes as C
+import struct
 from pathlib import Path
 
 import torch
@@ -69,7 +70,26 @@ def ref(d):
     return None if d is None else C.byref(d)
 
 
+_PACK = struct.Struct("=Qii6q6qq").pack
+_PAD = [(0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1)]
+
+
+def packed(t: torch.Tensor | None):
+    """As desc, as the descriptor's bytes (None -> NULL), for the entries whose
+    signature takes _D: a third of the time of filling a ctypes structure, which
+    is what a call on a few rows spends its time on."""
+    if t is None:
+        return None
+    shape = t.shape
+    n = len(shape)
+    if n > MAX_DIMS:
+        raise ValueError(f"rank {n} exceeds {MAX_DIMS}")
+    pad = _PAD[n]
+    return _PACK(t.data_ptr(), _TORCH_TO_L3D[t.dtype], n, *shape, *pad, *t.stride(), *pad, 0)
+
+
 _P = C.POINTER(L3dTensor)
+_D = C.c_char_p  # an l3d_tensor as bytes (packed)
 _S = C.c_void_p
 _SIGS = {
     "l3d_abi_version": ([], C.c_int),
@@ -121,13 +141,13 @@ _SIGS = {
     "l3d_attention_selftest_timeout": ([_P, _P, _P, C.c_float, _P, C.c_void_p, C.c_size_t,
                                         C.c_uint32, _S], C.c_int),
     "l3d_lora_linear_workspace_size": ([C.c_int64, C.c_int64], C.c_size_t),
-    "l3d_lora_linear": ([_P, _P, _P, _P, _P, _P, _P, _P, C.c_int, _P, _P, _P, C.c_void_p,
+    "l3d_lora_linear": ([_D, _D, _D, _D, _D, _D, _D, _D, C.c_int, _D, _D, _D, C.c_void_p,
                          C.c_size_t, _S], C.c_int),
     "l3d_shared_prefix_attention_workspace_size": ([C.c_int64] * 7, C.c_size_t),
-    "l3d_shared_prefix_attention": ([_P, _P, _P, _P, _P, _P, C.c_int, C.c_float, _P, C.c_void_p,
+    "l3d_shared_prefix_attention": ([_D, _D, _D, _D, _D, _D, C.c_int, C.c_float, _D, C.c_void_p,
                                      C.c_size_t, _S], C.c_int),
-    "l3d_sandwich_residual_norm": ([_P, _P, C.c_int, _P, _P, _P, C.c_float, _P, _P, _P, _P,
-                                    C.c_float, C.c_float, _P, _P, _S], C.c_int),
+    "l3d_sandwich_residual_norm": ([_D, _D, C.c_int, _D, _D, _D, C.c_float, _D, _D, _D, _D,
+                                    C.c_float, C.c_float, _D, _D, _S], C.c_int),
     "l3d_gguf_index": ([C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.POINTER(C.c_int64),
                         C.POINTER(C.c_uint32), C.POINTER(C.c_uint64)], C.c_int),
     "l3d_gguf_metadata_string": ([C.c_void_p, C.c_uint64, C.c_char_p, C.POINTER(C.c_void_p),
@@ -168,6 +188,11 @@ def lib():
 
 def stream_handle(device=None) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of a CUDA tensor's device, without building a Stream object."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
 
 
 def call(name: str, *args):

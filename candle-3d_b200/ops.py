@@ -15,7 +15,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import call, desc, ref, stream_handle
+from ._lib import call, desc, packed, ref, stream_handle, stream_of
 
 ACT = {"none": 0, "silu": 1, "gelu_erf": 2, "gelu_tanh": 3}
 
@@ -533,27 +533,27 @@ class LoraAdapters:
         if not a or len(a) != len(b):
             raise ValueError("LoraAdapters needs as many a as b, at least one")
         _check_cuda(*a, *b)
-        K, N, dev = a[0].shape[1], b[0].shape[0], a[0].device
-        ranks = [t.shape[0] for t in a]
+        K, N, dev = a[0].shape[-1], b[0].shape[0], a[0].device
         for i, (u, w) in enumerate(zip(a, b)):
-            if u.dim() != 2 or w.dim() != 2 or u.shape[1] != K or w.shape != (N, ranks[i]):
+            if u.dim() != 2 or w.dim() != 2 or u.shape[1] != K or w.shape != (N, u.shape[0]):
                 raise ValueError(f"adapter {i}: a [rank, {K}] and b [{N}, rank] expected")
         scales = [1.0] * len(a) if scales is None else [float(v) for v in scales]
         if len(scales) != len(a):
             raise ValueError("LoraAdapters needs one scale per adapter")
+        ranks = [u.shape[0] for u in a]
         R = max(16, -(-max(ranks) // 16) * 16)
         self.n, self.k, self.rank, self.count = N, K, R, len(a)
         self.a = torch.zeros((len(a), R, K), dtype=torch.bfloat16, device=dev)
         self.b = torch.zeros((len(a), N, R), dtype=torch.bfloat16, device=dev)
-        for i, (u, w) in enumerate(zip(a, b)):
-            self.a[i, :ranks[i]] = u
-            self.b[i, :, :ranks[i]] = w
+        torch._foreach_copy_([self.a[i, :r] for i, r in enumerate(ranks)], a)
+        torch._foreach_copy_([self.b[i, :, :r] for i, r in enumerate(ranks)], b)
         self.scales = torch.tensor(scales, dtype=torch.float32, device=dev)
         self.ranks = torch.tensor(ranks, dtype=torch.int32, device=dev)
         # A row of another request meets these weights multiplied by zero.
-        if not (all(np.isfinite(scales)) and bool(torch.isfinite(self.a).all())
-                and bool(torch.isfinite(self.b).all())):
+        if not all(np.isfinite(scales)) or \
+                not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
             raise ValueError("LoraAdapters: weights and scales must be finite")
+        self._desc = tuple(map(packed, (self.a, self.b, self.scales, self.ranks)))
 
 
 def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, gate=None, out=None,
@@ -564,20 +564,17 @@ def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, ga
     or per request); an id outside [0, adapters.count) means no adapter."""
     _check_cuda(x, weight, ids, bias, residual, gate, out)
     n, k = weight.shape
-    x2 = x.reshape(-1, k)
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
     m = x2.shape[0]
-    if out is not None:
-        y = out.view(-1, n)
-    else:
-        y = torch.empty((m, n), dtype=out_dtype or x.dtype, device=x.device)
+    y = x.new_empty((m, n), dtype=out_dtype or x.dtype) if out is None else out.view(-1, n)
     need = _lib.lib().l3d_lora_linear_workspace_size(m, adapters.rank)
-    ws = torch.empty(need, dtype=torch.uint8, device=x.device)
-    r2 = None if residual is None else residual.reshape(-1, n)
-    call("l3d_lora_linear", ref(desc(x2)), ref(desc(weight)), ref(desc(bias)),
-         ref(desc(adapters.a)), ref(desc(adapters.b)), ref(desc(adapters.scales)),
-         ref(desc(adapters.ranks)), ref(desc(ids.reshape(-1))), ACT_CODES[act], ref(desc(r2)),
-         ref(desc(gate)), ref(desc(y)), ws.data_ptr(), need, _s(x))
-    return y.reshape(*x.shape[:-1], n)
+    ws = x.new_empty(need, dtype=torch.uint8)
+    if residual is not None and residual.dim() != 2:
+        residual = residual.reshape(-1, n)
+    call("l3d_lora_linear", packed(x2), packed(weight), packed(bias), *adapters._desc, packed(ids),
+         ACT_CODES[act], packed(residual), packed(gate), packed(y), ws.data_ptr(), need,
+         stream_of(x))
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None, causal=False,
@@ -591,15 +588,15 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None,
     _check_cuda(q, prefix_k, prefix_v, k, v, lengths, out)
     B, H, N, D = q.shape
     if out is None:
-        out = torch.empty((B, N, H, D), dtype=q.dtype, device=q.device).transpose(1, 2)
+        out = q.new_empty((B, N, H, D)).transpose(1, 2)
     Hkv, P = prefix_k.shape[:2]
     need = _lib.lib().l3d_shared_prefix_attention_workspace_size(
         B, H, Hkv, N, P, 0 if k is None else k.shape[2], D)
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    call("l3d_shared_prefix_attention", ref(desc(q)), ref(desc(prefix_k)), ref(desc(prefix_v)),
-         ref(desc(k)), ref(desc(v)), ref(desc(lengths)), int(bool(causal)),
-         D ** -0.5 if scale is None else float(scale), ref(desc(out)),
-         ws.data_ptr() if need else None, need, _s(q))
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
+    call("l3d_shared_prefix_attention", packed(q), packed(prefix_k), packed(prefix_v),
+         packed(k), packed(v), packed(lengths), int(bool(causal)),
+         D ** -0.5 if scale is None else float(scale), packed(out),
+         ws.data_ptr() if need else None, need, stream_of(q))
     return out
 
 
@@ -615,10 +612,10 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
     "rms" or "layer"; next_norm=False (the last block) returns (r, None); with
     inplace=True the residual stream x is updated in place (r is x)."""
     _check_cuda(x, h, post_weight, post_bias, gate, weight, bias, shift, scale)
-    r = x if inplace else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if next_norm else None
-    call("l3d_sandwich_residual_norm", ref(desc(x)), ref(desc(h)), NORMS[norm],
-         ref(desc(post_weight)), ref(desc(post_bias)), ref(desc(gate)), float(res_scale),
-         ref(desc(weight)), ref(desc(bias)), ref(desc(shift)), ref(desc(scale)),
-         eps if post_eps is None else post_eps, eps, ref(desc(r)), ref(desc(y)), _s(x))
+    r = x if inplace else x.new_empty(x.shape)
+    y = x.new_empty(x.shape) if next_norm else None
+    call("l3d_sandwich_residual_norm", packed(x), packed(h), NORMS[norm],
+         packed(post_weight), packed(post_bias), packed(gate), float(res_scale),
+         packed(weight), packed(bias), packed(shift), packed(scale),
+         eps if post_eps is None else post_eps, eps, packed(r), packed(y), stream_of(x))
     return r, y
