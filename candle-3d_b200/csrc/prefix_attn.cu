@@ -22,7 +22,9 @@
 //
 // Within an item the roles are those of attn.cu: a TMA warp fills a ring of
 // 128-key K and V tiles; MMA warps issue S = Q K^T and O += P V (P read from
-// tensor memory); four softmax warps per row tile, one row per thread, which
+// tensor memory); eight softmax warps per row tile, two threads per row with
+// half of its scores each (a row's chain from S to P is half as long as with
+// one thread; they exchange the row's maximum through shared memory), which
 // also load Q (their rows have no common stride) and zero the V rows past an
 // element's keys: a masked probability is 0, but 0 x NaN is not.
 // Every mbarrier wait is bounded (%globaltimer, 2 s); on expiry the block
@@ -46,26 +48,39 @@ constexpr float RESCALE_LOG2 = 8.f;
 
 __device__ int g_pattn_status;
 
+#ifndef POLY64
+#define POLY64 2
+#endif
+#ifndef POLY128
+#define POLY128 0
+#endif
 // NT row tiles of 128 rows per block.
 template <int D, int NT>
 struct Cfg {
   static constexpr int DC = D / 64;
   static constexpr int Q_BYTES = BQ * D * 2;
   static constexpr int KV_BYTES = BKV * D * 2;
-  static constexpr int STAGES = (227 * 1024 - 256 - NT * Q_BYTES) / (2 * KV_BYTES) < 6
-                                    ? (227 * 1024 - 256 - NT * Q_BYTES) / (2 * KV_BYTES) : 6;
-  static constexpr int SMEM = NT * Q_BYTES + STAGES * 2 * KV_BYTES + 256;
   static constexpr uint32_t COL_S = 0, COL_O = NT * BKV;
   // P_t has columns of its own where they fit, so that S_t(j + 1) is computed
   // while the softmax of tile j runs; otherwise it goes over S_t.
   static constexpr bool SEP_P = COL_O + NT * D + NT * (BKV / 2) <= TMEM_COLS;
   static constexpr uint32_t COL_P = SEP_P ? COL_O + NT * D : COL_S;
   static constexpr uint32_t P_STRIDE = SEP_P ? BKV / 2 : BKV;
+  // Floats that the two threads of a row exchange.  Without SEP_P one buffer
+  // serves: S_t(j + 1) complete means that all have read those of tile j.
+  static constexpr int TURNS = SEP_P ? 2 : 1;
+  static constexpr int REST = 384 + TURNS * NT * 2 * BQ * 4;
+  // K and V tiles in rings of their own, each released when its product has
+  // read it.
+  static constexpr int FIT = (227 * 1024 - REST - NT * Q_BYTES) / KV_BYTES;
+  static constexpr int BUFS = FIT < 12 ? FIT : 12;
+  static constexpr int KST = BUFS / 2, VST = BUFS - KST;
+  static constexpr int SMEM = NT * Q_BYTES + BUFS * KV_BYTES + REST;
   static constexpr int NMMA = SEP_P ? NT : 1;
-  static constexpr int THREADS = (1 + NMMA + 4 * NT) * 32;
-  static constexpr int POLY = D == 64 ? 2 : 0;  // of 8 pairs of P, those of ex2_poly2
+  static constexpr int THREADS = (4 + 8 * NT) * 32;    // TMA and MMA warps, softmax warps
+  static constexpr int POLY = D == 64 ? POLY64 : POLY128;  // of 8 pairs of P, those of ex2_poly2
   static_assert(COL_O + NT * D <= TMEM_COLS, "TMEM budget");
-  static_assert((2 * STAGES + 5 * NT + NMMA) * 8 + 16 <= 256, "barrier area");
+  static_assert((2 * BUFS + 4 * NT + NMMA) * 8 + 16 <= 384, "barrier area");
 };
 
 struct View {        // a K or V map: heads listed before rows; 0 for a broadcast dimension
@@ -75,7 +90,7 @@ struct View {        // a K or V map: heads listed before rows; 0 for a broadcas
 struct Params {
   int B, N, G, Hkv;
   int RG, F;                 // rows of one element, of the batch (per key head)
-  int64_t P, S;
+  int P, S;                  // at most 2^30
   View pk, pv, k, v;
   const void* q;
   void* out;
@@ -91,11 +106,29 @@ struct Params {
   uint64_t wait_ns;
 };
 
-__device__ __forceinline__ int64_t own_length(const Params& p, int b) {
+__device__ __forceinline__ int own_length(const Params& p, int b) {
   if (!p.lengths) return p.S;
   const int64_t v = p.len64 ? static_cast<const int64_t*>(p.lengths)[b]
                             : static_cast<const int32_t*>(p.lengths)[b];
-  return v < 0 ? 0 : v < p.S ? v : p.S;
+  return v < 0 ? 0 : v < p.S ? int(v) : p.S;
+}
+// Row f of a key head is query i of head h G + g of element b, f = (b N + i) G + g.
+struct Row {
+  int b, i, g;
+};
+__device__ __forceinline__ Row row_at(const Params& p, int f) {
+  const int b = f / p.RG, i = (f - b * p.RG) / p.G;
+  return {b, i, f - b * p.RG - i * p.G};
+}
+
+// 16 consecutive 32-bit TMEM columns of this thread's lane <- registers.
+__device__ __forceinline__ void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, "
+      "%11, %12, %13, %14, %15, %16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+      "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
 }
 
 template <typename T> __device__ __forceinline__ uint32_t pack_pair(float a, float b);
@@ -128,27 +161,30 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     return;
   }
   uint8_t* sq = smem_raw;                            // [NT][DC][128 x 64]
-  uint8_t* sk = sq + NT * C::Q_BYTES;                // [STAGES][DC][128 x 64]
-  uint8_t* sv = sk + C::STAGES * C::KV_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sv + C::STAGES * C::KV_BYTES);
-  uint64_t* q_full = bars;                           // [NT]
-  uint64_t* kv_full = q_full + NT;                   // [STAGES]
-  uint64_t* kv_empty = kv_full + C::STAGES;          // [STAGES]
-  uint64_t* s_full = kv_empty + C::STAGES;           // [NT]
+  uint8_t* sk = sq + NT * C::Q_BYTES;                // [KST][DC][128 x 64]
+  uint8_t* sv = sk + C::KST * C::KV_BYTES;           // [VST][DC][128 x 64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sv + C::VST * C::KV_BYTES);
+  uint64_t* k_full = bars;                           // [KST]
+  uint64_t* k_empty = k_full + C::KST;               // [KST]
+  uint64_t* v_full = k_empty + C::KST;               // [VST]
+  uint64_t* v_empty = v_full + C::VST;               // [VST]
+  uint64_t* s_full = v_empty + C::VST;               // [NT]
   uint64_t* p_full = s_full + NT;                    // [NT]
   uint64_t* pv_done = p_full + NT;                   // [NT] (SEP_P: every P V; else the last)
   uint64_t* s_free = pv_done + NT;                   // [NT] (SEP_P only)
   uint64_t* mma_drain = s_free + NT;                 // [NMMA] abort teardown only
   volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + C::NMMA);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + C::NMMA + 1);
+  float* xch = reinterpret_cast<float*>(bars + 48);  // [TURNS][NT][2][BQ]
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (The shuffle tells the compiler that the role is the same in all lanes.)
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");
   // ---- this block's item: rows [f0, fend) of key head h, prefix tiles
   // [pa, pa + np), own tiles [sa, sa + nkv - np) of element b.
   int idx = blockIdx.x;
   int f0, fend, h, b = 0, pa, np, sa = 0, nkv, slot;
-  int64_t len = 0;
+  int len = 0;
   if (idx < p.prefix_items) {
     const int qt = idx % p.tiles_p;
     idx /= p.tiles_p;
@@ -156,7 +192,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     slot = idx / p.Hkv;
     f0 = qt * (NT * BQ);
     fend = p.F;
-    const int tiles = int((p.P + BKV - 1) / BKV);
+    const int tiles = (p.P + BKV - 1) / BKV;
     pa = slot * p.chunk_p;
     np = max(min(p.chunk_p, tiles - pa), 0);
     nkv = np;
@@ -172,13 +208,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     fend = (b + 1) * p.RG;
     len = own_length(p, b);
     // Own keys that the last of the item's rows sees.
-    int64_t seen = len;
-    if (p.causal) {
-      const int64_t last = (min(f0 + NT * BQ, fend) - 1 - b * p.RG) / p.G;
-      seen = max(min(len, len - p.N + last + 1), int64_t(0));
-    }
-    const int own = int((seen + BKV - 1) / BKV);
-    const int pre = p.joint ? int((p.P + BKV - 1) / BKV) : 0;
+    int seen = len;
+    if (p.causal) seen = max(min(len, len - p.N + row_at(p, min(f0 + NT * BQ, fend) - 1).i + 1), 0);
+    const int own = (seen + BKV - 1) / BKV;
+    const int pre = p.joint ? (p.P + BKV - 1) / BKV : 0;
     const int c0 = part * p.chunk_o;
     const int c1 = min(c0 + p.chunk_o, pre + own);
     pa = min(c0, pre);
@@ -189,48 +222,76 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   }
   const int ntv = min((fend - f0 + BQ - 1) / BQ, NT);  // row tiles that hold rows
   const int nmma = C::SEP_P ? ntv : 1;
-  int nload[C::STAGES];
-#pragma unroll
-  for (int s = 0; s < C::STAGES; ++s) nload[s] = 0;
-  // Key tile j (K and V) into ring stage j % STAGES (thread 0).
-  auto load_kv = [&](int j) {
-    const int s = j % C::STAGES;
-    ++nload[s];
-    mbar_expect_tx(&kv_full[s], 2 * C::KV_BYTES);
+  // Key tile j of K or V into its ring (thread 0).
+  int loaded_k = 0, loaded_v = 0;
+  auto load = [&](uint8_t* dst, uint64_t* bar, int j, const CUtensorMap* mp, const CUtensorMap* mo,
+                  const View& wp, const View& wo) {
+    mbar_expect_tx(bar, C::KV_BYTES);
     const bool pre = j < np;
     const int row = (pre ? pa + j : sa + j - np) * BKV;
-    auto put = [&](uint8_t* dst, const CUtensorMap* map, const View& w) {
-      const int hh = h * w.hm, bb = pre ? 0 : b * w.bm;
-      for (int dc = 0; dc < C::DC; ++dc)
-        tma_load_4d(dst + dc * (BKV * 128), map, &kv_full[s], dc * 64, w.hn ? hh : row,
-                    w.hn ? row : hh, bb);
-    };
-    put(sk + s * C::KV_BYTES, pre ? &map_pk : &map_k, pre ? p.pk : p.k);
-    put(sv + s * C::KV_BYTES, pre ? &map_pv : &map_v, pre ? p.pv : p.v);
+    const View& w = pre ? wp : wo;
+    const int hh = h * w.hm, bb = pre ? 0 : b * w.bm;
+    for (int dc = 0; dc < C::DC; ++dc)
+      tma_load_4d(dst + dc * (BKV * 128), pre ? mp : mo, bar, dc * 64, w.hn ? hh : row, w.hn ? row : hh, bb);
+  };
+  auto load_k = [&] {
+    const int s = loaded_k % C::KST;
+    load(sk + s * C::KV_BYTES, &k_full[s], loaded_k++, &map_pk, &map_k, p.pk, p.k);
+  };
+  auto load_v = [&] {
+    const int s = loaded_v % C::VST;
+    load(sv + s * C::KV_BYTES, &v_full[s], loaded_v++, &map_pv, &map_v, p.pv, p.v);
   };
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], nmma);
+    for (int s = 0; s < C::KST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], nmma);
+    }
+    for (int s = 0; s < C::VST; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], nmma);
     }
     for (int t = 0; t < NT; ++t) {
-      mbar_init(&q_full[t], 4);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&s_free[t], 4);
+      mbar_init(&p_full[t], 8);
+      mbar_init(&s_free[t], 8);
       mbar_init(&pv_done[t], 1);
     }
     for (int w = 0; w < C::NMMA; ++w) mbar_init(&mma_drain[w], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    for (int j = 0; j < nkv && j < C::STAGES; ++j) load_kv(j);
+    for (int j = 0; j < nkv && j < C::VST; ++j) {
+      if (j < C::KST) load_k();
+      load_v();
+    }
   }
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
                  "r"(TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  // The softmax threads' row (tile st, TMEM lane quarter warp % 4): two threads
+  // per row, `half` of its scores, of its output and of Q each.
+  const int sw = warp - 4, st = sw >> 3, half = (sw >> 2) & 1;
+  const int r = (warp & 3) * 32 + lane;
+  const int f = f0 + st * BQ + r;                // flattened row
+  const bool valid = f < fend;
+  if (sw >= 0 && st < ntv) {
+    const Row w = row_at(p, valid ? f : fend - 1);
+    const T* qr = static_cast<const T*>(p.q) + w.b * p.qb + int64_t(h * p.G + w.g) * p.qh + w.i * p.qn;
+    uint8_t* qt = sq + st * C::Q_BYTES + r * 128;
+    uint4 u[D / 16];
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      u[c] = valid ? __ldg(reinterpret_cast<const uint4*>(qr) + half * (D / 16) + c) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      const int c = half * (D / 16) + i;
+      *reinterpret_cast<uint4*>(qt + (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4)) = u[i];
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
@@ -240,12 +301,24 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     return mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, p.wait_ns);
   };
 
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {  // the warp's lanes stay together
+    const bool got = __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    __syncwarp();  // before the warp-wide (.aligned) instructions that follow
+    return got;
+  };
+
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (lane == 0) {
-      for (int j = C::STAGES; j < nkv && !*abort_flag; ++j) {
-        if (!wait(&kv_empty[j % C::STAGES], ((j / C::STAGES) - 1) & 1)) break;
-        load_kv(j);
+      while ((loaded_k < nkv || loaded_v < nkv) && !*abort_flag) {
+        if (loaded_k < nkv) {
+          if (!wait(&k_empty[loaded_k % C::KST], (loaded_k / C::KST - 1) & 1)) break;
+          load_k();
+        }
+        if (loaded_v < nkv) {
+          if (!wait(&v_empty[loaded_v % C::VST], (loaded_v / C::VST - 1) & 1)) break;
+          load_v();
+        }
       }
     }
   } else if (warp <= C::NMMA) {
@@ -253,242 +326,261 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     constexpr int TPW = NT / C::NMMA;
     const int t0 = (warp - 1) * TPW;
     const int t1 = min(t0 + TPW, ntv);  // this warp's row tiles: t0 .. t1 - 1
-    if (lane == 0 && t0 < t1 && nkv > 0) {
+    // The whole warp keeps step and one elected lane issues, so that loop state
+    // and descriptors stay in uniform registers.
+    const bool leader = elect_one();
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+    };
+    if (t0 < t1 && nkv > 0) {
       auto issue_s = [&](int t, int j) {
-        const uint8_t* kt = sk + (j % C::STAGES) * C::KV_BYTES;
+        const uint8_t* kt = sk + (j % C::KST) * C::KV_BYTES;
         const uint8_t* qt = sq + t * C::Q_BYTES;
+        const uint64_t da0 = smem_desc_sw128(qt), db0 = smem_desc_sw128(kt);
+        if (leader) {
 #pragma unroll
-        for (int dc = 0; dc < C::DC; ++dc) {
-          const uint64_t da = smem_desc_sw128(qt + dc * (BQ * 128));
-          const uint64_t db = smem_desc_sw128(kt + dc * (BKV * 128));
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            umma_f16<IDESC_S>(tmem_base + C::COL_S + t * BKV, da + uint64_t(2 * k),
-                              db + uint64_t(2 * k), (dc | k) ? 1u : 0u);
+          for (int k = 0; k < D / 16; ++k) {
+            const uint64_t off = uint64_t((k >> 2) * (BQ * 128 >> 4) + 2 * (k & 3));
+            umma_f16<IDESC_S>(tmem_base + C::COL_S + t * BKV, da0 + off, db0 + off, k ? 1u : 0u);
+          }
         }
-        umma_commit(&s_full[t]);
+        commit(&s_full[t]);
+        if (t == t1 - 1) commit(&k_empty[j % C::KST]);
       };
       auto issue_pv = [&](int t, int j) {
-        const uint64_t db = smem_desc_sw128_mn(sv + (j % C::STAGES) * C::KV_BYTES, BKV * 128);
+        const uint64_t db = smem_desc_sw128_mn(sv + (j % C::VST) * C::KV_BYTES, BKV * 128);
         const uint32_t ta = tmem_base + C::COL_P + t * C::P_STRIDE;
+        if (leader) {
 #pragma unroll
-        for (int ks = 0; ks < BKV / 16; ++ks)
-          umma_f16_ts<IDESC_O>(tmem_base + C::COL_O + t * D, ta + uint32_t(ks * 8),
-                               db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
+          for (int ks = 0; ks < BKV / 16; ++ks)
+            umma_f16_ts<IDESC_O>(tmem_base + C::COL_O + t * D, ta + uint32_t(ks * 8),
+                                 db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
+        }
+        if (t == t1 - 1) commit(&v_empty[j % C::VST]);
+        if (C::SEP_P || j + 1 == nkv) commit(&pv_done[t]);  // the last one: the block waits for it
       };
-      bool ok = true;
-      for (int t = t0; ok && t < t1; ++t) ok = wait(&q_full[t], 0);
-      ok = ok && wait(&kv_full[0], 0);
+      auto wait_k = [&](int j) { return wait_warp(&k_full[j % C::KST], (j / C::KST) & 1); };
+      bool ok = wait_k(0);
       if (ok) {
         tc_fence_after();
         for (int t = t0; t < t1; ++t) issue_s(t, 0);
       }
       for (int j = 0; ok && j < nkv; ++j) {
         const bool more = j + 1 < nkv;
-        bool kv_ready = !more;
-        auto wait_kv = [&]() {
-          if (!kv_ready) kv_ready = wait(&kv_full[(j + 1) % C::STAGES], ((j + 1) / C::STAGES) & 1);
-          return kv_ready;
-        };
         for (int t = t0; ok && t < t1; ++t) {
-          if constexpr (C::SEP_P) {
-            // S_t(j+1) once the softmax warps have copied S_t(j), then P_t(j) V.
-            if (more) {
-              if (!wait_kv() || !wait(&s_free[t], j & 1)) { ok = false; break; }
-              tc_fence_after();
-              issue_s(t, j + 1);
-            }
-            if (!wait(&p_full[t], j & 1)) { ok = false; break; }
+          // SEP_P: S_t(j+1) once the softmax warps have copied S_t(j), then
+          // P_t(j) V.  Else P_t(j) V, then S_t(j+1) over the consumed P_t(j).
+          if (C::SEP_P && more) {
+            ok = (t > t0 || wait_k(j + 1)) && wait_warp(&s_free[t], j & 1);
+            if (!ok) break;
             tc_fence_after();
-            issue_pv(t, j);
-            umma_commit(&pv_done[t]);
-            if (t == t1 - 1) umma_commit(&kv_empty[j % C::STAGES]);
-          } else {
-            // P_t(j) V, then S_t(j+1) over the consumed P_t(j).
-            if (!wait(&p_full[t], j & 1)) { ok = false; break; }
+            issue_s(t, j + 1);
+          }
+          ok = wait_warp(&p_full[t], j & 1) && (t > t0 || wait_warp(&v_full[j % C::VST], (j / C::VST) & 1));
+          if (!ok) break;
+          tc_fence_after();
+          issue_pv(t, j);
+          if (!C::SEP_P && more) {
+            ok = t > t0 || wait_k(j + 1);
+            if (!ok) break;
             tc_fence_after();
-            issue_pv(t, j);
-            if (t == t1 - 1) umma_commit(&kv_empty[j % C::STAGES]);
-            if (more) {
-              if (!wait_kv()) { ok = false; break; }
-              tc_fence_after();
-              issue_s(t, j + 1);
-            } else {
-              umma_commit(&pv_done[t]);
-            }
+            issue_s(t, j + 1);
           }
         }
       }
     }
-  } else if ((warp - 1 - C::NMMA) >> 2 < ntv) {
+  } else if (warp >= 4 && st < ntv) {
     // ------------------------------------------------------ softmax / epilogue
-    const int t = (warp - 1 - C::NMMA) >> 2;
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) {  // the warp's lanes stay together
-      return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
-    };
-    const int quarter = warp & 3;
-    const int r = quarter * 32 + lane;
-    const int f = f0 + t * BQ + r;
-    const bool valid = f < fend;
+    const int t = st, quarter = warp & 3;
     const bool active = f - lane < fend;  // the warp holds rows
-    // Row f = (fb N + fi) G + fg.
-    const int ff = valid ? f : fend - 1;
-    const int fb = ff / p.RG, fi = (ff - fb * p.RG) / p.G, fg = ff - fb * p.RG - fi * p.G;
-    {
-      const T* qr = static_cast<const T*>(p.q) + fb * p.qb + int64_t(h * p.G + fg) * p.qh + fi * p.qn;
-      uint8_t* qt = sq + t * C::Q_BYTES + r * 128;
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 u = make_uint4(0, 0, 0, 0);
-        if (valid) u = __ldg(reinterpret_cast<const uint4*>(qr) + c);
-        *reinterpret_cast<uint4*>(qt + (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4)) = u;
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&q_full[t]);
-    }
     // Own keys that this row sees.
-    const int64_t lim = p.causal ? min(len, len - p.N + fi + 1) : len;
+    const int lim = p.causal ? min(len, len - p.N + row_at(p, valid ? f : fend - 1).i + 1) : len;
     const uint32_t lane_off = uint32_t(quarter * 32) << 16;
-    const uint32_t t_s = tmem_base + C::COL_S + t * BKV + lane_off;
-    const uint32_t t_o = tmem_base + C::COL_O + t * D + lane_off;
-    const uint32_t t_p = tmem_base + C::COL_P + t * C::P_STRIDE + lane_off;
+    const uint32_t t_s = tmem_base + C::COL_S + t * BKV + half * (BKV / 2) + lane_off;
+    const uint32_t t_o = tmem_base + C::COL_O + t * D + half * (D / 2) + lane_off;
+    const uint32_t t_p = tmem_base + C::COL_P + t * C::P_STRIDE + half * (BKV / 4) + lane_off;
     const float2 sc2 = f2(p.scale_log2);
-    float m = -INFINITY;                         // running max, log2 units
-    float2 l2 = f2(0.f);                         // running row sum (two halves)
+    float m = -INFINITY;                         // running max, log2 units (both threads')
+    float2 l2 = f2(0.f);                         // running sum of this half (two parts)
     bool ok = true;
+    // A warp whose wait has run out goes on to the next exchange, where the
+    // pair of warps that share rows leaves together.
+    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
+      if (ok) ok = wait_warp(bar, parity);
+      return ok;
+    };
+    // The other half's value; false once either warp has failed.
+    int turn = 0;
+    auto exchange = [&](float mine, float& other) {
+      float* x = xch + ((turn * NT + t) * 2) * BQ + r;
+      turn = (turn + 1) % C::TURNS;
+      x[half * BQ] = mine;
+      uint32_t both;
+      asm volatile(
+          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+          "bar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+          : "=r"(both)
+          : "r"(uint32_t(ok)), "r"(1 + t * 4 + quarter)
+          : "memory");
+      other = x[(half ^ 1) * BQ];
+      return both != 0;
+    };
     for (int j = 0; j < nkv; ++j) {
-      if (!wait_all(&s_full[t], j & 1)) { ok = false; break; }
-      tc_fence_after();
+      if (wait_all(&s_full[t], j & 1)) tc_fence_after();
       const bool pre = j < np;
-      const int64_t key0 = int64_t(pre ? pa + j : sa + j - np) * BKV;
-      // V rows past the element's keys may hold anything (S(j) complete means
-      // that the tile has landed).
-      const int held = int(min(pre ? int64_t(BKV) : len - key0, int64_t(BKV)));
-      if (r >= held) {
-        uint8_t* vr = sv + (j % C::STAGES) * C::KV_BYTES + r * 128;
+      const int key0 = (pre ? pa + j : sa + j - np) * BKV;
+      // V rows past the element's keys may hold anything: zero them, once the
+      // tile has landed.
+      const int held = pre ? BKV : min(len - key0, BKV);
+      if (held < BKV) {
+        if (wait_all(&v_full[j % C::VST], (j / C::VST) & 1) && r >= held) {
+          uint8_t* vr = sv + (j % C::VST) * C::KV_BYTES + r * 128;
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c)
-          *reinterpret_cast<uint4*>(vr + (c >> 3) * (BKV * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          for (int i = 0; i < D / 16; ++i) {
+            const int c = half * (D / 16) + i;
+            *reinterpret_cast<uint4*>(vr + (c >> 3) * (BKV * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+          }
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
       }
-      if (held < BKV) asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      __syncwarp();
       bool pv_waited = !C::SEP_P || j == 0;
       auto wait_pv = [&]() {  // P_t(j-1) V has read P_t and O_t is stable
-        if (pv_waited) return true;
-        pv_waited = wait_all(&pv_done[t], (j - 1) & 1);
-        tc_fence_after();
-        return pv_waited;
+        if (!pv_waited) {
+          pv_waited = true;
+          if (wait_all(&pv_done[t], (j - 1) & 1)) tc_fence_after();
+        }
       };
-      if (!active) {  // no rows: keep the other warps' pace
+      if (!active) {  // no rows (in either half): keep the other warps' pace
+        if (!ok) break;
         if constexpr (C::SEP_P) {
           if (lane == 0) mbar_arrive(&s_free[t]);
         }
-        if (!wait_pv()) { ok = false; break; }
-        __syncwarp();
+        wait_pv();
+        if (!ok) break;
         if (lane == 0) mbar_arrive(&p_full[t]);
         continue;
       }
-      float sv_[BKV];
+      float s[BKV / 2];
+      float mx = -INFINITY;
+      if (ok) {
+        tmem_ld64(t_s, s);
+        if constexpr (C::SEP_P) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s_free[t]);
+        }
+        // Keys of this half of the tile that the row sees.
+        const int kvalid = (pre ? p.P : lim) - key0 - half * (BKV / 2);
+        if (kvalid < BKV / 2) {
 #pragma unroll
-      for (int c = 0; c < BKV; c += 64) tmem_ld64(t_s + uint32_t(c), sv_ + c);
-      if constexpr (C::SEP_P) {
-        tc_fence_before();
+          for (int e = 0; e < BKV / 2; ++e)
+            if (e >= kvalid) s[e] = -INFINITY;
+        }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s_free[t]);
-      }
-      const int64_t kv64 = (pre ? p.P : lim) - key0;  // keys of this tile that the row sees
-      if (kv64 < BKV) {
-        const int kvalid = int(max(kv64, int64_t(0)));
+        float mx0 = s[0], mx1 = s[1];
 #pragma unroll
-        for (int e = 0; e < BKV; ++e)
-          if (e >= kvalid) sv_[e] = -INFINITY;
+        for (int e = 2; e < BKV / 2; e += 2) {
+          mx0 = fmaxf(mx0, s[e]);
+          mx1 = fmaxf(mx1, s[e + 1]);
+        }
+        mx = fmaxf(mx0, mx1);
       }
-      __syncwarp();
-      float mx0 = sv_[0], mx1 = sv_[1];
-#pragma unroll
-      for (int e = 2; e < BKV; e += 2) {
-        mx0 = fmaxf(mx0, sv_[e]);
-        mx1 = fmaxf(mx1, sv_[e + 1]);
-      }
-      const float mxs = fmaxf(mx0, mx1) * p.scale_log2;  // scale > 0
-      const bool grow = mxs > m + RESCALE_LOG2;          // always on the first key a row sees
+      float other;
+      // (Past the exchange both halves have copied S_t: P_t may go over it.)
+      if (!exchange(mx, other)) { ok = false; break; }
+      const float mxs = fmaxf(mx, other) * p.scale_log2;  // scale > 0
+      const bool grow = mxs > m + RESCALE_LOG2;           // always on the first key a row sees
       const float m_new = grow ? mxs : m;
-      const float alpha = grow ? ex2f(m - m_new) : 1.f;  // 0 on the first
+      const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        if (!wait_pv()) { ok = false; break; }
+        wait_pv();
+        if (ok) {
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          tmem_ld32(t_o + uint32_t(c), o);
-          uint32_t u[32];
+          for (int c = 0; c < D / 2; c += 16) {  // (s is live: few columns at a time)
+            float o[16];
+            tmem_ld16(t_o + uint32_t(c), o);
+            uint32_t u[16];
 #pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
-            u[e] = __float_as_uint(v.x);
-            u[e + 1] = __float_as_uint(v.y);
+            for (int e = 0; e < 16; e += 2) {
+              const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
+              u[e] = __float_as_uint(v.x);
+              u[e + 1] = __float_as_uint(v.y);
+            }
+            tmem_st16u(t_o + uint32_t(c), u);
           }
-          tmem_st32u(t_o + uint32_t(c), u);
         }
       }
       // P = exp2(s * scale * log2 e - m); a row that has seen no key yet has
       // m = -inf and all its scores masked: subtract 0, so that P = 0.
       const float2 nm2 = f2(m_new == -INFINITY ? 0.f : -m_new);
       l2 = mul2(l2, f2(alpha));
-      uint32_t u[BKV / 2];
+      // In pieces of 32 scores, stored to TMEM as they are formed.
+      wait_pv();
 #pragma unroll
-      for (int e = 0; e < BKV; e += 2) {
-        const float2 x = fma2(make_float2(sv_[e], sv_[e + 1]), sc2, nm2);
-        const float2 pr = ((e >> 1) & 7) < C::POLY ? ex2_poly2(x)
-                                                   : make_float2(ex2f(x.x), ex2f(x.y));
-        l2 = add2(l2, pr);
-        u[e >> 1] = pack_pair<T>(pr.x, pr.y);
+      for (int c = 0; c < BKV / 2; c += 32) {
+        uint32_t u[16];
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+          const float2 x = fma2(make_float2(s[c + e], s[c + e + 1]), sc2, nm2);
+          const float2 pr = ((e >> 1) & 7) < C::POLY ? ex2_poly2(x)
+                                                     : make_float2(ex2f(x.x), ex2f(x.y));
+          l2 = add2(l2, pr);
+          u[e >> 1] = pack_pair<T>(pr.x, pr.y);
+        }
+        if (ok) tmem_st16u(t_p + uint32_t(c / 2), u);
       }
-      if (!wait_pv()) { ok = false; break; }
-#pragma unroll
-      for (int c = 0; c < BKV / 2; c += 32) tmem_st32u(t_p + uint32_t(c), u + c);
-      tmem_wait_st();
       m = m_new;
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[t]);
+      if (ok) {
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
     }
     // Epilogue, after the last P V: the output, or this part's O / l and log2 sum.
-    if (ok && nkv > 0)
-      ok = wait_all(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0);
-    if (ok && active) {
-      tc_fence_after();
+    if (active) {
+      if (nkv > 0 && wait_all(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0)) tc_fence_after();
       // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)
-      const float l = m == -INFINITY && l2.x == l2.x && l2.y == l2.y ? 0.f : l2.x + l2.y;
-      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
-      const int64_t pr = (int64_t(slot) * p.Hkv + h) * p.F + f;
-      if (p.slots > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
-      T* orow = static_cast<T*>(p.out) + fb * p.ob + int64_t(h * p.G + fg) * p.oh + fi * p.on;
+      const float own = l2.x + l2.y;
+      float other;
+      // ok is the pair's here or, where the loop was left, false in both.
+      if (exchange(own, other)) {
+        float l = own + other;
+        if (m == -INFINITY && l == l) l = 0.f;
+        const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
+        const int64_t pr = (int64_t(slot) * p.Hkv + h) * p.F + f;
+        if (p.slots > 1 && valid && half == 0)
+          p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
+        const Row w = row_at(p, valid ? f : fend - 1);
+        T* orow = static_cast<T*>(p.out) + w.b * p.ob + int64_t(h * p.G + w.g) * p.oh + w.i * p.on + half * (D / 2);
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        float o[32];
-        if (nkv > 0) {
-          tmem_ld32(t_o + uint32_t(c), o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0.f;
-        }
-        if (valid) {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] *= inv;
-          if (p.slots > 1) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+        for (int c = 0; c < D / 2; c += 32) {
+          float o[32];
+          if (nkv > 0) {
+            tmem_ld32(t_o + uint32_t(c), o);
           } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              float w[8];
+            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+          }
+          if (valid) {
 #pragma unroll
-              for (int e = 0; e < 8; ++e) w[e] = o[8 * q + e];
-              *reinterpret_cast<uint4*>(orow + c + 8 * q) = pack(w, T());
+            for (int e = 0; e < 32; ++e) o[e] *= inv;
+            if (p.slots > 1) {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + half * (D / 2) + c);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+            } else {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) w[e] = o[8 * q + e];
+                *reinterpret_cast<uint4*>(orow + c + 8 * q) = pack(w, T());
+              }
             }
           }
+          __syncwarp();
         }
       }
     }
@@ -499,14 +591,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (warp >= 1 && warp <= C::NMMA && lane == 0) {
+    if (warp >= 1 && warp <= C::NMMA && elect_one()) {  // the lane that issued
       umma_commit(&mma_drain[warp - 1]);
       mbar_drain(&mma_drain[warp - 1], 0, p.wait_ns);
     }
     if (threadIdx.x == 0) {
-#pragma unroll
-      for (int s = 0; s < C::STAGES; ++s)
-        if (nload[s] > 0) mbar_drain(&kv_full[s], uint32_t(nload[s] - 1) & 1u, p.wait_ns);
+      // The newest load of each ring buffer.
+      for (int i = max(loaded_k - C::KST, 0); i < loaded_k; ++i)
+        mbar_drain(&k_full[i % C::KST], uint32_t(i / C::KST) & 1u, p.wait_ns);
+      for (int i = max(loaded_v - C::VST, 0); i < loaded_v; ++i)
+        mbar_drain(&v_full[i % C::VST], uint32_t(i / C::VST) & 1u, p.wait_ns);
     }
   }
   __syncthreads();
@@ -570,9 +664,9 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
     }
   }
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  const int f = int(row % p.F), h = int(row / p.F);
-  const int fb = f / p.RG, fi = (f - fb * p.RG) / p.G, fg = f - fb * p.RG - fi * p.G;
-  T* orow = static_cast<T*>(p.out) + fb * p.ob + int64_t(h * p.G + fg) * p.oh + fi * p.on + lane * E;
+  const int h = int(row / p.F);
+  const Row at = row_at(p, int(row % p.F));
+  T* orow = static_cast<T*>(p.out) + at.b * p.ob + int64_t(h * p.G + at.g) * p.oh + at.i * p.on + lane * E;
 #pragma unroll
   for (int e = 0; e < E; ++e) orow[e] = from_f<T>(acc[e] * inv);
 }
@@ -723,7 +817,7 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
   }
   if (!(scale > 0.f) || !(scale < 3.0e38f))
     return fail(L3D_E_UNSUPPORTED, "%s: scale must be positive and finite", op);
-  const int64_t big = int64_t(1) << 30;
+  const int64_t big = int64_t(1) << 30;  // also keeps key and row arithmetic in 32 bits
   if (B > 65535 || Hq > 65535 || N > big || P > big || S > big || B * Hq * N > big)
     return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large", op);
   const l3d_tensor* kvs[] = {prefix_k, prefix_v, k, v};
@@ -751,7 +845,7 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
   Params p{};
   p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);
   p.RG = int(N * p.G); p.F = int(B) * p.RG;
-  p.P = P; p.S = S;
+  p.P = int(P); p.S = int(S);
   p.q = elem_ptr(q);
   p.out = const_cast<char*>(elem_ptr(out));
   p.qb = q->strides[0]; p.qh = q->strides[1]; p.qn = q->strides[2];
