@@ -20,13 +20,16 @@
 // weighs the parts of each row.  Parts have fixed places, so results do not
 // depend on the order in which blocks run.
 //
-// Within an item the roles are those of attn.cu: a TMA warp fills a ring of
-// 128-key K and V tiles; MMA warps issue S = Q K^T and O += P V (P read from
-// tensor memory); eight softmax warps per row tile, two threads per row with
-// half of its scores each (a row's chain from S to P is half as long as with
-// one thread; they exchange the row's maximum through shared memory), which
-// also load Q (their rows have no common stride) and zero the V rows past an
-// element's keys: a masked probability is 0, but 0 x NaN is not.
+// Within an item a TMA warp fills rings of 64-key K and V tiles; one MMA warp
+// per row tile issues S = Q K^T and O += P V (P read from tensor memory); four
+// softmax warps per row tile, one row per thread, turn S into P, and also load
+// Q (their rows have no common stride) and zero the V rows past an element's
+// keys: a masked probability is 0, but 0 x NaN is not.  S has two buffers of 64
+// columns per row tile, P going over the scores it comes from: S(j + 2) is
+// issued right after P(j) V, while softmax(j + 1) runs, so that neither the
+// tensor core nor the softmax warps wait for a whole round trip of the other.
+// (With one 128-column buffer a row tile's softmax warps waited 1,500 of 3,830
+// clocks per 128 keys at D = 128, and both pipes were about half busy.)
 // Every mbarrier wait is bounded (%globaltimer, 2 s); on expiry the block
 // records an error in the device's status word and stops.
 #include <type_traits>
@@ -40,8 +43,7 @@ namespace pattn {
 
 using namespace l3d::attn;
 
-constexpr int BQ = 128, BKV = 128;
-constexpr int TMEM_COLS = 512;
+constexpr int BQ = 128, BKV = 64;
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 // As in attn.cu: the running max moves only when it grows past 2^8.
 constexpr float RESCALE_LOG2 = 8.f;
@@ -54,33 +56,27 @@ __device__ int g_pattn_status;
 #ifndef POLY128
 #define POLY128 0
 #endif
-// NT row tiles of 128 rows per block.
+// NT row tiles of 128 rows per block; NT = 1 blocks share an SM in pairs, for
+// short items, whose set-up one block's work then hides for the other.
 template <int D, int NT>
 struct Cfg {
   static constexpr int DC = D / 64;
+  static constexpr int CTAS = NT == 1 ? 2 : 1;        // per SM
   static constexpr int Q_BYTES = BQ * D * 2;
   static constexpr int KV_BYTES = BKV * D * 2;
-  static constexpr uint32_t COL_S = 0, COL_O = NT * BKV;
-  // P_t has columns of its own where they fit, so that S_t(j + 1) is computed
-  // while the softmax of tile j runs; otherwise it goes over S_t.
-  static constexpr bool SEP_P = COL_O + NT * D + NT * (BKV / 2) <= TMEM_COLS;
-  static constexpr uint32_t COL_P = SEP_P ? COL_O + NT * D : COL_S;
-  static constexpr uint32_t P_STRIDE = SEP_P ? BKV / 2 : BKV;
-  // Floats that the two threads of a row exchange.  Without SEP_P one buffer
-  // serves: S_t(j + 1) complete means that all have read those of tile j.
-  static constexpr int TURNS = SEP_P ? 2 : 1;
-  static constexpr int REST = 384 + TURNS * NT * 2 * BQ * 4;
+  static constexpr int REST = 512;                    // barriers
   // K and V tiles in rings of their own, each released when its product has
   // read it.
-  static constexpr int FIT = (227 * 1024 - REST - NT * Q_BYTES) / KV_BYTES;
-  static constexpr int BUFS = FIT < 12 ? FIT : 12;
+  static constexpr int FIT = ((227 * 1024 - (CTAS - 1) * 1024) / CTAS - REST - NT * Q_BYTES) / KV_BYTES;
+  static constexpr int BUFS = FIT < 16 ? FIT : 16;
   static constexpr int KST = BUFS / 2, VST = BUFS - KST;
   static constexpr int SMEM = NT * Q_BYTES + BUFS * KV_BYTES + REST;
-  static constexpr int NMMA = SEP_P ? NT : 1;
-  static constexpr int THREADS = (4 + 8 * NT) * 32;    // TMA and MMA warps, softmax warps
+  static constexpr uint32_t COL_S = 0, COL_O = NT * 2 * BKV;
+  static constexpr uint32_t TMEM_COLS = COL_O + NT * D <= 256 ? 256 : 512;
+  static constexpr int THREADS = (4 + 4 * NT) * 32;   // TMA and MMA warps, softmax warps
   static constexpr int POLY = D == 64 ? POLY64 : POLY128;  // of 8 pairs of P, those of ex2_poly2
-  static_assert(COL_O + NT * D <= TMEM_COLS, "TMEM budget");
-  static_assert((2 * BUFS + 4 * NT + NMMA) * 8 + 16 <= 384, "barrier area");
+  static_assert(COL_O + NT * D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
+  static_assert((2 * BUFS + 6 * NT) * 8 + 16 <= REST, "barrier area");
 };
 
 struct View {        // a K or V map: heads listed before rows; 0 for a broadcast dimension
@@ -146,7 +142,7 @@ constexpr uint32_t idesc_of(int m, int n) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
+__global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     prefix_kernel(const __grid_constant__ CUtensorMap map_pk,
                   const __grid_constant__ CUtensorMap map_pv,
                   const __grid_constant__ CUtensorMap map_k,
@@ -168,14 +164,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   uint64_t* k_empty = k_full + C::KST;               // [KST]
   uint64_t* v_full = k_empty + C::KST;               // [VST]
   uint64_t* v_empty = v_full + C::VST;               // [VST]
-  uint64_t* s_full = v_empty + C::VST;               // [NT]
-  uint64_t* p_full = s_full + NT;                    // [NT]
-  uint64_t* pv_done = p_full + NT;                   // [NT] (SEP_P: every P V; else the last)
-  uint64_t* s_free = pv_done + NT;                   // [NT] (SEP_P only)
-  uint64_t* mma_drain = s_free + NT;                 // [NMMA] abort teardown only
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + C::NMMA);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + C::NMMA + 1);
-  float* xch = reinterpret_cast<float*>(bars + 48);  // [TURNS][NT][2][BQ]
+  uint64_t* s_full = v_empty + C::VST;               // [NT][2] (by S buffer)
+  uint64_t* p_full = s_full + 2 * NT;                // [NT][2]
+  uint64_t* pv_done = p_full + 2 * NT;               // [NT]
+  uint64_t* mma_drain = pv_done + NT;                // [NT] abort teardown only
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + NT);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + NT + 1);
 
   // (The shuffle tells the compiler that the role is the same in all lanes.)
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -221,7 +215,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     slot = (p.joint ? 0 : p.slots_p) + part;
   }
   const int ntv = min((fend - f0 + BQ - 1) / BQ, NT);  // row tiles that hold rows
-  const int nmma = C::SEP_P ? ntv : 1;
   // Key tile j of K or V into its ring (thread 0).
   int loaded_k = 0, loaded_v = 0;
   auto load = [&](uint8_t* dst, uint64_t* bar, int j, const CUtensorMap* mp, const CUtensorMap* mo,
@@ -246,19 +239,20 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::KST; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], nmma);
+      mbar_init(&k_empty[s], ntv);  // one commit per MMA warp with rows
     }
     for (int s = 0; s < C::VST; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], nmma);
+      mbar_init(&v_empty[s], ntv);
+    }
+    for (int i = 0; i < 2 * NT; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
     }
     for (int t = 0; t < NT; ++t) {
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 8);
-      mbar_init(&s_free[t], 8);
       mbar_init(&pv_done[t], 1);
+      mbar_init(&mma_drain[t], 1);
     }
-    for (int w = 0; w < C::NMMA; ++w) mbar_init(&mma_drain[w], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int j = 0; j < nkv && j < C::VST; ++j) {
@@ -269,28 +263,25 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(tmem_slot)),
-                 "r"(TMEM_COLS));
+                 "r"(C::TMEM_COLS));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
-  // The softmax threads' row (tile st, TMEM lane quarter warp % 4): two threads
-  // per row, `half` of its scores, of its output and of Q each.
-  const int sw = warp - 4, st = sw >> 3, half = (sw >> 2) & 1;
+  // The softmax threads' row: row tile st, TMEM lane quarter warp % 4.
+  const int st = (warp - 4) >> 2;
   const int r = (warp & 3) * 32 + lane;
   const int f = f0 + st * BQ + r;                // flattened row
   const bool valid = f < fend;
-  if (sw >= 0 && st < ntv) {
+  if (warp >= 4 && st < ntv) {
     const Row w = row_at(p, valid ? f : fend - 1);
     const T* qr = static_cast<const T*>(p.q) + w.b * p.qb + int64_t(h * p.G + w.g) * p.qh + w.i * p.qn;
     uint8_t* qt = sq + st * C::Q_BYTES + r * 128;
-    uint4 u[D / 16];
+    uint4 u[D / 8];
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-      u[c] = valid ? __ldg(reinterpret_cast<const uint4*>(qr) + half * (D / 16) + c) : make_uint4(0, 0, 0, 0);
+    for (int c = 0; c < D / 8; ++c)
+      u[c] = valid ? __ldg(reinterpret_cast<const uint4*>(qr) + c) : make_uint4(0, 0, 0, 0);
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      const int c = half * (D / 16) + i;
-      *reinterpret_cast<uint4*>(qt + (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4)) = u[i];
-    }
+    for (int c = 0; c < D / 8; ++c)
+      *reinterpret_cast<uint4*>(qt + (c >> 3) * (BQ * 128) + (((c & 7) ^ (r & 7)) << 4)) = u[c];
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
   tc_fence_before();
@@ -321,72 +312,58 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
         }
       }
     }
-  } else if (warp <= C::NMMA) {
+  } else if (warp <= ntv) {
     // ------------------------------------------------------------------ MMA
-    constexpr int TPW = NT / C::NMMA;
-    const int t0 = (warp - 1) * TPW;
-    const int t1 = min(t0 + TPW, ntv);  // this warp's row tiles: t0 .. t1 - 1
-    // The whole warp keeps step and one elected lane issues, so that loop state
-    // and descriptors stay in uniform registers.
+    // One warp per row tile.  The whole warp keeps step and one elected lane
+    // issues, so that loop state and descriptors stay in uniform registers
+    // (issuing from a divergent branch took 27% longer per key tile).
+    const int t = warp - 1;
     const bool leader = elect_one();
     auto commit = [&](uint64_t* bar) {
       if (leader) umma_commit(bar);
     };
-    if (t0 < t1 && nkv > 0) {
-      auto issue_s = [&](int t, int j) {
-        const uint8_t* kt = sk + (j % C::KST) * C::KV_BYTES;
-        const uint8_t* qt = sq + t * C::Q_BYTES;
-        const uint64_t da0 = smem_desc_sw128(qt), db0 = smem_desc_sw128(kt);
-        if (leader) {
+    const uint32_t t_s = tmem_base + C::COL_S + t * (2 * BKV), t_o = tmem_base + C::COL_O + t * D;
+    auto issue_s = [&](int j) {
+      const uint64_t da = smem_desc_sw128(sq + t * C::Q_BYTES);
+      const uint64_t db = smem_desc_sw128(sk + (j % C::KST) * C::KV_BYTES);
+      if (leader) {
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t off = uint64_t((k >> 2) * (BQ * 128 >> 4) + 2 * (k & 3));
-            umma_f16<IDESC_S>(tmem_base + C::COL_S + t * BKV, da0 + off, db0 + off, k ? 1u : 0u);
-          }
-        }
-        commit(&s_full[t]);
-        if (t == t1 - 1) commit(&k_empty[j % C::KST]);
-      };
-      auto issue_pv = [&](int t, int j) {
-        const uint64_t db = smem_desc_sw128_mn(sv + (j % C::VST) * C::KV_BYTES, BKV * 128);
-        const uint32_t ta = tmem_base + C::COL_P + t * C::P_STRIDE;
-        if (leader) {
-#pragma unroll
-          for (int ks = 0; ks < BKV / 16; ++ks)
-            umma_f16_ts<IDESC_O>(tmem_base + C::COL_O + t * D, ta + uint32_t(ks * 8),
-                                 db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
-        }
-        if (t == t1 - 1) commit(&v_empty[j % C::VST]);
-        if (C::SEP_P || j + 1 == nkv) commit(&pv_done[t]);  // the last one: the block waits for it
-      };
-      auto wait_k = [&](int j) { return wait_warp(&k_full[j % C::KST], (j / C::KST) & 1); };
-      bool ok = wait_k(0);
-      if (ok) {
-        tc_fence_after();
-        for (int t = t0; t < t1; ++t) issue_s(t, 0);
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16<IDESC_S>(t_s + (j & 1) * BKV, da + uint64_t((k >> 2) * (BQ * 128 >> 4) + 2 * (k & 3)),
+                            db + uint64_t((k >> 2) * (BKV * 128 >> 4) + 2 * (k & 3)), k ? 1u : 0u);
       }
-      for (int j = 0; ok && j < nkv; ++j) {
-        const bool more = j + 1 < nkv;
-        for (int t = t0; ok && t < t1; ++t) {
-          // SEP_P: S_t(j+1) once the softmax warps have copied S_t(j), then
-          // P_t(j) V.  Else P_t(j) V, then S_t(j+1) over the consumed P_t(j).
-          if (C::SEP_P && more) {
-            ok = (t > t0 || wait_k(j + 1)) && wait_warp(&s_free[t], j & 1);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t, j + 1);
-          }
-          ok = wait_warp(&p_full[t], j & 1) && (t > t0 || wait_warp(&v_full[j % C::VST], (j / C::VST) & 1));
-          if (!ok) break;
-          tc_fence_after();
-          issue_pv(t, j);
-          if (!C::SEP_P && more) {
-            ok = t > t0 || wait_k(j + 1);
-            if (!ok) break;
-            tc_fence_after();
-            issue_s(t, j + 1);
-          }
-        }
+      commit(&s_full[2 * t + (j & 1)]);
+      commit(&k_empty[j % C::KST]);
+    };
+    auto issue_pv = [&](int j) {
+      const uint64_t db = smem_desc_sw128_mn(sv + (j % C::VST) * C::KV_BYTES, BKV * 128);
+      if (leader) {
+#pragma unroll
+        for (int ks = 0; ks < BKV / 16; ++ks)
+          umma_f16_ts<IDESC_O>(t_o, t_s + (j & 1) * BKV + uint32_t(ks * 8),
+                               db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
+      }
+      commit(&v_empty[j % C::VST]);
+      commit(&pv_done[t]);  // the last commit of an item: the block waits for it
+    };
+    bool ok = true;
+    for (int j = 0; ok && j < 2 && j < nkv; ++j) {
+      ok = wait_warp(&k_full[j % C::KST], (j / C::KST) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      issue_s(j);
+    }
+    for (int j = 0; ok && j < nkv; ++j) {
+      ok = wait_warp(&p_full[2 * t + (j & 1)], (j >> 1) & 1) &&
+           wait_warp(&v_full[j % C::VST], (j / C::VST) & 1);
+      if (!ok) break;
+      tc_fence_after();
+      issue_pv(j);
+      if (j + 2 < nkv) {
+        ok = wait_warp(&k_full[(j + 2) % C::KST], ((j + 2) / C::KST) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        issue_s(j + 2);  // over P(j), which the product before it has read
       }
     }
   } else if (warp >= 4 && st < ntv) {
@@ -396,119 +373,73 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
     // Own keys that this row sees.
     const int lim = p.causal ? min(len, len - p.N + row_at(p, valid ? f : fend - 1).i + 1) : len;
     const uint32_t lane_off = uint32_t(quarter * 32) << 16;
-    const uint32_t t_s = tmem_base + C::COL_S + t * BKV + half * (BKV / 2) + lane_off;
-    const uint32_t t_o = tmem_base + C::COL_O + t * D + half * (D / 2) + lane_off;
-    const uint32_t t_p = tmem_base + C::COL_P + t * C::P_STRIDE + half * (BKV / 4) + lane_off;
+    const uint32_t t_s = tmem_base + C::COL_S + t * (2 * BKV) + lane_off;
+    const uint32_t t_o = tmem_base + C::COL_O + t * D + lane_off;
     const float2 sc2 = f2(p.scale_log2);
-    float m = -INFINITY;                         // running max, log2 units (both threads')
-    float2 l2 = f2(0.f);                         // running sum of this half (two parts)
+    float m = -INFINITY;                         // running max, log2 units
+    float2 l2 = f2(0.f);                         // running row sum (two parts)
     bool ok = true;
-    // A warp whose wait has run out goes on to the next exchange, where the
-    // pair of warps that share rows leaves together.
-    auto wait_all = [&](uint64_t* bar, uint32_t parity) {
-      if (ok) ok = wait_warp(bar, parity);
-      return ok;
-    };
-    // The other half's value; false once either warp has failed.
-    int turn = 0;
-    auto exchange = [&](float mine, float& other) {
-      float* x = xch + ((turn * NT + t) * 2) * BQ + r;
-      turn = (turn + 1) % C::TURNS;
-      x[half * BQ] = mine;
-      uint32_t both;
-      asm volatile(
-          "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
-          "bar.red.and.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
-          : "=r"(both)
-          : "r"(uint32_t(ok)), "r"(1 + t * 4 + quarter)
-          : "memory");
-      other = x[(half ^ 1) * BQ];
-      return both != 0;
-    };
     for (int j = 0; j < nkv; ++j) {
-      if (wait_all(&s_full[t], j & 1)) tc_fence_after();
+      ok = wait_warp(&s_full[2 * t + (j & 1)], (j >> 1) & 1);
+      if (!ok) break;
+      tc_fence_after();
       const bool pre = j < np;
       const int key0 = (pre ? pa + j : sa + j - np) * BKV;
       // V rows past the element's keys may hold anything: zero them, once the
-      // tile has landed.
+      // tile has landed (two threads per row).
       const int held = pre ? BKV : min(len - key0, BKV);
       if (held < BKV) {
-        if (wait_all(&v_full[j % C::VST], (j / C::VST) & 1) && r >= held) {
-          uint8_t* vr = sv + (j % C::VST) * C::KV_BYTES + r * 128;
+        ok = wait_warp(&v_full[j % C::VST], (j / C::VST) & 1);
+        if (!ok) break;
+        const int vrow = r & (BKV - 1);
+        if (vrow >= held) {
+          uint8_t* vr = sv + (j % C::VST) * C::KV_BYTES + vrow * 128;
 #pragma unroll
           for (int i = 0; i < D / 16; ++i) {
-            const int c = half * (D / 16) + i;
+            const int c = (r / BKV) * (D / 16) + i;
             *reinterpret_cast<uint4*>(vr + (c >> 3) * (BKV * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
       }
-      bool pv_waited = !C::SEP_P || j == 0;
-      auto wait_pv = [&]() {  // P_t(j-1) V has read P_t and O_t is stable
-        if (!pv_waited) {
-          pv_waited = true;
-          if (wait_all(&pv_done[t], (j - 1) & 1)) tc_fence_after();
-        }
-      };
-      if (!active) {  // no rows (in either half): keep the other warps' pace
-        if (!ok) break;
-        if constexpr (C::SEP_P) {
-          if (lane == 0) mbar_arrive(&s_free[t]);
-        }
-        wait_pv();
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(&p_full[t]);
+      if (!active) {  // no rows: keep the other warps' pace
+        if (lane == 0) mbar_arrive(&p_full[2 * t + (j & 1)]);
         continue;
       }
-      float s[BKV / 2];
-      float mx = -INFINITY;
-      if (ok) {
-        tmem_ld64(t_s, s);
-        if constexpr (C::SEP_P) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&s_free[t]);
-        }
-        // Keys of this half of the tile that the row sees.
-        const int kvalid = (pre ? p.P : lim) - key0 - half * (BKV / 2);
-        if (kvalid < BKV / 2) {
+      const uint32_t t_sj = t_s + (j & 1) * BKV;
+      float s[BKV];
+      tmem_ld64(t_sj, s);
+      const int kvalid = (pre ? p.P : lim) - key0;  // keys of this tile that the row sees
+      if (kvalid < BKV) {
 #pragma unroll
-          for (int e = 0; e < BKV / 2; ++e)
-            if (e >= kvalid) s[e] = -INFINITY;
-        }
-        __syncwarp();
-        float mx0 = s[0], mx1 = s[1];
-#pragma unroll
-        for (int e = 2; e < BKV / 2; e += 2) {
-          mx0 = fmaxf(mx0, s[e]);
-          mx1 = fmaxf(mx1, s[e + 1]);
-        }
-        mx = fmaxf(mx0, mx1);
+        for (int e = 0; e < BKV; ++e)
+          if (e >= kvalid) s[e] = -INFINITY;
       }
-      float other;
-      // (Past the exchange both halves have copied S_t: P_t may go over it.)
-      if (!exchange(mx, other)) { ok = false; break; }
-      const float mxs = fmaxf(mx, other) * p.scale_log2;  // scale > 0
+      __syncwarp();
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int e = 4; e < BKV; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
+      const float mxs = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;  // scale > 0
       const bool grow = mxs > m + RESCALE_LOG2;           // always on the first key a row sees
       const float m_new = grow ? mxs : m;
       const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        wait_pv();
-        if (ok) {
+        ok = wait_warp(&pv_done[t], (j - 1) & 1);         // O_t is stable
+        if (!ok) break;
+        tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 16) {  // (s is live: few columns at a time)
-            float o[16];
-            tmem_ld16(t_o + uint32_t(c), o);
-            uint32_t u[16];
+        for (int c = 0; c < D; c += 16) {  // (s is live: few columns at a time)
+          float o[16];
+          tmem_ld16(t_o + uint32_t(c), o);
+          uint32_t u[16];
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
-              u[e] = __float_as_uint(v.x);
-              u[e + 1] = __float_as_uint(v.y);
-            }
-            tmem_st16u(t_o + uint32_t(c), u);
+          for (int e = 0; e < 16; e += 2) {
+            const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
+            u[e] = __float_as_uint(v.x);
+            u[e + 1] = __float_as_uint(v.y);
           }
+          tmem_st16u(t_o + uint32_t(c), u);
         }
       }
       // P = exp2(s * scale * log2 e - m); a row that has seen no key yet has
@@ -516,9 +447,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
       const float2 nm2 = f2(m_new == -INFINITY ? 0.f : -m_new);
       l2 = mul2(l2, f2(alpha));
       // In pieces of 32 scores, stored to TMEM as they are formed.
-      wait_pv();
 #pragma unroll
-      for (int c = 0; c < BKV / 2; c += 32) {
+      for (int c = 0; c < BKV; c += 32) {
         uint32_t u[16];
 #pragma unroll
         for (int e = 0; e < 32; e += 2) {
@@ -528,60 +458,55 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
           l2 = add2(l2, pr);
           u[e >> 1] = pack_pair<T>(pr.x, pr.y);
         }
-        if (ok) tmem_st16u(t_p + uint32_t(c / 2), u);
+        tmem_st16u(t_sj + uint32_t(c / 2), u);
       }
       m = m_new;
-      if (ok) {
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
-      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&p_full[2 * t + (j & 1)]);
     }
     // Epilogue, after the last P V: the output, or this part's O / l and log2 sum.
-    if (active) {
-      if (nkv > 0 && wait_all(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0)) tc_fence_after();
+    // (One phase after the other: S(nkv - 1) complete says only that the product
+    // two tiles before the last is done, and a wait must not be two phases ahead.)
+    for (int j = max(nkv - 2, 0); ok && j < nkv; ++j) ok = wait_warp(&pv_done[t], j & 1);
+    tc_fence_after();
+    if (ok && active) {
       // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)
-      const float own = l2.x + l2.y;
-      float other;
-      // ok is the pair's here or, where the loop was left, false in both.
-      if (exchange(own, other)) {
-        float l = own + other;
-        if (m == -INFINITY && l == l) l = 0.f;
-        const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
-        const int64_t pr = (int64_t(slot) * p.Hkv + h) * p.F + f;
-        if (p.slots > 1 && valid && half == 0)
-          p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
-        const Row w = row_at(p, valid ? f : fend - 1);
-        T* orow = static_cast<T*>(p.out) + w.b * p.ob + int64_t(h * p.G + w.g) * p.oh + w.i * p.on + half * (D / 2);
+      float l = l2.x + l2.y;
+      if (m == -INFINITY && l == l) l = 0.f;
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
+      const int64_t pr = (int64_t(slot) * p.Hkv + h) * p.F + f;
+      if (p.slots > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
+      const Row w = row_at(p, valid ? f : fend - 1);
+      T* orow = static_cast<T*>(p.out) + w.b * p.ob + int64_t(h * p.G + w.g) * p.oh + w.i * p.on;
 #pragma unroll 1
-        for (int c = 0; c < D / 2; c += 32) {
-          float o[32];
-          if (nkv > 0) {
-            tmem_ld32(t_o + uint32_t(c), o);
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (nkv > 0) {
+          tmem_ld32(t_o + uint32_t(c), o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
+          if (p.slots > 1) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
           } else {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0.f;
-          }
-          if (valid) {
+            for (int q = 0; q < 4; ++q) {
+              float v[8];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] *= inv;
-            if (p.slots > 1) {
-              float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + half * (D / 2) + c);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            } else {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w[e] = o[8 * q + e];
-                *reinterpret_cast<uint4*>(orow + c + 8 * q) = pack(w, T());
-              }
+              for (int e = 0; e < 8; ++e) v[e] = o[8 * q + e];
+              *reinterpret_cast<uint4*>(orow + c + 8 * q) = pack(v, T());
             }
           }
-          __syncwarp();
         }
+        __syncwarp();
       }
     }
   }
@@ -591,7 +516,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   tc_fence_before();
   __syncthreads();
   if (*abort_flag) {
-    if (warp >= 1 && warp <= C::NMMA && elect_one()) {  // the lane that issued
+    if (warp >= 1 && warp <= NT && elect_one()) {  // the lane that issued
       umma_commit(&mma_drain[warp - 1]);
       mbar_drain(&mma_drain[warp - 1], 0, p.wait_ns);
     }
@@ -607,7 +532,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, 1)
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
-                 "r"(TMEM_COLS));
+                 "r"(C::TMEM_COLS));
   }
 }
 
@@ -692,8 +617,8 @@ static Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t P, 
   const int64_t joint = Hkv * B * pl.tiles_o * (kp + ko);
   pl.joint = S > 0 && joint * 10 <= packed * 11;
   const int64_t work = pl.joint ? joint : packed;
-  int64_t chunk = up(work, sm_count());
-  if (chunk < 2) chunk = 2;
+  int64_t chunk = up(work, int64_t(sm_count()) * (pl.nt == 1 ? 2 : 1));
+  if (chunk < 4) chunk = 4;
   const int64_t kmax = pl.joint ? kp + ko : kp > ko ? kp : ko;
   const int64_t half = MAX_SLOTS / 2;
   if (chunk * half < kmax) chunk = up(kmax, half);
