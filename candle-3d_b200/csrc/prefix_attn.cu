@@ -54,7 +54,7 @@ __device__ int g_pattn_status;
 #define POLY64 2
 #endif
 #ifndef POLY128
-#define POLY128 0
+#define POLY128 1
 #endif
 // NT row tiles of 128 rows per block; NT = 1 blocks share an SM in pairs, for
 // short items, whose set-up one block's work then hides for the other.
@@ -76,7 +76,7 @@ struct Cfg {
   static constexpr int THREADS = (4 + 4 * NT) * 32;   // TMA and MMA warps, softmax warps
   static constexpr int POLY = D == 64 ? POLY64 : POLY128;  // of 8 pairs of P, those of ex2_poly2
   static_assert(COL_O + NT * D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
-  static_assert((2 * BUFS + 6 * NT) * 8 + 16 <= REST, "barrier area");
+  static_assert((2 * BUFS + 7 * NT) * 8 + 16 <= REST, "barrier area");
 };
 
 struct View {        // a K or V map: heads listed before rows; 0 for a broadcast dimension
@@ -166,8 +166,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   uint64_t* v_empty = v_full + C::VST;               // [VST]
   uint64_t* s_full = v_empty + C::VST;               // [NT][2] (by S buffer)
   uint64_t* p_full = s_full + 2 * NT;                // [NT][2]
-  uint64_t* pv_done = p_full + 2 * NT;               // [NT]
-  uint64_t* mma_drain = pv_done + NT;                // [NT] abort teardown only
+  uint64_t* pv_done = p_full + 2 * NT;               // [NT][2]
+  uint64_t* mma_drain = pv_done + 2 * NT;            // [NT] abort teardown only
   volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + NT);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + NT + 1);
 
@@ -248,11 +248,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     for (int i = 0; i < 2 * NT; ++i) {
       mbar_init(&s_full[i], 1);
       mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
     }
-    for (int t = 0; t < NT; ++t) {
-      mbar_init(&pv_done[t], 1);
-      mbar_init(&mma_drain[t], 1);
-    }
+    for (int t = 0; t < NT; ++t) mbar_init(&mma_drain[t], 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     for (int j = 0; j < nkv && j < C::VST; ++j) {
@@ -344,7 +342,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
                                db + uint64_t(ks * (16 * 128 >> 4)), (j | ks) ? 1u : 0u);
       }
       commit(&v_empty[j % C::VST]);
-      commit(&pv_done[t]);  // the last commit of an item: the block waits for it
+      commit(&pv_done[2 * t + (j & 1)]);  // the last commit of an item: the block waits for it
     };
     bool ok = true;
     for (int j = 0; ok && j < 2 && j < nkv; ++j) {
@@ -425,7 +423,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       const float m_new = grow ? mxs : m;
       const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
-        ok = wait_warp(&pv_done[t], (j - 1) & 1);         // O_t is stable
+        ok = wait_warp(&pv_done[2 * t + ((j - 1) & 1)], ((j - 1) >> 1) & 1);  // O_t is stable
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -446,7 +444,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       // m = -inf and all its scores masked: subtract 0, so that P = 0.
       const float2 nm2 = f2(m_new == -INFINITY ? 0.f : -m_new);
       l2 = mul2(l2, f2(alpha));
-      // In pieces of 32 scores, stored to TMEM as they are formed.
+      // In pieces of 32 scores, stored to TMEM as they are formed (one store of
+      // all 64 measured 7% slower over short key ranges).
 #pragma unroll
       for (int c = 0; c < BKV; c += 32) {
         uint32_t u[16];
@@ -467,9 +466,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       if (lane == 0) mbar_arrive(&p_full[2 * t + (j & 1)]);
     }
     // Epilogue, after the last P V: the output, or this part's O / l and log2 sum.
-    // (One phase after the other: S(nkv - 1) complete says only that the product
-    // two tiles before the last is done, and a wait must not be two phases ahead.)
-    for (int j = max(nkv - 2, 0); ok && j < nkv; ++j) ok = wait_warp(&pv_done[t], j & 1);
+    // (A barrier per S buffer: of one barrier for all products, two phases could
+    // pass before this thread looks.  S(j) complete says that P(j - 2) V is done.)
+    if (ok && nkv > 0) ok = wait_warp(&pv_done[2 * t + ((nkv - 1) & 1)], ((nkv - 1) >> 1) & 1);
     tc_fence_after();
     if (ok && active) {
       // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)
@@ -536,20 +535,22 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   }
 }
 
-// The parts of each row weighed by 2^(their log2 sum - the largest): one warp
-// per row, D / 32 elements per lane.
+// The parts of each row weighed by 2^(their log2 sum - the largest): a block of
+// four warps per row, each with every fourth part, D / 32 elements per lane;
+// added up in a fixed order.
 constexpr int MAX_SLOTS = 64;
 template <typename T, int D>
-__global__ void __launch_bounds__(256) combine_kernel(const Params p) {
-  constexpr int E = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);  // h F + f
+__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+  constexpr int E = D / 32, W = 4, PER = MAX_SLOTS / W;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  __shared__ Vec red[W - 1][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;  // h F + f
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (row >= int64_t(p.Hkv) * p.F) return;
   const int64_t stride = int64_t(p.Hkv) * p.F;
-  float w[MAX_SLOTS / 32], mx = -INFINITY;
+  float w[2], mx = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
+  for (int i = 0; i < 2; ++i) {
     const int s = lane + 32 * i;
     w[i] = s < p.slots ? p.part_l[s * stride + row] : -INFINITY;
     mx = fmaxf(mx, w[i]);
@@ -558,42 +559,47 @@ __global__ void __launch_bounds__(256) combine_kernel(const Params p) {
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float sum = 0.f;
 #pragma unroll
-  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
+  for (int i = 0; i < 2; ++i) {
     w[i] = w[i] == -INFINITY ? 0.f : exp2f(w[i] - mx);
     sum += w[i];
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-  float acc[E];
+  alignas(16) float acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  const Vec* src = reinterpret_cast<const Vec*>(p.part_o + row * D) + lane;
 #pragma unroll
-  for (int i = 0; i < MAX_SLOTS / 32; ++i) {
-    const int n = min(p.slots - 32 * i, 32);
-#pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float ws = __shfl_sync(0xffffffffu, w[i], s);
-      if (ws == 0.f) continue;  // a part without keys
-      const float* src = p.part_o + ((32 * i + s) * stride + row) * D + lane * E;
-      if constexpr (E == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] = fmaf(ws, v.x, acc[0]);
-        acc[1] = fmaf(ws, v.y, acc[1]);
-        acc[2] = fmaf(ws, v.z, acc[2]);
-        acc[3] = fmaf(ws, v.w, acc[3]);
-      } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(ws, v.x, acc[0]);
-        acc[1] = fmaf(ws, v.y, acc[1]);
-      }
+  for (int i = 0; i < PER; ++i) {
+    const int s = i * W + warp;
+    if (s >= p.slots) break;
+    const float ws = __shfl_sync(0xffffffffu, i * W < 32 ? w[0] : w[1], s & 31);
+    if (ws == 0.f) continue;  // a part without keys: nothing is stored there
+    const Vec v = src[s * stride * (D / E)];
+    acc[0] = fmaf(ws, v.x, acc[0]);
+    acc[1] = fmaf(ws, v.y, acc[1]);
+    if constexpr (E == 4) {
+      acc[2] = fmaf(ws, v.z, acc[2]);
+      acc[3] = fmaf(ws, v.w, acc[3]);
     }
   }
+  if (warp > 0) red[warp - 1][lane] = *reinterpret_cast<const Vec*>(acc);
+  __syncthreads();
+  if (warp > 0) return;
   const float inv = sum != 0.f ? 1.f / sum : 0.f;
   const int h = int(row / p.F);
   const Row at = row_at(p, int(row % p.F));
   T* orow = static_cast<T*>(p.out) + at.b * p.ob + int64_t(h * p.G + at.g) * p.oh + at.i * p.on + lane * E;
+  alignas(8) T o[E];
 #pragma unroll
-  for (int e = 0; e < E; ++e) orow[e] = from_f<T>(acc[e] * inv);
+  for (int e = 0; e < E; ++e) {
+    float t = acc[e];
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) t += reinterpret_cast<const float*>(&red[i][lane])[e];
+    o[e] = from_f<T>(t * inv);
+  }
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(o);
+  else *reinterpret_cast<uint32_t*>(orow) = *reinterpret_cast<const uint32_t*>(o);
 }
 
 // How the rows and keys are divided into items (host).
@@ -618,7 +624,7 @@ static Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t P, 
   pl.joint = S > 0 && joint * 10 <= packed * 11;
   const int64_t work = pl.joint ? joint : packed;
   int64_t chunk = up(work, int64_t(sm_count()) * (pl.nt == 1 ? 2 : 1));
-  if (chunk < 4) chunk = 4;
+  if (chunk < 2) chunk = 2;
   const int64_t kmax = pl.joint ? kp + ko : kp > ko ? kp : ko;
   const int64_t half = MAX_SLOTS / 2;
   if (chunk * half < kmax) chunk = up(kmax, half);
@@ -647,8 +653,8 @@ static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int ite
   if (p.slots <= 1) return cudaGetLastError();
   // The combination may be scheduled while the items finish; it waits for them.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned((int64_t(p.Hkv) * p.F + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(unsigned(p.Hkv) * unsigned(p.F));
+  cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
