@@ -65,12 +65,23 @@ __device__ __forceinline__ void epi_post(const Params& p, int row, int col0, flo
                   : __ldg(reinterpret_cast<const float*>(rrow) + i);
       }
     }
+    if (p.gate && c + 8 <= p.N && (reinterpret_cast<uintptr_t>(p.gate) & 15) == 0) {
+      if (p.gate_dtype == L3D_F32) {
+        const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + c));
+        const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + c) + 1);
+        g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w; g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
+      } else {
+        unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.gate) + c)), g,
+               __nv_bfloat16());
+      }
+    } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int col = c + e < p.N ? c + e : p.N - 1;
       g[e] = !p.gate ? 1.f
              : p.gate_dtype == L3D_F32 ? __ldg(static_cast<const float*>(p.gate) + col)
                                        : __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[col]);
+    }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)

@@ -46,6 +46,7 @@ struct Params {
   const int32_t* ranks;   // [A] or null (= R)
   const void* ids;        // row m has id ids[m / per]
   int ids64, per;
+  int x_rows;             // rows of an x tile that are loaded
   const void* bias;
   int bias_dtype, bias_vec;
   const void* gate;
@@ -262,7 +263,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   int* total = list_end + 2 * BM;        // [2]
   int* wsum = total + 2;                 // [8] per-warp sums of the list builders
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  // (The shuffle tells the compiler that the role is the same in all lanes.)
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int num_n = (p.N + BN - 1) / BN;
   const int tiles = ((p.M + BM - 1) / BM) * num_n;
   const int kblocks = (p.K + BK - 1) / BK;
@@ -271,7 +273,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
       mbar_init(&tgo[s], 1);
-      mbar_init(&tfull[s], 4);
+      mbar_init(&tfull[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
@@ -303,12 +305,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       int it = 0;  // ring position
       bool ok = true;
       int nt = 0;
+      const uint32_t x_bytes = uint32_t(p.x_rows) * (BK * 2);
       for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++nt) {
         const int m0 = (tile / num_n) * BM, n0 = (tile % num_n) * BN;
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % NST;
           if (it >= NST && !wait(&empty[s], (it / NST - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(&full[s], A_BYTES + C::B_BYTES);
+          mbar_expect_tx(&full[s], x_bytes + C::B_BYTES);
           tma_load_2d(sa + s * A_BYTES, &map_x, &full[s], kb * BK, m0);
           tma_load_2d(sb + s * C::B_BYTES, &map_w, &full[s], kb * BK, n0);
         }
@@ -332,41 +335,53 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------------ MMA
-    if (lane == 0) {
-      int it = 0, nt = 0;
-      uint32_t tph = 0;  // parity of each stage's next tfull phase
-      bool ok = true;
-      for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++nt) {
-        const int acc = nt & 1;
-        if (nt >= 2 && !wait(&acc_empty[acc], (nt / 2 - 1) & 1)) break;
+    // The whole warp keeps step and one elected lane issues, so that loop state
+    // and descriptors stay in uniform registers.
+    const bool leader = elect_one();
+    auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    };
+    int it = 0, nt = 0;
+    uint32_t tph = 0;  // parity of each stage's next tfull phase
+    bool ok = true;
+    for (int tile = blockIdx.x; ok && tile < tiles; tile += gridDim.x, ++nt) {
+      const int acc = nt & 1;
+      if (nt >= 2 && !wait_warp(&acc_empty[acc], (nt / 2 - 1) & 1)) break;
+      tc_fence_after();
+      const uint32_t d = tmem_base + uint32_t(acc * BN);
+      for (int kb = 0; kb < kblocks; ++kb, ++it) {
+        const int s = it % NST;
+        if (!wait_warp(&full[s], (it / NST) & 1)) { ok = false; break; }
         tc_fence_after();
-        const uint32_t d = tmem_base + uint32_t(acc * BN);
-        for (int kb = 0; kb < kblocks; ++kb, ++it) {
-          const int s = it % NST;
-          if (!wait(&full[s], (it / NST) & 1)) { ok = false; break; }
-          tc_fence_after();
-          const uint64_t da = smem_desc_sw128(sa + s * A_BYTES), db = smem_desc_sw128(sb + s * C::B_BYTES);
+        const uint64_t da = smem_desc_sw128(sa + s * A_BYTES), db = smem_desc_sw128(sb + s * C::B_BYTES);
+        if (leader) {
 #pragma unroll
           for (int k = 0; k < BK / 16; ++k)
             umma_f16<IDESC>(d, da + uint64_t(2 * k), db + uint64_t(2 * k), (kb | k) ? 1u : 0u);
           umma_commit(&empty[s]);
         }
-        if (!ok || !wait(&list_full[acc], (nt >> 1) & 1)) break;
-        const int slots = total[acc];
-        mbar_arrive(&list_empty[acc]);
-        for (int q0 = 0; q0 < slots; q0 += PER_STAGE, ++it) {
-          const int s = it % NST, n = min(PER_STAGE, slots - q0);
-          if (!wait(&full[s], (it / NST) & 1) || !wait(&tfull[s], (tph >> s) & 1)) { ok = false; break; }
-          tph ^= 1u << s;
-          tc_fence_after();
-          for (int q = 0; q < n; ++q)
+      }
+      if (!ok || !wait_warp(&list_full[acc], (nt >> 1) & 1)) break;
+      const int slots = total[acc];
+      __syncwarp();
+      if (leader) mbar_arrive(&list_empty[acc]);
+      for (int q0 = 0; q0 < slots; q0 += PER_STAGE, ++it) {
+        const int s = it % NST, n = min(PER_STAGE, slots - q0);
+        ok = wait_warp(&full[s], (it / NST) & 1) && wait_warp(&tfull[s], (tph >> s) & 1);
+        if (!ok) break;
+        tph ^= 1u << s;
+        tc_fence_after();
+        if (leader) {
+          for (int q = 0; q < n; ++q) {
+            const uint64_t db = smem_desc_sw32(sb + s * C::B_BYTES + q * C::SLOT_B);
+#pragma unroll
             for (int part = 0; part < PARTS; ++part)
-              umma_f16<IDESC>(d, smem_desc_sw32(sa + s * A_BYTES + (q * PARTS + part) * SLOT_A),
-                              smem_desc_sw32(sb + s * C::B_BYTES + q * C::SLOT_B), 1u);
+              umma_f16<IDESC>(d, smem_desc_sw32(sa + s * A_BYTES + (q * PARTS + part) * SLOT_A), db, 1u);
+          }
           umma_commit(&empty[s]);
         }
-        if (ok) umma_commit(&acc_full[acc]);
       }
+      if (ok && leader) umma_commit(&acc_full[acc]);
     }
   } else if (warp < 6) {
     // -------------------------------------- adapter lists and t pieces
@@ -425,33 +440,66 @@ __global__ void __launch_bounds__(THREADS, 1)
         asm volatile("griddepcontrol.wait;" ::: "memory");  // shrink_kernel's t
         arrived = true;
       }
-      const __nv_bfloat16* trow = p.t + int64_t(m < p.M ? m : 0) * p.R;
+      // Stage s belongs to warp 2 + s % 4, which writes all rows of its t pieces
+      // (four per lane): four stages' loads of t are in flight at once, and a
+      // warp meets the phases of its stages' tgo in order.
+      int ad[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ad[i] = ids[lane + 32 * i];
+      const int m0 = (tile / num_n) * BM, rows = min(p.M - m0, BM);
       int d = 0, start = 0;
-      for (int q0 = 0; ok && q0 < all; q0 += PER_STAGE, ++it) {
+      for (int q0 = 0; q0 < all; q0 += PER_STAGE, ++it) {
         const int s = it % NST, cnt = min(PER_STAGE, all - q0);
-        ok = __all_sync(0xffffffffu, wait(&tgo[s], (tph >> s) & 1));
-        if (!ok) break;
+        const uint32_t ph = (tph >> s) & 1;
         tph ^= 1u << s;
-        for (int q = q0; q < q0 + cnt; ++q) {
-          while (q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
-          const bool mine = a >= 0 && list_id[lb * BM + d] == a;
-          for (int part = 0; part < PARTS; ++part) {
-            uint4 v0 = make_uint4(0, 0, 0, 0), v1 = v0;
-            if (mine) {
-              const uint4* src = reinterpret_cast<const uint4*>(trow + int64_t(part) * p.M * p.R + (q - start) * 16);
-              v0 = __ldcg(src);
-              v1 = __ldcg(src + 1);
+        if ((s & 3) != warp - 2) {
+          for (int q = q0; q < q0 + cnt; ++q)
+            while (q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
+          continue;
+        }
+        // The pieces of t, before the stage is free.
+        uint4 v[PER_STAGE][4][PARTS][2];
+#pragma unroll
+        for (int q = 0; q < PER_STAGE; ++q) {
+          if (q >= cnt) break;
+          while (q0 + q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
+          const int a_q = list_id[lb * BM + d], c_q = (q0 + q - start) * 16;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              v[q][i][part][0] = v[q][i][part][1] = make_uint4(0, 0, 0, 0);
+              if (ad[i] == a_q) {
+                const uint4* src = reinterpret_cast<const uint4*>(
+                    p.t + (int64_t(part) * p.M + m0 + lane + 32 * i) * p.R + c_q);
+                v[q][i][part][0] = __ldcg(src);
+                v[q][i][part][1] = __ldcg(src + 1);
+              }
             }
-            uint8_t* dst = sa + s * A_BYTES + ((q - q0) * PARTS + part) * SLOT_A + r * 32;
-            const int sw = ((r >> 2) & 1) << 4;
-            *reinterpret_cast<uint4*>(dst + sw) = v0;
-            *reinterpret_cast<uint4*>(dst + (16 ^ sw)) = v1;
+        }
+        if (ok) ok = __all_sync(0xffffffffu, wait(&tgo[s], ph)) != 0;
+        if (!ok) continue;
+#pragma unroll
+        for (int q = 0; q < PER_STAGE; ++q) {
+          if (q >= cnt) break;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int row = lane + 32 * i;
+            if (row >= rows) continue;  // (rows past M: their products are not stored)
+#pragma unroll
+            for (int part = 0; part < PARTS; ++part) {
+              uint8_t* dst = sa + s * A_BYTES + (q * PARTS + part) * SLOT_A + row * 32;
+              const int sw = ((row >> 2) & 1) << 4;
+              *reinterpret_cast<uint4*>(dst + sw) = v[q][i][part][0];
+              *reinterpret_cast<uint4*>(dst + (16 ^ sw)) = v[q][i][part][1];
+            }
           }
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&tfull[s]);
       }
+      // (ids is written again only after all four warps have met.)
     }
   } else {
     // ------------------------------------------------------------- epilogue
@@ -518,7 +566,7 @@ __global__ void __launch_bounds__(THREADS, 1)
   // and give TMA loads still in flight 1 ms to land.
   tc_fence_before();
   __syncthreads();
-  if (*abort_flag && threadIdx.x == 32) {
+  if (*abort_flag && warp == 1 && elect_one()) {  // the lane that issued
     umma_commit(drain);
     mbar_drain(drain, 0, p.wait_ns);
     const uint64_t t0 = globaltimer();
@@ -754,8 +802,11 @@ extern "C" int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight,
   p.act = act;
   p.t = static_cast<__nv_bfloat16*>(workspace);
   p.wait_ns = l3d::tc::WAIT_LIMIT_NS;
+  // Of a tile with fewer rows only those are loaded (in groups of 8, the
+  // swizzle's unit); the other rows' products are not stored.
+  p.x_rows = M < BM ? int((M + 7) / 8 * 8) : BM;
   CUtensorMap mx;
-  if (!make_map2(&mx, p.x, uint64_t(M), uint64_t(k), uint64_t(x_ld), BM))
+  if (!make_map2(&mx, p.x, uint64_t(M), uint64_t(k), uint64_t(x_ld), uint32_t(p.x_rows)))
     return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed for x", op);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   // Few rows: 16 per block, all warps along K, the group's adapters in
