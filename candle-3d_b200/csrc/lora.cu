@@ -93,9 +93,9 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
 // order).  A lane loads 8 consecutive k of a row at once and uses them as the
 // operands of two K-16 products: both operands permute k alike, so the sums
 // are the same and every load is 16 bytes.  blockIdx.y strides over the
-// distinct adapters of the group.
-template <int MT, int WR, int WN, int WK>
-__global__ void __launch_bounds__(256, 2) shrink_kernel(const Params p) {
+// distinct adapters of the group, blockIdx.z over their ranks.
+template <int MT, int WR, int WN, int WK, int UNROLL>
+__global__ void __launch_bounds__(256, UNROLL > 2 ? 1 : 2) shrink_kernel(const Params p) {
   constexpr int ROWS = 16 * MT * WR, NT = 4, RB = 32 * WN;
   static_assert(WR * WN * WK == 8, "eight warps");
   __shared__ float red[WK][ROWS][RB + 4];
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256, 2) shrink_kernel(const Params p) {
   for (int d = blockIdx.y; d < count; d += gridDim.y) {
     const int a = s_list[d];
     const int rank = slots_of(p, a) * 16;
-    for (int r0 = 0; r0 < rank; r0 += RB) {
+    for (int r0 = blockIdx.z * RB; r0 < rank; r0 += gridDim.z * RB) {
       const int rb = r0 + wn * 32;
       const int nt = min((rank - rb) / 8, NT);  // 8-rank tiles of this warp
       float c[MT][NT][4];
@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(256, 2) shrink_kernel(const Params p) {
           for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
       const __nv_bfloat16* ar = p.a + (int64_t(a) * p.R + rb + g) * p.K + 8 * t4;
       if (nt > 0) {
-#pragma unroll 2
+#pragma unroll UNROLL
         for (int kc = wk; kc < chunks; kc += WK) {
           const int k = kc * 32;
           const bool kok = k + 8 * t4 < p.K;
@@ -205,16 +205,22 @@ __global__ void __launch_bounds__(256, 2) shrink_kernel(const Params p) {
 constexpr int BM = 128, BK = 64;
 constexpr int A_BYTES = BM * BK * 2;
 constexpr int SLOT_A = BM * 32;          // a t piece: 128 rows of 32 bytes
-constexpr int PER_STAGE = A_BYTES / (PARTS * SLOT_A);  // slots of a stage
 constexpr int THREADS = 14 * 32;
 
 template <int BN>
 struct Cfg {
+  // Blocks of 64 along K per stage: two for the narrow tiles of few rows, which
+  // wait for memory (whole 256-byte pieces of a weight row, half the barriers).
+  static constexpr int KS = BN <= 64 ? 2 : 1;
+  static constexpr int A_STAGE = KS * A_BYTES;
   static constexpr int B_BYTES = BN * BK * 2;
+  static constexpr int B_STAGE = KS * B_BYTES;
   static constexpr int SLOT_B = BN * 32;
-  static constexpr int NST = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+  static constexpr int PER_STAGE = A_STAGE / (PARTS * SLOT_A);  // slots of a stage
+  static constexpr int NST = BN == 256 || BN == 64 ? 4 : BN == 128 ? 6 : 5;
   static constexpr int LISTS = 2 * (2 * BM + 1) * 4 + BM * 4 + 64;
-  static constexpr int SMEM = NST * (A_BYTES + B_BYTES) + 512 + LISTS;
+  static constexpr int STG = 8 * 32 * 17 * 4;  // per epilogue warp: 32 rows x 16 columns, padded
+  static constexpr int SMEM = NST * (A_STAGE + B_STAGE) + 512 + LISTS + STG;
   static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;  // a power of two
   static_assert(SMEM <= 227 * 1024, "shared memory budget");
   static_assert((4 * NST + 9) * 8 + 16 <= 512, "barrier area");
@@ -237,13 +243,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_b, const Params p) {
   using C = Cfg<BN>;
-  constexpr int NST = C::NST;
+  constexpr int NST = C::NST, PER_STAGE = C::PER_STAGE;
   constexpr uint32_t IDESC = make_idesc(BM, BN);
   int* const status = &g_lora_status;
   extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: 1024-byte aligned
   uint8_t* sa = smem;
-  uint8_t* sb = sa + NST * A_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sb + NST * C::B_BYTES);
+  uint8_t* sb = sa + NST * C::A_STAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sb + NST * C::B_STAGE);
   uint64_t* full = bars;                 // [NST] TMA landed
   uint64_t* empty = full + NST;          // [NST] MMA has read the stage
   uint64_t* tgo = empty + NST;           // [NST] the stage is free for t pieces
@@ -262,12 +268,13 @@ __global__ void __launch_bounds__(THREADS, 1)
   int* list_end = list_id + 2 * BM;      // [2][BM] slots up to and with this adapter
   int* total = list_end + 2 * BM;        // [2]
   int* wsum = total + 2;                 // [8] per-warp sums of the list builders
+  float* stg = reinterpret_cast<float*>(wsum + 8);  // [8][32][17] epilogue staging
 
   // (The shuffle tells the compiler that the role is the same in all lanes.)
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int num_n = (p.N + BN - 1) / BN;
   const int tiles = ((p.M + BM - 1) / BM) * num_n;
-  const int kblocks = (p.K + BK - 1) / BK;
+  const int kblocks = (p.K + C::KS * BK - 1) / (C::KS * BK);
   if (threadIdx.x == 0) {
     for (int s = 0; s < NST; ++s) {
       mbar_init(&full[s], 1);
@@ -311,9 +318,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int kb = 0; kb < kblocks; ++kb, ++it) {
           const int s = it % NST;
           if (it >= NST && !wait(&empty[s], (it / NST - 1) & 1)) { ok = false; break; }
-          mbar_expect_tx(&full[s], x_bytes + C::B_BYTES);
-          tma_load_2d(sa + s * A_BYTES, &map_x, &full[s], kb * BK, m0);
-          tma_load_2d(sb + s * C::B_BYTES, &map_w, &full[s], kb * BK, n0);
+          mbar_expect_tx(&full[s], C::KS * (x_bytes + C::B_BYTES));
+#pragma unroll
+          for (int i = 0; i < C::KS; ++i) {  // (blocks past K read as zero)
+            const int k = (kb * C::KS + i) * BK;
+            tma_load_2d(sb + s * C::B_STAGE + i * C::B_BYTES, &map_w, &full[s], k, n0);
+            tma_load_2d(sa + s * C::A_STAGE + i * A_BYTES, &map_x, &full[s], k, m0);
+          }
         }
         const int lb = nt & 1;
         if (!ok || !wait(&list_full[lb], (nt >> 1) & 1)) break;
@@ -326,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           mbar_expect_tx(&full[s], n * C::SLOT_B);
           for (int q = q0; q < q0 + n; ++q) {
             while (q >= list_end[lb * BM + d]) first = list_end[lb * BM + d++];
-            tma_load_3d(sb + s * C::B_BYTES + (q - q0) * C::SLOT_B, &map_b, &full[s], (q - first) * 16,
+            tma_load_3d(sb + s * C::B_STAGE + (q - q0) * C::SLOT_B, &map_b, &full[s], (q - first) * 16,
                         n0, list_id[lb * BM + d]);
           }
         }
@@ -353,11 +364,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         const int s = it % NST;
         if (!wait_warp(&full[s], (it / NST) & 1)) { ok = false; break; }
         tc_fence_after();
-        const uint64_t da = smem_desc_sw128(sa + s * A_BYTES), db = smem_desc_sw128(sb + s * C::B_BYTES);
+        const uint64_t da = smem_desc_sw128(sa + s * C::A_STAGE), db = smem_desc_sw128(sb + s * C::B_STAGE);
         if (leader) {
 #pragma unroll
-          for (int k = 0; k < BK / 16; ++k)
-            umma_f16<IDESC>(d, da + uint64_t(2 * k), db + uint64_t(2 * k), (kb | k) ? 1u : 0u);
+          for (int k = 0; k < C::KS * BK / 16; ++k)
+            umma_f16<IDESC>(d, da + uint64_t((k >> 2) * (A_BYTES >> 4) + 2 * (k & 3)),
+                            db + uint64_t((k >> 2) * (C::B_BYTES >> 4) + 2 * (k & 3)), (kb | k) ? 1u : 0u);
           umma_commit(&empty[s]);
         }
       }
@@ -373,10 +385,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_after();
         if (leader) {
           for (int q = 0; q < n; ++q) {
-            const uint64_t db = smem_desc_sw32(sb + s * C::B_BYTES + q * C::SLOT_B);
+            const uint64_t db = smem_desc_sw32(sb + s * C::B_STAGE + q * C::SLOT_B);
 #pragma unroll
             for (int part = 0; part < PARTS; ++part)
-              umma_f16<IDESC>(d, smem_desc_sw32(sa + s * A_BYTES + (q * PARTS + part) * SLOT_A), db, 1u);
+              umma_f16<IDESC>(d, smem_desc_sw32(sa + s * C::A_STAGE + (q * PARTS + part) * SLOT_A), db, 1u);
           }
           umma_commit(&empty[s]);
         }
@@ -457,44 +469,32 @@ __global__ void __launch_bounds__(THREADS, 1)
             while (q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
           continue;
         }
-        // The pieces of t, before the stage is free.
-        uint4 v[PER_STAGE][4][PARTS][2];
-#pragma unroll
-        for (int q = 0; q < PER_STAGE; ++q) {
-          if (q >= cnt) break;
-          while (q0 + q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
-          const int a_q = list_id[lb * BM + d], c_q = (q0 + q - start) * 16;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int part = 0; part < PARTS; ++part) {
-              v[q][i][part][0] = v[q][i][part][1] = make_uint4(0, 0, 0, 0);
-              if (ad[i] == a_q) {
-                const uint4* src = reinterpret_cast<const uint4*>(
-                    p.t + (int64_t(part) * p.M + m0 + lane + 32 * i) * p.R + c_q);
-                v[q][i][part][0] = __ldcg(src);
-                v[q][i][part][1] = __ldcg(src + 1);
-              }
-            }
-        }
         if (ok) ok = __all_sync(0xffffffffu, wait(&tgo[s], ph)) != 0;
         if (!ok) continue;
-#pragma unroll
-        for (int q = 0; q < PER_STAGE; ++q) {
-          if (q >= cnt) break;
+        for (int q = 0; q < cnt; ++q) {
+          while (q0 + q >= list_end[lb * BM + d]) start = list_end[lb * BM + d++];
+          const int a_q = list_id[lb * BM + d], c_q = (q0 + q - start) * 16;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int row = lane + 32 * i;
             if (row >= rows) continue;  // (rows past M: their products are not stored)
+            const int sw = ((row >> 2) & 1) << 4;
 #pragma unroll
             for (int part = 0; part < PARTS; ++part) {
-              uint8_t* dst = sa + s * A_BYTES + (q * PARTS + part) * SLOT_A + row * 32;
-              const int sw = ((row >> 2) & 1) << 4;
-              *reinterpret_cast<uint4*>(dst + sw) = v[q][i][part][0];
-              *reinterpret_cast<uint4*>(dst + (16 ^ sw)) = v[q][i][part][1];
+              uint8_t* dst = sa + s * C::A_STAGE + (q * PARTS + part) * SLOT_A + row * 32;
+              if (ad[i] == a_q) {
+                const __nv_bfloat16* src = p.t + (int64_t(part) * p.M + m0 + row) * p.R + c_q;
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + sw)), "l"(src) : "memory");
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + (16 ^ sw))), "l"(src + 8)
+                             : "memory");
+              } else {
+                *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+                *reinterpret_cast<uint4*>(dst + 16) = make_uint4(0, 0, 0, 0);
+              }
             }
           }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         __syncwarp();
         if (lane == 0) mbar_arrive(&tfull[s]);
@@ -507,6 +507,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     // 32-column chunks of this warp: [c_lo, c_hi).
     const int c_lo = BN >= 64 ? half * (BN / 2) : half * 32;
     const int c_hi = BN >= 64 ? c_lo + BN / 2 : min(c_lo + 32, BN);
+    const bool vec = p.y_vec && (!p.res || p.res_vec);
     int nt = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++nt) {
       const int m0 = (tile / num_n) * BM, n0 = (tile % num_n) * BN, acc = nt & 1;
@@ -522,12 +523,13 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (col0 >= p.N) break;
         float v[32];
         tmem_ld32(ta + uint32_t(c), v);
-        if (row < p.M) {
-          if (p.bias) gemm::add_bias<32>(p, col0, v);
+        if (p.bias) gemm::add_bias<32>(p, col0, v);
+        if (vec && col0 + 32 <= p.N) {
+          // Aligned rows: 64 (or 128) consecutive bytes of a row per thread.
           if (p.act || p.res) gemm::epi_post<32>(p, row, col0, v);
-          if (p.y_dtype == L3D_BF16) {
-            __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + int64_t(row) * p.y_ld + col0;
-            if (col0 + 32 <= p.N && p.y_vec) {
+          if (row < p.M) {
+            if (p.y_dtype == L3D_BF16) {
+              __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + int64_t(row) * p.y_ld + col0;
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
                 float f[8];
@@ -536,21 +538,43 @@ __global__ void __launch_bounds__(THREADS, 1)
                 *reinterpret_cast<uint4*>(yr + q * 8) = pack(f, __nv_bfloat16());
               }
             } else {
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col0 + i < p.N) yr[i] = __float2bfloat16_rn(v[i]);
-            }
-          } else {
-            float* yr = static_cast<float*>(p.y) + int64_t(row) * p.y_ld + col0;
-            if (col0 + 32 <= p.N && p.y_vec) {
+              float* yr = static_cast<float*>(p.y) + int64_t(row) * p.y_ld + col0;
 #pragma unroll
               for (int q = 0; q < 8; ++q)
                 *reinterpret_cast<float4*>(yr + q * 4) =
                     make_float4(v[q * 4], v[q * 4 + 1], v[q * 4 + 2], v[q * 4 + 3]);
-            } else {
+            }
+          }
+        } else {
+          // Any alignment, and the last columns: through shared memory, so that
+          // a half warp reads and writes 16 consecutive elements of a row (a
+          // thread per row took 8 times as long over 24685 x 261).
+          if (p.act) gemm::epi_act<32>(p.act, p.y_dtype != L3D_F32, v);
+          float* st = stg + (warp - 6) * (32 * 17);
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (col0 + i < p.N) yr[i] = v[i];
+          for (int hc = 0; hc < 32; hc += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[lane * 17 + e] = v[hc + e];
+            __syncwarp();
+            const int col = col0 + hc + (lane & 15);
+            if (col >= p.N) continue;
+            const float g = !p.res || !p.gate ? 1.f
+                            : p.gate_dtype == L3D_F32
+                                ? static_cast<const float*>(p.gate)[col]
+                                : __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[col]);
+#pragma unroll 8
+            for (int i = 0; i < 16; ++i) {
+              const int rl = 2 * i + (lane >> 4), m = m0 + quarter * 32 + rl;
+              if (m >= p.M) continue;
+              float o = st[rl * 17 + (lane & 15)];
+              if (p.y_dtype == L3D_BF16) {
+                if (p.res) o = fmaf(g, o, to_f(static_cast<const __nv_bfloat16*>(p.res)[int64_t(m) * p.res_ld + col]));
+                static_cast<__nv_bfloat16*>(p.y)[int64_t(m) * p.y_ld + col] = __float2bfloat16_rn(o);
+              } else {
+                if (p.res) o = fmaf(g, o, static_cast<const float*>(p.res)[int64_t(m) * p.res_ld + col]);
+                static_cast<float*>(p.y)[int64_t(m) * p.y_ld + col] = o;
+              }
             }
           }
         }
@@ -809,14 +833,15 @@ extern "C" int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight,
   if (!make_map2(&mx, p.x, uint64_t(M), uint64_t(k), uint64_t(x_ld), uint32_t(p.x_rows)))
     return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed for x", op);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // Few rows: 16 per block, all warps along K, the group's adapters in
-  // parallel blocks.  Many: 64 per block, so that A is read less often.
+  // Few rows: 16 per block, all warps along K, the group's adapters and their
+  // ranks in parallel blocks.  Many: 64 per block, so that A is read less often.
   if (M <= int64_t(sm_count()) * 64) {
-    const int64_t y_blocks = A < M ? (A < 16 ? A : 16) : (M < 16 ? M : 16);
-    const int64_t groups = (M + 15) / 16;
-    shrink_kernel<1, 1, 1, 8><<<dim3(unsigned(groups), unsigned(groups > sm_count() ? 1 : y_blocks)), 256, 0, s>>>(p);
+    const int64_t groups = (M + 15) / 16, most = A < 16 ? A : 16;
+    const int64_t y_blocks = groups > sm_count() ? 1 : most < M ? most : M;
+    const int64_t z_blocks = groups > sm_count() ? 1 : (R + 31) / 32;
+    shrink_kernel<1, 1, 1, 8, 4><<<dim3(unsigned(groups), unsigned(y_blocks), unsigned(z_blocks)), 256, 0, s>>>(p);
   } else {
-    shrink_kernel<2, 2, 2, 2><<<dim3(unsigned((M + 63) / 64), 1), 256, 0, s>>>(p);
+    shrink_kernel<2, 2, 2, 2, 2><<<dim3(unsigned((M + 63) / 64), 1), 256, 0, s>>>(p);
   }
   if (cudaGetLastError() != cudaSuccess) return fail(L3D_E_CUDA, "%s: launch failed", op);
   const void* w = elem_ptr(weight);
