@@ -65,23 +65,12 @@ __device__ __forceinline__ void epi_post(const Params& p, int row, int col0, flo
                   : __ldg(reinterpret_cast<const float*>(rrow) + i);
       }
     }
-    if (p.gate && c + 8 <= p.N && (reinterpret_cast<uintptr_t>(p.gate) & 15) == 0) {
-      if (p.gate_dtype == L3D_F32) {
-        const float4 a = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + c));
-        const float4 b = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p.gate) + c) + 1);
-        g[0] = a.x; g[1] = a.y; g[2] = a.z; g[3] = a.w; g[4] = b.x; g[5] = b.y; g[6] = b.z; g[7] = b.w;
-      } else {
-        unpack(__ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.gate) + c)), g,
-               __nv_bfloat16());
-      }
-    } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int col = c + e < p.N ? c + e : p.N - 1;
       g[e] = !p.gate ? 1.f
              : p.gate_dtype == L3D_F32 ? __ldg(static_cast<const float*>(p.gate) + col)
                                        : __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[col]);
-    }
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -124,6 +113,36 @@ __device__ __forceinline__ void add_bias(const Params& p, int col0, float (&v)[N
       v[i] += p.bias_dtype == L3D_F32
                   ? __ldg(static_cast<const float*>(p.bias) + col)
                   : __uint_as_float(uint32_t(__ldg(static_cast<const unsigned short*>(p.bias) + col)) << 16);
+  }
+}
+
+// v[i] *= gate[col0 + i] for NC columns inside N: 16-byte loads where the gate
+// is so aligned.
+template <int NC, typename Params>
+__device__ __forceinline__ void mul_gate(const Params& p, int col0, float (&v)[NC]) {
+  const bool al = (reinterpret_cast<uintptr_t>(p.gate) & 15) == 0;
+  if (p.gate_dtype == L3D_F32) {
+    const float* g = static_cast<const float*>(p.gate) + col0;
+#pragma unroll
+    for (int q = 0; q < NC / 4; ++q) {
+      const float4 t = al ? __ldg(reinterpret_cast<const float4*>(g) + q)
+                          : make_float4(g[4 * q], g[4 * q + 1], g[4 * q + 2], g[4 * q + 3]);
+      v[4 * q] *= t.x; v[4 * q + 1] *= t.y; v[4 * q + 2] *= t.z; v[4 * q + 3] *= t.w;
+    }
+  } else {
+    const __nv_bfloat16* g = static_cast<const __nv_bfloat16*>(p.gate) + col0;
+#pragma unroll
+    for (int q = 0; q < NC / 8; ++q) {
+      float t[8];
+      if (al) {
+        unpack(__ldg(reinterpret_cast<const uint4*>(g) + q), t, __nv_bfloat16());
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) t[e] = __bfloat162float(g[8 * q + e]);
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[8 * q + e] *= t[e];
+    }
   }
 }
 

@@ -5,10 +5,10 @@
 // (crate/runtime/nn_blocks.rs:82,179-195) with the element-wise ops of its
 // blocks; the adapters have no counterpart there.
 //
-// Two launches.  shrink_kernel forms t[m] = scale_a A_a x[m] (rank columns)
-// in f32 and stores it as two bf16 parts.  lora_gemm_kernel then runs one product whose K
-// axis is x's, followed by the ranks of the adapters that occur in a 128-row
-// tile, 16 at a time: a slot multiplies the 128 x 16 piece of t, zero in the
+// Two launches.  shrink_kernel (shrink_tc_kernel for many rows) forms
+// t[m] = scale_a A_a x[m] in f32 and stores it as two bf16 parts.
+// lora_gemm_kernel then runs one product whose K axis is x's, followed by the
+// ranks of the adapters that occur in a 128-row tile, 16 at a time: a slot multiplies the 128 x 16 piece of t, zero in the
 // rows of other adapters, by the BN x 16 piece of B_a.  The zeros add nothing,
 // so a row's result does not depend on its neighbours; and each B_a is read
 // once per tile however many rows use it, which is all that a row-by-row
@@ -28,6 +28,8 @@
 // t); the t warps wait for it.  Every mbarrier wait is bounded (%globaltimer,
 // 2 s); on expiry the block records an error in the device's status word,
 // stops issuing work and still releases its TMEM.
+#include <type_traits>
+
 #include "act.cuh"
 #include "common.cuh"
 #include "epilogue.cuh"
@@ -88,21 +90,18 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// t for a group of 16 MT WR rows; 8 warps = WR (rows) x WN (32 ranks each) x
-// WK (K interleaved in chunks of 32, summed through shared memory in a fixed
-// order).  A lane loads 8 consecutive k of a row at once and uses them as the
-// operands of two K-16 products: both operands permute k alike, so the sums
-// are the same and every load is 16 bytes.  blockIdx.y strides over the
-// distinct adapters of the group, blockIdx.z over their ranks.
-template <int MT, int WR, int WN, int WK, int UNROLL>
-__global__ void __launch_bounds__(256, UNROLL > 2 ? 1 : 2) shrink_kernel(const Params p) {
-  constexpr int ROWS = 16 * MT * WR, NT = 4, RB = 32 * WN;
-  static_assert(WR * WN * WK == 8, "eight warps");
+// t for a group of 16 rows: eight warps share K, interleaved in chunks of 32,
+// and add up through shared memory in a fixed order.  A lane loads 8
+// consecutive k of a row at once and uses them as the operands of two K-16
+// products: both operands permute k alike, so the sums are the same and every
+// load is 16 bytes.  blockIdx.y strides over the distinct adapters of the
+// group, blockIdx.z over their ranks, 32 at a time.
+__global__ void __launch_bounds__(256, 1) shrink_kernel(const Params p) {
+  constexpr int ROWS = 16, NT = 4, RB = 32, WK = 8;
   __shared__ float red[WK][ROWS][RB + 4];
   __shared__ int s_id[ROWS], s_list[ROWS], s_wcount[8];
   asm volatile("griddepcontrol.launch_dependents;");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int wk = warp % WK, wn = (warp / WK) % WN, wr = warp / (WK * WN);
   const int g = lane >> 2, t4 = lane & 3;
   const int m0 = blockIdx.x * ROWS;
   // The distinct adapters of the group, in the order of their first rows.
@@ -122,66 +121,52 @@ __global__ void __launch_bounds__(256, UNROLL > 2 ? 1 : 2) shrink_kernel(const P
   }
   if (first) s_list[before + __popc(firsts & ((1u << lane) - 1))] = mine;
   __syncthreads();
-  const __nv_bfloat16* xr[MT][2];
-  bool xok[MT][2];
+  const __nv_bfloat16* xr[2];
+  bool xok[2];
 #pragma unroll
-  for (int i = 0; i < MT; ++i)
-#pragma unroll
-    for (int hf = 0; hf < 2; ++hf) {
-      const int m = m0 + (wr * MT + i) * 16 + hf * 8 + g;
-      xok[i][hf] = m < p.M;
-      xr[i][hf] = p.x + int64_t(xok[i][hf] ? m : 0) * p.x_ld + 8 * t4;
-    }
+  for (int hf = 0; hf < 2; ++hf) {
+    const int m = m0 + hf * 8 + g;
+    xok[hf] = m < p.M;
+    xr[hf] = p.x + int64_t(xok[hf] ? m : 0) * p.x_ld + 8 * t4;
+  }
   const int chunks = (p.K + 31) / 32;
   for (int d = blockIdx.y; d < count; d += gridDim.y) {
     const int a = s_list[d];
     const int rank = slots_of(p, a) * 16;
     for (int r0 = blockIdx.z * RB; r0 < rank; r0 += gridDim.z * RB) {
-      const int rb = r0 + wn * 32;
-      const int nt = min((rank - rb) / 8, NT);  // 8-rank tiles of this warp
-      float c[MT][NT][4];
+      const int nt = min((rank - r0) / 8, NT);  // 8-rank tiles
+      float c[NT][4];
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[j][e] = 0.f;
+      const __nv_bfloat16* ar = p.a + (int64_t(a) * p.R + r0 + g) * p.K + 8 * t4;
+#pragma unroll 4
+      for (int kc = warp; kc < chunks; kc += WK) {
+        const int k = kc * 32;
+        const bool kok = k + 8 * t4 < p.K;
+        uint4 xv[2], av[NT];
+        const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf)
+          xv[hf] = kok && xok[hf] ? __ldg(reinterpret_cast<const uint4*>(xr[hf] + k)) : zero;
 #pragma unroll
         for (int j = 0; j < NT; ++j)
+          av[j] = kok && j < nt ? __ldg(reinterpret_cast<const uint4*>(ar + int64_t(8 * j) * p.K + k)) : zero;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) c[i][j][e] = 0.f;
-      const __nv_bfloat16* ar = p.a + (int64_t(a) * p.R + rb + g) * p.K + 8 * t4;
-      if (nt > 0) {
-#pragma unroll UNROLL
-        for (int kc = wk; kc < chunks; kc += WK) {
-          const int k = kc * 32;
-          const bool kok = k + 8 * t4 < p.K;
-          uint4 xv[MT][2], av[NT];
-          const uint4 zero = make_uint4(0, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int hf = 0; hf < 2; ++hf)
-              xv[i][hf] = kok && xok[i][hf] ? __ldg(reinterpret_cast<const uint4*>(xr[i][hf] + k)) : zero;
-#pragma unroll
-          for (int j = 0; j < NT; ++j)
-            av[j] = kok && j < nt ? __ldg(reinterpret_cast<const uint4*>(ar + int64_t(8 * j) * p.K + k)) : zero;
-#pragma unroll
-          for (int j = 0; j < NT; ++j) {
-            if (j < nt) {
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                mma_16816(c[i][j], xv[i][0].x, xv[i][1].x, xv[i][0].y, xv[i][1].y, av[j].x, av[j].y);
-                mma_16816(c[i][j], xv[i][0].z, xv[i][1].z, xv[i][0].w, xv[i][1].w, av[j].z, av[j].w);
-              }
-            }
+        for (int j = 0; j < NT; ++j) {
+          if (j < nt) {
+            mma_16816(c[j], xv[0].x, xv[1].x, xv[0].y, xv[1].y, av[j].x, av[j].y);
+            mma_16816(c[j], xv[0].z, xv[1].z, xv[0].w, xv[1].w, av[j].z, av[j].w);
           }
         }
       }
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          const int row = (wr * MT + i) * 16 + g, col = wn * 32 + j * 8 + 2 * t4;
-          *reinterpret_cast<float2*>(&red[wk][row][col]) = make_float2(c[i][j][0], c[i][j][1]);
-          *reinterpret_cast<float2*>(&red[wk][row + 8][col]) = make_float2(c[i][j][2], c[i][j][3]);
-        }
+      for (int j = 0; j < NT; ++j) {
+        const int col = j * 8 + 2 * t4;
+        *reinterpret_cast<float2*>(&red[warp][g][col]) = make_float2(c[j][0], c[j][1]);
+        *reinterpret_cast<float2*>(&red[warp][g + 8][col]) = make_float2(c[j][2], c[j][3]);
+      }
       __syncthreads();
       const float sc = p.scale[a];
       for (int e = tid; e < ROWS * RB; e += 256) {
@@ -198,6 +183,193 @@ __global__ void __launch_bounds__(256, UNROLL > 2 ? 1 : 2) shrink_kernel(const P
       }
       __syncthreads();
     }
+  }
+}
+
+// t for many rows, on the 5th-generation tensor cores: a block per 128-row tile,
+// two blocks per SM, and for each distinct adapter of the tile one product of
+// the tile with A_a (M 128, N R, K in steps of 64 by TMA).  31569 x 1536, rank
+// 64: 70 us by mma.sync (its loads, straight to registers, are the limit).
+//   warp 0 TMA, warp 1 MMA, warps 2..5 the tile's adapters and the epilogue
+struct ShrinkTc {
+  int stages, tmem;
+};
+constexpr int SHRINK_THREADS = 6 * 32;
+__device__ __forceinline__ void umma_f16_rt(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc,
+                                            uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__global__ void __launch_bounds__(SHRINK_THREADS, 2)
+    shrink_tc_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a,
+                     const Params p, const ShrinkTc sc) {
+  constexpr int BM = 128, BK = 64, X_BYTES = BM * BK * 2;
+  int* const status = &g_lora_status;
+  extern __shared__ __align__(1024) uint8_t smem[];  // no static shared memory: 1024-byte aligned
+  const int a_bytes = p.R * BK * 2, stage_bytes = X_BYTES + a_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + sc.stages * stage_bytes);
+  uint64_t* full = bars;                 // [stages]
+  uint64_t* empty = full + sc.stages;    // [stages]
+  uint64_t* acc_full = empty + sc.stages;
+  uint64_t* acc_free = acc_full + 1;
+  uint64_t* drain = acc_free + 1;
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1) + 1;
+  int* ids = reinterpret_cast<int*>(bars + 32);  // [BM]
+  int* list = ids + BM;                          // [BM] the distinct adapters, by their first rows
+  int* firsts = list + BM;                       // [4]
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  const int m0 = blockIdx.x * BM, kblocks = (p.K + BK - 1) / BK;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < sc.stages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(acc_full, 1);
+    mbar_init(acc_free, 4);
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(sc.tmem));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  const int r = threadIdx.x - 64;  // row of warps 2..5
+  int mine = -1, place = 0;
+  bool first = false;
+  if (warp >= 2) {
+    mine = m0 + r < p.M ? adapter_of(p, m0 + r) : -1;
+    ids[r] = mine;
+  }
+  __syncthreads();
+  if (warp >= 2) {
+    const uint32_t same = __match_any_sync(0xffffffffu, mine);
+    first = mine >= 0 && (same & ((1u << lane) - 1)) == 0;
+    for (int q = 0; first && q < (r & ~31); ++q) first = ids[q] != mine;
+    const uint32_t mask = __ballot_sync(0xffffffffu, first);
+    place = __popc(mask & ((1u << lane) - 1));
+    if (lane == 0) firsts[warp - 2] = __popc(mask);
+  }
+  __syncthreads();
+  int count = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp - 2) place += firsts[w];
+    count += firsts[w];
+  }
+  if (first) list[place] = mine;
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {
+    const bool got = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, p.wait_ns)) != 0;
+    __syncwarp();
+    return got;
+  };
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      bool ok = true;
+      for (int d = 0; ok && d < count; ++d)
+        for (int kb = 0; kb < kblocks; ++kb, ++it) {
+          const int s = it % sc.stages;
+          if (it >= sc.stages &&
+              !mbar_wait(&empty[s], (it / sc.stages - 1) & 1, abort_flag, status, ST_TIMEOUT, p.wait_ns)) {
+            ok = false;
+            break;
+          }
+          mbar_expect_tx(&full[s], uint32_t(stage_bytes));
+          tma_load_2d(smem + s * stage_bytes, &map_x, &full[s], kb * BK, m0);
+          tma_load_2d(smem + s * stage_bytes + X_BYTES, &map_a, &full[s], kb * BK, list[d] * p.R);
+        }
+    }
+  } else if (warp == 1) {
+    const bool leader = elect_one();
+    const uint32_t idesc = make_idesc(BM, p.R);
+    int it = 0;
+    bool ok = true;
+    for (int d = 0; ok && d < count; ++d) {
+      if (d > 0) ok = wait_warp(acc_free, (d - 1) & 1);
+      tc_fence_after();
+      for (int kb = 0; ok && kb < kblocks; ++kb, ++it) {
+        const int s = it % sc.stages;
+        ok = wait_warp(&full[s], (it / sc.stages) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t da = smem_desc_sw128(smem + s * stage_bytes);
+        const uint64_t db = smem_desc_sw128(smem + s * stage_bytes + X_BYTES);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_f16_rt(tmem_base, da + uint64_t(2 * k), db + uint64_t(2 * k), idesc, (kb | k) ? 1u : 0u);
+          umma_commit(&empty[s]);
+        }
+      }
+      if (ok && leader) umma_commit(acc_full);
+    }
+  } else {
+    const int quarter = warp & 3, row = quarter * 32 + lane, m = m0 + row;
+    const int a_row = ids[row];
+    for (int d = 0; d < count; ++d) {
+      if (!wait_warp(acc_full, d & 1)) break;
+      tc_fence_after();
+      const int a = list[d], rank = slots_of(p, a) * 16;
+      const float scale = p.scale[a];
+      for (int c = 0; c < rank; c += 16) {
+        float v[16];
+        tmem_ld16(tmem_base + (uint32_t(quarter * 32) << 16) + uint32_t(c), v);
+        if (a_row == a) {
+          uint4 u[PARTS][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float x = v[8 * h + e] * scale;
+              hi[e] = __bfloat162float(__float2bfloat16_rn(x));
+              lo[e] = x - hi[e];
+            }
+            u[0][h] = pack(hi, __nv_bfloat16());
+            u[1][h] = pack(lo, __nv_bfloat16());
+          }
+#pragma unroll
+          for (int part = 0; part < PARTS; ++part) {
+            uint4* dst = reinterpret_cast<uint4*>(p.t + (int64_t(part) * p.M + m) * p.R + c);
+            dst[0] = u[part][0];
+            dst[1] = u[part][1];
+          }
+        }
+        __syncwarp();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(acc_free);
+    }
+  }
+  // Teardown: after an abort, wait (bounded) for the MMAs this block issued,
+  // and give TMA loads still in flight 1 ms to land.
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag && warp == 1 && elect_one()) {
+    umma_commit(drain);
+    mbar_drain(drain, 0, p.wait_ns);
+    const uint64_t t0 = globaltimer();
+    while (globaltimer() - t0 < 1000000ull) {
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(sc.tmem));
   }
 }
 
@@ -238,7 +410,8 @@ __device__ __forceinline__ uint64_t smem_desc_sw32(const void* tile) {
   return d;
 }
 
-template <int BN>
+// RES: there is a residual.
+template <int BN, bool RES>
 __global__ void __launch_bounds__(THREADS, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
                      const __grid_constant__ CUtensorMap map_b, const Params p) {
@@ -507,38 +680,69 @@ __global__ void __launch_bounds__(THREADS, 1)
     // 32-column chunks of this warp: [c_lo, c_hi).
     const int c_lo = BN >= 64 ? half * (BN / 2) : half * 32;
     const int c_hi = BN >= 64 ? c_lo + BN / 2 : min(c_lo + 32, BN);
-    const bool vec = p.y_vec && (!p.res || p.res_vec);
+    const bool vec = p.y_vec && (!RES || p.res_vec);
     int nt = 0;
     for (int tile = blockIdx.x; tile < tiles; tile += gridDim.x, ++nt) {
       const int m0 = (tile / num_n) * BM, n0 = (tile % num_n) * BN, acc = nt & 1;
+      // The residual of the tile is brought to L2 while the products run.
+      const int row = m0 + quarter * 32 + lane;
+      if (RES && row < p.M) {
+        const int es = p.y_dtype == L3D_BF16 ? 2 : 4;
+        const char* rr = static_cast<const char*>(p.res) + (int64_t(row) * p.res_ld + n0) * es;
+        const int end = min(c_hi, p.N - n0) * es;
+        for (int b = c_lo * es; b < end; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(rr + b));
+      }
       if (!__all_sync(0xffffffffu, mbar_wait_idle(&acc_full[acc], (nt / 2) & 1, abort_flag, status,
                                                    ST_TIMEOUT, p.wait_ns)))
         break;
       tc_fence_after();
-      const int row = m0 + quarter * 32 + lane;
       const uint32_t ta = tmem_base + uint32_t(acc * BN) + (uint32_t(quarter * 32) << 16);
 #pragma unroll 1
       for (int c = c_lo; c < c_hi; c += 32) {
         const int col0 = n0 + c;
         if (col0 >= p.N) break;
+        const bool whole = vec && col0 + 32 <= p.N, bf = p.y_dtype == L3D_BF16;
+        // The residual is read before the accumulator, without branches between
+        // its loads: its latency is that of one load.
+        uint4 u[4];
+        if (RES && whole && bf && row < p.M) {
+          const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.res) +
+                                                            int64_t(row) * p.res_ld + col0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) u[q] = src[q];
+        }
         float v[32];
         tmem_ld32(ta + uint32_t(c), v);
         if (p.bias) gemm::add_bias<32>(p, col0, v);
-        if (vec && col0 + 32 <= p.N) {
+        if (p.act) gemm::epi_act<32>(p.act, bf, v);
+        if (whole) {
           // Aligned rows: 64 (or 128) consecutive bytes of a row per thread.
-          if (p.act || p.res) gemm::epi_post<32>(p, row, col0, v);
+          if (RES && p.gate) gemm::mul_gate<32>(p, col0, v);
           if (row < p.M) {
-            if (p.y_dtype == L3D_BF16) {
+            if (bf) {
               __nv_bfloat16* yr = static_cast<__nv_bfloat16*>(p.y) + int64_t(row) * p.y_ld + col0;
 #pragma unroll
               for (int q = 0; q < 4; ++q) {
-                float f[8];
+                float (&f)[8] = *reinterpret_cast<float(*)[8]>(&v[8 * q]);
+                if constexpr (RES) {
+                  float r[8];
+                  unpack(u[q], r, __nv_bfloat16());
 #pragma unroll
-                for (int e = 0; e < 8; ++e) f[e] = v[q * 8 + e];
+                  for (int e = 0; e < 8; ++e) f[e] += r[e];
+                }
                 *reinterpret_cast<uint4*>(yr + q * 8) = pack(f, __nv_bfloat16());
               }
             } else {
               float* yr = static_cast<float*>(p.y) + int64_t(row) * p.y_ld + col0;
+              if constexpr (RES) {
+                const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(p.res) +
+                                                                    int64_t(row) * p.res_ld + col0);
+#pragma unroll
+                for (int q = 0; q < 8; ++q) {
+                  const float4 t = src[q];
+                  v[4 * q] += t.x; v[4 * q + 1] += t.y; v[4 * q + 2] += t.z; v[4 * q + 3] += t.w;
+                }
+              }
 #pragma unroll
               for (int q = 0; q < 8; ++q)
                 *reinterpret_cast<float4*>(yr + q * 4) =
@@ -547,34 +751,40 @@ __global__ void __launch_bounds__(THREADS, 1)
           }
         } else {
           // Any alignment, and the last columns: through shared memory, so that
-          // a half warp reads and writes 16 consecutive elements of a row (a
-          // thread per row took 8 times as long over 24685 x 261).
-          if (p.act) gemm::epi_act<32>(p.act, p.y_dtype != L3D_F32, v);
+          // a half warp reads and writes 16 consecutive elements of a row.
+          // (Places outside the matrix read its last element: no branches.)
           float* st = stg + (warp - 6) * (32 * 17);
 #pragma unroll
           for (int hc = 0; hc < 32; hc += 16) {
+            const int col = col0 + hc + (lane & 15), cc = min(col, p.N - 1);
+            auto row_of = [&](int i) { return m0 + quarter * 32 + 2 * i + (lane >> 4); };
+            float r[16];
+            if (RES && bf) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                r[i] = to_f(static_cast<const __nv_bfloat16*>(p.res)[int64_t(min(row_of(i), p.M - 1)) * p.res_ld + cc]);
+            } else if (RES) {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                r[i] = static_cast<const float*>(p.res)[int64_t(min(row_of(i), p.M - 1)) * p.res_ld + cc];
+            }
             __syncwarp();
 #pragma unroll
             for (int e = 0; e < 16; ++e) st[lane * 17 + e] = v[hc + e];
             __syncwarp();
-            const int col = col0 + hc + (lane & 15);
             if (col >= p.N) continue;
-            const float g = !p.res || !p.gate ? 1.f
+            const float g = !RES || !p.gate ? 1.f
                             : p.gate_dtype == L3D_F32
                                 ? static_cast<const float*>(p.gate)[col]
                                 : __bfloat162float(static_cast<const __nv_bfloat16*>(p.gate)[col]);
-#pragma unroll 8
+#pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int rl = 2 * i + (lane >> 4), m = m0 + quarter * 32 + rl;
+              const int m = row_of(i);
               if (m >= p.M) continue;
-              float o = st[rl * 17 + (lane & 15)];
-              if (p.y_dtype == L3D_BF16) {
-                if (p.res) o = fmaf(g, o, to_f(static_cast<const __nv_bfloat16*>(p.res)[int64_t(m) * p.res_ld + col]));
-                static_cast<__nv_bfloat16*>(p.y)[int64_t(m) * p.y_ld + col] = __float2bfloat16_rn(o);
-              } else {
-                if (p.res) o = fmaf(g, o, static_cast<const float*>(p.res)[int64_t(m) * p.res_ld + col]);
-                static_cast<float*>(p.y)[int64_t(m) * p.y_ld + col] = o;
-              }
+              float o = st[(2 * i + (lane >> 4)) * 17 + (lane & 15)];
+              if (RES) o = fmaf(g, o, r[i]);
+              if (bf) static_cast<__nv_bfloat16*>(p.y)[int64_t(m) * p.y_ld + col] = __float2bfloat16_rn(o);
+              else static_cast<float*>(p.y)[int64_t(m) * p.y_ld + col] = o;
             }
           }
         }
@@ -633,10 +843,10 @@ static bool make_map_b(CUtensorMap* m, const void* base, uint64_t A, uint64_t n,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int BN>
+template <int BN, bool RES>
 static cudaError_t launch_gemm(const CUtensorMap& mx, const void* w, int64_t w_ld, const void* b,
                                const Params& p, cudaStream_t s) {
-  auto k = lora_gemm_kernel<BN>;
+  auto k = lora_gemm_kernel<BN, RES>;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<BN>::SMEM);
   if (e != cudaSuccess) return e;
   CUtensorMap mw, mb;
@@ -833,25 +1043,39 @@ extern "C" int l3d_lora_linear(const l3d_tensor* x, const l3d_tensor* weight,
   if (!make_map2(&mx, p.x, uint64_t(M), uint64_t(k), uint64_t(x_ld), uint32_t(p.x_rows)))
     return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed for x", op);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  // Few rows: 16 per block, all warps along K, the group's adapters and their
-  // ranks in parallel blocks.  Many: 64 per block, so that A is read less often.
-  if (M <= int64_t(sm_count()) * 64) {
-    const int64_t groups = (M + 15) / 16, most = A < 16 ? A : 16;
-    const int64_t y_blocks = groups > sm_count() ? 1 : most < M ? most : M;
-    const int64_t z_blocks = groups > sm_count() ? 1 : (R + 31) / 32;
-    shrink_kernel<1, 1, 1, 8, 4><<<dim3(unsigned(groups), unsigned(y_blocks), unsigned(z_blocks)), 256, 0, s>>>(p);
+  // Few rows: 16 per block, the group's adapters and their ranks in parallel
+  // blocks.  More than a device of such groups (2368 rows): the tensor-core form
+  // (both take 9 us at 4098 x 2048, rank 32; at 8587 rows 18 and 9).
+  const int64_t groups = (M + 15) / 16;
+  if (groups <= sm_count()) {
+    const int64_t most = A < 16 ? A : 16, y_blocks = most < M ? most : M, z_blocks = (R + 31) / 32;
+    shrink_kernel<<<dim3(unsigned(groups), unsigned(y_blocks), unsigned(z_blocks)), 256, 0, s>>>(p);
   } else {
-    shrink_kernel<2, 2, 2, 2, 2><<<dim3(unsigned((M + 63) / 64), 1), 256, 0, s>>>(p);
+    ShrinkTc sc{};
+    const int stage = 128 * 64 * 2 + int(R) * 64 * 2;
+    sc.stages = 104 * 1024 / stage < 6 ? 104 * 1024 / stage : 6;
+    for (sc.tmem = 32; sc.tmem < int(R);) sc.tmem *= 2;
+    const int smem = sc.stages * stage + 256 + (128 + 128 + 4) * 4;
+    CUtensorMap ma;
+    if (!make_map2(&ma, p.a, uint64_t(A) * uint64_t(R), uint64_t(k), uint64_t(k), uint32_t(R)))
+      return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed for lora_a", op);
+    if (set_smem_limit(reinterpret_cast<const void*>(shrink_tc_kernel), 110 * 1024) != cudaSuccess)
+      return fail(L3D_E_CUDA, "%s: cannot reserve shared memory", op);
+    shrink_tc_kernel<<<unsigned((M + 127) / 128), SHRINK_THREADS, size_t(smem), s>>>(mx, ma, p, sc);
   }
   if (cudaGetLastError() != cudaSuccess) return fail(L3D_E_CUDA, "%s: launch failed", op);
   const void* w = elem_ptr(weight);
   const void* b = elem_ptr(lora_b);
   cudaError_t e;
+  auto launch = [&](auto bn) {
+    constexpr int BN = decltype(bn)::value;
+    return residual ? launch_gemm<BN, true>(mx, w, w_ld, b, p, s) : launch_gemm<BN, false>(mx, w, w_ld, b, p, s);
+  };
   switch (pick_bn(M, n)) {
-    case 32: e = launch_gemm<32>(mx, w, w_ld, b, p, s); break;
-    case 64: e = launch_gemm<64>(mx, w, w_ld, b, p, s); break;
-    case 128: e = launch_gemm<128>(mx, w, w_ld, b, p, s); break;
-    default: e = launch_gemm<256>(mx, w, w_ld, b, p, s); break;
+    case 32: e = launch(std::integral_constant<int, 32>()); break;
+    case 64: e = launch(std::integral_constant<int, 64>()); break;
+    case 128: e = launch(std::integral_constant<int, 128>()); break;
+    default: e = launch(std::integral_constant<int, 256>()); break;
   }
   if (e != cudaSuccess) return fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
   return L3D_OK;

@@ -612,8 +612,8 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
     "rms" or "layer"; next_norm=False (the last block) returns (r, None); with
     inplace=True the residual stream x is updated in place (r is x)."""
     _check_cuda(x, h, post_weight, post_bias, gate, weight, bias, shift, scale)
-    r = x if inplace else x.new_empty(x.shape)
-    y = x.new_empty(x.shape) if next_norm else None
+    r = x if inplace else torch.empty_like(x, memory_format=torch.contiguous_format)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format) if next_norm else None
     call("l3d_sandwich_residual_norm", packed(x), packed(h), NORMS[norm],
          packed(post_weight), packed(post_bias), packed(gate), float(res_scale),
          packed(weight), packed(bias), packed(shift), packed(scale),

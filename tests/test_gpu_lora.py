@@ -123,6 +123,20 @@ def test_lora_linear_many_tiles(ops, dev):
     _case(ops, dev, 5000, 2560, 192, [16, 32, 64, 16], rng(9).integers(-1, 4, 5000).astype(np.int32))
 
 
+@pytest.mark.parametrize("M,N,K,ranks,kind", [
+    (2369, 96, 264, [16, 48], "scene"),     # around the row count where A x changes its kernel
+    (2368, 96, 264, [16, 48], "scene"),
+    (2500, 77, 136, [256, 8], "scene"),
+    (2600, 40, 72, [16] * 20, "row"),       # many adapters in every tile
+    (12001, 64, 520, [64], "request"),
+])
+def test_lora_linear_many_rows(ops, dev, M, N, K, ranks, kind):
+    A = len(ranks)
+    ids = {"scene": lambda: np.sort(rng(M).integers(-1, A, M)), "row": lambda: rng(M).integers(-1, A, M),
+           "request": lambda: np.asarray([0, -1, 0, -1, 0, 0, 0][:next(n for n in (7, 1) if M % n == 0)])}[kind]()
+    _case(ops, dev, M, N, K, ranks, ids.astype(np.int32))
+
+
 def test_lora_linear_strided_rows(ops, dev):
     """x and out as column ranges of wider matrices; nothing else is written."""
     import torch
