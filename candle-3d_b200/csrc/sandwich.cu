@@ -6,6 +6,8 @@
 // The reference composes such seams from its norms and residual adds
 // (crate/runtime/trellis2_blocks.rs:280-286,627-645, crate/runtime/vggt.rs:104-123);
 // here x and h are read once and r and y written once.
+#include <type_traits>
+
 #include "common.cuh"
 #include "ring.cuh"
 
@@ -105,7 +107,7 @@ __global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
 struct Coefs {
   int has_b1, has_b2;
   int ld;                  // floats of a coefficient row (a multiple of 4)
-  int chan_vec;            // the vectors are 16-byte aligned
+  int chan_vec;            // the vectors are 16-byte aligned, and 2: of the activations' type
 };
 
 // Place of channel c in a coefficient row read in vectors of VEC: in planes of
@@ -118,11 +120,48 @@ __device__ __forceinline__ int coef_at(int c, int ld) {
 }
 
 // One channel, or VEC consecutive ones, of batch element b folded into `coef`.
-template <int VEC>
+template <typename T, int VEC>
 __device__ __forceinline__ void fold(const Params& p, const Coefs& k, float* coef, int64_t b) {
   const int C = int(p.C);
   float* row = coef;
   float *a1 = row, *a2 = row + k.ld, *b1 = row + 2 * k.ld, *b2 = row + (2 + k.has_b1) * k.ld;
+  if constexpr (VEC > 1) {
+    if (k.chan_vec == 2) {
+      // All vectors' loads at once (without branches between them): this is what
+      // a call on a few rows waits for.
+      for (int c = int(threadIdx.x) * VEC; c < C; c += int(blockDim.x) * VEC) {
+        const ChanVec* const vecs[7] = {&p.gate, &p.pw, &p.pb, &p.scale, &p.w, &p.b, &p.shift};
+        uint4 raw[7];
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+          raw[i] = vecs[i]->ptr ? __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(vecs[i]->ptr) +
+                                                                       b * vecs[i]->bstride + c))
+                                : make_uint4(0, 0, 0, 0);
+        float f[7][VEC];
+#pragma unroll
+        for (int i = 0; i < 7; ++i) unpack(raw[i], f[i], T());
+        float o[4][VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float g = p.gate.ptr ? f[0][e] : 1.f, t = 1.f + f[3][e];
+          o[0][e] = g * (p.pw.ptr ? f[1][e] : 1.f);
+          o[1][e] = t * (p.w.ptr ? f[4][e] : 1.f);
+          o[2][e] = g * f[2][e];
+          o[3][e] = fmaf(t, f[5][e], f[6][e]);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; e += 4) {
+          const int at = coef_at<VEC>(c + e, k.ld);
+          auto four = [&](int i) { return make_float4(o[i][e], o[i][e + 1], o[i][e + 2], o[i][e + 3]); };
+          *reinterpret_cast<float4*>(a1 + at) = four(0);
+          *reinterpret_cast<float4*>(a2 + at) = four(1);
+          if (k.has_b1) *reinterpret_cast<float4*>(b1 + at) = four(2);
+          if (k.has_b2) *reinterpret_cast<float4*>(b2 + at) = four(3);
+        }
+      }
+      return;
+    }
+  }
   if (VEC > 1 && k.chan_vec) {
     for (int c = int(threadIdx.x) * VEC; c < C; c += int(blockDim.x) * VEC) {
       float g[VEC], w[VEC], t[VEC];
@@ -199,7 +238,7 @@ __device__ __forceinline__ float group_sum(float v, float* red, int& turn) {
   if constexpr (G > 32) {
     constexpr int W = G / 32;
     const int grp = threadIdx.x / G;
-    float* r = red + turn * 16 + grp * W;
+    float* r = red + turn * 20 + grp * W;
     turn ^= 1;
     if ((threadIdx.x & 31) == 0) r[(threadIdx.x % G) >> 5] = v;
     asm volatile("bar.sync %0, %1;" ::"r"(1 + grp), "n"(G) : "memory");
@@ -236,7 +275,9 @@ __device__ __forceinline__ bool unit_all(bool ok) {
 // Both norms' sums are taken in two passes over the registers (mean, then
 // centred squares: one pass of shifted moments loses digits where one channel
 // lies far out).
-constexpr int kThreads = 384;
+// Threads of a block: 12 warps of 168 registers for 8 vectors a thread, 20 of 96
+// for rows of half that length.
+constexpr int threads_of(int nv) { return nv == 8 ? 384 : 640; }
 constexpr int kSlots = 2;
 
 struct Ring {
@@ -248,13 +289,13 @@ struct Ring {
 
 __device__ int g_sandwich_status;
 
-template <typename T, int G, int NORM>
-__global__ void __launch_bounds__(kThreads, 1)
+template <typename T, int G, int NV, int NORM>
+__global__ void __launch_bounds__(threads_of(NV), 1)
     ring_kernel(const Params p, const Coefs kc, const Ring sp) {
-  constexpr int VEC = Vec16<T>::N, NV = 8, P = VEC / 2;  // vectors of a thread, pairs of a vector
+  constexpr int VEC = Vec16<T>::N, P = VEC / 2;          // pairs of a vector (NV of them a thread)
   constexpr int U = G < 32 ? 32 : G, RPU = U / G;        // threads and rows of a unit
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ float red[32];
+  __shared__ float red[40];
   float* coef = reinterpret_cast<float*>(smem);
   uint8_t* slots = smem + size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
   const uint32_t slot_bytes = 2 * RPU * sp.row_bytes;    // the pack's h rows, then its x rows
@@ -305,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int64_t b = s0 / sp.rows_per_batch;
     const int64_t s1 = min((b + 1) * sp.rows_per_batch, hi);
     if (s0 != lo) __syncthreads();
-    fold<VEC>(p, kc, coef, b);
+    fold<T, VEC>(p, kc, coef, b);
     __syncthreads();
     // Vector i of this thread of coefficient row k.
     auto coefs = [&](int k, int i, float2 (&o)[P]) {
@@ -428,12 +469,12 @@ __global__ void __launch_bounds__(kBlock, 2)
     elem_kernel(const Params p, const Coefs kc, const Blocks sp) {
   constexpr int NE = 32, RPB = kBlock / G;
   extern __shared__ __align__(16) float coef[];
-  __shared__ float red[32];
+  __shared__ float red[40];
   const int t = threadIdx.x % G, C = int(p.C);
   const int64_t b = blockIdx.x / sp.per_batch;
   const int64_t first = int64_t(blockIdx.x % sp.per_batch) * sp.rows_per_block;
   const int64_t last = min(first + sp.rows_per_block, sp.rows);
-  fold<1>(p, kc, coef, b);
+  fold<T, 1>(p, kc, coef, b);
   __syncthreads();
   const float *a1 = coef, *a2 = coef + kc.ld, *b1 = coef + 2 * kc.ld, *b2 = coef + (2 + kc.has_b1) * kc.ld;
   const float inv_c = 1.f / float(C);
@@ -501,21 +542,21 @@ constexpr int kSmem = 227 * 1024 - 1024;
 constexpr const char* kNoSmem = "l3d_sandwich_residual_norm: cannot reserve shared memory";
 
 // Returns 1 when launched, 0 when the row does not fit this kernel, or fails.
-template <typename T, int G, int NORM>
+template <typename T, int G, int NV, int NORM>
 static int launch_ring(const Params& p, const Coefs& kc, Ring sp, size_t coef, cudaStream_t s) {
   constexpr int U = G < 32 ? 32 : G, RPU = U / G;
   const size_t slot = size_t(kSlots) * (2 * RPU * sp.row_bytes + 8);
   if (coef + slot + 16 > size_t(kSmem)) return 0;
-  auto k = ring_kernel<T, G, NORM>;
+  auto k = ring_kernel<T, G, NV, NORM>;
   if (set_smem_limit(reinterpret_cast<const void*>(k), kSmem) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
   const int64_t packs = (p.rows + RPU - 1) / RPU;
   const int64_t blocks = packs < sm_count() ? packs : sm_count();
   const int64_t per_block = ((p.rows + blocks - 1) / blocks + RPU - 1) / RPU;
-  int64_t units = kThreads / U;
+  int64_t units = threads_of(NV) / U;
   if (units > per_block) units = per_block;
   const int64_t room = int64_t((size_t(kSmem) - coef - 16) / slot);
   sp.units = int(units < room ? units : room);
-  k<<<unsigned(blocks), kThreads, coef + size_t(sp.units) * slot + 16, s>>>(p, kc, sp);
+  k<<<unsigned(blocks), threads_of(NV), coef + size_t(sp.units) * slot + 16, s>>>(p, kc, sp);
   return 1;
 }
 
@@ -545,6 +586,11 @@ static int try_fast(const Params& p, bool vec_ok, bool chan_vec, int64_t batches
   kc.has_b2 = p.b.ptr || p.shift.ptr;
   kc.ld = int((p.C + 7) & ~int64_t(7));
   kc.chan_vec = chan_vec;
+  const int dt = std::is_same<T, float>::value ? L3D_F32 : std::is_same<T, __half>::value ? L3D_F16 : L3D_BF16;
+  bool same = chan_vec;
+  for (const ChanVec* v : {&p.gate, &p.pw, &p.pb, &p.scale, &p.w, &p.b, &p.shift})
+    if (v->ptr && v->dtype != dt) same = false;
+  if (same) kc.chan_vec = 2;
   const size_t coef = size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
   if (vec_ok) {
     Ring sp{};
@@ -552,11 +598,13 @@ static int try_fast(const Params& p, bool vec_ok, bool chan_vec, int64_t batches
     sp.row_bytes = uint32_t(p.C * sizeof(T));
     sp.wait_ns = 2000000000ull;
     constexpr int E = 8 * Vec16<T>::N;  // elements of a thread
-    const int rc = p.C <= 8 * E ? launch_ring<T, 8, NORM>(p, kc, sp, coef, s)
-                   : p.C <= 32 * E ? launch_ring<T, 32, NORM>(p, kc, sp, coef, s)
-                   : p.C <= 64 * E ? launch_ring<T, 64, NORM>(p, kc, sp, coef, s)
-                   : p.C <= 128 * E ? launch_ring<T, 128, NORM>(p, kc, sp, coef, s)
-                   : p.C <= 256 * E ? launch_ring<T, 256, NORM>(p, kc, sp, coef, s) : 0;
+    const int rc = p.C <= 4 * E ? launch_ring<T, 8, 4, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 8 * E ? launch_ring<T, 8, 8, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 16 * E ? launch_ring<T, 32, 4, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 32 * E ? launch_ring<T, 32, 8, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 64 * E ? launch_ring<T, 64, 8, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 128 * E ? launch_ring<T, 128, 8, NORM>(p, kc, sp, coef, s)
+                   : p.C <= 256 * E ? launch_ring<T, 256, 8, NORM>(p, kc, sp, coef, s) : 0;
     if (rc) return rc;
   }
   return p.C <= 32 * 32 ? launch_elem<T, 32, NORM>(p, kc, batches, coef, s)
