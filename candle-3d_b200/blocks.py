@@ -578,3 +578,136 @@ class Trellis2Slat:
                 # final non-affine LN eps 1e-5 (trellis2_dit.rs:572)
                 x, y = ops.residual_layer_norm_modulate(x, h, gate=g_mlp, eps=1e-5, inplace=True)
         return F.linear(y.view(N, C), *self.out_layer)
+
+
+# ==================================================== blocks served to many requests
+class SharedContextBlocks:
+    """Transformer blocks served to a batch of requests around one shared context
+    (the tokens of a scene, encoded once), each request with adapters of its own
+    and its own tokens, which arrive a few at a time:
+
+      y = LN(x); qkv = Wqkv y + adapter; q, k = RMSNorm per head (q, k)
+      a = softmax(q [context k, own k]) [context v, own v], causal in the own keys
+      x, y = x + g1 * RMS(Wo a + adapter) * w, RMS(x) * w'
+      x, y = x + g2 * RMS(fc2 gelu(fc1 y)) * w, the next block's RMS(x) * w'
+
+    One launch per seam, two per projection with adapters, and the context is
+    read once for the whole batch, whose elements do not hold copies of it."""
+
+    def __init__(self, depth=2, dim=512, heads=8, kv_heads=2, mlp=2048, ranks=(16, 8, 32), seed=0,
+                 device="cuda"):
+        g = torch.Generator().manual_seed(seed)
+        self.C, self.H, self.Hkv, self.D = dim, heads, kv_heads, dim // heads
+        self.depth, self.dtype, self.device = depth, torch.bfloat16, device
+
+        def proj(n, k):
+            ad = ops.LoraAdapters([_w(g, (r, k), k ** -0.5, device) for r in ranks],
+                                  [_w(g, (n, r), 0.5 * r ** -0.5, device) for r in ranks],
+                                  [0.5 + 0.25 * i for i in range(len(ranks))])
+            return _w(g, (n, k), k ** -0.5, device), ad
+
+        def vec(n, mean=1.0):
+            return (mean + 0.1 * torch.randn(n, generator=g)).to(device, self.dtype)
+
+        self.n0 = vec(dim), vec(dim, 0.0)
+        self.blocks = [
+            {"qkv": proj((heads + 2 * kv_heads) * self.D, dim), "out": proj(dim, dim),
+             "fc1": proj(mlp, dim), "fc2": proj(dim, mlp), "qn": vec(self.D), "kn": vec(self.D),
+             "post1": vec(dim), "g1": vec(dim, 0.5), "pre2": vec(dim),
+             "post2": vec(dim), "g2": vec(dim, 0.5), "pre": vec(dim)}  # pre: before the next block
+            for _ in range(depth)]
+
+    def _split(self, p, qkv):
+        """qkv [B, N, ..] -> q [B, Hq, N, D], k and v [B, Hkv, N, D] (views)."""
+        H, Hkv = self.H, self.Hkv
+        qkv = qkv.view(*qkv.shape[:2], H + 2 * Hkv, self.D)
+        q = ops.rms_norm_heads(qkv[:, :, :H], p["qn"])
+        k = ops.rms_norm_heads(qkv[:, :, H:H + Hkv], p["kn"])
+        return q.transpose(1, 2), k.transpose(1, 2), qkv[:, :, H + Hkv:].transpose(1, 2)
+
+    def _tail(self, p, x, a, ids):
+        """The block from its attention's output [B, N, C] on."""
+        o = ops.lora_linear(a, p["out"][0], p["out"][1], ids)
+        x, y = ops.sandwich_residual_norm(x, o, p["post1"], gate=p["g1"], weight=p["pre2"])
+        h = ops.lora_linear(y, p["fc1"][0], p["fc1"][1], ids, act="gelu")
+        h = ops.lora_linear(h, p["fc2"][0], p["fc2"][1], ids)
+        return ops.sandwich_residual_norm(x, h, p["post2"], gate=p["g2"], weight=p["pre"],
+                                          inplace=True)
+
+    def encode_context(self, tokens):
+        """tokens [P, C] -> per block the keys and values [Hkv, P, D] that every
+        request attends to (no adapters: the context belongs to none of them)."""
+        P = tokens.shape[0]
+        ids = torch.full((1,), -1, dtype=torch.int32, device=tokens.device)
+        x = tokens.view(1, P, self.C)
+        y = ops.layer_norm(x, *self.n0, eps=1e-6)
+        kv = []
+        for i, p in enumerate(self.blocks):
+            q, k, v = self._split(p, ops.lora_linear(y, p["qkv"][0], p["qkv"][1], ids))
+            kv.append((k[0], v[0]))
+            if i + 1 < self.depth:
+                a = ops.shared_prefix_attention(q, k[0], v[0])
+                x, y = self._tail(p, x, a.transpose(1, 2).reshape(1, P, self.C), ids)
+        return kv
+
+    def new_cache(self, batch, capacity):
+        """Room for `capacity` own tokens of each request: (k, v) per block."""
+        def room():
+            return torch.zeros((batch, self.Hkv, capacity, self.D), dtype=self.dtype,
+                               device=self.device)
+        return [(room(), room()) for _ in range(self.depth)]
+
+    def forward(self, x, context, cache, start, ids):
+        """x [B, N, C]: the next N tokens of each request, request b holding
+        start[b] (int32) already; ids [B]: its adapter, or one outside the range
+        for none.  Returns their final states [B, N, C]; the cache takes their
+        keys and values."""
+        B, N, C = x.shape
+        rows = torch.arange(B, device=x.device).view(B, 1)
+        at = start.view(B, 1).long() + torch.arange(N, device=x.device)
+        lengths = start + N
+        y = ops.layer_norm(x, *self.n0, eps=1e-6)
+        for p, (pk, pv), (ck, cv) in zip(self.blocks, context, cache):
+            q, k, v = self._split(p, ops.lora_linear(y, p["qkv"][0], p["qkv"][1], ids))
+            ck[rows, :, at] = k.transpose(1, 2)
+            cv[rows, :, at] = v.transpose(1, 2)
+            a = ops.shared_prefix_attention(q, pk, pv, ck, cv, lengths, causal=True)
+            x, y = self._tail(p, x, a.transpose(1, 2).reshape(B, N, C), ids)
+        return y
+
+
+def shared_context_reference(m: SharedContextBlocks, x, tokens, ids):
+    """SharedContextBlocks over whole requests x [B, L, C] at once, in torch f64:
+    every request's tokens follow a copy of the context `tokens` [P, C]."""
+    f = lambda a: a.double()  # noqa: E731
+    B, L, C = x.shape
+    P, H, Hkv, D = tokens.shape[0], m.H, m.Hkv, m.D
+
+    def rms(v, w):
+        return v / torch.sqrt(v.pow(2).mean(-1, keepdim=True) + 1e-6) * f(w)
+
+    def lin(v, wa):
+        w, ad = wa
+        y = F.linear(v, f(w))
+        for b, i in enumerate(ids.tolist()):
+            if 0 <= i < ad.count:  # the context rows take no adapter
+                y[b, P:] += f(ad.scales[i]) * (v[b, P:] @ f(ad.a[i]).T @ f(ad.b[i]).T)
+        return y
+
+    h = torch.cat([f(tokens).expand(B, P, C), f(x)], 1)
+    mask = torch.ones(P + L, P + L, dtype=torch.bool, device=x.device).tril()
+    mask[:P] = torch.arange(P + L, device=x.device) < P  # the context sees itself, both ways
+    mask[:, :P] = True
+    y = F.layer_norm(h, (C,), f(m.n0[0]), f(m.n0[1]), 1e-6)
+    for p in m.blocks:
+        qkv = lin(y, p["qkv"]).view(B, P + L, H + 2 * Hkv, D)
+        q = rms(qkv[:, :, :H], p["qn"]).transpose(1, 2)
+        k = rms(qkv[:, :, H:H + Hkv], p["kn"]).transpose(1, 2).repeat_interleave(H // Hkv, 1)
+        v = qkv[:, :, H + Hkv:].transpose(1, 2).repeat_interleave(H // Hkv, 1)
+        s = (q @ k.transpose(-1, -2) * D ** -0.5).masked_fill(~mask, float("-inf"))
+        a = (s.softmax(-1) @ v).transpose(1, 2).reshape(B, P + L, C)
+        h = h + f(p["g1"]) * rms(lin(a, p["out"]), p["post1"])
+        z = lin(F.gelu(lin(rms(h, p["pre2"]), p["fc1"]), approximate="tanh"), p["fc2"])
+        h = h + f(p["g2"]) * rms(z, p["post2"])
+        y = rms(h, p["pre"])
+    return y[:, P:]

@@ -543,15 +543,20 @@ class LoraAdapters:
         ranks = [u.shape[0] for u in a]
         R = max(16, -(-max(ranks) // 16) * 16)
         self.n, self.k, self.rank, self.count = N, K, R, len(a)
-        self.a = torch.zeros((len(a), R, K), dtype=torch.bfloat16, device=dev)
-        self.b = torch.zeros((len(a), N, R), dtype=torch.bfloat16, device=dev)
-        torch._foreach_copy_([self.a[i, :r] for i, r in enumerate(ranks)], a)
-        torch._foreach_copy_([self.b[i, :, :r] for i, r in enumerate(ranks)], b)
+        # One gather each: the ranks of all adapters side by side, and a zero one for the padding.
+        starts = np.cumsum([0, *ranks])
+        idx = np.full((len(a), R), starts[-1])
+        for i, r in enumerate(ranks):
+            idx[i, :r] = np.arange(starts[i], starts[i + 1])
+        idx = torch.from_numpy(idx.reshape(-1)).to(dev)
+        self.a = torch.cat([*a, a[0].new_zeros(1, K)]).to(torch.bfloat16)[idx].view(-1, R, K)
+        bs = torch.cat([*b, b[0].new_zeros(N, 1)], 1).to(torch.bfloat16)
+        self.b = bs[:, idx].view(N, -1, R).transpose(0, 1).contiguous()
         self.scales = torch.tensor(scales, dtype=torch.float32, device=dev)
         self.ranks = torch.tensor(ranks, dtype=torch.int32, device=dev)
         # A row of another request meets these weights multiplied by zero.
-        if not all(np.isfinite(scales)) or \
-                not bool(torch.isfinite(self.a).all() & torch.isfinite(self.b).all()):
+        largest = torch.maximum(*(torch.linalg.vector_norm(t, float("inf")) for t in (self.a, self.b)))
+        if not np.isfinite(np.asarray([*scales, float(largest)], np.float32)).all():
             raise ValueError("LoraAdapters: weights and scales must be finite")
         self._desc = tuple(map(packed, (self.a, self.b, self.scales, self.ranks)))
 

@@ -132,3 +132,54 @@ def test_trellis_slat_stack_matches_reference(pkg, ops, dev, attn):
     ref = F.linear(F.layer_norm(x, (C,), eps=1e-5).view(N, C), f(m.out_layer[0]), f(m.out_layer[1]))
     assert out.shape == (N, 32)
     assert rel_l2(out, ref) < 2e-2
+
+
+def _shared_context(dev, P, B, L):
+    import torch
+
+    from candle3d_b200 import blocks
+
+    m = blocks.SharedContextBlocks(device=dev)
+    g = torch.Generator().manual_seed(P)
+    tokens = torch.randn(P, m.C, generator=g).to(dev, torch.bfloat16)
+    x = torch.randn(B, L, m.C, generator=g).to(dev, torch.bfloat16)
+    ids = torch.tensor([b % 4 if b % 4 < 3 else -1 for b in range(B)], dtype=torch.int32, device=dev)
+    cache = m.new_cache(B, L + 9)
+    for k, v in cache:  # what lies past a request's own tokens must not matter
+        k.fill_(float("nan"))
+        v.fill_(float("nan"))
+    return m, x, ids, m.encode_context(tokens), cache, blocks.shared_context_reference(m, x, tokens, ids)
+
+
+@pytest.mark.parametrize("P,steps,B", [(200, (5, 1, 1, 3), 4), (64, (1, 1), 1), (1000, (33, 1), 7)])
+def test_shared_context_blocks_match_reference(pkg, dev, P, steps, B):
+    """Requests with adapters of their own around one context, their tokens in
+    steps through the caches, against whole sequences at once in f64."""
+    import torch
+
+    m, x, ids, context, cache, ref = _shared_context(dev, P, B, sum(steps))
+    outs, at = [], 0
+    for n in steps:
+        start = torch.full((B,), at, dtype=torch.int32, device=dev)
+        outs.append(m.forward(x[:, at:at + n].contiguous(), context, cache, start, ids))
+        at += n
+    assert rel_l2(torch.cat(outs, 1), ref) < 2e-2
+
+
+def test_shared_context_blocks_ragged_requests(pkg, dev):
+    """Requests that join with different numbers of tokens, then step together."""
+    import torch
+
+    have = [1, 17, 4, 30, 8]
+    m, x, ids, context, cache, ref = _shared_context(dev, 300, len(have), 32)
+    for b, n in enumerate(have):
+        own = [(k[b:b + 1], v[b:b + 1]) for k, v in cache]
+        y = m.forward(x[b:b + 1, :n].contiguous(), context, own,
+                      torch.zeros(1, dtype=torch.int32, device=dev), ids[b:b + 1])
+        assert rel_l2(y, ref[b:b + 1, :n]) < 2e-2
+    start = torch.tensor(have, dtype=torch.int32, device=dev)
+    for _ in range(2):
+        rows = torch.arange(len(have), device=dev)
+        y = m.forward(x[rows, start.long()].unsqueeze(1), context, cache, start, ids)
+        assert rel_l2(y[:, 0], ref[rows, start.long()]) < 2e-2
+        start = start + 1
