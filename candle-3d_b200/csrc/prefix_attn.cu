@@ -50,12 +50,6 @@ constexpr float RESCALE_LOG2 = 8.f;
 
 __device__ int g_pattn_status;
 
-#ifndef POLY64
-#define POLY64 2
-#endif
-#ifndef POLY128
-#define POLY128 1
-#endif
 // NT row tiles of 128 rows per block; NT = 1 blocks share an SM in pairs, for
 // short items, whose set-up one block's work then hides for the other.
 template <int D, int NT>
@@ -74,7 +68,10 @@ struct Cfg {
   static constexpr uint32_t COL_S = 0, COL_O = NT * 2 * BKV;
   static constexpr uint32_t TMEM_COLS = COL_O + NT * D <= 256 ? 256 : 512;
   static constexpr int THREADS = (4 + 4 * NT) * 32;   // TMA and MMA warps, softmax warps
-  static constexpr int POLY = D == 64 ? POLY64 : POLY128;  // of 8 pairs of P, those of ex2_poly2
+  // Of 8 pairs of P, those of ex2_poly2 (it takes twice ex2's time, on other units).
+  // 0, 1, 2 of them: 37 heads x 1024 x 4096 at D 64 70, 66, 64 us; at D 128 1370
+  // keys for 8 x 16 heads x 2049 rows 240 us without, 225 with one (and with two).
+  static constexpr int POLY = D == 64 ? 2 : 1;
   static_assert(COL_O + NT * D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
   static_assert((2 * BUFS + 7 * NT) * 8 + 16 <= REST, "barrier area");
 };
@@ -607,41 +604,62 @@ struct Plan {
   int nt, joint, tiles_p, tiles_o, chunk_p, chunk_o, slots_p, slots, items;
 };
 
-static Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t P, int64_t S) {
+// The plan with the least estimated time: one or two row tiles per block, the
+// prefix for the rows of the whole batch (packed) or of each element (joint),
+// and some lengths of an item.  An item of `len` key tiles takes about
+//   D = 128: 5.5 + 1.00 len us (one row tile, two blocks per SM), 7.5 + 0.96 len (two),
+//   D = 64:  2.0 + 0.89 len us,                                   2.5 + 0.87 len,
+// fitted to 37 heads x 1024 rows x 256 .. 16384 keys; a call takes 5 us besides, and
+// parts 3 us and their bytes.  Measured, with the estimate behind it:
+//   8 x 16 heads x 2049 rows, 1370 keys, D 128: one tile 194 us (197), two 225 (234);
+//   8 x 16 heads x 300 rows, 1370 + 300 keys, D 128: joint 66 us (70), packed 86 (84);
+//   64 x 4 key heads x 4 rows, 32768 + 512 keys: packed 41 us, joint 428.
+static Plan make_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t N, int64_t P, int64_t S, int64_t D) {
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  const int64_t RG = N * (Hq / Hkv), F = B * RG;
-  const int64_t kp = up(P, BKV), ko = up(S, BKV);
-  Plan pl{};
-  // One row tile per block while an element's rows fit it.
-  pl.nt = RG <= BQ && (S > 0 || F <= BQ) ? 1 : 2;
-  const int64_t rows = int64_t(pl.nt) * BQ;
-  pl.tiles_p = int(up(F, rows));
-  pl.tiles_o = int(up(RG, rows));
-  // Packed rows share the prefix between elements; joint items need no parts.
-  // Work in (row tile) x (key tile):
-  const int64_t packed = Hkv * (pl.tiles_p * kp + B * pl.tiles_o * ko);
-  const int64_t joint = Hkv * B * pl.tiles_o * (kp + ko);
-  pl.joint = S > 0 && joint * 10 <= packed * 11;
-  const int64_t work = pl.joint ? joint : packed;
-  int64_t chunk = up(work, int64_t(sm_count()) * (pl.nt == 1 ? 2 : 1));
-  if (chunk < 2) chunk = 2;
-  const int64_t kmax = pl.joint ? kp + ko : kp > ko ? kp : ko;
-  const int64_t half = MAX_SLOTS / 2;
-  if (chunk * half < kmax) chunk = up(kmax, half);
-  if (pl.joint) {
-    pl.chunk_o = int(chunk);
-    pl.slots = int(up(kp + ko, chunk));
-    if (pl.slots < 1) pl.slots = 1;
-    pl.items = int(Hkv * B * pl.tiles_o * pl.slots);
-  } else {
-    pl.chunk_p = pl.chunk_o = int(chunk);
-    pl.slots_p = int(up(kp, chunk));
-    const int64_t so = up(ko, chunk);
-    if (pl.slots_p + so < 1) pl.slots_p = 1;
-    pl.slots = pl.slots_p + int(so);
-    pl.items = int(Hkv * (pl.tiles_p * pl.slots_p + B * pl.tiles_o * so));
+  const int64_t RG = N * (Hq / Hkv), F = B * RG, kp = up(P, BKV), ko = up(S, BKV), half = MAX_SLOTS / 2;
+  Plan best{};
+  double least = 1e300;
+  for (int nt = 1; nt <= 2; ++nt) {
+    const double fixed = D == 64 ? (nt == 1 ? 2.0 : 2.5) : nt == 1 ? 5.5 : 7.5;
+    const double tile = D == 64 ? (nt == 1 ? 0.89 : 0.87) : nt == 1 ? 1.0 : 0.96;
+    const double cap = double(sm_count()) * (nt == 1 ? 2 : 1);
+    const int64_t tp = up(F, nt * BQ), to = up(RG, nt * BQ);
+    if (nt == 2 && F <= BQ) break;  // the second tile would be empty
+    for (int joint = 0; joint <= (S > 0 ? 1 : 0); ++joint) {
+      const int64_t kmax = joint ? kp + ko : kp > ko ? kp : ko;
+      const double work = double(Hkv) * (joint ? double(B * to) * double(kp + ko) : double(tp) * double(kp) + double(B * to) * double(ko));
+      const int64_t even = int64_t(work / cap) + 1;
+      for (const int64_t want : {kmax, even, even + even / 4 + 1}) {  // whole, or a device's worth
+        int64_t chunk = want < 2 ? 2 : want;
+        if (chunk * half < kmax) chunk = up(kmax, half);
+        Plan pl{nt, joint, int(tp), int(to), joint ? 0 : int(chunk), int(chunk), 0, 0, 0};
+        double time, items, longest;
+        if (joint) {
+          pl.slots = kmax > 0 ? int(up(kmax, chunk)) : 1;
+          items = double(Hkv * B * to) * pl.slots;
+          longest = fixed + tile * double(chunk < kmax ? chunk : kmax);
+          time = ceil(items / cap) * longest;
+        } else {
+          const int so = int(up(ko, chunk));
+          pl.slots_p = kp > 0 || so == 0 ? int(kp > 0 ? up(kp, chunk) : 1) : 0;
+          pl.slots = pl.slots_p + so;
+          const double np = double(Hkv * tp) * pl.slots_p, no = double(Hkv * B * to) * so;
+          const double lp = fixed + tile * double(chunk < kp ? chunk : kp), lo = fixed + tile * double(chunk < ko ? chunk : ko);
+          items = np + no;
+          longest = np > 0 && (no == 0 || lp > lo) ? lp : lo;
+          time = np == 0 || no == 0 ? ceil(items / cap) * longest : (np * lp + no * lo) / cap + 0.5 * longest;
+          if (time < longest) time = longest;
+        }
+        if (pl.slots > 1) time += 3.0 + double(pl.slots) * double(Hkv * F) * double(D) * 8.0 / 8e6;
+        if (time < least * 0.999 && items < 2147483648.0) {
+          least = time;
+          best = pl;
+          best.items = int(items);
+        }
+      }
+    }
   }
-  return pl;
+  return best;
 }
 
 template <typename T, int D, int NT>
@@ -698,7 +716,7 @@ extern "C" size_t l3d_shared_prefix_attention_workspace_size(int64_t b, int64_t 
                                                              int64_t n, int64_t p, int64_t s,
                                                              int64_t d) {
   if (b <= 0 || hq <= 0 || hkv <= 0 || n <= 0 || p < 0 || s < 0 || d <= 0 || hq % hkv) return 0;
-  const l3d::pattn::Plan pl = l3d::pattn::make_plan(b, hq, hkv, n, p, s);
+  const l3d::pattn::Plan pl = l3d::pattn::make_plan(b, hq, hkv, n, p, s, d);
   // O and the log2 sums of each row's parts, in f32.
   return pl.slots > 1 ? size_t(pl.slots) * size_t(b) * size_t(hq) * size_t(n) * (size_t(d) + 1) * 4 : 0;
 }
@@ -772,7 +790,7 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
       if (t->dims[d] > 1 && t->strides[d] % 8)
         return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
   }
-  const Plan pl = make_plan(B, Hq, Hkv, N, P, S);
+  const Plan pl = make_plan(B, Hq, Hkv, N, P, S, D);
   Params p{};
   p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);
   p.RG = int(N * p.G); p.F = int(B) * p.RG;
