@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(256, 1) shrink_kernel(const Params p) {
 // t for many rows, on the 5th-generation tensor cores: a block per 128-row tile,
 // two blocks per SM, and for each distinct adapter of the tile one product of
 // the tile with A_a (M 128, N R, K in steps of 64 by TMA).  31569 x 1536, rank
-// 64: 70 us by mma.sync (its loads, straight to registers, are the limit).
+// 64: about 20 us, and 70 by mma.sync (its loads, straight to registers, are the limit).
 //   warp 0 TMA, warp 1 MMA, warps 2..5 the tile's adapters and the epilogue
 struct ShrinkTc {
   int stages, tmem;
@@ -382,7 +382,8 @@ constexpr int THREADS = 14 * 32;
 template <int BN>
 struct Cfg {
   // Blocks of 64 along K per stage: two for the narrow tiles of few rows, which
-  // wait for memory (whole 256-byte pieces of a weight row, half the barriers).
+  // wait for memory (whole 256-byte pieces of a weight row, half the barriers):
+  // 16 x 2048 -> 2048 10.1 us, one 12.4; 64 x 2048 -> 8192 27.3 us, one 30.4.
   static constexpr int KS = BN <= 64 ? 2 : 1;
   static constexpr int A_STAGE = KS * A_BYTES;
   static constexpr int B_BYTES = BN * BK * 2;
@@ -410,7 +411,11 @@ __device__ __forceinline__ uint64_t smem_desc_sw32(const void* tile) {
   return d;
 }
 
-// RES: there is a residual.
+// RES: there is a residual (kept out of the registers of the other form, which
+// would spill).  Bound for few rows by the weight's bytes and the launches: 64 x
+// 2048 -> 8192, 32 adapters 27 us (the weight alone 5 us at the copy rate); for
+// many by the loads of a K step, 48 KB of L2 per 2.1 MFLOP x 2: 31569 x 1536 -> 8192,
+// rank 64 704 us in all (1155 TFLOP/s, 70% of a plain product's rate).
 template <int BN, bool RES>
 __global__ void __launch_bounds__(THREADS, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -869,6 +874,10 @@ static cudaError_t launch_gemm(const CUtensorMap& mx, const void* w, int64_t w_l
 
 // The tile width with the least estimated time: rounds of the device x the K
 // steps of a tile, each as long as its products (2 BN clocks) or its loads.
+// Measured (us) for widths 32, 64, 128, 256:
+//   16 x 2048 -> 2048     10.1   10.3   12.9   16.1     64 x 2048 -> 8192  42.6  27.3  28.9  35.7
+//   512 x 1024 -> 4096    25.4   20.0   17.7   21.5   4098 x 2048 -> 2048  94.2  64.7  53.1  47.1
+//   31569 x 1536 -> 8192  1834   1114    827    705
 static int pick_bn(int64_t M, int64_t N) {
   int best = 256;
   double least = 1e300;

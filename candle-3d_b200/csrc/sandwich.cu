@@ -27,7 +27,7 @@ struct Params {
   int norm;
 };
 
-constexpr int kBlock = 256;
+constexpr int kRowBlock = 1024, kBlock = 256;
 
 __device__ __forceinline__ float block_sum(float v, float* red) {
 #pragma unroll
@@ -37,7 +37,7 @@ __device__ __forceinline__ float block_sum(float v, float* red) {
   __syncthreads();
   float s = 0.f;
 #pragma unroll
-  for (int i = 0; i < kBlock / 32; ++i) s += red[i];
+  for (int i = 0; i < kRowBlock / 32; ++i) s += red[i];
   __syncthreads();
   return s;
 }
@@ -55,11 +55,11 @@ __device__ __forceinline__ void block_stats(int norm, const float* s, int64_t C,
   mean = 0.f;
   if (norm == NORM_LAYER) {
     float a = 0.f;
-    for (int64_t c = threadIdx.x; c < C; c += kBlock) a += s[c];
+    for (int64_t c = threadIdx.x; c < C; c += kRowBlock) a += s[c];
     mean = block_sum(a, red) / float(C);
   }
   float q = 0.f;
-  for (int64_t c = threadIdx.x; c < C; c += kBlock) {
+  for (int64_t c = threadIdx.x; c < C; c += kRowBlock) {
     const float d = s[c] - mean;
     q = fmaf(d, d, q);
   }
@@ -67,21 +67,22 @@ __device__ __forceinline__ void block_stats(int norm, const float* s, int64_t C,
 }
 
 // One row per block at a time, the row held in shared memory as f32; any
-// row length, alignment and strides.
+// row length, alignment and strides.  Bound by its element-wise accesses and the
+// waits between its passes: 4096 x 16384 bf16 501 us (1.1 TB/s; 256 threads 1145).
 template <typename T>
-__global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
+__global__ void __launch_bounds__(kRowBlock, 2) row_kernel(const Params p) {
   extern __shared__ float s[];
-  __shared__ float red[kBlock / 32];
+  __shared__ float red[kRowBlock / 32];
   for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
     const int64_t b = row / p.rows_per_batch;
     const T* xr = static_cast<const T*>(p.x) + row_offset(p.xm, row);
     const T* hr = static_cast<const T*>(p.h) + row_offset(p.hm, row);
-    for (int64_t c = threadIdx.x; c < p.C; c += kBlock) s[c] = to_f(hr[c]);
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowBlock) s[c] = to_f(hr[c]);
     __syncthreads();
     float mean, inv;
     block_stats(p.norm, s, p.C, p.post_eps, red, mean, inv);
     T* rr = static_cast<T*>(p.r) + row_offset(p.rm, row);
-    for (int64_t c = threadIdx.x; c < p.C; c += kBlock) {
+    for (int64_t c = threadIdx.x; c < p.C; c += kRowBlock) {
       const float n = (s[c] - mean) * inv * chan_or(p.pw, 0, c, 1.f) + chan_or(p.pb, 0, c, 0.f);
       const float r = fmaf(chan_or(p.gate, b, c, 1.f), n, p.res_scale * to_f(xr[c]));
       rr[c] = from_f<T>(r);
@@ -91,7 +92,7 @@ __global__ void __launch_bounds__(kBlock) row_kernel(const Params p) {
     if (p.y) {
       block_stats(p.norm, s, p.C, p.eps, red, mean, inv);
       T* yr = static_cast<T*>(p.y) + row_offset(p.ym, row);
-      for (int64_t c = threadIdx.x; c < p.C; c += kBlock) {
+      for (int64_t c = threadIdx.x; c < p.C; c += kRowBlock) {
         const float n = (s[c] - mean) * inv * chan_or(p.w, 0, c, 1.f) + chan_or(p.b, 0, c, 0.f);
         yr[c] = from_f<T>(fmaf(n, 1.f + chan_or(p.scale, b, c, 0.f), chan_or(p.shift, b, c, 0.f)));
       }
@@ -269,20 +270,24 @@ __device__ __forceinline__ bool unit_all(bool ok) {
 // a contiguous range of rows each, worked through by units of max(G, 32)
 // threads.  G threads hold a row's h in registers as f32 (64 elements a thread,
 // 32 of f32 rows), and r in its place; G = 8 puts four rows in a warp.  Each
-// unit keeps kSlots packs of rows (x and h) in shared memory that bulk copies
+// unit keeps two packs of rows (x and h) in shared memory that bulk copies
 // fill ahead of it, so that the loads in flight do not occupy registers; its
 // first thread issues the next copy once the unit has read a slot.
 // Both norms' sums are taken in two passes over the registers (mean, then
 // centred squares: one pass of shifted moments loses digits where one channel
 // lies far out).
+// Bound by memory: 131072 x 2048 bf16 takes 376 us (5.7 TB/s, 87% of a plain copy).
+// G and NV by the row's length, bf16: 65536 x 256 takes 34 us with 8 threads a row
+// and 4 vectors a thread, 41 with 8 and 8, 56 with 32 and 4; 65536 x 1024 102 us with
+// 32 and 4, 120 with 32 and 8; 8192 x 8192 117 us with 128 and 8, 169 with 256 and 4.
 // Threads of a block: 12 warps of 168 registers for 8 vectors a thread, 20 of 96
 // for rows of half that length.
 constexpr int threads_of(int nv) { return nv == 8 ? 384 : 640; }
-constexpr int kSlots = 2;
 
 struct Ring {
   int64_t rows_per_batch;  // rows that share per-batch vectors (all, without such vectors)
   int units;               // per block
+  int slots;               // of a unit: 2, or 1
   uint32_t row_bytes;
   uint64_t wait_ns;
 };
@@ -299,28 +304,28 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
   float* coef = reinterpret_cast<float*>(smem);
   uint8_t* slots = smem + size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
   const uint32_t slot_bytes = 2 * RPU * sp.row_bytes;    // the pack's h rows, then its x rows
-  uint64_t* full = reinterpret_cast<uint64_t*>(slots + size_t(sp.units) * kSlots * slot_bytes);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + sp.units * kSlots);
+  uint64_t* full = reinterpret_cast<uint64_t*>(slots + size_t(sp.units) * sp.slots * slot_bytes);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(full + sp.units * sp.slots);
   const int unit = threadIdx.x / U, tu = threadIdx.x % U;
   const int t = threadIdx.x % G, sub = tu / G;           // thread of the row, row of the pack
   const int nvec = int(p.C) / VEC;
   const int64_t lo = p.rows * blockIdx.x / gridDim.x, hi = p.rows * (blockIdx.x + 1) / gridDim.x;
   const int64_t packs = (hi - lo + RPU - 1) / RPU;       // pack k: rows lo + k RPU ..
   if (threadIdx.x == 0) {
-    for (int i = 0; i < sp.units * kSlots; ++i) ring_bar_init(&full[i], 2 * RPU);
+    for (int i = 0; i < sp.units * sp.slots; ++i) ring_bar_init(&full[i], 2 * RPU);
     *abort_flag = 0;
     ring_init_fence();
   }
   __syncthreads();
   const bool works = unit < sp.units;                    // the other threads only fold
-  uint8_t* my_slots = slots + size_t(works ? unit : 0) * kSlots * slot_bytes;
-  uint64_t* my_full = full + (works ? unit : 0) * kSlots;
-  // The unit's n-th pack (pack n units + unit) into slot n % kSlots.
+  uint8_t* my_slots = slots + size_t(works ? unit : 0) * sp.slots * slot_bytes;
+  uint64_t* my_full = full + (works ? unit : 0) * sp.slots;
+  // The unit's n-th pack (pack n units + unit) into slot n mod slots.
   auto issue = [&](int64_t n) {
     const int64_t k = n * sp.units + unit;
     if (k >= packs) return;
-    uint8_t* slot = my_slots + (n % kSlots) * slot_bytes;
-    uint64_t* bar = &my_full[n % kSlots];
+    uint8_t* slot = my_slots + (n & (sp.slots - 1)) * slot_bytes;
+    uint64_t* bar = &my_full[n & (sp.slots - 1)];
     for (int i = 0; i < RPU; ++i) {
       const int64_t row = lo + k * RPU + i;
       if (row < hi) {
@@ -335,7 +340,7 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
     }
   };
   if (works && tu == 0)
-    for (int n = 0; n < kSlots; ++n) issue(n);
+    for (int n = 0; n < sp.slots; ++n) issue(n);
   const float inv_c = 1.f / float(p.C);
   const float2 rs = f2(p.res_scale);
   int turn = 0;
@@ -361,8 +366,8 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
     for (; works && !dead; ++n) {
       const int64_t row0 = lo + (n * sp.units + unit) * RPU;  // first row of the pack
       if (row0 >= s1) break;
-      const int slot = int(n % kSlots);
-      if (!unit_all<G>(ring_wait(&my_full[slot], uint32_t(n / kSlots) & 1u, abort_flag, sp.wait_ns, false,
+      const int slot = int(n & (sp.slots - 1));
+      if (!unit_all<G>(ring_wait(&my_full[slot], uint32_t(n >> (sp.slots - 1)) & 1u, abort_flag, sp.wait_ns, false,
                                  &g_sandwich_status))) {
         dead = true;
         break;
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
       if (whole) {
         if constexpr (G <= 32) __syncwarp();
         else unit_all<G>(true);
-        if (tu == 0) issue(n + kSlots);
+        if (tu == 0) issue(n + sp.slots);
       }
       if (p.y) {
         iv = stats(p.eps);
@@ -453,21 +458,26 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
   }
   // After an abort no copy may still be in flight when the block exits.
   if (dead && tu == 0)
-    for (int64_t k = n; k < n + kSlots; ++k)
+    for (int64_t k = n; k < n + sp.slots; ++k)
       if (k * sp.units + unit < packs)
-        ring_wait(&my_full[k % kSlots], uint32_t(k / kSlots) & 1u, abort_flag, sp.wait_ns, true, &g_sandwich_status);
+        ring_wait(&my_full[k & (sp.slots - 1)], uint32_t(k >> (sp.slots - 1)) & 1u, abort_flag, sp.wait_ns, true, &g_sandwich_status);
 }
 
-// The element kernel (any alignment): G threads per row, 32 elements a thread,
-// blocks that keep to one batch element.
+// The element kernel (any alignment): G threads per row, NE elements a thread,
+// blocks that keep to one batch element.  Bound by the number of its accesses,
+// an element each: 65536 x 1023 bf16 takes 241 us (2.2 TB/s), where the ring
+// takes 102 for rows of 1024.  NE and G by the row's length: 262144 x 63 takes 119
+// us with 8 elements a thread, 407 with 32; 32768 x 2047 264 us with 64 threads
+// a row, 577 with 256.
 struct Blocks {
   int64_t rows, rows_per_block;  // of a batch element
   int per_batch;
 };
-template <typename T, int G, int NORM>
-__global__ void __launch_bounds__(kBlock, 2)
+constexpr int elem_blocks(int ne) { return ne == 8 ? 6 : 2; }  // per SM
+template <typename T, int G, int NE, int NORM>
+__global__ void __launch_bounds__(kBlock, elem_blocks(NE))
     elem_kernel(const Params p, const Coefs kc, const Blocks sp) {
-  constexpr int NE = 32, RPB = kBlock / G;
+  constexpr int RPB = kBlock / G;
   extern __shared__ __align__(16) float coef[];
   __shared__ float red[40];
   const int t = threadIdx.x % G, C = int(p.C);
@@ -485,9 +495,13 @@ __global__ void __launch_bounds__(kBlock, 2)
     const T* xs = static_cast<const T*>(p.x) + row_offset32(p.xm, at);
     T* rd = static_cast<T*>(p.r) + row_offset32(p.rm, at);
     T* yd = p.y ? static_cast<T*>(p.y) + row_offset32(p.ym, at) : nullptr;
-    float f[NE];
+    // Both rows' loads at once (a load of x in the loop below would wait for the
+    // stores before it: 65536 x 1024 bf16 took 476 us that way).
+    float f[NE], x[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) f[i] = t + i * G < C ? to_f(hs[t + i * G]) : 0.f;
+#pragma unroll
+    for (int i = 0; i < NE; ++i) x[i] = t + i * G < C ? to_f(xs[t + i * G]) : 0.f;
     float nm = 0.f;
     auto stats = [&](float eps) {
       if constexpr (NORM == NORM_LAYER) {
@@ -509,7 +523,7 @@ __global__ void __launch_bounds__(kBlock, 2)
     for (int i = 0; i < NE; ++i) {
       const int c = t + i * G;
       if (c >= C) continue;
-      const float base = fmaf(p.res_scale, to_f(xs[c]), kc.has_b1 ? b1[c] : 0.f);
+      const float base = fmaf(p.res_scale, x[i], kc.has_b1 ? b1[c] : 0.f);
       f[i] = fmaf(a1[c], (f[i] + nm) * iv, base);
       rd[c] = from_f<T>(f[i]);
     }
@@ -545,7 +559,11 @@ constexpr const char* kNoSmem = "l3d_sandwich_residual_norm: cannot reserve shar
 template <typename T, int G, int NV, int NORM>
 static int launch_ring(const Params& p, const Coefs& kc, Ring sp, size_t coef, cudaStream_t s) {
   constexpr int U = G < 32 ? 32 : G, RPU = U / G;
-  const size_t slot = size_t(kSlots) * (2 * RPU * sp.row_bytes + 8);
+  // One slot, not filled ahead, where two do not fit: 8192 x 8192 f32 with
+  // all vectors takes 205 us so, 1170 with a block per row.
+  size_t slot = 2 * (size_t(2) * RPU * sp.row_bytes + 8);
+  sp.slots = coef + slot + 16 > size_t(kSmem) ? 1 : 2;
+  if (sp.slots == 1) slot /= 2;
   if (coef + slot + 16 > size_t(kSmem)) return 0;
   auto k = ring_kernel<T, G, NV, NORM>;
   if (set_smem_limit(reinterpret_cast<const void*>(k), kSmem) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
@@ -560,17 +578,17 @@ static int launch_ring(const Params& p, const Coefs& kc, Ring sp, size_t coef, c
   return 1;
 }
 
-template <typename T, int G, int NORM>
+template <typename T, int G, int NE, int NORM>
 static int launch_elem(const Params& p, const Coefs& kc, int64_t batches, size_t coef, cudaStream_t s) {
   constexpr int RPB = kBlock / G;
   if (coef > 100 * 1024) return 0;
-  auto k = elem_kernel<T, G, NORM>;
+  auto k = elem_kernel<T, G, NE, NORM>;
   if (set_smem_limit(reinterpret_cast<const void*>(k), 100 * 1024) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
   Blocks sp{};
   sp.rows = p.rows / batches;
   // Two waves of blocks, shared out between the batch elements.
   const int64_t most = (sp.rows + RPB - 1) / RPB;
-  int64_t per = int64_t(sm_count()) * 4 / batches;
+  int64_t per = int64_t(sm_count()) * 2 * elem_blocks(NE) / batches;
   per = per < 1 ? 1 : per > most ? most : per;
   sp.rows_per_block = ((sp.rows + per - 1) / per + RPB - 1) / RPB * RPB;
   sp.per_batch = int((sp.rows + sp.rows_per_block - 1) / sp.rows_per_block);
@@ -607,8 +625,11 @@ static int try_fast(const Params& p, bool vec_ok, bool chan_vec, int64_t batches
                    : p.C <= 256 * E ? launch_ring<T, 256, 8, NORM>(p, kc, sp, coef, s) : 0;
     if (rc) return rc;
   }
-  return p.C <= 32 * 32 ? launch_elem<T, 32, NORM>(p, kc, batches, coef, s)
-         : p.C <= 256 * 32 ? launch_elem<T, 256, NORM>(p, kc, batches, coef, s) : 0;
+  return p.C <= 32 * 8 ? launch_elem<T, 32, 8, NORM>(p, kc, batches, coef, s)
+         : p.C <= 32 * 32 ? launch_elem<T, 32, 32, NORM>(p, kc, batches, coef, s)
+         : p.C <= 64 * 32 ? launch_elem<T, 64, 32, NORM>(p, kc, batches, coef, s)
+         : p.C <= 128 * 32 ? launch_elem<T, 128, 32, NORM>(p, kc, batches, coef, s)
+         : p.C <= 256 * 32 ? launch_elem<T, 256, 32, NORM>(p, kc, batches, coef, s) : 0;
 }
 
 template <typename T>
@@ -621,7 +642,7 @@ static int launch(const Params& p, bool vec_ok, bool chan_vec, int64_t batches, 
   if (set_smem_limit(reinterpret_cast<const void*>(k), int(kMaxC * 4)) != cudaSuccess)
     return fail(L3D_E_CUDA, "l3d_sandwich_residual_norm: cannot reserve shared memory");
   const int64_t cap = int64_t(sm_count()) * 8;
-  k<<<unsigned(p.rows < cap ? p.rows : cap), kBlock, size_t(p.C) * 4, s>>>(p);
+  k<<<unsigned(p.rows < cap ? p.rows : cap), kRowBlock, size_t(p.C) * 4, s>>>(p);
   return L3D_OK;
 }
 
