@@ -30,10 +30,10 @@
 // tensor core nor the softmax warps wait for a whole round trip of the other.
 // (With one 128-column buffer a row tile's softmax warps waited 1,500 of 3,830
 // clocks per 128 keys at D = 128, and both pipes were about half busy.)
-// Long items are bound by the round trip between the products and the softmax
-// (D = 128: 1234 TFLOP/s over 16384 keys, 75% of a plain product's rate; without the
-// softmax 1455) at D = 128, at D = 64 by the exponentials and conversions (694
-// TFLOP/s); short ones by an item's set-up and the rounds over the device.
+// Long items are bound at D = 128 by the round trip between the products and the
+// softmax (1234 TFLOP/s over 16384 keys, 75% of a plain product's rate; 1455 without
+// the softmax), at D = 64 by the softmax itself (694 TFLOP/s); short ones by an item's
+// set-up and the rounds over the device.
 // Every mbarrier wait is bounded (%globaltimer, 2 s); on expiry the block
 // records an error in the device's status word and stops.
 #include <type_traits>
@@ -536,7 +536,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
   }
 }
 
-// One token of 64 x 16 heads, 22 parts: about 3 us.  The parts of each row weighed by 2^(their log2 sum - the largest): a block of
+// Bound by the parts' bytes.  The parts of each row weighed by 2^(their log2 sum - the largest): a block of
 // four warps per row, each with every fourth part, D / 32 elements per lane;
 // added up in a fixed order.
 constexpr int MAX_SLOTS = 64;

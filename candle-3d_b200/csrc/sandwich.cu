@@ -108,7 +108,8 @@ __global__ void __launch_bounds__(kRowBlock, 2) row_kernel(const Params p) {
 struct Coefs {
   int has_b1, has_b2;
   int ld;                  // floats of a coefficient row (a multiple of 4)
-  int chan_vec;            // the vectors are 16-byte aligned, and 2: of the activations' type
+  int chan_vec;            // the vectors are 16-byte aligned
+  int same;                // and of the activations' type
 };
 
 // Place of channel c in a coefficient row read in vectors of VEC: in planes of
@@ -127,7 +128,7 @@ __device__ __forceinline__ void fold(const Params& p, const Coefs& k, float* coe
   float* row = coef;
   float *a1 = row, *a2 = row + k.ld, *b1 = row + 2 * k.ld, *b2 = row + (2 + k.has_b1) * k.ld;
   if constexpr (VEC > 1) {
-    if (k.chan_vec == 2) {
+    if (k.chan_vec && k.same) {
       // All vectors' loads at once (without branches between them): this is what
       // a call on a few rows waits for.
       for (int c = int(threadIdx.x) * VEC; c < C; c += int(blockDim.x) * VEC) {
@@ -158,6 +159,33 @@ __device__ __forceinline__ void fold(const Params& p, const Coefs& k, float* coe
           *reinterpret_cast<float4*>(a2 + at) = four(1);
           if (k.has_b1) *reinterpret_cast<float4*>(b1 + at) = four(2);
           if (k.has_b2) *reinterpret_cast<float4*>(b2 + at) = four(3);
+        }
+      }
+      return;
+    }
+  }
+  if constexpr (VEC == 1) {
+    if (k.same) {  // as above, four channels at once
+      constexpr int U = 4;
+      for (int c0 = threadIdx.x; c0 < C; c0 += U * int(blockDim.x)) {
+        const ChanVec* const vecs[7] = {&p.gate, &p.pw, &p.pb, &p.scale, &p.w, &p.b, &p.shift};
+        T raw[7][U];
+#pragma unroll
+        for (int i = 0; i < 7; ++i)
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            raw[i][u] = vecs[i]->ptr ? __ldg(static_cast<const T*>(vecs[i]->ptr) + b * vecs[i]->bstride +
+                                             min(c0 + u * int(blockDim.x), C - 1))
+                                     : from_f<T>(0.f);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int c = c0 + u * int(blockDim.x);
+          if (c >= C) break;
+          const float g = p.gate.ptr ? to_f(raw[0][u]) : 1.f, t = 1.f + to_f(raw[3][u]);
+          a1[c] = g * (p.pw.ptr ? to_f(raw[1][u]) : 1.f);
+          a2[c] = t * (p.w.ptr ? to_f(raw[4][u]) : 1.f);
+          if (k.has_b1) b1[c] = g * to_f(raw[2][u]);
+          if (k.has_b2) b2[c] = fmaf(t, to_f(raw[5][u]), to_f(raw[6][u]));
         }
       }
       return;
@@ -465,10 +493,11 @@ __global__ void __launch_bounds__(threads_of(NV), 1)
 
 // The element kernel (any alignment): G threads per row, NE elements a thread,
 // blocks that keep to one batch element.  Bound by the number of its accesses,
-// an element each: 65536 x 1023 bf16 takes 241 us (2.2 TB/s), where the ring
-// takes 102 for rows of 1024.  NE and G by the row's length: 262144 x 63 takes 119
-// us with 8 elements a thread, 407 with 32; 32768 x 2047 264 us with 64 threads
-// a row, 577 with 256.
+// an element each: 65536 x 1023 bf16 takes 237 us (2.3 TB/s), where the ring
+// takes 102 for rows of 1024; a few rows by the folding (572 x 5252 18 us, 36 with
+// a channel at a time and a second wave of blocks that folds again).  NE and G by
+// the row's length: 262144 x 63 takes 121 us with 8 elements a thread, 407 with 32;
+// 32768 x 2047 243 us with 64 threads a row, 577 with 256.
 struct Blocks {
   int64_t rows, rows_per_block;  // of a batch element
   int per_batch;
@@ -586,9 +615,9 @@ static int launch_elem(const Params& p, const Coefs& kc, int64_t batches, size_t
   if (set_smem_limit(reinterpret_cast<const void*>(k), 100 * 1024) != cudaSuccess) return -fail(L3D_E_CUDA, "%s", kNoSmem);
   Blocks sp{};
   sp.rows = p.rows / batches;
-  // Two waves of blocks, shared out between the batch elements.
+  // One wave of blocks, shared out between the batch elements.
   const int64_t most = (sp.rows + RPB - 1) / RPB;
-  int64_t per = int64_t(sm_count()) * 2 * elem_blocks(NE) / batches;
+  int64_t per = int64_t(sm_count()) * elem_blocks(NE) / batches;
   per = per < 1 ? 1 : per > most ? most : per;
   sp.rows_per_block = ((sp.rows + per - 1) / per + RPB - 1) / RPB * RPB;
   sp.per_batch = int((sp.rows + sp.rows_per_block - 1) / sp.rows_per_block);
@@ -605,10 +634,9 @@ static int try_fast(const Params& p, bool vec_ok, bool chan_vec, int64_t batches
   kc.ld = int((p.C + 7) & ~int64_t(7));
   kc.chan_vec = chan_vec;
   const int dt = std::is_same<T, float>::value ? L3D_F32 : std::is_same<T, __half>::value ? L3D_F16 : L3D_BF16;
-  bool same = chan_vec;
+  kc.same = 1;
   for (const ChanVec* v : {&p.gate, &p.pw, &p.pb, &p.scale, &p.w, &p.b, &p.shift})
-    if (v->ptr && v->dtype != dt) same = false;
-  if (same) kc.chan_vec = 2;
+    if (v->ptr && v->dtype != dt) kc.same = 0;
   const size_t coef = size_t(2 + kc.has_b1 + kc.has_b2) * kc.ld * 4;
   if (vec_ok) {
     Ring sp{};
