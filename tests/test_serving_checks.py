@@ -90,8 +90,8 @@ def _prefix_args(**over):
     (dict(scale=0.0), E_UNSUPPORTED, "scale"),
     (dict(scale=math.nan), E_UNSUPPORTED, "scale"),
     (dict(scale=math.inf), E_UNSUPPORTED, "scale"),
-    (dict(bytes=0), E_WORKSPACE, "workspace"),
-    (dict(workspace=264), E_ALIGN, "256"),
+    (dict(prefix_k=_zeros(2, 4096, 64), prefix_v=_zeros(2, 4096, 64), bytes=0), E_WORKSPACE, "workspace"),
+    (dict(prefix_k=_zeros(2, 4096, 64), prefix_v=_zeros(2, 4096, 64), workspace=264), E_ALIGN, "256"),
     (dict(k=_zeros(2, 2, 9, 68)[..., :64]), E_ALIGN, "multiples of 16"),
     (dict(k=_zeros(2, 2, 1, 64).expand(2, 2, 9, 64)), E_ALIGN, "expanded"),
 ])
