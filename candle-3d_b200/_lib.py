@@ -10,10 +10,11 @@ The library is required: importing this module on a machine without the built
 from __future__ import annotations
 
 import ctypes as C
-import struct
 from pathlib import Path
 
 import torch
+
+from . import _l3dpack  # built with the library (host/pack.cpp)
 
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libl3dops.so"
@@ -70,22 +71,8 @@ def ref(d):
     return None if d is None else C.byref(d)
 
 
-_PACK = struct.Struct("=Qii6q6qq").pack
-_PAD = [(0,) * (MAX_DIMS - n) for n in range(MAX_DIMS + 1)]
-
-
-def packed(t: torch.Tensor | None):
-    """As desc, as the descriptor's bytes (None -> NULL), for the entries whose
-    signature takes _D: a third of the time of filling a ctypes structure, which
-    is what a call on a few rows spends its time on."""
-    if t is None:
-        return None
-    shape = t.shape
-    n = len(shape)
-    if n > MAX_DIMS:
-        raise ValueError(f"rank {n} exceeds {MAX_DIMS}")
-    pad = _PAD[n]
-    return _PACK(t.data_ptr(), _TORCH_TO_L3D[t.dtype], n, *shape, *pad, *t.stride(), *pad, 0)
+packed = _l3dpack.packed  # as desc, as the descriptor's bytes (None -> NULL), for signatures with _D
+packs = _l3dpack.packs    # packed of each argument, which must be on a CUDA device
 
 
 _P = C.POINTER(L3dTensor)

@@ -1,4 +1,5 @@
-"""Build libl3dops.so (all CUDA kernels + the C ABI) for sm_100a with nvcc.
+"""Build libl3dops.so (all CUDA kernels + the C ABI) for sm_100a with nvcc, and
+_l3dpack.so (tensor descriptors for the Python front end) with the host compiler.
 
 Objects are compiled in parallel into `_build/` beside this file and linked
 into `libl3dops.so` in the package directory (in-tree, so the library travels
@@ -11,6 +12,7 @@ import concurrent.futures as cf
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -18,6 +20,7 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "libl3dops.so"
+PACK = PKG / "_l3dpack.so"
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xcompiler", "-fvisibility=hidden",
@@ -49,6 +52,24 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _pack_module() -> None:
+    """host/pack.cpp -> _l3dpack.so, against the headers of the installed torch."""
+    src, hdr = PKG / "host" / "pack.cpp", ROOT / "include" / "l3d_ops.h"
+    if PACK.exists() and PACK.stat().st_mtime > max(src.stat().st_mtime, hdr.stat().st_mtime):
+        return
+    import torch
+
+    t = Path(torch.__file__).resolve().parent
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{ROOT / 'include'}",
+           f"-isystem{t / 'include'}", f"-isystem{t / 'include/torch/csrc/api/include'}",
+           f"-isystem{sysconfig.get_paths()['include']}", str(src), "-o", str(PACK), f"-L{t / 'lib'}",
+           "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"{src.name} failed to compile:\n{r.stderr}")
+
+
 def build(verbose: bool = False) -> Path:
     BUILD.mkdir(exist_ok=True)
     srcs = _sources()
@@ -59,6 +80,7 @@ def build(verbose: bool = False) -> Path:
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
             raise RuntimeError(f"link failed:\n{r.stderr}")
+    _pack_module()
     if verbose:
         print(f"built {LIB}")
     return LIB

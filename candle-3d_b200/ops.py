@@ -15,7 +15,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import call, desc, packed, ref, stream_handle, stream_of
+from ._l3dpack import empty, workspace
+from ._lib import call, desc, packed, packs, ref, stream_handle, stream_of
 
 ACT = {"none": 0, "silu": 1, "gelu_erf": 2, "gelu_tanh": 3}
 
@@ -567,18 +568,22 @@ def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, ga
     projection: y = residual + gate * act(x . W^T + bias + s_a B_a A_a x), where
     a = ids[i] for the i-th of ids.numel() equal groups of rows (one id per row,
     or per request); an id outside [0, adapters.count) means no adapter."""
-    _check_cuda(x, weight, ids, bias, residual, gate, out)
     n, k = weight.shape
     x2 = x if x.dim() == 2 else x.reshape(-1, k)
     m = x2.shape[0]
-    y = x.new_empty((m, n), dtype=out_dtype or x.dtype) if out is None else out.view(-1, n)
-    need = _lib.lib().l3d_lora_linear_workspace_size(m, adapters.rank)
-    ws = x.new_empty(need, dtype=torch.uint8)
+    if out is not None:
+        y = out.view(-1, n)
+    elif out_dtype is None:
+        y = empty(x2, m, n)
+    else:
+        y = x.new_empty((m, n), dtype=out_dtype)
     if residual is not None and residual.dim() != 2:
         residual = residual.reshape(-1, n)
-    call("l3d_lora_linear", packed(x2), packed(weight), packed(bias), *adapters._desc, packed(ids),
-         ACT_CODES[act], packed(residual), packed(gate), packed(y), ws.data_ptr(), need,
-         stream_of(x))
+    dx, dw, db, di, dr, dg, dy = packs(x2, weight, bias, ids, residual, gate, y)
+    need = _lib.lib().l3d_lora_linear_workspace_size(m, adapters.rank)
+    ws = workspace(x2, need)
+    call("l3d_lora_linear", dx, dw, db, *adapters._desc, di, ACT_CODES[act], dr, dg, dy,
+         ws.data_ptr(), need, stream_of(x))
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
@@ -590,18 +595,17 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None,
     [B, Hkv, S, D] (lengths None: all S); causal: the rows are the last N of their
     element's own sequence.  BF16 or F16, D = 64 or 128; `out` defaults as in
     `attention`."""
-    _check_cuda(q, prefix_k, prefix_v, k, v, lengths, out)
     B, H, N, D = q.shape
     if out is None:
-        out = q.new_empty((B, N, H, D)).transpose(1, 2)
+        out = empty(q, B, N, H, D).transpose(1, 2)
     Hkv, P = prefix_k.shape[:2]
+    dq, dpk, dpv, dk, dv, dl, do = packs(q, prefix_k, prefix_v, k, v, lengths, out)
     need = _lib.lib().l3d_shared_prefix_attention_workspace_size(
         B, H, Hkv, N, P, 0 if k is None else k.shape[2], D)
-    ws = q.new_empty(need, dtype=torch.uint8) if need else None
-    call("l3d_shared_prefix_attention", packed(q), packed(prefix_k), packed(prefix_v),
-         packed(k), packed(v), packed(lengths), int(bool(causal)),
-         D ** -0.5 if scale is None else float(scale), packed(out),
-         ws.data_ptr() if need else None, need, stream_of(q))
+    ws = workspace(q, need) if need else None
+    call("l3d_shared_prefix_attention", dq, dpk, dpv, dk, dv, dl, int(bool(causal)),
+         D ** -0.5 if scale is None else float(scale), do, ws.data_ptr() if need else None, need,
+         stream_of(q))
     return out
 
 
@@ -616,11 +620,10 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
     y = Norm(r)[*weight][+bias][*(1+scale)+shift]; returns (r, y).  `norm` is
     "rms" or "layer"; next_norm=False (the last block) returns (r, None); with
     inplace=True the residual stream x is updated in place (r is x)."""
-    _check_cuda(x, h, post_weight, post_bias, gate, weight, bias, shift, scale)
-    r = x if inplace else torch.empty_like(x, memory_format=torch.contiguous_format)
-    y = torch.empty_like(x, memory_format=torch.contiguous_format) if next_norm else None
-    call("l3d_sandwich_residual_norm", packed(x), packed(h), NORMS[norm],
-         packed(post_weight), packed(post_bias), packed(gate), float(res_scale),
-         packed(weight), packed(bias), packed(shift), packed(scale),
-         eps if post_eps is None else post_eps, eps, packed(r), packed(y), stream_of(x))
+    r = x if inplace else empty(x)
+    y = empty(x) if next_norm else None
+    dx, dh, dpw, dpb, dg, dw, db, dsh, dsc, dr, dy = packs(x, h, post_weight, post_bias, gate, weight,
+                                                           bias, shift, scale, r, y)
+    call("l3d_sandwich_residual_norm", dx, dh, NORMS[norm], dpw, dpb, dg, float(res_scale), dw, db,
+         dsh, dsc, eps if post_eps is None else post_eps, eps, dr, dy, stream_of(x))
     return r, y
