@@ -879,11 +879,12 @@ static cudaError_t launch_gemm(const CUtensorMap& mx, const void* w, int64_t w_l
 //   512 x 1024 -> 4096    25.4   20.0   17.7   21.5   4098 x 2048 -> 2048  94.2  64.7  53.1  47.1
 //   31569 x 1536 -> 8192  1834   1114    827    705
 static int pick_bn(int64_t M, int64_t N) {
+  const int sms = sm_count();
   int best = 256;
   double least = 1e300;
   for (int bn = 256; bn >= 32; bn /= 2) {
     const int64_t tiles = ((M + BM - 1) / BM) * ((N + bn - 1) / bn);
-    const double rounds = double((tiles + sm_count() - 1) / sm_count());
+    const double rounds = double((tiles + sms - 1) / sms);
     const double step = 2.0 * bn > 200 + 1.0 * bn ? 2.0 * bn : 200 + 1.0 * bn;
     if (rounds * step < least * 0.999) {
       least = rounds * step;
