@@ -747,7 +747,8 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
       return fail(L3D_E_DTYPE, "%s: all tensors BF16 or all F16", op);
     if (t->ndim != nd)
       return fail(L3D_E_SHAPE, "%s: q, k, v, out [B, H, N, D], prefix_k, prefix_v [H, P, D]", op);
-    if (t->strides[nd - 1] != 1) return fail(L3D_E_ALIGN, "%s: the head dim must be contiguous", op);
+    if (numel(t) > 0 && t->strides[nd - 1] != 1)
+      return fail(L3D_E_ALIGN, "%s: the head dim must be contiguous", op);
   }
   const int64_t B = q->dims[0], Hq = q->dims[1], N = q->dims[2], D = q->dims[3];
   const int64_t Hkv = prefix_k->dims[0], P = prefix_k->dims[1], S = k ? k->dims[2] : 0;

@@ -113,6 +113,20 @@ def test_row_counts(ops, dev, N, causal):
     _run(ops, dev, 2, 2, 1, N, 64, 190, 600, [600, 333], causal)
 
 
+@pytest.mark.parametrize("B,Hq,H,N,D,P,S,causal", [
+    (8, 16, 16, 300, 128, 1370, 300, False),   # prefix and own keys in one item
+    (4, 12, 12, 128, 128, 1370, 500, True),
+    (2, 16, 16, 200, 64, 1370, 900, False),    # in parts
+    (8, 4, 4, 2049, 128, 1370, 0, False),      # several rounds of items
+    (20, 4, 2, 40, 64, 9000, 70, True),        # prefix items apart from own ones
+    (3, 4, 4, 1500, 128, 2, 590, True),
+    (5, 8, 1, 33, 64, 0, 333, True),
+])
+def test_divisions_into_items(ops, dev, B, Hq, H, N, D, P, S, causal):
+    lens = [S - (S * b) // B if not causal else max(min(N, S), S - 7 * b) for b in range(B)] if S else None
+    _run(ops, dev, B, Hq, H, N, D, P, S, lens, causal)
+
+
 @pytest.mark.parametrize("dt", ["bf16", "f16"])
 @pytest.mark.parametrize("N", [1, 300])
 def test_rows_without_keys_are_zero(ops, dev, N, dt):

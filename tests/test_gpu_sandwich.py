@@ -86,6 +86,21 @@ def test_sandwich_many_rows(ops, dev, B, T, C, dt):
     _run(ops, dev, B, T, C, "layer", dt, AFFINE)
 
 
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("dt,vdt", [("f32", None), ("bf16", None), ("bf16", "f32")])
+@pytest.mark.parametrize("C", [63, 255, 257, 1023, 1025, 2047, 2049, 4095, 4097, 8191, 8193])
+def test_sandwich_unaligned_row_lengths(ops, dev, C, dt, vdt, kind):
+    """Rows that do not start on 16 bytes: other threads per row from length to length."""
+    _run(ops, dev, 3, 7, C, kind, dt, ADA if kind == "rms" else AFFINE, vdt=vdt)
+
+
+@pytest.mark.parametrize("dt,C", [("f32", 8192), ("bf16", 16384)])
+@pytest.mark.parametrize("vecs", [{"pw": "C", "w": "C"}, {"pw": "C", "pb": "C", "g": "BC", "w": "C", "b": "C", "sc": "BC"}])
+def test_sandwich_rows_that_leave_little_room(ops, dev, dt, C, vecs):
+    """Long rows whose coefficients leave room for one row or two in shared memory."""
+    _run(ops, dev, 2, 170, C, "layer", dt, vecs)
+
+
 def test_sandwich_large_mean(ops, dev):
     """A branch far from zero: the variance is of the centred values."""
     _run(ops, dev, 1, 64, 512, "layer", "f32", {}, mean=100.0)

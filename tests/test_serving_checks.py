@@ -143,3 +143,25 @@ def test_workspace_sizes_without_a_device(pkg):
     assert lib.l3d_lora_linear_workspace_size(-1, 32) == 0
     # An empty batch has nothing to join.
     assert lib.l3d_shared_prefix_attention_workspace_size(0, 8, 2, 5, 1029, 77, 64) == 0
+
+
+def test_descriptors_as_bytes(pkg):
+    """The native descriptors are the ctypes ones; views keep their strides."""
+    import torch
+
+    L = pkg._lib
+    for t in (_zeros(4, 5, 6).transpose(0, 2)[1:], _zeros(7, dtype="int64")[3:], _zeros(2, 0, 3), _zeros(1, 4).expand(3, 4),
+              torch.zeros((), dtype=torch.uint8)):
+        got, want = L.L3dTensor.from_buffer_copy(L.packed(t)), L.desc(t)
+        assert (got.dtype, got.ndim) == (want.dtype, want.ndim)
+        assert list(got.dims)[:t.dim()] == list(t.shape) and list(got.strides)[:t.dim()] == list(t.stride())
+        assert (got.data or 0) + got.offset * t.element_size() == t.data_ptr()
+    assert L.packed(None) is None
+    with pytest.raises(TypeError):
+        L.packed(3)
+    with pytest.raises(TypeError, match="dtype"):
+        L.packed(_zeros(2, dtype="float64"))
+    with pytest.raises(ValueError, match="rank 7"):
+        L.packed(_zeros(1, 1, 1, 1, 1, 1, 1))
+    with pytest.raises(ValueError, match="CUDA"):
+        L.packs(None, _zeros(2))
