@@ -414,8 +414,9 @@ __device__ __forceinline__ uint64_t smem_desc_sw32(const void* tile) {
 // RES: there is a residual (kept out of the registers of the other form, which
 // would spill).  Bound for few rows by the weight's bytes and the launches: 64 x
 // 2048 -> 8192, 32 adapters 27 us (the weight alone 5 us at the copy rate); for
-// many by the loads of a K step, 48 KB from L2 for 4.2 MFLOP: 31569 x 1536 -> 8192,
-// rank 64 704 us in all (1155 TFLOP/s, 70% of a plain product's rate).
+// many by the loads of a K step, 48 KB from L2 for 512 clocks of products: the
+// tensor pipe is 64% busy, which is 63 bytes per clock and SM.  31569 x 1536 -> 8192,
+// rank 64 takes 704 us in all (1155 TFLOP/s, 70% of a plain product's rate).
 template <int BN, bool RES>
 __global__ void __launch_bounds__(THREADS, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
