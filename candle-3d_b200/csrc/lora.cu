@@ -440,8 +440,8 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* drain = list_empty + 2;
   volatile int* abort_flag = reinterpret_cast<volatile int*>(drain + 1);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1) + 1;
-  // Per tile parity: the distinct adapters and the first slot of each; the
-  // last entry of `first` + 1 is the number of slots (kept in `total`).
+  // Adapters of the rows of the tile; per tile parity the distinct ones, in the
+  // order of their first rows, the end of each one's slots, and their number.
   int* ids = reinterpret_cast<int*>(bars + 64);
   int* list_id = ids + BM;               // [2][BM]
   int* list_end = list_id + 2 * BM;      // [2][BM] slots up to and with this adapter
@@ -624,6 +624,11 @@ __global__ void __launch_bounds__(THREADS, 1)
         list_end[lb * BM + place] = base + sum;
       }
       if (r == 0) total[lb] = all;
+      // The adapters of this lane's rows, read before the four warps part: one that
+      // has no slot stage of this tile goes on and writes the next tile's ids.
+      int ad[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ad[i] = ids[lane + 32 * i];
       asm volatile("bar.sync 1, 128;" ::: "memory");
       if (lane == 0) mbar_arrive(&list_full[lb]);
       it += kblocks;
@@ -634,9 +639,6 @@ __global__ void __launch_bounds__(THREADS, 1)
       // Stage s belongs to warp 2 + s % 4, which writes all rows of its t pieces
       // (four per lane): four stages' loads of t are in flight at once, and a
       // warp meets the phases of its stages' tgo in order.
-      int ad[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) ad[i] = ids[lane + 32 * i];
       const int m0 = (tile / num_n) * BM, rows = min(p.M - m0, BM);
       int d = 0, start = 0;
       for (int q0 = 0; q0 < all; q0 += PER_STAGE, ++it) {
@@ -678,7 +680,6 @@ __global__ void __launch_bounds__(THREADS, 1)
         __syncwarp();
         if (lane == 0) mbar_arrive(&tfull[s]);
       }
-      // (ids is written again only after all four warps have met.)
     }
   } else {
     // ------------------------------------------------------------- epilogue

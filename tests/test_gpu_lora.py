@@ -233,3 +233,19 @@ def test_lora_linear_refusals(pkg, ops, dev):
         ops.LoraAdapters([], [])
     with pytest.raises(ValueError, match="CUDA"):
         ops.lora_linear(x.cpu(), w, ad, t)
+
+
+@pytest.mark.parametrize("ydt", ["bf16", "f32"])
+def test_lora_linear_stretches_of_rows(ops, dev, ydt):
+    """Rows in stretches of 128 to 400, one adapter each: every block works through
+    several row tiles with fewer slot stages than warps that fill them, and with
+    other adapters from tile to tile.  Equal bits on every call."""
+    import torch
+
+    r, M = rng(21), 20000
+    ids = np.concatenate([np.full(n, r.integers(-1, 40)) for n in r.integers(128, 401, 160)])[:M].astype(np.int32)
+    assert ids.size == M
+    ad, x, w, y = _case(ops, dev, M, 640, 128, [16] * 40, ids, bias=False, ydt=ydt)
+    t = torch.from_numpy(ids).to(dev)
+    for _ in range(20):
+        assert torch.equal(ops.lora_linear(x, w, ad, t, out_dtype=y.dtype), y)
