@@ -681,6 +681,9 @@ __global__ void __launch_bounds__(THREADS, 1)
         if (lane == 0) mbar_arrive(&tfull[s]);
       }
     }
+    // Where no row has an adapter nothing above has waited: without this, the end of
+    // this kernel would not say that shrink_kernel has read ids (and x) to the end.
+    if (!arrived) asm volatile("griddepcontrol.wait;" ::: "memory");
   } else {
     // ------------------------------------------------------------- epilogue
     const int quarter = warp & 3, half = (warp - 6) >> 2;

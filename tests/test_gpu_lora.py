@@ -249,3 +249,25 @@ def test_lora_linear_stretches_of_rows(ops, dev, ydt):
     t = torch.from_numpy(ids).to(dev)
     for _ in range(20):
         assert torch.equal(ops.lora_linear(x, w, ad, t, out_dtype=y.dtype), y)
+
+
+@pytest.mark.parametrize("M", [1, 40, 2368, 6000])
+def test_lora_linear_without_adapters_leaves_nothing_running(pkg, ops, dev, M):
+    """No row has an adapter, and the next operation on the stream gives every id a
+    value and the workspace another use: the call is then done with both."""
+    import torch
+
+    ad, x, w, y = _case(ops, dev, M, 64, 1024, [64, 64], np.full(M, -1, np.int32), bias=False)
+    t = torch.full((M,), -1, dtype=torch.int32, device=dev)
+    need = pkg._lib.lib().l3d_lora_linear_workspace_size(M, ad.rank)
+    ws = torch.empty(need, dtype=torch.uint8, device=dev)
+    out = torch.empty_like(y)
+    for _ in range(20):
+        t.fill_(-1)
+        dx, dw, dt, do = pkg._lib.packs(x, w, t, out)
+        pkg._lib.call("l3d_lora_linear", dx, dw, None, *ad._desc, dt, 0, None, None, do, ws.data_ptr(), need,
+                      pkg._lib.stream_of(x))
+        t.fill_(1)
+        ws.fill_(7)
+        torch.cuda.synchronize()
+        assert (ws == 7).all() and torch.equal(out, y)
