@@ -16,7 +16,8 @@ using namespace l3d::tc;
 // in [-1/2, 1/2], 2^f by a degree-3 minimax polynomial (Remez fit made for
 // this kernel, relative error 7.5e-5, far below the bf16 rounding of P), and
 // 2^j added to the exponent field.  x is clamped to -126 so that the exponent
-// stays in range; the inputs here are <= 2^8 (the rescale threshold).
+// stays in range; the inputs here are <= 2^8 (the rescale threshold).  A NaN
+// comes out as 2^-126: max_nan and minus_max carry it past this function.
 constexpr float EX2_C0 = 0.99992806f, EX2_C1 = 0.69326097f, EX2_C2 = 0.24261113f,
                 EX2_C3 = 0.05517167f;
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
@@ -30,6 +31,24 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
   return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
                      __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
 }
+
+// A score that is NaN or +inf has no softmax: its row is NaN, wherever in a tile
+// the score lies.  The running maximum carries it: the largest of the scores, NaN
+// where one is (fmaxf drops it), and what is added to the scaled scores for a
+// maximum m, NaN for an infinite one too.  m then has to move where !(largest <=
+// m + threshold), so that the rescaling spoils all that was summed before.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+  return y;
+}
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float y;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+  return y;
+}
+__device__ __forceinline__ float minus_max(float m) { return fmaf(m, 0.f, -m); }
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar,
                                             int c0, int c1, int c2, int c3) {
   asm volatile(

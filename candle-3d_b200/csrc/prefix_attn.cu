@@ -418,9 +418,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       __syncwarp();
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int e = 4; e < BKV; ++e) mx[e & 3] = fmaxf(mx[e & 3], s[e]);
-      const float mxs = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;  // scale > 0
-      const bool grow = mxs > m + RESCALE_LOG2;           // always on the first key a row sees
+      for (int e = 4; e < BKV; e += 2) mx[(e >> 1) & 3] = max_nan(mx[(e >> 1) & 3], s[e], s[e + 1]);
+      const float mxs = max_nan(max_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;  // scale > 0
+      const bool grow = !(mxs <= m + RESCALE_LOG2);       // always on the first key a row sees
       const float m_new = grow ? mxs : m;
       const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       }
       // P = exp2(s * scale * log2 e - m); a row that has seen no key yet has
       // m = -inf and all its scores masked: subtract 0, so that P = 0.
-      const float2 nm2 = f2(m_new == -INFINITY ? 0.f : -m_new);
+      const float2 nm2 = f2(m_new == -INFINITY ? 0.f : minus_max(m_new));
       l2 = mul2(l2, f2(alpha));
       // In pieces of 32 scores, stored to TMEM as they are formed (one store of
       // all 64 measured 7% slower over short key ranges).

@@ -250,3 +250,30 @@ def test_refusals(pkg, ops, dev):
         ops.shared_prefix_attention(**(ok | dict(q=ok["q"].cpu())))
     assert ops.shared_prefix_attention(z(0, 4, 3, 64), ok["prefix_k"], ok["prefix_v"]).shape == (0, 4, 3, 64)
     assert ops.shared_prefix_attention(z(2, 4, 0, 64), ok["prefix_k"], ok["prefix_v"]).shape == (2, 4, 0, 64)
+
+
+@pytest.mark.parametrize("N", [1, 150])
+@pytest.mark.parametrize("dt", ["bf16", "f16"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("value", ["nan", "inf"])
+def test_bad_key_is_seen_wherever_it_lies(ops, dev, value, own, D, dt, N):
+    """A key whose score is NaN or +inf makes the rows that see it NaN, at each of 16
+    consecutive places of a tile, and no other row differs."""
+    import torch
+
+    r = rng(N + D)
+    q, pk, pv, k, v = (_rand(r, s, dt, dev) for s in ((2, 4, N, D), (2, 100, D), (2, 100, D), (2, 2, 70, D), (2, 2, 70, D)))
+    q[..., 0] = 1
+    want = ops.shared_prefix_attention(q, pk, pv, k, v)
+    missed = []
+    for at in range(16, 32):
+        k2, pk2 = k.clone(), pk.clone()
+        (k2[1] if own else pk2)[1, at, 0] = float(value)
+        got = ops.shared_prefix_attention(q, pk2, pv, k2, v)
+        touched = torch.zeros_like(got, dtype=torch.bool)
+        touched[1 if own else slice(None), 2:] = True
+        assert torch.equal(got[~touched], want[~touched])
+        if not torch.isnan(got[touched]).all():
+            missed.append(at)
+    assert not missed
