@@ -326,11 +326,11 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       float mx0 = sv[0], mx1 = sv[1];
 #pragma unroll
       for (int e = 2; e < BKV; e += 2) {
-        mx0 = fmaxf(mx0, sv[e]);
-        mx1 = fmaxf(mx1, sv[e + 1]);
+        mx0 = max_nan(mx0, sv[e]);
+        mx1 = max_nan(mx1, sv[e + 1]);
       }
-      const float mxs = fmaxf(mx0, mx1) * p.scale_log2;  // scale > 0
-      const bool grow = mxs > m + RESCALE_LOG2;          // always on the first tile
+      const float mxs = max_nan(mx0, mx1) * p.scale_log2;  // scale > 0
+      const bool grow = !(mxs <= m + RESCALE_LOG2);        // always on the first tile
       const float m_new = grow ? mxs : m;
       const float alpha = grow ? ex2f(m - m_new) : 1.f;  // 0 on the first tile
       // Without SEP_P, S_t(j) complete implies P_t(j-1) V^T complete: O_t is
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       }
       // P = exp2(s * scale * log2 e - m) as packed bf16 pairs into the P
       // columns of this row, and the row sum.
-      const float2 nm2 = f2(-m_new);
+      const float2 nm2 = f2(minus_max(m_new));
       l2 = mul2(l2, f2(alpha));
       uint32_t u[BKV / 2];
 #pragma unroll

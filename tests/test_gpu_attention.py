@@ -184,3 +184,25 @@ def test_attention_bounded_wait_runs_out(pkg, ops, dev, D):
     got = ops.attention(q, k2, v2, D ** -0.5, check=True)
     ref_ = _ref(q, k2, v2, D ** -0.5)
     assert (got.float() - ref_).abs().max().item() < 2e-2
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("value", ["nan", "inf"])
+def test_bad_key_is_seen_wherever_it_lies(ops, dev, value, D):
+    """A key whose score is NaN or +inf makes its head's rows NaN at each of 16
+    consecutive places of a tile, and no other head differs."""
+    import torch
+
+    g = torch.Generator().manual_seed(D)
+    q, k, v = (torch.randn(1, 2, 200, D, generator=g).to(dev, torch.bfloat16) for _ in range(3))
+    q[..., 0] = 1
+    want = ops.attention(q, k, v)
+    missed = []
+    for at in range(16, 32):
+        k2 = k.clone()
+        k2[0, 1, at, 0] = float(value)
+        got = ops.attention(q, k2, v)
+        assert torch.equal(got[0, 0], want[0, 0])
+        if not torch.isnan(got[0, 1]).all():
+            missed.append(at)
+    assert not missed
