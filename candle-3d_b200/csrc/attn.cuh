@@ -15,13 +15,15 @@ using namespace l3d::tc;
 // range reduction x = j + f with j = round(x) (the 1.5 * 2^23 shifter) and f
 // in [-1/2, 1/2], 2^f by a degree-3 minimax polynomial (Remez fit made for
 // this kernel, relative error 7.5e-5, far below the bf16 rounding of P), and
-// 2^j added to the exponent field.  x is clamped to -126 so that the exponent
-// stays in range; the inputs here are <= 2^8 (the rescale threshold).  A NaN
-// comes out as 2^-126: max_nan and minus_max carry it past this function.
+// 2^j added to the exponent field.  x is clamped just above -127, where q > 1 and
+// the exponent field comes to 0: what is left, 1e-42, is 0 in either 16-bit type,
+// as a masked key's probability has to be (2^-126 would add 4 to an output where
+// its V is at the end of bf16's range).  The inputs here are <= 2^8 (the rescale
+// threshold).  A NaN is clamped too: max_nan and minus_max carry it past this function.
 constexpr float EX2_C0 = 0.99992806f, EX2_C1 = 0.69326097f, EX2_C2 = 0.24261113f,
-                EX2_C3 = 0.05517167f;
+                EX2_C3 = 0.05517167f, EX2_MIN = -127.f + 0x1p-12f;
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {
-  x = make_float2(fmaxf(x.x, -126.f), fmaxf(x.y, -126.f));
+  x = make_float2(fmaxf(x.x, EX2_MIN), fmaxf(x.y, EX2_MIN));
   const float2 t = add2(x, f2(12582912.f));          // low mantissa bits = round(x)
   const float2 r = add2(t, f2(-12582912.f));
   const float2 f = add2(x, make_float2(-r.x, -r.y));

@@ -472,7 +472,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
     if (ok && nkv > 0) ok = wait_warp(&pv_done[2 * t + ((nkv - 1) & 1)], ((nkv - 1) >> 1) & 1);
     tc_fence_after();
     if (ok && active) {
-      // (A row that has seen no key: ex2_poly2 gives 2^-126 for -inf, not 0.)
+      // (A row that has seen no key: ex2_poly2 gives 1e-42 for -inf, not 0.)
       float l = l2.x + l2.y;
       if (m == -INFINITY && l == l) l = 0.f;
       const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays

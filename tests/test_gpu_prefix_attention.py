@@ -277,3 +277,23 @@ def test_bad_key_is_seen_wherever_it_lies(ops, dev, value, own, D, dt, N):
         if not torch.isnan(got[touched]).all():
             missed.append(at)
     assert not missed
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("N", [40, 200])
+def test_masked_values_of_any_size_add_nothing(ops, dev, N, D):
+    """V of a key that a causal row does not see, at the end of bf16's range, at each
+    place of a tile: the rows before it keep their bits."""
+    import torch
+
+    r = rng(N + D)
+    q, pk, pv, k, v = (_rand(r, s, "bf16", dev) for s in ((1, 2, N, D), (2, 30, D), (2, 30, D), (1, 2, N, D), (1, 2, N, D)))
+    want = ops.shared_prefix_attention(q, pk, pv, k, v, causal=True)
+    changed = []
+    for at in range(1, 40):
+        v2 = v.clone()
+        v2[:, :, at] = 3e38
+        got = ops.shared_prefix_attention(q, pk, pv, k, v2, causal=True)
+        if not torch.equal(got[:, :, :at], want[:, :, :at]):
+            changed.append(at)
+    assert not changed
