@@ -66,6 +66,14 @@ struct Params {
 // is off by 2^-16 and costs one more K-16 product per slot (4% at rank 64 and
 // K = 1536).
 constexpr int PARTS = 2;
+// An infinite v, or one that bf16 rounds to infinity, has to leave the second part
+// with no infinity of the other sign (or inf - inf): the first part ends at bf16's
+// largest value, the second takes the rest (NaN and infinity among it).
+__device__ __forceinline__ void split(float v, float& hi, float& lo) {
+  constexpr float MOST = 0x1.fep127f;
+  hi = __bfloat162float(__float2bfloat16_rn(fminf(fmaxf(v, -MOST), MOST)));
+  lo = v - hi;
+}
 
 __device__ int g_lora_status;
 constexpr int ST_TIMEOUT = 5;
@@ -177,9 +185,10 @@ __global__ void __launch_bounds__(256, 1) shrink_kernel(const Params p) {
         for (int w = 0; w < WK; ++w) v += red[w][row][col];
         v *= sc;
         const int64_t at = int64_t(m0 + row) * p.R + r0 + col;
-        const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-        p.t[at] = hi;
-        p.t[int64_t(p.M) * p.R + at] = __float2bfloat16_rn(v - __bfloat162float(hi));
+        float hi, lo;
+        split(v, hi, lo);
+        p.t[at] = __float2bfloat16_rn(hi);
+        p.t[int64_t(p.M) * p.R + at] = __float2bfloat16_rn(lo);
       }
       __syncthreads();
     }
@@ -333,11 +342,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 2)
           for (int h = 0; h < 2; ++h) {
             float hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              const float x = v[8 * h + e] * scale;
-              hi[e] = __bfloat162float(__float2bfloat16_rn(x));
-              lo[e] = x - hi[e];
-            }
+            for (int e = 0; e < 8; ++e) split(v[8 * h + e] * scale, hi[e], lo[e]);
             u[0][h] = pack(hi, __nv_bfloat16());
             u[1][h] = pack(lo, __nv_bfloat16());
           }

@@ -271,3 +271,41 @@ def test_lora_linear_without_adapters_leaves_nothing_running(pkg, ops, dev, M):
         ws.fill_(7)
         torch.cuda.synchronize()
         assert (ws == 7).all() and torch.equal(out, y)
+
+
+def _one_row_apart(dev, M, rank, row):
+    """x zero but for one row; operands [M, 64], [48, 64], [rank, 64], [48, rank], all zero."""
+    import torch
+
+    z = lambda *s: torch.zeros(s, device=dev, dtype=torch.bfloat16)  # noqa: E731
+    return z(M, 64), z(48, 64), z(rank, 64), z(48, rank), torch.zeros(M, dtype=torch.int32, device=dev)
+
+
+@pytest.mark.parametrize("M", [5, 2400])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_lora_linear_infinite_row(ops, dev, M, sign):
+    """An infinite element of x under positive weights: the row is infinite, not NaN."""
+    import torch
+
+    x, w, a, b, ids = _one_row_apart(dev, M, 16, 3)
+    x.fill_(0.5)
+    w.fill_(0.25), a.fill_(0.125), b.fill_(0.5)
+    x[3, 7] = sign * float("inf")
+    y = ops.lora_linear(x, w, ops.LoraAdapters([a], [b]), ids)
+    assert (y[3] == sign * float("inf")).all()
+    assert torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()
+
+
+@pytest.mark.parametrize("M", [5, 2400])
+def test_lora_linear_a_x_at_the_end_of_the_range(ops, dev, M):
+    """A x between bf16's largest value and f32's: two parts hold it to 2^-16."""
+    import torch
+
+    x, w, a, b, ids = _one_row_apart(dev, M, 16, 2)
+    x[2, 0], x[2, 1] = 2.0 ** 127, 2.0 ** 119
+    a[0, 0], a[0, 1] = 255 / 128, 1.25
+    b[:, 0] = 2.0 ** -120
+    y = ops.lora_linear(x, w, ops.LoraAdapters([a], [b]), ids, out_dtype=torch.float32)
+    want = 255.0 + 1.25 * 2.0 ** -1  # 2^127 255/128 + 2^119 1.25, over 2^120
+    assert ((y[2].double() - want).abs() <= want * 2.0 ** -16).all()
+    assert not y[:2].any() and not y[3:].any()
