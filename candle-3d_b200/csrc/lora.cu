@@ -83,10 +83,12 @@ __device__ __forceinline__ int adapter_of(const Params& p, int m) {
   const int64_t id = p.ids64 ? static_cast<const int64_t*>(p.ids)[g] : static_cast<const int32_t*>(p.ids)[g];
   return id >= 0 && id < p.A ? int(id) : -1;
 }
-// Slots of 16 ranks that adapter a takes.
-__device__ __forceinline__ int slots_of(const Params& p, int a) {
-  return ((p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R) + 15) / 16;
+// Rank of adapter a, and the slots of 16 ranks that it takes.  t is 0 in the ranks
+// past its own: A's are 0 there, and 0 times an infinite x would be NaN.
+__device__ __forceinline__ int rank_of(const Params& p, int a) {
+  return p.ranks ? min(max(p.ranks[a], 0), p.R) : p.R;
 }
+__device__ __forceinline__ int slots_of(const Params& p, int a) { return (rank_of(p, a) + 15) / 16; }
 
 // --------------------------------------------------------------------- shrink
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
@@ -140,7 +142,7 @@ __global__ void __launch_bounds__(256, 1) shrink_kernel(const Params p) {
   const int chunks = (p.K + 31) / 32;
   for (int d = blockIdx.y; d < count; d += gridDim.y) {
     const int a = s_list[d];
-    const int rank = slots_of(p, a) * 16;
+    const int own = rank_of(p, a), rank = (own + 15) / 16 * 16;
     for (int r0 = blockIdx.z * RB; r0 < rank; r0 += gridDim.z * RB) {
       const int nt = min((rank - r0) / 8, NT);  // 8-rank tiles
       float c[NT][4];
@@ -183,7 +185,7 @@ __global__ void __launch_bounds__(256, 1) shrink_kernel(const Params p) {
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < WK; ++w) v += red[w][row][col];
-        v *= sc;
+        v = r0 + col < own ? v * sc : 0.f;
         const int64_t at = int64_t(m0 + row) * p.R + r0 + col;
         float hi, lo;
         split(v, hi, lo);
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 2)
     for (int d = 0; d < count; ++d) {
       if (!wait_warp(acc_full, d & 1)) break;
       tc_fence_after();
-      const int a = list[d], rank = slots_of(p, a) * 16;
+      const int a = list[d], rank = rank_of(p, a);
       const float scale = p.scale[a];
       for (int c = 0; c < rank; c += 16) {
         float v[16];
@@ -342,7 +344,7 @@ __global__ void __launch_bounds__(SHRINK_THREADS, 2)
           for (int h = 0; h < 2; ++h) {
             float hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) split(v[8 * h + e] * scale, hi[e], lo[e]);
+            for (int e = 0; e < 8; ++e) split(c + 8 * h + e < rank ? v[8 * h + e] * scale : 0.f, hi[e], lo[e]);
             u[0][h] = pack(hi, __nv_bfloat16());
             u[1][h] = pack(lo, __nv_bfloat16());
           }

@@ -309,3 +309,18 @@ def test_lora_linear_a_x_at_the_end_of_the_range(ops, dev, M):
     want = 255.0 + 1.25 * 2.0 ** -1  # 2^127 255/128 + 2^119 1.25, over 2^120
     assert ((y[2].double() - want).abs() <= want * 2.0 ** -16).all()
     assert not y[:2].any() and not y[3:].any()
+
+
+@pytest.mark.parametrize("M", [5, 2400])
+@pytest.mark.parametrize("rank", [1, 5, 33])
+def test_lora_linear_infinite_row_and_padded_ranks(ops, dev, M, rank):
+    """The ranks that an adapter is padded with take no part in an infinite row."""
+    import torch
+
+    x, w, a, b, ids = _one_row_apart(dev, M, rank, 3)
+    x.fill_(0.5)
+    w.fill_(0.25), a.fill_(0.125), b.fill_(0.5)
+    x[3, 7] = float("inf")
+    y = ops.lora_linear(x, w, ops.LoraAdapters([a, a.repeat(2, 1)], [b, b.repeat(1, 2)]), ids)
+    assert (y[3] == float("inf")).all()
+    assert torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()
