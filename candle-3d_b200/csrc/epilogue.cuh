@@ -18,14 +18,22 @@ __device__ __forceinline__ void act_chunk(float (&v)[NC]) {
 #pragma unroll
   for (int i = 0; i < NC; ++i) v[i] = act_t<A, FAST>(v[i]);
 }
-// One dispatch per chunk, so each variant's loop is contiguous code.
-template <int NC>
+// One dispatch per chunk, so each variant's loop is contiguous code.  REL: the
+// tanh GELU is accurate relative to its value (gelu_tanh_rel).
+template <int NC, bool REL = false>
 __device__ __forceinline__ void epi_act(int act, bool fast, float (&v)[NC]) {
   if (fast) {
     switch (act) {
       case ACT_SILU: act_chunk<ACT_SILU, true>(v); break;
       case ACT_GELU_ERF: act_chunk<ACT_GELU_ERF, true>(v); break;
-      case ACT_GELU_TANH: act_chunk<ACT_GELU_TANH, true>(v); break;
+      case ACT_GELU_TANH:
+        if constexpr (REL) {
+#pragma unroll
+          for (int i = 0; i < NC; ++i) v[i] = gelu_tanh_rel(v[i]);
+        } else {
+          act_chunk<ACT_GELU_TANH, true>(v);
+        }
+        break;
       default: break;
     }
   } else {

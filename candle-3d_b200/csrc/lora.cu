@@ -731,7 +731,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         float v[32];
         tmem_ld32(ta + uint32_t(c), v);
         if (p.bias) gemm::add_bias<32>(p, col0, v);
-        if (p.act) gemm::epi_act<32>(p.act, bf, v);
+        if (p.act) gemm::epi_act<32, true>(p.act, bf, v);
         if (whole) {
           // Aligned rows: 64 (or 128) consecutive bytes of a row per thread.
           if (RES && p.gate) gemm::mul_gate<32>(p, col0, v);

@@ -324,3 +324,28 @@ def test_lora_linear_infinite_row_and_padded_ranks(ops, dev, M, rank):
     y = ops.lora_linear(x, w, ops.LoraAdapters([a, a.repeat(2, 1)], [b, b.repeat(1, 2)]), ids)
     assert (y[3] == float("inf")).all()
     assert torch.isfinite(y[:3]).all() and torch.isfinite(y[4:]).all()
+
+
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("ydt", ["bf16", "f32"])
+def test_lora_linear_tanh_gelu_in_its_tail(ops, dev, M, ydt):
+    """The tanh GELU of z from -6 to 6, which the bias gives exactly: accurate relative
+    to its value.  A bf16 y is the rounding of a value within 2e-5 of the exact one
+    (an argument of the exponential up to 25 with a few f32 roundings), so it lies
+    between the roundings of that range's ends; an f32 y has the formula 0.5 z (1 +
+    tanh u) in f32, 2^-23 of |z| from its sum and 2e-6 of the value."""
+    import torch
+
+    N = 1024
+    z = torch.linspace(-6, 6, N, device=dev)
+    ad = ops.LoraAdapters([torch.zeros(1, 64, device=dev)], [torch.zeros(N, 1, device=dev)])
+    x, w = (torch.zeros(n, 64, device=dev, dtype=torch.bfloat16) for n in (M, N))
+    got = ops.lora_linear(x, w, ad, torch.zeros(M, dtype=torch.int32, device=dev), bias=z, act="gelu",
+                          out_dtype=torch.float32 if ydt == "f32" else torch.bfloat16).double()
+    zd = z.double()
+    want = zd / (1 + torch.exp(-2 * (2 / np.pi) ** 0.5 * (zd + 0.044715 * zd ** 3)))
+    if ydt == "bf16":
+        lo, hi = (t.to(torch.bfloat16).double() for t in (want - 2e-5 * want.abs(), want + 2e-5 * want.abs()))
+        assert ((got >= lo) & (got <= hi)).all()
+    else:
+        assert ((got - want).abs() <= zd.abs() * 2.0 ** -23 + want.abs() * 2e-6).all()
