@@ -562,23 +562,30 @@ class LoraAdapters:
         self._desc = tuple(map(packed, (self.a, self.b, self.scales, self.ranks)))
 
 
+def _row_len(t, x, name):
+    """Last dim of t, whose rows are taken in x's order: x's leading dims, or a matrix."""
+    if x.dim() != 2 and t.dim() != 2 and t.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"{name} has leading dims {tuple(t.shape[:-1])}, x {tuple(x.shape[:-1])}")
+    return t.shape[-1]
+
+
 def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, gate=None, out=None,
                 out_dtype=None):
     """`linear` with the low-rank adapter of each row's request beside the shared
     projection: y = residual + gate * act(x . W^T + bias + s_a B_a A_a x), where
     a = ids[i] for the i-th of ids.numel() equal groups of rows (one id per row,
     or per request); an id outside [0, adapters.count) means no adapter."""
-    n, k = weight.shape
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    n = weight.shape[0]
+    x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     m = x2.shape[0]
     if out is not None:
-        y = out.view(-1, n)
+        y = out.view(-1, _row_len(out, x, "out"))
     elif out_dtype is None:
         y = empty(x2, m, n)
     else:
         y = x.new_empty((m, n), dtype=out_dtype)
     if residual is not None and residual.dim() != 2:
-        residual = residual.reshape(-1, n)
+        residual = residual.reshape(-1, _row_len(residual, x, "residual"))
     dx, dw, db, di, dr, dg, dy = packs(x2, weight, bias, ids, residual, gate, y)
     need = _lib.lib().l3d_lora_linear_workspace_size(m, adapters.rank)
     ws = workspace(x2, need)

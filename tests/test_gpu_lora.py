@@ -349,3 +349,22 @@ def test_lora_linear_tanh_gelu_in_its_tail(ops, dev, M, ydt):
         assert ((got >= lo) & (got <= hi)).all()
     else:
         assert ((got - want).abs() <= zd.abs() * 2.0 ** -23 + want.abs() * 2e-6).all()
+
+
+def test_lora_linear_refuses_rows_of_another_length(pkg, ops, dev):
+    """A batch of rows that as many elements would fit otherwise is not cut anew."""
+    import torch
+
+    ad, x, w, _ = _case(ops, dev, 12, 64, 64, [16], np.zeros(12, np.int32), bias=False)
+    one = torch.zeros(2, device=dev, dtype=torch.int32)
+    z = lambda *s: torch.zeros(s, device=dev, dtype=torch.bfloat16)  # noqa: E731
+    for kw, match in [(dict(x=z(2, 3, 128)), "x last dim"), (dict(x=z(2, 3, 32)), "x last dim"),
+                      (dict(residual=z(2, 3, 128)), "residual"), (dict(out=z(2, 3, 32)), "y last dim"),
+                      (dict(residual=z(2, 6, 32)), "leading dims")]:
+        with pytest.raises((pkg._lib.L3dError, ValueError), match=match):
+            ops.lora_linear(**({"x": z(2, 3, 64), "weight": w, "adapters": ad, "ids": one} | kw))
+    r = torch.randn(2, 3, 64, device=dev).to(torch.bfloat16)
+    x3 = x[:6].view(2, 3, 64)
+    want = ops.lora_linear(x3, w, ad, one, residual=r)
+    assert torch.equal(ops.lora_linear(x3, w, ad, one, residual=r.view(6, 64)), want)
+    assert torch.equal(ops.lora_linear(x[:6], w, ad, one, residual=r), want.view(6, 64))

@@ -165,3 +165,13 @@ def test_descriptors_as_bytes(pkg):
         L.packed(_zeros(1, 1, 1, 1, 1, 1, 1))
     with pytest.raises(ValueError, match="CUDA"):
         L.packs(None, _zeros(2))
+
+
+@pytest.mark.parametrize("name,shape", [("residual", (3, 2, 40)), ("residual", (6, 1, 40)), ("out", (3, 2, 40))])
+def test_lora_linear_refuses_rows_in_another_order(pkg, name, shape):
+    """As many rows under other leading dims than x's are other rows."""
+    from types import SimpleNamespace
+
+    ad = SimpleNamespace(rank=16, _desc=(None,) * 4)
+    with pytest.raises(ValueError, match=f"{name} has leading dims"):
+        pkg.ops.lora_linear(_zeros(2, 3, 64), _zeros(40, 64), ad, _zeros(2, dtype="int32"), **{name: _zeros(*shape)})
