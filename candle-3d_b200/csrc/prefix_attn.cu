@@ -769,7 +769,8 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
       return fail(L3D_E_SHAPE, "%s: lengths must be contiguous [B]", op);
     if (no_data(lengths)) return fail(L3D_E_NULL, "%s: null data pointer", op);
   }
-  if (!(scale > 0.f) || !(scale < 3.0e38f))
+  const float scale_log2 = scale * 1.4426950408889634f;  // finite too
+  if (!(scale > 0.f) || !(scale_log2 < INFINITY))
     return fail(L3D_E_UNSUPPORTED, "%s: scale must be positive and finite", op);
   const int64_t big = int64_t(1) << 30;  // also keeps key and row arithmetic in 32 bits
   if (B > 65535 || Hq > 65535 || N > big || P > big || S > big || B * Hq * N > big)
@@ -807,7 +808,7 @@ extern "C" int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor
   p.lengths = lengths ? elem_ptr(lengths) : nullptr;
   p.len64 = lengths && lengths->dtype == L3D_I64;
   p.causal = causal != 0;
-  p.scale_log2 = scale * 1.4426950408889634f;
+  p.scale_log2 = scale_log2;
   p.slots = pl.slots; p.slots_p = pl.slots_p; p.joint = pl.joint;
   p.tiles_p = pl.tiles_p; p.tiles_o = pl.tiles_o;
   p.chunk_p = pl.chunk_p; p.chunk_o = pl.chunk_o;

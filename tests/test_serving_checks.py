@@ -175,3 +175,9 @@ def test_lora_linear_refuses_rows_in_another_order(pkg, name, shape):
     ad = SimpleNamespace(rank=16, _desc=(None,) * 4)
     with pytest.raises(ValueError, match=f"{name} has leading dims"):
         pkg.ops.lora_linear(_zeros(2, 3, 64), _zeros(40, 64), ad, _zeros(2, dtype="int32"), **{name: _zeros(*shape)})
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 2.9e38, 3.3e38])
+def test_shared_prefix_attention_refuses_a_scale_that_overflows(pkg, scale):
+    """The kernel multiplies by scale * log2(e): finite scales whose product is not."""
+    _refused(pkg, "l3d_shared_prefix_attention", _prefix_args(scale=scale), E_UNSUPPORTED, "scale")
