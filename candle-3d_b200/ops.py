@@ -9,6 +9,7 @@ Invalid inputs raise `L3dError` carrying the library's status and message.
 """
 from __future__ import annotations
 
+import ctypes
 import os
 
 import numpy as np
@@ -523,6 +524,26 @@ def attention(q, k, v, scale=None, out=None, check=None):
 
 
 # ------------------------------------- serving many requests around one context
+def kernel_status(device=None, reset=True):
+    """Status word of the kernels that keep none in a workspace (the row-norm rings
+    and the entries below) on `device`: 0, or 5 where a bounded wait ran out and an
+    output is unfinished.  Waits for the device's default stream only: synchronise
+    the stream of the calls first."""
+    st = ctypes.c_int(0)
+    with torch.cuda.device(device):
+        call("l3d_kernel_status", ctypes.byref(st), int(reset))
+    return st.value
+
+
+def _check_status(op, t, check):
+    """As `check` of `attention`, for the entries whose status word is the device's."""
+    if CHECK_STATUS if check is None else check:
+        torch.cuda.current_stream(t.device).synchronize()
+        st = kernel_status(t.device)
+        if st != 0:
+            raise _lib.L3dError(8, op, f"kernel status word {st} (bounded wait expired)")
+
+
 class LoraAdapters:
     """Low-rank adapters of the requests that share a projection, laid out once:
     adapter i adds scales[i] * b[i] @ (a[i] @ x), a[i] [rank, K], b[i] [N, rank]
@@ -570,11 +591,12 @@ def _row_len(t, x, name):
 
 
 def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, gate=None, out=None,
-                out_dtype=None):
+                out_dtype=None, check=None):
     """`linear` with the low-rank adapter of each row's request beside the shared
     projection: y = residual + gate * act(x . W^T + bias + s_a B_a A_a x), where
     a = ids[i] for the i-th of ids.numel() equal groups of rows (one id per row,
-    or per request); an id outside [0, adapters.count) means no adapter."""
+    or per request); an id outside [0, adapters.count) means no adapter.
+    `check` as in `attention` (here and in the two entries below)."""
     n = weight.shape[0]
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     m = x2.shape[0]
@@ -591,11 +613,12 @@ def lora_linear(x, weight, adapters, ids, bias=None, act=None, residual=None, ga
     ws = workspace(x2, need)
     call("l3d_lora_linear", dx, dw, db, *adapters._desc, di, ACT_CODES[act], dr, dg, dy,
          ws.data_ptr(), need, stream_of(x))
+    _check_status("l3d_lora_linear", x, check)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], n)
 
 
 def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None, causal=False,
-                            scale=None, out=None):
+                            scale=None, out=None, check=None):
     """exact_sdpa_heads (crate/runtime/attention_math.rs:199-259) for a batch that
     shares a prefix of keys: q [B, Hq, N, D] over prefix_k / prefix_v [Hkv, P, D]
     (one copy for the batch) and the first lengths[b] of each element's own k / v
@@ -613,6 +636,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k=None, v=None, lengths=None,
     call("l3d_shared_prefix_attention", dq, dpk, dpv, dk, dv, dl, int(bool(causal)),
          D ** -0.5 if scale is None else float(scale), do, ws.data_ptr() if need else None, need,
          stream_of(q))
+    _check_status("l3d_shared_prefix_attention", q, check)
     return out
 
 
@@ -621,7 +645,7 @@ NORMS = {"layer": 1, "rms": 2}
 
 def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, res_scale=1.0,
                            weight=None, bias=None, shift=None, scale=None, norm="rms", eps=1e-6,
-                           post_eps=None, next_norm=True, inplace=False):
+                           post_eps=None, next_norm=True, inplace=False, check=None):
     """Block seam with a norm on either side of the residual:
     r = res_scale * x + gate * (Norm(h)[*post_weight][+post_bias]);
     y = Norm(r)[*weight][+bias][*(1+scale)+shift]; returns (r, y).  `norm` is
@@ -633,4 +657,5 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
                                                            bias, shift, scale, r, y)
     call("l3d_sandwich_residual_norm", dx, dh, NORMS[norm], dpw, dpb, dg, float(res_scale), dw, db,
          dsh, dsc, eps if post_eps is None else post_eps, eps, dr, dy, stream_of(x))
+    _check_status("l3d_sandwich_residual_norm", x, check)
     return r, y

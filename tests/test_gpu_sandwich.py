@@ -198,3 +198,22 @@ def test_sandwich_refusals(pkg, ops, dev):
         ops.sandwich_residual_norm(x, x, norm="batch")
     with pytest.raises(ValueError, match="CUDA"):
         ops.sandwich_residual_norm(x.cpu(), x)
+
+
+def test_checked_calls_pass_on_an_idle_status_word(pkg, ops, dev):
+    """check=True after calls that finish: no error, the same bits, the word still 0."""
+    import torch
+
+    x = torch.randn(3, 40, 512, device=dev).to(torch.bfloat16)
+    r, y = ops.sandwich_residual_norm(x, x)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = ops.sandwich_residual_norm(x, x, check=True)
+        q = x.view(3, 40, 8, 64).transpose(1, 2)
+        ops.shared_prefix_attention(q, q[0], q[0], check=True)
+        ad = ops.LoraAdapters([torch.ones(4, 512, device=dev)], [torch.ones(64, 4, device=dev)])
+        w = torch.zeros(64, 512, device=dev, dtype=torch.bfloat16)
+        ops.lora_linear(x, w, ad, torch.zeros(3, device=dev, dtype=torch.int32), check=True)
+    assert torch.equal(got[0], r) and torch.equal(got[1], y)
+    assert ops.kernel_status(dev) == 0

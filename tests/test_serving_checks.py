@@ -181,3 +181,41 @@ def test_lora_linear_refuses_rows_in_another_order(pkg, name, shape):
 def test_shared_prefix_attention_refuses_a_scale_that_overflows(pkg, scale):
     """The kernel multiplies by scale * log2(e): finite scales whose product is not."""
     _refused(pkg, "l3d_shared_prefix_attention", _prefix_args(scale=scale), E_UNSUPPORTED, "scale")
+
+
+@pytest.mark.parametrize("op", ["lora_linear", "shared_prefix_attention", "sandwich_residual_norm"])
+def test_expired_waits_reach_the_caller(pkg, monkeypatch, op):
+    """A status word of 5 raises where it is asked for, by argument or for all calls,
+    and is read after the stream of the call has finished."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+
+    import torch
+
+    ops, seen = pkg.ops, []
+
+    def call(name, *args):
+        seen.append(name)
+        if name == "l3d_kernel_status":
+            args[0]._obj.value = 5
+
+    monkeypatch.setattr(ops, "call", call)
+    monkeypatch.setattr(ops, "packs", lambda *a: a)
+    monkeypatch.setattr(ops, "stream_of", lambda t: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda d: SimpleNamespace(synchronize=lambda: seen.append("synchronised")))
+    args = {"lora_linear": (_zeros(2, 64), _zeros(40, 64), SimpleNamespace(rank=16, _desc=()), None),
+            "shared_prefix_attention": (_zeros(1, 2, 3, 64), _zeros(2, 5, 64), _zeros(2, 5, 64)),
+            "sandwich_residual_norm": (_zeros(2, 64), _zeros(2, 64))}[op]
+    entry = f"l3d_{op}"
+    getattr(ops, op)(*args)
+    assert seen == [entry]  # a call does not wait unless it is asked to
+    for by_argument in (True, False):
+        seen.clear()
+        monkeypatch.setattr(ops, "CHECK_STATUS", not by_argument)
+        with pytest.raises(pkg._lib.L3dError, match=f"{entry}.*status word 5"):
+            getattr(ops, op)(*args, **({"check": True} if by_argument else {}))
+        assert seen == [entry, "synchronised", "l3d_kernel_status"]
+    getattr(ops, op)(*args, check=False)
+    assert seen[-1] == entry
