@@ -14,8 +14,6 @@ from pathlib import Path
 
 import torch
 
-from . import _l3dpack  # built with the library (host/pack.cpp)
-
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libl3dops.so"
 HEADER = PKG.parent / "include" / "l3d_ops.h"
@@ -71,8 +69,20 @@ def ref(d):
     return None if d is None else C.byref(d)
 
 
-packed = _l3dpack.packed  # as desc, as the descriptor's bytes (None -> NULL), for signatures with _D
-packs = _l3dpack.packs    # packed of each argument, which must be on a CUDA device
+# From _l3dpack.so (host/pack.cpp, built with the library).  It is bound to one torch:
+# where it cannot be loaded, the calls that need it fail, and nothing else.
+try:
+    from ._l3dpack import empty, packed, packs, workspace
+except ImportError as _e:
+    _why = str(_e)
+
+    def packed(*_):
+        """packed: as desc, as the descriptor's bytes (None -> NULL), for signatures with _D;
+        packs: packed of each argument, which must be on a CUDA device."""
+        raise RuntimeError(f"_l3dpack.so cannot be loaded ({_why}): build it with "
+                           "`python candle-3d_b200/build.py`")
+
+    empty = packs = workspace = packed
 
 
 _P = C.POINTER(L3dTensor)

@@ -9,6 +9,7 @@ header newer than the object).
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.metadata
 import os
 import subprocess
 import sys
@@ -52,12 +53,25 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def _pack_for() -> str:
+    """What _l3dpack.so is bound to: the interpreter and the installed torch."""
+    return f"{sysconfig.get_config_var('SOABI')} torch {importlib.metadata.version('torch')}"
+
+
+def _pack_needs() -> bool:
+    src, hdr, was = PKG / "host" / "pack.cpp", ROOT / "include" / "l3d_ops.h", BUILD / "_l3dpack.for"
+    if not PACK.exists() or not was.exists() or was.read_text() != _pack_for():
+        return True
+    return PACK.stat().st_mtime <= max(src.stat().st_mtime, hdr.stat().st_mtime)
+
+
 def _pack_module() -> None:
     """host/pack.cpp -> _l3dpack.so, against the headers of the installed torch."""
-    src, hdr = PKG / "host" / "pack.cpp", ROOT / "include" / "l3d_ops.h"
-    if PACK.exists() and PACK.stat().st_mtime > max(src.stat().st_mtime, hdr.stat().st_mtime):
+    if not _pack_needs():
         return
     import torch
+
+    src = PKG / "host" / "pack.cpp"
 
     t = Path(torch.__file__).resolve().parent
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
@@ -68,6 +82,7 @@ def _pack_module() -> None:
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"{src.name} failed to compile:\n{r.stderr}")
+    (BUILD / "_l3dpack.for").write_text(_pack_for())
 
 
 def build(verbose: bool = False) -> Path:

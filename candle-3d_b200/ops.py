@@ -16,8 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._l3dpack import empty, workspace
-from ._lib import call, desc, packed, packs, ref, stream_handle, stream_of
+from ._lib import call, desc, empty, packed, packs, ref, stream_handle, stream_of, workspace
 
 ACT = {"none": 0, "silu": 1, "gelu_erf": 2, "gelu_tanh": 3}
 

@@ -219,3 +219,58 @@ def test_expired_waits_reach_the_caller(pkg, monkeypatch, op):
         assert seen == [entry, "synchronised", "l3d_kernel_status"]
     getattr(ops, op)(*args, check=False)
     assert seen[-1] == entry
+
+
+def _without_pack(code):
+    """Runs `code` in a process where _l3dpack cannot be imported."""
+    import subprocess
+    import sys
+    from conftest import ROOT
+
+    head = ("import sys\n"
+            "class Refuse:\n"
+            "    def find_spec(self, name, path=None, target=None):\n"
+            "        if name.endswith('_l3dpack'): raise ImportError('undefined symbol: made for another torch')\n"
+            "sys.meta_path.insert(0, Refuse())\n"
+            "import __graft_entry__ as g\n"
+            "pkg = g.load_package()\n")
+    r = subprocess.run([sys.executable, "-c", head + code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr
+    return r.stdout
+
+
+def test_package_imports_without_the_native_descriptors(pkg):
+    """Entries that do not use them, GGUF reading and the library's own checks are there."""
+    out = _without_pack("import ctypes\n"
+                        "L = pkg._lib\n"
+                        "assert L.lib().l3d_abi_version() > 0\n"
+                        "assert pkg.gguf and L.lib().l3d_layer_norm(None, None, None, 1e-5, None, None) == 6\n"
+                        "print(L.lib().l3d_last_error().decode())\n")
+    assert out.strip()
+
+
+def test_calls_that_need_the_native_descriptors_say_why(pkg):
+    out = _without_pack("import torch\n"
+                        "z = torch.zeros(2, 5, 64, dtype=torch.bfloat16)\n"
+                        "for f in (lambda: pkg.ops.sandwich_residual_norm(z, z), lambda: pkg._lib.packed(z),\n"
+                        "          lambda: pkg.ops.shared_prefix_attention(z[None], z, z)):\n"
+                        "    try: f()\n"
+                        "    except RuntimeError as e: print(e)\n")
+    assert out.count("made for another torch") == 3 and out.count("build.py") == 3
+
+
+def test_native_descriptors_are_rebuilt_for_another_torch(pkg, monkeypatch, tmp_path):
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("l3d_build", Path(pkg.__file__).parent / "build.py")
+    b = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(b)
+    b.BUILD, b.PACK = tmp_path, tmp_path / "_l3dpack.so"
+    assert b._pack_needs()
+    b.PACK.write_bytes(b"")
+    assert b._pack_needs()  # of unknown origin
+    (tmp_path / "_l3dpack.for").write_text(b._pack_for())
+    assert not b._pack_needs()
+    monkeypatch.setattr(b.importlib.metadata, "version", lambda name: "0.1")
+    assert b._pack_needs()
