@@ -661,10 +661,17 @@ class SharedContextBlocks:
         """x [B, N, C]: the next N tokens of each request, request b holding
         start[b] (int32) already; ids [B]: its adapter, or one outside the range
         for none.  Returns their final states [B, N, C]; the cache takes their
-        keys and values."""
+        keys and values.  A request whose tokens do not fit its cache comes out
+        NaN, and no other differs (start lies on the device: no error can be raised
+        without waiting for it)."""
         B, N, C = x.shape
+        room = cache[0][0].shape[2]
+        if N > room:
+            raise ValueError(f"{N} tokens do not fit a cache of {room}")
         rows = torch.arange(B, device=x.device).view(B, 1)
-        at = start.view(B, 1).long() + torch.arange(N, device=x.device)
+        want = start.view(B, 1).long() + torch.arange(N, device=x.device)
+        at = want.clamp(0, room - 1)
+        x = x.masked_fill((at != want).any(1).view(B, 1, 1), float("nan"))
         lengths = start + N
         y = ops.layer_norm(x, *self.n0, eps=1e-6)
         for p, (pk, pv), (ck, cv) in zip(self.blocks, context, cache):

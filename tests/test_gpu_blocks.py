@@ -183,3 +183,28 @@ def test_shared_context_blocks_ragged_requests(pkg, dev):
         y = m.forward(x[rows, start.long()].unsqueeze(1), context, cache, start, ids)
         assert rel_l2(y[:, 0], ref[rows, start.long()]) < 2e-2
         start = start + 1
+
+
+@pytest.mark.parametrize("N", [1, 3])
+def test_shared_context_blocks_past_a_cache(pkg, dev, N):
+    """A request whose tokens do not fit its cache, or that claims to hold fewer than
+    none, comes out NaN; the others keep their bits and their caches."""
+    import torch
+
+    B, have = 4, 6
+    m, x, ids, context, cache, _ = _shared_context(dev, 100, B, 9)
+    room = cache[0][0].shape[2]
+    m.forward(x[:, :have].contiguous(), context, cache, torch.zeros(B, dtype=torch.int32, device=dev), ids)
+    step, start = x[:, have:have + N].contiguous(), torch.full((B,), have, dtype=torch.int32, device=dev)
+    copy = [(k.clone(), v.clone()) for k, v in cache]
+    want = m.forward(step, context, copy, start, ids)
+    bad = start.clone()
+    bad[1], bad[3] = room - N + 1, -1
+    got = m.forward(step, context, cache, bad, ids)
+    good = [0, 2]
+    assert torch.isnan(got[1]).all() and torch.isnan(got[3]).all() and torch.equal(got[good], want[good])
+    for (k, v), (k2, v2) in zip(cache, copy):
+        assert torch.equal(k[good][:, :, :have + N], k2[good][:, :, :have + N])
+        assert torch.equal(v[good][:, :, :have + N], v2[good][:, :, :have + N])
+    with pytest.raises(ValueError, match="do not fit"):
+        m.forward(torch.zeros(B, room + 1, m.C, device=dev, dtype=x.dtype), context, cache, start, ids)
