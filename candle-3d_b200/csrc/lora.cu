@@ -712,6 +712,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (!__all_sync(0xffffffffu, mbar_wait_idle(&acc_full[acc], (nt / 2) & 1, abort_flag, status,
                                                    ST_TIMEOUT, p.wait_ns)))
         break;
+      __syncwarp();
       tc_fence_after();
       const uint32_t ta = tmem_base + uint32_t(acc * BN) + (uint32_t(quarter * 32) << 16);
 #pragma unroll 1
@@ -728,6 +729,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 #pragma unroll
           for (int q = 0; q < 4; ++q) u[q] = src[q];
         }
+        __syncwarp();  // the load from tensor memory is the whole warp's
         float v[32];
         tmem_ld32(ta + uint32_t(c), v);
         if (p.bias) gemm::add_bias<32>(p, col0, v);

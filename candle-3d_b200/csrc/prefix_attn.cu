@@ -480,6 +480,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::THREADS, Cfg<D, NT>::CTAS)
       if (p.slots > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
       const Row w = row_at(p, valid ? f : fend - 1);
       T* orow = static_cast<T*>(p.out) + w.b * p.ob + int64_t(h * p.G + w.g) * p.oh + w.i * p.on;
+      __syncwarp();  // the loads from tensor memory are the whole warp's
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         float o[32];

@@ -368,3 +368,30 @@ def test_lora_linear_refuses_rows_of_another_length(pkg, ops, dev):
     want = ops.lora_linear(x3, w, ad, one, residual=r)
     assert torch.equal(ops.lora_linear(x3, w, ad, one, residual=r.view(6, 64)), want)
     assert torch.equal(ops.lora_linear(x[:6], w, ad, one, residual=r), want.view(6, 64))
+
+
+@pytest.mark.parametrize("M,N", [(1, 64), (33, 96), (129, 256), (300, 100), (2400, 512)])
+@pytest.mark.parametrize("ydt", ["bf16", "f32"])
+def test_lora_linear_residual_of_other_strides(ops, dev, M, N, ydt):
+    """A residual in memory of its own, with rows of another stride than y's and a
+    last row tile that is partly filled: the same bits as in place."""
+    import torch
+
+    ids = rng(M).integers(-1, 2, M).astype(np.int32)
+    ad, x, w, _ = _case(ops, dev, M, N, 128, [16, 40], ids, bias=False, ydt=ydt)
+    t, dt = torch.from_numpy(ids).to(dev), torch.float32 if ydt == "f32" else torch.bfloat16
+    g = torch.Generator().manual_seed(M)
+    res = torch.randn(M, N, generator=g).to(dev, dt)
+    gate = torch.randn(N, generator=g).to(dev)
+    y = res.clone()
+    ops.lora_linear(x, w, ad, t, residual=y, gate=gate, out=y)
+    wide = torch.zeros(M, N + 40, device=dev, dtype=dt)
+    for off in (0, 8, 3):  # 3: not 16-byte aligned
+        wide[:, off:off + N] = res
+        got = ops.lora_linear(x, w, ad, t, residual=wide[:, off:off + N], gate=gate, out_dtype=dt)
+        if off != 3 and N % 32 == 0:
+            assert torch.equal(got, y)
+        else:  # an unaligned row adds residual and gated product in one rounding, not two
+            far = (got.double() - y.double()).abs() - 2.0 ** -22 * (y.double().abs() + res.double().abs())
+            assert (far <= (2.0 ** -7 * y.double().abs() if ydt == "bf16" else 0.0)).all()
+        assert torch.equal(wide[:, off:off + N], res)
