@@ -361,8 +361,8 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
       }
       // P = exp2(s * scale * log2 e - m) as packed bf16 pairs into the P
       // columns of this row, and the row sum.
-      const float2 nm2 = f2(minus_max(m_new));
-      l2 = mul2(l2, f2(alpha));
+      const float2 nm2 = f2(-m_new);
+      l2 = fma2(l2, f2(alpha), f2(m_new * 0.f));  // NaN for a NaN or infinite maximum
       uint32_t u[BKV / 2];
 #pragma unroll
       for (int e = 0; e < BKV; e += 2) {
@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, 1)
         mbar_wait_idle(&pv_done[t], C::SEP_P ? (nkv - 1) & 1 : 0, abort_flag, p.status, ST_TIMEOUT, p.wait_ns)) {
       tc_fence_after();
       const float l = l2.x + l2.y;
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
       const int64_t qi = int64_t(q0) + t * BQ + r;
       __nv_bfloat16* orow = static_cast<__nv_bfloat16*>(p.out) + int64_t(b) * p.ob +
                             int64_t(h) * p.oh + qi * p.on;
