@@ -395,3 +395,38 @@ def test_lora_linear_residual_of_other_strides(ops, dev, M, N, ydt):
             far = (got.double() - y.double()).abs() - 2.0 ** -22 * (y.double().abs() + res.double().abs())
             assert (far <= (2.0 ** -7 * y.double().abs() if ydt == "bf16" else 0.0)).all()
         assert torch.equal(wide[:, off:off + N], res)
+
+
+@pytest.mark.parametrize("M", [1, 5, 130, 2369, 5000])
+def test_lora_linear_holds_a_x_in_two_parts(ops, dev, M):
+    """A x that needs 16 bits, picked out by B: y is exactly A x in f32, and its
+    rounding in bf16, for either kernel that forms A x."""
+    import torch
+
+    K, N, ranks = 136, 256, (1, 40, 256)
+    g = torch.Generator().manual_seed(M)
+    z = lambda *s: torch.zeros(s, device=dev, dtype=torch.bfloat16)  # noqa: E731
+    x, a, b, t = z(M, K), [], [], []
+    x[:, 3], x[:, 135] = 1, 2.0 ** -9
+    for r in ranks:
+        hi, lo = 128 + torch.randint(0, 128, (r,), generator=g), torch.randint(0, 128, (r,), generator=g)
+        a.append(z(r, K)), b.append(z(N, r))
+        a[-1][:, 3], a[-1][:, 135] = hi.to(dev), lo.to(dev)
+        pick = torch.arange(N) % r
+        b[-1][torch.arange(N), pick] = 1
+        t.append((hi + lo * 2.0 ** -9)[pick].to(dev, torch.float32))
+    ids = torch.randint(-1, 3, (M,), generator=g).to(dev, torch.int32)
+    want = torch.cat([torch.stack(t), torch.zeros(1, N, device=dev)])[ids.long()]
+    ad = ops.LoraAdapters(a, b)
+    assert torch.equal(ops.lora_linear(x, z(N, K), ad, ids, out_dtype=torch.float32), want)
+    assert torch.equal(ops.lora_linear(x, z(N, K), ad, ids), want.to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("M,N,K,ranks,kind", [
+    (2369, 96, 264, [16, 48], "scene"), (2500, 77, 136, [256, 8], "scene"), (2600, 40, 72, [16] * 20, "row"),
+    (12001, 64, 520, [64], "scene"), (5000, 2560, 192, [16, 32, 64, 16], "row"),
+])
+def test_lora_linear_many_rows_in_f32(ops, dev, M, N, K, ranks, kind):
+    """As the tests of many rows and tiles, with an output that does not round their errors away."""
+    ids = rng(M).integers(-1, len(ranks), M).astype(np.int32)
+    _case(ops, dev, M, N, K, ranks, np.sort(ids) if kind == "scene" else ids, ydt="f32")
