@@ -217,3 +217,36 @@ def test_checked_calls_pass_on_an_idle_status_word(pkg, ops, dev):
         ops.lora_linear(x, w, ad, torch.zeros(3, device=dev, dtype=torch.int32), check=True)
     assert torch.equal(got[0], r) and torch.equal(got[1], y)
     assert ops.kernel_status(dev) == 0
+
+
+@pytest.mark.parametrize("dt,u", [("f32", 2.0 ** -24), ("bf16", 2.0 ** -8), ("f16", 2.0 ** -11)])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("T,C", [(3, 64), (400, 256), (33, 1024), (170, 2048), (5, 8192), (7, 77), (9, 2047), (2, 20001)])
+def test_sandwich_is_as_near_as_its_output_type(ops, dev, T, C, kind, dt, u):
+    """Within the rounding of the stored value and 1e-5 of the terms that are added
+    up: f32 statistics of up to 20001 elements in sums of several parts, some 20
+    roundings, once each for r and for y's own norm of it."""
+    r = rng(77 + T * C)
+    names = {"pw": 1.0, "pb": 0.0, "g": 1.0, "w": 1.0, "b": 0.0, "sh": 0.0, "sc": 0.0}
+    x, xv = to_dev(r.standard_normal((2, T, C)), dt, dev)
+    h, hv = to_dev(3 * r.standard_normal((2, T, C)) + 0.3, dt, dev)
+    t, f = {}, {}
+    for name, mean in names.items():
+        t[name], v = to_dev(mean + 0.2 * r.standard_normal((2, C) if name in ("g", "sh", "sc") else (C,)), dt, dev)
+        f[name] = v.astype(np.float64)
+    ro, yo = ops.sandwich_residual_norm(x, h, post_weight=t["pw"], post_bias=t["pb"], gate=t["g"], res_scale=0.75,
+                                        weight=t["w"], bias=t["b"], shift=t["sh"], scale=t["sc"], norm=kind,
+                                        eps=1e-5, post_eps=1e-6)
+    xv, hv = xv.astype(np.float64), hv.astype(np.float64)
+    rr, yr = _ref(kind, xv, hv, f["pw"], f["pb"], f["g"], 0.75, f["w"], f["b"], f["sh"], f["sc"], 1e-6, 1e-5)
+    per = lambda n: f[n].reshape(2, 1, C)  # noqa: E731
+    nrm = np.abs(_norm(kind, hv, None, None, 1e-6))
+    terms = 0.75 * np.abs(xv) + np.abs(per("g")) * (nrm * np.abs(f["pw"]) + np.abs(f["pb"]))
+    v = rr - rr.mean(-1, keepdims=True) if kind == "layer" else rr
+    inv = 1 / np.sqrt((v * v).mean(-1, keepdims=True) + 1e-5)
+    terms_y = (1 + np.abs(per("sc"))) * (np.abs(f["w"]) * inv * (terms + terms.mean(-1, keepdims=True)) + np.abs(f["b"])) \
+        + np.abs(per("sh"))
+    for got, want, mag in ((ro, rr, terms), (yo, yr, terms_y)):
+        err = np.abs(got.double().cpu().numpy() - want)
+        bound = u * np.abs(want) + 1e-5 * mag + (2.0 ** -25 if dt == "f16" else 0.0)
+        assert (err <= bound).all(), (err / bound).max()
