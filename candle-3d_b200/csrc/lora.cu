@@ -419,11 +419,14 @@ __device__ __forceinline__ uint64_t smem_desc_sw32(const void* tile) {
 }
 
 // RES: there is a residual (kept out of the registers of the other form, which
-// would spill).  Bound for few rows by the weight's bytes and the launches: 64 x
-// 2048 -> 8192, 32 adapters 27 us (the weight alone 5 us at the copy rate); for
-// many by the loads of a K step, 48 KB from L2 for 512 clocks of products: the
+// would spill).  Bound for few rows by one block's chain of steps: 64 x 2048 ->
+// 8192 takes 13.6 us without adapters (the weight alone 5 us at the copy rate), 28
+// with 32 of them, since the slot stages, some 17 here, each fetch their pieces of t
+// from L2 after a wait for a free stage, and begin when shrink_kernel (9 us) is done;
+// for many rows by the loads of a K step, 48 KB from L2 for 512 clocks of products: the
 // tensor pipe is 64% busy, which is 63 bytes per clock and SM.  31569 x 1536 -> 8192,
-// rank 64 takes 704 us in all (1155 TFLOP/s, 70% of a plain product's rate).
+// rank 64 takes 701 to 711 us in all by graph replay after a pause (1145 TFLOP/s, 69% of
+// a plain product's rate), 780 to 830 in a loop, at the clock that the power limit leaves.
 template <int BN, bool RES>
 __global__ void __launch_bounds__(THREADS, 1)
     lora_gemm_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
