@@ -438,8 +438,8 @@ size_t l3d_lora_linear_workspace_size(int64_t m, int64_t r);
  * projection alone.  x [.., k] BF16, 16-byte aligned rows; weight [n, k] BF16
  * as for l3d_linear_ex; lora_a [adapters, R, k] and lora_b [adapters, n, R]
  * BF16 contiguous, R a multiple of 16 up to 256, zero beyond an adapter's own
- * rank; scale [adapters] F32; ranks [adapters] I32 (NULL: all R) lets the
- * kernels skip the zero ranks.  The adapters must be finite: a row of another
+ * rank; scale [adapters] F32; ranks [adapters] I32 (NULL: all R) keeps the
+ * ranks past an adapter's own out of the result.  The adapters must be finite: a row of another
  * request meets them multiplied by zero.  bias, act, residual, gate as for
  * l3d_linear_ex; y BF16 or F32; y must not overlap x (it may be residual).
  * A_a x is accumulated in f32 and enters the second product as the sum of two
@@ -464,10 +464,12 @@ size_t l3d_shared_prefix_attention_workspace_size(int64_t b, int64_t hq, int64_t
  * multiple of Hkv, query head h reading key head h / (Hq / Hkv).  causal: the
  * N rows are the last N of their element's own sequence, row i sees the own
  * keys j <= lengths[b] - N + i (and the whole prefix).  Own keys past
- * lengths[b] are never used, whatever they hold.  A row with no keys gives
- * zeros.  BF16 or F16, D = 64 or 128, head dim contiguous, strides otherwise
+ * lengths[b] are never used, whatever they hold; a key that a row does not see
+ * for `causal` adds nothing to it, as long as its V is finite.  A row with no keys
+ * gives zeros, one that sees a score that is NaN or +inf NaN.  BF16 or F16, D = 64 or 128, head dim contiguous, strides otherwise
  * free in multiples of 16 bytes; softmax and sums in f32, probabilities
- * rounded to the input type for the second product.  scale must be positive. */
+ * rounded to the input type for the second product.  scale must be positive, and
+ * scale * log2(e) finite. */
 int l3d_shared_prefix_attention(const l3d_tensor* q, const l3d_tensor* prefix_k,
                                 const l3d_tensor* prefix_v, const l3d_tensor* k,
                                 const l3d_tensor* v, const l3d_tensor* lengths, int causal,
