@@ -46,29 +46,29 @@ def _cross(name, B, N, Hq, Hkv, D, S, rows="equal", dtype="bf16"):
 def listed():
     return [
         # One token of one request: latency.
-        _append("append, one token", 1, 1, 8, 2, 64, 16, (32,), held=300),
+        _append("append one token", 1, 1, 8, 2, 64, 16, (32,), held=300),
         # One token for each of 64 requests, placed in a video (time, height, width).
-        _append("append, 64 requests", 64, 64, 16, 4, 128, 16, (16, 24, 24), held=4096),
+        _append("append 64 requests", 64, 64, 16, 4, 128, 16, (16, 24, 24), held=4096),
         # The views of five scenes arriving at once, positions on an image's axes, each axis a block of its own.
-        _append("append, views of scenes", 5, 10992, 16, 16, 64, 64, (16, 16), layout="axis", dtype="f16", held=1374),
+        _append("append views of scenes", 5, 10992, 16, 16, 64, 64, (16, 16), layout="axis", dtype="f16", held=1374),
         # Long prompts of 24 requests, pairs of neighbours rotated, part of the head left as it is, no norms.
-        _append("append, long prompts", 24, 49152, 16, 4, 128, 32, (48,), layout="interleaved", norm=False, held=100),
+        _append("append long prompts", 24, 49152, 16, 4, 128, 32, (48,), layout="interleaved", norm=False, held=100),
         # One token of one request with a short cache: latency.
-        _paged("paged, one request", 1, 1, 8, 2, 64, 16, 300),
+        _paged("paged one request", 1, 1, 8, 2, 64, 16, 300),
         # One token for each of 64 requests, caches of ragged lengths.
-        _paged("paged, 64 requests", 64, 1, 16, 4, 128, 16, 4096),
+        _paged("paged 64 requests", 64, 1, 16, 4, 128, 16, 4096),
         # A few tokens for each of 12 requests, a key head for each query head, pages of an odd size.
-        _paged("paged, few tokens", 12, 4, 12, 12, 128, 48, 4097, dtype="f16"),
+        _paged("paged few tokens", 12, 4, 12, 12, 128, 48, 4097, dtype="f16"),
         # One token for each of 8 requests behind very long caches.
-        _paged("paged, long caches", 8, 1, 16, 4, 128, 64, 65536, ragged=False),
+        _paged("paged long caches", 8, 1, 16, 4, 128, 64, 65536, ragged=False),
         # A few short sequences beside encoders of about a sentence's length: latency.
-        _cross("cross, short sequences", 3, 70, 8, 2, 64, 77, rows="ragged", dtype="f16"),
+        _cross("cross short sequences", 3, 70, 8, 2, 64, 77, rows="ragged", dtype="f16"),
         # One decoded token of each of 32 requests over its own image's tokens.
-        _cross("cross, single rows", 32, 1, 16, 16, 64, 1370),
+        _cross("cross single rows", 32, 1, 16, 16, 64, 1370),
         # Two objects of 2049 tokens, whose images gave different numbers of tokens.
-        _cross("cross, two objects", 2, 2049, 16, 16, 128, 1370),
+        _cross("cross two objects", 2, 2049, 16, 16, 128, 1370),
         # The voxel rows of three scenes, each with an image of its own.
-        _cross("cross, voxel scenes", 3, 31569, 12, 12, 128, 1370),
+        _cross("cross voxel scenes", 3, 31569, 12, 12, 128, 1370),
     ]
 
 
