@@ -72,17 +72,18 @@ def ref(d):
 # From _l3dpack.so (host/pack.cpp, built with the library).  It is bound to one torch:
 # where it cannot be loaded, the calls that need it fail, and nothing else.
 try:
-    from ._l3dpack import empty, packed, packs, workspace
+    from ._l3dpack import empty, packed, packs, packs_here, workspace
 except ImportError as _e:
     _why = str(_e)
 
     def packed(*_):
         """packed: as desc, as the descriptor's bytes (None -> NULL), for signatures with _D;
-        packs: packed of each argument, which must be on a CUDA device."""
+        packs: packed of each argument, which must be on a CUDA device; packs_here: on
+        the current one."""
         raise RuntimeError(f"_l3dpack.so cannot be loaded ({_why}): build it with "
                            "`python candle-3d_b200/build.py`")
 
-    empty = packs = workspace = packed
+    empty = packs = packs_here = workspace = packed
 
 
 _P = C.POINTER(L3dTensor)
@@ -145,6 +146,11 @@ _SIGS = {
                                      C.c_size_t, _S], C.c_int),
     "l3d_sandwich_residual_norm": ([_D, _D, C.c_int, _D, _D, _D, C.c_float, _D, _D, _D, _D,
                                     C.c_float, C.c_float, _D, _D, _S], C.c_int),
+    "l3d_paged_append": ([_D, _D, _D, _D, _D, C.c_float, _D, _D, C.c_int, _D, _D, _D, _D, _D, _D, _D,
+                          _S], C.c_int),
+    "l3d_paged_attention_workspace_size": ([C.c_int64] * 6, C.c_size_t),
+    "l3d_paged_attention": ([_D, _D, _D, _D, _D, C.c_float, _D, C.c_void_p, C.c_size_t, _S],
+                            C.c_int),
     "l3d_gguf_index": ([C.c_void_p, C.c_uint64, C.c_void_p, C.c_int64, C.POINTER(C.c_int64),
                         C.POINTER(C.c_uint32), C.POINTER(C.c_uint64)], C.c_int),
     "l3d_gguf_metadata_string": ([C.c_void_p, C.c_uint64, C.c_char_p, C.POINTER(C.c_void_p),

@@ -1,0 +1,653 @@
+// Attention of the newest token (or a few) of each request over its cached keys:
+//   out[b, i, h] = sum_j softmax_j(scale q[b, i, h] . K[j]) V[j]
+// over the keys j < lengths[b] - N + 1 + i, which lie in pages: key j of request b in slot j % size of page
+// table[b, j / size]; or, for single rows of cross attention, over a packed stretch of an encoder's states.
+// The reference's attention core is exact_sdpa_heads (crate/runtime/attention_math.rs:199-259); it has no cache.
+//
+// Bound by the bytes of K and V, each read once: a key head's rows (i, g) = N G of them in tiles of 16, the
+// height of mma.m16n8k16, whose rate is some four times what the loads need (at one row of 16 as well).  The
+// 5th-generation tensor core takes tiles of 128 rows, and a round trip through its memory for each.
+//
+// Work is divided by keys alone: all (request, key head, row tile) have their keys in tiles of 16, the tiles of
+// all of them in one line, and every warp of the device takes an equal stretch of the line, whatever the
+// lengths are; the lengths are read on the device, and each block sums them up for itself.  A warp works
+// alone: its own ring of tiles in shared memory, filled by 16-byte asynchronous copies that run on across the
+// ends of requests, its own running maximum and sum, no barrier.  Where a stretch holds all the keys of a
+// request's head, the warp stores the output; otherwise O / l and the log2 of the sum in f32, and
+// combine_kernel weighs the parts of each row.  A part's place follows from the lengths, so results do not
+// depend on the order in which warps run.
+//
+// S = Q K^T with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability (the products are not
+// what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
+// A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
+#include <type_traits>
+
+#include "attn.cuh"
+#include "decode_attn.cuh"
+
+namespace l3d {
+namespace decode {
+
+using attn::ex2f;
+using attn::max_nan;
+using attn::minus_max;
+
+constexpr int WARPS = 8, KT = 16;       // warps of a block (one per SM), keys of a tile
+constexpr int MIN_TILES = 2;            // of a warp, where there are as many
+constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
+
+template <int D>
+struct Cfg {
+  static constexpr int ROW = D * 2, TILE = KT * ROW;       // bytes
+  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int RING = STAGES * 2 * TILE;           // of one warp
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
+
+__device__ __forceinline__ int64_t value_at(const void* p, int is64, int64_t i) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+}
+// First packed row of sequence b (the end of b - 1).
+__device__ __forceinline__ int packed_start(const Params& p, int b) {
+  const int64_t v = value_at(p.lengths, p.len64, b);
+  return v < 0 ? 0 : v < p.keys ? int(v) : p.keys;
+}
+// Keys of sequence b that can be read, and whether its length does not fit its table.
+__device__ __forceinline__ int length_of(const Params& p, int b, bool* bad) {
+  *bad = false;
+  if (p.size == 0) return max(packed_start(p, b + 1) - packed_start(p, b), 0);
+  const int64_t v = value_at(p.lengths, p.len64, b), room = int64_t(p.width) * p.size;
+  *bad = v > room;
+  return v < 0 ? 0 : int(v < room ? v : room);
+}
+
+// The line of tiles: sequence b's begin at starts[b] * heads, heads = Hkv * row tiles.
+struct Line {
+  int64_t total, per;   // tiles, tiles of a warp
+};
+__device__ __forceinline__ Line line_of(const Params& p, int tiles) {
+  const int64_t total = int64_t(tiles) * p.Hkv * p.tiles;
+  const int64_t even = (total + p.total_warps - 1) / p.total_warps;
+  return {total, even > MIN_TILES ? even : MIN_TILES};
+}
+
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  // a, b as a pair of the type, and what the pair leaves of them.
+  static __device__ __forceinline__ uint32_t split(float a, float b, uint32_t& rest) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - __low2float(h), b - __high2float(h));
+    rest = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <> struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t split(float a, float b, uint32_t& rest) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const __half2 l = __floats2half2_rn(a - __low2float(h), b - __high2float(h));
+    rest = *reinterpret_cast<const uint32_t*>(&l);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// 16 bytes to shared memory; `bytes` 0: zeros, and nothing is read.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// A place in the line of tiles: sequence b, head and row tile hr, key tile t of `tiles`.
+struct Cursor {
+  int b, hr, t, tiles;
+  __device__ __forceinline__ void seek(const int* starts, int B, int heads, int64_t x) {
+    const int64_t y = x / heads;
+    int lo = 0, hi = B;  // the last b with starts[b] <= y
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts[mid] <= y) lo = mid;
+      else hi = mid;
+    }
+    b = lo;
+    tiles = starts[b + 1] - starts[b];
+    const int64_t rem = x - int64_t(starts[b]) * heads;
+    hr = int(rem / tiles);
+    t = int(rem - int64_t(hr) * tiles);
+  }
+  // (Not past the line's last tile.)
+  __device__ __forceinline__ void next(const int* starts, int heads) {
+    if (++t < tiles) return;
+    t = 0;
+    if (++hr < heads) return;
+    hr = 0;
+    do {
+      ++b;
+      tiles = starts[b + 1] - starts[b];
+    } while (tiles == 0);
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const Params p) {
+  using C = Cfg<D>;
+  constexpr int CHUNKS = D / 8;          // 16-byte pieces of a row
+  constexpr int NT = D / 8;              // 8-wide column tiles of O
+  extern __shared__ __align__(1024) uint8_t smem[];
+  int* starts = reinterpret_cast<int*>(smem + WARPS * C::RING);  // [B + 1]
+  __shared__ int s_warp[WARPS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  // ---- key tiles before each sequence: a sum over the batch, a stretch of it per thread
+  {
+    const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(int(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      bool bad;
+      const int n = (length_of(p, b, &bad) + KT - 1) / KT;
+      starts[b] = n;
+      sum += n;
+    }
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    if (lane == 31) s_warp[warp] = incl;
+    __syncthreads();
+    int at = incl - sum;
+    for (int w = 0; w < warp; ++w) at += s_warp[w];
+    for (int b = b0; b < b1; ++b) {
+      const int n = starts[b];
+      starts[b] = at;
+      at += n;
+    }
+    if (threadIdx.x == WARPS * 32 - 1) starts[p.B] = at;  // (its stretch is the last, or empty)
+    __syncthreads();
+    if (blockIdx.x == 0)
+      for (int b = threadIdx.x; b <= p.B; b += WARPS * 32) p.starts[b] = starts[b];
+  }
+  const int heads = p.Hkv * p.tiles;
+  const Line line = line_of(p, starts[p.B]);
+  const int me = warp * gridDim.x + blockIdx.x;  // a short line spreads over the device first
+  const int64_t x0 = int64_t(me) * line.per;
+  if (x0 >= line.total) return;
+  const int count = int(min(line.per, line.total - x0));
+
+  // ---- loads: tile by tile ahead of the work.  Lane l looks up key l % 16 of the next tile one tile early,
+  // so that the table's latency is not waited for.
+  const uint32_t ring = smem_u32(smem) + warp * C::RING;
+  Cursor ld;
+  ld.seek(starts, p.B, heads, x0);
+  int ld_page = 0, ld_slot = 0, ld_ok = 0;  // of key lane % 16 of the cursor's tile
+  auto look_up = [&] {
+    bool bad;
+    const int len = length_of(p, ld.b, &bad), j = ld.t * KT + (lane & 15);
+    ld_ok = j < len;
+    if (p.size) {
+      const int page = j / p.size;
+      ld_slot = j - page * p.size;
+      ld_page = ld_ok ? p.table[ld.b * p.table_stride + page] : 0;
+    } else {
+      ld_page = 0;
+      ld_slot = packed_start(p, ld.b) + j;
+    }
+  };
+  look_up();
+  int issued = 0;
+  uint32_t bad_keys[C::STAGES];
+  auto issue = [&](int stage, uint32_t& bad_mask) {
+    if (issued < count) {
+      // (Only now is the table's entry needed.)
+      const bool out = p.size && ld_ok && (ld_page < 0 || ld_page >= p.keys);
+      bad_mask = __ballot_sync(0xffffffffu, out) & 0xffffu;
+      const int have = ld_ok && !out ? 16 : 0, h = ld.hr / p.tiles;
+      const uint32_t kd = ring + stage * (2 * C::TILE), vd = kd + C::TILE;
+      constexpr int PER = 32 / CHUNKS;             // rows of a turn
+      const int c = lane % CHUNKS;
+#pragma unroll
+      for (int i = 0; i < KT / PER; ++i) {
+        const int r = i * PER + lane / CHUNKS;
+        const int page = __shfl_sync(0xffffffffu, ld_page, r), slot = __shfl_sync(0xffffffffu, ld_slot, r);
+        const int bytes = __shfl_sync(0xffffffffu, have, r);
+        const uint32_t at = r * C::ROW + ((c ^ (r & 7)) << 4);
+        const T* ks = reinterpret_cast<const T*>(p.k) + (bytes ? page * p.ks[0] + slot * p.ks[1] + h * p.ks[2] + c * 8 : 0);
+        const T* vs = reinterpret_cast<const T*>(p.v) + (bytes ? page * p.vs[0] + slot * p.vs[1] + h * p.vs[2] + c * 8 : 0);
+        copy16(kd + at, ks, bytes);
+        copy16(vd + at, vs, bytes);
+      }
+      if (++issued < count) {
+        ld.next(starts, heads);
+        look_up();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < C::STAGES; ++s) issue(s, bad_keys[s]);
+
+  // ---- work
+  Cursor cu;
+  cu.seek(starts, p.B, heads, x0);
+  const int rg = lane >> 2, cq = (lane & 3) * 2;  // this thread's rows rg and rg + 8, columns cq, cq + 1 of 8
+  const int R = p.N * p.G;
+  uint32_t qf[D / 16][4];
+  float o[NT][4];
+  float m[2], l[2];
+  int lim[2], len = 0, t_first = 0, left = count, least = 0;
+  bool fresh = true;
+  auto row_of = [&](int e, int* i, int* g) {
+    const int f = (cu.hr % p.tiles) * 16 + rg + 8 * e;
+    *i = f / p.G;
+    *g = f - *i * p.G;
+    return f < R;
+  };
+  for (int n0 = 0; n0 < count; n0 += C::STAGES) {
+#pragma unroll
+    for (int s = 0; s < C::STAGES; ++s) {
+      if (n0 + s >= count) break;
+      if (fresh) {  // the first tile of a part
+        fresh = false;
+        t_first = cu.t;
+        bool bad;
+        len = length_of(p, cu.b, &bad);
+        least = p.causal ? len - p.N + 1 : len;
+        const int h = cu.hr / p.tiles;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          int i, g;
+          const bool in = row_of(e, &i, &g);
+          lim[e] = !in ? 0 : p.causal ? len - p.N + 1 + i : len;
+          m[e] = -INFINITY;
+          l[e] = bad && in ? __int_as_float(0x7fffffff) : 0.f;
+          const T* qr = reinterpret_cast<const T*>(p.q) + cu.b * p.qb + i * p.qn + (h * p.G + g) * p.qh;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            qf[k][e] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq) : 0u;
+            qf[k][e + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq + 8) : 0u;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
+      __syncwarp();
+      const uint32_t kt = ring + s * (2 * C::TILE), vt = kt + C::TILE;
+      // S = Q K^T: two tiles of 8 keys
+      float sc[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
+        uint32_t b[4];
+        ldsm4(b, kt + r * C::ROW + ((c ^ (r & 7)) << 4));
+        Mma<T>::run(sc[0], qf[k], b[0], b[1]);
+        Mma<T>::run(sc[1], qf[k], b[2], b[3]);
+      }
+      const int key0 = cu.t * KT;
+      if (bad_keys[s]) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (bad_keys[s] >> ((e >> 2) * 8 + cq + (e & 1)) & 1) sc[e >> 2][e & 3] = __int_as_float(0x7fffffff);
+      }
+      const bool edge = key0 + KT > least;  // some row does not see some key
+      if (edge) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (key0 + (e >> 2) * 8 + cq + (e & 1) >= lim[(e >> 1) & 1]) sc[e >> 2][e & 3] = -INFINITY;
+      }
+      float al[2];
+      bool grow[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float mx = max_nan(max_nan(sc[0][2 * e], sc[0][2 * e + 1]), sc[1][2 * e], sc[1][2 * e + 1]) * p.scale_log2;
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        grow[e] = !(mx <= m[e] + RESCALE_LOG2);
+        al[e] = grow[e] ? ex2f(m[e] - mx) : 1.f;  // 0 on the first key a row sees
+        if (grow[e]) m[e] = mx;
+      }
+      if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          o[i][0] *= al[0];
+          o[i][1] *= al[0];
+          o[i][2] *= al[1];
+          o[i][3] *= al[1];
+        }
+      }
+      float pr[2][4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const float nm = m[e] == -INFINITY ? 0.f : minus_max(m[e]);
+        l[e] *= al[e];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          pr[i][2 * e] = ex2f(fmaf(sc[i][2 * e], p.scale_log2, nm));
+          pr[i][2 * e + 1] = ex2f(fmaf(sc[i][2 * e + 1], p.scale_log2, nm));
+          l[e] += pr[i][2 * e] + pr[i][2 * e + 1];
+        }
+      }
+      if (!edge || least == len) {
+        uint32_t hi[4], lo[4];
+        hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
+        hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
+        hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
+        hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          const int r = lane & 15, c = 2 * i + (lane >> 4);
+          uint32_t b[4];
+          ldsm4t(b, vt + r * C::ROW + ((c ^ (r & 7)) << 4));
+          Mma<T>::run(o[2 * i], hi, b[0], b[1]);
+          Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
+          Mma<T>::run(o[2 * i], lo, b[0], b[1]);
+          Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
+        }
+      } else {
+        // Keys that only the later rows see: what an earlier row does not see, it does not meet times zero
+        // either, for V may be infinite or NaN there.
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int half = e >> 1, par = e & 1;
+#pragma unroll 1
+          for (int quad = 0; quad < 4; ++quad) {
+            const int key = half * 8 + quad * 2 + par, src = (lane & ~3) | quad;
+            const float p0 = __shfl_sync(0xffffffffu, pr[half][par], src);
+            const float p1 = __shfl_sync(0xffffffffu, pr[half][2 + par], src);
+            const bool see0 = key0 + key < lim[0], see1 = key0 + key < lim[1];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+              T v[2];
+              uint32_t raw;
+              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(vt + key * C::ROW + ((i ^ (key & 7)) << 4) + cq * 2) : "memory");
+              *reinterpret_cast<uint32_t*>(v) = raw;
+              if (see0) {
+                o[i][0] = fmaf(p0, to_f(v[0]), o[i][0]);
+                o[i][1] = fmaf(p0, to_f(v[1]), o[i][1]);
+              }
+              if (see1) {
+                o[i][2] = fmaf(p1, to_f(v[0]), o[i][2]);
+                o[i][3] = fmaf(p1, to_f(v[1]), o[i][3]);
+              }
+            }
+          }
+        }
+      }
+      __syncwarp();
+      issue(s, bad_keys[s]);
+      --left;
+      if (cu.t + 1 == cu.tiles || left == 0) {
+        // The end of a part: the output, or O / l and the log2 sum.
+        fresh = true;
+        const bool whole = t_first == 0 && cu.t + 1 == cu.tiles;
+        const int h = cu.hr / p.tiles;
+        const int64_t part = (2 * int64_t(me) + (t_first == 0 ? 1 : 0)) * p.rows;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+          const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+          int i, g;
+          if (!row_of(e, &i, &g)) continue;
+          if (whole) {
+            T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh;
+#pragma unroll
+            for (int c = 0; c < NT; ++c) {
+              T v[2] = {from_f<T>(o[c][2 * e] * inv), from_f<T>(o[c][2 * e + 1] * inv)};
+              *reinterpret_cast<uint32_t*>(orow + c * 8 + cq) = *reinterpret_cast<const uint32_t*>(v);
+            }
+          } else {
+            const int64_t row = part + rg + 8 * e;
+            if (cq == 0) p.part_l[row] = sum > 0.f ? m[e] + log2f(sum) : sum == sum ? -INFINITY : sum;
+#pragma unroll
+            for (int c = 0; c < NT; ++c)
+              *reinterpret_cast<float2*>(p.part_o + row * D + c * 8 + cq) = make_float2(o[c][2 * e] * inv, o[c][2 * e + 1] * inv);
+          }
+        }
+      }
+      if (left > 0) cu.next(starts, heads);
+    }
+  }
+}
+
+// The parts of each row weighed by 2^(their log2 sum - the largest), in a fixed order: a block per row, W warps
+// with every W-th part each, D / 32 elements per lane.  Rows without keys are zeroed here, and no others
+// touched that one warp has finished.
+template <typename T, int D, int W>
+__global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
+  constexpr int E = D / 32;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  __shared__ alignas(16) float red[W][D];
+  __shared__ float red_m[W], red_l[W];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int R = p.N * p.G;
+  const int f = int(blockIdx.x % R), h = int(blockIdx.x / R % p.Hkv), b = int(blockIdx.x / R / p.Hkv);
+  const int i = f / p.G, rt = f / 16, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
+  T* orow = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + (h * p.G + f - i * p.G) * p.oh;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int before = p.starts[b], tiles = p.starts[b + 1] - before;
+  if (tiles == 0) {
+    bool bad;
+    length_of(p, b, &bad);
+    if (warp == 0) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) orow[lane * E + e] = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
+    }
+    return;
+  }
+  const Line line = line_of(p, p.starts[p.B]);
+  const int64_t first = int64_t(before) * heads + int64_t(hr) * tiles, last = first + tiles - 1;
+  const int w0 = int(first / line.per), parts = int(last / line.per) - w0 + 1;
+  if (parts == 1) return;
+  float m = -INFINITY, l = 0.f;
+  alignas(16) float acc[E] = {};
+  // (The first part lies in its warp's second place: it holds the row's first key.)
+  auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + (f & 15); };
+  constexpr int U = 4;
+  for (int k0 = warp; k0 < parts; k0 += W * U) {
+    float pl[U];
+    Vec v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * W;
+      pl[u] = k < parts ? p.part_l[row_at(k)] : -INFINITY;
+      v[u] = reinterpret_cast<const Vec*>(p.part_o + row_at(k < parts ? k : 0) * D)[lane];
+    }
+    float mx = m;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mx = max_nan(mx, pl[u]);
+    if (mx == -INFINITY) continue;
+    const float a = exp2f(m - mx);
+    l *= a;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] *= a;
+    m = mx;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (pl[u] == -INFINITY) continue;
+      const float wgt = exp2f(pl[u] - m);
+      l += wgt;
+      const float* vv = reinterpret_cast<const float*>(&v[u]);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(wgt, vv[e], acc[e]);
+    }
+  }
+  *reinterpret_cast<Vec*>(&red[warp][lane * E]) = *reinterpret_cast<const Vec*>(acc);
+  if (lane == 0) {
+    red_m[warp] = m;
+    red_l[warp] = l;
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < D; d += W * 32) {
+    float mx = -INFINITY, sum = 0.f, val = 0.f;
+    for (int w = 0; w < W; ++w) mx = max_nan(mx, red_m[w]);
+    if (mx != -INFINITY)
+      for (int w = 0; w < W; ++w) {
+        if (red_m[w] == -INFINITY) continue;
+        const float wgt = exp2f(red_m[w] - mx);
+        sum = fmaf(wgt, red_l[w], sum);
+        val = fmaf(wgt, red[w][d], val);
+      }
+    orow[d] = from_f<T>(sum > 0.f ? val / sum : sum == sum ? 0.f : sum);
+  }
+}
+
+static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest) {
+  // (Warps past the line's end only cost their start.)
+  const int64_t most = B * Hkv * ((N * G + 15) / 16) * ((longest + KT - 1) / KT);
+  const int64_t want = (most + MIN_TILES - 1) / MIN_TILES;
+  return int(want < 1 ? 1 : want < sm_count() ? want : sm_count());
+}
+
+size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
+  if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0) return 0;
+  const int64_t rows = N * G < 16 ? N * G : 16, parts = 2 * int64_t(blocks_for(B, N, G, Hkv, longest)) * WARPS;
+  return (size_t(B + 1) * 4 + 255) / 256 * 256 + (size_t(parts * rows) * 4 + 255) / 256 * 256 + size_t(parts * rows * D) * 4;
+}
+
+template <typename T, int D>
+static cudaError_t launch_t(const Params& p, int blocks, cudaStream_t s) {
+  auto k = decode_kernel<T, D>;
+  const int most = WARPS * Cfg<D>::RING + (MAX_BATCH + 1) * 4;
+  cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), most);
+  if (e != cudaSuccess) return e;
+  k<<<unsigned(blocks), WARPS * 32, WARPS * Cfg<D>::RING + (p.B + 1) * 4, s>>>(p);
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  // The combination may be scheduled while the parts are formed; it waits for them.
+  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G;
+  const bool few = rows <= 2 * sm_count();  // then their parts are many
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned(rows));
+  cfg.blockDim = dim3(few ? 512 : 128);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 4>, p);
+}
+
+cudaError_t launch(Params p, bool f16, int D, int64_t longest, void* workspace, cudaStream_t s) {
+  const int R = p.N * p.G, blocks = blocks_for(p.B, p.N, p.G, p.Hkv, longest);
+  p.tiles = (R + 15) / 16;
+  p.rows = R < 16 ? R : 16;
+  p.total_warps = blocks * WARPS;
+  char* w = static_cast<char*>(workspace);
+  p.starts = reinterpret_cast<int*>(w);
+  w += (size_t(p.B + 1) * 4 + 255) / 256 * 256;
+  p.part_l = reinterpret_cast<float*>(w);
+  w += (size_t(2) * p.total_warps * p.rows * 4 + 255) / 256 * 256;
+  p.part_o = reinterpret_cast<float*>(w);
+  if (f16) return D == 64 ? launch_t<__half, 64>(p, blocks, s) : launch_t<__half, 128>(p, blocks, s);
+  return D == 64 ? launch_t<__nv_bfloat16, 64>(p, blocks, s) : launch_t<__nv_bfloat16, 128>(p, blocks, s);
+}
+
+}  // namespace decode
+}  // namespace l3d
+
+using namespace l3d;
+
+extern "C" size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t n, int64_t capacity,
+                                                     int64_t d) {
+  if (hkv <= 0 || hq <= 0 || hq % hkv) return 0;
+  return l3d::decode::workspace_size(b, n, hq / hkv, hkv, capacity, d);
+}
+
+extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
+                                   const l3d_tensor* table, const l3d_tensor* lengths, float scale,
+                                   const l3d_tensor* out, void* workspace, size_t workspace_bytes,
+                                   l3d_stream stream) {
+  const char* op = "l3d_paged_attention";
+  if (!q || !k_pages || !v_pages || !table || !lengths || !out)
+    return fail(L3D_E_NULL, "%s: q, k_pages, v_pages, table, lengths and out are required", op);
+  const l3d_tensor* all[] = {q, out, k_pages, v_pages};
+  for (const l3d_tensor* t : all) {
+    if (t->dtype != q->dtype || (t->dtype != L3D_BF16 && t->dtype != L3D_F16))
+      return fail(L3D_E_DTYPE, "%s: q, the pages and out all BF16 or all F16", op);
+    if (t->ndim != 4) return fail(L3D_E_SHAPE, "%s: q and out [B, N, H, D], pages [pages, size, Hkv, D]", op);
+    if (numel(t) > 0 && t->strides[3] != 1) return fail(L3D_E_ALIGN, "%s: the head dim must be contiguous", op);
+  }
+  const int64_t B = q->dims[0], N = q->dims[1], Hq = q->dims[2], D = q->dims[3];
+  const int64_t pages = k_pages->dims[0], size = k_pages->dims[1], Hkv = k_pages->dims[2];
+  if (D != 64 && D != 128) return fail(L3D_E_UNSUPPORTED, "%s: head dim must be 64 or 128", op);
+  for (int i = 0; i < 4; ++i) {
+    if (out->dims[i] != q->dims[i]) return fail(L3D_E_SHAPE, "%s: out must have q's shape", op);
+    if (v_pages->dims[i] != k_pages->dims[i] || (i == 3 && k_pages->dims[i] != D))
+      return fail(L3D_E_SHAPE, "%s: k_pages and v_pages [pages, size, Hkv, D]", op);
+  }
+  if (Hq > 0 && (Hkv <= 0 || Hq % Hkv))
+    return fail(L3D_E_SHAPE, "%s: query heads must be a multiple of the key heads", op);
+  if (table->dtype != L3D_I32) return fail(L3D_E_DTYPE, "%s: table must be I32", op);
+  if (table->ndim != 2 || table->dims[0] != B || (table->dims[1] > 1 && table->strides[1] != 1))
+    return fail(L3D_E_SHAPE, "%s: table must be [B, pages of a request] with contiguous rows", op);
+  if (lengths->dtype != L3D_I32 && lengths->dtype != L3D_I64)
+    return fail(L3D_E_DTYPE, "%s: lengths must be I32 or I64", op);
+  if (lengths->ndim != 1 || lengths->dims[0] != B || (B > 1 && lengths->strides[0] != 1))
+    return fail(L3D_E_SHAPE, "%s: lengths must be contiguous [B]", op);
+  const float scale_log2 = scale * 1.4426950408889634f;  // finite too
+  if (!(scale > 0.f) || !(scale_log2 < INFINITY))
+    return fail(L3D_E_UNSUPPORTED, "%s: scale must be positive and finite", op);
+  const int64_t big = int64_t(1) << 30, width = table->dims[1];
+  if (size <= 0 || pages > big || size > big || width > big || width * size > big || B > l3d::decode::MAX_BATCH ||
+      N > 65535 || Hq > 65535 || B * N * Hq > big || B * (width * size / 16 + 1) > big)
+    return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large (at most %d requests), or pages of no tokens", op,
+                l3d::decode::MAX_BATCH);
+  if (B * N * Hq == 0) return L3D_OK;
+  const size_t need = l3d::decode::workspace_size(B, N, Hq / Hkv, Hkv, width * size, D);
+  if (!workspace || workspace_bytes < need)
+    return fail(L3D_E_WORKSPACE, "%s: workspace of %zu bytes required", op, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(L3D_E_ALIGN, "%s: workspace must be 256-byte aligned", op);
+  for (const l3d_tensor* t : all) {
+    if (no_data(t)) return fail(L3D_E_NULL, "%s: null data pointer", op);
+    if (numel(t) == 0) continue;
+    if (reinterpret_cast<uintptr_t>(elem_ptr(t)) % 16)
+      return fail(L3D_E_ALIGN, "%s: tensors must be 16-byte aligned", op);
+    for (int d = 0; d < 3; ++d)
+      if (t->dims[d] > 1 && t->strides[d] % 8)
+        return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
+  }
+  if (no_data(table) || no_data(lengths)) return fail(L3D_E_NULL, "%s: null data pointer", op);
+  l3d::decode::Params p{};
+  p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);
+  p.q = elem_ptr(q);
+  p.out = const_cast<char*>(elem_ptr(out));
+  p.qb = q->strides[0]; p.qn = q->strides[1]; p.qh = q->strides[2];
+  p.ob = out->strides[0]; p.on = out->strides[1]; p.oh = out->strides[2];
+  p.k = elem_ptr(k_pages);
+  p.v = elem_ptr(v_pages);
+  for (int i = 0; i < 3; ++i) {
+    p.ks[i] = k_pages->strides[i];
+    p.vs[i] = v_pages->strides[i];
+  }
+  p.keys = int(pages); p.size = int(size); p.width = int(width);
+  p.table = reinterpret_cast<const int32_t*>(elem_ptr(table));
+  p.table_stride = table->strides[0];
+  p.lengths = elem_ptr(lengths);
+  p.len64 = lengths->dtype == L3D_I64;
+  p.causal = 1;
+  p.scale_log2 = scale_log2;
+  const cudaError_t e = l3d::decode::launch(p, q->dtype == L3D_F16, int(D), width * size, workspace,
+                                            reinterpret_cast<cudaStream_t>(stream));
+  return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+}

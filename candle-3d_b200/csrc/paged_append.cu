@@ -1,0 +1,339 @@
+// The step between a block's projection and its attention over a paged cache, in one pass: for the newest
+// tokens of a batch of requests, the queries and keys normed per head and rotated by the tokens' positions,
+// and the keys and values put into the cache's pages.
+//   n = x / sqrt(mean(x^2) + eps) * w                    per head (where weights are given)
+//   (n_lo, n_hi) -> (n_lo cos t - n_hi sin t, n_hi cos t + n_lo sin t),   t = position[axis(i)] * freq(i)
+// for the pairs i of a head; elements in no pair stay as they are.  The reference norms and rotates q and k
+// for two fixed models (crate/runtime/attention_math.rs:104-146, crate/runtime/trellis2_blocks.rs:85-161,
+// :306-319) and keeps no cache.
+//
+// Bound by bytes: q, k and v are read once, q and the new cache rows written once.  Eight elements (16 bytes)
+// per thread, a head's D / 8 threads side by side in a warp, so that the norm's sum and the other half of a
+// pair are a shuffle away.  A block takes a few tokens and forms their angles once for all heads, in 64 bits:
+// at position 100,000 a product in 32 bits is off by up to 4e-3 radians, as much as bf16's rounding.  What is
+// left after whole turns are taken off is at most half a turn, and goes on in 32 bits.
+#include "common.cuh"
+
+namespace l3d {
+namespace paged {
+
+constexpr int THREADS = 256;
+constexpr int MAX_TOKENS = 8;   // of one block
+constexpr int UNROLL = 3;       // rows that a thread loads before it works on the first
+
+struct Rows {                   // a [T, H, D] view
+  char* p;
+  int64_t st, sh;               // element strides
+};
+
+struct Params {
+  int T, B, Hq, Hkv;
+  int tokens;                   // of one block
+  Rows q, k, v, qo;
+  char *kp, *vp;                // pages [pages, size, Hkv, D]
+  int64_t ks[3], vs[3];         // strides of page, slot, head
+  int pages, size, width;
+  const int32_t* table;
+  int64_t table_stride;
+  const void *held, *offsets, *positions;
+  int held64, offsets64, positions64, axes;
+  int64_t position_stride, position_axis;
+  ChanVec qw, kw;
+  float eps;
+  const float2* freqs;          // high and low part of each pair's frequency
+  const int32_t* axis;
+  int pairs, half;              // half 0: neighbours; else pairs lie `half` apart in blocks of 2 half
+};
+
+__device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) {
+  return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+}
+
+// Request of token t, -1 for a token of none (before the first or behind the last).
+__device__ __forceinline__ int request_of(const Params& p, int t, int64_t* first) {
+  if (!p.offsets) {
+    const int per = p.T / p.B, b = t / per;
+    *first = int64_t(b) * per;
+    return b;
+  }
+  int lo = -1, hi = p.B;  // the last b with offsets[b] <= t
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (index_at(p.offsets, p.offsets64, mid) <= t) lo = mid;
+    else hi = mid;
+  }
+  if (lo < 0 || t >= index_at(p.offsets, p.offsets64, lo + 1)) return -1;
+  *first = index_at(p.offsets, p.offsets64, lo);
+  return lo;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
+  constexpr int LANES = D / 8;                  // threads of a row
+  constexpr int SLOTS = THREADS / LANES;        // rows of a block at a time
+  __shared__ alignas(16) float s_cos[MAX_TOKENS][D / 2], s_sin[MAX_TOKENS][D / 2];
+  __shared__ int64_t s_place[MAX_TOKENS];       // in the request's sequence; -1: a token of no request
+  __shared__ int s_page[MAX_TOKENS];            // -1: no room
+  const int t0 = blockIdx.x * p.tokens, n = min(p.tokens, p.T - t0);
+  if (threadIdx.x < n) {
+    int64_t first = 0, place = -1;
+    int page = -1;
+    const int b = request_of(p, t0 + threadIdx.x, &first);
+    if (b >= 0) {
+      place = index_at(p.held, p.held64, b) + (t0 + threadIdx.x - first);
+      if (place >= 0 && place < int64_t(p.width) * p.size) {
+        page = p.table[b * p.table_stride + place / p.size];
+        if (page >= p.pages) page = -1;
+      }
+      if (page < 0) place = max(place, int64_t(0));
+    }
+    s_place[threadIdx.x] = place;
+    s_page[threadIdx.x] = page;
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < n * p.pairs; i += THREADS) {
+    const int t = i / p.pairs, pair = i - t * p.pairs;
+    int64_t at = s_place[t];
+    if (p.positions)
+      at = index_at(p.positions, p.positions64,
+                    (t0 + t) * p.position_stride + min(max(p.axis[pair], 0), p.axes - 1) * p.position_axis);
+    const float2 f = p.freqs[pair];
+    const double turns = double(at) * (double(f.x) + double(f.y)) * 0.15915494309189533577;  // 1 / 2 pi
+    sincospif(2.f * float(turns - rint(turns)), &s_sin[t][pair], &s_cos[t][pair]);
+  }
+  __syncthreads();
+
+  const int lane = threadIdx.x % LANES, e0 = lane * 8, slot = threadIdx.x / LANES;
+  const int heads = p.Hq + 2 * p.Hkv, rows = n * heads;
+  // Where this thread's elements stand in their pairs.
+  const int block = p.half ? e0 / (2 * p.half) : 0, off = p.half ? e0 - block * 2 * p.half : 0;
+  const bool second = p.half && off >= p.half;
+  const int pair0 = p.half ? block * p.half + off - (second ? p.half : 0) : e0 / 2;
+  const int other = (second ? lane - p.half / 8 : lane + p.half / 8) & (LANES - 1);
+  const bool rotated = pair0 < p.pairs;
+  // (All threads of a warp take every turn: they meet in its shuffles.)
+  for (int r0 = 0; r0 < rows; r0 += SLOTS * UNROLL) {
+    uint4 raw[UNROLL];
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = r0 + u * SLOTS + slot;
+      raw[u] = make_uint4(0, 0, 0, 0);
+      if (r < rows) {
+        const int t = r / heads, h = r - t * heads;
+        const bool isq = h < p.Hq, isk = !isq && h < p.Hq + p.Hkv;
+        const Rows& w = isq ? p.q : isk ? p.k : p.v;
+        const int64_t at = (t0 + t) * w.st + (isq ? h : isk ? h - p.Hq : h - p.Hq - p.Hkv) * w.sh + e0;
+        raw[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(w.p) + at);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int r = min(r0 + u * SLOTS + slot, rows - 1);
+      const bool mine = r0 + u * SLOTS + slot < rows;
+      const int t = r / heads, h = r - t * heads;
+      const bool isq = h < p.Hq, isk = !isq && h < p.Hq + p.Hkv;
+      float x[8];
+      unpack(raw[u], x, T());
+      if (p.qw.ptr) {
+        float sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+#pragma unroll
+        for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float inv = 1.f / sqrtf(sum * (1.f / D) + p.eps);
+        if (isq || isk) {
+          float w[8];
+          load_chan<8>(isq ? p.qw : p.kw, isq ? h : h - p.Hq, e0, w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+        }
+      }
+      float y[8];
+      if (p.half == 0) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool in = pair0 + e < p.pairs;
+          const float c = in ? s_cos[t][pair0 + e] : 1.f, s = in ? s_sin[t][pair0 + e] : 0.f;
+          y[2 * e] = in ? x[2 * e] * c - x[2 * e + 1] * s : x[2 * e];
+          y[2 * e + 1] = in ? x[2 * e + 1] * c + x[2 * e] * s : x[2 * e + 1];
+        }
+      } else {
+        float z[8];  // the other elements of the pairs
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = __shfl_sync(0xffffffffu, x[e], other, LANES);
+        if (rotated) {
+          float c[8], s[8];
+#pragma unroll
+          for (int e = 0; e < 8; e += 4) {
+            *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(&s_cos[t][pair0 + e]);
+            *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(&s_sin[t][pair0 + e]);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], c[e], second ? z[e] * s[e] : -(z[e] * s[e]));
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = x[e];
+        }
+      }
+      const int64_t place = s_place[t];
+      const int page = s_page[t];
+      if (!mine || place < 0) continue;  // (the shuffles are behind us)
+      if (isq) {
+        if (page < 0) {  // no room: nothing is stored, and the request's attention is not finite
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fffffff);
+        }
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.qo.p) + (t0 + t) * p.qo.st + h * p.qo.sh + e0) = pack(y, T());
+      } else if (page >= 0) {
+        const int hk = isk ? h - p.Hq : h - p.Hq - p.Hkv;
+        const int64_t in_page = place % p.size;
+        if (isk)
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.kp) + page * p.ks[0] + in_page * p.ks[1] + hk * p.ks[2] + e0) = pack(y, T());
+        else
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.vp) + page * p.vs[0] + in_page * p.vs[1] + hk * p.vs[2] + e0) = raw[u];
+      }
+    }
+  }
+}
+
+}  // namespace paged
+}  // namespace l3d
+
+using namespace l3d;
+
+extern "C" int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const l3d_tensor* v,
+                                const l3d_tensor* q_weight, const l3d_tensor* k_weight, float eps,
+                                const l3d_tensor* freqs, const l3d_tensor* axes, int half,
+                                const l3d_tensor* positions, const l3d_tensor* table,
+                                const l3d_tensor* held, const l3d_tensor* offsets,
+                                const l3d_tensor* q_out, const l3d_tensor* k_pages,
+                                const l3d_tensor* v_pages, l3d_stream stream) {
+  using namespace l3d::paged;
+  const char* op = "l3d_paged_append";
+  if (!q || !k || !v || !table || !held || !q_out || !k_pages || !v_pages)
+    return fail(L3D_E_NULL, "%s: q, k, v, table, held, q_out, k_pages and v_pages are required", op);
+  if (!q_weight != !k_weight) return fail(L3D_E_NULL, "%s: q_weight and k_weight come together", op);
+  if (!freqs != !axes) return fail(L3D_E_NULL, "%s: freqs and axes come together", op);
+  if (positions && !freqs) return fail(L3D_E_SHAPE, "%s: positions need freqs", op);
+  const l3d_tensor* all[] = {q, k, v, q_out, k_pages, v_pages};
+  for (int i = 0; i < 6; ++i) {
+    const l3d_tensor* t = all[i];
+    const int nd = i < 4 ? 3 : 4;
+    if (t->dtype != q->dtype || (t->dtype != L3D_BF16 && t->dtype != L3D_F16))
+      return fail(L3D_E_DTYPE, "%s: q, k, v, q_out and the pages all BF16 or all F16", op);
+    if (t->ndim != nd)
+      return fail(L3D_E_SHAPE, "%s: q, k, v, q_out [T, H, D], pages [pages, size, H, D]", op);
+    if (numel(t) > 0 && t->strides[nd - 1] != 1)
+      return fail(L3D_E_ALIGN, "%s: the head dim must be contiguous", op);
+  }
+  const int64_t T = q->dims[0], Hq = q->dims[1], D = q->dims[2], Hkv = k->dims[1];
+  const int64_t pages = k_pages->dims[0], size = k_pages->dims[1], B = table->ndim == 2 ? table->dims[0] : 0;
+  if (D != 64 && D != 128) return fail(L3D_E_UNSUPPORTED, "%s: head dim must be 64 or 128", op);
+  for (int i = 0; i < 3; ++i) {
+    if (q_out->dims[i] != q->dims[i]) return fail(L3D_E_SHAPE, "%s: q_out must have q's shape", op);
+    if (v->dims[i] != k->dims[i]) return fail(L3D_E_SHAPE, "%s: k and v [T, Hkv, D]", op);
+  }
+  if (k->dims[0] != T || k->dims[2] != D) return fail(L3D_E_SHAPE, "%s: k and v [T, Hkv, D]", op);
+  for (int i = 0; i < 4; ++i)
+    if (v_pages->dims[i] != k_pages->dims[i] || (i == 2 && k_pages->dims[i] != Hkv) || (i == 3 && k_pages->dims[i] != D))
+      return fail(L3D_E_SHAPE, "%s: k_pages and v_pages [pages, size, Hkv, D]", op);
+  if (table->ndim != 2 || table->dtype != L3D_I32 || (table->dims[1] > 1 && table->strides[1] != 1))
+    return fail(table->ndim == 2 && table->dtype != L3D_I32 ? L3D_E_DTYPE : L3D_E_SHAPE,
+                "%s: table must be [B, pages of a request] I32 with contiguous rows", op);
+  auto index_list = [&](const l3d_tensor* t, int64_t n) {
+    return (t->dtype == L3D_I32 || t->dtype == L3D_I64) && t->ndim == 1 && t->dims[0] == n && (n <= 1 || t->strides[0] == 1);
+  };
+  if (!index_list(held, B)) return fail(L3D_E_SHAPE, "%s: held must be contiguous [B] I32 or I64", op);
+  if (offsets && !index_list(offsets, B + 1))
+    return fail(L3D_E_SHAPE, "%s: offsets must be contiguous [B + 1] I32 or I64", op);
+  if (!offsets && (B > 0 ? T % B != 0 : T > 0))
+    return fail(L3D_E_SHAPE, "%s: without offsets the tokens must divide evenly among the requests", op);
+  const int64_t big = int64_t(1) << 30;
+  if (T > big || B > big || pages > big || size > big || table->dims[1] > big || Hq + 2 * Hkv > 65535 || size <= 0)
+    return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large, or pages of no tokens", op);
+  if (!(eps >= 0.f) || !(eps < INFINITY)) return fail(L3D_E_UNSUPPORTED, "%s: eps must be finite and >= 0", op);
+  int64_t pairs = 0;
+  if (freqs) {
+    pairs = freqs->dims[0];
+    if (freqs->dtype != L3D_F32 || axes->dtype != L3D_I32) return fail(L3D_E_DTYPE, "%s: freqs F32, axes I32", op);
+    if (freqs->ndim != 2 || freqs->dims[1] != 2 || axes->ndim != 1 || axes->dims[0] != pairs || pairs < 1 ||
+        2 * pairs > D || freqs->strides[1] != 1 || (pairs > 1 && (freqs->strides[0] != 2 || axes->strides[0] != 1)))
+      return fail(L3D_E_SHAPE, "%s: freqs [pairs, 2] and axes [pairs], contiguous, at most D / 2 pairs", op);
+    if (half < 0 || half % 8 || (half && pairs % half))
+      return fail(L3D_E_UNSUPPORTED, "%s: half must be 0 or a multiple of 8 that divides the pairs", op);
+    if (no_data(freqs) || no_data(axes) || reinterpret_cast<uintptr_t>(elem_ptr(freqs)) % 8)
+      return fail(L3D_E_ALIGN, "%s: freqs must be 8-byte aligned", op);
+  }
+  if (positions) {
+    if (positions->dtype != L3D_I32 && positions->dtype != L3D_I64)
+      return fail(L3D_E_DTYPE, "%s: positions must be I32 or I64", op);
+    if (positions->ndim != 2 || positions->dims[0] != T || positions->dims[1] < 1)
+      return fail(L3D_E_SHAPE, "%s: positions must be [T, axes]", op);
+  }
+  Params p{};
+  if (q_weight) {
+    bool aligned = true;
+    const l3d_tensor* w[] = {q_weight, k_weight};
+    const char* names[] = {"q_weight", "k_weight"};
+    for (int i = 0; i < 2; ++i) {
+      if (int e = make_chanvec(w[i], names[i], D, i ? Hkv : Hq, i ? &p.kw : &p.qw, &aligned)) return e;
+      if (!aligned) return fail(L3D_E_ALIGN, "%s: %s must be 16-byte aligned", op, names[i]);
+    }
+  }
+  if (T == 0) return L3D_OK;
+  for (const l3d_tensor* t : all) {
+    if (no_data(t)) return fail(L3D_E_NULL, "%s: null data pointer", op);
+    if (numel(t) == 0) continue;
+    if (reinterpret_cast<uintptr_t>(elem_ptr(t)) % 16)
+      return fail(L3D_E_ALIGN, "%s: tensors must be 16-byte aligned", op);
+    for (int d = 0; d < t->ndim - 1; ++d)
+      if (t->dims[d] > 1 && t->strides[d] % 8)
+        return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
+  }
+  const l3d_tensor* lists[] = {table, held, offsets, positions};
+  for (const l3d_tensor* t : lists)
+    if (t && no_data(t)) return fail(L3D_E_NULL, "%s: null data pointer", op);
+  auto rows = [](const l3d_tensor* t) {
+    return Rows{const_cast<char*>(elem_ptr(t)), t->strides[0], t->strides[1]};
+  };
+  p.T = int(T); p.B = int(B); p.Hq = int(Hq); p.Hkv = int(Hkv);
+  p.q = rows(q); p.k = rows(k); p.v = rows(v); p.qo = rows(q_out);
+  p.kp = const_cast<char*>(elem_ptr(k_pages));
+  p.vp = const_cast<char*>(elem_ptr(v_pages));
+  for (int i = 0; i < 3; ++i) {
+    p.ks[i] = k_pages->strides[i];
+    p.vs[i] = v_pages->strides[i];
+  }
+  p.pages = int(pages); p.size = int(size); p.width = int(table->dims[1]);
+  p.table = reinterpret_cast<const int32_t*>(elem_ptr(table));
+  p.table_stride = table->strides[0];
+  p.held = elem_ptr(held);
+  p.held64 = held->dtype == L3D_I64;
+  p.offsets = offsets ? elem_ptr(offsets) : nullptr;
+  p.offsets64 = offsets && offsets->dtype == L3D_I64;
+  if (positions) {
+    p.positions = elem_ptr(positions);
+    p.positions64 = positions->dtype == L3D_I64;
+    p.axes = int(positions->dims[1]);
+    p.position_stride = positions->strides[0];
+    p.position_axis = positions->strides[1];
+  }
+  p.eps = eps;
+  p.freqs = freqs ? reinterpret_cast<const float2*>(elem_ptr(freqs)) : nullptr;
+  p.axis = axes ? reinterpret_cast<const int32_t*>(elem_ptr(axes)) : nullptr;
+  p.pairs = int(pairs);
+  p.half = freqs ? half : 0;
+  // One token per block as long as the device is not full, so that a few tokens spread over it.
+  const int64_t per = T / (8 * int64_t(sm_count()));
+  p.tokens = per < 1 ? 1 : per > MAX_TOKENS ? MAX_TOKENS : int(per);
+  const unsigned grid = unsigned((T + p.tokens - 1) / p.tokens);
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (q->dtype == L3D_BF16) {
+    if (D == 64) append_kernel<__nv_bfloat16, 64><<<grid, THREADS, 0, s>>>(p);
+    else append_kernel<__nv_bfloat16, 128><<<grid, THREADS, 0, s>>>(p);
+  } else {
+    if (D == 64) append_kernel<__half, 64><<<grid, THREADS, 0, s>>>(p);
+    else append_kernel<__half, 128><<<grid, THREADS, 0, s>>>(p);
+  }
+  return check_launch(op);
+}

@@ -6,6 +6,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <exception>
@@ -27,15 +28,22 @@ int dtype_code(at::ScalarType t) {
   }
 }
 
-PyObject* describe(PyObject* o, bool on_device) {
+// `device`: ANY of them, the host too; CUDA; or a device's index.
+constexpr int ANY = -2, CUDA = -1;
+
+PyObject* describe(PyObject* o, int device) {
   if (o == Py_None) Py_RETURN_NONE;
   if (!THPVariable_Check(o)) {
     PyErr_SetString(PyExc_TypeError, "a tensor or None expected");
     return nullptr;
   }
   const at::Tensor& t = THPVariable_Unpack(o);
-  if (on_device && !t.is_cuda()) {
+  if (device != ANY && !t.is_cuda()) {
     PyErr_SetString(PyExc_ValueError, "libl3dops ops take CUDA tensors (no CPU implementation exists)");
+    return nullptr;
+  }
+  if (device >= 0 && t.get_device() != device) {
+    PyErr_Format(PyExc_ValueError, "a tensor lies on cuda:%d, the current device is cuda:%d", int(t.get_device()), device);
     return nullptr;
   }
   const int code = dtype_code(t.scalar_type());
@@ -72,22 +80,36 @@ PyObject* guarded(F f) {
 }
 
 PyObject* packed(PyObject*, PyObject* o) {
-  return guarded([&] { return describe(o, false); });
+  return guarded([&] { return describe(o, ANY); });
+}
+
+PyObject* describe_all(PyObject* const* args, Py_ssize_t n, int device) {
+  PyObject* out = PyTuple_New(n);
+  if (!out) return nullptr;
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    PyObject* b = describe(args[i], device);
+    if (!b) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, i, b);
+  }
+  return out;
 }
 
 PyObject* packs(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  return guarded([&] { return describe_all(args, n, CUDA); });
+}
+
+PyObject* packs_here(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    PyObject* out = PyTuple_New(n);
-    if (!out) return nullptr;
+    // (Asked of the runtime only once a tensor is on a device: on a machine without one that is the error.)
     for (Py_ssize_t i = 0; i < n; ++i) {
-      PyObject* b = describe(args[i], true);
-      if (!b) {
-        Py_DECREF(out);
-        return nullptr;
-      }
-      PyTuple_SET_ITEM(out, i, b);
+      if (!THPVariable_Check(args[i]) || !THPVariable_Unpack(args[i]).is_cuda()) continue;
+      const c10::impl::VirtualGuardImpl impl(c10::DeviceType::CUDA);
+      return describe_all(args, n, int(impl.getDevice().index()));
     }
-    return out;
+    return describe_all(args, n, CUDA);
   });
 }
 
@@ -124,6 +146,8 @@ PyMethodDef methods[] = {
     {"packed", packed, METH_O, "l3d_tensor of a tensor view as bytes (None -> None)"},
     {"packs", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(packs)), METH_FASTCALL,
      "packed of each argument, which must be on a CUDA device, as a tuple"},
+    {"packs_here", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(packs_here)), METH_FASTCALL,
+     "packed of each argument, which must be on the current CUDA device, as a tuple"},
     {"empty", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(empty)), METH_FASTCALL,
      "contiguous tensor of the first argument's type and device, of its shape or the sizes given"},
     {"workspace", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(workspace)), METH_FASTCALL,

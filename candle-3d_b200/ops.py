@@ -16,7 +16,8 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import call, desc, empty, packed, packs, ref, stream_handle, stream_of, workspace
+from ._lib import (call, desc, empty, packed, packs, packs_here, ref, stream_handle, stream_of,
+                   workspace)
 
 ACT = {"none": 0, "silu": 1, "gelu_erf": 2, "gelu_tanh": 3}
 
@@ -658,3 +659,92 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
          dsh, dsc, eps if post_eps is None else post_eps, eps, dr, dy, stream_of(x))
     _check_status("l3d_sandwich_residual_norm", x, check)
     return r, y
+
+
+# ------------------------------------------- decoding over a paged cache
+class RotaryAxes:
+    """Frequencies of a rotation by positions on several axes (time, height, width;
+    or one), laid out once for `paged_append`: sections[a] pairs of a head turn with
+    axis a, pair j of its n at theta^(-j / n) radians a position.  Pairs are taken in
+    the axes' order; layout "interleaved": pair i is elements 2i and 2i + 1; "half":
+    i and i + pairs (the pairs a multiple of 8); "axis": each axis a block of its
+    own, its halves paired (equal sections, multiples of 8).  Elements past twice the
+    pairs are not rotated.  `frequencies` (f64 values, one per pair) replaces theta's."""
+
+    def __init__(self, head_dim, sections, theta=10000.0, layout="half", frequencies=None, device="cuda"):
+        sections = tuple(int(n) for n in sections)
+        pairs = sum(sections)
+        if not sections or min(sections) < 1 or 2 * pairs > head_dim:
+            raise ValueError(f"RotaryAxes: sections {sections} do not fit a head of {head_dim}")
+        if layout not in ("half", "interleaved", "axis"):
+            raise ValueError(f"RotaryAxes: unknown layout {layout!r}")
+        if layout == "axis" and len(set(sections)) > 1:
+            raise ValueError("RotaryAxes: layout 'axis' needs equal sections")
+        self.half = {"interleaved": 0, "half": pairs, "axis": sections[0]}[layout]
+        if self.half % 8:
+            raise ValueError(f"RotaryAxes: layout {layout!r} pairs elements {self.half} apart, "
+                             "which must be a multiple of 8")
+        if frequencies is None:
+            frequencies = np.concatenate([float(theta) ** (-np.arange(n) / n) for n in sections])
+        f = np.asarray(frequencies, np.float64)
+        if f.shape != (pairs,) or not np.isfinite(f).all():
+            raise ValueError(f"RotaryAxes: {pairs} finite frequencies expected")
+        high = f.astype(np.float32)
+        self.head_dim, self.sections, self.axes = head_dim, sections, len(sections)
+        self.freqs = torch.from_numpy(np.stack([high, (f - high).astype(np.float32)], 1)).to(device)
+        self.axis = torch.from_numpy(np.repeat(np.arange(self.axes), sections).astype(np.int32)).to(device)
+
+
+def paged_append(q, k, v, k_pages, v_pages, table, held, offsets=None, rope=None, positions=None,
+                 q_weight=None, k_weight=None, eps=1e-6, out=None):
+    """The newest tokens of a batch of requests into a paged cache, one pass: q and k
+    RMS-normed per head (with weights [D] or [H, D]) and rotated (`rope`, a
+    RotaryAxes, by `positions` [T, axes], or by each token's place in its request), k
+    and v put into the pages; returns q.  q [T, Hq, D], k and v [T, Hkv, D], pages
+    [pages, size, Hkv, D]; request b holds held[b] tokens already, and its next ones,
+    rows offsets[b] .. offsets[b + 1] - 1 (offsets None: T / B rows each), go behind
+    them, place p to slot p % size of page table[b, p / size] (table int32).  A token
+    without a place in the cache is not stored, and its q comes out NaN (held and
+    table lie on the device: no error can be raised without waiting for them)."""
+    if out is None:
+        out = empty(q, *q.shape)
+    if rope is None:
+        freqs = axis = None
+        half = 0
+    else:
+        freqs, axis, half = rope.freqs, rope.axis, rope.half
+        if q.shape[-1] != rope.head_dim:
+            raise ValueError(f"heads of {q.shape[-1]}, the rotation is for {rope.head_dim}")
+        if positions is not None:
+            if positions.dim() == 1:
+                positions = positions.unsqueeze(1)
+            if positions.shape[-1] != rope.axes:
+                raise ValueError(f"positions on {positions.shape[-1]} axes, the rotation has {rope.axes}")
+    dq, dk, dv, dqw, dkw, df, da, dp, dt, dh, do, dout, dkp, dvp = packs_here(
+        q, k, v, q_weight, k_weight, freqs, axis, positions, table, held, offsets, out, k_pages, v_pages)
+    call("l3d_paged_append", dq, dk, dv, dqw, dkw, eps, df, da, half, dp, dt, dh, do, dout, dkp, dvp,
+         stream_of(q))
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None):
+    """exact_sdpa_heads (crate/runtime/attention_math.rs:199-259) of each request's
+    newest tokens over its paged cache, which holds them already: q [B, N, Hq, D],
+    or [B, Hq, D] for one token each; row i of request b sees the first
+    lengths[b] - N + 1 + i of its keys (pages and table as for `paged_append`).
+    BF16 or F16, D = 64 or 128; made for one token or a few: every 16 rows of a key
+    head (N * Hq / Hkv) read its keys once."""
+    if out is None:
+        out = empty(q, *q.shape)
+    one = q.dim() == 3
+    dq, dk, dv, dt, dl, do = packs_here(q.unsqueeze(1) if one else q, k_pages, v_pages, table, lengths,
+                                        out.unsqueeze(1) if out.dim() == 3 else out)
+    need = 0
+    if table.dim() == 2 and k_pages.dim() == 4:  # (the entry refuses anything else)
+        B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
+        need = _lib.lib().l3d_paged_attention_workspace_size(
+            B, H, k_pages.shape[2], 1 if one else q.shape[1], table.shape[1] * k_pages.shape[1], D)
+    ws = workspace(q, need)
+    call("l3d_paged_attention", dq, dk, dv, dt, dl, q.shape[-1] ** -0.5 if scale is None else float(scale), do, ws.data_ptr(), need,
+         stream_of(q))
+    return out

@@ -494,6 +494,59 @@ int l3d_sandwich_residual_norm(const l3d_tensor* x, const l3d_tensor* h, int nor
                                const l3d_tensor* scale, float post_eps, float eps,
                                const l3d_tensor* r_out, const l3d_tensor* y, l3d_stream stream);
 
+/* The step between a block's projection and its attention over a paged cache,
+ * one pass: per-head RMS norm of q and k, rotation by the tokens' positions, and
+ * k and v put into the cache.  q and q_out [T, Hq, D], k and v [T, Hkv, D] (views
+ * of one projection are accepted; q_out may be q), k_pages and v_pages
+ * [pages, size, Hkv, D] with any strides.  Token i of request b goes to place
+ * held[b] + i of its sequence: slot place % size of page table[b, place / size]
+ * (table [B, W] I32, held [B] I32/I64: the tokens already there).  offsets
+ * [B + 1] I32/I64, not decreasing: request b's tokens are rows offsets[b] ..
+ * offsets[b + 1] - 1, rows before the first and behind the last are left as they
+ * are; NULL: B equal groups.  A token whose place lies past its table, or whose
+ * page is not one of the cache, is not stored and its q_out is NaN.  No slot may
+ * be given to two tokens of a call.
+ * q_weight and k_weight [D] or [H, D] (or both NULL: no norm): x / sqrt(mean(x^2)
+ * + eps) * w.  freqs [pairs, 2] F32 (the high and the low part of each pair's
+ * frequency, radians a position) and axes [pairs] I32 (or both NULL: no
+ * rotation); positions [T, A] I32/I64, NULL: the token's place, for every axis;
+ * angles are formed in 64 bits, to 2^-48 of themselves.  half 0: pair i is elements 2i and 2i + 1; else a
+ * multiple of 8 that divides the pairs: pairs lie half apart in blocks of 2 half
+ * elements (half = pairs: one block).  Elements in no pair are not rotated.
+ * BF16 or F16, D = 64 or 128, one rounding.  The reference's forms for fixed
+ * models: crate/runtime/attention_math.rs:104-146,
+ * crate/runtime/trellis2_blocks.rs:85-161, :306-319. */
+int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const l3d_tensor* v,
+                     const l3d_tensor* q_weight, const l3d_tensor* k_weight, float eps,
+                     const l3d_tensor* freqs, const l3d_tensor* axes, int half,
+                     const l3d_tensor* positions, const l3d_tensor* table, const l3d_tensor* held,
+                     const l3d_tensor* offsets, const l3d_tensor* q_out,
+                     const l3d_tensor* k_pages, const l3d_tensor* v_pages, l3d_stream stream);
+
+/* Workspace bytes for l3d_paged_attention; capacity: the keys that a request's
+ * row of the table has room for (W * size). */
+size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t n,
+                                          int64_t capacity, int64_t d);
+
+/* The attention core (exact_sdpa_heads, crate/runtime/attention_math.rs:199-259)
+ * of the newest N tokens of each request over its paged cache, which holds them
+ * already: q and out [B, N, Hq, D]; row i of request b sees the keys
+ * j < lengths[b] - N + 1 + i, key j in slot j % size of page table[b, j / size].
+ * k_pages, v_pages, table as for l3d_paged_append; lengths [B] I32/I64, negative
+ * ones taken as 0.  Made for one token, or a few: every 16 rows of a key head
+ * (N * Hq / Hkv of them) read its keys once.  What a row does not see does not
+ * reach it, whatever it holds.  A row with no keys gives zeros; one that sees a
+ * score that is NaN or +inf, or a key whose page is not one of the cache, and all
+ * rows of a request whose length is more than its table has room for, NaN.  BF16
+ * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
+ * otherwise free in multiples of 16 bytes; softmax, sums and probabilities in f32
+ * (the latter enter the second product as two 16-bit parts).  scale must be
+ * positive, and scale * log2(e) finite. */
+int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
+                        const l3d_tensor* table, const l3d_tensor* lengths, float scale,
+                        const l3d_tensor* out, void* workspace, size_t workspace_bytes,
+                        l3d_stream stream);
+
 /* ---- GGUF tensor index (the on-disk format feeding a13) ------------------------ */
 
 /* One tensor of a GGUF file.  name points into the caller's buffer (not

@@ -1,0 +1,154 @@
+"""CPU: the entries of a paged cache refuse invalid requests on the host, before any launch."""
+import math
+
+import numpy as np
+import pytest
+
+from test_serving_checks import E_ALIGN, E_DTYPE, E_NULL, E_SHAPE, E_UNSUPPORTED, E_WORKSPACE, _refused, _zeros
+
+
+def _append_args(**over):
+    T, Hq, Hkv, D, B = 6, 4, 2, 64, 3
+    a = dict(q=_zeros(T, Hq, D), k=_zeros(T, Hkv, D), v=_zeros(T, Hkv, D), q_weight=_zeros(D), k_weight=_zeros(D),
+             eps=1e-6, freqs=_zeros(32, 2, dtype="float32"), axes=_zeros(32, dtype="int32"), half=32,
+             positions=_zeros(T, 2, dtype="int32"), table=_zeros(B, 5, dtype="int32"), held=_zeros(B, dtype="int32"),
+             offsets=_zeros(B + 1, dtype="int32"), q_out=_zeros(T, Hq, D), k_pages=_zeros(7, 16, Hkv, D),
+             v_pages=_zeros(7, 16, Hkv, D))
+    assert not set(over) - set(a)
+    return [*(a | over).values(), None]
+
+
+@pytest.mark.parametrize("over,code,word", [
+    (dict(q=None), E_NULL, "required"),
+    (dict(table=None), E_NULL, "required"),
+    (dict(held=None), E_NULL, "required"),
+    (dict(k_weight=None), E_NULL, "together"),
+    (dict(axes=None), E_NULL, "together"),
+    (dict(freqs=None, axes=None), E_SHAPE, "positions need freqs"),
+    (dict(q=_zeros(6, 4, 64, dtype="float32")), E_DTYPE, "BF16"),
+    (dict(k_pages=_zeros(7, 16, 2, 64, dtype="float16")), E_DTYPE, "F16"),
+    (dict(v=_zeros(6, 128)), E_SHAPE, "[T, H, D]"),
+    (dict(k_pages=_zeros(7, 32, 64)), E_SHAPE, "[pages, size, H, D]"),
+    (dict(k=_zeros(6, 64, 2).transpose(1, 2)), E_ALIGN, "contiguous"),
+    (dict(q=_zeros(6, 4, 32), q_out=_zeros(6, 4, 32)), E_UNSUPPORTED, "64 or 128"),
+    (dict(q_out=_zeros(6, 5, 64)), E_SHAPE, "q_out"),
+    (dict(v=_zeros(6, 3, 64)), E_SHAPE, "k and v"),
+    (dict(k=_zeros(5, 2, 64), v=_zeros(5, 2, 64)), E_SHAPE, "k and v"),
+    (dict(v_pages=_zeros(7, 17, 2, 64)), E_SHAPE, "k_pages and v_pages"),
+    (dict(k_pages=_zeros(7, 16, 3, 64), v_pages=_zeros(7, 16, 3, 64)), E_SHAPE, "k_pages and v_pages"),
+    (dict(k_pages=_zeros(7, 0, 2, 64), v_pages=_zeros(7, 0, 2, 64)), E_UNSUPPORTED, "pages of no tokens"),
+    (dict(table=_zeros(3, 5, dtype="int64")), E_DTYPE, "table"),
+    (dict(table=_zeros(15, dtype="int32")), E_SHAPE, "table"),
+    (dict(table=_zeros(5, 3, dtype="int32").t()), E_SHAPE, "contiguous rows"),
+    (dict(held=_zeros(4, dtype="int32")), E_SHAPE, "held"),
+    (dict(held=_zeros(3, dtype="float32")), E_SHAPE, "held"),
+    (dict(offsets=_zeros(3, dtype="int32")), E_SHAPE, "offsets"),
+    (dict(offsets=_zeros(8, dtype="int32")[::2]), E_SHAPE, "offsets"),
+    (dict(offsets=None, q=_zeros(7, 4, 64), k=_zeros(7, 2, 64), v=_zeros(7, 2, 64), q_out=_zeros(7, 4, 64),
+          positions=None), E_SHAPE, "divide evenly"),
+    (dict(eps=-1.0), E_UNSUPPORTED, "eps"),
+    (dict(eps=math.nan), E_UNSUPPORTED, "eps"),
+    (dict(freqs=_zeros(32, 2)), E_DTYPE, "freqs"),
+    (dict(freqs=_zeros(33, 2, dtype="float32"), axes=_zeros(33, dtype="int32")), E_SHAPE, "D / 2 pairs"),
+    (dict(axes=_zeros(31, dtype="int32")), E_SHAPE, "pairs"),
+    (dict(half=12), E_UNSUPPORTED, "half"),
+    (dict(half=24), E_UNSUPPORTED, "half"),
+    (dict(half=-8), E_UNSUPPORTED, "half"),
+    (dict(positions=_zeros(6, 2, dtype="float32")), E_DTYPE, "positions"),
+    (dict(positions=_zeros(5, 2, dtype="int32")), E_SHAPE, "positions"),
+    (dict(q_weight=_zeros(63)), E_SHAPE, "q_weight"),
+    (dict(k_weight=_zeros(3, 64)), E_SHAPE, "k_weight"),
+    (dict(q=_zeros(6, 4, 68)[..., 2:66]), E_ALIGN, "16-byte"),
+    (dict(k=_zeros(6, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
+])
+def test_paged_append_refuses(pkg, over, code, word):
+    _refused(pkg, "l3d_paged_append", _append_args(**over), code, word)
+
+
+def _paged_args(**over):
+    B, N, Hq, Hkv, D = 3, 2, 4, 2, 64
+    a = dict(q=_zeros(B, N, Hq, D), k_pages=_zeros(7, 16, Hkv, D), v_pages=_zeros(7, 16, Hkv, D),
+             table=_zeros(B, 5, dtype="int32"), lengths=_zeros(B, dtype="int32"), scale=0.125,
+             out=_zeros(B, N, Hq, D), workspace=256, bytes=1 << 30)
+    assert not set(over) - set(a)
+    return [*(a | over).values(), None]
+
+
+@pytest.mark.parametrize("over,code,word", [
+    (dict(q=None), E_NULL, "required"),
+    (dict(lengths=None), E_NULL, "required"),
+    (dict(q=_zeros(3, 2, 4, 64, dtype="float32")), E_DTYPE, "BF16"),
+    (dict(v_pages=_zeros(7, 16, 2, 64, dtype="float16")), E_DTYPE, "F16"),
+    (dict(q=_zeros(3, 4, 64)), E_SHAPE, "[B, N, H, D]"),
+    (dict(q=_zeros(3, 2, 64, 4).transpose(2, 3)), E_ALIGN, "contiguous"),
+    (dict(q=_zeros(3, 2, 4, 96), out=_zeros(3, 2, 4, 96)), E_UNSUPPORTED, "64 or 128"),
+    (dict(out=_zeros(3, 1, 4, 64)), E_SHAPE, "out"),
+    (dict(v_pages=_zeros(8, 16, 2, 64)), E_SHAPE, "k_pages and v_pages"),
+    (dict(k_pages=_zeros(7, 16, 2, 128), v_pages=_zeros(7, 16, 2, 128)), E_SHAPE, "k_pages and v_pages"),
+    (dict(q=_zeros(3, 2, 3, 64), out=_zeros(3, 2, 3, 64)), E_SHAPE, "multiple of the key heads"),
+    (dict(table=_zeros(3, 5, dtype="int64")), E_DTYPE, "table"),
+    (dict(table=_zeros(2, 5, dtype="int32")), E_SHAPE, "table"),
+    (dict(table=_zeros(5, 3, dtype="int32").t()), E_SHAPE, "contiguous rows"),
+    (dict(lengths=_zeros(3, dtype="float32")), E_DTYPE, "lengths"),
+    (dict(lengths=_zeros(4, dtype="int32")), E_SHAPE, "lengths"),
+    (dict(lengths=_zeros(6, dtype="int32")[::2]), E_SHAPE, "lengths"),
+    (dict(scale=0.0), E_UNSUPPORTED, "scale"),
+    (dict(scale=math.nan), E_UNSUPPORTED, "scale"),
+    (dict(scale=2.9e38), E_UNSUPPORTED, "scale"),
+    (dict(k_pages=_zeros(7, 0, 2, 64), v_pages=_zeros(7, 0, 2, 64)), E_UNSUPPORTED, "no tokens"),
+    (dict(q=_zeros(4097, 1, 4, 64), out=_zeros(4097, 1, 4, 64), table=_zeros(4097, 5, dtype="int32"),
+          lengths=_zeros(4097, dtype="int32")), E_UNSUPPORTED, "4096"),
+    (dict(bytes=0), E_WORKSPACE, "workspace"),
+    (dict(workspace=None), E_WORKSPACE, "workspace"),
+    (dict(workspace=264), E_ALIGN, "256"),
+    (dict(k_pages=_zeros(7, 16, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
+])
+def test_paged_attention_refuses(pkg, over, code, word):
+    _refused(pkg, "l3d_paged_attention", _paged_args(**over), code, word)
+
+
+def test_nothing_to_do(pkg):
+    """Empty batches are no error, and need no device."""
+    L = pkg._lib
+    e = {n: _zeros(0, 2, 4, 64) for n in ("q", "out")}
+    args = _paged_args(**e, table=_zeros(0, 5, dtype="int32"), lengths=_zeros(0, dtype="int32"), workspace=None, bytes=0)
+    assert L.lib().l3d_paged_attention(*[L.packed(a) if hasattr(a, "dim") else a for a in args]) == 0
+    assert L.lib().l3d_paged_attention_workspace_size(0, 4, 2, 1, 80, 64) == 0
+    assert L.lib().l3d_paged_attention_workspace_size(3, 5, 2, 1, 80, 64) == 0
+    args = _append_args(q=_zeros(0, 4, 64), k=_zeros(0, 2, 64), v=_zeros(0, 2, 64), q_out=_zeros(0, 4, 64),
+                        positions=_zeros(0, 2, dtype="int32"))
+    assert L.lib().l3d_paged_append(*[L.packed(a) if hasattr(a, "dim") else a for a in args]) == 0
+
+
+def test_rotary_axes(pkg):
+    R = pkg.ops.RotaryAxes
+    r = R(128, (16, 24, 24), theta=1e6, device="cpu")
+    assert r.half == 64 and r.axes == 3 and r.axis.tolist() == [0] * 16 + [1] * 24 + [2] * 24
+    want = np.concatenate([1e6 ** (-np.arange(n) / n) for n in (16, 24, 24)])
+    got = r.freqs.double().sum(1).numpy()
+    assert np.abs(got / want - 1).max() < 2.0 ** -46  # the low part holds what the high one rounds off
+    assert R(64, (16, 16), layout="axis", device="cpu").half == 16
+    assert R(64, (5, 6), layout="interleaved", device="cpu").half == 0
+    f = np.linspace(0.1, 1, 8)
+    assert np.allclose(R(64, (8,), frequencies=f, device="cpu").freqs.double().sum(1).numpy(), f, rtol=1e-14)
+    for bad, word in (((64, (33,)), "do not fit"), ((64, ()), "do not fit"), ((64, (0, 8)), "do not fit"),
+                      ((64, (12,)), "multiple of 8"), ((64, (16, 8), 1e4, "axis"), "equal sections"),
+                      ((64, (8,), 1e4, "pairs"), "unknown layout"), ((64, (8,), 1e4, "half", f[:7]), "8 finite"),
+                      ((64, (8,), 1e4, "half", f * np.inf), "8 finite")):
+        with pytest.raises(ValueError, match=word):
+            R(*bad, device="cpu")
+
+
+def test_front_end_refuses(pkg):
+    ops = pkg.ops
+    q, kv, pages = _zeros(2, 4, 64), _zeros(2, 2, 64), _zeros(3, 16, 2, 64)
+    table, held = _zeros(2, 1, dtype="int32"), _zeros(2, dtype="int32")
+    rope = ops.RotaryAxes(64, (16, 16), device="cpu")
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_append(q, kv, kv, pages, pages, table, held)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.paged_attention(q, pages, pages, table, held)
+    with pytest.raises(ValueError, match="axes"):
+        ops.paged_append(q, kv, kv, pages, pages, table, held, rope=rope, positions=_zeros(2, 3, dtype="int32"))
+    with pytest.raises(ValueError, match="heads of 64"):
+        ops.paged_append(q, kv, kv, pages, pages, table, held, rope=ops.RotaryAxes(128, (16,), device="cpu"))
