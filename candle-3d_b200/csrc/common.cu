@@ -162,7 +162,8 @@ extern "C" int l3d_kernel_status(int* status, int reset) {
   using namespace l3d;
   if (!status) return fail(L3D_E_NULL, "l3d_kernel_status: status is required");
   cudaError_t (*const words[])(int*, int) = {norm_status_read, sandwich::status_read,
-                                               pattn::status_read, lora::status_read};
+                                               pattn::status_read, lora::status_read,
+                                               cross::status_read};
   *status = 0;
   for (auto read : words) {
     int one = 0;

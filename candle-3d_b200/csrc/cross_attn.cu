@@ -1,0 +1,731 @@
+// Attention of packed sequences to keys of other lengths (cross attention to an encoder's states; attention of
+// each of several scenes to itself, where the keys are its own rows), on the 5th-generation tensor cores:
+//   out[t, h] = sum_j softmax_j(scale q[t, h] . K[j]) V[j]
+// over the keys k_offsets[b] <= j < k_offsets[b + 1] of the sequence b that row t belongs to; query heads
+// h G .. h G + G - 1 read key head h.  The reference's attention core is exact_sdpa_heads
+// (crate/runtime/attention_math.rs:199-259); it takes one sequence after the other.
+//
+// An item is a tile of up to 128 rows of one sequence and key head (128 / G tokens with their G query heads) by
+// all of the sequence's keys.  Blocks are persistent, two to an SM, and walk over the items, which they find from
+// the offsets themselves (lengths are never on the host): K and V rings run on from one item to the next, and
+// the next item's first scores are formed while the last one's output is divided and stored.
+//   warp 0     loads Q tiles and the ring of 64-key K tiles, warp 2 the ring of V tiles (TMA);
+//   warp 1     issues S = Q K^T (two buffers of 64 columns, so that S(n + 2) is formed while softmax(n + 1) runs)
+//              and O += P V (P read from tensor memory, over the scores it comes from);
+//   warps 4-7  one row per thread: S to P in registers, the running maximum and sum, O's rescaling where the
+//              maximum has grown past 2^8, zeros over V rows past a sequence's end (another sequence's, or
+//              anything: a masked probability is 0, but 0 x NaN is not), and the output.
+// Where there are fewer items than blocks, each is cut into parts along its keys, and combine_kernel weighs the
+// parts of each row; an item's parts have fixed places.  A row or two per sequence goes to decode_attn.cu instead.
+// Every mbarrier wait is bounded (%globaltimer, 2 s); on expiry the block records an error in the device's
+// status word and stops.
+#include <type_traits>
+
+#include "attn.cuh"
+#include "common.cuh"
+#include "decode_attn.cuh"
+#include "tc.cuh"
+
+namespace l3d {
+namespace cross {
+
+using namespace l3d::attn;
+
+constexpr int BQ = 128, BKV = 64, THREADS = 256, CTAS = 2;
+constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
+constexpr float RESCALE_LOG2 = 8.f;   // as in attn.cu
+constexpr int MAX_PARTS = 16;
+
+__device__ int g_cross_status;
+
+template <int D>
+struct Cfg {
+  static constexpr int DC = D / 64;
+  static constexpr int Q_BYTES = BQ * D * 2, KV_BYTES = BKV * D * 2;
+  static constexpr int REST = 512;    // barriers
+  static constexpr int FIT = (226 * 1024 / CTAS - REST - Q_BYTES) / KV_BYTES;
+  static constexpr int BUFS = FIT < 12 ? FIT : 12;
+  static constexpr int KST = BUFS / 2, VST = BUFS - KST;
+  static constexpr int SMEM = Q_BYTES + BUFS * KV_BYTES + REST;
+  static constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TMEM_COLS = 256;
+  static_assert(COL_O + D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
+  static_assert((2 * BUFS + 9) * 8 + 8 <= REST, "barrier area");
+  // Of 8 pairs of P, those of ex2_poly2, as in prefix_attn.cu.
+  static constexpr int POLY = D == 64 ? 2 : 1;
+};
+
+struct Params {
+  int B, G, Hkv, Tq, Tk;
+  int N;                       // rows of every sequence; 0: q_offsets
+  int tpt;                     // tokens of a tile
+  int q_th;                    // a tile lists its tokens before its heads
+  int k_hn, v_hn;              // the K / V maps list heads before rows
+  int k_hm, v_hm;              // 0: heads expanded (stride 0)
+  const void *q_offsets, *k_offsets;
+  int q64, k64;
+  void* out;
+  int64_t ot, oh;              // element strides
+  float scale_log2;            // softmax scale * log2(e), > 0
+  int parts;
+  float *part_l, *part_o;      // [parts, Tq, Hq], [parts, Tq, Hq, D]
+  uint64_t wait_ns;
+};
+
+// offsets[i], clamped to [0, most].
+__device__ __forceinline__ int offset_at(const void* p, int is64, int i, int most) {
+  const int64_t v = is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
+  return v < 0 ? 0 : v < most ? int(v) : most;
+}
+
+struct Item {
+  int h, part;
+  int row0, rows;              // the tile's first token, its tokens
+  int key0, keys;              // the sequence's first key, its keys
+  int t0, tiles;               // the part's first key tile and its number
+};
+
+// Walks over the items idx = blockIdx.x, + gridDim.x, ...: (tile, key head, part), the part fastest.  The warp
+// holds 32 sequences at a time, one per lane.
+struct Finder {
+  int idx, window;
+  int64_t base;                // tiles before the window
+  int cnt, incl, q0, q1, k0, k1;
+  bool more;
+  __device__ __forceinline__ void load(const Params& p) {
+    const int b = window * 32 + (threadIdx.x & 31);
+    q0 = q1 = k0 = k1 = 0;
+    if (b < p.B) {
+      q0 = p.N ? b * p.N : offset_at(p.q_offsets, p.q64, b, p.Tq);
+      q1 = p.N ? q0 + p.N : offset_at(p.q_offsets, p.q64, b + 1, p.Tq);
+      k0 = offset_at(p.k_offsets, p.k64, b, p.Tk);
+      k1 = offset_at(p.k_offsets, p.k64, b + 1, p.Tk);
+    }
+    cnt = q1 > q0 ? (q1 - q0 + p.tpt - 1) / p.tpt : 0;
+    incl = cnt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (int(threadIdx.x & 31) >= o) incl += up;
+    }
+  }
+  __device__ __forceinline__ void start(const Params& p) {
+    idx = int(blockIdx.x) - int(gridDim.x);
+    base = 0;
+    window = 0;
+    load(p);
+  }
+  // The next item, of any number of keys.
+  __device__ __forceinline__ bool next(const Params& p, Item& it) {
+    idx += gridDim.x;
+    const int per = p.Hkv * p.parts, tile = idx / per;
+    int all;
+    while (tile - base >= (all = __shfl_sync(0xffffffffu, incl, 31))) {
+      base += all;
+      if (++window * 32 >= p.B) {
+        --window;  // stay: a further call ends here too
+        base -= all;
+        return more = false;
+      }
+      load(p);
+    }
+    const int rel = int(tile - base);
+    const int lane = __ffs(__ballot_sync(0xffffffffu, incl > rel)) - 1;
+    const int first = rel - (__shfl_sync(0xffffffffu, incl, lane) - __shfl_sync(0xffffffffu, cnt, lane));
+    const int a = __shfl_sync(0xffffffffu, q0, lane), e = __shfl_sync(0xffffffffu, q1, lane);
+    it.key0 = __shfl_sync(0xffffffffu, k0, lane);
+    it.keys = max(__shfl_sync(0xffffffffu, k1, lane) - it.key0, 0);
+    const int rest = idx - tile * per;
+    it.h = rest / p.parts;
+    it.part = rest - it.h * p.parts;
+    it.row0 = a + first * p.tpt;
+    it.rows = min(e - it.row0, p.tpt);
+    const int tiles = (it.keys + BKV - 1) / BKV, chunk = (tiles + p.parts - 1) / p.parts;
+    it.t0 = min(it.part * chunk, tiles);
+    it.tiles = min(chunk, tiles - it.t0);
+    return more = true;
+  }
+  __device__ __forceinline__ bool next_with_keys(const Params& p, Item& it) {
+    while (next(p, it))
+      if (it.tiles > 0) return true;
+    return false;
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(THREADS, CTAS)
+    cross_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                 const __grid_constant__ CUtensorMap map_v, const Params p) {
+  using C = Cfg<D>;
+  constexpr uint32_t IDESC_S = idesc_of<T>(128, BKV);
+  constexpr uint32_t IDESC_O = idesc_of<T>(128, D) | (1u << 16);  // B (V) MN-major
+  int* const status = &g_cross_status;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  if (smem_u32(smem_raw) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, ST_MISALIGNED);
+    return;
+  }
+  uint8_t* sq = smem_raw;                            // [DC][128 x 64]
+  uint8_t* sk = sq + C::Q_BYTES;                     // [KST][DC][64 x 64]
+  uint8_t* sv = sk + C::KST * C::KV_BYTES;           // [VST][DC][64 x 64]
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sv + C::VST * C::KV_BYTES);
+  uint64_t* k_full = bars;                           // [KST]
+  uint64_t* k_empty = k_full + C::KST;               // [KST]
+  uint64_t* v_full = k_empty + C::KST;               // [VST]
+  uint64_t* v_empty = v_full + C::VST;               // [VST]
+  uint64_t* s_full = v_empty + C::VST;               // [2] (by S buffer)
+  uint64_t* p_full = s_full + 2;                     // [2]
+  uint64_t* pv_done = p_full + 2;                    // [2]
+  uint64_t* q_full = pv_done + 2;
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* mma_drain = q_empty + 1;                 // abort teardown only
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + 1);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 2);
+
+  // (The shuffle tells the compiler that the role is the same in all lanes.)
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::KST; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < C::VST; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+      mbar_init(&pv_done[i], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(mma_drain, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(tmem_slot)),
+                 "r"(C::TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {
+    return mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, p.wait_ns);
+  };
+  auto wait_warp = [&](uint64_t* bar, uint32_t parity) {  // the warp's lanes stay together
+    const bool got = __all_sync(0xffffffffu, wait(bar, parity)) != 0;
+    __syncwarp();  // before the warp-wide (.aligned) instructions that follow
+    return got;
+  };
+  Finder find;
+  Item it;
+  int loads = 0, q_loads = 0;  // of this warp's ring, of Q (abort teardown)
+
+  if (warp == 0 || warp == 2) {
+    // ------------------------------------------------------- loads of Q and K; of V
+    const bool isk = warp == 0;
+    uint64_t* full = isk ? k_full : v_full;
+    uint64_t* empty = isk ? k_empty : v_empty;
+    uint8_t* ring = isk ? sk : sv;
+    const int stages = isk ? C::KST : C::VST;
+    const CUtensorMap* map = isk ? &map_k : &map_v;
+    const int hn = isk ? p.k_hn : p.v_hn, hm = isk ? p.k_hm : p.v_hm;
+    int s = 0, turn = 0;
+    bool ok = true;
+    find.start(p);
+    while (ok && find.next_with_keys(p, it)) {
+      if (isk) {
+        if (q_loads > 0) ok = wait_warp(q_empty, (q_loads - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          mbar_expect_tx(q_full, C::DC * 128 * p.tpt * p.G);
+          for (int dc = 0; dc < C::DC; ++dc)
+            tma_load_3d(sq + dc * (BQ * 128), &map_q, q_full, dc * 64, p.q_th ? it.row0 : it.h * p.G,
+                        p.q_th ? it.h * p.G : it.row0);
+        }
+        ++q_loads;
+      }
+      const int hh = it.h * hm;
+      for (int j = 0; j < it.tiles; ++j) {
+        if (turn > 0) ok = wait_warp(&empty[s], (turn - 1) & 1);
+        if (!ok) break;
+        if (lane == 0) {
+          const int row = it.key0 + (it.t0 + j) * BKV;
+          mbar_expect_tx(&full[s], C::KV_BYTES);
+          for (int dc = 0; dc < C::DC; ++dc)
+            tma_load_4d(ring + s * C::KV_BYTES + dc * (BKV * 128), map, &full[s], dc * 64, hn ? hh : row, hn ? row : hh, 0);
+        }
+        ++loads;
+        if (++s == stages) {
+          s = 0;
+          ++turn;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ MMA
+    // The whole warp keeps step and one elected lane issues.  Scores run two tiles ahead of P V, across the
+    // ends of items.
+    const bool leader = elect_one();
+    auto commit = [&](uint64_t* bar) {
+      if (leader) umma_commit(bar);
+    };
+    const uint32_t t_s = tmem_base + C::COL_S, t_o = tmem_base + C::COL_O;
+    int ns = 0, js = 0, ks = 0, kturn = 0, items = 0;  // of the next scores: number, tile of its item, K slot, Q
+    find.start(p);
+    bool more = find.next_with_keys(p, it), ok = true;
+    auto issue_s = [&] {
+      if (js == 0) ok = wait_warp(q_full, items & 1);
+      ok = ok && wait_warp(&k_full[ks], kturn & 1);
+      if (!ok) return;
+      tc_fence_after();
+      const uint64_t da = smem_desc_sw128(sq), db = smem_desc_sw128(sk + ks * C::KV_BYTES);
+      if (leader) {
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          umma_f16<IDESC_S>(t_s + (ns & 1) * BKV, da + uint64_t((k >> 2) * (BQ * 128 >> 4) + 2 * (k & 3)),
+                            db + uint64_t((k >> 2) * (BKV * 128 >> 4) + 2 * (k & 3)), k ? 1u : 0u);
+      }
+      commit(&s_full[ns & 1]);
+      commit(&k_empty[ks]);
+      if (++ks == C::KST) {
+        ks = 0;
+        ++kturn;
+      }
+      ++ns;
+      if (++js == it.tiles) {
+        commit(q_empty);
+        js = 0;
+        ++items;
+        more = find.next_with_keys(p, it);
+      }
+    };
+    Finder find_v;
+    Item iv;
+    find_v.start(p);
+    int n = 0, vs = 0, vturn = 0;
+    for (int i = 0; i < 2 && ok && more; ++i) issue_s();
+    while (ok && find_v.next_with_keys(p, iv)) {
+      for (int j = 0; ok && j < iv.tiles; ++j) {
+        ok = wait_warp(&p_full[n & 1], (n >> 1) & 1) && wait_warp(&v_full[vs], vturn & 1);
+        if (!ok) break;
+        tc_fence_after();
+        // (P of an item's first tile comes after the last item's output was read: O is free.)
+        const uint64_t db = smem_desc_sw128_mn(sv + vs * C::KV_BYTES, BKV * 128);
+        if (leader) {
+#pragma unroll
+          for (int k = 0; k < BKV / 16; ++k)
+            umma_f16_ts<IDESC_O>(t_o, t_s + (n & 1) * BKV + uint32_t(k * 8), db + uint64_t(k * (16 * 128 >> 4)),
+                                 (j | k) ? 1u : 0u);
+        }
+        commit(&v_empty[vs]);
+        commit(&pv_done[n & 1]);  // the last commit of all: the block waits for it
+        if (++vs == C::VST) {
+          vs = 0;
+          ++vturn;
+        }
+        ++n;
+        if (more) issue_s();  // over the P that the product before it has read
+      }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------ softmax / epilogue
+    const int r = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem_base + C::COL_S + lane_off, t_o = tmem_base + C::COL_O + lane_off;
+    // This thread's row of a tile: token i, query head g of the key head's.
+    const int i = p.q_th ? r % p.tpt : r / p.G, g = p.q_th ? r / p.tpt : r - i * p.G;
+    const float2 sc2 = f2(p.scale_log2);
+    int n = 0, vs = 0, vturn = 0;
+    bool ok = true;
+    find.start(p);
+    while (ok && find.next(p, it)) {
+      const bool valid = i < it.rows && g < p.G;
+      const bool active = __any_sync(0xffffffffu, valid);  // the warp holds rows
+      float m = -INFINITY;                         // running max, log2 units
+      float2 l2 = f2(0.f);                         // running row sum (two parts)
+      for (int j = 0; j < it.tiles; ++j, ++n) {
+        ok = wait_warp(&s_full[n & 1], (n >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        // V rows past the sequence's keys may hold anything: zero them, once the tile has landed.
+        const int held = it.keys - (it.t0 + j) * BKV;
+        if (held < BKV) {
+          ok = wait_warp(&v_full[vs], vturn & 1);
+          if (!ok) break;
+          const int vrow = r & (BKV - 1);
+          if (vrow >= held) {
+            uint8_t* vr = sv + vs * C::KV_BYTES + vrow * 128;
+#pragma unroll
+            for (int x = 0; x < D / 16; ++x) {
+              const int c = (r / BKV) * (D / 16) + x;
+              *reinterpret_cast<uint4*>(vr + (c >> 3) * (BKV * 128) + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+        }
+        if (++vs == C::VST) {
+          vs = 0;
+          ++vturn;
+        }
+        if (!active) {  // no rows: keep the other warps' pace
+          if (lane == 0) mbar_arrive(&p_full[n & 1]);
+          continue;
+        }
+        const uint32_t t_sn = t_s + (n & 1) * BKV;
+        float s[BKV];
+        tmem_ld64(t_sn, s);
+        if (held < BKV) {
+#pragma unroll
+          for (int e = 0; e < BKV; ++e)
+            if (e >= held) s[e] = -INFINITY;
+        }
+        __syncwarp();
+        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+        for (int e = 4; e < BKV; e += 2) mx[(e >> 1) & 3] = max_nan(mx[(e >> 1) & 3], s[e], s[e + 1]);
+        const float mxs = max_nan(max_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;  // scale > 0
+        const bool grow = !(mxs <= m + RESCALE_LOG2);       // always on the first key a row sees
+        const float m_new = grow ? mxs : m;
+        const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
+        if (j > 0 && __any_sync(0xffffffffu, grow)) {
+          ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);  // O is stable
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < D; c += 16) {  // (s is live: few columns at a time)
+            float o[16];
+            tmem_ld16(t_o + uint32_t(c), o);
+            uint32_t u[16];
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 v = mul2(make_float2(o[e], o[e + 1]), f2(alpha));
+              u[e] = __float_as_uint(v.x);
+              u[e + 1] = __float_as_uint(v.y);
+            }
+            tmem_st16u(t_o + uint32_t(c), u);
+          }
+        }
+        // P = exp2(s * scale * log2 e - m); all scores of -inf so far: subtract 0, so that P = 0.
+        const float2 nm2 = f2(m_new == -INFINITY ? 0.f : minus_max(m_new));
+        l2 = mul2(l2, f2(alpha));
+#pragma unroll
+        for (int c = 0; c < BKV; c += 32) {
+          uint32_t u[16];
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float2 x = fma2(make_float2(s[c + e], s[c + e + 1]), sc2, nm2);
+            const float2 pr = ((e >> 1) & 7) < C::POLY ? ex2_poly2(x) : make_float2(ex2f(x.x), ex2f(x.y));
+            l2 = add2(l2, pr);
+            u[e >> 1] = pack_pair<T>(pr.x, pr.y);
+          }
+          tmem_st16u(t_sn + uint32_t(c / 2), u);
+        }
+        m = m_new;
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[n & 1]);
+      }
+      // The output, or this part's O / l and log2 sum, after the item's last P V.
+      if (ok && it.tiles > 0) ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+      tc_fence_after();
+      if (!ok || !active) continue;
+      float l = l2.x + l2.y;
+      if (m == -INFINITY && l == l) l = 0.f;  // (ex2_poly2 gives 1e-42 for -inf, not 0)
+      const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;  // no keys: zeros; NaN stays
+      const int64_t token = it.row0 + i;
+      const int64_t pr = (int64_t(it.part) * p.Tq + token) * (p.Hkv * p.G) + it.h * p.G + g;
+      if (p.parts > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
+      T* orow = static_cast<T*>(p.out) + token * p.ot + int64_t(it.h * p.G + g) * p.oh;
+      __syncwarp();  // the loads from tensor memory are the whole warp's
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        float o[32];
+        if (it.tiles > 0) {
+          tmem_ld32(t_o + uint32_t(c), o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0.f;
+        }
+        if (valid) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] *= inv;
+          if (p.parts > 1) {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              float v[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) v[e] = o[8 * x + e];
+              *reinterpret_cast<uint4*>(orow + c + 8 * x) = pack(v, T());
+            }
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  // Teardown, as in attn.cu: after an abort nothing the block started may still be running when it frees TMEM
+  // and exits.
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    if (warp == 1 && elect_one()) {  // the lane that issued
+      umma_commit(mma_drain);
+      mbar_drain(mma_drain, 0, p.wait_ns);
+    }
+    if ((warp == 0 || warp == 2) && lane == 0) {  // the newest load of each slot, and of Q
+      const int stages = warp == 0 ? C::KST : C::VST;
+      for (int i = max(loads - stages, 0); i < loads; ++i)
+        mbar_drain(warp == 0 ? &k_full[i % stages] : &v_full[i % stages], uint32_t(i / stages) & 1u, p.wait_ns);
+      if (q_loads > 0) mbar_drain(q_full, uint32_t(q_loads - 1) & 1u, p.wait_ns);
+    }
+  }
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base),
+                 "r"(C::TMEM_COLS));
+  }
+}
+
+// The parts of each row weighed by 2^(their log2 sum - the largest), a warp per row of a sequence.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) combine_kernel(const Params p) {
+  constexpr int E = D / 32;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  const int lane = threadIdx.x & 31, Hq = p.Hkv * p.G;
+  const int64_t rows = int64_t(p.Tq) * Hq, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  if (row >= rows) return;
+  const int64_t token = row / Hq;
+  if (!p.N && (token < offset_at(p.q_offsets, p.q64, 0, p.Tq) || token >= offset_at(p.q_offsets, p.q64, p.B, p.Tq)))
+    return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  float w = lane < p.parts ? p.part_l[lane * rows + row] : -INFINITY, mx = w;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  w = w == -INFINITY ? 0.f : exp2f(w - mx);
+  float sum = w;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  alignas(16) float acc[E] = {};
+  for (int k = 0; k < p.parts; ++k) {
+    const float wk = __shfl_sync(0xffffffffu, w, k);
+    if (wk == 0.f) continue;
+    const Vec v = reinterpret_cast<const Vec*>(p.part_o + (k * rows + row) * D)[lane];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(wk, reinterpret_cast<const float*>(&v)[e], acc[e]);
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  T* orow = static_cast<T*>(p.out) + token * p.ot + (row - token * Hq) * p.oh + lane * E;
+  alignas(8) T o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = from_f<T>(acc[e] * inv);
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(o);
+  else *reinterpret_cast<uint32_t*>(orow) = *reinterpret_cast<const uint32_t*>(o);
+}
+
+// Parts of an item: none cut while the items fill the device; else as many as its blocks take, of four key
+// tiles at least by the keys' average.
+static int parts_for(int64_t B, int64_t Tq, int64_t Tk, int64_t G, int64_t Hkv) {
+  const int64_t tpt = BQ / G, items = Hkv * (Tq / tpt + B), tiles = (Tk / B + BKV - 1) / BKV;
+  int64_t parts = CTAS * int64_t(sm_count()) / items;
+  if (parts > tiles / 4) parts = tiles / 4;
+  return int(parts < 1 ? 1 : parts > MAX_PARTS ? MAX_PARTS : parts);
+}
+
+// Single rows (or a few) of every sequence: their work is reading the keys.
+// (The last two: what decode_attn.cu takes, and counts in 32 bits.)
+static bool few_rows(int64_t B, int64_t N, int64_t G, int64_t Tk) {
+  return N > 0 && N * G <= 16 && B <= decode::MAX_BATCH && B * (Tk / 16 + 1) <= int64_t(1) << 30;
+}
+
+cudaError_t status_read(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_cross_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_cross_status, &zero, sizeof(int));
+  }
+  return e;
+}
+
+template <typename T, int D>
+static cudaError_t launch(const CUtensorMap (&maps)[3], const Params& p, int blocks, cudaStream_t s) {
+  auto k = cross_kernel<T, D>;
+  cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<D>::SMEM);
+  if (e != cudaSuccess) return e;
+  k<<<unsigned(blocks), THREADS, Cfg<D>::SMEM, s>>>(maps[0], maps[1], maps[2], p);
+  if (p.parts <= 1) return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(unsigned((int64_t(p.Tq) * p.Hkv * p.G + 3) / 4));
+  cfg.blockDim = dim3(128);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p);
+}
+
+// The map of q [T, Hq, D] with boxes of G heads x tpt tokens, the nearer in memory listed first.
+static bool make_q_map(CUtensorMap* m, const void* base, int64_t T, int64_t Hq, int64_t D, int64_t st, int64_t sh, int G,
+                       int tpt, int* th) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  if (T <= 1) st = Hq <= 1 ? D : (sh > 0 ? sh * Hq : D);
+  if (Hq <= 1) sh = st * T;
+  *th = st < sh ? 1 : 0;
+  const cuuint64_t dims[3] = {uint64_t(D), uint64_t(*th ? T : Hq), uint64_t(*th ? Hq : T)};
+  const cuuint64_t strides[2] = {uint64_t(*th ? st : sh) * 2, uint64_t(*th ? sh : st) * 2};
+  const cuuint32_t box[3] = {64u, uint32_t(*th ? tpt : G), uint32_t(*th ? G : tpt)};
+  const cuuint32_t es[3] = {1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+}  // namespace cross
+}  // namespace l3d
+
+using namespace l3d;
+
+extern "C" size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int64_t hq, int64_t hkv,
+                                                     int64_t d, int ragged) {
+  if (b <= 0 || tq <= 0 || tk < 0 || hq <= 0 || hkv <= 0 || hq % hkv || hq / hkv > l3d::cross::BQ || d <= 0) return 0;
+  const int64_t G = hq / hkv, N = ragged || tq % b ? 0 : tq / b;
+  if (l3d::cross::few_rows(b, N, G, tk)) return l3d::decode::workspace_size(b, N, G, hkv, tk, d);
+  const int parts = l3d::cross::parts_for(b, tq, tk, G, hkv);
+  if (parts <= 1) return 0;
+  return (size_t(parts) * size_t(tq * hq) * 4 + 255) / 256 * 256 + size_t(parts) * size_t(tq * hq) * size_t(d) * 4;
+}
+
+extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, const l3d_tensor* v,
+                                   const l3d_tensor* k_offsets, const l3d_tensor* q_offsets, float scale,
+                                   const l3d_tensor* out, void* workspace, size_t workspace_bytes,
+                                   l3d_stream stream) {
+  using namespace l3d::cross;
+  const char* op = "l3d_cross_attention";
+  if (!q || !k || !v || !k_offsets || !out)
+    return fail(L3D_E_NULL, "%s: q, k, v, k_offsets and out are required", op);
+  const l3d_tensor* all[] = {q, out, k, v};
+  for (const l3d_tensor* t : all) {
+    if (t->dtype != q->dtype || (t->dtype != L3D_BF16 && t->dtype != L3D_F16))
+      return fail(L3D_E_DTYPE, "%s: q, k, v and out all BF16 or all F16", op);
+    if (t->ndim != 3) return fail(L3D_E_SHAPE, "%s: q, out [Tq, Hq, D], k, v [Tk, Hkv, D]", op);
+    if (numel(t) > 0 && t->strides[2] != 1) return fail(L3D_E_ALIGN, "%s: the head dim must be contiguous", op);
+  }
+  const int64_t Tq = q->dims[0], Hq = q->dims[1], D = q->dims[2], Tk = k->dims[0], Hkv = k->dims[1];
+  if (D != 64 && D != 128) return fail(L3D_E_UNSUPPORTED, "%s: head dim must be 64 or 128", op);
+  for (int i = 0; i < 3; ++i) {
+    if (out->dims[i] != q->dims[i]) return fail(L3D_E_SHAPE, "%s: out must have q's shape", op);
+    if (v->dims[i] != k->dims[i] || (i == 2 && k->dims[i] != D))
+      return fail(L3D_E_SHAPE, "%s: k and v [Tk, Hkv, D]", op);
+  }
+  if (Hq > 0 && (Hkv <= 0 || Hq % Hkv))
+    return fail(L3D_E_SHAPE, "%s: query heads must be a multiple of the key heads", op);
+  auto index_list = [](const l3d_tensor* t) {
+    return (t->dtype == L3D_I32 || t->dtype == L3D_I64) && t->ndim == 1 && t->dims[0] >= 1 &&
+           (t->dims[0] == 1 || t->strides[0] == 1);
+  };
+  if (!index_list(k_offsets)) return fail(L3D_E_SHAPE, "%s: k_offsets must be contiguous [B + 1] I32 or I64", op);
+  const int64_t B = k_offsets->dims[0] - 1;
+  if (q_offsets && (!index_list(q_offsets) || q_offsets->dims[0] != B + 1))
+    return fail(L3D_E_SHAPE, "%s: q_offsets must be contiguous [B + 1] I32 or I64, as k_offsets", op);
+  if (!q_offsets && (B > 0 ? Tq % B != 0 : Tq > 0))
+    return fail(L3D_E_SHAPE, "%s: without q_offsets the rows must divide evenly among the sequences", op);
+  const float scale_log2 = scale * 1.4426950408889634f;  // finite too
+  if (!(scale > 0.f) || !(scale_log2 < INFINITY))
+    return fail(L3D_E_UNSUPPORTED, "%s: scale must be positive and finite", op);
+  const int64_t big = int64_t(1) << 30;
+  if (Tq > big || Tk > big || B > big || Hq > 65535 || Tq * Hq > big || Hkv * (B + Tq) > big)
+    return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large", op);
+  if (Hkv > 0 && Hq / Hkv > BQ) return fail(L3D_E_UNSUPPORTED, "%s: at most %d query heads per key head", op, BQ);
+  if (Tq * Hq == 0 || B == 0) return L3D_OK;
+  for (const l3d_tensor* t : {k, v})
+    if (Tk > 1 && t->strides[0] == 0) return fail(L3D_E_ALIGN, "%s: the keys must not be expanded (stride 0)", op);
+  if ((Tq > 1 && q->strides[0] == 0) || (Hq > 1 && q->strides[1] == 0))
+    return fail(L3D_E_ALIGN, "%s: q must not be expanded (stride 0)", op);
+  const size_t need = l3d_cross_attention_workspace_size(B, Tq, Tk, Hq, Hkv, D, q_offsets != nullptr);
+  if (need && (!workspace || workspace_bytes < need))
+    return fail(L3D_E_WORKSPACE, "%s: workspace of %zu bytes required", op, need);
+  if (reinterpret_cast<uintptr_t>(workspace) % 256)
+    return fail(L3D_E_ALIGN, "%s: workspace must be 256-byte aligned", op);
+  for (const l3d_tensor* t : all) {
+    if (no_data(t)) return fail(L3D_E_NULL, "%s: null data pointer", op);
+    if (numel(t) == 0) continue;
+    if (reinterpret_cast<uintptr_t>(elem_ptr(t)) % 16)
+      return fail(L3D_E_ALIGN, "%s: tensors must be 16-byte aligned", op);
+    for (int d = 0; d < 2; ++d)
+      if (t->dims[d] > 1 && t->strides[d] % 8)
+        return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
+  }
+  if (no_data(k_offsets) || (q_offsets && no_data(q_offsets))) return fail(L3D_E_NULL, "%s: null data pointer", op);
+  const int64_t G = Hq / Hkv, N = q_offsets ? 0 : Tq / B;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (few_rows(B, N, G, Tk)) {
+    l3d::decode::Params p{};
+    p.B = int(B); p.N = int(N); p.G = int(G); p.Hkv = int(Hkv);
+    p.q = elem_ptr(q);
+    p.out = const_cast<char*>(elem_ptr(out));
+    p.qb = q->strides[0] * N; p.qn = q->strides[0]; p.qh = q->strides[1];
+    p.ob = out->strides[0] * N; p.on = out->strides[0]; p.oh = out->strides[1];
+    p.k = elem_ptr(k);
+    p.v = elem_ptr(v);
+    for (int i = 0; i < 2; ++i) {
+      p.ks[i + 1] = k->strides[i];
+      p.vs[i + 1] = v->strides[i];
+    }
+    p.keys = int(Tk);
+    p.lengths = elem_ptr(k_offsets);
+    p.len64 = k_offsets->dtype == L3D_I64;
+    p.scale_log2 = scale_log2;
+    e = l3d::decode::launch(p, q->dtype == L3D_F16, int(D), Tk, workspace, s);
+    return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  }
+  Params p{};
+  p.B = int(B); p.G = int(G); p.Hkv = int(Hkv); p.Tq = int(Tq); p.Tk = int(Tk); p.N = int(N);
+  p.tpt = BQ / p.G;
+  p.q_offsets = q_offsets ? elem_ptr(q_offsets) : nullptr;
+  p.q64 = q_offsets && q_offsets->dtype == L3D_I64;
+  p.k_offsets = elem_ptr(k_offsets);
+  p.k64 = k_offsets->dtype == L3D_I64;
+  p.out = const_cast<char*>(elem_ptr(out));
+  p.ot = out->strides[0]; p.oh = out->strides[1];
+  p.scale_log2 = scale_log2;
+  p.parts = parts_for(B, Tq, Tk, G, Hkv);
+  p.part_l = static_cast<float*>(workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t(p.parts) * size_t(Tq * Hq) * 4 + 255) / 256 * 256);
+  p.wait_ns = l3d::tc::WAIT_LIMIT_NS;
+  CUtensorMap maps[3];
+  p.k_hm = Hkv > 1 && k->strides[1] == 0 ? 0 : 1;
+  p.v_hm = Hkv > 1 && v->strides[1] == 0 ? 0 : 1;
+  bool ok = make_q_map(&maps[0], elem_ptr(q), Tq, Hq, D, q->strides[0], q->strides[1], p.G, p.tpt, &p.q_th);
+  if (Tk > 0)
+    ok = ok && make_map4(&maps[1], elem_ptr(k), 1, p.k_hm ? Hkv : 1, Tk, D, k->strides[0], k->strides[1], 0, BKV, &p.k_hn) &&
+         make_map4(&maps[2], elem_ptr(v), 1, p.v_hm ? Hkv : 1, Tk, D, v->strides[0], v->strides[1], 0, BKV, &p.v_hn);
+  else
+    maps[1] = maps[2] = maps[0];  // never read
+  if (!ok) return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed", op);
+  const int64_t items = (Hkv * (Tq / p.tpt + B)) * p.parts, most = CTAS * int64_t(sm_count());
+  const int blocks = int(items < most ? items : most);
+  if (q->dtype == L3D_BF16)
+    e = D == 64 ? launch<__nv_bfloat16, 64>(maps, p, blocks, s) : launch<__nv_bfloat16, 128>(maps, p, blocks, s);
+  else
+    e = D == 64 ? launch<__half, 64>(maps, p, blocks, s) : launch<__half, 128>(maps, p, blocks, s);
+  return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+}

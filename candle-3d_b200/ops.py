@@ -748,3 +748,26 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None):
     call("l3d_paged_attention", dq, dk, dv, dt, dl, q.shape[-1] ** -0.5 if scale is None else float(scale), do, ws.data_ptr(), need,
          stream_of(q))
     return out
+
+
+def cross_attention(q, k, v, k_offsets, q_offsets=None, scale=None, out=None, check=None):
+    """exact_sdpa_heads (crate/runtime/attention_math.rs:199-259) of sequences packed one
+    behind the other over keys of other lengths (an encoder's states), packed too: q
+    [Tq, Hq, D], k and v [Tk, Hkv, D]; every row of sequence b (rows q_offsets[b] ..
+    q_offsets[b + 1] - 1; None: equal groups) sees the keys k_offsets[b] ..
+    k_offsets[b + 1] - 1.  The same offsets for both: each sequence attends to
+    itself.  Rows of no sequence are left as they are (in `out`, where it is given).
+    BF16 or F16, D = 64 or 128; `check` as in `attention`."""
+    if out is None:
+        out = empty(q, *q.shape)
+    dq, dk, dv, dko, dqo, do = packs_here(q, k, v, k_offsets, q_offsets, out)
+    need = 0
+    if q.dim() == 3 and k.dim() == 3:  # (the entry refuses anything else)
+        need = _lib.lib().l3d_cross_attention_workspace_size(
+            k_offsets.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
+            q_offsets is not None)
+    ws = workspace(q, need) if need else None
+    call("l3d_cross_attention", dq, dk, dv, dko, dqo, q.shape[-1] ** -0.5 if scale is None else float(scale),
+         do, ws.data_ptr() if need else None, need, stream_of(q))
+    _check_status("l3d_cross_attention", q, check)
+    return out

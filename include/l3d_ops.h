@@ -101,8 +101,8 @@ int l3d_layer_norm(const l3d_tensor* x, const l3d_tensor* weight, const l3d_tens
 /* Status of the kernels that take no workspace, on the current device (no
  * counterpart in the reference: Candle ops report errors only on the host).
  * The row-norm entries stream long inputs through shared memory with bounded
- * waits, and so do l3d_lora_linear, l3d_shared_prefix_attention and
- * l3d_sandwich_residual_norm; a wait that runs out (status 5) is recorded in a
+ * waits, and so do l3d_lora_linear, l3d_shared_prefix_attention,
+ * l3d_cross_attention and l3d_sandwich_residual_norm; a wait that runs out (status 5) is recorded in a
  * per-device word, since none of them has a status word in a workspace.
  * This call copies it to *status (synchronising with the device) and clears
  * it when reset != 0.  0 = no wait has expired. */
@@ -544,6 +544,32 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * positive, and scale * log2(e) finite. */
 int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
                         const l3d_tensor* table, const l3d_tensor* lengths, float scale,
+                        const l3d_tensor* out, void* workspace, size_t workspace_bytes,
+                        l3d_stream stream);
+
+/* Workspace bytes for l3d_cross_attention (0: none needed); ragged: q_offsets
+ * are given. */
+size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int64_t hq,
+                                          int64_t hkv, int64_t d, int ragged);
+
+/* The attention core (exact_sdpa_heads, crate/runtime/attention_math.rs:199-259)
+ * of sequences packed one behind the other over keys of other lengths, packed
+ * too: q and out [Tq, Hq, D], k and v [Tk, Hkv, D]; every row of sequence b (rows
+ * q_offsets[b] .. q_offsets[b + 1] - 1; NULL: B equal groups) sees the keys
+ * k_offsets[b] .. k_offsets[b + 1] - 1.  With the same offsets for both it is the
+ * attention of each sequence to itself.  Offsets [B + 1] I32/I64, contiguous, not
+ * decreasing, clamped to the rows there are; rows of out that belong to no
+ * sequence are left as they were, and keys of none are never used, whatever they
+ * hold.  Hq a multiple of Hkv, at most 128 times as many, query head h reading key
+ * head h / (Hq / Hkv).  A row with no keys gives zeros, one that sees a score
+ * that is NaN or +inf NaN.  BF16 or F16, D = 64 or 128, head dim contiguous,
+ * strides otherwise free in multiples of 16 bytes (keys and q not expanded along
+ * the rows); softmax and sums in f32, probabilities rounded to the input type for
+ * the second product (not where every sequence has N rows and N * Hq / Hkv is at
+ * most 16: they then enter as two 16-bit parts).  scale must be positive, and
+ * scale * log2(e) finite. */
+int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, const l3d_tensor* v,
+                        const l3d_tensor* k_offsets, const l3d_tensor* q_offsets, float scale,
                         const l3d_tensor* out, void* workspace, size_t workspace_bytes,
                         l3d_stream stream);
 

@@ -152,3 +152,83 @@ def test_front_end_refuses(pkg):
         ops.paged_append(q, kv, kv, pages, pages, table, held, rope=rope, positions=_zeros(2, 3, dtype="int32"))
     with pytest.raises(ValueError, match="heads of 64"):
         ops.paged_append(q, kv, kv, pages, pages, table, held, rope=ops.RotaryAxes(128, (16,), device="cpu"))
+
+
+def _cross_args(**over):
+    Tq, Tk, Hq, Hkv, D = 60, 40, 4, 2, 64
+    a = dict(q=_zeros(Tq, Hq, D), k=_zeros(Tk, Hkv, D), v=_zeros(Tk, Hkv, D), k_offsets=_zeros(4, dtype="int32"),
+             q_offsets=_zeros(4, dtype="int64"), scale=0.125, out=_zeros(Tq, Hq, D), workspace=256, bytes=1 << 30)
+    assert not set(over) - set(a)
+    return [*(a | over).values(), None]
+
+
+@pytest.mark.parametrize("over,code,word", [
+    (dict(q=None), E_NULL, "required"),
+    (dict(k_offsets=None), E_NULL, "required"),
+    (dict(q=_zeros(60, 4, 64, dtype="float32")), E_DTYPE, "BF16"),
+    (dict(v=_zeros(40, 2, 64, dtype="float16")), E_DTYPE, "F16"),
+    (dict(q=_zeros(1, 60, 4, 64)), E_SHAPE, "[Tq, Hq, D]"),
+    (dict(k=_zeros(40, 64, 2).transpose(1, 2)), E_ALIGN, "contiguous"),
+    (dict(q=_zeros(60, 4, 80), out=_zeros(60, 4, 80)), E_UNSUPPORTED, "64 or 128"),
+    (dict(out=_zeros(59, 4, 64)), E_SHAPE, "out"),
+    (dict(v=_zeros(41, 2, 64)), E_SHAPE, "k and v"),
+    (dict(k=_zeros(40, 2, 128), v=_zeros(40, 2, 128)), E_SHAPE, "k and v"),
+    (dict(k=_zeros(40, 3, 64), v=_zeros(40, 3, 64)), E_SHAPE, "multiple of the key heads"),
+    (dict(k_offsets=_zeros(4, dtype="float32")), E_SHAPE, "k_offsets"),
+    (dict(k_offsets=_zeros(0, dtype="int32")), E_SHAPE, "k_offsets"),
+    (dict(k_offsets=_zeros(8, dtype="int32")[::2]), E_SHAPE, "k_offsets"),
+    (dict(q_offsets=_zeros(5, dtype="int32")), E_SHAPE, "q_offsets"),
+    (dict(q_offsets=None, k_offsets=_zeros(8, dtype="int32")), E_SHAPE, "divide evenly"),
+    (dict(q_offsets=None, k_offsets=_zeros(1, dtype="int32")), E_SHAPE, "divide evenly"),
+    (dict(scale=-1.0), E_UNSUPPORTED, "scale"),
+    (dict(scale=math.nan), E_UNSUPPORTED, "scale"),
+    (dict(scale=3e38), E_UNSUPPORTED, "scale"),
+    (dict(q=_zeros(60, 258, 64), out=_zeros(60, 258, 64)), E_UNSUPPORTED, "128 query heads"),
+    (dict(k=_zeros(1, 2, 64).expand(40, 2, 64)), E_ALIGN, "expanded"),
+    (dict(q=_zeros(60, 1, 64).expand(60, 4, 64)), E_ALIGN, "expanded"),
+    (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), bytes=0), E_WORKSPACE, "workspace"),
+    (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), workspace=264), E_ALIGN, "256"),
+    (dict(q_offsets=None, q=_zeros(3, 4, 64), out=_zeros(3, 4, 64), workspace=None), E_WORKSPACE, "workspace"),
+    (dict(k=_zeros(40, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
+    (dict(q=_zeros(60, 4, 68)[..., 2:66]), E_ALIGN, "16-byte"),
+])
+def test_cross_attention_refuses(pkg, over, code, word):
+    _refused(pkg, "l3d_cross_attention", _cross_args(**over), code, word)
+
+
+def test_cross_attention_nothing_to_do(pkg):
+    L = pkg._lib
+    args = _cross_args(q=_zeros(0, 4, 64), out=_zeros(0, 4, 64), workspace=None, bytes=0)
+    assert L.lib().l3d_cross_attention(*[L.packed(a) if hasattr(a, "dim") else a for a in args]) == 0
+    size = L.lib().l3d_cross_attention_workspace_size
+    assert size(0, 60, 40, 4, 2, 64, 1) == 0 and size(3, 60, 40, 4, 3, 64, 1) == 0 and size(3, 60, 0, 4, 2, 64, 1) == 0
+    with pytest.raises(ValueError, match="CUDA"):
+        pkg.ops.cross_attention(_zeros(3, 4, 64), _zeros(5, 4, 64), _zeros(5, 4, 64), _zeros(2, dtype="int32"))
+
+
+def test_cross_attention_status_reaches_the_caller(pkg, monkeypatch):
+    """A wait that ran out raises where it is asked for, as in the other serving entries."""
+    from contextlib import nullcontext
+    from types import SimpleNamespace
+
+    import torch
+
+    ops, seen = pkg.ops, []
+
+    def call(name, *args):
+        seen.append(name)
+        if name == "l3d_kernel_status":
+            args[0]._obj.value = 5
+
+    monkeypatch.setattr(ops, "call", call)
+    monkeypatch.setattr(ops, "packs_here", lambda *a: a)
+    monkeypatch.setattr(ops, "stream_of", lambda t: None)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
+    monkeypatch.setattr(torch.cuda, "current_stream",
+                        lambda d: SimpleNamespace(synchronize=lambda: seen.append("synchronised")))
+    args = _zeros(60, 4, 64), _zeros(40, 2, 64), _zeros(40, 2, 64), _zeros(4, dtype="int32"), _zeros(4, dtype="int32")
+    ops.cross_attention(*args)
+    assert seen == ["l3d_cross_attention"]
+    with pytest.raises(pkg._lib.L3dError, match="l3d_cross_attention.*status word 5"):
+        ops.cross_attention(*args, check=True)
+    assert seen[1:] == ["l3d_cross_attention", "synchronised", "l3d_kernel_status"]
