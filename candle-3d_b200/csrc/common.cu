@@ -163,7 +163,7 @@ extern "C" int l3d_kernel_status(int* status, int reset) {
   if (!status) return fail(L3D_E_NULL, "l3d_kernel_status: status is required");
   cudaError_t (*const words[])(int*, int) = {norm_status_read, sandwich::status_read,
                                                pattn::status_read, lora::status_read,
-                                               cross::status_read};
+                                               decode::status_read, cross::status_read};
   *status = 0;
   for (auto read : words) {
     int one = 0;

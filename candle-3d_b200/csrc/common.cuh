@@ -40,7 +40,7 @@ int sm_count();
 // the result of the first attempt on this device.
 cudaError_t set_smem_limit(const void* kernel, int bytes);
 // Per-device status words of the kernels that keep none in a workspace (the
-// row-norm rings, the shared-prefix and cross attention, the adapters): copy to *status, clear
+// row-norm rings, the shared-prefix, paged and cross attention, the adapters): copy to *status, clear
 // when reset != 0.
 cudaError_t norm_status_read(int* status, int reset);
 namespace pattn {
@@ -50,6 +50,9 @@ namespace lora {
 cudaError_t status_read(int* status, int reset);
 }
 namespace sandwich {
+cudaError_t status_read(int* status, int reset);
+}
+namespace decode {
 cudaError_t status_read(int* status, int reset);
 }
 namespace cross {

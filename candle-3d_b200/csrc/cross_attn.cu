@@ -684,18 +684,13 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
     p.out = const_cast<char*>(elem_ptr(out));
     p.qb = q->strides[0] * N; p.qn = q->strides[0]; p.qh = q->strides[1];
     p.ob = out->strides[0] * N; p.on = out->strides[0]; p.oh = out->strides[1];
-    p.k = elem_ptr(k);
-    p.v = elem_ptr(v);
-    for (int i = 0; i < 2; ++i) {
-      p.ks[i + 1] = k->strides[i];
-      p.vs[i + 1] = v->strides[i];
-    }
     p.keys = int(Tk);
     p.lengths = elem_ptr(k_offsets);
     p.len64 = k_offsets->dtype == L3D_I64;
     p.scale_log2 = scale_log2;
-    e = l3d::decode::launch(p, q->dtype == L3D_F16, int(D), Tk, workspace, s);
-    return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+    const l3d::decode::Keys kv{elem_ptr(k), elem_ptr(v), {0, k->strides[0], k->strides[1]},
+                               {0, v->strides[0], v->strides[1]}, D};
+    return l3d::decode::launch(op, p, kv, q->dtype == L3D_F16, Tk, workspace, s);
   }
   Params p{};
   p.B = int(B); p.G = int(G); p.Hkv = int(Hkv); p.Tq = int(Tq); p.Tk = int(Tk); p.N = int(N);

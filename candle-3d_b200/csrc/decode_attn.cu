@@ -11,39 +11,45 @@
 // Work is divided by keys alone: all (request, key head, row tile) have their keys in tiles of 16, the tiles of
 // all of them in one line, and every warp of the device takes an equal stretch of the line, whatever the
 // lengths are; the lengths are read on the device, and each block sums them up for itself.  A warp works
-// alone: its own ring of tiles in shared memory, filled by 16-byte asynchronous copies that run on across the
-// ends of requests, its own running maximum and sum, no barrier.  Where a stretch holds all the keys of a
-// request's head, the warp stores the output; otherwise O / l and the log2 of the sum in f32, and
+// alone: its own ring of tiles in shared memory, filled by TMA boxes that lie in one page each and run on across
+// the ends of requests, its own running maximum and sum, no barrier with another warp.  Where a stretch holds all
+// the keys of a request's head, the warp stores the output; otherwise O / l and the log2 of the sum in f32, and
 // combine_kernel weighs the parts of each row.  A part's place follows from the lengths, so results do not
 // depend on the order in which warps run.
 //
-// S = Q K^T with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability (the products are not
-// what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
+// S = Q K^T with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability
+// (the products are not what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
+// Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
+// status word and stops.
 #include <type_traits>
 
 #include "attn.cuh"
 #include "decode_attn.cuh"
+#include "tc.cuh"
 
 namespace l3d {
 namespace decode {
 
-using attn::ex2f;
-using attn::max_nan;
-using attn::minus_max;
+using namespace l3d::attn;
 
 constexpr int WARPS = 8, KT = 16;       // warps of a block (one per SM), keys of a tile
 constexpr int MIN_TILES = 2;            // of a warp, where there are as many
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
 
+constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
+
+__device__ int g_decode_status;
+
 template <int D>
 struct Cfg {
-  static constexpr int ROW = D * 2, TILE = KT * ROW;       // bytes
+  static constexpr int DC = D / 64, HALF = KT * 128;       // a tile lies as DC pieces of 16 rows x 128 bytes
+  static constexpr int TILE = DC * HALF;                   // bytes of 16 keys
   static constexpr int STAGES = D == 128 ? 3 : 6;
   static constexpr int RING = STAGES * 2 * TILE;           // of one warp
+  static constexpr int BARS = 512;                         // barriers of all warps
+  static_assert(WARPS * STAGES * 8 + 8 <= BARS, "barrier area");
 };
-
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
 __device__ __forceinline__ int64_t value_at(const void* p, int is64, int64_t i) {
   return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
@@ -106,9 +112,15 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-// 16 bytes to shared memory; `bytes` 0: zeros, and nothing is read.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t dst, uint32_t v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(v) : "memory");
 }
 
 // A place in the line of tiles: sequence b, head and row tile hr, key tile t of `tiles`.
@@ -128,30 +140,41 @@ struct Cursor {
     hr = int(rem / tiles);
     t = int(rem - int64_t(hr) * tiles);
   }
-  // (Not past the line's last tile.)
-  __device__ __forceinline__ void next(const int* starts, int heads) {
-    if (++t < tiles) return;
+  // To the next tile (not past the line's last one); whether its head or row tile is another one.
+  __device__ __forceinline__ bool next(const int* starts, int heads) {
+    if (++t < tiles) return false;
     t = 0;
-    if (++hr < heads) return;
+    if (++hr < heads) return true;
     hr = 0;
     do {
       ++b;
       tiles = starts[b + 1] - starts[b];
     } while (tiles == 0);
+    return true;
   }
 };
 
 template <typename T, int D>
-__global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const Params p) {
+__global__ void __launch_bounds__(WARPS * 32, 1)
+    decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
-  constexpr int CHUNKS = D / 8;          // 16-byte pieces of a row
   constexpr int NT = D / 8;              // 8-wide column tiles of O
+  int* const status = &g_decode_status;
   extern __shared__ __align__(1024) uint8_t smem[];
-  int* starts = reinterpret_cast<int*>(smem + WARPS * C::RING);  // [B + 1]
+  if (smem_u32(smem) & 1023u) {
+    if (threadIdx.x == 0) atomicCAS(status, 0, ST_MISALIGNED);
+    return;
+  }
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * C::RING);  // [WARPS][STAGES]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + WARPS * C::STAGES);
+  int* starts = reinterpret_cast<int*>(smem + WARPS * C::RING + C::BARS);  // [B + 1]
   __shared__ int s_warp[WARPS];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");
 
+  if (threadIdx.x < WARPS * C::STAGES) mbar_init(&bars[threadIdx.x], 1);
+  if (threadIdx.x == 0) *abort_flag = 0;
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   // ---- key tiles before each sequence: a sum over the batch, a stretch of it per thread
   {
     const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(int(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
@@ -189,242 +212,268 @@ __global__ void __launch_bounds__(WARPS * 32, 1) decode_kernel(const Params p) {
   if (x0 >= line.total) return;
   const int count = int(min(line.per, line.total - x0));
 
-  // ---- loads: tile by tile ahead of the work.  Lane l looks up key l % 16 of the next tile one tile early,
-  // so that the table's latency is not waited for.
+  // ---- loads, STAGES tiles ahead of the work: lane i takes box i of a tile.  A tile's table entries are looked
+  // up one tile early, so that their latency is not waited for.
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
+  uint64_t* full = bars + warp * C::STAGES;
   Cursor ld;
   ld.seek(starts, p.B, heads, x0);
-  int ld_page = 0, ld_slot = 0, ld_ok = 0;  // of key lane % 16 of the cursor's tile
+  int ld_page = 0, ld_slot = 0, ld_h = 0, ld_len = 0, ld_first = 0;
+  bool ld_ok = false, ld_new = true;
   auto look_up = [&] {
-    bool bad;
-    const int len = length_of(p, ld.b, &bad), j = ld.t * KT + (lane & 15);
-    ld_ok = j < len;
+    if (ld_new) {
+      bool bad;
+      ld_len = length_of(p, ld.b, &bad);
+      ld_first = p.size ? 0 : packed_start(p, ld.b);
+      ld_h = ld.hr / p.tiles;
+    }
+    const int j = ld.t * KT + lane * p.box;
+    ld_ok = lane * p.box < KT && j < ld_len;
+    ld_page = 0;
+    ld_slot = ld_first + j;
     if (p.size) {
-      const int page = j / p.size;
+      const int page = p.size == 1 ? j : int(__umulhi(uint32_t(j), p.mul) >> p.shift);
       ld_slot = j - page * p.size;
-      ld_page = ld_ok ? p.table[ld.b * p.table_stride + page] : 0;
-    } else {
-      ld_page = 0;
-      ld_slot = packed_start(p, ld.b) + j;
+      if (ld_ok) ld_page = p.table[ld.b * p.table_stride + page];
     }
   };
   look_up();
-  int issued = 0;
-  uint32_t bad_keys[C::STAGES];
-  auto issue = [&](int stage, uint32_t& bad_mask) {
-    if (issued < count) {
-      // (Only now is the table's entry needed.)
-      const bool out = p.size && ld_ok && (ld_page < 0 || ld_page >= p.keys);
-      bad_mask = __ballot_sync(0xffffffffu, out) & 0xffffu;
-      const int have = ld_ok && !out ? 16 : 0, h = ld.hr / p.tiles;
-      const uint32_t kd = ring + stage * (2 * C::TILE), vd = kd + C::TILE;
-      constexpr int PER = 32 / CHUNKS;             // rows of a turn
-      const int c = lane % CHUNKS;
+  int issued = 0, ld_stage = 0;
+  auto issue = [&] {
+    if (issued >= count) return;
+    // (Only now is the table's entry needed.)
+    const bool in = ld_ok && (p.size == 0 || (ld_page >= 0 && ld_page < p.keys));
+    const uint32_t kd = ring + ld_stage * (2 * C::TILE), vd = kd + C::TILE;
+    const int boxes = __popc(__ballot_sync(0xffffffffu, in));
+    if (lane == 0) mbar_expect_tx(&full[ld_stage], boxes * p.box * (128 * 2 * C::DC));
+    __syncwarp();
+    if (in) {
+      const uint32_t at = lane * p.box * 128, bar = smem_u32(&full[ld_stage]);
 #pragma unroll
-      for (int i = 0; i < KT / PER; ++i) {
-        const int r = i * PER + lane / CHUNKS;
-        const int page = __shfl_sync(0xffffffffu, ld_page, r), slot = __shfl_sync(0xffffffffu, ld_slot, r);
-        const int bytes = __shfl_sync(0xffffffffu, have, r);
-        const uint32_t at = r * C::ROW + ((c ^ (r & 7)) << 4);
-        const T* ks = reinterpret_cast<const T*>(p.k) + (bytes ? page * p.ks[0] + slot * p.ks[1] + h * p.ks[2] + c * 8 : 0);
-        const T* vs = reinterpret_cast<const T*>(p.v) + (bytes ? page * p.vs[0] + slot * p.vs[1] + h * p.vs[2] + c * 8 : 0);
-        copy16(kd + at, ks, bytes);
-        copy16(vd + at, vs, bytes);
+      for (int dc = 0; dc < C::DC; ++dc) {
+        tma_box(kd + dc * C::HALF + at, &map_k, bar, dc * 64, p.kw.hn ? ld_h * p.kw.hm : ld_slot,
+                p.kw.hn ? ld_slot : ld_h * p.kw.hm, ld_page);
+        tma_box(vd + dc * C::HALF + at, &map_v, bar, dc * 64, p.vw.hn ? ld_h * p.vw.hm : ld_slot,
+                p.vw.hn ? ld_slot : ld_h * p.vw.hm, ld_page);
       }
-      if (++issued < count) {
-        ld.next(starts, heads);
-        look_up();
-      }
+    } else if (ld_ok) {  // a page that is none of the cache: K of NaN
+      for (int r = lane * p.box; r < (lane + 1) * p.box; ++r)
+        for (int c = 0; c < 8 * C::DC; ++c) store16(kd + (c >> 3) * C::HALF + r * 128 + (c & 7) * 16, 0xffffffffu);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++ld_stage == C::STAGES) ld_stage = 0;
+    if (++issued < count) {
+      ld_new = ld.next(starts, heads);
+      look_up();
+    }
   };
-#pragma unroll
-  for (int s = 0; s < C::STAGES; ++s) issue(s, bad_keys[s]);
+  for (int s = 0; s < C::STAGES; ++s) issue();
 
   // ---- work
   Cursor cu;
   cu.seek(starts, p.B, heads, x0);
   const int rg = lane >> 2, cq = (lane & 3) * 2;  // this thread's rows rg and rg + 8, columns cq, cq + 1 of 8
   const int R = p.N * p.G;
+  // Addresses of this lane's rows for ldmatrix, within a piece: 16-byte chunk c of row r at (c ^ r % 8) * 16.
+  const int kr = (lane & 7) + ((lane >> 4) << 3), vr = lane & 15;
+  uint32_t k_at[4], v_at[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    k_at[i] = kr * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (kr & 7)) << 4);
+    v_at[i] = C::TILE + vr * 128 + (((2 * i + (lane >> 4)) ^ (vr & 7)) << 4);
+  }
   uint32_t qf[D / 16][4];
   float o[NT][4];
   float m[2], l[2];
-  int lim[2], len = 0, t_first = 0, left = count, least = 0;
-  bool fresh = true;
+  int lim[2], len = 0, t_first = 0, least = 0, stage = 0, turn = 0;
+  bool fresh = true, ok = true;
   auto row_of = [&](int e, int* i, int* g) {
     const int f = (cu.hr % p.tiles) * 16 + rg + 8 * e;
     *i = f / p.G;
     *g = f - *i * p.G;
     return f < R;
   };
-  for (int n0 = 0; n0 < count; n0 += C::STAGES) {
-#pragma unroll
-    for (int s = 0; s < C::STAGES; ++s) {
-      if (n0 + s >= count) break;
-      if (fresh) {  // the first tile of a part
-        fresh = false;
-        t_first = cu.t;
-        bool bad;
-        len = length_of(p, cu.b, &bad);
-        least = p.causal ? len - p.N + 1 : len;
-        const int h = cu.hr / p.tiles;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          int i, g;
-          const bool in = row_of(e, &i, &g);
-          lim[e] = !in ? 0 : p.causal ? len - p.N + 1 + i : len;
-          m[e] = -INFINITY;
-          l[e] = bad && in ? __int_as_float(0x7fffffff) : 0.f;
-          const T* qr = reinterpret_cast<const T*>(p.q) + cu.b * p.qb + i * p.qn + (h * p.G + g) * p.qh;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            qf[k][e] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq) : 0u;
-            qf[k][e + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq + 8) : 0u;
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < NT; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
-      }
-      asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
-      __syncwarp();
-      const uint32_t kt = ring + s * (2 * C::TILE), vt = kt + C::TILE;
-      // S = Q K^T: two tiles of 8 keys
-      float sc[2][4] = {};
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int r = (lane & 7) + ((lane >> 4) << 3), c = 2 * k + ((lane >> 3) & 1);
-        uint32_t b[4];
-        ldsm4(b, kt + r * C::ROW + ((c ^ (r & 7)) << 4));
-        Mma<T>::run(sc[0], qf[k], b[0], b[1]);
-        Mma<T>::run(sc[1], qf[k], b[2], b[3]);
-      }
-      const int key0 = cu.t * KT;
-      if (bad_keys[s]) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (bad_keys[s] >> ((e >> 2) * 8 + cq + (e & 1)) & 1) sc[e >> 2][e & 3] = __int_as_float(0x7fffffff);
-      }
-      const bool edge = key0 + KT > least;  // some row does not see some key
-      if (edge) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (key0 + (e >> 2) * 8 + cq + (e & 1) >= lim[(e >> 1) & 1]) sc[e >> 2][e & 3] = -INFINITY;
-      }
-      float al[2];
-      bool grow[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float mx = max_nan(max_nan(sc[0][2 * e], sc[0][2 * e + 1]), sc[1][2 * e], sc[1][2 * e + 1]) * p.scale_log2;
-        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        grow[e] = !(mx <= m[e] + RESCALE_LOG2);
-        al[e] = grow[e] ? ex2f(m[e] - mx) : 1.f;  // 0 on the first key a row sees
-        if (grow[e]) m[e] = mx;
-      }
-      if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          o[i][0] *= al[0];
-          o[i][1] *= al[0];
-          o[i][2] *= al[1];
-          o[i][3] *= al[1];
-        }
-      }
-      float pr[2][4];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const float nm = m[e] == -INFINITY ? 0.f : minus_max(m[e]);
-        l[e] *= al[e];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          pr[i][2 * e] = ex2f(fmaf(sc[i][2 * e], p.scale_log2, nm));
-          pr[i][2 * e + 1] = ex2f(fmaf(sc[i][2 * e + 1], p.scale_log2, nm));
-          l[e] += pr[i][2 * e] + pr[i][2 * e + 1];
-        }
-      }
-      if (!edge || least == len) {
-        uint32_t hi[4], lo[4];
-        hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
-        hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
-        hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
-        hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
-#pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          const int r = lane & 15, c = 2 * i + (lane >> 4);
-          uint32_t b[4];
-          ldsm4t(b, vt + r * C::ROW + ((c ^ (r & 7)) << 4));
-          Mma<T>::run(o[2 * i], hi, b[0], b[1]);
-          Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
-          Mma<T>::run(o[2 * i], lo, b[0], b[1]);
-          Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
-        }
-      } else {
-        // Keys that only the later rows see: what an earlier row does not see, it does not meet times zero
-        // either, for V may be infinite or NaN there.
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int half = e >> 1, par = e & 1;
 #pragma unroll 1
-          for (int quad = 0; quad < 4; ++quad) {
-            const int key = half * 8 + quad * 2 + par, src = (lane & ~3) | quad;
-            const float p0 = __shfl_sync(0xffffffffu, pr[half][par], src);
-            const float p1 = __shfl_sync(0xffffffffu, pr[half][2 + par], src);
-            const bool see0 = key0 + key < lim[0], see1 = key0 + key < lim[1];
+  for (int n = 0; n < count; ++n) {
+    if (fresh) {  // the first tile of a part
+      fresh = false;
+      t_first = cu.t;
+      bool bad;
+      len = length_of(p, cu.b, &bad);
+      least = p.causal ? len - p.N + 1 : len;
+      const int h = cu.hr / p.tiles;
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-              T v[2];
-              uint32_t raw;
-              asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(vt + key * C::ROW + ((i ^ (key & 7)) << 4) + cq * 2) : "memory");
-              *reinterpret_cast<uint32_t*>(v) = raw;
-              if (see0) {
-                o[i][0] = fmaf(p0, to_f(v[0]), o[i][0]);
-                o[i][1] = fmaf(p0, to_f(v[1]), o[i][1]);
-              }
-              if (see1) {
-                o[i][2] = fmaf(p1, to_f(v[0]), o[i][2]);
-                o[i][3] = fmaf(p1, to_f(v[1]), o[i][3]);
-              }
-            }
-          }
+      for (int e = 0; e < 2; ++e) {
+        int i, g;
+        const bool in = row_of(e, &i, &g);
+        lim[e] = !in ? 0 : p.causal ? len - p.N + 1 + i : len;
+        m[e] = -INFINITY;
+        l[e] = bad && in ? __int_as_float(0x7fffffff) : 0.f;
+        const T* qr = reinterpret_cast<const T*>(p.q) + cu.b * p.qb + i * p.qn + (h * p.G + g) * p.qh;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          qf[k][e] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq) : 0u;
+          qf[k][e + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq + 8) : 0u;
         }
       }
-      __syncwarp();
-      issue(s, bad_keys[s]);
-      --left;
-      if (cu.t + 1 == cu.tiles || left == 0) {
-        // The end of a part: the output, or O / l and the log2 sum.
-        fresh = true;
-        const bool whole = t_first == 0 && cu.t + 1 == cu.tiles;
-        const int h = cu.hr / p.tiles;
-        const int64_t part = (2 * int64_t(me) + (t_first == 0 ? 1 : 0)) * p.rows;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          float sum = l[e];
-          sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-          sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-          const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
-          int i, g;
-          if (!row_of(e, &i, &g)) continue;
-          if (whole) {
-            T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh;
+      for (int i = 0; i < NT; ++i)
 #pragma unroll
-            for (int c = 0; c < NT; ++c) {
-              T v[2] = {from_f<T>(o[c][2 * e] * inv), from_f<T>(o[c][2 * e + 1] * inv)};
-              *reinterpret_cast<uint32_t*>(orow + c * 8 + cq) = *reinterpret_cast<const uint32_t*>(v);
-            }
-          } else {
-            const int64_t row = part + rg + 8 * e;
-            if (cq == 0) p.part_l[row] = sum > 0.f ? m[e] + log2f(sum) : sum == sum ? -INFINITY : sum;
-#pragma unroll
-            for (int c = 0; c < NT; ++c)
-              *reinterpret_cast<float2*>(p.part_o + row * D + c * 8 + cq) = make_float2(o[c][2 * e] * inv, o[c][2 * e + 1] * inv);
-          }
-        }
-      }
-      if (left > 0) cu.next(starts, heads);
+        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     }
+    ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], turn & 1, abort_flag, status, ST_TIMEOUT, p.wait_ns));
+    if (!ok) break;
+    __syncwarp();
+    const uint32_t tile = ring + stage * (2 * C::TILE);
+    // S = Q K^T: two tiles of 8 keys, even and odd steps of 16 summed apart (two chains of products each)
+    float sc[2][4] = {}, sd[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; k += 2) {
+      uint32_t b[4], c[4];
+      ldsm4(b, tile + (k >> 2) * C::HALF + k_at[k & 3]);
+      ldsm4(c, tile + (k >> 2) * C::HALF + k_at[(k & 3) + 1]);
+      Mma<T>::run(sc[0], qf[k], b[0], b[1]);
+      Mma<T>::run(sc[1], qf[k], b[2], b[3]);
+      Mma<T>::run(sd[0], qf[k + 1], c[0], c[1]);
+      Mma<T>::run(sd[1], qf[k + 1], c[2], c[3]);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] += sd[e >> 2][e & 3];
+    const int key0 = cu.t * KT;
+    const bool edge = key0 + KT > least;  // some row does not see some key
+    if (edge) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (key0 + (e >> 2) * 8 + cq + (e & 1) >= lim[(e >> 1) & 1]) sc[e >> 2][e & 3] = -INFINITY;
+      if (least == len) {  // V rows past the keys may hold anything: zero them, for 0 x NaN is not 0
+        const int r = lane >> 1;
+        if (key0 + r >= len)
+#pragma unroll
+          for (int c = 0; c < 4 * C::DC; ++c)
+            store16(tile + C::TILE + (c >> 2) * C::HALF + r * 128 + ((lane & 1) * 4 + (c & 3)) * 16, 0u);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+      }
+    }
+    float al[2];
+    bool grow[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float mx = max_nan(max_nan(sc[0][2 * e], sc[0][2 * e + 1]), sc[1][2 * e], sc[1][2 * e + 1]) * p.scale_log2;
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      grow[e] = !(mx <= m[e] + RESCALE_LOG2);
+      al[e] = grow[e] ? ex2f(m[e] - mx) : 1.f;  // 0 on the first key a row sees
+      if (grow[e]) m[e] = mx;
+    }
+    if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        o[i][0] *= al[0];
+        o[i][1] *= al[0];
+        o[i][2] *= al[1];
+        o[i][3] *= al[1];
+      }
+    }
+    float pr[2][4];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float nm = m[e] == -INFINITY ? 0.f : minus_max(m[e]);
+      l[e] *= al[e];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        pr[i][2 * e] = ex2f(fmaf(sc[i][2 * e], p.scale_log2, nm));
+        pr[i][2 * e + 1] = ex2f(fmaf(sc[i][2 * e + 1], p.scale_log2, nm));
+        l[e] += pr[i][2 * e] + pr[i][2 * e + 1];
+      }
+    }
+    if (!edge || least == len) {
+      uint32_t hi[4], lo[4];
+      hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
+      hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
+      hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
+      hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        uint32_t b[4];
+        ldsm4t(b, tile + (i >> 2) * C::HALF + v_at[i & 3]);
+        Mma<T>::run(o[2 * i], hi, b[0], b[1]);
+        Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
+        Mma<T>::run(o[2 * i], lo, b[0], b[1]);
+        Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
+      }
+    } else {
+      // Keys that only the later rows see: what an earlier row does not see, it does not meet times zero
+      // either, for V may be infinite or NaN there.
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int half = e >> 1, par = e & 1;
+#pragma unroll 1
+        for (int quad = 0; quad < 4; ++quad) {
+          const int key = half * 8 + quad * 2 + par, src = (lane & ~3) | quad;
+          const float p0 = __shfl_sync(0xffffffffu, pr[half][par], src);
+          const float p1 = __shfl_sync(0xffffffffu, pr[half][2 + par], src);
+          const bool see0 = key0 + key < lim[0], see1 = key0 + key < lim[1];
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            T v[2];
+            uint32_t raw;
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw)
+                         : "r"(tile + C::TILE + (i >> 3) * C::HALF + key * 128 + (((i & 7) ^ (key & 7)) << 4) + cq * 2) : "memory");
+            *reinterpret_cast<uint32_t*>(v) = raw;
+            if (see0) {
+              o[i][0] = fmaf(p0, to_f(v[0]), o[i][0]);
+              o[i][1] = fmaf(p0, to_f(v[1]), o[i][1]);
+            }
+            if (see1) {
+              o[i][2] = fmaf(p1, to_f(v[0]), o[i][2]);
+              o[i][3] = fmaf(p1, to_f(v[1]), o[i][3]);
+            }
+          }
+        }
+      }
+    }
+    __syncwarp();
+    issue();
+    if (++stage == C::STAGES) {
+      stage = 0;
+      ++turn;
+    }
+    if (cu.t + 1 == cu.tiles || n + 1 == count) {
+      // The end of a part: the output, or O / l and the log2 sum.
+      fresh = true;
+      const bool whole = t_first == 0 && cu.t + 1 == cu.tiles;
+      const int h = cu.hr / p.tiles;
+      const int64_t part = (2 * int64_t(me) + (t_first == 0 ? 1 : 0)) * p.rows;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float sum = l[e];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+        int i, g;
+        if (!row_of(e, &i, &g)) continue;
+        if (whole) {
+          T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh;
+#pragma unroll
+          for (int c = 0; c < NT; ++c) {
+            T v[2] = {from_f<T>(o[c][2 * e] * inv), from_f<T>(o[c][2 * e + 1] * inv)};
+            *reinterpret_cast<uint32_t*>(orow + c * 8 + cq) = *reinterpret_cast<const uint32_t*>(v);
+          }
+        } else {
+          const int64_t row = part + rg + 8 * e;
+          if (cq == 0) p.part_l[row] = sum > 0.f ? m[e] + log2f(sum) : sum == sum ? -INFINITY : sum;
+#pragma unroll
+          for (int c = 0; c < NT; ++c)
+            *reinterpret_cast<float2*>(p.part_o + row * D + c * 8 + cq) = make_float2(o[c][2 * e] * inv, o[c][2 * e + 1] * inv);
+        }
+      }
+    }
+    if (n + 1 < count) cu.next(starts, heads);
+  }
+  if (!ok && lane == 0) {  // the newest load of each stage: no copy may be in flight when the block exits
+    for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
+      mbar_drain(&full[i % C::STAGES], uint32_t(i / C::STAGES) & 1u, p.wait_ns);
   }
 }
 
@@ -524,12 +573,12 @@ size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
 }
 
 template <typename T, int D>
-static cudaError_t launch_t(const Params& p, int blocks, cudaStream_t s) {
+static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int blocks, cudaStream_t s) {
   auto k = decode_kernel<T, D>;
-  const int most = WARPS * Cfg<D>::RING + (MAX_BATCH + 1) * 4;
-  cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), most);
+  constexpr int fixed = WARPS * Cfg<D>::RING + Cfg<D>::BARS;
+  cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), fixed + (MAX_BATCH + 1) * 4);
   if (e != cudaSuccess) return e;
-  k<<<unsigned(blocks), WARPS * 32, WARPS * Cfg<D>::RING + (p.B + 1) * 4, s>>>(p);
+  k<<<unsigned(blocks), WARPS * 32, fixed + (p.B + 1) * 4, s>>>(maps[0], maps[1], p);
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   // The combination may be scheduled while the parts are formed; it waits for them.
@@ -547,19 +596,52 @@ static cudaError_t launch_t(const Params& p, int blocks, cudaStream_t s) {
   return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 4>, p);
 }
 
-cudaError_t launch(Params p, bool f16, int D, int64_t longest, void* workspace, cudaStream_t s) {
+int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
   const int R = p.N * p.G, blocks = blocks_for(p.B, p.N, p.G, p.Hkv, longest);
   p.tiles = (R + 15) / 16;
   p.rows = R < 16 ? R : 16;
   p.total_warps = blocks * WARPS;
+  p.wait_ns = tc::WAIT_LIMIT_NS;
   char* w = static_cast<char*>(workspace);
   p.starts = reinterpret_cast<int*>(w);
   w += (size_t(p.B + 1) * 4 + 255) / 256 * 256;
   p.part_l = reinterpret_cast<float*>(w);
   w += (size_t(2) * p.total_warps * p.rows * 4 + 255) / 256 * 256;
   p.part_o = reinterpret_cast<float*>(w);
-  if (f16) return D == 64 ? launch_t<__half, 64>(p, blocks, s) : launch_t<__half, 128>(p, blocks, s);
-  return D == 64 ? launch_t<__nv_bfloat16, 64>(p, blocks, s) : launch_t<__nv_bfloat16, 128>(p, blocks, s);
+  p.box = KT;
+  if (p.size) {
+    while (p.size % p.box) p.box /= 2;
+    // shift = floor(log2(size - 1)): mul exceeds 2^(32 + shift) / size by at most 1, so that the product is
+    // over by less than j / 2^(32 + shift) < 1 / size for j < 2^30.
+    while (p.size > 1 && (int64_t(2) << p.shift) <= p.size - 1) ++p.shift;
+    if (p.size > 1) p.mul = uint32_t((uint64_t(1) << (32 + p.shift)) / uint64_t(p.size) + 1);
+  }
+  CUtensorMap maps[2] = {};
+  if (p.keys > 0) {  // (without keys nothing is loaded)
+    const int64_t pages = p.size ? p.keys : 1, slots = p.size ? p.size : p.keys;
+    const void* base[] = {kv.k, kv.v};
+    const int64_t* st[] = {kv.ks, kv.vs};
+    View* view[] = {&p.kw, &p.vw};
+    for (int i = 0; i < 2; ++i) {
+      view[i]->hm = p.Hkv > 1 && st[i][2] == 0 ? 0 : 1;
+      if (!make_map4(&maps[i], base[i], pages, view[i]->hm ? p.Hkv : 1, slots, kv.D, st[i][1], st[i][2], st[i][0],
+                     uint32_t(p.box), &view[i]->hn))
+        return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed", op);
+    }
+  }
+  const cudaError_t e = f16 ? (kv.D == 64 ? launch_t<__half, 64>(maps, p, blocks, s) : launch_t<__half, 128>(maps, p, blocks, s))
+                            : (kv.D == 64 ? launch_t<__nv_bfloat16, 64>(maps, p, blocks, s)
+                                          : launch_t<__nv_bfloat16, 128>(maps, p, blocks, s));
+  return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+}
+
+cudaError_t status_read(int* status, int reset) {
+  cudaError_t e = cudaMemcpyFromSymbol(status, g_decode_status, sizeof(int));
+  if (e == cudaSuccess && reset) {
+    const int zero = 0;
+    e = cudaMemcpyToSymbol(g_decode_status, &zero, sizeof(int));
+  }
+  return e;
 }
 
 }  // namespace decode
@@ -627,6 +709,9 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
       if (t->dims[d] > 1 && t->strides[d] % 8)
         return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
   }
+  for (const l3d_tensor* t : {k_pages, v_pages})
+    if ((pages > 1 && t->strides[0] == 0) || (size > 1 && t->strides[1] == 0))
+      return fail(L3D_E_ALIGN, "%s: the pages must not be expanded (stride 0)", op);
   if (no_data(table) || no_data(lengths)) return fail(L3D_E_NULL, "%s: null data pointer", op);
   l3d::decode::Params p{};
   p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);
@@ -634,11 +719,10 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
   p.out = const_cast<char*>(elem_ptr(out));
   p.qb = q->strides[0]; p.qn = q->strides[1]; p.qh = q->strides[2];
   p.ob = out->strides[0]; p.on = out->strides[1]; p.oh = out->strides[2];
-  p.k = elem_ptr(k_pages);
-  p.v = elem_ptr(v_pages);
+  l3d::decode::Keys kv{elem_ptr(k_pages), elem_ptr(v_pages), {}, {}, D};
   for (int i = 0; i < 3; ++i) {
-    p.ks[i] = k_pages->strides[i];
-    p.vs[i] = v_pages->strides[i];
+    kv.ks[i] = k_pages->strides[i];
+    kv.vs[i] = v_pages->strides[i];
   }
   p.keys = int(pages); p.size = int(size); p.width = int(width);
   p.table = reinterpret_cast<const int32_t*>(elem_ptr(table));
@@ -647,7 +731,5 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
   p.len64 = lengths->dtype == L3D_I64;
   p.causal = 1;
   p.scale_log2 = scale_log2;
-  const cudaError_t e = l3d::decode::launch(p, q->dtype == L3D_F16, int(D), width * size, workspace,
-                                            reinterpret_cast<cudaStream_t>(stream));
-  return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
+  return l3d::decode::launch(op, p, kv, q->dtype == L3D_F16, width * size, workspace, reinterpret_cast<cudaStream_t>(stream));
 }

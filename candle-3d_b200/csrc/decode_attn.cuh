@@ -6,15 +6,28 @@
 namespace l3d {
 namespace decode {
 
+// How a K or V map [pages, slots, heads, D] lists its dimensions.
+struct View {
+  int hn, hm;                   // heads before slots; 0: heads expanded (stride 0)
+};
+// K and V as the caller has them: element strides of page, slot, head (packed: of row and head).
+struct Keys {
+  const void *k, *v;
+  int64_t ks[3], vs[3];
+  int64_t D;
+};
+
 struct Params {
   int B, N, G, Hkv;             // N rows a sequence, query heads h G .. h G + G - 1 read key head h
   const char* q;
   char* out;
   int64_t qb, qn, qh, ob, on, oh;   // element strides
-  const char *k, *v;
-  int64_t ks[3], vs[3];         // strides of page, slot, head (packed: unused, row, head)
+  View kw, vw;
   int keys;                     // pages, or packed rows
   int size, width;              // tokens of a page, pages of a request (packed: size 0)
+  int box;                      // rows of a load: the largest power of two, up to 16, that divides the size
+  uint32_t mul;                 // j / size = (j * mul) >> (32 + shift), j < 2^30 (size > 1)
+  int shift;
   const int32_t* table;
   int64_t table_stride;
   const void* lengths;          // paged: [B]; packed: offsets [B + 1]
@@ -22,6 +35,7 @@ struct Params {
   float scale_log2;             // softmax scale * log2(e), > 0
   int tiles, rows;              // row tiles of a key head, rows of a tile's part
   int total_warps;
+  uint64_t wait_ns;
   int* starts;                  // workspace: key tiles before each sequence [B + 1]
   float *part_l, *part_o;       // [2 warps, rows], [2 warps, rows, D]
 };
@@ -29,9 +43,9 @@ struct Params {
 constexpr int MAX_BATCH = 4096;
 // Workspace bytes, the same for every division of the keys; 0: nothing to do.
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D);
-// Fills in tiles, rows, total_warps and the workspace's places, and launches.  `longest`: the most keys a
-// sequence can have.
-cudaError_t launch(Params p, bool f16, int D, int64_t longest, void* workspace, cudaStream_t s);
+// Fills in what follows from the sizes and the workspace, and launches; an entry's status.  `longest`: the most
+// keys a sequence can have.
+int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s);
 
 }  // namespace decode
 }  // namespace l3d

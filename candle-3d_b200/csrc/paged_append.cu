@@ -19,7 +19,7 @@ namespace paged {
 
 constexpr int THREADS = 256;
 constexpr int MAX_TOKENS = 8;   // of one block
-constexpr int UNROLL = 3;       // rows that a thread loads before it works on the first
+constexpr int TPU = 4;          // tokens of a thread's unit
 
 struct Rows {                   // a [T, H, D] view
   char* p;
@@ -72,28 +72,28 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   constexpr int LANES = D / 8;                  // threads of a row
   constexpr int SLOTS = THREADS / LANES;        // rows of a block at a time
   __shared__ alignas(16) float s_cos[MAX_TOKENS][D / 2], s_sin[MAX_TOKENS][D / 2];
-  __shared__ int64_t s_place[MAX_TOKENS];       // in the request's sequence; -1: a token of no request
-  __shared__ int s_page[MAX_TOKENS];            // -1: no room
+  __shared__ int64_t s_at[MAX_TOKENS];          // place in the request's sequence
+  __shared__ int64_t s_k[MAX_TOKENS], s_v[MAX_TOKENS];  // where its key and value go; -1: no room
+  __shared__ int s_out[MAX_TOKENS];             // -1: a token of no request
   const int t0 = blockIdx.x * p.tokens, n = min(p.tokens, p.T - t0);
   if (threadIdx.x < n) {
-    int64_t first = 0, place = -1;
+    int64_t first = 0, place = 0;
     int page = -1;
     const int b = request_of(p, t0 + threadIdx.x, &first);
     if (b >= 0) {
       place = index_at(p.held, p.held64, b) + (t0 + threadIdx.x - first);
-      if (place >= 0 && place < int64_t(p.width) * p.size) {
-        page = p.table[b * p.table_stride + place / p.size];
-        if (page >= p.pages) page = -1;
-      }
-      if (page < 0) place = max(place, int64_t(0));
+      if (place >= 0 && place < int64_t(p.width) * p.size) page = p.table[b * p.table_stride + place / p.size];
     }
-    s_place[threadIdx.x] = place;
-    s_page[threadIdx.x] = page;
+    const bool room = page >= 0 && page < p.pages;
+    s_out[threadIdx.x] = b;
+    s_at[threadIdx.x] = place;
+    s_k[threadIdx.x] = room ? page * p.ks[0] + place % p.size * p.ks[1] : -1;
+    s_v[threadIdx.x] = room ? page * p.vs[0] + place % p.size * p.vs[1] : -1;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < n * p.pairs; i += THREADS) {
     const int t = i / p.pairs, pair = i - t * p.pairs;
-    int64_t at = s_place[t];
+    int64_t at = s_at[t];
     if (p.positions)
       at = index_at(p.positions, p.positions64,
                     (t0 + t) * p.position_stride + min(max(p.axis[pair], 0), p.axes - 1) * p.position_axis);
@@ -103,59 +103,57 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   }
   __syncthreads();
 
+  // A thread's unit is one head of TPU tokens of the block, whose loads it issues together; the head's address
+  // and weights are worked out once for them.  (One token at a time took 320 instructions per 16 bytes, and issue
+  // bound the kernel: 61 us for 10992 tokens x 48 heads x 64.)
   const int lane = threadIdx.x % LANES, e0 = lane * 8, slot = threadIdx.x / LANES;
-  const int heads = p.Hq + 2 * p.Hkv, rows = n * heads;
+  const int groups = (n + TPU - 1) / TPU;
   // Where this thread's elements stand in their pairs.
   const int block = p.half ? e0 / (2 * p.half) : 0, off = p.half ? e0 - block * 2 * p.half : 0;
   const bool second = p.half && off >= p.half;
   const int pair0 = p.half ? block * p.half + off - (second ? p.half : 0) : e0 / 2;
   const int other = (second ? lane - p.half / 8 : lane + p.half / 8) & (LANES - 1);
   const bool rotated = pair0 < p.pairs;
-  // (All threads of a warp take every turn: they meet in its shuffles.)
-  for (int r0 = 0; r0 < rows; r0 += SLOTS * UNROLL) {
-    uint4 raw[UNROLL];
+
+  // ---- queries and keys (all threads of a warp take every turn: they meet in its shuffles)
+  const int units = (p.Hq + p.Hkv) * groups;
+  for (int u0 = 0; u0 < units; u0 += SLOTS) {
+    const int u = min(u0 + slot, units - 1), grp = u / (p.Hq + p.Hkv), hh = u - grp * (p.Hq + p.Hkv);
+    const bool mine = u0 + slot < units, isq = hh < p.Hq;
+    const int h = isq ? hh : hh - p.Hq, ta = grp * TPU, tn = mine ? min(n - ta, TPU) : 0;
+    const T* src = reinterpret_cast<const T*>(isq ? p.q.p : p.k.p) + (t0 + ta) * (isq ? p.q.st : p.k.st) +
+                   h * (isq ? p.q.sh : p.k.sh) + e0;
+    const int64_t step = isq ? p.q.st : p.k.st;
+    uint4 raw[TPU];
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int r = r0 + u * SLOTS + slot;
-      raw[u] = make_uint4(0, 0, 0, 0);
-      if (r < rows) {
-        const int t = r / heads, h = r - t * heads;
-        const bool isq = h < p.Hq, isk = !isq && h < p.Hq + p.Hkv;
-        const Rows& w = isq ? p.q : isk ? p.k : p.v;
-        const int64_t at = (t0 + t) * w.st + (isq ? h : isk ? h - p.Hq : h - p.Hq - p.Hkv) * w.sh + e0;
-        raw[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(w.p) + at);
-      }
-    }
+    for (int i = 0; i < TPU; ++i)
+      raw[i] = i < tn ? *reinterpret_cast<const uint4*>(src + i * step) : make_uint4(0, 0, 0, 0);
+    float w[8];
+    if (p.qw.ptr) load_chan<8>(isq ? p.qw : p.kw, h, e0, w);
 #pragma unroll
-    for (int u = 0; u < UNROLL; ++u) {
-      const int r = min(r0 + u * SLOTS + slot, rows - 1);
-      const bool mine = r0 + u * SLOTS + slot < rows;
-      const int t = r / heads, h = r - t * heads;
-      const bool isq = h < p.Hq, isk = !isq && h < p.Hq + p.Hkv;
+    for (int i = 0; i < TPU; ++i) {
+      const int t = min(ta + i, n - 1);
       float x[8];
-      unpack(raw[u], x, T());
+      unpack(raw[i], x, T());
       if (p.qw.ptr) {
         float sum = 0.f;
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = 1.f / sqrtf(sum * (1.f / D) + p.eps);
-        if (isq || isk) {
-          float w[8];
-          load_chan<8>(isq ? p.qw : p.kw, isq ? h : h - p.Hq, e0, w);
+        const float inv = rsqrtf(sum * (1.f / D) + p.eps);  // to 2 ulp; what it goes into is rounded to 16 bits
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
-        }
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
       }
-      float y[8];
       if (p.half == 0) {
+        if (rotated) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const bool in = pair0 + e < p.pairs;
-          const float c = in ? s_cos[t][pair0 + e] : 1.f, s = in ? s_sin[t][pair0 + e] : 0.f;
-          y[2 * e] = in ? x[2 * e] * c - x[2 * e + 1] * s : x[2 * e];
-          y[2 * e + 1] = in ? x[2 * e + 1] * c + x[2 * e] * s : x[2 * e + 1];
+          for (int e = 0; e < 4; ++e) {
+            if (pair0 + e >= p.pairs) continue;
+            const float c = s_cos[t][pair0 + e], s = s_sin[t][pair0 + e], a = x[2 * e], b = x[2 * e + 1];
+            x[2 * e] = a * c - b * s;
+            x[2 * e + 1] = b * c + a * s;
+          }
         }
       } else {
         float z[8];  // the other elements of the pairs
@@ -169,30 +167,34 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
             *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(&s_sin[t][pair0 + e]);
           }
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = fmaf(x[e], c[e], second ? z[e] * s[e] : -(z[e] * s[e]));
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = x[e];
+          for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], second ? z[e] * s[e] : -(z[e] * s[e]));
         }
       }
-      const int64_t place = s_place[t];
-      const int page = s_page[t];
-      if (!mine || place < 0) continue;  // (the shuffles are behind us)
-      if (isq) {
-        if (page < 0) {  // no room: nothing is stored, and the request's attention is not finite
+      if (i < tn && s_out[t] >= 0) {  // (the shuffles are behind us)
+        if (isq) {
+          if (s_k[t] < 0) {  // no room: nothing is stored, and the request's attention is not finite
 #pragma unroll
-          for (int e = 0; e < 8; ++e) y[e] = __int_as_float(0x7fffffff);
+            for (int e = 0; e < 8; ++e) x[e] = __int_as_float(0x7fffffff);
+          }
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.qo.p) + (t0 + t) * p.qo.st + h * p.qo.sh + e0) = pack(x, T());
+        } else if (s_k[t] >= 0) {
+          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.kp) + s_k[t] + h * p.ks[2] + e0) = pack(x, T());
         }
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.qo.p) + (t0 + t) * p.qo.st + h * p.qo.sh + e0) = pack(y, T());
-      } else if (page >= 0) {
-        const int hk = isk ? h - p.Hq : h - p.Hq - p.Hkv;
-        const int64_t in_page = place % p.size;
-        if (isk)
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.kp) + page * p.ks[0] + in_page * p.ks[1] + hk * p.ks[2] + e0) = pack(y, T());
-        else
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.vp) + page * p.vs[0] + in_page * p.vs[1] + hk * p.vs[2] + e0) = raw[u];
       }
     }
+  }
+  // ---- values
+  for (int u = slot; u < p.Hkv * groups; u += SLOTS) {
+    const int grp = u / p.Hkv, h = u - grp * p.Hkv, ta = grp * TPU, tn = min(n - ta, TPU);
+    const T* src = reinterpret_cast<const T*>(p.v.p) + (t0 + ta) * p.v.st + h * p.v.sh + e0;
+    uint4 raw[TPU];
+#pragma unroll
+    for (int i = 0; i < TPU; ++i)
+      if (i < tn) raw[i] = *reinterpret_cast<const uint4*>(src + i * p.v.st);
+#pragma unroll
+    for (int i = 0; i < TPU; ++i)
+      if (i < tn && s_k[ta + i] >= 0)
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.vp) + s_v[ta + i] + h * p.vs[2] + e0) = raw[i];
   }
 }
 

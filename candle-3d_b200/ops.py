@@ -727,13 +727,13 @@ def paged_append(q, k, v, k_pages, v_pages, table, held, offsets=None, rope=None
     return out
 
 
-def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None):
+def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None, check=None):
     """exact_sdpa_heads (crate/runtime/attention_math.rs:199-259) of each request's
     newest tokens over its paged cache, which holds them already: q [B, N, Hq, D],
     or [B, Hq, D] for one token each; row i of request b sees the first
     lengths[b] - N + 1 + i of its keys (pages and table as for `paged_append`).
     BF16 or F16, D = 64 or 128; made for one token or a few: every 16 rows of a key
-    head (N * Hq / Hkv) read its keys once."""
+    head (N * Hq / Hkv) read its keys once.  `check` as in `attention`."""
     if out is None:
         out = empty(q, *q.shape)
     one = q.dim() == 3
@@ -745,8 +745,9 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None):
         need = _lib.lib().l3d_paged_attention_workspace_size(
             B, H, k_pages.shape[2], 1 if one else q.shape[1], table.shape[1] * k_pages.shape[1], D)
     ws = workspace(q, need)
-    call("l3d_paged_attention", dq, dk, dv, dt, dl, q.shape[-1] ** -0.5 if scale is None else float(scale), do, ws.data_ptr(), need,
-         stream_of(q))
+    call("l3d_paged_attention", dq, dk, dv, dt, dl, q.shape[-1] ** -0.5 if scale is None else float(scale),
+         do, ws.data_ptr(), need, stream_of(q))
+    _check_status("l3d_paged_attention", q, check)
     return out
 
 

@@ -102,7 +102,7 @@ int l3d_layer_norm(const l3d_tensor* x, const l3d_tensor* weight, const l3d_tens
  * counterpart in the reference: Candle ops report errors only on the host).
  * The row-norm entries stream long inputs through shared memory with bounded
  * waits, and so do l3d_lora_linear, l3d_shared_prefix_attention,
- * l3d_cross_attention and l3d_sandwich_residual_norm; a wait that runs out (status 5) is recorded in a
+ * l3d_paged_attention, l3d_cross_attention and l3d_sandwich_residual_norm; a wait that runs out (status 5) is recorded in a
  * per-device word, since none of them has a status word in a workspace.
  * This call copies it to *status (synchronising with the device) and clears
  * it when reset != 0.  0 = no wait has expired. */
@@ -539,7 +539,7 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * score that is NaN or +inf, or a key whose page is not one of the cache, and all
  * rows of a request whose length is more than its table has room for, NaN.  BF16
  * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
- * otherwise free in multiples of 16 bytes; softmax, sums and probabilities in f32
+ * otherwise free in multiples of 16 bytes (pages and slots not expanded); softmax, sums and probabilities in f32
  * (the latter enter the second product as two 16-bit parts).  scale must be
  * positive, and scale * log2(e) finite. */
 int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
