@@ -35,6 +35,7 @@ using namespace l3d::attn;
 
 constexpr int WARPS = 8, KT = 16;       // warps of a block (one per SM), keys of a tile
 constexpr int MIN_TILES = 2;            // of a warp, where there are as many
+constexpr int OWN_SUM = 256;            // requests up to which combine_kernel sums their keys up itself
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
 
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
@@ -123,6 +124,21 @@ __device__ __forceinline__ void store16(uint32_t dst, uint32_t v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst), "r"(v) : "memory");
 }
 
+// The exponent of infinities and NaN.
+template <typename T>
+constexpr uint32_t INF_BITS = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+// Whether one of the 8 values at a shared address is not finite.
+template <typename T>
+__device__ __forceinline__ bool not_finite(uint32_t at) {
+  uint32_t r[4];
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    any |= (r[i] & INF_BITS<T>) == INF_BITS<T> || (r[i] >> 16 & INF_BITS<T>) == INF_BITS<T>;
+  return any;
+}
+
 // A place in the line of tiles: sequence b, head and row tile hr, key tile t of `tiles`.
 struct Cursor {
   int b, hr, t, tiles;
@@ -202,7 +218,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     if (threadIdx.x == WARPS * 32 - 1) starts[p.B] = at;  // (its stretch is the last, or empty)
     __syncthreads();
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0 && p.B > OWN_SUM)
       for (int b = threadIdx.x; b <= p.B; b += WARPS * 32) p.starts[b] = starts[b];
   }
   const int heads = p.Hkv * p.tiles;
@@ -340,20 +356,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 #pragma unroll
     for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] += sd[e >> 2][e & 3];
     const int key0 = cu.t * KT;
-    const bool edge = key0 + KT > least;  // some row does not see some key
-    if (edge) {
+    bool mixed = false;
+    if (key0 + KT > least) {  // some row does not see some key
 #pragma unroll
       for (int e = 0; e < 8; ++e)
         if (key0 + (e >> 2) * 8 + cq + (e & 1) >= lim[(e >> 1) & 1]) sc[e >> 2][e & 3] = -INFINITY;
-      if (least == len) {  // V rows past the keys may hold anything: zero them, for 0 x NaN is not 0
-        const int r = lane >> 1;
-        if (key0 + r >= len)
+      // V rows past the keys may hold anything: zero them, for 0 x NaN is not 0.  Two lanes per row.
+      const int r = lane >> 1;
+      bool wild = false;  // a V that is not finite, of a key that only the later rows see
 #pragma unroll
-          for (int c = 0; c < 4 * C::DC; ++c)
-            store16(tile + C::TILE + (c >> 2) * C::HALF + r * 128 + ((lane & 1) * 4 + (c & 3)) * 16, 0u);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
+      for (int c = 0; c < 4 * C::DC; ++c) {
+        const uint32_t at = tile + C::TILE + (c >> 2) * C::HALF + r * 128 + ((lane & 1) * 4 + (c & 3)) * 16;
+        if (key0 + r >= len) store16(at, 0u);
+        else if (key0 + r >= least) wild |= not_finite<T>(at);
       }
+      mixed = __any_sync(0xffffffffu, wild);
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
     }
     float al[2];
     bool grow[2];
@@ -387,24 +406,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         l[e] += pr[i][2 * e] + pr[i][2 * e + 1];
       }
     }
-    if (!edge || least == len) {
-      uint32_t hi[4], lo[4];
-      hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
-      hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
-      hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
-      hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
-#pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        uint32_t b[4];
-        ldsm4t(b, tile + (i >> 2) * C::HALF + v_at[i & 3]);
-        Mma<T>::run(o[2 * i], hi, b[0], b[1]);
-        Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
-        Mma<T>::run(o[2 * i], lo, b[0], b[1]);
-        Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
-      }
-    } else {
-      // Keys that only the later rows see: what an earlier row does not see, it does not meet times zero
-      // either, for V may be infinite or NaN there.
+    if (mixed) {
+      // What a row does not see, it does not meet times zero either: such elements go to the rows that see them
+      // one by one, and out of the tile.
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int half = e >> 1, par = e & 1;
@@ -416,22 +420,47 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           const bool see0 = key0 + key < lim[0], see1 = key0 + key < lim[1];
 #pragma unroll
           for (int i = 0; i < NT; ++i) {
-            T v[2];
+            const uint32_t at = tile + C::TILE + (i >> 3) * C::HALF + key * 128 + (((i & 7) ^ (key & 7)) << 4) + cq * 2;
             uint32_t raw;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw)
-                         : "r"(tile + C::TILE + (i >> 3) * C::HALF + key * 128 + (((i & 7) ^ (key & 7)) << 4) + cq * 2) : "memory");
-            *reinterpret_cast<uint32_t*>(v) = raw;
-            if (see0) {
-              o[i][0] = fmaf(p0, to_f(v[0]), o[i][0]);
-              o[i][1] = fmaf(p0, to_f(v[1]), o[i][1]);
-            }
-            if (see1) {
-              o[i][2] = fmaf(p1, to_f(v[0]), o[i][2]);
-              o[i][3] = fmaf(p1, to_f(v[1]), o[i][3]);
+            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(at) : "memory");
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint16_t bits = uint16_t(raw >> (16 * x));
+              if ((bits & INF_BITS<T>) != INF_BITS<T>) continue;
+              const float v = to_f(*reinterpret_cast<const T*>(&bits));
+              if (see0) o[i][x] = fmaf(p0, v, o[i][x]);
+              if (see1) o[i][2 + x] = fmaf(p1, v, o[i][2 + x]);
             }
           }
         }
       }
+      __syncwarp();
+      for (int c = 0; c < 16 * C::DC; ++c) {  // (a lane's 4-byte words of half a row)
+        const int r = lane >> 1;
+        const uint32_t at = tile + C::TILE + (c >> 4) * C::HALF + r * 128 + (lane & 1) * 64 + (c & 15) * 4;
+        uint32_t raw;
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(at) : "memory");
+        if (key0 + r < least) continue;
+        if ((raw & INF_BITS<T>) == INF_BITS<T>) raw &= 0xffff0000u;
+        if ((raw >> 16 & INF_BITS<T>) == INF_BITS<T>) raw &= 0xffffu;
+        asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(raw) : "memory");
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    }
+    uint32_t hi[4], lo[4];
+    hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
+    hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
+    hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
+    hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) {
+      uint32_t b[4];
+      ldsm4t(b, tile + (i >> 2) * C::HALF + v_at[i & 3]);
+      Mma<T>::run(o[2 * i], hi, b[0], b[1]);
+      Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
+      Mma<T>::run(o[2 * i], lo, b[0], b[1]);
+      Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
     }
     __syncwarp();
     issue();
@@ -491,18 +520,45 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
   const int f = int(blockIdx.x % R), h = int(blockIdx.x / R % p.Hkv), b = int(blockIdx.x / R / p.Hkv);
   const int i = f / p.G, rt = f / 16, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + (h * p.G + f - i * p.G) * p.oh;
+  // The row's place in the line: summed up here from the lengths while the parts are formed, or, for a large
+  // batch, read from what the first kernel's first block has left.
+  bool bad;
+  int before = 0, tiles = (length_of(p, b, &bad) + KT - 1) / KT, all = 0;
+  if (p.B <= OWN_SUM) {
+    __shared__ int s_before[W], s_all[W];
+    for (int x = threadIdx.x; x < p.B; x += W * 32) {
+      bool ignored;
+      const int n = (length_of(p, x, &ignored) + KT - 1) / KT;
+      all += n;
+      if (x < b) before += n;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) {
+      s_before[warp] = before;
+      s_all[warp] = all;
+    }
+    __syncthreads();
+    before = all = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      before += s_before[w];
+      all += s_all[w];
+    }
+  }
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int before = p.starts[b], tiles = p.starts[b + 1] - before;
+  if (p.B > OWN_SUM) {
+    before = p.starts[b];
+    all = p.starts[p.B];
+  }
   if (tiles == 0) {
-    bool bad;
-    length_of(p, b, &bad);
     if (warp == 0) {
 #pragma unroll
       for (int e = 0; e < E; ++e) orow[lane * E + e] = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
     }
     return;
   }
-  const Line line = line_of(p, p.starts[p.B]);
+  const Line line = line_of(p, all);
   const int64_t first = int64_t(before) * heads + int64_t(hr) * tiles, last = first + tiles - 1;
   const int w0 = int(first / line.per), parts = int(last / line.per) - w0 + 1;
   if (parts == 1) return;
