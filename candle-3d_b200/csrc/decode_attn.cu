@@ -4,12 +4,14 @@
 // table[b, j / size]; or, for single rows of cross attention, over a packed stretch of an encoder's states.
 // The reference's attention core is exact_sdpa_heads (crate/runtime/attention_math.rs:199-259); it has no cache.
 //
-// Bound by the bytes of K and V, each read once: a key head's rows (i, g) = N G of them in tiles of 16, the
-// height of mma.m16n8k16, whose rate is some four times what the loads need (at one row of 16 as well).  The
-// 5th-generation tensor core takes tiles of 128 rows, and a round trip through its memory for each.
+// Bound by the bytes of K and V, each read once: a key head's rows (i, g), N G of them, in tiles of 8 or 16.
+// The products are taken the other way round, S^T = K Q^T and O^T = V^T P^T, so that keys and head dim fill the 16
+// rows of mma.m16n8k16 and the query rows its 8 columns: up to 8 rows cost half of what they would as the 16 rows
+// of S = Q K^T (in instructions, products and registers).  The 5th-generation tensor core takes tiles of 128
+// rows, and a round trip through its memory for each.
 //
-// Work is divided by keys alone: all (request, key head, row tile) have their keys in tiles of 16, the tiles of
-// all of them in one line, and every warp of the device takes an equal stretch of the line, whatever the
+// Work is divided by keys alone: all (request, key head, row tile) have their keys in tiles of 16 (32 at
+// D = 64: 8 KB of K and V either way), the tiles of all of them in one line, and every warp of the device takes an equal stretch of the line, whatever the
 // lengths are; the lengths are read on the device, and each block sums them up for itself.  A warp works
 // alone: its own ring of tiles in shared memory, filled by TMA boxes that lie in one page each and run on across
 // the ends of requests, its own running maximum and sum, no barrier with another warp.  Where a stretch holds all
@@ -17,7 +19,7 @@
 // combine_kernel weighs the parts of each row.  A part's place follows from the lengths, so results do not
 // depend on the order in which warps run.
 //
-// S = Q K^T with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability
+// Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability
 // (the products are not what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
@@ -33,23 +35,27 @@ namespace decode {
 
 using namespace l3d::attn;
 
-constexpr int WARPS = 8, KT = 16;       // warps of a block (one per SM), keys of a tile
-constexpr int MIN_TILES = 2;            // of a warp, where there are as many
+constexpr int WARPS = 12;               // of a block (one per SM)
+constexpr int MIN_TILES = 1;            // of a warp
 constexpr int OWN_SUM = 256;            // requests up to which combine_kernel sums their keys up itself
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
-
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 
 __device__ int g_decode_status;
 
+// Keys of a tile.
+__host__ __device__ constexpr int tile_keys(int D) { return D == 64 ? 32 : 16; }
+
 template <int D>
 struct Cfg {
-  static constexpr int DC = D / 64, HALF = KT * 128;       // a tile lies as DC pieces of 16 rows x 128 bytes
-  static constexpr int TILE = DC * HALF;                   // bytes of 16 keys
-  static constexpr int STAGES = D == 128 ? 3 : 6;
+  static constexpr int KT = tile_keys(D), MK = KT / 16;
+  static constexpr int DC = D / 64, HALF = KT * 128;       // a tile lies as DC pieces of KT rows x 128 bytes
+  static constexpr int TILE = DC * HALF;                   // bytes of K, or of V
+  static constexpr int STAGES = 2;
   static constexpr int RING = STAGES * 2 * TILE;           // of one warp
   static constexpr int BARS = 512;                         // barriers of all warps
   static_assert(WARPS * STAGES * 8 + 8 <= BARS, "barrier area");
+  static_assert(WARPS * RING + BARS + (MAX_BATCH + 1) * 4 <= 226 * 1024, "shared memory");
 };
 
 __device__ __forceinline__ int64_t value_at(const void* p, int is64, int64_t i) {
@@ -113,6 +119,12 @@ __device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
+// An 8 x 8 matrix of 16-bit values across the warp, transposed.
+__device__ __forceinline__ uint32_t transposed(uint32_t a) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
@@ -170,11 +182,12 @@ struct Cursor {
   }
 };
 
-template <typename T, int D>
+// NB: columns of 8 rows in a row tile.
+template <typename T, int D, int NB>
 __global__ void __launch_bounds__(WARPS * 32, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
-  constexpr int NT = D / 8;              // 8-wide column tiles of O
+  constexpr int KT = C::KT, MK = C::MK, NT = D / 16;   // 16-key tiles of S^T, 16-wide tiles of O^T
   int* const status = &g_decode_status;
   extern __shared__ __align__(1024) uint8_t smem[];
   if (smem_u32(smem) & 1023u) {
@@ -288,27 +301,23 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   // ---- work
   Cursor cu;
   cu.seek(starts, p.B, heads, x0);
-  const int rg = lane >> 2, cq = (lane & 3) * 2;  // this thread's rows rg and rg + 8, columns cq, cq + 1 of 8
+  // This thread's keys (or head dims) g and g + 8 of 16, its rows q2 and q2 + 1 of 8; Q is loaded for row g.
+  const int g8 = lane >> 2, q2 = (lane & 3) * 2;
   const int R = p.N * p.G;
   // Addresses of this lane's rows for ldmatrix, within a piece: 16-byte chunk c of row r at (c ^ r % 8) * 16.
-  const int kr = (lane & 7) + ((lane >> 4) << 3), vr = lane & 15;
+  const int r8 = lane & 7, mi = lane >> 3;
+  const uint32_t k_row = (r8 + (mi & 1) * 8) * 128, v_row = C::TILE + (r8 + (mi >> 1) * 8) * 128;
   uint32_t k_at[4], v_at[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    k_at[i] = kr * 128 + (((2 * i + ((lane >> 3) & 1)) ^ (kr & 7)) << 4);
-    v_at[i] = C::TILE + vr * 128 + (((2 * i + (lane >> 4)) ^ (vr & 7)) << 4);
+    k_at[i] = k_row + (((2 * i + (mi >> 1)) ^ r8) << 4);
+    v_at[i] = v_row + (((2 * i + (mi & 1)) ^ r8) << 4);
   }
-  uint32_t qf[D / 16][4];
-  float o[NT][4];
-  float m[2], l[2];
-  int lim[2], len = 0, t_first = 0, least = 0, stage = 0, turn = 0;
+  uint32_t qf[D / 16][NB][2];
+  float o[NT][NB][4];
+  float m[NB][2], l[NB][2];
+  int lim[NB][2], len = 0, t_first = 0, least = 0, stage = 0, turn = 0;
   bool fresh = true, ok = true;
-  auto row_of = [&](int e, int* i, int* g) {
-    const int f = (cu.hr % p.tiles) * 16 + rg + 8 * e;
-    *i = f / p.G;
-    *g = f - *i * p.G;
-    return f < R;
-  };
 #pragma unroll 1
   for (int n = 0; n < count; ++n) {
     if (fresh) {  // the first tile of a part
@@ -317,56 +326,63 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       bool bad;
       len = length_of(p, cu.b, &bad);
       least = p.causal ? len - p.N + 1 : len;
-      const int h = cu.hr / p.tiles;
+      const int h = cu.hr / p.tiles, f0 = (cu.hr - h * p.tiles) * (8 * NB);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        int i, g;
-        const bool in = row_of(e, &i, &g);
-        lim[e] = !in ? 0 : p.causal ? len - p.N + 1 + i : len;
-        m[e] = -INFINITY;
-        l[e] = bad && in ? __int_as_float(0x7fffffff) : 0.f;
-        const T* qr = reinterpret_cast<const T*>(p.q) + cu.b * p.qb + i * p.qn + (h * p.G + g) * p.qh;
+      for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          qf[k][e] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq) : 0u;
-          qf[k][e + 2] = in ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + cq + 8) : 0u;
+        for (int e = 0; e < 2; ++e) {
+          const int f = f0 + nb * 8 + q2 + e;
+          lim[nb][e] = f >= R ? 0 : p.causal ? len - p.N + 1 + f / p.G : len;
+          m[nb][e] = -INFINITY;
+          l[nb][e] = bad ? __int_as_float(0x7fffffff) : 0.f;
         }
+        const int f = f0 + nb * 8 + g8, i = f / p.G, g = f - i * p.G;
+        const T* qr = reinterpret_cast<const T*>(p.q) + cu.b * p.qb + i * p.qn + (h * p.G + g) * p.qh + q2;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            qf[k][nb][x] = f < R ? *reinterpret_cast<const uint32_t*>(qr + k * 16 + x * 8) : 0u;
+#pragma unroll
+        for (int i2 = 0; i2 < NT; ++i2)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i2][nb][e] = 0.f;
       }
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[i][e] = 0.f;
     }
     ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], turn & 1, abort_flag, status, ST_TIMEOUT, p.wait_ns));
     if (!ok) break;
     __syncwarp();
     const uint32_t tile = ring + stage * (2 * C::TILE);
-    // S = Q K^T: two tiles of 8 keys, even and odd steps of 16 summed apart (two chains of products each)
-    float sc[2][4] = {}, sd[2][4] = {};
+    // S^T = K Q^T; even and odd steps of 16 head dims summed apart (two chains of products)
+    float sc[MK][NB][4], sd[MK][NB][4];
 #pragma unroll
-    for (int k = 0; k < D / 16; k += 2) {
-      uint32_t b[4], c[4];
-      ldsm4(b, tile + (k >> 2) * C::HALF + k_at[k & 3]);
-      ldsm4(c, tile + (k >> 2) * C::HALF + k_at[(k & 3) + 1]);
-      Mma<T>::run(sc[0], qf[k], b[0], b[1]);
-      Mma<T>::run(sc[1], qf[k], b[2], b[3]);
-      Mma<T>::run(sd[0], qf[k + 1], c[0], c[1]);
-      Mma<T>::run(sd[1], qf[k + 1], c[2], c[3]);
-    }
+    for (int i = 0; i < MK * NB * 4; ++i) (&sc[0][0][0])[i] = (&sd[0][0][0])[i] = 0.f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sc[e >> 2][e & 3] += sd[e >> 2][e & 3];
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int mk = 0; mk < MK; ++mk) {
+        uint32_t a[4];
+        ldsm4(a, tile + (k >> 2) * C::HALF + mk * (16 * 128) + k_at[k & 3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) Mma<T>::run(k & 1 ? sd[mk][nb] : sc[mk][nb], a, qf[k][nb][0], qf[k][nb][1]);
+      }
+#pragma unroll
+    for (int i = 0; i < MK * NB * 4; ++i) (&sc[0][0][0])[i] += (&sd[0][0][0])[i];
     const int key0 = cu.t * KT;
     bool mixed = false;
     if (key0 + KT > least) {  // some row does not see some key
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (key0 + (e >> 2) * 8 + cq + (e & 1) >= lim[(e >> 1) & 1]) sc[e >> 2][e & 3] = -INFINITY;
-      // V rows past the keys may hold anything: zero them, for 0 x NaN is not 0.  Two lanes per row.
-      const int r = lane >> 1;
-      bool wild = false;  // a V that is not finite, of a key that only the later rows see
+      for (int mk = 0; mk < MK; ++mk)
 #pragma unroll
-      for (int c = 0; c < 4 * C::DC; ++c) {
-        const uint32_t at = tile + C::TILE + (c >> 2) * C::HALF + r * 128 + ((lane & 1) * 4 + (c & 3)) * 16;
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + mk * 16 + g8 + (e >> 1) * 8 >= lim[nb][e & 1]) sc[mk][nb][e] = -INFINITY;
+      // V rows past the keys may hold anything: zero them, for 0 x NaN is not 0.
+      bool wild = false;  // a V that is not finite, of a key that only the later rows see
+      for (int c = lane; c < C::TILE / 16; c += 32) {
+        const int r = (c >> 3) % KT;
+        const uint32_t at = tile + C::TILE + c * 16;
         if (key0 + r >= len) store16(at, 0u);
         else if (key0 + r >= least) wild |= not_finite<T>(at);
       }
@@ -374,73 +390,84 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    float al[2];
-    bool grow[2];
+    // The running maximum and sum of this thread's two rows (the maximum over all its warp's keys, the sum over
+    // its own ones).
+    bool grown = false;
+    float al[NB][2];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      float mx = max_nan(max_nan(sc[0][2 * e], sc[0][2 * e + 1]), sc[1][2 * e], sc[1][2 * e + 1]) * p.scale_log2;
-      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      grow[e] = !(mx <= m[e] + RESCALE_LOG2);
-      al[e] = grow[e] ? ex2f(m[e] - mx) : 1.f;  // 0 on the first key a row sees
-      if (grow[e]) m[e] = mx;
-    }
-    if (__any_sync(0xffffffffu, grow[0] || grow[1])) {
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) {
-        o[i][0] *= al[0];
-        o[i][1] *= al[0];
-        o[i][2] *= al[1];
-        o[i][3] *= al[1];
+      for (int e = 0; e < 2; ++e) {
+        float mx = max_nan(sc[0][nb][e], sc[0][nb][e + 2]);
+#pragma unroll
+        for (int mk = 1; mk < MK; ++mk) mx = max_nan(mx, sc[mk][nb][e], sc[mk][nb][e + 2]);
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) * p.scale_log2;
+        const bool grow = !(mx <= m[nb][e] + RESCALE_LOG2);
+        al[nb][e] = grow ? ex2f(m[nb][e] - mx) : 1.f;  // 0 on the first key a row sees
+        if (grow) m[nb][e] = mx;
+        grown |= grow;
+      }
+    if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) l[nb][e] *= al[nb][e];
+#pragma unroll
+        for (int i = 0; i < NT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[i][nb][e] *= al[nb][e & 1];
       }
     }
-    float pr[2][4];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float nm = m[e] == -INFINITY ? 0.f : minus_max(m[e]);
-      l[e] *= al[e];
+    for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        pr[i][2 * e] = ex2f(fmaf(sc[i][2 * e], p.scale_log2, nm));
-        pr[i][2 * e + 1] = ex2f(fmaf(sc[i][2 * e + 1], p.scale_log2, nm));
-        l[e] += pr[i][2 * e] + pr[i][2 * e + 1];
+      for (int e = 0; e < 2; ++e) {
+        const float nm = m[nb][e] == -INFINITY ? 0.f : minus_max(m[nb][e]);
+#pragma unroll
+        for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+          for (int x = 0; x < 4; x += 2) {
+            sc[mk][nb][e + x] = ex2f(fmaf(sc[mk][nb][e + x], p.scale_log2, nm));
+            l[nb][e] += sc[mk][nb][e + x];
+          }
       }
-    }
     if (mixed) {
       // What a row does not see, it does not meet times zero either: such elements go to the rows that see them
       // one by one, and out of the tile.
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int half = e >> 1, par = e & 1;
+      for (int mk = 0; mk < MK; ++mk)
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
 #pragma unroll 1
-        for (int quad = 0; quad < 4; ++quad) {
-          const int key = half * 8 + quad * 2 + par, src = (lane & ~3) | quad;
-          const float p0 = __shfl_sync(0xffffffffu, pr[half][par], src);
-          const float p1 = __shfl_sync(0xffffffffu, pr[half][2 + par], src);
-          const bool see0 = key0 + key < lim[0], see1 = key0 + key < lim[1];
+          for (int x = 0; x < 8; ++x) {
+            const int key = mk * 16 + half * 8 + x, src = x * 4 + (lane & 3);
 #pragma unroll
-          for (int i = 0; i < NT; ++i) {
-            const uint32_t at = tile + C::TILE + (i >> 3) * C::HALF + key * 128 + (((i & 7) ^ (key & 7)) << 4) + cq * 2;
-            uint32_t raw;
-            asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(at) : "memory");
+            for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-              const uint16_t bits = uint16_t(raw >> (16 * x));
-              if ((bits & INF_BITS<T>) != INF_BITS<T>) continue;
-              const float v = to_f(*reinterpret_cast<const T*>(&bits));
-              if (see0) o[i][x] = fmaf(p0, v, o[i][x]);
-              if (see1) o[i][2 + x] = fmaf(p1, v, o[i][2 + x]);
-            }
+              for (int e = 0; e < 2; ++e) {
+                const float pv = __shfl_sync(0xffffffffu, sc[mk][nb][half * 2 + e], src);
+                if (key0 + key < lim[nb][e]) {
+#pragma unroll
+                  for (int i = 0; i < 2 * NT; ++i) {
+                    const uint32_t at = tile + C::TILE + (i >> 3) * C::HALF + key * 128 + (((i & 7) ^ (key & 7)) << 4) + g8 * 2;
+                    uint16_t bits;
+                    asm volatile("ld.shared.b16 %0, [%1];" : "=h"(bits) : "r"(at) : "memory");
+                    if ((bits & INF_BITS<T>) == INF_BITS<T>) {
+                      float& acc = o[i >> 1][nb][(i & 1) * 2 + e];
+                      acc = fmaf(pv, to_f(*reinterpret_cast<const T*>(&bits)), acc);
+                    }
+                  }
+                }
+              }
           }
-        }
-      }
       __syncwarp();
-      for (int c = 0; c < 16 * C::DC; ++c) {  // (a lane's 4-byte words of half a row)
-        const int r = lane >> 1;
-        const uint32_t at = tile + C::TILE + (c >> 4) * C::HALF + r * 128 + (lane & 1) * 64 + (c & 15) * 4;
+      for (int c = lane; c < C::TILE / 4; c += 32) {
+        if (key0 + (c >> 5) % KT < least) continue;
+        const uint32_t at = tile + C::TILE + c * 4;
         uint32_t raw;
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(raw) : "r"(at) : "memory");
-        if (key0 + r < least) continue;
         if ((raw & INF_BITS<T>) == INF_BITS<T>) raw &= 0xffff0000u;
         if ((raw >> 16 & INF_BITS<T>) == INF_BITS<T>) raw &= 0xffffu;
         asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(raw) : "memory");
@@ -448,19 +475,28 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    uint32_t hi[4], lo[4];
-    hi[0] = Mma<T>::split(pr[0][0], pr[0][1], lo[0]);
-    hi[1] = Mma<T>::split(pr[0][2], pr[0][3], lo[1]);
-    hi[2] = Mma<T>::split(pr[1][0], pr[1][1], lo[2]);
-    hi[3] = Mma<T>::split(pr[1][2], pr[1][3], lo[3]);
+    // O^T += V^T P^T
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      uint32_t b[4];
-      ldsm4t(b, tile + (i >> 2) * C::HALF + v_at[i & 3]);
-      Mma<T>::run(o[2 * i], hi, b[0], b[1]);
-      Mma<T>::run(o[2 * i + 1], hi, b[2], b[3]);
-      Mma<T>::run(o[2 * i], lo, b[0], b[1]);
-      Mma<T>::run(o[2 * i + 1], lo, b[2], b[3]);
+    for (int mk = 0; mk < MK; ++mk) {
+      uint32_t hi[NB][2], lo[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          uint32_t rest;
+          hi[nb][x] = transposed(Mma<T>::split(sc[mk][nb][2 * x], sc[mk][nb][2 * x + 1], rest));
+          lo[nb][x] = transposed(rest);
+        }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        uint32_t a[4];
+        ldsm4t(a, tile + (i >> 2) * C::HALF + mk * (16 * 128) + v_at[i & 3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          Mma<T>::run(o[i][nb], a, hi[nb][0], hi[nb][1]);
+          Mma<T>::run(o[i][nb], a, lo[nb][0], lo[nb][1]);
+        }
+      }
     }
     __syncwarp();
     issue();
@@ -472,29 +508,40 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       // The end of a part: the output, or O / l and the log2 sum.
       fresh = true;
       const bool whole = t_first == 0 && cu.t + 1 == cu.tiles;
-      const int h = cu.hr / p.tiles;
+      const int h = cu.hr / p.tiles, f0 = (cu.hr - h * p.tiles) * (8 * NB);
       const int64_t part = (2 * int64_t(me) + (t_first == 0 ? 1 : 0)) * p.rows;
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float sum = l[e];
-        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        const float inv = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
-        int i, g;
-        if (!row_of(e, &i, &g)) continue;
-        if (whole) {
-          T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh;
+      for (int nb = 0; nb < NB; ++nb) {
+        float inv[2];
 #pragma unroll
-          for (int c = 0; c < NT; ++c) {
-            T v[2] = {from_f<T>(o[c][2 * e] * inv), from_f<T>(o[c][2 * e + 1] * inv)};
-            *reinterpret_cast<uint32_t*>(orow + c * 8 + cq) = *reinterpret_cast<const uint32_t*>(v);
+        for (int e = 0; e < 2; ++e) {
+          float sum = l[nb][e];
+          sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+          sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+          inv[e] = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
+          const int r = nb * 8 + q2 + e;
+          if (!whole && g8 == 0 && f0 + r < R)
+            p.part_l[part + r] = sum > 0.f ? m[nb][e] + log2f(sum) : sum == sum ? -INFINITY : sum;
+        }
+        if (whole) {
+          const int f = f0 + nb * 8 + g8, i = f / p.G, g = f - i * p.G;
+          T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh + q2;
+#pragma unroll
+          for (int c = 0; c < 2 * NT; ++c) {
+            const float* v = &o[c >> 1][nb][(c & 1) * 2];
+            const uint32_t pair = transposed(pack_pair<T>(v[0] * inv[0], v[1] * inv[1]));
+            if (f < R) *reinterpret_cast<uint32_t*>(orow + c * 8) = pair;
           }
         } else {
-          const int64_t row = part + rg + 8 * e;
-          if (cq == 0) p.part_l[row] = sum > 0.f ? m[e] + log2f(sum) : sum == sum ? -INFINITY : sum;
 #pragma unroll
-          for (int c = 0; c < NT; ++c)
-            *reinterpret_cast<float2*>(p.part_o + row * D + c * 8 + cq) = make_float2(o[c][2 * e] * inv, o[c][2 * e + 1] * inv);
+          for (int e = 0; e < 2; ++e) {
+            const int r = nb * 8 + q2 + e;
+            if (f0 + r >= R) continue;
+            float* orow = p.part_o + (part + r) * D + g8;
+#pragma unroll
+            for (int c = 0; c < 2 * NT; ++c) orow[c * 8] = o[c >> 1][nb][(c & 1) * 2 + e] * inv[e];
+          }
         }
       }
     }
@@ -518,10 +565,11 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int R = p.N * p.G;
   const int f = int(blockIdx.x % R), h = int(blockIdx.x / R % p.Hkv), b = int(blockIdx.x / R / p.Hkv);
-  const int i = f / p.G, rt = f / 16, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
+  const int i = f / p.G, rt = f / p.height, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + (h * p.G + f - i * p.G) * p.oh;
   // The row's place in the line: summed up here from the lengths while the parts are formed, or, for a large
   // batch, read from what the first kernel's first block has left.
+  constexpr int KT = tile_keys(D);
   bool bad;
   int before = 0, tiles = (length_of(p, b, &bad) + KT - 1) / KT, all = 0;
   if (p.B <= OWN_SUM) {
@@ -565,7 +613,7 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
   float m = -INFINITY, l = 0.f;
   alignas(16) float acc[E] = {};
   // (The first part lies in its warp's second place: it holds the row's first key.)
-  auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + (f & 15); };
+  auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + f - rt * p.height; };
   constexpr int U = 4;
   for (int k0 = warp; k0 < parts; k0 += W * U) {
     float pl[U];
@@ -615,22 +663,26 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
   }
 }
 
-static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest) {
+// Rows of a row tile: 8 hold all of a key head's, or 16.
+static int height_for(int64_t R) { return R <= 8 ? 8 : 16; }
+
+static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
   // (Warps past the line's end only cost their start.)
-  const int64_t most = B * Hkv * ((N * G + 15) / 16) * ((longest + KT - 1) / KT);
+  const int64_t h = height_for(N * G), most = B * Hkv * ((N * G + h - 1) / h) * ((longest + tile_keys(int(D)) - 1) / tile_keys(int(D)));
   const int64_t want = (most + MIN_TILES - 1) / MIN_TILES;
   return int(want < 1 ? 1 : want < sm_count() ? want : sm_count());
 }
 
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
-  if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0) return 0;
-  const int64_t rows = N * G < 16 ? N * G : 16, parts = 2 * int64_t(blocks_for(B, N, G, Hkv, longest)) * WARPS;
+  if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0 || D <= 0) return 0;
+  const int64_t h = height_for(N * G), rows = N * G < h ? N * G : h;
+  const int64_t parts = 2 * int64_t(blocks_for(B, N, G, Hkv, longest, D)) * WARPS;
   return (size_t(B + 1) * 4 + 255) / 256 * 256 + (size_t(parts * rows) * 4 + 255) / 256 * 256 + size_t(parts * rows * D) * 4;
 }
 
 template <typename T, int D>
 static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int blocks, cudaStream_t s) {
-  auto k = decode_kernel<T, D>;
+  auto k = p.height == 8 ? decode_kernel<T, D, 1> : decode_kernel<T, D, 2>;
   constexpr int fixed = WARPS * Cfg<D>::RING + Cfg<D>::BARS;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), fixed + (MAX_BATCH + 1) * 4);
   if (e != cudaSuccess) return e;
@@ -653,9 +705,10 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
 }
 
 int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
-  const int R = p.N * p.G, blocks = blocks_for(p.B, p.N, p.G, p.Hkv, longest);
-  p.tiles = (R + 15) / 16;
-  p.rows = R < 16 ? R : 16;
+  const int R = p.N * p.G, blocks = blocks_for(p.B, p.N, p.G, p.Hkv, longest, kv.D);
+  p.height = height_for(R);
+  p.tiles = (R + p.height - 1) / p.height;
+  p.rows = R < p.height ? R : p.height;
   p.total_warps = blocks * WARPS;
   p.wait_ns = tc::WAIT_LIMIT_NS;
   char* w = static_cast<char*>(workspace);
@@ -664,7 +717,7 @@ int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, 
   p.part_l = reinterpret_cast<float*>(w);
   w += (size_t(2) * p.total_warps * p.rows * 4 + 255) / 256 * 256;
   p.part_o = reinterpret_cast<float*>(w);
-  p.box = KT;
+  p.box = tile_keys(int(kv.D));
   if (p.size) {
     while (p.size % p.box) p.box /= 2;
     // shift = floor(log2(size - 1)): mul exceeds 2^(32 + shift) / size by at most 1, so that the product is

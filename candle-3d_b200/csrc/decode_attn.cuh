@@ -25,7 +25,7 @@ struct Params {
   View kw, vw;
   int keys;                     // pages, or packed rows
   int size, width;              // tokens of a page, pages of a request (packed: size 0)
-  int box;                      // rows of a load: the largest power of two, up to 16, that divides the size
+  int box;                      // rows of a load: the largest power of two, up to a tile's keys, that divides the size
   uint32_t mul;                 // j / size = (j * mul) >> (32 + shift), j < 2^30 (size > 1)
   int shift;
   const int32_t* table;
@@ -33,7 +33,7 @@ struct Params {
   const void* lengths;          // paged: [B]; packed: offsets [B + 1]
   int len64, causal;
   float scale_log2;             // softmax scale * log2(e), > 0
-  int tiles, rows;              // row tiles of a key head, rows of a tile's part
+  int height, tiles, rows;      // rows of a row tile, row tiles of a key head, rows of a tile's part
   int total_warps;
   uint64_t wait_ns;
   int* starts;                  // workspace: key tiles before each sequence [B + 1]
