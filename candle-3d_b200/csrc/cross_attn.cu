@@ -49,7 +49,7 @@ struct Cfg {
   static constexpr int SMEM = Q_BYTES + BUFS * KV_BYTES + REST;
   static constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TMEM_COLS = 256;
   static_assert(COL_O + D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
-  static_assert((2 * BUFS + 9) * 8 + 8 <= REST, "barrier area");
+  static_assert((2 * BUFS + 11) * 8 + 8 <= REST, "barrier area");
   // Of 8 pairs of P, those of ex2_poly2, as in prefix_attn.cu.
   static constexpr int POLY = D == 64 ? 2 : 1;
 };
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   uint64_t* v_full = k_empty + C::KST;               // [VST]
   uint64_t* v_empty = v_full + C::VST;               // [VST]
   uint64_t* s_full = v_empty + C::VST;               // [2] (by S buffer)
-  uint64_t* p_full = s_full + 2;                     // [2]
-  uint64_t* pv_done = p_full + 2;                    // [2]
+  uint64_t* p_full = s_full + 2;                     // [2][2] (by half of the keys)
+  uint64_t* pv_done = p_full + 4;                    // [2]
   uint64_t* q_full = pv_done + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* mma_drain = q_empty + 1;                 // abort teardown only
@@ -195,7 +195,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&p_full[i], 4);
+      mbar_init(&p_full[2 * i], 4);
+      mbar_init(&p_full[2 * i + 1], 4);
       mbar_init(&pv_done[i], 1);
     }
     mbar_init(q_full, 1);
@@ -312,17 +313,22 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     for (int i = 0; i < 2 && ok && more; ++i) issue_s();
     while (ok && find_v.next_with_keys(p, iv)) {
       for (int j = 0; ok && j < iv.tiles; ++j) {
-        ok = wait_warp(&p_full[n & 1], (n >> 1) & 1) && wait_warp(&v_full[vs], vturn & 1);
-        if (!ok) break;
-        tc_fence_after();
         // (P of an item's first tile comes after the last item's output was read: O is free.)
         const uint64_t db = smem_desc_sw128_mn(sv + vs * C::KV_BYTES, BKV * 128);
-        if (leader) {
+        ok = wait_warp(&v_full[vs], vturn & 1);
 #pragma unroll
-          for (int k = 0; k < BKV / 16; ++k)
-            umma_f16_ts<IDESC_O>(t_o, t_s + (n & 1) * BKV + uint32_t(k * 8), db + uint64_t(k * (16 * 128 >> 4)),
-                                 (j | k) ? 1u : 0u);
+        for (int half = 0; half < 2; ++half) {
+          ok = ok && wait_warp(&p_full[2 * (n & 1) + half], (n >> 1) & 1);
+          if (!ok) break;
+          tc_fence_after();
+          if (leader) {
+#pragma unroll
+            for (int k = 2 * half; k < 2 * half + 2; ++k)
+              umma_f16_ts<IDESC_O>(t_o, t_s + (n & 1) * BKV + uint32_t(k * 8), db + uint64_t(k * (16 * 128 >> 4)),
+                                   (j | k) ? 1u : 0u);
+          }
         }
+        if (!ok) break;
         commit(&v_empty[vs]);
         commit(&pv_done[n & 1]);  // the last commit of all: the block waits for it
         if (++vs == C::VST) {
@@ -375,7 +381,10 @@ __global__ void __launch_bounds__(THREADS, CTAS)
           ++vturn;
         }
         if (!active) {  // no rows: keep the other warps' pace
-          if (lane == 0) mbar_arrive(&p_full[n & 1]);
+          if (lane == 0) {
+            mbar_arrive(&p_full[2 * (n & 1)]);
+            mbar_arrive(&p_full[2 * (n & 1) + 1]);
+          }
           continue;
         }
         const uint32_t t_sn = t_s + (n & 1) * BKV;
@@ -426,12 +435,12 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             u[e >> 1] = pack_pair<T>(pr.x, pr.y);
           }
           tmem_st16u(t_sn + uint32_t(c / 2), u);
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * (n & 1) + c / 32]);
         }
         m = m_new;
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[n & 1]);
       }
       // The output, or this part's O / l and log2 sum, after the item's last P V.
       if (ok && it.tiles > 0) ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
