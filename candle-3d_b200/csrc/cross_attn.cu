@@ -65,6 +65,7 @@ struct Params {
   int q64, k64;
   void* out;
   int64_t ot, oh;              // element strides
+  int o_tma, o_th;             // the output's map can be used; it lists tokens before heads
   float scale_log2;            // softmax scale * log2(e), > 0
   int parts;
   float *part_l, *part_o;      // [parts, Tq, Hq], [parts, Tq, Hq, D]
@@ -151,10 +152,18 @@ struct Finder {
   }
 };
 
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];" ::"l"(
+          reinterpret_cast<uint64_t>(map)),
+      "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(THREADS, CTAS)
     cross_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                 const __grid_constant__ CUtensorMap map_v, const Params p) {
+                 const __grid_constant__ CUtensorMap map_v, const __grid_constant__ CUtensorMap map_o, const Params p) {
   using C = Cfg<D>;
   constexpr uint32_t IDESC_S = idesc_of<T>(128, BKV);
   constexpr uint32_t IDESC_O = idesc_of<T>(128, D) | (1u << 16);  // B (V) MN-major
@@ -337,7 +346,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
           ++vturn;
         }
         ++n;
-        if (more) issue_s();  // over the P that the product before it has read
+        // Scores up to two ahead, over the P that the product before it has read.  An item's first ones are not
+        // waited for while a product is still to come: its Q is on its way (that wait held up the last P V of
+        // the item before, 1,600 clocks of the 37,000 that an item of 18 tiles took).
+        while (ok && more && ns < n + 2 && (js > 0 || ns == n || __all_sync(0xffffffffu, mbar_try_wait(q_full, items & 1))))
+          issue_s();
       }
     }
   } else if (warp >= 4) {
@@ -349,9 +362,12 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     const int i = p.q_th ? r % p.tpt : r / p.G, g = p.q_th ? r / p.tpt : r - i * p.G;
     const float2 sc2 = f2(p.scale_log2);
     int n = 0, vs = 0, vturn = 0;
-    bool ok = true;
+    bool ok = true, stored = false;
     find.start(p);
-    while (ok && find.next(p, it)) {
+    Item coming;
+    bool any = find.next(p, coming);
+    while (ok && any) {
+      it = coming;
       const bool valid = i < it.rows && g < p.G;
       const bool active = __any_sync(0xffffffffu, valid);  // the warp holds rows
       float m = -INFINITY;                         // running max, log2 units
@@ -443,6 +459,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
         m = m_new;
       }
+      any = find.next(p, coming);  // (while the last product runs)
       // The output, or this part's O / l and log2 sum, after the item's last P V.
       if (ok && it.tiles > 0) ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
       tc_fence_after();
@@ -470,11 +487,19 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
         continue;
       }
-      // 64 columns of the warp's 32 rows at a time through shared memory, then whole 128-byte lines of four rows
-      // per store.  (Each thread storing its own row took 7,400 clocks an item, of 33,000.)
+      // 64 columns of the warp's 32 rows at a time through shared memory, then a TMA store; or, where some of the
+      // rows are no part of the sequence, whole 128-byte lines of four rows per store.  (Each thread storing its
+      // own row took 7,400 clocks an item, of 33,000, lines of four rows 3,300.)
       uint8_t* stage = so + (warp & 3) * (32 * 128);
+      const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+      const bool box = p.o_tma && rows == 0xffffffffu;
+      const int t_box = it.row0 + (warp & 3) * 32 / p.G, h_box = it.h * p.G;
 #pragma unroll 1
       for (int c = 0; c < D; c += 64) {
+        if (stored) {  // the last store has read the stage
+          if (lane == 0) bulk_wait_read0();
+          __syncwarp();
+        }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
           float o[32] = {};
@@ -487,8 +512,17 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * x + q) ^ (lane & 7)) << 4)) = pack(v, T());
           }
         }
+        stored = box;
+        if (box) {
+          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+          __syncwarp();
+          if (lane == 0) {
+            tma_store_3d(&map_o, stage, c, p.o_th ? t_box : h_box, p.o_th ? h_box : t_box);
+            bulk_commit();
+          }
+          continue;
+        }
         __syncwarp();
-        const uint32_t rows = __ballot_sync(0xffffffffu, valid);
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
           const int row = 4 * x + (lane >> 3);
@@ -499,6 +533,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         __syncwarp();
       }
     }
+    if (lane == 0) bulk_wait0();
   }
 
   // Teardown, as in attn.cu: after an abort nothing the block started may still be running when it frees TMEM
@@ -586,11 +621,11 @@ cudaError_t status_read(int* status, int reset) {
 }
 
 template <typename T, int D>
-static cudaError_t launch(const CUtensorMap (&maps)[3], const Params& p, int blocks, cudaStream_t s) {
+static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int blocks, cudaStream_t s) {
   auto k = cross_kernel<T, D>;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<D>::SMEM);
   if (e != cudaSuccess) return e;
-  k<<<unsigned(blocks), THREADS, Cfg<D>::SMEM, s>>>(maps[0], maps[1], maps[2], p);
+  k<<<unsigned(blocks), THREADS, Cfg<D>::SMEM, s>>>(maps[0], maps[1], maps[2], maps[3], p);
   if (p.parts <= 1) return cudaGetLastError();
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -606,8 +641,8 @@ static cudaError_t launch(const CUtensorMap (&maps)[3], const Params& p, int blo
   return cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p);
 }
 
-// The map of q [T, Hq, D] with boxes of G heads x tpt tokens, the nearer in memory listed first.
-static bool make_q_map(CUtensorMap* m, const void* base, int64_t T, int64_t Hq, int64_t D, int64_t st, int64_t sh, int G,
+// The map of q or out [T, Hq, D] with boxes of G heads x tpt tokens, the nearer in memory listed first.
+static bool make_row_map(CUtensorMap* m, const void* base, int64_t T, int64_t Hq, int64_t D, int64_t st, int64_t sh, int G,
                        int tpt, int* th) {
   auto fn = encode_fn();
   if (!fn) return false;
@@ -731,10 +766,16 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
   p.part_l = static_cast<float*>(workspace);
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (size_t(p.parts) * size_t(Tq * Hq) * 4 + 255) / 256 * 256);
   p.wait_ns = l3d::tc::WAIT_LIMIT_NS;
-  CUtensorMap maps[3];
+  CUtensorMap maps[4];
   p.k_hm = Hkv > 1 && k->strides[1] == 0 ? 0 : 1;
   p.v_hm = Hkv > 1 && v->strides[1] == 0 ? 0 : 1;
-  bool ok = make_q_map(&maps[0], elem_ptr(q), Tq, Hq, D, q->strides[0], q->strides[1], p.G, p.tpt, &p.q_th);
+  bool ok = make_row_map(&maps[0], elem_ptr(q), Tq, Hq, D, q->strides[0], q->strides[1], p.G, p.tpt, &p.q_th);
+  // A warp's 32 rows as a box of the output: whole tokens with their heads, listed as the rows are.
+  maps[3] = maps[0];
+  if (p.parts == 1 && 32 % p.G == 0 && (p.G == 1 || !p.q_th)) {
+    ok = ok && make_row_map(&maps[3], elem_ptr(out), Tq, Hq, D, out->strides[0], out->strides[1], p.G, 32 / p.G, &p.o_th);
+    p.o_tma = ok && (p.G == 1 || !p.o_th);
+  }
   if (Tk > 0)
     ok = ok && make_map4(&maps[1], elem_ptr(k), 1, p.k_hm ? Hkv : 1, Tk, D, k->strides[0], k->strides[1], 0, BKV, &p.k_hn) &&
          make_map4(&maps[2], elem_ptr(v), 1, p.v_hm ? Hkv : 1, Tk, D, v->strides[0], v->strides[1], 0, BKV, &p.v_hn);
