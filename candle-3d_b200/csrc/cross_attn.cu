@@ -6,12 +6,16 @@
 // (crate/runtime/attention_math.rs:199-259); it takes one sequence after the other.
 //
 // An item is a tile of up to 128 rows of one sequence and key head (128 / G tokens with their G query heads) by
-// all of the sequence's keys.  Blocks are persistent, two to an SM, and walk over the items, which they find from
-// the offsets themselves (lengths are never on the host): K and V rings run on from one item to the next, and
-// the next item's first scores are formed while the last one's output is divided and stored.
+// all of the sequence's keys.  The grid has a block per item; two blocks run on an SM, and each, while it
+// works, takes further items off the grid (cluster launch control), so that set-up is paid once and no SM waits for
+// the slowest.  K and V rings run on from one item to the next, and the next item's first scores are formed while
+// the last one's output is divided and stored.
 //   warp 0     loads Q tiles and the ring of 64-key K tiles, warp 2 the ring of V tiles (TMA);
 //   warp 1     issues S = Q K^T (two buffers of 64 columns, so that S(n + 2) is formed while softmax(n + 1) runs)
 //              and O += P V (P read from tensor memory, over the scores it comes from);
+//   warp 3     takes the items, one ahead of the loads, finds their rows and keys from the offsets (lengths are never
+//              on the host) and lists them in shared memory for the other warps, whose code this keeps small; those
+//              without keys it answers itself;
 //   warps 4-7  one row per thread: S to P in registers, the running maximum and sum, O's rescaling where the
 //              maximum has grown past 2^8, zeros over V rows past a sequence's end (another sequence's, or
 //              anything: a masked probability is 0, but 0 x NaN is not), and the output.
@@ -35,6 +39,9 @@ constexpr int BQ = 128, BKV = 64, THREADS = 256, CTAS = 2;
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 constexpr float RESCALE_LOG2 = 8.f;   // as in attn.cu
 constexpr int MAX_PARTS = 16;
+// Places of the list of items: the one that is looked for while up to three before it are not done with (the one
+// whose last product was just issued, and two of a tile each whose scores were).
+constexpr int LISTED = 4;
 
 __device__ int g_cross_status;
 
@@ -49,7 +56,7 @@ struct Cfg {
   static constexpr int SMEM = Q_BYTES + BUFS * KV_BYTES + OUT_BYTES + REST;
   static constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TMEM_COLS = 256;
   static_assert(COL_O + D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
-  static_assert((2 * BUFS + 11) * 8 + 8 <= REST, "barrier area");
+  static_assert((2 * BUFS + 13 + 2 * LISTED) * 8 + 8 + 16 + LISTED * 32 <= REST, "barrier area");
   // Of 8 pairs of P, those of ex2_poly2, as in prefix_attn.cu.
   static constexpr int POLY = D == 64 ? 2 : 0;
 };
@@ -78,20 +85,20 @@ __device__ __forceinline__ int offset_at(const void* p, int is64, int i, int mos
   return v < 0 ? 0 : v < most ? int(v) : most;
 }
 
-struct Item {
-  int h, part;
+struct alignas(16) Item {
+  int h, part;                 // h < 0: no further item
   int row0, rows;              // the tile's first token, its tokens
   int key0, keys;              // the sequence's first key, its keys
   int t0, tiles;               // the part's first key tile and its number
 };
+static_assert(sizeof(Item) == 32, "two 16-byte loads");
 
-// Walks over the items idx = blockIdx.x, + gridDim.x, ...: (tile, key head, part), the part fastest.  The warp
-// holds 32 sequences at a time, one per lane.
+// Finds items by their numbers, (tile, key head, part) with the part fastest.  The warp holds 32 sequences at a
+// time, one per lane.
 struct Finder {
-  int idx, window;
+  int window;
   int64_t base;                // tiles before the window
   int cnt, incl, q0, q1, k0, k1;
-  bool more;
   __device__ __forceinline__ void load(const Params& p) {
     const int b = window * 32 + (threadIdx.x & 31);
     q0 = q1 = k0 = k1 = 0;
@@ -110,23 +117,19 @@ struct Finder {
     }
   }
   __device__ __forceinline__ void start(const Params& p) {
-    idx = int(blockIdx.x) - int(gridDim.x);
     base = 0;
     window = 0;
     load(p);
   }
-  // The next item, of any number of keys.
-  __device__ __forceinline__ bool next(const Params& p, Item& it) {
-    idx += gridDim.x;
+  // False: past the last item.
+  __device__ __forceinline__ bool at(const Params& p, int idx, Item& it) {
     const int per = p.Hkv * p.parts, tile = idx / per;
+    if (tile < base) start(p);
     int all;
     while (tile - base >= (all = __shfl_sync(0xffffffffu, incl, 31))) {
+      if ((window + 1) * 32 >= p.B) return false;
       base += all;
-      if (++window * 32 >= p.B) {
-        --window;  // stay: a further call ends here too
-        base -= all;
-        return more = false;
-      }
+      ++window;
       load(p);
     }
     const int rel = int(tile - base);
@@ -143,14 +146,31 @@ struct Finder {
     const int tiles = (it.keys + BKV - 1) / BKV, chunk = (tiles + p.parts - 1) / p.parts;
     it.t0 = min(it.part * chunk, tiles);
     it.tiles = min(chunk, tiles - it.t0);
-    return more = true;
-  }
-  __device__ __forceinline__ bool next_with_keys(const Params& p, Item& it) {
-    while (next(p, it))
-      if (it.tiles > 0) return true;
-    return false;
+    return true;
   }
 };
+
+// Asks for a block of the grid that has not started yet; the answer comes to 16 bytes of shared memory.
+__device__ __forceinline__ void take_block(uint32_t answer, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(answer),
+      "r"(smem_u32(bar))
+      : "memory");
+}
+// The block's number, -1: none was left.
+__device__ __forceinline__ int taken_block(uint32_t answer) {
+  uint32_t got, x;
+  asm volatile(
+      "{\n\t.reg .b128 r;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\tmov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(answer)
+      : "memory");
+  return got ? int(x) : -1;
+}
 
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, const void* src, int c0, int c1, int c2) {
   asm volatile(
@@ -188,8 +208,14 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   uint64_t* q_full = pv_done + 2;
   uint64_t* q_empty = q_full + 1;
   uint64_t* mma_drain = q_empty + 1;                 // abort teardown only
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(mma_drain + 1);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(mma_drain + 2);
+  uint64_t* answered = mma_drain + 1;
+  uint64_t* started = answered + 1;                  // an item's loads have begun
+  uint64_t* listed = started + 1;                    // [LISTED]
+  uint64_t* unlisted = listed + LISTED;              // [LISTED]
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(unlisted + LISTED);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(unlisted + LISTED) + 1;
+  uint8_t* answer = so + C::OUT_BYTES + C::REST - 16 - LISTED * 32;
+  Item* list = reinterpret_cast<Item*>(answer + 16);  // [LISTED]
 
   // (The shuffle tells the compiler that the role is the same in all lanes.)
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -212,6 +238,12 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
     mbar_init(mma_drain, 1);
+    mbar_init(answered, 1);
+    mbar_init(started, 1);
+    for (int i = 0; i < LISTED; ++i) {
+      mbar_init(&listed[i], 1);
+      mbar_init(&unlisted[i], 7);  // two loading warps, the MMA warp, four softmax warps
+    }
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -233,9 +265,20 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     __syncwarp();  // before the warp-wide (.aligned) instructions that follow
     return got;
   };
-  Finder find;
   Item it;
-  int loads = 0, q_loads = 0;  // of this warp's ring, of Q (abort teardown)
+  int loads = 0, q_loads = 0, asked = 0;  // of this warp's ring, of Q, for blocks (abort teardown)
+  // The listed item number i (of this block); false: there is none, or a wait ran out.
+  auto item = [&](int i, Item& t) {
+    if (!wait_warp(&listed[i % LISTED], (i / LISTED) & 1)) return false;
+    const int4* src = reinterpret_cast<const int4*>(list + i % LISTED);
+    reinterpret_cast<int4*>(&t)[0] = src[0];
+    reinterpret_cast<int4*>(&t)[1] = src[1];
+    return t.h >= 0;
+  };
+  auto done_with = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&unlisted[i % LISTED]);
+  };
 
   if (warp == 0 || warp == 2) {
     // ------------------------------------------------------- loads of Q and K; of V
@@ -248,11 +291,11 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     const int hn = isk ? p.k_hn : p.v_hn, hm = isk ? p.k_hm : p.v_hm;
     int s = 0, turn = 0;
     bool ok = true;
-    find.start(p);
-    while (ok && find.next_with_keys(p, it)) {
+    for (int i = 0; ok && item(i, it); done_with(i++)) {
       if (isk) {
+        if (lane == 0) mbar_arrive(started);
         if (q_loads > 0) ok = wait_warp(q_empty, (q_loads - 1) & 1);
-        if (!ok) break;
+        if (!ok) continue;
         if (lane == 0) {
           mbar_expect_tx(q_full, C::DC * 128 * p.tpt * p.G);
           for (int dc = 0; dc < C::DC; ++dc)
@@ -288,8 +331,15 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     };
     const uint32_t t_s = tmem_base + C::COL_S, t_o = tmem_base + C::COL_O;
     int ns = 0, js = 0, ks = 0, kturn = 0, items = 0;  // of the next scores: number, tile of its item, K slot, Q
-    find.start(p);
-    bool more = find.next_with_keys(p, it), ok = true;
+    int is = 0, tiles_s = 0;                           // its item's number and tiles
+    bool ok = true;
+    auto next_s = [&] {
+      Item t;
+      const bool got = item(is, t);
+      tiles_s = t.tiles;
+      return got;
+    };
+    bool more = next_s();
     auto issue_s = [&] {
       if (js == 0) ok = wait_warp(q_full, items & 1);
       ok = ok && wait_warp(&k_full[ks], kturn & 1);
@@ -309,20 +359,18 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         ++kturn;
       }
       ++ns;
-      if (++js == it.tiles) {
+      if (++js == tiles_s) {
         commit(q_empty);
         js = 0;
         ++items;
-        more = find.next_with_keys(p, it);
+        ++is;
+        more = next_s();
       }
     };
-    Finder find_v;
-    Item iv;
-    find_v.start(p);
     int n = 0, vs = 0, vturn = 0;
     for (int i = 0; i < 2 && ok && more; ++i) issue_s();
-    while (ok && find_v.next_with_keys(p, iv)) {
-      for (int j = 0; ok && j < iv.tiles; ++j) {
+    for (int i = 0; ok && item(i, it); done_with(i++)) {
+      for (int j = 0; ok && j < it.tiles; ++j) {
         // (P of an item's first tile comes after the last item's output was read: O is free.)
         const uint64_t db = smem_desc_sw128_mn(sv + vs * C::KV_BYTES, BKV * 128);
         ok = wait_warp(&v_full[vs], vturn & 1);
@@ -353,7 +401,56 @@ __global__ void __launch_bounds__(THREADS, CTAS)
           issue_s();
       }
     }
-  } else if (warp >= 4) {
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- items
+    // (An item can take longer than any wait for a tile: the waits here are bounded by 30 times as long.)
+    auto wait_item = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, ST_TIMEOUT, 30 * p.wait_ns)) != 0;
+    };
+    Finder find;
+    find.start(p);
+    int idx = int(blockIdx.x), i = 0;
+    bool ok = true;
+    while (ok && idx >= 0) {
+      if (find.at(p, idx, it)) {
+        if (it.tiles > 0) {
+          if (i >= LISTED) ok = wait_item(&unlisted[i % LISTED], ((i / LISTED) - 1) & 1);
+          if (!ok) break;
+          if (lane == 0) {
+            list[i % LISTED] = it;
+            mbar_arrive(&listed[i % LISTED]);
+          }
+          ok = wait_item(started, i & 1);
+          ++i;
+        } else if (p.parts > 1) {
+          for (int x = lane; x < it.rows * p.G; x += 32)
+            p.part_l[(int64_t(it.part) * p.Tq + it.row0 + x / p.G) * (p.Hkv * p.G) + it.h * p.G + x % p.G] = -INFINITY;
+        } else {  // no keys: zeros
+          for (int x = lane; x < it.rows * p.G * (D / 8); x += 32) {
+            const int r = x / (D / 8);
+            T* dst = static_cast<T*>(p.out) + (it.row0 + r / p.G) * p.ot + int64_t(it.h * p.G + r % p.G) * p.oh;
+            *reinterpret_cast<uint4*>(dst + x % (D / 8) * 8) = make_uint4(0, 0, 0, 0);
+          }
+        }
+      }
+      if (!ok) break;
+      if (lane == 0) {
+        mbar_expect_tx(answered, 16);
+        take_block(smem_u32(answer), answered);
+      }
+      ++asked;
+      ok = wait_warp(answered, (asked - 1) & 1);
+      if (ok) idx = taken_block(smem_u32(answer));
+      // (The answer's place is written again by the async proxy.)
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+    }
+    if (ok && i >= LISTED) ok = wait_item(&unlisted[i % LISTED], ((i / LISTED) - 1) & 1);
+    if (ok && lane == 0) {
+      list[i % LISTED].h = -1;
+      mbar_arrive(&listed[i % LISTED]);
+    }
+  } else {
     // ------------------------------------------------------ softmax / epilogue
     const int r = (warp & 3) * 32 + lane;
     const uint32_t lane_off = uint32_t((warp & 3) * 32) << 16;
@@ -363,11 +460,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     const float2 sc2 = f2(p.scale_log2);
     int n = 0, vs = 0, vturn = 0;
     bool ok = true, stored = false;
-    find.start(p);
-    Item coming;
-    bool any = find.next(p, coming);
-    while (ok && any) {
-      it = coming;
+    for (int at = 0; ok && item(at, it); done_with(at++)) {
       const bool valid = i < it.rows && g < p.G;
       const bool active = __any_sync(0xffffffffu, valid);  // the warp holds rows
       float m = -INFINITY;                         // running max, log2 units
@@ -459,9 +552,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
         m = m_new;
       }
-      any = find.next(p, coming);  // (while the last product runs)
       // The output, or this part's O / l and log2 sum, after the item's last P V.
-      if (ok && it.tiles > 0) ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
+      if (ok) ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);
       tc_fence_after();
       if (!ok || !active) continue;
       float l = l2.x + l2.y;
@@ -475,8 +567,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
       if (p.parts > 1) {
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
-          float o[32] = {};
-          if (it.tiles > 0) tmem_ld32(t_o + uint32_t(c), o);
+          float o[32];
+          tmem_ld32(t_o + uint32_t(c), o);
           if (valid) {
             float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
 #pragma unroll
@@ -502,8 +594,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          float o[32] = {};
-          if (it.tiles > 0) tmem_ld32(t_o + uint32_t(c + 32 * x), o);
+          float o[32];
+          tmem_ld32(t_o + uint32_t(c + 32 * x), o);
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             float v[8];
@@ -545,6 +637,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
       umma_commit(mma_drain);
       mbar_drain(mma_drain, 0, p.wait_ns);
     }
+    if (warp == 3 && lane == 0 && asked > 0) mbar_drain(answered, uint32_t(asked - 1) & 1u, p.wait_ns);
     if ((warp == 0 || warp == 2) && lane == 0) {  // the newest load of each slot, and of Q
       const int stages = warp == 0 ? C::KST : C::VST;
       for (int i = max(loads - stages, 0); i < loads; ++i)
@@ -621,11 +714,11 @@ cudaError_t status_read(int* status, int reset) {
 }
 
 template <typename T, int D>
-static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int blocks, cudaStream_t s) {
+static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int64_t items, cudaStream_t s) {
   auto k = cross_kernel<T, D>;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), Cfg<D>::SMEM);
   if (e != cudaSuccess) return e;
-  k<<<unsigned(blocks), THREADS, Cfg<D>::SMEM, s>>>(maps[0], maps[1], maps[2], maps[3], p);
+  k<<<unsigned(items), THREADS, Cfg<D>::SMEM, s>>>(maps[0], maps[1], maps[2], maps[3], p);
   if (p.parts <= 1) return cudaGetLastError();
   e = cudaGetLastError();
   if (e != cudaSuccess) return e;
@@ -782,11 +875,10 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
   else
     maps[1] = maps[2] = maps[0];  // never read
   if (!ok) return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed", op);
-  const int64_t items = (Hkv * (Tq / p.tpt + B)) * p.parts, most = CTAS * int64_t(sm_count());
-  const int blocks = int(items < most ? items : most);
+  const int64_t items = Hkv * (Tq / p.tpt + B) * p.parts;  // at most: a sequence's last tile may be cut short
   if (q->dtype == L3D_BF16)
-    e = D == 64 ? launch<__nv_bfloat16, 64>(maps, p, blocks, s) : launch<__nv_bfloat16, 128>(maps, p, blocks, s);
+    e = D == 64 ? launch<__nv_bfloat16, 64>(maps, p, items, s) : launch<__nv_bfloat16, 128>(maps, p, items, s);
   else
-    e = D == 64 ? launch<__half, 64>(maps, p, blocks, s) : launch<__half, 128>(maps, p, blocks, s);
+    e = D == 64 ? launch<__half, 64>(maps, p, items, s) : launch<__half, 128>(maps, p, items, s);
   return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
 }
