@@ -57,8 +57,9 @@ struct Cfg {
   static constexpr uint32_t COL_S = 0, COL_O = 2 * BKV, TMEM_COLS = 256;
   static_assert(COL_O + D <= TMEM_COLS && TMEM_COLS * CTAS <= 512, "TMEM budget");
   static_assert((2 * BUFS + 13 + 2 * LISTED) * 8 + 8 + 16 + LISTED * 32 <= REST, "barrier area");
-  // Of 8 pairs of P, those of ex2_poly2, as in prefix_attn.cu.
-  static constexpr int POLY = D == 64 ? 2 : 0;
+  // Of 8 pairs of P, those of ex2_poly2: none at D = 128 (voxel scenes 657 us, 669 with one), one at D = 64
+  // (4 x 8192 rows x 16 heads over 1370 keys: 198 us, 214 without, 200 with two).
+  static constexpr int POLY = D == 64 ? 1 : 0;
 };
 
 struct Params {

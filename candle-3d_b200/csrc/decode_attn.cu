@@ -201,6 +201,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   asm volatile("griddepcontrol.launch_dependents;");
 
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_k) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_v) : "memory");
+  }
   if (threadIdx.x < WARPS * C::STAGES) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) *abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -694,14 +698,14 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   const bool few = rows <= 2 * sm_count();  // then their parts are many
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(unsigned(rows));
-  cfg.blockDim = dim3(few ? 512 : 128);
+  cfg.blockDim = dim3(few ? 512 : 256);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
-  return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 4>, p);
+  return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 8>, p);
 }
 
 int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {

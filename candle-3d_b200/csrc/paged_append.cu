@@ -7,9 +7,10 @@
 // for two fixed models (crate/runtime/attention_math.rs:104-146, crate/runtime/trellis2_blocks.rs:85-161,
 // :306-319) and keeps no cache.
 //
-// Bound by bytes: q, k and v are read once, q and the new cache rows written once.  Eight elements (16 bytes)
-// per thread, a head's D / 8 threads side by side in a warp, so that the norm's sum and the other half of a
-// pair are a shuffle away.  A block takes a few tokens and forms their angles once for all heads, in 64 bits:
+// Bound by bytes: q, k and v are read once, q and the new cache rows written once.  Eight elements per thread, a
+// head's D / 8 threads side by side in a warp: four pairs, both of whose elements a thread holds (two loads of 8 bytes
+// where they lie apart), so that only the norm's sum is shuffled.  (With 16 bytes in a row per thread and the other
+// half of a pair by shuffles the kernel was bound by issue: 36 us for 10992 tokens x 48 heads x 64.)  A block takes a few tokens and forms their angles once for all heads, in 64 bits:
 // at position 100,000 a product in 32 bits is off by up to 4e-3 radians, as much as bf16's rounding.  What is
 // left after whole turns are taken off is at most half a turn, and goes on in 32 bits.
 #include "common.cuh"
@@ -18,7 +19,7 @@ namespace l3d {
 namespace paged {
 
 constexpr int THREADS = 256;
-constexpr int MAX_TOKENS = 8;   // of one block
+constexpr int MAX_TOKENS = 32;  // of one block
 constexpr int TPU = 4;          // tokens of a thread's unit
 
 struct Rows {                   // a [T, H, D] view
@@ -49,25 +50,40 @@ __device__ __forceinline__ int64_t index_at(const void* p, int is64, int64_t i) 
   return is64 ? static_cast<const int64_t*>(p)[i] : int64_t(static_cast<const int32_t*>(p)[i]);
 }
 
-// Request of token t, -1 for a token of none (before the first or behind the last).
-__device__ __forceinline__ int request_of(const Params& p, int t, int64_t* first) {
-  if (!p.offsets) {
-    const int per = p.T / p.B, b = t / per;
-    *first = int64_t(b) * per;
-    return b;
-  }
-  int lo = -1, hi = p.B;  // the last b with offsets[b] <= t
+// The last place of the offsets with a value up to t, -1: none.  A warp looks, 32 places at a time.
+__device__ __forceinline__ int request_of(const Params& p, int t, int lane) {
+  if (!p.offsets) return 0;
+  int lo = -1, hi = p.B + 1;  // offsets[lo] <= t < offsets[hi], as far as there are such
   while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (index_at(p.offsets, p.offsets64, mid) <= t) lo = mid;
-    else hi = mid;
+    const int step = (hi - lo - 1 + 31) / 32, at = lo + (lane + 1) * step;
+    const bool below = at < hi && index_at(p.offsets, p.offsets64, at) <= t;
+    const int n = __popc(__ballot_sync(0xffffffffu, below));
+    hi = min(hi, lo + (n + 1) * step);
+    lo += n * step;
   }
-  if (lo < 0 || t >= index_at(p.offsets, p.offsets64, lo + 1)) return -1;
-  *first = index_at(p.offsets, p.offsets64, lo);
   return lo;
 }
 
-template <typename T, int D>
+// Four values of a 16-bit type as two pairs of f32, and back.
+__device__ __forceinline__ void unpack4(uint2 u, float2 (&f)[2], __nv_bfloat16) {
+  f[0] = make_float2(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u));
+  f[1] = make_float2(__uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+__device__ __forceinline__ void unpack4(uint2 u, float2 (&f)[2], __half) {
+  f[0] = __half22float2(*reinterpret_cast<const __half2*>(&u.x));
+  f[1] = __half22float2(*reinterpret_cast<const __half2*>(&u.y));
+}
+__device__ __forceinline__ uint2 pack4(const float2 (&f)[2], __nv_bfloat16) {
+  const __nv_bfloat162 a = __float22bfloat162_rn(f[0]), b = __float22bfloat162_rn(f[1]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+__device__ __forceinline__ uint2 pack4(const float2 (&f)[2], __half) {
+  const __half2 a = __float22half2_rn(f[0]), b = __float22half2_rn(f[1]);
+  return make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// APART: the elements of a pair do not lie side by side.
+template <typename T, int D, bool APART>
 __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   constexpr int LANES = D / 8;                  // threads of a row
   constexpr int SLOTS = THREADS / LANES;        // rows of a block at a time
@@ -75,13 +91,42 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   __shared__ int64_t s_at[MAX_TOKENS];          // place in the request's sequence
   __shared__ int64_t s_k[MAX_TOKENS], s_v[MAX_TOKENS];  // where its key and value go; -1: no room
   __shared__ int s_out[MAX_TOKENS];             // -1: a token of no request
+  __shared__ int s_ends[2];
   const int t0 = blockIdx.x * p.tokens, n = min(p.tokens, p.T - t0);
+  const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, groups = (n + TPU - 1) / TPU;
+  // This thread's elements: lo .. lo + 3 and hi .. hi + 3, the pairs pair0 .. pair0 + 3; or neighbours, the pairs
+  // pair0 .. of lo .. lo + 7.
+  const int pair0 = 4 * lane;
+  int lo = 8 * lane, hi = lo + 4;
+  if (APART && pair0 < p.pairs) {
+    const int block = pair0 / p.half;
+    lo = block * 2 * p.half + (pair0 - block * p.half);
+    hi = lo + p.half;
+  }
+  // The tokens' places: the requests of the first and of the last by a warp each, of the others between them.
+  if (threadIdx.x < 64) {
+    const int end = threadIdx.x / 32, b = request_of(p, end ? t0 + n - 1 : t0, threadIdx.x % 32);
+    if (threadIdx.x % 32 == 0) s_ends[end] = b;
+  }
+  __syncthreads();
   if (threadIdx.x < n) {
+    const int t = t0 + threadIdx.x;
+    int b = s_ends[0], hi = s_ends[1] + 1;
     int64_t first = 0, place = 0;
     int page = -1;
-    const int b = request_of(p, t0 + threadIdx.x, &first);
+    if (p.offsets) {
+      while (hi - b > 1) {
+        const int mid = (b + hi) >> 1;
+        if (index_at(p.offsets, p.offsets64, mid) <= t) b = mid;
+        else hi = mid;
+      }
+      if (b >= p.B) b = -1;
+    } else {
+      b = t / (p.T / p.B);
+    }
     if (b >= 0) {
-      place = index_at(p.held, p.held64, b) + (t0 + threadIdx.x - first);
+      first = p.offsets ? index_at(p.offsets, p.offsets64, b) : int64_t(b) * (p.T / p.B);
+      place = index_at(p.held, p.held64, b) + (t - first);
       if (place >= 0 && place < int64_t(p.width) * p.size) page = p.table[b * p.table_stride + place / p.size];
     }
     const bool room = page >= 0 && page < p.pages;
@@ -103,90 +148,93 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   }
   __syncthreads();
 
-  // A thread's unit is one head of TPU tokens of the block, whose loads it issues together; the head's address
-  // and weights are worked out once for them.  (One token at a time took 320 instructions per 16 bytes, and issue
-  // bound the kernel: 61 us for 10992 tokens x 48 heads x 64.)
-  const int lane = threadIdx.x % LANES, e0 = lane * 8, slot = threadIdx.x / LANES;
-  const int groups = (n + TPU - 1) / TPU;
-  // Where this thread's elements stand in their pairs.
-  const int block = p.half ? e0 / (2 * p.half) : 0, off = p.half ? e0 - block * 2 * p.half : 0;
-  const bool second = p.half && off >= p.half;
-  const int pair0 = p.half ? block * p.half + off - (second ? p.half : 0) : e0 / 2;
-  const int other = (second ? lane - p.half / 8 : lane + p.half / 8) & (LANES - 1);
-  const bool rotated = pair0 < p.pairs;
-
-  // ---- queries and keys (all threads of a warp take every turn: they meet in its shuffles)
-  const int units = (p.Hq + p.Hkv) * groups;
+  // ---- queries and keys.  A thread's unit is one head of TPU tokens of the block, whose loads it issues together; the
+  // head's address and weights are worked out once for them.  (All threads of a warp take every turn: they meet in
+  // its shuffles.)
+  const int heads = p.Hq + p.Hkv, units = heads * groups;
   for (int u0 = 0; u0 < units; u0 += SLOTS) {
-    const int u = min(u0 + slot, units - 1), grp = u / (p.Hq + p.Hkv), hh = u - grp * (p.Hq + p.Hkv);
-    const bool mine = u0 + slot < units, isq = hh < p.Hq;
-    const int h = isq ? hh : hh - p.Hq, ta = grp * TPU, tn = mine ? min(n - ta, TPU) : 0;
-    const T* src = reinterpret_cast<const T*>(isq ? p.q.p : p.k.p) + (t0 + ta) * (isq ? p.q.st : p.k.st) +
-                   h * (isq ? p.q.sh : p.k.sh) + e0;
+    const int u = min(u0 + slot, units - 1), grp = u / heads, hh = u - grp * heads;
+    const bool isq = hh < p.Hq;
+    const int h = isq ? hh : hh - p.Hq, ta = grp * TPU, tn = u0 + slot < units ? min(n - ta, TPU) : 0;
     const int64_t step = isq ? p.q.st : p.k.st;
-    uint4 raw[TPU];
-#pragma unroll
-    for (int i = 0; i < TPU; ++i)
-      raw[i] = i < tn ? *reinterpret_cast<const uint4*>(src + i * step) : make_uint4(0, 0, 0, 0);
-    float w[8];
-    if (p.qw.ptr) load_chan<8>(isq ? p.qw : p.kw, h, e0, w);
+    const T* src = reinterpret_cast<const T*>(isq ? p.q.p : p.k.p) + (t0 + ta) * step + h * (isq ? p.q.sh : p.k.sh);
+    uint2 raw[TPU][2];
 #pragma unroll
     for (int i = 0; i < TPU; ++i) {
-      const int t = min(ta + i, n - 1);
-      float x[8];
-      unpack(raw[i], x, T());
-      if (p.qw.ptr) {
-        float sum = 0.f;
+      if constexpr (APART) {
+        raw[i][0] = i < tn ? *reinterpret_cast<const uint2*>(src + i * step + lo) : make_uint2(0, 0);
+        raw[i][1] = i < tn ? *reinterpret_cast<const uint2*>(src + i * step + hi) : make_uint2(0, 0);
+      } else {
+        const uint4 v = i < tn ? *reinterpret_cast<const uint4*>(src + i * step + lo) : make_uint4(0, 0, 0, 0);
+        raw[i][0] = make_uint2(v.x, v.y);
+        raw[i][1] = make_uint2(v.z, v.w);
+      }
+    }
+    float2 w[2][2];
+    if (p.qw.ptr) {
+      load_chan<4>(isq ? p.qw : p.kw, h, lo, *reinterpret_cast<float(*)[4]>(w[0]));
+      load_chan<4>(isq ? p.qw : p.kw, h, hi, *reinterpret_cast<float(*)[4]>(w[1]));
+    }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sum = fmaf(x[e], x[e], sum);
+    for (int i = 0; i < TPU; ++i) {
+      if (i >= n) break;  // (as many tokens in the block: the same for all threads)
+      const int t = min(ta + i, n - 1);
+      float2 x[2][2];
+      unpack4(raw[i][0], x[0], T());
+      unpack4(raw[i][1], x[1], T());
+      if (p.qw.ptr) {
+        float2 sq = mul2(x[0][0], x[0][0]);
+        sq = fma2(x[0][1], x[0][1], sq);
+        sq = fma2(x[1][0], x[1][0], sq);
+        sq = fma2(x[1][1], x[1][1], sq);
+        float sum = sq.x + sq.y;
 #pragma unroll
         for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        const float inv = rsqrtf(sum * (1.f / D) + p.eps);  // to 2 ulp; what it goes into is rounded to 16 bits
+        const float2 inv = f2(rsqrtf(sum * (1.f / D) + p.eps));  // to 2 ulp; what it goes into is rounded to 16 bits
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * inv * w[e];
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) x[a][e] = mul2(x[a][e], mul2(inv, w[a][e]));
       }
-      if (p.half == 0) {
-        if (rotated) {
+      if (pair0 < p.pairs) {
+        const float4 c4 = *reinterpret_cast<const float4*>(&s_cos[t][pair0]), s4 = *reinterpret_cast<const float4*>(&s_sin[t][pair0]);
+        if constexpr (APART) {
+          const float2 c[2] = {make_float2(c4.x, c4.y), make_float2(c4.z, c4.w)};
+          const float2 s[2] = {make_float2(s4.x, s4.y), make_float2(s4.z, s4.w)};
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 a = x[0][e], b = x[1][e], bs = mul2(b, s[e]);
+            x[0][e] = fma2(a, c[e], make_float2(-bs.x, -bs.y));
+            x[1][e] = fma2(b, c[e], mul2(a, s[e]));
+          }
+        } else {
+          const float c[4] = {c4.x, c4.y, c4.z, c4.w}, s[4] = {s4.x, s4.y, s4.z, s4.w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if (pair0 + e >= p.pairs) continue;
-            const float c = s_cos[t][pair0 + e], s = s_sin[t][pair0 + e], a = x[2 * e], b = x[2 * e + 1];
-            x[2 * e] = a * c - b * s;
-            x[2 * e + 1] = b * c + a * s;
+            if (pair0 + e >= p.pairs) continue;  // (of a place behind the last pair, which may hold anything)
+            float2& z = x[e >> 1][e & 1];
+            z = make_float2(z.x * c[e] - z.y * s[e], z.y * c[e] + z.x * s[e]);
           }
-        }
-      } else {
-        float z[8];  // the other elements of the pairs
-#pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = __shfl_sync(0xffffffffu, x[e], other, LANES);
-        if (rotated) {
-          float c[8], s[8];
-#pragma unroll
-          for (int e = 0; e < 8; e += 4) {
-            *reinterpret_cast<float4*>(c + e) = *reinterpret_cast<const float4*>(&s_cos[t][pair0 + e]);
-            *reinterpret_cast<float4*>(s + e) = *reinterpret_cast<const float4*>(&s_sin[t][pair0 + e]);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = fmaf(x[e], c[e], second ? z[e] * s[e] : -(z[e] * s[e]));
         }
       }
-      if (i < tn && s_out[t] >= 0) {  // (the shuffles are behind us)
-        if (isq) {
-          if (s_k[t] < 0) {  // no room: nothing is stored, and the request's attention is not finite
-#pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] = __int_as_float(0x7fffffff);
-          }
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.qo.p) + (t0 + t) * p.qo.st + h * p.qo.sh + e0) = pack(x, T());
-        } else if (s_k[t] >= 0) {
-          *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.kp) + s_k[t] + h * p.ks[2] + e0) = pack(x, T());
-        }
+      if (i >= tn || s_out[t] < 0 || (!isq && s_k[t] < 0)) continue;  // (the shuffles are behind us)
+      uint2 y[2] = {pack4(x[0], T()), pack4(x[1], T())};
+      if (isq && s_k[t] < 0)  // no room: nothing is stored, and the request's attention is not finite
+        y[0] = y[1] = make_uint2(0x7fff7fffu, 0x7fff7fffu);
+      T* dst = isq ? reinterpret_cast<T*>(p.qo.p) + (t0 + t) * p.qo.st + h * p.qo.sh
+                   : reinterpret_cast<T*>(p.kp) + s_k[t] + h * p.ks[2];
+      if constexpr (APART) {
+        *reinterpret_cast<uint2*>(dst + lo) = y[0];
+        *reinterpret_cast<uint2*>(dst + hi) = y[1];
+      } else {
+        *reinterpret_cast<uint4*>(dst + lo) = make_uint4(y[0].x, y[0].y, y[1].x, y[1].y);
       }
     }
   }
   // ---- values
   for (int u = slot; u < p.Hkv * groups; u += SLOTS) {
     const int grp = u / p.Hkv, h = u - grp * p.Hkv, ta = grp * TPU, tn = min(n - ta, TPU);
-    const T* src = reinterpret_cast<const T*>(p.v.p) + (t0 + ta) * p.v.st + h * p.v.sh + e0;
+    const T* src = reinterpret_cast<const T*>(p.v.p) + (t0 + ta) * p.v.st + h * p.v.sh + 8 * lane;
     uint4 raw[TPU];
 #pragma unroll
     for (int i = 0; i < TPU; ++i)
@@ -194,7 +242,18 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
 #pragma unroll
     for (int i = 0; i < TPU; ++i)
       if (i < tn && s_k[ta + i] >= 0)
-        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.vp) + s_v[ta + i] + h * p.vs[2] + e0) = raw[i];
+        *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.vp) + s_v[ta + i] + h * p.vs[2] + 8 * lane) = raw[i];
+  }
+}
+
+template <typename T>
+static void launch(int D, const Params& p, unsigned grid, cudaStream_t s) {
+  if (D == 64) {
+    if (p.half) append_kernel<T, 64, true><<<grid, THREADS, 0, s>>>(p);
+    else append_kernel<T, 64, false><<<grid, THREADS, 0, s>>>(p);
+  } else {
+    if (p.half) append_kernel<T, 128, true><<<grid, THREADS, 0, s>>>(p);
+    else append_kernel<T, 128, false><<<grid, THREADS, 0, s>>>(p);
   }
 }
 
@@ -325,17 +384,13 @@ extern "C" int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const 
   p.axis = axes ? reinterpret_cast<const int32_t*>(elem_ptr(axes)) : nullptr;
   p.pairs = int(pairs);
   p.half = freqs ? half : 0;
-  // One token per block as long as the device is not full, so that a few tokens spread over it.
-  const int64_t per = T / (8 * int64_t(sm_count()));
-  p.tokens = per < 1 ? 1 : per > MAX_TOKENS ? MAX_TOKENS : int(per);
+  // One token per block as long as the device (four blocks an SM) is not full, so that a few tokens spread over it;
+  // then as many as fill it once, for a block's tokens are looked up together.
+  const int64_t per = (T + 4 * int64_t(sm_count()) - 1) / (4 * int64_t(sm_count()));
+  p.tokens = per > MAX_TOKENS ? MAX_TOKENS : int(per);
   const unsigned grid = unsigned((T + p.tokens - 1) / p.tokens);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (q->dtype == L3D_BF16) {
-    if (D == 64) append_kernel<__nv_bfloat16, 64><<<grid, THREADS, 0, s>>>(p);
-    else append_kernel<__nv_bfloat16, 128><<<grid, THREADS, 0, s>>>(p);
-  } else {
-    if (D == 64) append_kernel<__half, 64><<<grid, THREADS, 0, s>>>(p);
-    else append_kernel<__half, 128><<<grid, THREADS, 0, s>>>(p);
-  }
+  if (q->dtype == L3D_BF16) launch<__nv_bfloat16>(int(D), p, grid, s);
+  else launch<__half>(int(D), p, grid, s);
   return check_launch(op);
 }
