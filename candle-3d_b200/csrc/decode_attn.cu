@@ -155,7 +155,8 @@ __device__ __forceinline__ bool not_finite(uint32_t at) {
 struct Cursor {
   int b, hr, t, tiles;
   __device__ __forceinline__ void seek(const int* starts, int B, int heads, int64_t x) {
-    const int64_t y = x / heads;
+    const bool small = x >> 31 == 0;  // (a 64-bit division takes some 150 clocks more)
+    const int64_t y = small ? int64_t(uint32_t(x) / uint32_t(heads)) : x / heads;
     int lo = 0, hi = B;  // the last b with starts[b] <= y
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -165,7 +166,7 @@ struct Cursor {
     b = lo;
     tiles = starts[b + 1] - starts[b];
     const int64_t rem = x - int64_t(starts[b]) * heads;
-    hr = int(rem / tiles);
+    hr = small ? int(uint32_t(rem) / uint32_t(tiles)) : int(rem / tiles);
     t = int(rem - int64_t(hr) * tiles);
   }
   // To the next tile (not past the line's last one); whether its head or row tile is another one.
@@ -208,6 +209,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   if (threadIdx.x < WARPS * C::STAGES) mbar_init(&bars[threadIdx.x], 1);
   if (threadIdx.x == 0) *abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before: nothing global is touched earlier
   // ---- key tiles before each sequence: a sum over the batch, a stretch of it per thread
   {
     const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(int(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
@@ -690,21 +692,24 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   constexpr int fixed = WARPS * Cfg<D>::RING + Cfg<D>::BARS;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), fixed + (MAX_BATCH + 1) * 4);
   if (e != cudaSuccess) return e;
-  k<<<unsigned(blocks), WARPS * 32, fixed + (p.B + 1) * 4, s>>>(maps[0], maps[1], p);
-  e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  // The combination may be scheduled while the parts are formed; it waits for them.
-  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G;
-  const bool few = rows <= 2 * sm_count();  // then their parts are many
+  // Both may be scheduled while the kernel before them runs, and wait for it.
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(unsigned(rows));
-  cfg.blockDim = dim3(few ? 512 : 256);
-  cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &at;
   cfg.numAttrs = 1;
+  cfg.stream = s;
+  cfg.gridDim = dim3(unsigned(blocks));
+  cfg.blockDim = dim3(WARPS * 32);
+  cfg.dynamicSmemBytes = fixed + (p.B + 1) * 4;
+  e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], p);
+  if (e != cudaSuccess) return e;
+  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G;
+  const bool few = rows <= 2 * sm_count();  // then their parts are many
+  cfg.gridDim = dim3(unsigned(rows));
+  cfg.blockDim = dim3(few ? 512 : 256);
+  cfg.dynamicSmemBytes = 0;
   return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 8>, p);
 }
 

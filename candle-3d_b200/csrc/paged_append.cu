@@ -92,6 +92,8 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   __shared__ int64_t s_k[MAX_TOKENS], s_v[MAX_TOKENS];  // where its key and value go; -1: no room
   __shared__ int s_out[MAX_TOKENS];             // -1: a token of no request
   __shared__ int s_ends[2];
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before: nothing global is touched earlier
   const int t0 = blockIdx.x * p.tokens, n = min(p.tokens, p.T - t0);
   const int lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, groups = (n + TPU - 1) / TPU;
   // This thread's elements: lo .. lo + 3 and hi .. hi + 3, the pairs pair0 .. pair0 + 3; or neighbours, the pairs
@@ -246,15 +248,19 @@ __global__ void __launch_bounds__(THREADS) append_kernel(const Params p) {
   }
 }
 
-template <typename T>
-static void launch(int D, const Params& p, unsigned grid, cudaStream_t s) {
-  if (D == 64) {
-    if (p.half) append_kernel<T, 64, true><<<grid, THREADS, 0, s>>>(p);
-    else append_kernel<T, 64, false><<<grid, THREADS, 0, s>>>(p);
-  } else {
-    if (p.half) append_kernel<T, 128, true><<<grid, THREADS, 0, s>>>(p);
-    else append_kernel<T, 128, false><<<grid, THREADS, 0, s>>>(p);
-  }
+template <typename T, int D>
+static cudaError_t launch(const Params& p, unsigned grid, cudaStream_t s) {
+  // The kernel may be scheduled while the one before it runs, and waits for it.
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(grid);
+  cfg.blockDim = dim3(THREADS);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, p.half ? append_kernel<T, D, true> : append_kernel<T, D, false>, p);
 }
 
 }  // namespace paged
@@ -390,7 +396,8 @@ extern "C" int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const 
   p.tokens = per > MAX_TOKENS ? MAX_TOKENS : int(per);
   const unsigned grid = unsigned((T + p.tokens - 1) / p.tokens);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  if (q->dtype == L3D_BF16) launch<__nv_bfloat16>(int(D), p, grid, s);
-  else launch<__half>(int(D), p, grid, s);
-  return check_launch(op);
+  cudaError_t e;
+  if (q->dtype == L3D_BF16) e = D == 64 ? launch<__nv_bfloat16, 64>(p, grid, s) : launch<__nv_bfloat16, 128>(p, grid, s);
+  else e = D == 64 ? launch<__half, 64>(p, grid, s) : launch<__half, 128>(p, grid, s);
+  return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
 }
