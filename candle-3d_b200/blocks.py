@@ -295,9 +295,15 @@ class TripoSgDit:
         o = split.return_heads_uneven(a, counts)
         return F.linear(o.view(1, L, C), p["o1_w"], p["o1_b"])
 
-    def _cross_attn(self, p, y, cond):
+    def _cross_attn(self, p, y, cond, cond_offsets=None):
         B, L, C = y.shape
         H, D = self.H, self.D
+        if cond_offsets is not None:  # encoder tokens of all objects packed, of different numbers
+            q = ops.rms_norm_heads(F.linear(y, p["q2_w"]).view(B * L, H, D), p["nq2"], 1e-6)
+            kv = F.linear(cond, p["kv2_w"]).view(-1, H, 2 * D)
+            k = ops.rms_norm_heads(kv[..., :D], p["nk2"], 1e-6)
+            a = ops.cross_attention(q, k, kv[..., D:], cond_offsets)
+            return F.linear(a.view(B, L, C), p["o2_w"], p["o2_b"])
         q = ops.rms_norm_heads(F.linear(y, p["q2_w"]).view(B, L, H, D).transpose(1, 2), p["nq2"], 1e-6)
         kv = F.linear(cond, p["kv2_w"]).view(B, cond.shape[1], H, 2 * D)
         k = ops.rms_norm_heads(kv[..., :D].transpose(1, 2), p["nk2"], 1e-6)
@@ -313,8 +319,10 @@ class TripoSgDit:
         h = ops.linear_small(h, self.t2[0], self.t2[1])
         return h.view(1, 1, self.C).expand(B, 1, self.C)
 
-    def forward(self, latents, t, cond, split=None, counts=None, prefix=True):
-        """latents [B, L, 64], cond [B, S, 1024] -> [B, L, 64].
+    def forward(self, latents, t, cond, split=None, counts=None, prefix=True, cond_offsets=None):
+        """latents [B, L, 64], cond [B, S, 1024] -> [B, L, 64]; with cond_offsets [B + 1]
+        (int32 on the device) the encoder tokens are packed, [T, 1024], and object b has
+        the rows cond_offsets[b] .. cond_offsets[b + 1] - 1 of them, as many as its images gave.
 
         With `split` (shard.SceneSplit over W ranks, 16 heads divisible by W)
         and `counts` (tokens per rank of the 1 + L token sequence, the
@@ -326,6 +334,8 @@ class TripoSgDit:
         attention reads all of cond on every rank)."""
         B, L, _ = latents.shape
         C = self.C
+        if cond_offsets is not None and (cond.dim() != 2 or cond_offsets.shape != (B + 1,)):
+            raise ValueError(f"packed encoder tokens are [T, C] with {B + 1} offsets")
         if split is not None and split.world > 1:
             if (B != 1 or self.H % split.world or counts is None
                     or int(counts[split.rank]) != L + int(prefix)):
@@ -350,7 +360,7 @@ class TripoSgDit:
                 y = ops.layer_norm(x, p["n1w"], p["n1b"], 1e-5)
             a = self._self_attn(p, y) if split is None else self._self_attn_split(p, y, split, counts)
             x, y = ops.residual_layer_norm_modulate(x, a, weight=p["n2w"], bias=p["n2b"], eps=1e-5)
-            x, y = ops.residual_layer_norm_modulate(x, self._cross_attn(p, y, cond),
+            x, y = ops.residual_layer_norm_modulate(x, self._cross_attn(p, y, cond, cond_offsets),
                                                     weight=p["n3w"], bias=p["n3b"], eps=1e-5)
             ff = F.linear(ops.gelu_erf(F.linear(y, p["ff1_w"], p["ff1_b"])), p["ff2_w"], p["ff2_b"])
             nxt = self.blocks[i + 1] if i + 1 < self.layers else None
@@ -528,8 +538,14 @@ class Trellis2Slat:
         o = split.return_heads_uneven(a, counts, groups)
         return p["to_out"](o.view(1, L, C))
 
-    def forward(self, feats, coords, t_model, cond, split=None, counts=None, head_groups=None):
+    def forward(self, feats, coords, t_model, cond, split=None, counts=None, head_groups=None,
+                scene_offsets=None, cond_offsets=None):
         """feats [N, in_ch], coords [N, 3] int32, cond [1, Lc, cond_dim] -> [N, in_ch].
+
+        With `scene_offsets` and `cond_offsets` ([B + 1] int32 on the device) the voxel rows of B
+        scenes lie packed one behind the other, and so do their encoder tokens (cond
+        [T, cond_dim]): scene b is rows scene_offsets[b] .. scene_offsets[b + 1] - 1, which
+        attend to each other and to the tokens cond_offsets[b] .. cond_offsets[b + 1] - 1.
 
         With `split` (shard.SceneSplit over W ranks) and `counts` (rows per
         rank), feats / coords are this rank's consecutive rows of the sorted
@@ -539,6 +555,10 @@ class Trellis2Slat:
         shared by W / head_groups ranks, which split its queries)."""
         N = feats.shape[0]
         C, H, D = self.C, self.H, self.D
+        packed = scene_offsets is not None
+        if packed != (cond_offsets is not None) or (packed and (cond.dim() != 2 or split is not None)):
+            raise ValueError("packed scenes need scene_offsets, cond_offsets and encoder tokens "
+                             "[T, C], and cannot be split")
         if split is not None and split.world > 1:
             G = math.gcd(H, split.world) if head_groups is None else int(head_groups)
             if (H % G or split.world % G or counts is None
@@ -550,7 +570,7 @@ class Trellis2Slat:
         x = F.linear(feats, *self.input_layer).view(1, N, C).contiguous()
         mods = self.block_mods(self.t_emb(t_model))
         y = ops.layer_norm_modulate(x, mods[0][0], mods[0][1], eps=1e-6)
-        Lc = cond.shape[1]
+        Lc = cond.shape[-2]
         for i, p in enumerate(self.blocks):
             sh_msa, sc_msa, g_msa, sh_mlp, sc_mlp, g_mlp = mods[i]
             if split is not None:
@@ -559,15 +579,23 @@ class Trellis2Slat:
                 qkv = p["to_qkv"](y).view(1, N, 3, H, D)
                 q = ops.qk_l2norm_rope3d(qkv[:, :, 0], p["qg"], coords)
                 k = ops.qk_l2norm_rope3d(qkv[:, :, 1], p["kg"], coords)
-                a = _attend(q.transpose(1, 2), k.transpose(1, 2), qkv[:, :, 2].transpose(1, 2))
-                o = p["to_out"](a.transpose(1, 2).reshape(1, N, C))
+                if packed:
+                    a = ops.cross_attention(q[0], k[0], qkv[0, :, 2], scene_offsets, scene_offsets)
+                    o = p["to_out"](a.view(1, N, C))
+                else:
+                    a = _attend(q.transpose(1, 2), k.transpose(1, 2), qkv[:, :, 2].transpose(1, 2))
+                    o = p["to_out"](a.transpose(1, 2).reshape(1, N, C))
             x, y = ops.residual_layer_norm_modulate(x, o, gate=g_msa, weight=p["n2w"], bias=p["n2b"],
                                                     eps=1e-6, inplace=True)
             cq = ops.qk_l2norm_rope3d(p["c_q"](y).view(1, N, H, D), p["cqg"], None)
             kv = p["c_kv"](cond).view(1, Lc, 2, H, D)
             ck = ops.qk_l2norm_rope3d(kv[:, :, 0], p["ckg"], None)
-            ca = _attend(cq.transpose(1, 2), ck.transpose(1, 2), kv[:, :, 1].transpose(1, 2))
-            co = p["c_out"](ca.transpose(1, 2).reshape(1, N, C))
+            if packed:
+                ca = ops.cross_attention(cq[0], ck[0], kv[0, :, 1], cond_offsets, scene_offsets)
+                co = p["c_out"](ca.view(1, N, C))
+            else:
+                ca = _attend(cq.transpose(1, 2), ck.transpose(1, 2), kv[:, :, 1].transpose(1, 2))
+                co = p["c_out"](ca.transpose(1, 2).reshape(1, N, C))
             x, y = ops.residual_layer_norm_modulate(x, co, shift=sh_mlp, scale=sc_mlp, eps=1e-6,
                                                     inplace=True)
             h = p["mlp2"](p["mlp0"](y, act="gelu"))  # tanh-GELU in mlp.0's epilogue
@@ -718,3 +746,127 @@ def shared_context_reference(m: SharedContextBlocks, x, tokens, ids):
         h = h + f(p["g2"]) * rms(z, p["post2"])
         y = rms(h, p["pre"])
     return y[:, P:]
+
+
+class PagedRequestBlocks(SharedContextBlocks):
+    """The blocks of SharedContextBlocks for requests that share no context: each has an
+    encoder's states of its own (an image's tokens, as many as it gave), its tokens
+    lie at places on several axes (time, height, width), and its keys and values in
+    pages of one cache:
+
+      y = LN(x); qkv = Wqkv y + adapter; q, k = RMSNorm per head, rotated by the token's place
+      a = softmax(q [cached k, own k]) [cached v, own v], causal in the own keys
+      x, y = x + g1 * RMS(Wo a + adapter) * w, RMS(x) * w'
+      c = softmax(RMSNorm(Wq y) [state k]) [state v], over the request's own states
+      x, y = x + g3 * RMS(Wc c) * w, RMS(x) * w'
+      x, y = x + g2 * RMS(fc2 gelu(fc1 y)) * w, the next block's RMS(x) * w'
+
+    One launch puts a step's keys and values into the cache, normed and rotated."""
+
+    def __init__(self, depth=2, dim=512, heads=8, kv_heads=2, mlp=2048, ranks=(16, 8, 32), state_dim=1024,
+                 sections=(8, 12, 12), theta=10000.0, seed=0, device="cuda"):
+        super().__init__(depth, dim, heads, kv_heads, mlp, ranks, seed, device)
+        g = torch.Generator().manual_seed(seed + 1)
+        self.rope = ops.RotaryAxes(self.D, sections, theta, device=device)
+
+        def vec(n, mean=1.0):
+            return (mean + 0.1 * torch.randn(n, generator=g)).to(device, self.dtype)
+
+        for p in self.blocks:
+            p["cq"] = _w(g, (dim, dim), dim ** -0.5, device)
+            p["ckv"] = _w(g, (2 * kv_heads * self.D, state_dim), state_dim ** -0.5, device)
+            p["cout"] = _w(g, (dim, dim), dim ** -0.5, device)
+            p["cqn"], p["ckn"] = vec(self.D), vec(self.D)
+            p["post3"], p["g3"], p["pre3"] = vec(dim), vec(dim, 0.5), vec(dim)
+
+    def encode_states(self, states):
+        """states [T, state_dim], the requests' one behind the other -> per block their keys
+        and values [T, Hkv, D]."""
+        kv = []
+        for p in self.blocks:
+            both = F.linear(states, p["ckv"]).view(-1, 2 * self.Hkv, self.D)
+            kv.append((ops.rms_norm_heads(both[:, :self.Hkv], p["ckn"]), both[:, self.Hkv:]))
+        return kv
+
+    def new_pages(self, pages, size=16):
+        """A cache of `pages` pages of `size` tokens: (k, v) per block."""
+        def room():
+            return torch.zeros((pages, size, self.Hkv, self.D), dtype=self.dtype, device=self.device)
+        return [(room(), room()) for _ in range(self.depth)]
+
+    def forward(self, x, states, state_offsets, cache, table, held, ids, positions=None):
+        """x [B, N, C]: the next N tokens of each request, request b holding held[b] (int32)
+        already in the pages table[b] (int32, -1 behind the last); states and state_offsets
+        [B + 1]: encode_states and whose rows they are; positions [B, N, axes] (None: the
+        token's place in its request, for every axis); ids [B]: its adapter, or one outside
+        the range for none.  Returns the final states [B, N, C]; the cache takes the new keys
+        and values.  A request whose tokens have no place in its pages comes out NaN, and no
+        other differs."""
+        B, N, C = x.shape
+        H, Hkv, D = self.H, self.Hkv, self.D
+        total = held + N
+        if positions is not None:
+            positions = positions.reshape(B * N, -1)
+        y = ops.layer_norm(x, *self.n0, eps=1e-6)
+        for p, (pk, pv), (sk, sv) in zip(self.blocks, cache, states):
+            qkv = ops.lora_linear(y, p["qkv"][0], p["qkv"][1], ids).view(B * N, H + 2 * Hkv, D)
+            q = ops.paged_append(qkv[:, :H], qkv[:, H:H + Hkv], qkv[:, H + Hkv:], pk, pv, table, held,
+                                 rope=self.rope, positions=positions, q_weight=p["qn"], k_weight=p["kn"])
+            a = ops.paged_attention(q.view(B, N, H, D), pk, pv, table, total)
+            o = ops.lora_linear(a.view(B, N, C), p["out"][0], p["out"][1], ids)
+            x, y = ops.sandwich_residual_norm(x, o, p["post1"], gate=p["g1"], weight=p["pre3"])
+            q = ops.rms_norm_heads(F.linear(y, p["cq"]).view(B * N, H, D), p["cqn"])
+            c = ops.cross_attention(q, sk, sv, state_offsets)
+            x, y = ops.sandwich_residual_norm(x, F.linear(c.view(B, N, C), p["cout"]), p["post3"], gate=p["g3"],
+                                              weight=p["pre2"], inplace=True)
+            h = ops.lora_linear(y, p["fc1"][0], p["fc1"][1], ids, act="gelu")
+            h = ops.lora_linear(h, p["fc2"][0], p["fc2"][1], ids)
+            x, y = ops.sandwich_residual_norm(x, h, p["post2"], gate=p["g2"], weight=p["pre"], inplace=True)
+        return y
+
+
+def paged_request_reference(m: PagedRequestBlocks, x, states, positions, ids):
+    """PagedRequestBlocks over one whole request x [L, C] at once, in torch f64; states
+    [S, state_dim], positions [L, axes], ids its adapter."""
+    f = lambda a: a.double()  # noqa: E731
+    L, C = x.shape
+    H, Hkv, D, G = m.H, m.Hkv, m.D, m.H // m.Hkv
+
+    def rms(v, w):
+        return v / torch.sqrt(v.pow(2).mean(-1, keepdim=True) + 1e-6) * f(w)
+
+    def lin(v, wa):
+        w, ad = wa
+        y = F.linear(v, f(w))
+        if 0 <= ids < ad.count:
+            y = y + f(ad.scales[ids]) * (v @ f(ad.a[ids]).T @ f(ad.b[ids]).T)
+        return y
+
+    ang = f(positions)[:, m.rope.axis.long()] * m.rope.freqs.double().sum(1)  # [L, D / 2]: pairs i and i + D / 2
+    turn = torch.polar(torch.ones_like(ang), ang)[:, None]
+
+    def turned(v):
+        z = torch.complex(v[..., :D // 2].contiguous(), v[..., D // 2:].contiguous()) * turn
+        return torch.cat([z.real, z.imag], -1)
+
+    def attend(q, k, v, mask=None):
+        s = torch.einsum("lhd,shd->hls", q, k.repeat_interleave(G, 1)) * D ** -0.5
+        if mask is not None:
+            s = s.masked_fill(~mask, float("-inf"))
+        return torch.einsum("hls,shd->lhd", s.softmax(-1), v.repeat_interleave(G, 1)).reshape(L, C)
+
+    h = f(x)
+    y = F.layer_norm(h, (C,), f(m.n0[0]), f(m.n0[1]), 1e-6)
+    past = torch.ones(L, L, dtype=torch.bool, device=x.device).tril()
+    for p in m.blocks:
+        qkv = lin(y, p["qkv"]).view(L, H + 2 * Hkv, D)
+        a = attend(turned(rms(qkv[:, :H], p["qn"])), turned(rms(qkv[:, H:H + Hkv], p["kn"])), qkv[:, H + Hkv:], past)
+        h = h + f(p["g1"]) * rms(lin(a, p["out"]), p["post1"])
+        y = rms(h, p["pre3"])
+        kv = F.linear(f(states), f(p["ckv"])).view(-1, 2 * Hkv, D)
+        c = attend(rms(F.linear(y, f(p["cq"])).view(L, H, D), p["cqn"]), rms(kv[:, :Hkv], p["ckn"]), kv[:, Hkv:])
+        h = h + f(p["g3"]) * rms(F.linear(c, f(p["cout"])), p["post3"])
+        z = lin(F.gelu(lin(rms(h, p["pre2"]), p["fc1"]), approximate="tanh"), p["fc2"])
+        h = h + f(p["g2"]) * rms(z, p["post2"])
+        y = rms(h, p["pre"])
+    return y
