@@ -72,18 +72,19 @@ def ref(d):
 # From _l3dpack.so (host/pack.cpp, built with the library).  It is bound to one torch:
 # where it cannot be loaded, the calls that need it fail, and nothing else.
 try:
-    from ._l3dpack import empty, packed, packs, packs_here, workspace
+    from . import _l3dpack as native
+    from ._l3dpack import empty, packed, packs, workspace
 except ImportError as _e:
     _why = str(_e)
 
     def packed(*_):
         """packed: as desc, as the descriptor's bytes (None -> NULL), for signatures with _D;
-        packs: packed of each argument, which must be on a CUDA device; packs_here: on
-        the current one."""
+        packs: packed of each argument, which must be on a CUDA device."""
         raise RuntimeError(f"_l3dpack.so cannot be loaded ({_why}): build it with "
                            "`python candle-3d_b200/build.py`")
 
-    empty = packs = packs_here = workspace = packed
+    empty = packs = workspace = packed
+    native = None
 
 
 _P = C.POINTER(L3dTensor)
@@ -207,6 +208,27 @@ def call(name: str, *args):
     if rc != 0:
         raise L3dError(rc, name, lib().l3d_last_error().decode())
     return rc
+
+
+_addresses = {}
+
+
+def address(name: str) -> int:
+    """Where an entry point lies, for the native calls (host/pack.cpp)."""
+    if name not in _addresses:
+        _addresses[name] = C.cast(getattr(lib(), name), C.c_void_p).value
+    return _addresses[name]
+
+
+def invoke(name: str, *args):
+    """An entry point through its native call, which describes the tensors and allocates
+    output and workspace (host/pack.cpp); the output, or L3dError."""
+    if native is None:
+        packed()  # says why
+    rc, out = getattr(native, name[4:])(address(name), *args)
+    if rc != 0:
+        raise L3dError(rc, name, lib().l3d_last_error().decode())
+    return out
 
 
 def declared_symbols() -> list[str]:

@@ -357,6 +357,11 @@ extern "C" int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const 
       if (t->dims[d] > 1 && t->strides[d] % 8)
         return fail(L3D_E_ALIGN, "%s: strides must be multiples of 16 bytes", op);
   }
+  const l3d_tensor* written[] = {q_out, k_pages, v_pages};
+  for (const l3d_tensor* t : written)
+    for (int d = 0; d < t->ndim - 1; ++d)
+      if (t->dims[d] > 1 && t->strides[d] == 0)
+        return fail(L3D_E_ALIGN, "%s: q_out and the pages must not be expanded (stride 0)", op);
   const l3d_tensor* lists[] = {table, held, offsets, positions};
   for (const l3d_tensor* t : lists)
     if (t && no_data(t)) return fail(L3D_E_NULL, "%s: null data pointer", op);

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from ._lib import (call, desc, empty, packed, packs, packs_here, ref, stream_handle, stream_of,
+from ._lib import (address, call, desc, empty, invoke, packed, packs, ref, stream_handle, stream_of,
                    workspace)
 
 ACT = {"none": 0, "silu": 1, "gelu_erf": 2, "gelu_tanh": 3}
@@ -662,6 +662,11 @@ def sandwich_residual_norm(x, h, post_weight=None, post_bias=None, gate=None, re
 
 
 # ------------------------------------------- decoding over a paged cache
+def _stream(t):
+    """The current stream of a tensor's device; 0 for a host tensor, which the call refuses."""
+    return stream_of(t) if t.is_cuda else 0
+
+
 class RotaryAxes:
     """Frequencies of a rotation by positions on several axes (time, height, width;
     or one), laid out once for `paged_append`: sections[a] pairs of a head turn with
@@ -706,8 +711,6 @@ def paged_append(q, k, v, k_pages, v_pages, table, held, offsets=None, rope=None
     them, place p to slot p % size of page table[b, p / size] (table int32).  A token
     without a place in the cache is not stored, and its q comes out NaN (held and
     table lie on the device: no error can be raised without waiting for them)."""
-    if out is None:
-        out = empty(q, *q.shape)
     if rope is None:
         freqs = axis = None
         half = 0
@@ -720,11 +723,8 @@ def paged_append(q, k, v, k_pages, v_pages, table, held, offsets=None, rope=None
                 positions = positions.unsqueeze(1)
             if positions.shape[-1] != rope.axes:
                 raise ValueError(f"positions on {positions.shape[-1]} axes, the rotation has {rope.axes}")
-    dq, dk, dv, dqw, dkw, df, da, dp, dt, dh, do, dout, dkp, dvp = packs_here(
-        q, k, v, q_weight, k_weight, freqs, axis, positions, table, held, offsets, out, k_pages, v_pages)
-    call("l3d_paged_append", dq, dk, dv, dqw, dkw, eps, df, da, half, dp, dt, dh, do, dout, dkp, dvp,
-         stream_of(q))
-    return out
+    return invoke("l3d_paged_append", _stream(q), eps, half, q, k, v, q_weight, k_weight, freqs, axis, positions,
+                  table, held, offsets, out, k_pages, v_pages)
 
 
 def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None, check=None):
@@ -734,19 +734,8 @@ def paged_attention(q, k_pages, v_pages, table, lengths, scale=None, out=None, c
     lengths[b] - N + 1 + i of its keys (pages and table as for `paged_append`).
     BF16 or F16, D = 64 or 128; made for one token or a few: every 16 rows of a key
     head (N * Hq / Hkv) read its keys once.  `check` as in `attention`."""
-    if out is None:
-        out = empty(q, *q.shape)
-    one = q.dim() == 3
-    dq, dk, dv, dt, dl, do = packs_here(q.unsqueeze(1) if one else q, k_pages, v_pages, table, lengths,
-                                        out.unsqueeze(1) if out.dim() == 3 else out)
-    need = 0
-    if table.dim() == 2 and k_pages.dim() == 4:  # (the entry refuses anything else)
-        B, H, D = q.shape[0], q.shape[-2], q.shape[-1]
-        need = _lib.lib().l3d_paged_attention_workspace_size(
-            B, H, k_pages.shape[2], 1 if one else q.shape[1], table.shape[1] * k_pages.shape[1], D)
-    ws = workspace(q, need)
-    call("l3d_paged_attention", dq, dk, dv, dt, dl, q.shape[-1] ** -0.5 if scale is None else float(scale),
-         do, ws.data_ptr(), need, stream_of(q))
+    out = invoke("l3d_paged_attention", address("l3d_paged_attention_workspace_size"), _stream(q),
+                 q.shape[-1] ** -0.5 if scale is None else scale, q, k_pages, v_pages, table, lengths, out)
     _check_status("l3d_paged_attention", q, check)
     return out
 
@@ -759,16 +748,7 @@ def cross_attention(q, k, v, k_offsets, q_offsets=None, scale=None, out=None, ch
     k_offsets[b + 1] - 1.  The same offsets for both: each sequence attends to
     itself.  Rows of no sequence are left as they are (in `out`, where it is given).
     BF16 or F16, D = 64 or 128; `check` as in `attention`."""
-    if out is None:
-        out = empty(q, *q.shape)
-    dq, dk, dv, dko, dqo, do = packs_here(q, k, v, k_offsets, q_offsets, out)
-    need = 0
-    if q.dim() == 3 and k.dim() == 3:  # (the entry refuses anything else)
-        need = _lib.lib().l3d_cross_attention_workspace_size(
-            k_offsets.numel() - 1, q.shape[0], k.shape[0], q.shape[1], k.shape[1], q.shape[2],
-            q_offsets is not None)
-    ws = workspace(q, need) if need else None
-    call("l3d_cross_attention", dq, dk, dv, dko, dqo, q.shape[-1] ** -0.5 if scale is None else float(scale),
-         do, ws.data_ptr() if need else None, need, stream_of(q))
+    out = invoke("l3d_cross_attention", address("l3d_cross_attention_workspace_size"), _stream(q),
+                 q.shape[-1] ** -0.5 if scale is None else scale, q, k, v, k_offsets, q_offsets, out)
     _check_status("l3d_cross_attention", q, check)
     return out

@@ -488,3 +488,41 @@ def test_tokens_decoded_one_by_one(ops, dev):
             bound = U["bf16"] * o.abs() + (4e-3 + 1.6e-4) * mag + 1e-7
             assert ((out[b].double() - o).abs() <= bound).all()
     assert at == L
+
+
+def test_front_end_refuses(pkg, ops, dev):
+    """The library's refusals come through the native calls with its words, each argument in its place."""
+    import torch
+
+    E = pkg._lib.L3dError
+
+    def z(*shape, dtype=torch.bfloat16):
+        return torch.zeros(shape, dtype=dtype, device=dev)
+    q, kv, pages, table, held = z(2, 4, 64), z(2, 2, 64), z(3, 16, 2, 64), z(2, 1, dtype=torch.int32), z(2, dtype=torch.int32)
+    ok = dict(q=q, k=kv, v=kv, k_pages=pages, v_pages=pages.clone(), table=table, held=held)
+    assert ops.paged_append(**ok).shape == q.shape
+    for over, word in ((dict(q=q.float()), "BF16"), (dict(k=kv[:1]), "k and v"), (dict(v=kv[:, :1]), "k and v"),
+                       (dict(k_pages=pages[:2]), "k_pages and v_pages"), (dict(table=held), "table"),
+                       (dict(held=held[:1]), "held"), (dict(offsets=held), "offsets"), (dict(q_weight=z(64)), "together"),
+                       (dict(q_weight=z(64), k_weight=z(63)), "k_weight"), (dict(out=q[:1]), "q_out"), (dict(eps=-1.0), "eps")):
+        with pytest.raises(E, match=word):
+            ops.paged_append(**(ok | over))
+    ok = dict(q=q, k_pages=pages, v_pages=pages, table=table, lengths=held)
+    assert (ops.paged_attention(**ok) == 0).all()
+    for over, word in ((dict(q=q[None, None]), r"\[B, N, H, D\]"), (dict(v_pages=pages[:2]), "k_pages and v_pages"),
+                       (dict(table=table[:1]), "table"), (dict(lengths=held[:1]), "lengths"), (dict(out=q[:1]), "out"),
+                       (dict(scale=0.0), "scale"), (dict(table=held), "table"), (dict(k_pages=kv, v_pages=kv), r"\[B, N, H, D\]")):
+        with pytest.raises(E, match=word):
+            ops.paged_attention(**(ok | over))
+    off = torch.tensor([0, 1, 2], dtype=torch.int32, device=dev)
+    ok = dict(q=q, k=kv, v=kv, k_offsets=off)
+    assert ops.cross_attention(**ok).shape == q.shape
+    for over, word in ((dict(v=kv[:1]), "k and v"), (dict(k_offsets=off.float()), "k_offsets"), (dict(q_offsets=off[:2]), "q_offsets"),
+                       (dict(k_offsets=off[None]), "k_offsets"), (dict(scale=-1.0), "scale"), (dict(out=q[:, :2]), "out"),
+                       (dict(q=q[0]), "Tq, Hq, D"), (dict(k=kv[0], v=kv[0]), "Tk, Hkv, D")):
+        with pytest.raises(E, match=word):
+            ops.cross_attention(**(ok | over))
+    for f, args in ((ops.paged_append, (q, kv.cpu(), kv, pages, pages, table, held)), (ops.paged_attention, (q, pages, pages, table.cpu(), held)),
+                    (ops.cross_attention, (q, kv, kv, off.cpu()))):
+        with pytest.raises(ValueError, match="CUDA"):
+            f(*args)

@@ -60,6 +60,8 @@ def _append_args(**over):
     (dict(k_weight=_zeros(3, 64)), E_SHAPE, "k_weight"),
     (dict(q=_zeros(6, 4, 68)[..., 2:66]), E_ALIGN, "16-byte"),
     (dict(k=_zeros(6, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
+    (dict(q_out=_zeros(6, 1, 64).expand(6, 4, 64)), E_ALIGN, "expanded"),
+    (dict(k_pages=_zeros(1, 16, 2, 64).expand(7, 16, 2, 64)), E_ALIGN, "expanded"),
 ])
 def test_paged_append_refuses(pkg, over, code, word):
     _refused(pkg, "l3d_paged_append", _append_args(**over), code, word)
@@ -102,6 +104,7 @@ def _paged_args(**over):
     (dict(workspace=None), E_WORKSPACE, "workspace"),
     (dict(workspace=264), E_ALIGN, "256"),
     (dict(k_pages=_zeros(7, 16, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
+    (dict(k_pages=_zeros(1, 16, 2, 64).expand(7, 16, 2, 64)), E_ALIGN, "expanded"),
 ])
 def test_paged_attention_refuses(pkg, over, code, word):
     _refused(pkg, "l3d_paged_attention", _paged_args(**over), code, word)
@@ -206,7 +209,8 @@ def test_cross_attention_nothing_to_do(pkg):
         pkg.ops.cross_attention(_zeros(3, 4, 64), _zeros(5, 4, 64), _zeros(5, 4, 64), _zeros(2, dtype="int32"))
 
 
-def test_cross_attention_status_reaches_the_caller(pkg, monkeypatch):
+@pytest.mark.parametrize("op", ["paged_attention", "cross_attention"])
+def test_status_reaches_the_caller(pkg, monkeypatch, op):
     """A wait that ran out raises where it is asked for, as in the other serving entries."""
     from contextlib import nullcontext
     from types import SimpleNamespace
@@ -217,18 +221,47 @@ def test_cross_attention_status_reaches_the_caller(pkg, monkeypatch):
 
     def call(name, *args):
         seen.append(name)
-        if name == "l3d_kernel_status":
-            args[0]._obj.value = 5
+        args[0]._obj.value = 5
 
     monkeypatch.setattr(ops, "call", call)
-    monkeypatch.setattr(ops, "packs_here", lambda *a: a)
-    monkeypatch.setattr(ops, "stream_of", lambda t: None)
+    monkeypatch.setattr(ops, "invoke", lambda name, *a: seen.append(name))
     monkeypatch.setattr(torch.cuda, "device", lambda d: nullcontext())
     monkeypatch.setattr(torch.cuda, "current_stream",
                         lambda d: SimpleNamespace(synchronize=lambda: seen.append("synchronised")))
-    args = _zeros(60, 4, 64), _zeros(40, 2, 64), _zeros(40, 2, 64), _zeros(4, dtype="int32"), _zeros(4, dtype="int32")
-    ops.cross_attention(*args)
-    assert seen == ["l3d_cross_attention"]
-    with pytest.raises(pkg._lib.L3dError, match="l3d_cross_attention.*status word 5"):
-        ops.cross_attention(*args, check=True)
-    assert seen[1:] == ["l3d_cross_attention", "synchronised", "l3d_kernel_status"]
+    args = (_zeros(60, 4, 64), *[_zeros(40, 2, 64)] * 2, *[_zeros(4, dtype="int32")] * 2)
+    getattr(ops, op)(*args)
+    assert seen == [f"l3d_{op}"]
+    with pytest.raises(pkg._lib.L3dError, match=f"l3d_{op}.*status word 5"):
+        getattr(ops, op)(*args, check=True)
+    assert seen[1:] == [f"l3d_{op}", "synchronised", "l3d_kernel_status"]
+
+
+def test_native_calls_check_their_arguments(pkg):
+    L = pkg._lib
+    with pytest.raises(TypeError, match="tensor expected"):
+        L.invoke("l3d_paged_append", 0, 1e-6, 0, *[None] * 14)
+    with pytest.raises(ValueError, match="CUDA"):
+        L.invoke("l3d_paged_append", 0, 1e-6, 0, *[None] * 11, _zeros(3), None, None)
+    with pytest.raises(TypeError, match="tensor expected"):
+        L.invoke("l3d_paged_append", 0, 1e-6, 0, 7, *[None] * 13)
+    for name in ("l3d_paged_attention", "l3d_cross_attention"):
+        with pytest.raises(TypeError, match="tensor expected"):
+            L.invoke(name, L.address(name + "_workspace_size"), 0, 0.125, *[None] * 6)
+        with pytest.raises(TypeError, match="10 arguments"):
+            L.invoke(name, 0)
+    with pytest.raises(TypeError, match="18 arguments"):
+        L.invoke("l3d_paged_append", 0)
+    with pytest.raises(TypeError):
+        L.invoke("l3d_paged_append", 0, "eps", 0, *[None] * 14)
+
+
+def test_calls_without_the_native_module_say_why(pkg):
+    from test_serving_checks import _without_pack
+
+    out = _without_pack("import torch\n"
+                        "z, i = torch.zeros(2, 4, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)\n"
+                        "for f in (lambda: pkg.ops.cross_attention(z, z, z, i), lambda: pkg.ops.paged_attention(z, z, z, i, i),\n"
+                        "          lambda: pkg.ops.paged_append(z, z, z, z, z, i, i)):\n"
+                        "    try: f()\n"
+                        "    except RuntimeError as e: print(e)\n")
+    assert out.count("made for another torch") == 3
