@@ -395,11 +395,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
           ++vturn;
         }
         ++n;
-        // Scores up to two ahead, over the P that the product before it has read.  An item's first ones are not
-        // waited for while a product is still to come: its Q is on its way (that wait held up the last P V of
-        // the item before, 1,600 clocks of the 37,000 that an item of 18 tiles took).
-        while (ok && more && ns < n + 2 && (js > 0 || ns == n || __all_sync(0xffffffffu, mbar_try_wait(q_full, items & 1))))
-          issue_s();
+        if (more) issue_s();  // over the P that the product before it has read
       }
     }
   } else if (warp == 3) {

@@ -18,6 +18,8 @@
 // the keys of a request's head, the warp stores the output; otherwise O / l and the log2 of the sum in f32, and
 // combine_kernel weighs the parts of each row.  A part's place follows from the lengths, so results do not
 // depend on the order in which warps run.
+// Short caches of a few requests need neither line nor second kernel: a block takes all the keys of a head and row
+// tile, a stretch of them per warp, and joins the parts in shared memory (ALONE).
 //
 // Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability
 // (the products are not what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
@@ -37,6 +39,7 @@ using namespace l3d::attn;
 
 constexpr int WARPS = 12;               // of a block (one per SM)
 constexpr int MIN_TILES = 1;            // of a warp
+constexpr int ALONE_TILES = 4;          // of a warp, up to which a block takes a head's keys alone
 constexpr int OWN_SUM = 256;            // requests up to which combine_kernel sums their keys up itself
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
@@ -184,7 +187,7 @@ struct Cursor {
 };
 
 // NB: columns of 8 rows in a row tile.
-template <typename T, int D, int NB>
+template <typename T, int D, int NB, bool ALONE>
 __global__ void __launch_bounds__(WARPS * 32, 1)
     decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Params p) {
   using C = Cfg<D>;
@@ -210,8 +213,12 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   if (threadIdx.x == 0) *abort_flag = 0;
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // for the kernel before: nothing global is touched earlier
+  const int heads = p.Hkv * p.tiles;
+  const int me = warp * gridDim.x + blockIdx.x;  // a short line spreads over the device first
+  int64_t x0 = 0;
+  int count = 0;
   // ---- key tiles before each sequence: a sum over the batch, a stretch of it per thread
-  {
+  if constexpr (!ALONE) {
     const int per = (p.B + WARPS * 32 - 1) / (WARPS * 32), b0 = min(int(threadIdx.x) * per, p.B), b1 = min(b0 + per, p.B);
     int sum = 0;
     for (int b = b0; b < b1; ++b) {
@@ -240,19 +247,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     if (blockIdx.x == 0 && p.B > OWN_SUM)
       for (int b = threadIdx.x; b <= p.B; b += WARPS * 32) p.starts[b] = starts[b];
   }
-  const int heads = p.Hkv * p.tiles;
-  const Line line = line_of(p, starts[p.B]);
-  const int me = warp * gridDim.x + blockIdx.x;  // a short line spreads over the device first
-  const int64_t x0 = int64_t(me) * line.per;
-  if (x0 >= line.total) return;
-  const int count = int(min(line.per, line.total - x0));
+  if constexpr (!ALONE) {
+    const Line line = line_of(p, starts[p.B]);
+    x0 = int64_t(me) * line.per;
+    if (x0 >= line.total) return;
+    count = int(min(line.per, line.total - x0));
+  } else {
+    __syncthreads();  // (the barriers are there)
+  }
+  // Where this warp begins.
+  auto seek = [&](Cursor& c) {
+    if constexpr (ALONE) {
+      c.b = blockIdx.x / heads;
+      c.hr = blockIdx.x - c.b * heads;
+      bool bad;
+      c.tiles = (length_of(p, c.b, &bad) + KT - 1) / KT;
+      const int per = (c.tiles + WARPS - 1) / WARPS;
+      c.t = warp * per;
+      count = max(min(c.tiles - c.t, per), 0);
+    } else {
+      c.seek(starts, p.B, heads, x0);
+    }
+  };
 
   // ---- loads, STAGES tiles ahead of the work: lane i takes box i of a tile.  A tile's table entries are looked
   // up one tile early, so that their latency is not waited for.
   const uint32_t ring = smem_u32(smem) + warp * C::RING;
   uint64_t* full = bars + warp * C::STAGES;
   Cursor ld;
-  ld.seek(starts, p.B, heads, x0);
+  seek(ld);
   int ld_page = 0, ld_slot = 0, ld_h = 0, ld_len = 0, ld_first = 0;
   bool ld_ok = false, ld_new = true;
   auto look_up = [&] {
@@ -272,7 +295,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       if (ld_ok) ld_page = p.table[ld.b * p.table_stride + page];
     }
   };
-  look_up();
+  if (count > 0) look_up();
   int issued = 0, ld_stage = 0;
   auto issue = [&] {
     if (issued >= count) return;
@@ -306,7 +329,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
 
   // ---- work
   Cursor cu;
-  cu.seek(starts, p.B, heads, x0);
+  seek(cu);
   // This thread's keys (or head dims) g and g + 8 of 16, its rows q2 and q2 + 1 of 8; Q is loaded for row g.
   const int g8 = lane >> 2, q2 = (lane & 3) * 2;
   const int R = p.N * p.G;
@@ -319,6 +342,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     k_at[i] = k_row + (((2 * i + (mi >> 1)) ^ r8) << 4);
     v_at[i] = v_row + (((2 * i + (mi & 1)) ^ r8) << 4);
   }
+  // ALONE: this warp's part, over its ring.
+  float* const alone_o = reinterpret_cast<float*>(smem + warp * C::RING);
+  float* const alone_l = alone_o + 8 * NB * D;
+  if (ALONE && count == 0 && lane < 8 * NB) alone_l[lane] = -INFINITY;
   uint32_t qf[D / 16][NB][2];
   float o[NT][NB][4];
   float m[NB][2], l[NB][2];
@@ -514,6 +541,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       // The end of a part: the output, or O / l and the log2 sum.
       fresh = true;
       const bool whole = t_first == 0 && cu.t + 1 == cu.tiles;
+      if constexpr (ALONE) __syncwarp();  // (the tiles are read: the part goes over them)
       const int h = cu.hr / p.tiles, f0 = (cu.hr - h * p.tiles) * (8 * NB);
       const int64_t part = (2 * int64_t(me) + (t_first == 0 ? 1 : 0)) * p.rows;
 #pragma unroll
@@ -527,10 +555,16 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
           sum += __shfl_xor_sync(0xffffffffu, sum, 16);
           inv[e] = sum > 0.f ? 1.f / sum : sum == sum ? 0.f : sum;
           const int r = nb * 8 + q2 + e;
-          if (!whole && g8 == 0 && f0 + r < R)
-            p.part_l[part + r] = sum > 0.f ? m[nb][e] + log2f(sum) : sum == sum ? -INFINITY : sum;
+          if (ALONE ? g8 == 0 : !whole && g8 == 0 && f0 + r < R)
+            (ALONE ? alone_l + r : p.part_l + part + r)[0] = sum > 0.f ? m[nb][e] + log2f(sum) : sum == sum ? -INFINITY : sum;
         }
-        if (whole) {
+        if constexpr (ALONE) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int c = 0; c < 2 * NT; ++c)
+              alone_o[(nb * 8 + q2 + e) * D + c * 8 + g8] = o[c >> 1][nb][(c & 1) * 2 + e] * inv[e];
+        } else if (whole) {
           const int f = f0 + nb * 8 + g8, i = f / p.G, g = f - i * p.G;
           T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + g) * p.oh + q2;
 #pragma unroll
@@ -556,6 +590,41 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   if (!ok && lane == 0) {  // the newest load of each stage: no copy may be in flight when the block exits
     for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
       mbar_drain(&full[i % C::STAGES], uint32_t(i / C::STAGES) & 1u, p.wait_ns);
+  }
+  if constexpr (ALONE) {
+    // The warps' parts of each row weighed by 2^(their log2 sum - the largest), in the warps' order.
+    __syncthreads();
+    if (*abort_flag) return;
+    constexpr int E = D / 32;
+    bool bad;
+    length_of(p, cu.b, &bad);
+    const int h = cu.hr / p.tiles, f0 = (cu.hr - h * p.tiles) * (8 * NB);
+    for (int r = warp; r < 8 * NB && f0 + r < R; r += WARPS) {
+      auto part_l = [&](int w) { return reinterpret_cast<const float*>(smem + w * C::RING)[8 * NB * D + r]; };
+      float wgt = lane < WARPS ? part_l(lane) : -INFINITY, mx = wgt;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, x));
+      wgt = wgt == -INFINITY ? 0.f : exp2f(wgt - mx);
+      float sum = wgt;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      float acc[E] = {};
+      for (int w = 0; w < WARPS; ++w) {
+        const float ww = __shfl_sync(0xffffffffu, wgt, w);
+        if (ww == 0.f) continue;  // a part without keys: nothing is stored there
+        const float* src = reinterpret_cast<const float*>(smem + w * C::RING) + r * D + lane * E;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(ww, src[e], acc[e]);
+      }
+      const float inv = bad ? __int_as_float(0x7fffffff) : sum != 0.f ? 1.f / sum : 0.f;
+      const int i = (f0 + r) / p.G;
+      T* orow = reinterpret_cast<T*>(p.out) + cu.b * p.ob + i * p.on + (h * p.G + f0 + r - i * p.G) * p.oh + lane * E;
+      alignas(8) T v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = from_f<T>(acc[e] * inv);
+      if constexpr (E == 4) *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(v);
+      else *reinterpret_cast<uint32_t*>(orow) = *reinterpret_cast<const uint32_t*>(v);
+    }
   }
 }
 
@@ -679,8 +748,14 @@ static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
   return int(want < 1 ? 1 : want < sm_count() ? want : sm_count());
 }
 
+// A block for each head and row tile: as many as run at once, with few tiles for each warp.
+static bool alone(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
+  const int64_t h = height_for(N * G);
+  return B * Hkv * ((N * G + h - 1) / h) <= sm_count() && longest <= ALONE_TILES * WARPS * tile_keys(int(D));
+}
+
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
-  if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0 || D <= 0) return 0;
+  if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0 || D <= 0 || alone(B, N, G, Hkv, longest, D)) return 0;
   const int64_t h = height_for(N * G), rows = N * G < h ? N * G : h;
   const int64_t parts = 2 * int64_t(blocks_for(B, N, G, Hkv, longest, D)) * WARPS;
   return (size_t(B + 1) * 4 + 255) / 256 * 256 + (size_t(parts * rows) * 4 + 255) / 256 * 256 + size_t(parts * rows * D) * 4;
@@ -688,7 +763,9 @@ size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
 
 template <typename T, int D>
 static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int blocks, cudaStream_t s) {
-  auto k = p.height == 8 ? decode_kernel<T, D, 1> : decode_kernel<T, D, 2>;
+  const bool one = p.total_warps == 0;
+  auto k = p.height == 8 ? (one ? decode_kernel<T, D, 1, true> : decode_kernel<T, D, 1, false>)
+                         : (one ? decode_kernel<T, D, 2, true> : decode_kernel<T, D, 2, false>);
   constexpr int fixed = WARPS * Cfg<D>::RING + Cfg<D>::BARS;
   cudaError_t e = set_smem_limit(reinterpret_cast<const void*>(k), fixed + (MAX_BATCH + 1) * 4);
   if (e != cudaSuccess) return e;
@@ -702,9 +779,9 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   cfg.stream = s;
   cfg.gridDim = dim3(unsigned(blocks));
   cfg.blockDim = dim3(WARPS * 32);
-  cfg.dynamicSmemBytes = fixed + (p.B + 1) * 4;
+  cfg.dynamicSmemBytes = fixed + (one ? 0 : (p.B + 1) * 4);
   e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], p);
-  if (e != cudaSuccess) return e;
+  if (e != cudaSuccess || one) return e;
   const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G;
   const bool few = rows <= 2 * sm_count();  // then their parts are many
   cfg.gridDim = dim3(unsigned(rows));
@@ -714,11 +791,13 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
 }
 
 int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
-  const int R = p.N * p.G, blocks = blocks_for(p.B, p.N, p.G, p.Hkv, longest, kv.D);
+  const int R = p.N * p.G;
+  const bool one = alone(p.B, p.N, p.G, p.Hkv, longest, kv.D);
   p.height = height_for(R);
   p.tiles = (R + p.height - 1) / p.height;
   p.rows = R < p.height ? R : p.height;
-  p.total_warps = blocks * WARPS;
+  const int blocks = one ? p.B * p.Hkv * p.tiles : blocks_for(p.B, p.N, p.G, p.Hkv, longest, kv.D);
+  p.total_warps = one ? 0 : blocks * WARPS;
   p.wait_ns = tc::WAIT_LIMIT_NS;
   char* w = static_cast<char*>(workspace);
   p.starts = reinterpret_cast<int*>(w);
@@ -814,7 +893,7 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
                 l3d::decode::MAX_BATCH);
   if (B * N * Hq == 0) return L3D_OK;
   const size_t need = l3d::decode::workspace_size(B, N, Hq / Hkv, Hkv, width * size, D);
-  if (!workspace || workspace_bytes < need)
+  if (need && (!workspace || workspace_bytes < need))
     return fail(L3D_E_WORKSPACE, "%s: workspace of %zu bytes required", op, need);
   if (reinterpret_cast<uintptr_t>(workspace) % 256)
     return fail(L3D_E_ALIGN, "%s: workspace must be 256-byte aligned", op);

@@ -34,14 +34,14 @@ struct Params {
   int len64, causal;
   float scale_log2;             // softmax scale * log2(e), > 0
   int height, tiles, rows;      // rows of a row tile, row tiles of a key head, rows of a tile's part
-  int total_warps;
+  int total_warps;              // 0: a block for each head and row tile
   uint64_t wait_ns;
   int* starts;                  // workspace: key tiles before each sequence [B + 1]
   float *part_l, *part_o;       // [2 warps, rows], [2 warps, rows, D]
 };
 
 constexpr int MAX_BATCH = 4096;
-// Workspace bytes, the same for every division of the keys; 0: nothing to do.
+// Workspace bytes, whatever the lengths are; 0: none needed.
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D);
 // Fills in what follows from the sizes and the workspace, and launches; an entry's status.  `longest`: the most
 // keys a sequence can have.

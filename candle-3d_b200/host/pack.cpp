@@ -236,8 +236,9 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (d.ptr[0] && d.ptr[1] && d.ptr[3] && d.at[0].ndim == 4 && d.at[1].ndim == 4 && d.at[3].ndim == 2)  // (else refused)
       need = size(d.at[0].dims[0], d.at[0].dims[2], d.at[1].dims[2], d.at[0].dims[1], d.at[3].dims[1] * d.at[1].dims[1],
                   d.at[0].dims[3]);
-    const at::Tensor ws = workspace_for(out, need);
-    void* wp = ws.data_ptr();
+    at::Tensor ws;
+    if (need) ws = workspace_for(out, need);
+    void* wp = need ? ws.data_ptr() : nullptr;
     const auto& p = d.ptr;
     return result(without_lock([&] { return fn(p[0], p[1], p[2], p[3], p[4], float(scale), p[5], wp, need, stream); }), out);
   });

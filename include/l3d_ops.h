@@ -523,8 +523,8 @@ int l3d_paged_append(const l3d_tensor* q, const l3d_tensor* k, const l3d_tensor*
                      const l3d_tensor* offsets, const l3d_tensor* q_out,
                      const l3d_tensor* k_pages, const l3d_tensor* v_pages, l3d_stream stream);
 
-/* Workspace bytes for l3d_paged_attention; capacity: the keys that a request's
- * row of the table has room for (W * size). */
+/* Workspace bytes for l3d_paged_attention (0: none needed); capacity: the keys
+ * that a request's row of the table has room for (W * size). */
 size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, int64_t n,
                                           int64_t capacity, int64_t d);
 

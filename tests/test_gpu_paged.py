@@ -259,8 +259,10 @@ def _check_attention(out, q, k_pages, v_pages, table, lens, dt, scale=None):
             f"request {b} of {n} keys: max err {err.max().item():.3e}, worst ratio {(err / bound).max().item():.2f}"
 
 
-def _run_attention(ops, dev, lens, N, Hq, Hkv, D, size, dt="bf16", layout="token", std=1.0, scale=None, bits=32):
-    """Slots that no request has reached and pages of nobody hold NaN."""
+def _run_attention(ops, dev, lens, N, Hq, Hkv, D, size, dt="bf16", layout="token", std=1.0, scale=None, bits=32,
+                   wide=False):
+    """Slots that no request has reached and pages of nobody hold NaN.  `wide`: tables with room for many more
+    keys, which few requests then divide over the device."""
     import torch
 
     r = rng(len(lens) * 31 + N * 7 + Hq + D + size + sum(lens))
@@ -272,8 +274,9 @@ def _run_attention(ops, dev, lens, N, Hq, Hkv, D, size, dt="bf16", layout="token
             vp[table[b, n // size].long(), n % size:] = float("inf") if b % 2 else float("nan")
     for p in free.tolist():
         kp[p] = vp[p] = float("nan")
-    out = ops.paged_attention(q, kp, vp, table, _ints(lens, dev, bits), scale=scale)
-    torch.cuda.synchronize()
+    if wide:
+        table = torch.cat([table, torch.full((len(lens), 9000 // size), -1, dtype=torch.int32, device=dev)], 1)
+    out = ops.paged_attention(q, kp, vp, table, _ints(lens, dev, bits), scale=scale, check=True)
     _check_attention(out, q, kp, vp, table, lens, dt, scale)
     return q, kp, vp, table, out
 
@@ -298,9 +301,11 @@ def test_paged_attention(ops, dev, lens, N, Hq, Hkv, size, layout, D, dt):
 
 
 @pytest.mark.parametrize("n", [1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 47, 48, 49, 63, 64, 65, 511, 512, 513, 4095, 4096, 4097])
-def test_paged_lengths(ops, dev, n):
-    _run_attention(ops, dev, [n, n + 1, max(n - 1, 0)], 1, 8, 2, 128, 16)
-    _run_attention(ops, dev, [n, n + 1, max(n - 1, 0)], 3, 2, 2, 64, 24)
+@pytest.mark.parametrize("wide", [False, True])
+def test_paged_lengths(ops, dev, n, wide):
+    _run_attention(ops, dev, [n, n + 1, max(n - 1, 0)], 1, 8, 2, 128, 16, wide=wide)
+    _run_attention(ops, dev, [n, n + 1, max(n - 1, 0)], 3, 2, 2, 64, 24, wide=wide)
+    _run_attention(ops, dev, [n, 0, 1], 5, 4, 2, 64, 1 if n < 600 else 40, "f16", wide=wide)  # ten rows
 
 
 def test_paged_attention_scores_far_apart(ops, dev):
@@ -332,12 +337,13 @@ def test_one_row_form_and_strides(ops, dev):
     assert torch.equal(big[:, 1:2], out) and (big[:, 0] == 5).all() and (big[:, 2] == 5).all()
 
 
-def test_rows_that_do_not_see_a_key_are_untouched_by_it(ops, dev):
+@pytest.mark.parametrize("wide", [False, True])
+def test_rows_that_do_not_see_a_key_are_untouched_by_it(ops, dev, wide):
     """A later token's K or V that is not finite reaches the rows that see it, and no earlier row."""
     import torch
 
     for D, what, val in ((64, "v", math.nan), (128, "v", math.inf), (64, "k", math.nan), (128, "k", math.inf)):
-        q, kp, vp, table, out = _run_attention(ops, dev, [70, 50], 4, 8, 2, D, 16)
+        q, kp, vp, table, out = _run_attention(ops, dev, [70, 50], 4, 8, 2, D, 16, wide=wide)
         lens = _ints([70, 50], dev)
         page, slot = int(table[0, 68 // 16]), 68 % 16
         q[0, :, :, 0] = 1.0  # a K of +inf then scores +inf, not NaN
@@ -354,11 +360,12 @@ def test_rows_that_do_not_see_a_key_are_untouched_by_it(ops, dev):
 
 @pytest.mark.parametrize("key", [0, 7, 8, 100, 199])
 @pytest.mark.parametrize("val", [math.nan, math.inf, -math.inf])
-def test_scores_without_a_softmax(ops, dev, key, val):
+@pytest.mark.parametrize("wide", [False, True])
+def test_scores_without_a_softmax(ops, dev, key, val, wide):
     """A score of NaN or +inf makes its row NaN wherever it lies; one of -inf has no weight."""
     import torch
 
-    q, kp, vp, table, out = _run_attention(ops, dev, [200, 200], 1, 4, 2, 128, 16)
+    q, kp, vp, table, out = _run_attention(ops, dev, [200, 200], 1, 4, 2, 128, 16, wide=wide)
     q[:, :, :, 3] = 1.0
     kp[int(table[1, key // 16]), key % 16, 1, 3] = val
     got = ops.paged_attention(q, kp, vp, table, _ints([200, 200], dev))
@@ -369,11 +376,12 @@ def test_scores_without_a_softmax(ops, dev, key, val):
     assert torch.isfinite(got[0]).all() and torch.isfinite(got[1, 0, :2]).all()
 
 
-def test_bad_pages_and_lengths(ops, dev):
+@pytest.mark.parametrize("wide", [False, True])
+def test_bad_pages_and_lengths(ops, dev, wide):
     """A page that is none of the cache, or a length past the table: that request's rows are NaN, no other's."""
     import torch
 
-    q, kp, vp, table, out = _run_attention(ops, dev, [300, 280, 260, 40], 1, 8, 2, 64, 16)
+    q, kp, vp, table, out = _run_attention(ops, dev, [300, 280, 260, 40], 1, 8, 2, 64, 16, wide=wide)
     tab, lens = table.clone(), _ints([300, 280, 10 ** 9, -4], dev)
     tab[0, 7] = kp.shape[0]
     tab[3, 0] = 10 ** 9  # of a request without keys: never looked at

@@ -100,8 +100,8 @@ def _paged_args(**over):
     (dict(k_pages=_zeros(7, 0, 2, 64), v_pages=_zeros(7, 0, 2, 64)), E_UNSUPPORTED, "no tokens"),
     (dict(q=_zeros(4097, 1, 4, 64), out=_zeros(4097, 1, 4, 64), table=_zeros(4097, 5, dtype="int32"),
           lengths=_zeros(4097, dtype="int32")), E_UNSUPPORTED, "4096"),
-    (dict(bytes=0), E_WORKSPACE, "workspace"),
-    (dict(workspace=None), E_WORKSPACE, "workspace"),
+    (dict(table=_zeros(3, 900, dtype="int32"), bytes=0), E_WORKSPACE, "workspace"),
+    (dict(table=_zeros(3, 900, dtype="int32"), workspace=None), E_WORKSPACE, "workspace"),
     (dict(workspace=264), E_ALIGN, "256"),
     (dict(k_pages=_zeros(7, 16, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
     (dict(k_pages=_zeros(1, 16, 2, 64).expand(7, 16, 2, 64)), E_ALIGN, "expanded"),
@@ -191,7 +191,8 @@ def _cross_args(**over):
     (dict(q=_zeros(60, 1, 64).expand(60, 4, 64)), E_ALIGN, "expanded"),
     (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), bytes=0), E_WORKSPACE, "workspace"),
     (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), workspace=264), E_ALIGN, "256"),
-    (dict(q_offsets=None, q=_zeros(3, 4, 64), out=_zeros(3, 4, 64), workspace=None), E_WORKSPACE, "workspace"),
+    (dict(q_offsets=None, q=_zeros(3, 4, 64), out=_zeros(3, 4, 64), k=_zeros(9000, 2, 64), v=_zeros(9000, 2, 64),
+          workspace=None), E_WORKSPACE, "workspace"),
     (dict(k=_zeros(40, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
     (dict(q=_zeros(60, 4, 68)[..., 2:66]), E_ALIGN, "16-byte"),
 ])
