@@ -39,8 +39,6 @@ using namespace l3d::attn;
 
 constexpr int WARPS = 12;               // of a block (one per SM)
 constexpr int MIN_TILES = 1;            // of a warp
-constexpr int ALONE_TILES = 4;          // of a warp, up to which a block takes a head's keys alone
-constexpr int OWN_SUM = 256;            // requests up to which combine_kernel sums their keys up itself
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 
@@ -244,7 +242,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     if (threadIdx.x == WARPS * 32 - 1) starts[p.B] = at;  // (its stretch is the last, or empty)
     __syncthreads();
-    if (blockIdx.x == 0 && p.B > OWN_SUM)
+    if (blockIdx.x == 0)
       for (int b = threadIdx.x; b <= p.B; b += WARPS * 32) p.starts[b] = starts[b];
   }
   if constexpr (!ALONE) {
@@ -628,60 +626,35 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   }
 }
 
-// The parts of each row weighed by 2^(their log2 sum - the largest), in a fixed order: a block per row, W warps
-// with every W-th part each, D / 32 elements per lane.  Rows without keys are zeroed here, and no others
-// touched that one warp has finished.
+// The parts of each row weighed by 2^(their log2 sum - the largest), in a fixed order: W warps for a row, with
+// every W-th part each, D / 32 elements per lane; a block of 4 rows where one warp does.  Rows without keys are
+// zeroed here, and no others touched that one warp has finished.
 template <typename T, int D, int W>
-__global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
-  constexpr int E = D / 32;
+__global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Params p) {
+  constexpr int E = D / 32, KT = tile_keys(D);
   using Vec = typename std::conditional<E == 4, float4, float2>::type;
   __shared__ alignas(16) float red[W][D];
   __shared__ float red_m[W], red_l[W];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
   const int R = p.N * p.G;
-  const int f = int(blockIdx.x % R), h = int(blockIdx.x / R % p.Hkv), b = int(blockIdx.x / R / p.Hkv);
+  const int64_t row = W == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  if (W == 1 && row >= int64_t(p.B) * p.Hkv * R) return;
+  const int f = int(row % R), h = int(row / R % p.Hkv), b = int(row / R / p.Hkv);
   const int i = f / p.G, rt = f / p.height, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + (h * p.G + f - i * p.G) * p.oh;
-  // The row's place in the line: summed up here from the lengths while the parts are formed, or, for a large
-  // batch, read from what the first kernel's first block has left.
-  constexpr int KT = tile_keys(D);
-  bool bad;
-  int before = 0, tiles = (length_of(p, b, &bad) + KT - 1) / KT, all = 0;
-  if (p.B <= OWN_SUM) {
-    __shared__ int s_before[W], s_all[W];
-    for (int x = threadIdx.x; x < p.B; x += W * 32) {
-      bool ignored;
-      const int n = (length_of(p, x, &ignored) + KT - 1) / KT;
-      all += n;
-      if (x < b) before += n;
-    }
-    before = __reduce_add_sync(0xffffffffu, before);
-    all = __reduce_add_sync(0xffffffffu, all);
-    if (lane == 0) {
-      s_before[warp] = before;
-      s_all[warp] = all;
-    }
-    __syncthreads();
-    before = all = 0;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      before += s_before[w];
-      all += s_all[w];
-    }
-  }
+  asm volatile("griddepcontrol.launch_dependents;");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (p.B > OWN_SUM) {
-    before = p.starts[b];
-    all = p.starts[p.B];
-  }
+  const int before = p.starts[b], tiles = p.starts[b + 1] - before;
   if (tiles == 0) {
+    bool bad;
+    length_of(p, b, &bad);
     if (warp == 0) {
 #pragma unroll
       for (int e = 0; e < E; ++e) orow[lane * E + e] = from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
     }
     return;
   }
-  const Line line = line_of(p, all);
+  const Line line = line_of(p, p.starts[p.B]);
   const int64_t first = int64_t(before) * heads + int64_t(hr) * tiles, last = first + tiles - 1;
   const int w0 = int(first / line.per), parts = int(last / line.per) - w0 + 1;
   if (parts == 1) return;
@@ -689,7 +662,7 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
   alignas(16) float acc[E] = {};
   // (The first part lies in its warp's second place: it holds the row's first key.)
   auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + f - rt * p.height; };
-  constexpr int U = 4;
+  constexpr int U = W == 1 ? 8 : 4;
   for (int k0 = warp; k0 < parts; k0 += W * U) {
     float pl[U];
     Vec v[U];
@@ -697,7 +670,7 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u * W;
       pl[u] = k < parts ? p.part_l[row_at(k)] : -INFINITY;
-      v[u] = reinterpret_cast<const Vec*>(p.part_o + row_at(k < parts ? k : 0) * D)[lane];
+      v[u] = reinterpret_cast<const Vec*>(p.part_o + row_at(k < parts ? k : k0) * D)[lane];
     }
     float mx = m;
 #pragma unroll
@@ -717,6 +690,15 @@ __global__ void __launch_bounds__(W * 32) combine_kernel(const Params p) {
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = fmaf(wgt, vv[e], acc[e]);
     }
+  }
+  if constexpr (W == 1) {
+    const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+    alignas(8) T o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f<T>(acc[e] * inv);
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(orow + lane * E) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint32_t*>(orow + lane * E) = *reinterpret_cast<const uint32_t*>(o);
+    return;
   }
   *reinterpret_cast<Vec*>(&red[warp][lane * E]) = *reinterpret_cast<const Vec*>(acc);
   if (lane == 0) {
@@ -748,10 +730,14 @@ static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
   return int(want < 1 ? 1 : want < sm_count() ? want : sm_count());
 }
 
-// A block for each head and row tile: as many as run at once, with few tiles for each warp.
+// A block for each head and row tile: as many as run at once, with few tiles for each warp, more the nearer the
+// blocks come to filling the device.  A block's own t tiles a warp take about 5.0 + 1.15 t us; divided over the
+// device, 8.5 us for both kernels and the bytes' time.  At t = 4 for 2, 64, 128 blocks: 9.6, 10.1, 10.1 us alone, 8.6,
+// 12.0, 14.0 divided; at 16 for 16, 128: 22.4, 24.2 and 14.4, 33.2 (but then the longest cache decides alone).
 static bool alone(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
   const int64_t h = height_for(N * G);
-  return B * Hkv * ((N * G + h - 1) / h) <= sm_count() && longest <= ALONE_TILES * WARPS * tile_keys(int(D));
+  const int64_t blocks = B * Hkv * ((N * G + h - 1) / h), stretch = WARPS * tile_keys(int(D));
+  return blocks <= sm_count() && longest <= (3 + blocks / 24) * stretch;
 }
 
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
@@ -782,12 +768,15 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   cfg.dynamicSmemBytes = fixed + (one ? 0 : (p.B + 1) * 4);
   e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], p);
   if (e != cudaSuccess || one) return e;
-  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G;
-  const bool few = rows <= 2 * sm_count();  // then their parts are many
-  cfg.gridDim = dim3(unsigned(rows));
-  cfg.blockDim = dim3(few ? 512 : 256);
+  // Warps for a row by the parts that it has on average: one takes eight in a round.  (64 requests, 7 parts: 53.8 us
+  // with one, 54.6 with eight; 12 requests x 12 heads, 12 parts, up to 29: 576 rows 47.2 and 41.3, 144 rows 37.5 with
+  // eight, 34.9 with sixteen.)
+  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G, parts = p.total_warps / (int64_t(p.B) * p.Hkv * p.tiles);
+  const int warps = parts <= 8 ? 1 : rows > 2 * sm_count() ? 8 : 16;
+  cfg.gridDim = dim3(unsigned(warps > 1 ? rows : (rows + 3) / 4));
+  cfg.blockDim = dim3(warps > 1 ? warps * 32 : 128);
   cfg.dynamicSmemBytes = 0;
-  return few ? cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 16>, p) : cudaLaunchKernelEx(&cfg, combine_kernel<T, D, 8>, p);
+  return cudaLaunchKernelEx(&cfg, warps == 1 ? combine_kernel<T, D, 1> : warps == 8 ? combine_kernel<T, D, 8> : combine_kernel<T, D, 16>, p);
 }
 
 int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
