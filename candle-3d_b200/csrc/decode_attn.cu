@@ -11,8 +11,9 @@
 // rows, and a round trip through its memory for each.
 //
 // Work is divided by keys alone: all (request, key head, row tile) have their keys in tiles of 16 (32 at
-// D = 64: 8 KB of K and V either way), the tiles of all of them in one line, and every warp of the device takes an equal stretch of the line, whatever the
-// lengths are; the lengths are read on the device, and each block sums them up for itself.  A warp works
+// D = 64: 8 KB of K and V either way), the tiles of all of them in one line, and every warp of the device takes an
+// equal stretch of the line, whatever the lengths are; the lengths are read on the device, and each block sums them
+// up for itself.  A warp works
 // alone: its own ring of tiles in shared memory, filled by TMA boxes that lie in one page each and run on across
 // the ends of requests, its own running maximum and sum, no barrier with another warp.  Where a stretch holds all
 // the keys of a request's head, the warp stores the output; otherwise O / l and the log2 of the sum in f32, and
@@ -26,6 +27,9 @@
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
 // status word and stops.
+// Measured, D = 128: 8 x 65536 keys x 4 heads 170 us (6.31 TB/s, 96% of a plain copy); 64 x up to 4096 keys x 4 heads
+// 53 us (4.56 TB/s): 3.7 us until the first loads go out, 4 for the second kernel.  One request of 300 keys x 2 heads of
+// 64: 5.7 us.
 #include <type_traits>
 
 #include "attn.cuh"
@@ -76,13 +80,18 @@ __device__ __forceinline__ int length_of(const Params& p, int b, bool* bad) {
   return v < 0 ? 0 : int(v < room ? v : room);
 }
 
+// a / b of values that are seldom past 32 bits (a 64-bit division takes some 150 clocks more).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  return ((a | b) >> 32) == 0 ? int64_t(uint32_t(a) / uint32_t(b)) : a / b;
+}
+
 // The line of tiles: sequence b's begin at starts[b] * heads, heads = Hkv * row tiles.
 struct Line {
   int64_t total, per;   // tiles, tiles of a warp
 };
 __device__ __forceinline__ Line line_of(const Params& p, int tiles) {
   const int64_t total = int64_t(tiles) * p.Hkv * p.tiles;
-  const int64_t even = (total + p.total_warps - 1) / p.total_warps;
+  const int64_t even = quotient(total + p.total_warps - 1, p.total_warps);
   return {total, even > MIN_TILES ? even : MIN_TILES};
 }
 
@@ -156,8 +165,7 @@ __device__ __forceinline__ bool not_finite(uint32_t at) {
 struct Cursor {
   int b, hr, t, tiles;
   __device__ __forceinline__ void seek(const int* starts, int B, int heads, int64_t x) {
-    const bool small = x >> 31 == 0;  // (a 64-bit division takes some 150 clocks more)
-    const int64_t y = small ? int64_t(uint32_t(x) / uint32_t(heads)) : x / heads;
+    const int64_t y = quotient(x, heads);
     int lo = 0, hi = B;  // the last b with starts[b] <= y
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
@@ -167,7 +175,7 @@ struct Cursor {
     b = lo;
     tiles = starts[b + 1] - starts[b];
     const int64_t rem = x - int64_t(starts[b]) * heads;
-    hr = small ? int(uint32_t(rem) / uint32_t(tiles)) : int(rem / tiles);
+    hr = int(quotient(rem, tiles));
     t = int(rem - int64_t(hr) * tiles);
   }
   // To the next tile (not past the line's last one); whether its head or row tile is another one.
@@ -637,9 +645,9 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Pa
   __shared__ float red_m[W], red_l[W];
   const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
   const int R = p.N * p.G;
-  const int64_t row = W == 1 ? int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
-  if (W == 1 && row >= int64_t(p.B) * p.Hkv * R) return;
-  const int f = int(row % R), h = int(row / R % p.Hkv), b = int(row / R / p.Hkv);
+  const uint32_t row = W == 1 ? blockIdx.x * 4 + (threadIdx.x >> 5) : blockIdx.x;  // at most 2^30 of them
+  if (W == 1 && row >= uint32_t(p.B) * p.Hkv * R) return;
+  const int head = int(row / uint32_t(R)), f = int(row) - head * R, b = head / p.Hkv, h = head - b * p.Hkv;
   const int i = f / p.G, rt = f / p.height, hr = h * p.tiles + rt, heads = p.Hkv * p.tiles;
   T* orow = reinterpret_cast<T*>(p.out) + b * p.ob + i * p.on + (h * p.G + f - i * p.G) * p.oh;
   asm volatile("griddepcontrol.launch_dependents;");
@@ -656,7 +664,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Pa
   }
   const Line line = line_of(p, p.starts[p.B]);
   const int64_t first = int64_t(before) * heads + int64_t(hr) * tiles, last = first + tiles - 1;
-  const int w0 = int(first / line.per), parts = int(last / line.per) - w0 + 1;
+  const int w0 = int(quotient(first, line.per)), parts = int(quotient(last, line.per)) - w0 + 1;
   if (parts == 1) return;
   float m = -INFINITY, l = 0.f;
   alignas(16) float acc[E] = {};
