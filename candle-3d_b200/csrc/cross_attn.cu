@@ -54,7 +54,8 @@ struct Cfg {
   static constexpr int DC = D / 64;
   static constexpr int Q_BYTES = BQ * D * 2, KV_BYTES = BKV * D * 2;
   static constexpr int REST = 512;    // barriers
-  static constexpr int OUT_BYTES = BQ * 128;  // 64 columns of the output on their way to memory
+  // The output of a softmax warp's 32 rows on its way to memory: one place of 64 columns, or two of 32.
+  static constexpr int OUT_COLS = D == 64 ? 64 : 32, OUT_BYTES = BQ * 128;
   static constexpr int BUFS = (226 * 1024 / CTAS - REST - Q_BYTES - OUT_BYTES) / KV_BYTES;
   static constexpr int KST = BUFS / 2, VST = BUFS - KST;
   static constexpr int SMEM = Q_BYTES + BUFS * KV_BYTES + OUT_BYTES + REST;
@@ -201,7 +202,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
   uint8_t* sq = smem_raw;                            // [DC][128 x 64]
   uint8_t* sk = sq + C::Q_BYTES;                     // [KST][DC][64 x 64]
   uint8_t* sv = sk + C::KST * C::KV_BYTES;           // [VST][DC][64 x 64]
-  uint8_t* so = sv + C::VST * C::KV_BYTES;           // [128 x 64]
+  uint8_t* so = sv + C::VST * C::KV_BYTES;           // [4][32 x 64], or [4][2][32 x 32]
   uint64_t* bars = reinterpret_cast<uint64_t*>(so + C::OUT_BYTES);
   uint64_t* k_full = bars;                           // [KST]
   uint64_t* k_empty = k_full + C::KST;               // [KST]
@@ -460,7 +461,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     const int i = p.q_th ? r % p.tpt : r / p.G, g = p.q_th ? r / p.tpt : r - i * p.G;
     const float2 sc2 = f2(p.scale_log2);
     int n = 0, vs = 0, vturn = 0;
-    bool ok = true, stored = false;
+    bool ok = true;
     for (int at = 0; ok && item(at, it); done_with(at++)) {
       const bool valid = i < it.rows && g < p.G;
       const bool active = __any_sync(0xffffffffu, valid);  // the warp holds rows
@@ -580,21 +581,25 @@ __global__ void __launch_bounds__(THREADS, CTAS)
         }
         continue;
       }
-      // 64 columns of the warp's 32 rows at a time through shared memory, then a TMA store; or, where some of the
-      // rows are no part of the sequence, whole 128-byte lines of four rows per store.  (Each thread storing its
-      // own row took 7,400 clocks an item, of 33,000, lines of four rows 3,300.)
-      uint8_t* stage = so + (warp & 3) * (32 * 128);
+      // OC columns of the warp's 32 rows at a time through shared memory, at D = 128 two places in turn, then a TMA
+      // store; or, where some of the rows are no part of the sequence, whole lines of several rows per store.  (Each
+      // thread storing its own row took 7,400 clocks an item of 18 tiles, of 33,000; one place of 64 columns at
+      // D = 128 3 to 4% of the whole.)
+      constexpr int OC = C::OUT_COLS, ROW = OC * 2, CHUNKS = OC / 8;
+      auto place = [&](int row, int j) { return row * ROW + ((j ^ (OC == 64 ? row & 7 : row >> 1 & 3)) << 4); };
       const uint32_t rows = __ballot_sync(0xffffffffu, valid);
       const bool box = p.o_tma && rows == 0xffffffffu;
       const int t_box = it.row0 + (warp & 3) * 32 / p.G, h_box = it.h * p.G;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 64) {
-        if (stored) {  // the last store has read the stage
-          if (lane == 0) bulk_wait_read0();
-          __syncwarp();
+      for (int c = 0; c < D; c += OC) {
+        uint8_t* stage = so + (warp & 3) * (32 * 128) + (OC == 64 ? 0 : (c & 32) * 64);
+        if (lane == 0) {  // the last store from this place has read it
+          if constexpr (OC == 64) bulk_wait_read0();
+          else bulk_wait_read1();
         }
+        __syncwarp();
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
+        for (int x = 0; x < OC / 32; ++x) {
           float o[32];
           tmem_ld32(t_o + uint32_t(c + 32 * x), o);
 #pragma unroll
@@ -602,28 +607,25 @@ __global__ void __launch_bounds__(THREADS, CTAS)
             float v[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = o[8 * q + e] * inv;
-            *reinterpret_cast<uint4*>(stage + lane * 128 + (((4 * x + q) ^ (lane & 7)) << 4)) = pack(v, T());
+            *reinterpret_cast<uint4*>(stage + place(lane, 4 * x + q)) = pack(v, T());
           }
         }
-        stored = box;
         if (box) {
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
           __syncwarp();
-          if (lane == 0) {
-            tma_store_3d(&map_o, stage, c, p.o_th ? t_box : h_box, p.o_th ? h_box : t_box);
-            bulk_commit();
-          }
-          continue;
-        }
-        __syncwarp();
+          if (lane == 0) tma_store_3d(&map_o, stage, c, p.o_th ? t_box : h_box, p.o_th ? h_box : t_box);
+        } else {
+          __syncwarp();
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-          const int row = 4 * x + (lane >> 3);
-          T* dst = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), row));
-          const uint4 v = *reinterpret_cast<const uint4*>(stage + row * 128 + (((lane & 7) ^ (row & 7)) << 4));
-          if (rows >> row & 1) *reinterpret_cast<uint4*>(dst + c + (lane & 7) * 8) = v;
+          for (int x = 0; x < CHUNKS; ++x) {
+            const int row = 32 / CHUNKS * x + lane / CHUNKS, j = lane % CHUNKS;
+            T* dst = reinterpret_cast<T*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(orow), row));
+            const uint4 v = *reinterpret_cast<const uint4*>(stage + place(row, j));
+            if (rows >> row & 1) *reinterpret_cast<uint4*>(dst + c + j * 8) = v;
+          }
+          __syncwarp();
         }
-        __syncwarp();
+        if (lane == 0) bulk_commit();  // (an empty group where nothing was stored: the places take turns)
       }
     }
     if (lane == 0) bulk_wait0();
@@ -735,9 +737,10 @@ static cudaError_t launch(const CUtensorMap (&maps)[4], const Params& p, int64_t
   return cudaLaunchKernelEx(&cfg, combine_kernel<T, D>, p);
 }
 
-// The map of q or out [T, Hq, D] with boxes of G heads x tpt tokens, the nearer in memory listed first.
+// The map of q or out [T, Hq, D] with boxes of G heads x tpt tokens x 64 columns (or 32), the nearer of
+// heads and tokens in memory listed first.
 static bool make_row_map(CUtensorMap* m, const void* base, int64_t T, int64_t Hq, int64_t D, int64_t st, int64_t sh, int G,
-                       int tpt, int* th) {
+                         int tpt, int cols, int* th) {
   auto fn = encode_fn();
   if (!fn) return false;
   if (T <= 1) st = Hq <= 1 ? D : (sh > 0 ? sh * Hq : D);
@@ -745,11 +748,11 @@ static bool make_row_map(CUtensorMap* m, const void* base, int64_t T, int64_t Hq
   *th = st < sh ? 1 : 0;
   const cuuint64_t dims[3] = {uint64_t(D), uint64_t(*th ? T : Hq), uint64_t(*th ? Hq : T)};
   const cuuint64_t strides[2] = {uint64_t(*th ? st : sh) * 2, uint64_t(*th ? sh : st) * 2};
-  const cuuint32_t box[3] = {64u, uint32_t(*th ? tpt : G), uint32_t(*th ? G : tpt)};
+  const cuuint32_t box[3] = {uint32_t(cols), uint32_t(*th ? tpt : G), uint32_t(*th ? G : tpt)};
   const cuuint32_t es[3] = {1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+            CU_TENSOR_MAP_INTERLEAVE_NONE, cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 }  // namespace cross
@@ -863,11 +866,12 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
   CUtensorMap maps[4];
   p.k_hm = Hkv > 1 && k->strides[1] == 0 ? 0 : 1;
   p.v_hm = Hkv > 1 && v->strides[1] == 0 ? 0 : 1;
-  bool ok = make_row_map(&maps[0], elem_ptr(q), Tq, Hq, D, q->strides[0], q->strides[1], p.G, p.tpt, &p.q_th);
+  bool ok = make_row_map(&maps[0], elem_ptr(q), Tq, Hq, D, q->strides[0], q->strides[1], p.G, p.tpt, 64, &p.q_th);
   // A warp's 32 rows as a box of the output: whole tokens with their heads, listed as the rows are.
   maps[3] = maps[0];
   if (p.parts == 1 && 32 % p.G == 0 && (p.G == 1 || !p.q_th)) {
-    ok = ok && make_row_map(&maps[3], elem_ptr(out), Tq, Hq, D, out->strides[0], out->strides[1], p.G, 32 / p.G, &p.o_th);
+    ok = ok && make_row_map(&maps[3], elem_ptr(out), Tq, Hq, D, out->strides[0], out->strides[1], p.G, 32 / p.G,
+                            D == 64 ? Cfg<64>::OUT_COLS : Cfg<128>::OUT_COLS, &p.o_th);
     p.o_tma = ok && (p.G == 1 || !p.o_th);
   }
   if (Tk > 0)
