@@ -539,7 +539,8 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * score that is NaN or +inf, or a key whose page is not one of the cache, and all
  * rows of a request whose length is more than its table has room for, NaN.  BF16
  * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
- * otherwise free in multiples of 16 bytes (pages and slots not expanded); softmax, sums and probabilities in f32
+ * otherwise free in multiples of 16 bytes (pages and slots not expanded); out may
+ * be q; softmax, sums and probabilities in f32
  * (the latter enter the second product as two 16-bit parts).  scale must be
  * positive, and scale * log2(e) finite. */
 int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,

@@ -534,3 +534,31 @@ def test_front_end_refuses(pkg, ops, dev):
                     (ops.cross_attention, (q, kv, kv, off.cpu()))):
         with pytest.raises(ValueError, match="CUDA"):
             f(*args)
+
+
+@pytest.mark.parametrize("wide", [False, True])
+def test_pages_shared_between_requests_and_caches_laid_out_unlike(ops, dev, wide):
+    """Requests whose first pages are the same ones; keys by slot, values by head; tables with rows apart."""
+    import torch
+
+    r = rng(31)
+    kp = _rand(r, (9, 16, 2, 64), "bf16", dev)
+    vp = _rand(r, (9, 2, 16, 64), "bf16", dev).transpose(1, 2)
+    tab = torch.full((3, 800 if wide else 20), 10 ** 6, dtype=torch.int32, device=dev)
+    tab[:, 1:6] = _ints([[4, 0, 7, 2, 8], [4, 0, 7, 1, 3], [4, 5, 6, 6, 6]], dev)
+    lens = [80, 61, 47]
+    q = _rand(r, (3, 2, 4, 64), "bf16", dev)
+    table = tab[:, 1:] if wide else tab[:, 1:6]
+    out = ops.paged_attention(q, kp, vp, table, _ints(lens, dev), check=True)
+    _check_attention(out, q, kp, vp, table, lens, "bf16")
+
+
+def test_append_and_attend_in_place(ops, dev):
+    """The queries may be written over: append's into the projection's rows, the attention's output over its queries."""
+    import torch
+
+    for lens in ([40, 7], [3000, 900]):
+        q, kp, vp, table, out = _run_attention(ops, dev, lens, 1, 8, 2, 64, 16, wide=lens[0] > 100)
+        got = q.clone()
+        assert ops.paged_attention(got, kp, vp, table, _ints(lens, dev), out=got) is got
+        assert torch.equal(got, out)
