@@ -135,11 +135,18 @@ __device__ __forceinline__ uint32_t transposed(uint32_t a) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+// (Keys and values are the first to leave L2: the parts written meanwhile are read again.)
+__device__ __forceinline__ uint64_t first_to_leave() {
+  uint64_t policy;
+  asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(policy));
+  return policy;
+}
+__device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, uint32_t bar, uint64_t policy, int c0, int c1,
+                                        int c2, int c3) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+      " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy)
       : "memory");
 }
 __device__ __forceinline__ void store16(uint32_t dst, uint32_t v) {
@@ -303,6 +310,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   };
   if (count > 0) look_up();
   int issued = 0, ld_stage = 0;
+  const uint64_t policy = first_to_leave();
   auto issue = [&] {
     if (issued >= count) return;
     // (Only now is the table's entry needed.)
@@ -315,9 +323,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       const uint32_t at = lane * p.box * 128, bar = smem_u32(&full[ld_stage]);
 #pragma unroll
       for (int dc = 0; dc < C::DC; ++dc) {
-        tma_box(kd + dc * C::HALF + at, &map_k, bar, dc * 64, p.kw.hn ? ld_h * p.kw.hm : ld_slot,
+        tma_box(kd + dc * C::HALF + at, &map_k, bar, policy, dc * 64, p.kw.hn ? ld_h * p.kw.hm : ld_slot,
                 p.kw.hn ? ld_slot : ld_h * p.kw.hm, ld_page);
-        tma_box(vd + dc * C::HALF + at, &map_v, bar, dc * 64, p.vw.hn ? ld_h * p.vw.hm : ld_slot,
+        tma_box(vd + dc * C::HALF + at, &map_v, bar, policy, dc * 64, p.vw.hn ? ld_h * p.vw.hm : ld_slot,
                 p.vw.hn ? ld_slot : ld_h * p.vw.hm, ld_page);
       }
     } else if (ld_ok) {  // a page that is none of the cache: K of NaN
