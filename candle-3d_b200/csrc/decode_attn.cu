@@ -678,7 +678,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Pa
   alignas(16) float acc[E] = {};
   // (The first part lies in its warp's second place: it holds the row's first key.)
   auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + f - rt * p.height; };
-  constexpr int U = W == 1 ? 8 : 4;
+  constexpr int U = W == 1 || W == 32 ? 8 : 4;
   for (int k0 = warp; k0 < parts; k0 += W * U) {
     float pl[U];
     Vec v[U];
@@ -764,7 +764,7 @@ size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
 }
 
 template <typename T, int D>
-static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int blocks, cudaStream_t s) {
+static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int blocks, int64_t longest, cudaStream_t s) {
   const bool one = p.total_warps == 0;
   auto k = p.height == 8 ? (one ? decode_kernel<T, D, 1, true> : decode_kernel<T, D, 1, false>)
                          : (one ? decode_kernel<T, D, 2, true> : decode_kernel<T, D, 2, false>);
@@ -784,15 +784,20 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   cfg.dynamicSmemBytes = fixed + (one ? 0 : (p.B + 1) * 4);
   e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], p);
   if (e != cudaSuccess || one) return e;
-  // Warps for a row by the parts that it has on average: one takes eight in a round.  (64 requests, 7 parts: 53.8 us
-  // with one, 54.6 with eight; 12 requests x 12 heads, 12 parts, up to 29: 576 rows 47.2 and 41.3, 144 rows 37.5 with
-  // eight, 34.9 with sixteen.)
-  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G, parts = p.total_warps / (int64_t(p.B) * p.Hkv * p.tiles);
-  const int warps = parts <= 8 ? 1 : rows > 2 * sm_count() ? 8 : 16;
+  // Warps for a row by the parts that it has where the caches are full: one takes eight in a round, sixteen 64,
+  // thirty-two 256.  (64 requests, 7 parts: 53.8 us with one, 54.6 with eight; 12 requests x 12 heads, 13 parts, up to 29:
+  // 576 rows 47.2 with one, 41.3 with eight, 144 rows 37.5 with eight, 34.9 with sixteen; one request x 8 heads, 125
+  // parts: 12.8 with sixteen, 13.3 with thirty-two; 2 x 2 heads, 417 parts: 22.8 and 18.1.)
+  const int64_t rows = int64_t(p.B) * p.Hkv * p.N * p.G, items = int64_t(p.B) * p.Hkv * p.tiles;
+  const int64_t tiles = (longest + tile_keys(D) - 1) / tile_keys(D), per = (items * tiles + p.total_warps - 1) / p.total_warps;
+  const int64_t parts = tiles / (per > MIN_TILES ? per : MIN_TILES);
+  const int warps = parts <= 8 ? 1 : rows > 2 * sm_count() ? 8 : parts <= 160 ? 16 : 32;
   cfg.gridDim = dim3(unsigned(warps > 1 ? rows : (rows + 3) / 4));
   cfg.blockDim = dim3(warps > 1 ? warps * 32 : 128);
   cfg.dynamicSmemBytes = 0;
-  return cudaLaunchKernelEx(&cfg, warps == 1 ? combine_kernel<T, D, 1> : warps == 8 ? combine_kernel<T, D, 8> : combine_kernel<T, D, 16>, p);
+  auto join = warps == 1 ? combine_kernel<T, D, 1> : warps == 8 ? combine_kernel<T, D, 8>
+              : warps == 16 ? combine_kernel<T, D, 16> : combine_kernel<T, D, 32>;
+  return cudaLaunchKernelEx(&cfg, join, p);
 }
 
 int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
@@ -831,9 +836,9 @@ int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, 
         return fail(L3D_E_CUDA, "%s: cuTensorMapEncodeTiled failed", op);
     }
   }
-  const cudaError_t e = f16 ? (kv.D == 64 ? launch_t<__half, 64>(maps, p, blocks, s) : launch_t<__half, 128>(maps, p, blocks, s))
-                            : (kv.D == 64 ? launch_t<__nv_bfloat16, 64>(maps, p, blocks, s)
-                                          : launch_t<__nv_bfloat16, 128>(maps, p, blocks, s));
+  const cudaError_t e = f16 ? (kv.D == 64 ? launch_t<__half, 64>(maps, p, blocks, longest, s) : launch_t<__half, 128>(maps, p, blocks, longest, s))
+                            : (kv.D == 64 ? launch_t<__nv_bfloat16, 64>(maps, p, blocks, longest, s)
+                                          : launch_t<__nv_bfloat16, 128>(maps, p, blocks, longest, s));
   return e == cudaSuccess ? L3D_OK : fail(L3D_E_CUDA, "%s: %s", op, cudaGetErrorString(e));
 }
 
