@@ -23,8 +23,8 @@
 // parts of each row; an item's parts have fixed places.  A row or two per sequence goes to decode_attn.cu instead.
 // Every mbarrier wait is bounded (%globaltimer, 2 s; those for an item 60 s); on expiry the block records an error
 // in the device's status word and stops.
-// Measured: 3 x 31569 rows x 12 heads of 128 over up to 1370 keys 643 us (1060 TFLOP/s, 64% of a plain product; at the
-// power limit 756); 4 x 8192 rows x 16 heads of 64 over up to 1370 keys 198 us (513 TFLOP/s).  A 64-key tile takes an SM
+// Measured: 3 x 31569 rows x 12 heads of 128 over up to 1370 keys 627 us (1087 TFLOP/s, 66% of a plain product; at the
+// power limit 740); 4 x 8192 rows x 16 heads of 64 over up to 1370 keys 194 us (522 TFLOP/s).  A 64-key tile takes an SM
 // some 1000 clocks either way, of which the exponentials need 512: the softmax warps' chain, with the products'
 // round trip (scores of 64 keys read all of Q from shared memory, 384 clocks for 256 of products) partly under it.
 #include <type_traits>

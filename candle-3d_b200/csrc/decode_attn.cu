@@ -747,13 +747,13 @@ static int blocks_for(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
 }
 
 // A block for each head and row tile: as many as run at once, with few tiles for each warp, more the nearer the
-// blocks come to filling the device.  A block's own t tiles a warp take about 5.0 + 1.15 t us; divided over the
-// device, 8.5 us for both kernels and the bytes' time.  At t = 4 for 2, 64, 128 blocks: 9.6, 10.1, 10.1 us alone, 8.6,
-// 12.0, 14.0 divided; at 16 for 16, 128: 22.4, 24.2 and 14.4, 33.2 (but then the longest cache decides alone).
+// blocks come to filling the device.  t tiles a warp, D = 128, us: 8 blocks, t = 2 7.7 alone, 9.8 divided over the device;
+// 8, 4 9.8, 10.0; 32, 4 10.1, 10.6; 32, 6 12.1, 11.9; 64, 4 9.9, 11.6; 64, 6 12.1, 13.7; 128, 8 15.0, 20.5; 128, 16 24.2,
+// 30.9; but 16, 16 22.4, 14.0, and alone the longest cache decides, so that t stays small.
 static bool alone(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
   const int64_t h = height_for(N * G);
   const int64_t blocks = B * Hkv * ((N * G + h - 1) / h), stretch = WARPS * tile_keys(int(D));
-  return blocks <= sm_count() && longest <= (3 + blocks / 24) * stretch;
+  return blocks <= sm_count() && longest <= (4 + blocks / 24) * stretch;
 }
 
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D) {
