@@ -692,11 +692,12 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   else *reinterpret_cast<uint32_t*>(orow) = *reinterpret_cast<const uint32_t*>(o);
 }
 
-// Parts of an item: none cut while the items fill the device; else as many as its blocks take, of four key
-// tiles at least by the keys' average.
+// Parts of an item: as many as two rounds of the device take, for an item's time is that of its keys (some 0.7 us a
+// tile) however few items there are; of four key tiles at least by the keys' average.  (2 x up to 1273 rows x 16 / 4
+// heads of 64 over up to 3299 keys: 43 us whole, @@ in parts.)
 static int parts_for(int64_t B, int64_t Tq, int64_t Tk, int64_t G, int64_t Hkv) {
   const int64_t tpt = BQ / G, items = Hkv * (Tq / tpt + B), tiles = (Tk / B + BKV - 1) / BKV;
-  int64_t parts = CTAS * int64_t(sm_count()) / items;
+  int64_t parts = 2 * CTAS * int64_t(sm_count()) / items;
   if (parts > tiles / 4) parts = tiles / 4;
   return int(parts < 1 ? 1 : parts > MAX_PARTS ? MAX_PARTS : parts);
 }

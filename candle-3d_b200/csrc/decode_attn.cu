@@ -257,14 +257,32 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     }
     if (threadIdx.x == WARPS * 32 - 1) starts[p.B] = at;  // (its stretch is the last, or empty)
     __syncthreads();
-    if (blockIdx.x == 0)
+    if (p.edges) {  // rows without keys, which no warp comes to
+      for (int b = blockIdx.x; b < p.B; b += gridDim.x) {
+        if (starts[b + 1] != starts[b]) continue;
+        bool bad;
+        length_of(p, b, &bad);
+        const int Hq = p.Hkv * p.G;
+        for (int x = threadIdx.x; x < p.N * Hq * D; x += WARPS * 32) {
+          const int row = x / D, i = row / Hq;
+          reinterpret_cast<T*>(p.out)[b * p.ob + i * p.on + (row - i * Hq) * p.oh + x % D] =
+              from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
+        }
+      }
+    } else if (blockIdx.x == 0) {
       for (int b = threadIdx.x; b <= p.B; b += WARPS * 32) p.starts[b] = starts[b];
+    }
   }
+  int64_t per = 0;  // tiles of a warp
   if constexpr (!ALONE) {
     const Line line = line_of(p, starts[p.B]);
-    x0 = int64_t(me) * line.per;
-    if (x0 >= line.total) return;
-    count = int(min(line.per, line.total - x0));
+    per = line.per;
+    x0 = int64_t(me) * per;
+    if (x0 >= line.total) {
+      if (p.edges && lane == 0) p.edges[me] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    count = int(min(per, line.total - x0));
   } else {
     __syncthreads();  // (the barriers are there)
   }
@@ -600,6 +618,10 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       }
     }
     if (n + 1 < count) cu.next(starts, heads);
+    else if (!ALONE && p.edges && lane == 0) {  // the item that begins in this stretch and goes on behind it, if any
+      const int rest = cu.tiles - (cu.t + 1);
+      p.edges[me] = make_int4(cu.b, cu.hr, t_first == 0 && rest > 0 ? 1 + int((rest + per - 1) / per) : 0, 0);
+    }
   }
   if (!ok && lane == 0) {  // the newest load of each stage: no copy may be in flight when the block exits
     for (int i = max(issued - C::STAGES, 0); i < issued; ++i)
@@ -642,13 +664,66 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   }
 }
 
-// The parts of each row weighed by 2^(their log2 sum - the largest), in a fixed order: W warps for a row, with
-// every W-th part each, D / 32 elements per lane; a block of 4 rows where one warp does.  Rows without keys are
-// zeroed here, and no others touched that one warp has finished.
+// A running sum of parts, each weighed by 2^(its log2 sum - the largest): D / 32 elements per lane.
+template <int D>
+struct Joined {
+  static constexpr int E = D / 32;
+  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  float m = -INFINITY, l = 0.f;
+  alignas(16) float acc[E] = {};
+  // Parts k0, k0 + step, .. up to `parts`, U of them at a time.  The first part lies in its warp's second place: it
+  // holds the row's first key.
+  template <int U>
+  __device__ __forceinline__ void add(const Params& p, int w0, int parts, int r, int k0, int step) {
+    const int lane = threadIdx.x & 31;
+    auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + r; };
+    for (; k0 < parts; k0 += step * U) {
+      float pl[U];
+      Vec v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int k = k0 + u * step;
+        pl[u] = k < parts ? p.part_l[row_at(k)] : -INFINITY;
+        v[u] = reinterpret_cast<const Vec*>(p.part_o + row_at(k < parts ? k : k0) * D)[lane];
+      }
+      float mx = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mx = max_nan(mx, pl[u]);
+      if (mx == -INFINITY) continue;
+      const float a = exp2f(m - mx);
+      l *= a;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= a;
+      m = mx;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (pl[u] == -INFINITY) continue;
+        const float wgt = exp2f(pl[u] - m);
+        l += wgt;
+        const float* vv = reinterpret_cast<const float*>(&v[u]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(wgt, vv[e], acc[e]);
+      }
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ void store(T* orow) const {
+    const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
+    alignas(8) T o[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = from_f<T>(acc[e] * inv);
+    orow += (threadIdx.x & 31) * E;
+    if constexpr (E == 4) *reinterpret_cast<uint2*>(orow) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint32_t*>(orow) = *reinterpret_cast<const uint32_t*>(o);
+  }
+};
+
+// The parts of each row joined, in a fixed order: W warps for a row, with every W-th part each; a block of 4 rows
+// where one warp does.  Rows without keys are zeroed here, and no others touched that one warp has finished.
 template <typename T, int D, int W>
 __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Params p) {
-  constexpr int E = D / 32, KT = tile_keys(D);
-  using Vec = typename std::conditional<E == 4, float4, float2>::type;
+  constexpr int E = D / 32;
+  using Vec = typename Joined<D>::Vec;
   __shared__ alignas(16) float red[W][D];
   __shared__ float red_m[W], red_l[W];
   const int lane = threadIdx.x & 31, warp = W == 1 ? 0 : threadIdx.x >> 5;
@@ -674,65 +749,47 @@ __global__ void __launch_bounds__(W == 1 ? 128 : W * 32) combine_kernel(const Pa
   const int64_t first = int64_t(before) * heads + int64_t(hr) * tiles, last = first + tiles - 1;
   const int w0 = int(quotient(first, line.per)), parts = int(quotient(last, line.per)) - w0 + 1;
   if (parts == 1) return;
-  float m = -INFINITY, l = 0.f;
-  alignas(16) float acc[E] = {};
-  // (The first part lies in its warp's second place: it holds the row's first key.)
-  auto row_at = [&](int k) { return (2 * int64_t(w0 + k) + (k == 0 ? 1 : 0)) * p.rows + f - rt * p.height; };
-  constexpr int U = W == 1 || W == 32 ? 8 : 4;
-  for (int k0 = warp; k0 < parts; k0 += W * U) {
-    float pl[U];
-    Vec v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = k0 + u * W;
-      pl[u] = k < parts ? p.part_l[row_at(k)] : -INFINITY;
-      v[u] = reinterpret_cast<const Vec*>(p.part_o + row_at(k < parts ? k : k0) * D)[lane];
-    }
-    float mx = m;
-#pragma unroll
-    for (int u = 0; u < U; ++u) mx = max_nan(mx, pl[u]);
-    if (mx == -INFINITY) continue;
-    const float a = exp2f(m - mx);
-    l *= a;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= a;
-    m = mx;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (pl[u] == -INFINITY) continue;
-      const float wgt = exp2f(pl[u] - m);
-      l += wgt;
-      const float* vv = reinterpret_cast<const float*>(&v[u]);
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(wgt, vv[e], acc[e]);
-    }
-  }
+  Joined<D> sum;
+  sum.template add<W == 1 || W == 32 ? 8 : 4>(p, w0, parts, f - rt * p.height, warp, W);
   if constexpr (W == 1) {
-    const float inv = l > 0.f ? 1.f / l : l == l ? 0.f : l;
-    alignas(8) T o[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = from_f<T>(acc[e] * inv);
-    if constexpr (E == 4) *reinterpret_cast<uint2*>(orow + lane * E) = *reinterpret_cast<const uint2*>(o);
-    else *reinterpret_cast<uint32_t*>(orow + lane * E) = *reinterpret_cast<const uint32_t*>(o);
+    sum.store(orow);
     return;
   }
-  *reinterpret_cast<Vec*>(&red[warp][lane * E]) = *reinterpret_cast<const Vec*>(acc);
+  *reinterpret_cast<Vec*>(&red[warp][lane * E]) = *reinterpret_cast<const Vec*>(sum.acc);
   if (lane == 0) {
-    red_m[warp] = m;
-    red_l[warp] = l;
+    red_m[warp] = sum.m;
+    red_l[warp] = sum.l;
   }
   __syncthreads();
   for (int d = threadIdx.x; d < D; d += W * 32) {
-    float mx = -INFINITY, sum = 0.f, val = 0.f;
+    float mx = -INFINITY, all = 0.f, val = 0.f;
     for (int w = 0; w < W; ++w) mx = max_nan(mx, red_m[w]);
     if (mx != -INFINITY)
       for (int w = 0; w < W; ++w) {
         if (red_m[w] == -INFINITY) continue;
         const float wgt = exp2f(red_m[w] - mx);
-        sum = fmaf(wgt, red_l[w], sum);
+        all = fmaf(wgt, red_l[w], all);
         val = fmaf(wgt, red[w][d], val);
       }
-    orow[d] = from_f<T>(sum > 0.f ? val / sum : sum == sum ? 0.f : sum);
+    orow[d] = from_f<T>(all > 0.f ? val / all : all == all ? 0.f : all);
+  }
+}
+
+// The same where there are more heads and row tiles than warps: few of them are divided at all, at most one per
+// end of a warp's stretch, and those are listed there.  A block per end, a row per warp.  (Looking at every row took
+// 90 of 119 us for 237 requests x 16 heads x 64 rows of 3 keys.)
+template <typename T, int D>
+__global__ void __launch_bounds__(128) combine_edges_kernel(const Params p) {
+  asm volatile("griddepcontrol.launch_dependents;");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 edge = p.edges[blockIdx.x];  // request, head and row tile, parts
+  if (edge.z == 0) return;
+  const int h = edge.y / p.tiles, f0 = (edge.y - h * p.tiles) * p.height;
+  for (int r = threadIdx.x >> 5; r < p.rows && f0 + r < p.N * p.G; r += 4) {
+    const int i = (f0 + r) / p.G;
+    Joined<D> sum;
+    sum.template add<8>(p, blockIdx.x, edge.z, r, 0, 1);
+    sum.store(reinterpret_cast<T*>(p.out) + edge.x * p.ob + i * p.on + (h * p.G + f0 + r - i * p.G) * p.oh);
   }
 }
 
@@ -760,7 +817,7 @@ size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t long
   if (B <= 0 || N <= 0 || G <= 0 || Hkv <= 0 || longest < 0 || D <= 0 || alone(B, N, G, Hkv, longest, D)) return 0;
   const int64_t h = height_for(N * G), rows = N * G < h ? N * G : h;
   const int64_t parts = 2 * int64_t(blocks_for(B, N, G, Hkv, longest, D)) * WARPS;
-  return (size_t(B + 1) * 4 + 255) / 256 * 256 + (size_t(parts * rows) * 4 + 255) / 256 * 256 + size_t(parts * rows * D) * 4;
+  return (size_t(B + 1) * 4 + 255) / 256 * 256 + size_t(parts) * 8 + (size_t(parts * rows) * 4 + 255) / 256 * 256 + size_t(parts * rows * D) * 4;
 }
 
 template <typename T, int D>
@@ -784,6 +841,12 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   cfg.dynamicSmemBytes = fixed + (one ? 0 : (p.B + 1) * 4);
   e = cudaLaunchKernelEx(&cfg, k, maps[0], maps[1], p);
   if (e != cudaSuccess || one) return e;
+  if (p.edges) {
+    cfg.gridDim = dim3(unsigned(p.total_warps));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    return cudaLaunchKernelEx(&cfg, combine_edges_kernel<T, D>, p);
+  }
   // Warps for a row by the parts that it has where the caches are full: one takes eight in a round, sixteen 64,
   // thirty-two 256.  (64 requests, 7 parts: 53.8 us with one, 54.6 with eight; 12 requests x 12 heads, 13 parts, up to 29:
   // 576 rows 47.2 with one, 41.3 with eight, 144 rows 37.5 with eight, 34.9 with sixteen; one request x 8 heads, 125
@@ -812,6 +875,8 @@ int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, 
   char* w = static_cast<char*>(workspace);
   p.starts = reinterpret_cast<int*>(w);
   w += (size_t(p.B + 1) * 4 + 255) / 256 * 256;
+  p.edges = int64_t(p.B) * p.Hkv * p.tiles > p.total_warps ? reinterpret_cast<int4*>(w) : nullptr;
+  w += size_t(p.total_warps) * 16;
   p.part_l = reinterpret_cast<float*>(w);
   w += (size_t(2) * p.total_warps * p.rows * 4 + 255) / 256 * 256;
   p.part_o = reinterpret_cast<float*>(w);

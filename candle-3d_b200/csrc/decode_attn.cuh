@@ -36,7 +36,8 @@ struct Params {
   int height, tiles, rows;      // rows of a row tile, row tiles of a key head, rows of a tile's part
   int total_warps;              // 0: a block for each head and row tile
   uint64_t wait_ns;
-  int* starts;                  // workspace: key tiles before each sequence [B + 1]
+  int* starts;                  // workspace: key tiles before each sequence [B + 1],
+  int4* edges;                  // the item divided at the end of each warp's stretch [warps], where items outnumber warps,
   float *part_l, *part_o;       // [2 warps, rows], [2 warps, rows, D]
 };
 
