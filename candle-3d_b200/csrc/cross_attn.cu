@@ -566,16 +566,25 @@ __global__ void __launch_bounds__(THREADS, CTAS)
       if (p.parts > 1 && valid) p.part_l[pr] = l > 0.f ? m + log2f(l) : l == l ? -INFINITY : l;
       T* orow = static_cast<T*>(p.out) + token * p.ot + int64_t(it.h * p.G + g) * p.oh;
       __syncwarp();  // the loads from tensor memory are the whole warp's
-      if (p.parts > 1) {
+      const uint32_t rows = __ballot_sync(0xffffffffu, valid);
+      if (p.parts > 1) {  // 16 columns at a time through shared memory, 64 bytes of eight rows per store
+        uint8_t* stage = so + (warp & 3) * (32 * 128);
+        float* prow = p.part_o + pr * D;
 #pragma unroll 1
-        for (int c = 0; c < D; c += 32) {
-          float o[32];
-          tmem_ld32(t_o + uint32_t(c), o);
-          if (valid) {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + pr * D + c);
+        for (int c = 0; c < D; c += 16) {
+          float o[16];
+          tmem_ld16(t_o + uint32_t(c), o);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              dst[e] = make_float4(o[4 * e] * inv, o[4 * e + 1] * inv, o[4 * e + 2] * inv, o[4 * e + 3] * inv);
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<float4*>(stage + lane * 64 + ((q ^ (lane >> 1 & 3)) << 4)) =
+                make_float4(o[4 * q] * inv, o[4 * q + 1] * inv, o[4 * q + 2] * inv, o[4 * q + 3] * inv);
+          __syncwarp();
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int row = 8 * x + (lane >> 2);
+            float* dst = reinterpret_cast<float*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(prow), row));
+            const float4 v = *reinterpret_cast<const float4*>(stage + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
+            if (rows >> row & 1) *reinterpret_cast<float4*>(dst + c + (lane & 3) * 4) = v;
           }
           __syncwarp();
         }
@@ -587,7 +596,6 @@ __global__ void __launch_bounds__(THREADS, CTAS)
       // D = 128 3 to 4% of the whole.)
       constexpr int OC = C::OUT_COLS, ROW = OC * 2, CHUNKS = OC / 8;
       auto place = [&](int row, int j) { return row * ROW + ((j ^ (OC == 64 ? row & 7 : row >> 1 & 3)) << 4); };
-      const uint32_t rows = __ballot_sync(0xffffffffu, valid);
       const bool box = p.o_tma && rows == 0xffffffffu;
       const int t_box = it.row0 + (warp & 3) * 32 / p.G, h_box = it.h * p.G;
 #pragma unroll 1
@@ -694,7 +702,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
 
 // Parts of an item: as many as two rounds of the device take, for an item's time is that of its keys (some 0.7 us a
 // tile) however few items there are; of four key tiles at least by the keys' average.  (2 x up to 1273 rows x 16 / 4
-// heads of 64 over up to 3299 keys: 43 us whole, @@ in parts.)
+// heads of 64 over up to 3299 keys: 41 us whole, 32 in two parts.)
 static int parts_for(int64_t B, int64_t Tq, int64_t Tk, int64_t G, int64_t Hkv) {
   const int64_t tpt = BQ / G, items = Hkv * (Tq / tpt + B), tiles = (Tk / B + BKV - 1) / BKV;
   int64_t parts = 2 * CTAS * int64_t(sm_count()) / items;
