@@ -27,8 +27,8 @@
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
 // status word and stops.
-// Measured, D = 128: 8 x 65536 keys x 4 heads 170 us (6.31 TB/s, 96% of a plain copy); 64 x up to 4096 keys x 4 heads
-// 53 us (4.56 TB/s): 3.7 us until the first loads go out, 4 for the second kernel.  One request of 300 keys x 2 heads of
+// Measured, D = 128: 8 x 65536 keys x 4 heads 171 us (6.28 TB/s, 96% of a plain copy); 64 x up to 4096 keys x 4 heads
+// 50 us (4.86 TB/s): 3.7 us until the first loads go out, 2 for the second kernel.  One request of 300 keys x 2 heads of
 // 64: 5.7 us.
 #include <type_traits>
 
