@@ -823,8 +823,9 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
   if (Tq * Hq == 0 || B == 0) return L3D_OK;
   for (const l3d_tensor* t : {k, v})
     if (Tk > 1 && t->strides[0] == 0) return fail(L3D_E_ALIGN, "%s: the keys must not be expanded (stride 0)", op);
-  if ((Tq > 1 && q->strides[0] == 0) || (Hq > 1 && q->strides[1] == 0))
-    return fail(L3D_E_ALIGN, "%s: q must not be expanded (stride 0)", op);
+  for (const l3d_tensor* t : {q, out})
+    if ((Tq > 1 && t->strides[0] == 0) || (Hq > 1 && t->strides[1] == 0))
+      return fail(L3D_E_ALIGN, "%s: q and out must not be expanded (stride 0)", op);
   const size_t need = l3d_cross_attention_workspace_size(B, Tq, Tk, Hq, Hkv, D, q_offsets != nullptr);
   if (need && (!workspace || workspace_bytes < need))
     return fail(L3D_E_WORKSPACE, "%s: workspace of %zu bytes required", op, need);

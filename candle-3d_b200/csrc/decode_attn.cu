@@ -984,6 +984,8 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
   for (const l3d_tensor* t : {k_pages, v_pages})
     if ((pages > 1 && t->strides[0] == 0) || (size > 1 && t->strides[1] == 0))
       return fail(L3D_E_ALIGN, "%s: the pages must not be expanded (stride 0)", op);
+  for (int d = 0; d < 3; ++d)
+    if (out->dims[d] > 1 && out->strides[d] == 0) return fail(L3D_E_ALIGN, "%s: out must not be expanded (stride 0)", op);
   if (no_data(table) || no_data(lengths)) return fail(L3D_E_NULL, "%s: null data pointer", op);
   l3d::decode::Params p{};
   p.B = int(B); p.N = int(N); p.G = int(Hq / Hkv); p.Hkv = int(Hkv);

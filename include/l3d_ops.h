@@ -539,7 +539,7 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * score that is NaN or +inf, or a key whose page is not one of the cache, and all
  * rows of a request whose length is more than its table has room for, NaN.  BF16
  * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
- * otherwise free in multiples of 16 bytes (pages and slots not expanded); out may
+ * otherwise free in multiples of 16 bytes (pages, slots and out not expanded); out may
  * be q; softmax, sums and probabilities in f32
  * (the latter enter the second product as two 16-bit parts).  scale must be
  * positive, and scale * log2(e) finite. */
@@ -564,8 +564,8 @@ size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int
  * hold.  Hq a multiple of Hkv, at most 128 times as many, query head h reading key
  * head h / (Hq / Hkv).  A row with no keys gives zeros, one that sees a score
  * that is NaN or +inf NaN.  BF16 or F16, D = 64 or 128, head dim contiguous,
- * strides otherwise free in multiples of 16 bytes (keys and q not expanded along
- * the rows); softmax and sums in f32, probabilities rounded to the input type for
+ * strides otherwise free in multiples of 16 bytes (keys not expanded along the rows,
+ * q and out not at all); softmax and sums in f32, probabilities rounded to the input type for
  * the second product (not where every sequence has N rows and N * Hq / Hkv is at
  * most 16: they then enter as two 16-bit parts).  scale must be positive, and
  * scale * log2(e) finite. */

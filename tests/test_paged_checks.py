@@ -105,6 +105,8 @@ def _paged_args(**over):
     (dict(workspace=264), E_ALIGN, "256"),
     (dict(k_pages=_zeros(7, 16, 2, 68)[..., :64]), E_ALIGN, "multiples of 16"),
     (dict(k_pages=_zeros(1, 16, 2, 64).expand(7, 16, 2, 64)), E_ALIGN, "expanded"),
+    (dict(out=_zeros(3, 2, 1, 64).expand(3, 2, 4, 64)), E_ALIGN, "out must not be expanded"),
+    (dict(out=_zeros(1, 2, 4, 64).expand(3, 2, 4, 64)), E_ALIGN, "out must not be expanded"),
 ])
 def test_paged_attention_refuses(pkg, over, code, word):
     _refused(pkg, "l3d_paged_attention", _paged_args(**over), code, word)
@@ -189,6 +191,8 @@ def _cross_args(**over):
     (dict(q=_zeros(60, 258, 64), out=_zeros(60, 258, 64)), E_UNSUPPORTED, "128 query heads"),
     (dict(k=_zeros(1, 2, 64).expand(40, 2, 64)), E_ALIGN, "expanded"),
     (dict(q=_zeros(60, 1, 64).expand(60, 4, 64)), E_ALIGN, "expanded"),
+    (dict(out=_zeros(60, 1, 64).expand(60, 4, 64)), E_ALIGN, "out must not be expanded"),
+    (dict(out=_zeros(1, 4, 64).expand(60, 4, 64)), E_ALIGN, "out must not be expanded"),
     (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), bytes=0), E_WORKSPACE, "workspace"),
     (dict(k=_zeros(4096, 2, 64), v=_zeros(4096, 2, 64), workspace=264), E_ALIGN, "256"),
     (dict(q_offsets=None, q=_zeros(3, 4, 64), out=_zeros(3, 4, 64), k=_zeros(9000, 2, 64), v=_zeros(9000, 2, 64),
