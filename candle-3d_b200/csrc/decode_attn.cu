@@ -263,8 +263,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         bool bad;
         length_of(p, b, &bad);
         const int Hq = p.Hkv * p.G;
-        for (int x = threadIdx.x; x < p.N * Hq * D; x += WARPS * 32) {
-          const int row = x / D, i = row / Hq;
+        for (int64_t x = threadIdx.x; x < int64_t(p.N) * Hq * D; x += WARPS * 32) {
+          const int row = int(x / D), i = row / Hq;
           reinterpret_cast<T*>(p.out)[b * p.ob + i * p.on + (row - i * Hq) * p.oh + x % D] =
               from_f<T>(bad ? __int_as_float(0x7fffffff) : 0.f);
         }

@@ -553,6 +553,19 @@ def test_pages_shared_between_requests_and_caches_laid_out_unlike(ops, dev, wide
     _check_attention(out, q, kp, vp, table, lens, "bf16")
 
 
+def test_elements_past_32_bits_without_keys(ops, dev):
+    """2^31 elements of a request without keys come out zero; of the other one the last row sees a key."""
+    import torch
+
+    N, H, D = 16384, 1024, 128
+    q = torch.full((2, N, H, D), 7.0, dtype=torch.bfloat16, device=dev)
+    k, v = (_rand(rng(i), (1, 16, 1, D), "bf16", dev) for i in range(2))
+    table = torch.zeros((2, 1), dtype=torch.int32, device=dev)
+    ops.paged_attention(q, k, v, table, _ints([0, 1], dev), out=q, check=True)
+    assert not q[0].any() and not q[1, :-1].any()
+    assert torch.equal(q[1, -1], v[0, 0].expand(H, D))
+
+
 def test_append_and_attend_in_place(ops, dev):
     """The queries may be written over: append's into the projection's rows, the attention's output over its queries."""
     import torch
