@@ -673,9 +673,9 @@ __global__ void __launch_bounds__(128) combine_kernel(const Params p) {
   const int64_t rows = int64_t(p.Tq) * Hq, row = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 5);
   if (row >= rows) return;
   const int64_t token = row / Hq;
-  if (!p.N && (token < offset_at(p.q_offsets, p.q64, 0, p.Tq) || token >= offset_at(p.q_offsets, p.q64, p.B, p.Tq)))
-    return;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const bool none = !p.N && (token < offset_at(p.q_offsets, p.q64, 0, p.Tq) || token >= offset_at(p.q_offsets, p.q64, p.B, p.Tq));
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (of rows of no sequence too: the kernel ends after the one before)
+  if (none) return;
   float w = lane < p.parts ? p.part_l[lane * rows + row] : -INFINITY, mx = w;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
