@@ -43,6 +43,9 @@ constexpr int BQ = 128, BKV = 64, THREADS = 256, CTAS = 2;
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 constexpr float RESCALE_LOG2 = 8.f;   // as in attn.cu
 constexpr int MAX_PARTS = 16;
+// Sequences, and key heads of them all: while a block passes over items without rows or keys, its other warps wait
+// for the next one, and those waits are bounded (2 s).  2^20 sequences without rows or keys x 64 heads: 110 ms.
+constexpr int64_t MAX_BATCH = int64_t(1) << 20, MAX_HEADS = int64_t(1) << 26;
 // Places of the list of items: the one that is looked for while up to three before it are not done with (the one
 // whose last product was just issued, and two of a tile each whose scores were).
 constexpr int LISTED = 4;
@@ -817,8 +820,8 @@ extern "C" int l3d_cross_attention(const l3d_tensor* q, const l3d_tensor* k, con
   if (!(scale > 0.f) || !(scale_log2 < INFINITY))
     return fail(L3D_E_UNSUPPORTED, "%s: scale must be positive and finite", op);
   const int64_t big = int64_t(1) << 30;
-  if (Tq > big || Tk > big || B > big || Hq > 65535 || Tq * Hq > big || Hkv * (B + Tq) > big)
-    return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large", op);
+  if (Tq > big || Tk > big || B > MAX_BATCH || Hq > 65535 || Tq * Hq > big || Hkv * B > MAX_HEADS || Hkv * Tq > big)
+    return fail(L3D_E_UNSUPPORTED, "%s: dimensions too large (at most 2^20 sequences, 2^26 times their key heads)", op);
   if (Hkv > 0 && Hq / Hkv > BQ) return fail(L3D_E_UNSUPPORTED, "%s: at most %d query heads per key head", op, BQ);
   if (Tq * Hq == 0 || B == 0) return L3D_OK;
   for (const l3d_tensor* t : {k, v})

@@ -562,7 +562,7 @@ size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int
  * decreasing, clamped to the rows there are; rows of out that belong to no
  * sequence are left as they were, and keys of none are never used, whatever they
  * hold.  Hq a multiple of Hkv, at most 128 times as many, query head h reading key
- * head h / (Hq / Hkv).  A row with no keys gives zeros, one that sees a score
+ * head h / (Hq / Hkv); at most 2^20 sequences, and 2^26 key heads of all of them.  A row with no keys gives zeros, one that sees a score
  * that is NaN or +inf NaN.  BF16 or F16, D = 64 or 128, head dim contiguous,
  * strides otherwise free in multiples of 16 bytes (keys not expanded along the rows,
  * q and out not at all); softmax and sums in f32, probabilities rounded to the input type for

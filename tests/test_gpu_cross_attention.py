@@ -137,6 +137,27 @@ def test_many_sequences(ops, dev, B):
     _run(ops, dev, rows, keys, 2, 1, 64, layout="head")
 
 
+@pytest.mark.parametrize("empty", ["rows", "keys"])
+def test_most_sequences_most_of_them_empty(ops, dev, empty):
+    """2^20 sequences x 64 heads, all but the last two without rows, or without keys."""
+    import torch
+
+    B, H, D = 1 << 20, 64, 64
+    r = rng(5)
+    front = 0 if empty == "rows" else 4096  # rows of sequences without keys, one for each 256th
+    q, k, v = (_rand(r, (n, H, D), "bf16", dev) for n in (front + 64, 90, 90))
+    qo, ko = (torch.zeros(B + 1, dtype=torch.int32, device=dev) for _ in range(2))
+    if front:
+        qo[:] = (torch.arange(B + 1, device=dev) // 256).clamp_max(front)
+    a, b, c = front, front + 30, front + 64
+    qo[-3:] = _ints([a, b, c], dev)
+    ko[-2:] = _ints([50, 90], dev)
+    out = torch.full_like(q, 7.0)
+    ops.cross_attention(q, k, v, ko, qo, out=out, check=True)
+    _check(out, q, k, v, [(a, b), (b, c)], [(0, 50), (50, 90)], "bf16")
+    assert not out[:a].any()
+
+
 def test_parts_along_the_keys(ops, dev):
     """Few rows, many keys: an item's keys are cut into parts; ragged, so that some parts are empty."""
     for D in (64, 128):

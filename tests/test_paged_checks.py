@@ -185,6 +185,10 @@ def _cross_args(**over):
     (dict(q_offsets=_zeros(5, dtype="int32")), E_SHAPE, "q_offsets"),
     (dict(q_offsets=None, k_offsets=_zeros(8, dtype="int32")), E_SHAPE, "divide evenly"),
     (dict(q_offsets=None, k_offsets=_zeros(1, dtype="int32")), E_SHAPE, "divide evenly"),
+    (dict(q_offsets=None, k_offsets=_zeros((1 << 20) + 2, dtype="int32"), q=_zeros(0, 4, 64), out=_zeros(0, 4, 64)),
+     E_UNSUPPORTED, "2^20 sequences"),
+    (dict(k_offsets=_zeros((1 << 20) + 1, dtype="int32"), q_offsets=_zeros((1 << 20) + 1, dtype="int32"),
+          q=_zeros(1, 65, 64), out=_zeros(1, 65, 64), k=_zeros(1, 65, 64), v=_zeros(1, 65, 64)), E_UNSUPPORTED, "2^26"),
     (dict(scale=-1.0), E_UNSUPPORTED, "scale"),
     (dict(scale=math.nan), E_UNSUPPORTED, "scale"),
     (dict(scale=3e38), E_UNSUPPORTED, "scale"),
