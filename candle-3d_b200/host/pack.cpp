@@ -8,6 +8,7 @@
 #include <ATen/ATen.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 
 #include <exception>
 
@@ -181,21 +182,18 @@ PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const double eps = PyFloat_AsDouble(a[2]);
     const long half = PyLong_AsLong(a[3]);
     if (PyErr_Occurred()) return nullptr;
-    PyObject* out = out_or_new(a[15], a[4]);
+    THPObjectPtr out(out_or_new(a[15], a[4]));
     if (!out) return nullptr;
     PyObject* args[14];
-    for (int i = 0; i < 14; ++i) args[i] = i == 11 ? out : a[4 + i];
+    for (int i = 0; i < 14; ++i) args[i] = i == 11 ? out.get() : a[4 + i];
     Descriptors<14> d;
-    if (!d.fill(args)) {
-      Py_DECREF(out);
-      return nullptr;
-    }
+    if (!d.fill(args)) return nullptr;
     const auto& p = d.ptr;
     return result(without_lock([&] {
                     return fn(p[0], p[1], p[2], p[3], p[4], float(eps), p[5], p[6], int(half), p[7], p[8], p[9], p[10],
                               p[11], p[12], p[13], stream);
                   }),
-                  out);
+                  out.release());
   });
 }
 
@@ -214,14 +212,11 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto stream = entry<l3d_stream>(a[2]);
     const double scale = PyFloat_AsDouble(a[3]);
     if (PyErr_Occurred()) return nullptr;
-    PyObject* out = out_or_new(a[9], a[4]);
+    THPObjectPtr out(out_or_new(a[9], a[4]));
     if (!out) return nullptr;
-    PyObject* args[6] = {a[4], a[5], a[6], a[7], a[8], out};
+    PyObject* args[6] = {a[4], a[5], a[6], a[7], a[8], out.get()};
     Descriptors<6> d;
-    if (!d.fill(args)) {
-      Py_DECREF(out);
-      return nullptr;
-    }
+    if (!d.fill(args)) return nullptr;
     for (int i : {0, 5}) {  // one token each: [B, H, D] as [B, 1, H, D]
       l3d_tensor& t = d.at[i];
       if (!d.ptr[i] || t.ndim != 3) continue;
@@ -237,10 +232,10 @@ PyObject* paged_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
       need = size(d.at[0].dims[0], d.at[0].dims[2], d.at[1].dims[2], d.at[0].dims[1], d.at[3].dims[1] * d.at[1].dims[1],
                   d.at[0].dims[3]);
     at::Tensor ws;
-    if (need) ws = workspace_for(out, need);
+    if (need) ws = workspace_for(out.get(), need);
     void* wp = need ? ws.data_ptr() : nullptr;
     const auto& p = d.ptr;
-    return result(without_lock([&] { return fn(p[0], p[1], p[2], p[3], p[4], float(scale), p[5], wp, need, stream); }), out);
+    return result(without_lock([&] { return fn(p[0], p[1], p[2], p[3], p[4], float(scale), p[5], wp, need, stream); }), out.release());
   });
 }
 
@@ -253,23 +248,20 @@ PyObject* cross_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const auto stream = entry<l3d_stream>(a[2]);
     const double scale = PyFloat_AsDouble(a[3]);
     if (PyErr_Occurred()) return nullptr;
-    PyObject* out = out_or_new(a[9], a[4]);
+    THPObjectPtr out(out_or_new(a[9], a[4]));
     if (!out) return nullptr;
-    PyObject* args[6] = {a[4], a[5], a[6], a[7], a[8], out};
+    PyObject* args[6] = {a[4], a[5], a[6], a[7], a[8], out.get()};
     Descriptors<6> d;
-    if (!d.fill(args)) {
-      Py_DECREF(out);
-      return nullptr;
-    }
+    if (!d.fill(args)) return nullptr;
     size_t need = 0;
     if (d.ptr[0] && d.ptr[1] && d.ptr[3] && d.at[0].ndim == 3 && d.at[1].ndim == 3 && d.at[3].ndim == 1)  // (else refused)
       need = size(d.at[3].dims[0] - 1, d.at[0].dims[0], d.at[1].dims[0], d.at[0].dims[1], d.at[1].dims[1], d.at[0].dims[2],
                   d.ptr[4] != nullptr);
     at::Tensor ws;
-    if (need) ws = workspace_for(out, need);
+    if (need) ws = workspace_for(out.get(), need);
     void* wp = need ? ws.data_ptr() : nullptr;
     const auto& p = d.ptr;
-    return result(without_lock([&] { return fn(p[0], p[1], p[2], p[3], p[4], float(scale), p[5], wp, need, stream); }), out);
+    return result(without_lock([&] { return fn(p[0], p[1], p[2], p[3], p[4], float(scale), p[5], wp, need, stream); }), out.release());
   });
 }
 

@@ -274,3 +274,24 @@ def test_keys_past_32_bits(ops, dev):
         q = _rand(r, (2 * n, 2, D), "bf16", dev)
         out = ops.cross_attention(q, k, v, _ints([0, 9, 80], dev), check=True)
         _check(out, q, k, v, [(0, n), (n, 2 * n)], [(0, 9), (9, 80)], "bf16")
+
+
+def test_no_room_for_the_workspace(pkg, ops, dev):
+    """An allocation that fails is an error, and holds no output."""
+    import ctypes
+    import sys
+
+    import torch
+
+    q, k = (torch.zeros((n, 2, 64), dtype=torch.bfloat16, device=dev) for n in (4, 9))
+    pages, out = k.view(1, 9, 2, 64), torch.zeros_like(q)
+    ko, table, n = _ints([0, 9], dev), torch.zeros((4, 1), dtype=torch.int32, device=dev), _ints([9] * 4, dev)
+    huge = ctypes.CFUNCTYPE(ctypes.c_size_t)(lambda: 1 << 60)
+    size = ctypes.cast(huge, ctypes.c_void_p).value
+    before = sys.getrefcount(out)
+    for name, args in (("l3d_cross_attention", (q, k, k, ko, None, out)),
+                       ("l3d_paged_attention", (q, pages, pages, table, n, out))):
+        with pytest.raises(RuntimeError, match="memory"):
+            pkg._lib.invoke(name, size, 0, 0.125, *args)
+    del args  # (it holds the output too)
+    assert sys.getrefcount(out) == before
