@@ -152,6 +152,8 @@ _SIGS = {
     "l3d_paged_attention_workspace_size": ([C.c_int64] * 6, C.c_size_t),
     "l3d_paged_attention": ([_D, _D, _D, _D, _D, C.c_float, _D, C.c_void_p, C.c_size_t, _S],
                             C.c_int),
+    "l3d_paged_attention_selftest_timeout": ([_D, _D, _D, _D, _D, C.c_float, _D, C.c_void_p, C.c_size_t,
+                                              C.c_uint32, _S], C.c_int),
     "l3d_cross_attention_workspace_size": ([C.c_int64] * 6 + [C.c_int], C.c_size_t),
     "l3d_cross_attention": ([_D, _D, _D, _D, _D, C.c_float, _D, C.c_void_p, C.c_size_t, _S],
                             C.c_int),

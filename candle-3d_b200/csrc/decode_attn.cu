@@ -207,10 +207,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
   constexpr int KT = C::KT, MK = C::MK, NT = D / 16;   // 16-key tiles of S^T, 16-wide tiles of O^T
   int* const status = &g_decode_status;
   extern __shared__ __align__(1024) uint8_t smem[];
-  if (smem_u32(smem) & 1023u) {
-    if (threadIdx.x == 0) atomicCAS(status, 0, ST_MISALIGNED);
-    return;
-  }
+  const bool aligned = (smem_u32(smem) & 1023u) == 0;  // (else no tile is loaded, but what is joined is still told)
+  if (!aligned && threadIdx.x == 0) atomicCAS(status, 0, ST_MISALIGNED);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + WARPS * C::RING);  // [WARPS][STAGES]
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bars + WARPS * C::STAGES);
   int* starts = reinterpret_cast<int*>(smem + WARPS * C::RING + C::BARS);  // [B + 1]
@@ -278,10 +276,9 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const Line line = line_of(p, starts[p.B]);
     per = line.per;
     x0 = int64_t(me) * per;
-    if (x0 >= line.total) {
-      if (p.edges && lane == 0) p.edges[me] = make_int4(0, 0, 0, 0);
-      return;
-    }
+    // (Nothing to join, until the stretch is done: also where a wait runs out, for the joining kernel follows either way.)
+    if (p.edges && lane == 0) p.edges[me] = make_int4(0, 0, 0, 0);
+    if (x0 >= line.total || !aligned) return;
     count = int(min(per, line.total - x0));
   } else {
     __syncthreads();  // (the barriers are there)
@@ -295,7 +292,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       c.tiles = (length_of(p, c.b, &bad) + KT - 1) / KT;
       const int per = (c.tiles + WARPS - 1) / WARPS;
       c.t = warp * per;
-      count = max(min(c.tiles - c.t, per), 0);
+      count = aligned ? max(min(c.tiles - c.t, per), 0) : 0;
     } else {
       c.seek(starts, p.B, heads, x0);
     }
@@ -335,7 +332,7 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
     const bool in = ld_ok && (p.size == 0 || (ld_page >= 0 && ld_page < p.keys));
     const uint32_t kd = ring + ld_stage * (2 * C::TILE), vd = kd + C::TILE;
     const int boxes = __popc(__ballot_sync(0xffffffffu, in));
-    if (lane == 0) mbar_expect_tx(&full[ld_stage], boxes * p.box * (128 * 2 * C::DC));
+    if (lane == 0) mbar_expect_tx(&full[ld_stage], boxes * p.box_bytes);
     __syncwarp();
     if (in) {
       const uint32_t at = lane * p.box * 128, bar = smem_u32(&full[ld_stage]);
@@ -863,7 +860,8 @@ static cudaError_t launch_t(const CUtensorMap (&maps)[2], const Params& p, int b
   return cudaLaunchKernelEx(&cfg, join, p);
 }
 
-int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s) {
+int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s,
+           uint64_t timeout_ns) {
   const int R = p.N * p.G;
   const bool one = alone(p.B, p.N, p.G, p.Hkv, longest, kv.D);
   p.height = height_for(R);
@@ -871,7 +869,7 @@ int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, 
   p.rows = R < p.height ? R : p.height;
   const int blocks = one ? p.B * p.Hkv * p.tiles : blocks_for(p.B, p.N, p.G, p.Hkv, longest, kv.D);
   p.total_warps = one ? 0 : blocks * WARPS;
-  p.wait_ns = tc::WAIT_LIMIT_NS;
+  p.wait_ns = timeout_ns ? timeout_ns : tc::WAIT_LIMIT_NS;
   char* w = static_cast<char*>(workspace);
   p.starts = reinterpret_cast<int*>(w);
   w += (size_t(p.B + 1) * 4 + 255) / 256 * 256;
@@ -888,6 +886,7 @@ int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, 
     while (p.size > 1 && (int64_t(2) << p.shift) <= p.size - 1) ++p.shift;
     if (p.size > 1) p.mul = uint32_t((uint64_t(1) << (32 + p.shift)) / uint64_t(p.size) + 1);
   }
+  p.box_bytes = p.box * 2 * int(kv.D) * 2 + (timeout_ns ? 16 : 0);
   CUtensorMap maps[2] = {};
   if (p.keys > 0) {  // (without keys nothing is loaded)
     const int64_t pages = p.size ? p.keys : 1, slots = p.size ? p.size : p.keys;
@@ -927,11 +926,10 @@ extern "C" size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int6
   return l3d::decode::workspace_size(b, n, hq / hkv, hkv, capacity, d);
 }
 
-extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
-                                   const l3d_tensor* table, const l3d_tensor* lengths, float scale,
-                                   const l3d_tensor* out, void* workspace, size_t workspace_bytes,
-                                   l3d_stream stream) {
-  const char* op = "l3d_paged_attention";
+static int run_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
+                               const l3d_tensor* table, const l3d_tensor* lengths, float scale, const l3d_tensor* out,
+                               void* workspace, size_t workspace_bytes, l3d_stream stream, uint64_t timeout_ns,
+                               const char* op) {
   if (!q || !k_pages || !v_pages || !table || !lengths || !out)
     return fail(L3D_E_NULL, "%s: q, k_pages, v_pages, table, lengths and out are required", op);
   const l3d_tensor* all[] = {q, out, k_pages, v_pages};
@@ -1005,5 +1003,26 @@ extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_page
   p.len64 = lengths->dtype == L3D_I64;
   p.causal = 1;
   p.scale_log2 = scale_log2;
-  return l3d::decode::launch(op, p, kv, q->dtype == L3D_F16, width * size, workspace, reinterpret_cast<cudaStream_t>(stream));
+  return l3d::decode::launch(op, p, kv, q->dtype == L3D_F16, width * size, workspace, reinterpret_cast<cudaStream_t>(stream),
+                             timeout_ns);
+}
+
+extern "C" int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3d_tensor* v_pages,
+                                   const l3d_tensor* table, const l3d_tensor* lengths, float scale,
+                                   const l3d_tensor* out, void* workspace, size_t workspace_bytes,
+                                   l3d_stream stream) {
+  return run_paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, workspace_bytes, stream, 0,
+                             "l3d_paged_attention");
+}
+
+extern "C" int l3d_paged_attention_selftest_timeout(const l3d_tensor* q, const l3d_tensor* k_pages,
+                                                    const l3d_tensor* v_pages, const l3d_tensor* table,
+                                                    const l3d_tensor* lengths, float scale, const l3d_tensor* out,
+                                                    void* workspace, size_t workspace_bytes, uint32_t wait_limit_ms,
+                                                    l3d_stream stream) {
+  const char* op = "l3d_paged_attention_selftest_timeout";
+  if (wait_limit_ms == 0 || wait_limit_ms > 2000)
+    return fail(L3D_E_UNSUPPORTED, "%s: wait_limit_ms must be in [1, 2000]", op);
+  return run_paged_attention(q, k_pages, v_pages, table, lengths, scale, out, workspace, workspace_bytes, stream,
+                             uint64_t(wait_limit_ms) * 1000000ull, op);
 }

@@ -26,6 +26,7 @@ struct Params {
   int keys;                     // pages, or packed rows
   int size, width;              // tokens of a page, pages of a request (packed: size 0)
   int box;                      // rows of a load: the largest power of two, up to a tile's keys, that divides the size
+  int box_bytes;                // what a load of K and V brings (failure self-test: 16 more, which never come)
   uint32_t mul;                 // j / size = (j * mul) >> (32 + shift), j < 2^30 (size > 1)
   int shift;
   const int32_t* table;
@@ -45,8 +46,9 @@ constexpr int MAX_BATCH = 4096;
 // Workspace bytes, whatever the lengths are; 0: none needed.
 size_t workspace_size(int64_t B, int64_t N, int64_t G, int64_t Hkv, int64_t longest, int64_t D);
 // Fills in what follows from the sizes and the workspace, and launches; an entry's status.  `longest`: the most
-// keys a sequence can have.
-int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s);
+// keys a sequence can have.  timeout_ns: 0, or the failure self-test, in which every wait for a load runs out then.
+int launch(const char* op, Params p, const Keys& kv, bool f16, int64_t longest, void* workspace, cudaStream_t s,
+           uint64_t timeout_ns = 0);
 
 }  // namespace decode
 }  // namespace l3d

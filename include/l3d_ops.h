@@ -548,6 +548,20 @@ int l3d_paged_attention(const l3d_tensor* q, const l3d_tensor* k_pages, const l3
                         const l3d_tensor* out, void* workspace, size_t workspace_bytes,
                         l3d_stream stream);
 
+/* Failure-handling self-test of l3d_paged_attention (no counterpart in the
+ * reference): the same launches, except that every wait for a tile of keys counts
+ * on bytes that never come and gives up after wait_limit_ms (1 .. 2000).  The
+ * kernel must then record status 5 (timeout) for l3d_kernel_status, wait for the
+ * copies it started and return, and the kernel that joins the parts must stay
+ * within the tensors and the workspace, whatever the latter held; out is not
+ * meaningful, and the context stays usable. */
+int l3d_paged_attention_selftest_timeout(const l3d_tensor* q, const l3d_tensor* k_pages,
+                                         const l3d_tensor* v_pages, const l3d_tensor* table,
+                                         const l3d_tensor* lengths, float scale,
+                                         const l3d_tensor* out, void* workspace,
+                                         size_t workspace_bytes, uint32_t wait_limit_ms,
+                                         l3d_stream stream);
+
 /* Workspace bytes for l3d_cross_attention (0: none needed); ragged: q_offsets
  * are given. */
 size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int64_t hq,
