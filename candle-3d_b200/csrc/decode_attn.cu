@@ -22,8 +22,8 @@
 // Short caches of a few requests need neither line nor second kernel: a block takes all the keys of a head and row
 // tile, a stretch of them per warp, and joins the parts in shared memory (ALONE).
 //
-// Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits or more of each probability
-// (the products are not what bounds the kernel): the output is as near the 64-bit one as its rounding allows.
+// Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits of each probability, or in f16 2^-32 of
+// the row's largest where that is more (the products are not what bounds the kernel).
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
 // status word and stops.
@@ -44,6 +44,10 @@ using namespace l3d::attn;
 constexpr int WARPS = 12;               // of a block (one per SM)
 constexpr int MIN_TILES = 1;            // of a warp
 constexpr float RESCALE_LOG2 = 8.f;     // the running maximum moves only when it grows past 2^8
+// log2 of a row's largest probability: f16 goes down to 2^-24 only, and up to 2^15 there is room.  (At 2^0 the
+// weight of 255 keys of 2^-18 each beside one of 1 was off by up to 1%.)
+template <typename T>
+constexpr float HELD_LOG2 = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 
 __device__ int g_decode_status;
@@ -452,8 +456,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       __syncwarp();
     }
-    // The running maximum and sum of this thread's two rows (the maximum over all its warp's keys, the sum over
-    // its own ones).
+    // The running maximum (less HELD_LOG2) and sum of this thread's two rows (the maximum over all its warp's keys,
+    // the sum over its own ones).
     bool grown = false;
     float al[NB][2];
 #pragma unroll
@@ -466,7 +470,8 @@ __global__ void __launch_bounds__(WARPS * 32, 1)
         mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) * p.scale_log2;
-        const bool grow = !(mx <= m[nb][e] + RESCALE_LOG2);
+        const bool grow = !(mx <= m[nb][e] + (RESCALE_LOG2 + HELD_LOG2<T>));
+        mx -= HELD_LOG2<T>;
         al[nb][e] = grow ? ex2f(m[nb][e] - mx) : 1.f;  // 0 on the first key a row sees
         if (grow) m[nb][e] = mx;
         grown |= grow;
