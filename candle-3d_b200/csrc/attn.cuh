@@ -1,4 +1,4 @@
-// Pieces shared by the attention kernels (attn.cu, prefix_attn.cu): 4-D TMA
+// Pieces shared by the attention kernels (attn.cu, prefix_attn.cu, cross_attn.cu, decode_attn.cu): 4-D TMA
 // tile loads and maps, the MN-major V operand, P read from tensor memory, wide
 // TMEM accesses and the exponentials.
 #pragma once
@@ -20,8 +20,9 @@ using namespace l3d::tc;
 // 2^j added to the exponent field.  x is clamped just above -127, where q > 1 and
 // the exponent field comes to 0: what is left, 1e-42, is 0 in either 16-bit type,
 // as a masked key's probability has to be (2^-126 would add 4 to an output where
-// its V is at the end of bf16's range).  The inputs here are <= 2^8 (the rescale
-// threshold).  A NaN is clamped too: the running maximum carries it past this function (max_nan).
+// its V is at the end of bf16's range).  The inputs here are <= 8 (the rescale
+// threshold), or 15 where f16 probabilities are held higher.  A NaN is clamped
+// too: the running maximum carries it past this function (max_nan).
 constexpr float EX2_C0 = 0.99992806f, EX2_C1 = 0.69326097f, EX2_C2 = 0.24261113f,
                 EX2_C3 = 0.05517167f, EX2_MIN = -127.f + 0x1p-12f;
 __device__ __forceinline__ float2 ex2_poly2(float2 x) {

@@ -42,6 +42,10 @@ using namespace l3d::attn;
 constexpr int BQ = 128, BKV = 64, THREADS = 256, CTAS = 2;
 constexpr int ST_TIMEOUT = 5, ST_MISALIGNED = 6;
 constexpr float RESCALE_LOG2 = 8.f;   // as in attn.cu
+// log2 of a row's largest probability: f16 goes down to 2^-24 only, and up to 2^15 there is room.  (At 2^0 the
+// weight of 255 keys of 2^-18 each beside one of 1 was off by up to 1%.)
+template <typename T>
+constexpr float HELD_LOG2 = std::is_same<T, __half>::value ? 7.f : 0.f;
 constexpr int MAX_PARTS = 16;
 // Sequences, and key heads of them all: while a block passes over items without rows or keys, its other warps wait
 // for the next one, and those waits are bounded (2 s).  2^20 sequences without rows or keys x 64 heads: 110 ms.
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, CTAS)
     for (int at = 0; ok && item(at, it); done_with(at++)) {
       const bool valid = i < it.rows && g < p.G;
       const bool active = __any_sync(0xffffffffu, valid);  // the warp holds rows
-      float m = -INFINITY;                         // running max, log2 units
+      float m = -INFINITY;                         // running max less HELD_LOG2, log2 units
       float2 l2 = f2(0.f);                         // running row sum (two parts)
       for (int j = 0; j < it.tiles; ++j, ++n) {
         ok = wait_warp(&s_full[n & 1], (n >> 1) & 1);
@@ -515,8 +519,8 @@ __global__ void __launch_bounds__(THREADS, CTAS)
 #pragma unroll
         for (int e = 4; e < BKV; e += 2) mx[(e >> 1) & 3] = max_nan(mx[(e >> 1) & 3], s[e], s[e + 1]);
         const float mxs = max_nan(max_nan(mx[0], mx[1], mx[2]), mx[3]) * p.scale_log2;  // scale > 0
-        const bool grow = !(mxs <= m + RESCALE_LOG2);       // always on the first key a row sees
-        const float m_new = grow ? mxs : m;
+        const bool grow = !(mxs <= m + (RESCALE_LOG2 + HELD_LOG2<T>));  // always on the first key a row sees
+        const float m_new = grow ? mxs - HELD_LOG2<T> : m;
         const float alpha = grow ? ex2f(m - m_new) : 1.f;   // 0 on the first
         if (j > 0 && __any_sync(0xffffffffu, grow)) {
           ok = wait_warp(&pv_done[(n - 1) & 1], ((n - 1) >> 1) & 1);  // O is stable

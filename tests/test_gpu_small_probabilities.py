@@ -51,3 +51,22 @@ def test_small_probabilities_of_two_parts(ops, dev, form, D, gap):
     bound = U["f16"] * want + (1.4e-4 + 2.0 ** -16 + 1e-5) * want + n * 2.0 ** -31 * p.max() * 2 + 2.0 ** -25
     err = (out.double() - want).abs()
     assert (err <= bound).all(), f"worst ratio {(err / bound).max().item():.2f}"
+
+
+@pytest.mark.parametrize("gap", GAPS)
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,n", [(40, 4096), (128, 1024)])
+def test_small_probabilities_of_one_part(ops, dev, rows, n, D, gap):
+    """Many rows over packed keys: each probability rounded once, to 2^-11 of itself or 2^-32 of the row's largest."""
+    import torch
+
+    B, H = 80, 4
+    q1, k1, v1 = _few_large(rng(D), n, D, gap, dev)
+    q = q1.expand(B * rows, H, D).contiguous()
+    k, v = (t[:, None].expand(n, H, D).repeat(B, 1, 1) for t in (k1, v1))
+    out = ops.cross_attention(q, k, v, torch.arange(B + 1, dtype=torch.int32, device=dev) * n, check=True)
+    p = torch.softmax((k1.double() @ q1.double()) * D ** -0.5, 0)
+    want = p @ v1.double()
+    bound = (2 * U["f16"] + 4e-4) * want + n * 2.0 ** -32 * p.max() * 2 + 2.0 ** -25
+    err = (out.double() - want).abs()
+    assert (err <= bound).all(), f"worst ratio {(err / bound).max().item():.2f}"
