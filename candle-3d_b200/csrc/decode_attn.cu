@@ -22,7 +22,7 @@
 // Short caches of a few requests need neither line nor second kernel: a block takes all the keys of a head and row
 // tile, a stretch of them per warp, and joins the parts in shared memory (ALONE).
 //
-// Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits of each probability, or in f16 2^-32 of
+// Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits of each probability, or in f16 2^-31 of
 // the row's largest where that is more (the products are not what bounds the kernel).
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
@@ -99,18 +99,25 @@ __device__ __forceinline__ Line line_of(const Params& p, int tiles) {
   return {total, even > MIN_TILES ? even : MIN_TILES};
 }
 
+// The second part of a probability, at least the type's smallest number where the first is not 0: it meets an infinite
+// V too, and 0 times that (or an infinity less another, were the first rounded up) is no number.  Values without a sign
+// are ordered as their bits.
+__device__ __forceinline__ uint32_t not_zero(uint32_t second, uint32_t first) {
+  return __vmaxu2(second, __vminu2(first, 0x00010001u));
+}
+
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  // a, b as a pair of the type, and what the pair leaves of them.
+  // a, b >= 0 cut off to a pair of the type, and what that leaves of them, rounded.
   static __device__ __forceinline__ uint32_t split(float a, float b, uint32_t& rest) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const __nv_bfloat162 l = __floats2bfloat162_rn(a - __low2float(h), b - __high2float(h));
-    rest = *reinterpret_cast<const uint32_t*>(&l);
-    return *reinterpret_cast<const uint32_t*>(&h);
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b), hi = __byte_perm(x, y, 0x7632);
+    const __nv_bfloat162 l = __floats2bfloat162_rn(a - __uint_as_float(x & 0xffff0000u), b - __uint_as_float(y & 0xffff0000u));
+    rest = not_zero(*reinterpret_cast<const uint32_t*>(&l), hi);
+    return hi;
   }
 };
 template <> struct Mma<__half> {
@@ -119,10 +126,12 @@ template <> struct Mma<__half> {
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t split(float a, float b, uint32_t& rest) {
-    const __half2 h = __floats2half2_rn(a, b);
+    uint32_t hi;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
+    const __half2 h = *reinterpret_cast<const __half2*>(&hi);
     const __half2 l = __floats2half2_rn(a - __low2float(h), b - __high2float(h));
-    rest = *reinterpret_cast<const uint32_t*>(&l);
-    return *reinterpret_cast<const uint32_t*>(&h);
+    rest = not_zero(*reinterpret_cast<const uint32_t*>(&l), hi);
+    return hi;
   }
 };
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t addr) {

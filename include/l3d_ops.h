@@ -537,7 +537,9 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * (N * Hq / Hkv of them) read its keys once.  What a row does not see does not
  * reach it, whatever it holds.  A row with no keys gives zeros; one that sees a
  * score that is NaN or +inf, or a key whose page is not one of the cache, and all
- * rows of a request whose length is more than its table has room for, NaN.  BF16
+ * rows of a request whose length is more than its table has room for, NaN.  An
+ * infinite V makes the elements that it is weighed into infinite (NaN where its
+ * probability is below 2^-126 of the row's largest, in f16 2^-31, or both signs meet).  BF16
  * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
  * otherwise free in multiples of 16 bytes (pages, slots and out not expanded); out may
  * be q; softmax, sums and probabilities in f32
@@ -577,7 +579,7 @@ size_t l3d_cross_attention_workspace_size(int64_t b, int64_t tq, int64_t tk, int
  * sequence are left as they were, and keys of none are never used, whatever they
  * hold.  Hq a multiple of Hkv, at most 128 times as many, query head h reading key
  * head h / (Hq / Hkv); at most 2^20 sequences, and 2^26 key heads of all of them.  A row with no keys gives zeros, one that sees a score
- * that is NaN or +inf NaN.  BF16 or F16, D = 64 or 128, head dim contiguous,
+ * that is NaN or +inf NaN; an infinite V as in l3d_paged_attention.  BF16 or F16, D = 64 or 128, head dim contiguous,
  * strides otherwise free in multiples of 16 bytes (keys not expanded along the rows,
  * q and out not at all); softmax and sums in f32, probabilities rounded to the input type for
  * the second product (not where every sequence has N rows and N * Hq / Hkv is at
