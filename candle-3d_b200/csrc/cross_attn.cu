@@ -20,13 +20,18 @@
 //              maximum has grown past 2^8, zeros over V rows past a sequence's end (another sequence's, or
 //              anything: a masked probability is 0, but 0 x NaN is not), and the output.
 // Where there are fewer items than blocks, each is cut into parts along its keys, and combine_kernel weighs the
-// parts of each row; an item's parts have fixed places.  A row or two per sequence goes to decode_attn.cu instead.
+// parts of each row; an item's parts have fixed places.  Where every sequence has as many rows, up to 16 a key head,
+// decode_attn.cu takes the call instead (few_rows).
+// P is rounded to the input type for the second product, as tensor memory takes it: two parts would be half as many
+// products again.  Against 64 bits the error is 2.3e-3 of the output's norm where the output's type alone gives 1.7e-3
+// (2 x 2049 rows, bf16).
 // Every mbarrier wait is bounded (%globaltimer, 2 s; those for an item 60 s); on expiry the block records an error
 // in the device's status word and stops.
-// Measured: 3 x 31569 rows x 12 heads of 128 over up to 1370 keys 627 us (1087 TFLOP/s, 66% of a plain product; at the
-// power limit 740); 4 x 8192 rows x 16 heads of 64 over up to 1370 keys 194 us (522 TFLOP/s).  A 64-key tile takes an SM
-// some 1000 clocks either way, of which the exponentials need 512: the softmax warps' chain, with the products'
-// round trip (scores of 64 keys read all of Q from shared memory, 384 clocks for 256 of products) partly under it.
+// Measured: 3 x 31569 rows x 12 heads of 128 over up to 1370 keys 641 us (1063 TFLOP/s, 64% of a plain product; call
+// after call, at the power limit, 744: 916); 2 x 2049 rows x 16 heads of 128 53.6 us (673 TFLOP/s); 4 x 8192 rows x 16
+// heads of 64 over up to 1370 keys 194 us (522 TFLOP/s).  A 64-key tile takes an SM some 1000 clocks either way, of which
+// the exponentials need 512: the softmax warps' chain, with the products' round trip (scores of 64 keys read all of Q
+// from shared memory, 384 clocks for 256 of products) partly under it.
 #include <type_traits>
 
 #include "attn.cuh"
@@ -717,7 +722,11 @@ static int parts_for(int64_t B, int64_t Tq, int64_t Tk, int64_t G, int64_t Hkv) 
   return int(parts < 1 ? 1 : parts > MAX_PARTS ? MAX_PARTS : parts);
 }
 
-// Single rows (or a few) of every sequence: their work is reading the keys.
+// Single rows (or a few) of every sequence: their work is reading the keys.  us here and in the kernel above: 32 x 16
+// heads of 64, up to 1370 keys: 1 row 26.9 and 37.9, 8 28.6 and 37.4, 12 32.6 and 37.5, 16 40.8 and 37.8, 32 59.8 and
+// 38.1; 64 x 4 heads of 128, 1029 keys: 8 24.3 and 27.5, 16 32.9 and 27.9; 2 x 2 heads of 64, 600 keys: 16 8.5 and
+// 11.6, 128 8.9 and 10.9.  Up to 16 rows (two columns of 8) the forms are near each other, and this one keeps two parts
+// of each probability.
 // (The last two: what decode_attn.cu takes, and counts in 32 bits.)
 static bool few_rows(int64_t B, int64_t N, int64_t G, int64_t Tk) {
   return N > 0 && N * G <= 16 && B <= decode::MAX_BATCH && B * (Tk / 16 + 1) <= int64_t(1) << 30;

@@ -20,16 +20,18 @@
 // combine_kernel weighs the parts of each row.  A part's place follows from the lengths, so results do not
 // depend on the order in which warps run.
 // Short caches of a few requests need neither line nor second kernel: a block takes all the keys of a head and row
-// tile, a stretch of them per warp, and joins the parts in shared memory (ALONE).
+// tile, a stretch of them per warp, and joins the parts in shared memory (ALONE).  What a table has room for decides, for
+// lengths are not on the host: 300 keys in a table for 16384 take 3.6 us more than in one for 304.
 //
 // Scores with f32 accumulators, P in two 16-bit parts whose sum keeps 16 bits of each probability, or in f16 2^-31 of
 // the row's largest where that is more (the products are not what bounds the kernel).
 // A table entry outside the cache makes the key's score NaN, and so its row; a length past the table the same.
 // Every wait for a load is bounded (%globaltimer, 2 s); on expiry the warp records an error in the device's
 // status word and stops.
-// Measured, D = 128: 8 x 65536 keys x 4 heads 171 us (6.28 TB/s, 96% of a plain copy); 64 x up to 4096 keys x 4 heads
-// 50 us (4.86 TB/s): 3.7 us until the first loads go out, 2 for the second kernel.  One request of 300 keys x 2 heads of
-// 64: 5.7 us.
+// Measured, D = 128: 8 x 65536 keys x 4 heads 172 us (6.25 TB/s, 95% of a plain copy); 64 x up to 4096 keys x 4 heads
+// 50 us (4.82 TB/s): 3.7 us until the first loads go out, 2 for the second kernel.  One request of 300 keys x 2 heads of
+// 64: 5.7 us.  The 64 requests with pages of 17 tokens, or of one, whose loads bring one row each: 73 us (D = 64: 47
+// for 34.5).
 #include <type_traits>
 
 #include "attn.cuh"

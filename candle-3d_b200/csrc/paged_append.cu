@@ -13,8 +13,8 @@
 // half of a pair by shuffles the kernel was bound by issue: 36 us for 10992 tokens x 48 heads x 64.)  A block takes a few tokens and forms their angles once for all heads, in 64 bits:
 // at position 100,000 a product in 32 bits is off by up to 4e-3 radians, as much as bf16's rounding.  What is
 // left after whole turns are taken off is at most half a turn, and goes on in 32 bits.
-// Measured: 49152 tokens x 24 heads x 128, bf16: 109 us (5.52 TB/s, 84% of a plain copy); 10992 x 48 x 64, f16: 31 us
-// (4.36 TB/s: the places and angles come before the first row); one token 4.5 us.
+// Measured: 49152 tokens x 24 heads x 128, bf16: 109 us (5.55 TB/s, 84% of a plain copy; call after call 112); 10992 x
+// 48 x 64, f16: 31 us (4.38 TB/s; each block looks its places and angles up before its first row); one token 4.5 us.
 #include "common.cuh"
 
 namespace l3d {

@@ -538,8 +538,9 @@ size_t l3d_paged_attention_workspace_size(int64_t b, int64_t hq, int64_t hkv, in
  * reach it, whatever it holds.  A row with no keys gives zeros; one that sees a
  * score that is NaN or +inf, or a key whose page is not one of the cache, and all
  * rows of a request whose length is more than its table has room for, NaN.  An
- * infinite V makes the elements that it is weighed into infinite (NaN where its
- * probability is below 2^-126 of the row's largest, in f16 2^-31, or both signs meet).  BF16
+ * infinite V makes the elements that it is weighed into infinite, NaN where both
+ * signs meet (a probability below 2^-126 of the row's largest, in f16 2^-31, may
+ * count as 0: then NaN, or as if the key were not there).  BF16
  * or F16, D = 64 or 128, at most 4096 requests, head dim contiguous, strides
  * otherwise free in multiples of 16 bytes (pages, slots and out not expanded); out may
  * be q; softmax, sums and probabilities in f32
